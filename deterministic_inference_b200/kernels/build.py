@@ -49,6 +49,9 @@ SOURCES = {
     "state_space": "state_space.cu",
     "retention": "retention.cu",
     "gated_linear_attention": "gated_linear_attention.cu",
+    "cache_int8": "cache_int8.cu",
+    "attention_int8": "attention_int8.cu",
+    "gemm_int8": "gemm_int8.cu",
 }
 HEADERS = ("common.cuh", "attention_merge.cuh")
 # further headers a library includes

@@ -1,0 +1,268 @@
+"""Serving in 8-bit integers: weights and activations with a scale for each output channel and each token, and a paged
+cache of keys and values with a scale for each token and head.  ``ops`` exports what is here.
+
+One rule quantises every row (a token's activations, an output channel of a weight, a token's key or value of one head):
+
+    a = max(max |x|, 2^-100),  code = rint(x * (127 / a)) (ties to even),  scale = a / 127,  value = scale * code
+
+in float32, whatever the row's type.  A row that holds an infinity or a NaN has the scale NaN and reads back as NaN.
+
+``Int8Weight``          a weight [N, K], quantised once (``Int8Weight.of``) or given as codes and scales
+``quantize_rows``       activations [M, K] -> ``Int8Rows``; ``int8_linear`` takes either
+``int8_linear``         y = x @ weight^T: an exact 32-bit sum of products of codes, times the two scales
+``Int8Cache``           the cache of one layer: data int8 [pages, 2, Hkv, page_size, D], scales float32 [.., page_size]
+``int8_cache_write``    keys and values into their slots
+``int8_cache_read``     what the rows of given slots stand for
+``int8_paged_attention``  attention of a step's new tokens over the cache
+"""
+
+from __future__ import annotations
+
+from ctypes import c_float, c_int, c_longlong
+
+import torch
+
+MAX_K = 133144          # 127^2 * K stays below 2^31
+MAX_HEAD_DIM = 256
+
+
+def _ops():
+    from . import ops
+    return ops
+
+
+def _same_device(what: str, *tensors) -> None:
+    if len({t.device for t in tensors}) > 1:
+        raise _ops().KernelError(f"{what}: tensors on different devices ({sorted({str(t.device) for t in tensors})})")
+
+
+def _padded(k: int) -> int:
+    return -(-k // 16) * 16
+
+
+class Int8Rows:
+    """Rows [M, K] in 8 bits: ``codes`` int8 [M, K rounded up to 16] (zeros behind K), ``scales`` float32 [M]; ``dtype`` is
+    the type of the tensor they were made from, which a product's output takes."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, k: int, dtype: torch.dtype):
+        self.codes, self.scales, self.k, self.dtype = codes, scales, int(k), dtype
+
+    @property
+    def shape(self):
+        return torch.Size((self.codes.shape[0], self.k))
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def tensor(self) -> torch.Tensor:
+        """The values the codes stand for, float32."""
+        return self.codes[:, :self.k].float() * self.scales[:, None]
+
+
+class Int8Weight:
+    """A weight [N, K] in 8 bits with a scale for each output channel: ``codes`` int8 [N, K rounded up to 16] on 16 bytes,
+    ``scales`` float32 [N].  ``Int8Weight(codes [N, K], scales [N])`` lays out codes that were made elsewhere, -128 not
+    among them.  A constant, like every weight: the products read it ahead of their wait for the kernel in front."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        ops = _ops()
+        ops._need(codes, "codes", torch.int8, 2)
+        ops._need(scales, "scales", torch.float32, 1)
+        n, k = codes.shape
+        if scales.shape[0] != n or k < 1 or k > MAX_K:
+            raise ops.KernelError(f"Int8Weight: codes {tuple(codes.shape)}, scales {tuple(scales.shape)} "
+                                  f"(K from 1 to {MAX_K})")
+        _same_device("Int8Weight", codes, scales)
+        self.k = k
+        if _padded(k) != k or codes.data_ptr() % 16:
+            padded = torch.zeros(n, _padded(k), dtype=torch.int8, device=codes.device)
+            padded[:, :k] = codes
+            codes = padded
+        self.codes, self.scales = codes, scales
+
+    @classmethod
+    def of(cls, weight: torch.Tensor) -> "Int8Weight":
+        """Quantises a float32 or bfloat16 weight [N, K]."""
+        rows = _quantize(weight, "weight", early=False)
+        out = cls.__new__(cls)
+        out.codes, out.scales, out.k = rows.codes, rows.scales, rows.k
+        return out
+
+    @property
+    def shape(self):
+        return torch.Size((self.codes.shape[0], self.k))
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def tensor(self) -> torch.Tensor:
+        """The values the codes stand for, float32."""
+        return self.codes[:, :self.k].float() * self.scales[:, None]
+
+
+def _quantize(x: torch.Tensor, name: str, early: bool) -> Int8Rows:
+    ops = _ops()
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise ops.KernelError(f"{name} must be a CUDA tensor: this package has no CPU path")
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ops.KernelError(f"{name} must be rows of consecutive values (shape {tuple(x.shape)}, stride {x.stride()})")
+    m, k = x.shape
+    if k < 1 or k > MAX_K:
+        raise ops.KernelError(f"{name} has rows of {k} values (1 to {MAX_K})")
+    codes = torch.empty(m, _padded(k), dtype=torch.int8, device=x.device)
+    scales = torch.empty(m, dtype=torch.float32, device=x.device)
+    st = ops._lib("cache_int8").dib_quantize_rows(
+        ops._ptr(x), c_longlong(x.stride(0)), ops._ptr(codes), ops._ptr(scales), c_longlong(m), c_int(k),
+        c_int(ops._dt(x, name)), c_int(1 if early else 0), ops._stream())
+    ops._check(st, "quantize_rows", f"rows {m} x {k}")
+    return Int8Rows(codes, scales, k, x.dtype)
+
+
+def quantize_rows(x) -> Int8Rows:
+    """Rows [M, K] (float32 or bfloat16, any distance between rows; or the partial sums of a product) in 8 bits."""
+    return _quantize(_ops().as_tensor(x), "x", early=True)
+
+
+def int8_linear(x, weight: Int8Weight, out_dtype=None) -> torch.Tensor:
+    """y = x @ weight^T, [M, N]: ``x`` [M, K] is quantised row by row (or is an ``Int8Rows``); the sum of the codes'
+    products is exact in 32 bits, so a row's bits depend on the row and the weight alone; times the token's and the
+    channel's scale in float32, rounded once to ``out_dtype`` (float32 or bfloat16; x's type if not given)."""
+    ops = _ops()
+    if not isinstance(weight, Int8Weight):
+        raise ops.KernelError("int8_linear: weight must be an Int8Weight")
+    if not isinstance(x, Int8Rows):
+        x = ops.as_tensor(x)
+        if x.dim() == 2 and x.shape[1] != weight.k:
+            raise ops.KernelError(f"int8_linear: x {tuple(x.shape)} against weight {tuple(weight.shape)}")
+        x = quantize_rows(x)
+    if x.k != weight.k:
+        raise ops.KernelError(f"int8_linear: x {tuple(x.shape)} against weight {tuple(weight.shape)}")
+    _same_device("int8_linear", x.codes, weight.codes)
+    m, n = x.codes.shape[0], weight.codes.shape[0]
+    out = torch.empty(m, n, dtype=out_dtype or x.dtype, device=x.device)
+    st = ops._lib("gemm_int8").dib_gemm_int8(
+        ops._ptr(x.codes), ops._ptr(x.scales), ops._ptr(weight.codes), ops._ptr(weight.scales), ops._ptr(out), c_int(m),
+        c_int(n), c_int(x.codes.shape[1]), c_int(ops._dt(out, "out")), c_int(_sms(x.device)), ops._stream())
+    ops._check(st, "int8_linear", f"M={m} N={n} K={x.k}")
+    return out
+
+
+def _sms(device) -> int:
+    from . import gemm_bf16
+    return gemm_bf16._sms(device)
+
+
+class Int8Cache:
+    """One layer's paged cache in 8 bits: ``data`` int8 [pages, 2, Hkv, page_size, D], ``scales`` float32
+    [pages, 2, Hkv, page_size]; [:, 0] are keys, [:, 1] values.  D a multiple of 16, at most 256."""
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor):
+        ops = _ops()
+        ops._need(data, "data", torch.int8, 5)
+        ops._need(scales, "scales", torch.float32, 4)
+        pages, two, hkv, page_size, d = data.shape
+        if tuple(scales.shape) != (pages, two, hkv, page_size) or two != 2 or hkv < 1 or page_size < 1:
+            raise ops.KernelError(f"Int8Cache: data {tuple(data.shape)}, scales {tuple(scales.shape)}")
+        if d < 16 or d > MAX_HEAD_DIM or d % 16:
+            raise ops.KernelError(f"Int8Cache: heads of {d} (a multiple of 16, at most {MAX_HEAD_DIM})")
+        if data.data_ptr() % 16:
+            raise ops.KernelError("Int8Cache: data must lie on 16 bytes")
+        _same_device("Int8Cache", data, scales)
+        self.data, self.scales = data, scales
+
+    @classmethod
+    def zeros(cls, num_pages: int, num_kv_heads: int, page_size: int, head_dim: int, device="cuda") -> "Int8Cache":
+        return cls(torch.zeros(num_pages, 2, num_kv_heads, page_size, head_dim, dtype=torch.int8, device=device),
+                   torch.zeros(num_pages, 2, num_kv_heads, page_size, dtype=torch.float32, device=device))
+
+    @property
+    def shape(self):
+        return self.data.shape
+
+    @property
+    def device(self):
+        return self.data.device
+
+
+def _row_stride(x: torch.Tensor, name: str, hkv: int, d: int) -> int:
+    """Distance of a token's rows [Hkv, D], which lie together (a column range of a fused projection, say)."""
+    ops = _ops()
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise ops.KernelError(f"{name} must be a CUDA tensor: this package has no CPU path")
+    if x.dim() != 3 or tuple(x.shape[1:]) != (hkv, d):
+        raise ops.KernelError(f"{name} has shape {tuple(x.shape)}, the cache's heads are [{hkv}, {d}]")
+    if x.stride(2) != 1 or (hkv > 1 and x.stride(1) != d):
+        raise ops.KernelError(f"{name}: a token's heads must lie together (stride {x.stride()})")
+    return x.stride(0) if x.shape[0] > 1 else hkv * d
+
+
+def int8_cache_write(k: torch.Tensor, v: torch.Tensor, cache: Int8Cache, slot_mapping: torch.Tensor) -> None:
+    """k, v [T, Hkv, D] (float32 or bfloat16; column ranges of wider rows too) into the rows ``slot_mapping`` (int32 [T],
+    page * page_size + offset) of the cache; a negative slot is skipped.  Slots are distinct."""
+    ops = _ops()
+    pages, _, hkv, page_size, d = cache.shape
+    ks, vs = _row_stride(k, "k", hkv, d), _row_stride(v, "v", hkv, d)
+    ops._need(slot_mapping, "slot_mapping", torch.int32, 1)
+    t = k.shape[0]
+    if v.shape[0] != t or v.dtype != k.dtype or slot_mapping.shape[0] < t:
+        raise ops.KernelError(f"int8_cache_write: k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}, "
+                              f"{slot_mapping.shape[0]} slots")
+    _same_device("int8_cache_write", k, v, cache.data, slot_mapping)
+    st = ops._lib("cache_int8").dib_int8_cache_write(
+        ops._ptr(k), ops._ptr(v), c_longlong(ks), c_longlong(vs), ops._ptr(cache.data), ops._ptr(cache.scales),
+        ops._ptr(slot_mapping), c_int(t), c_int(hkv), c_int(d), c_int(page_size), c_longlong(pages), c_int(ops._dt(k, "k")),
+        ops._stream())
+    ops._check(st, "int8_cache_write", f"heads {hkv} x {d}")
+
+
+def int8_cache_read(cache: Int8Cache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
+    """(k, v) [T, Hkv, D] in ``dtype``: what the rows ``slots`` (int32 [T]) of the cache stand for; zeros for a negative
+    slot."""
+    ops = _ops()
+    pages, _, hkv, page_size, d = cache.shape
+    ops._need(slots, "slots", torch.int32, 1)
+    _same_device("int8_cache_read", cache.data, slots)
+    k = torch.empty(slots.shape[0], hkv, d, dtype=dtype, device=cache.device)
+    v = torch.empty_like(k)
+    st = ops._lib("cache_int8").dib_int8_cache_read(
+        ops._ptr(cache.data), ops._ptr(cache.scales), ops._ptr(slots), ops._ptr(k), ops._ptr(v), c_int(slots.shape[0]),
+        c_int(hkv), c_int(d), c_int(page_size), c_longlong(pages), c_int(ops._dt(k, "out")), ops._stream())
+    ops._check(st, "int8_cache_read", f"heads {hkv} x {d}")
+    return k, v
+
+
+def int8_paged_attention(q: torch.Tensor, cache: Int8Cache, meta, scale: float, window=None) -> torch.Tensor:
+    """Causal attention of every token of the step over its sequence's keys in the cache, as ``ops.paged_attention``: q
+    [T, Hq, D] float32 or bfloat16, ``meta`` the step's ``AttentionMeta``.  A sequence's new tokens are its last ones
+    (``seq_lens`` counts them); each sees the keys up to its own position, the last ``window`` of them if given.  The
+    codes of keys and values enter the products as they are, the scales join scores and probabilities in float32.  A
+    token that sees no key gives zeros."""
+    ops = _ops()
+    ops._need(q, "q", None, 3)
+    t, hq, d = q.shape
+    pages, _, hkv, page_size, d2 = cache.shape
+    if d2 != d or hq < 1 or hq % hkv:
+        raise ops.KernelError(f"int8_paged_attention: q {tuple(q.shape)} vs cache {tuple(cache.shape)}")
+    b = meta.block_table.shape[0] if meta.block_table.dim() == 2 else -1
+    ops._need(meta.block_table, "block_table", torch.int32, 2)
+    for x, name, n in ((meta.token_seq, "token_seq", t), (meta.cu_q_lens, "cu_q_lens", b + 1),
+                       (meta.seq_lens, "seq_lens", b)):
+        ops._need(x, name, torch.int32, 1)
+        if x.shape[0] < n:
+            raise ops.KernelError(f"int8_paged_attention: {name} has {x.shape[0]} entries, the step needs {n}")
+    win = int(window) if window else 0
+    if win < 0:
+        raise ops.KernelError(f"int8_paged_attention: a window of {win} keys")
+    _same_device("int8_paged_attention", q, cache.data, meta.block_table, meta.token_seq, meta.cu_q_lens, meta.seq_lens)
+    out = torch.empty_like(q)
+    if t == 0:
+        return out
+    st = ops._lib("attention_int8").dib_int8_attention_any(
+        ops._ptr(q), ops._ptr(out), ops._ptr(cache.data), ops._ptr(cache.scales), ops._ptr(meta.block_table),
+        c_int(meta.block_table.shape[1]), ops._ptr(meta.token_seq), ops._ptr(meta.cu_q_lens), ops._ptr(meta.seq_lens),
+        c_int(t), c_int(hq), c_int(hkv), c_int(d), c_int(page_size), c_float(scale), c_int(win), c_int(ops._dt(q, "q")),
+        ops._stream())
+    ops._check(st, "int8_paged_attention", f"head_dim {d}, heads {hq}/{hkv}")
+    return out

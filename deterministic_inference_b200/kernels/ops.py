@@ -640,6 +640,8 @@ def qkv_project(x: torch.Tensor, w_qkv: torch.Tensor, num_heads: int, num_kv_hea
 def reshape_and_cache(k: torch.Tensor, v: torch.Tensor, kv_cache: torch.Tensor,
                       slot_mapping: torch.Tensor) -> None:
     """k, v [T, Hkv, D] into their slots of the paged cache (negative slot: skip)."""
+    if isinstance(kv_cache, Int8Cache):
+        return int8_cache_write(k, v, kv_cache, slot_mapping)
     _need(k, "k", None, 3)
     _need(v, "v", k.dtype, 3)
     _need(kv_cache, "kv_cache", k.dtype, 5)
@@ -665,7 +667,10 @@ def paged_attention(q: torch.Tensor, kv_cache: torch.Tensor, meta, scale: float,
     seq_lens [B], host copies of the lengths, number of leading decode
     sequences).  A query at position p sees keys max(0, p-window+1) .. p.
     ``defer``: a step of one-token sequences only may come back as a ``SplitAttention``
-    (its splits not yet merged) for the matrix product that follows to merge."""
+    (its splits not yet merged) for the matrix product that follows to merge.  ``kv_cache`` may be an
+    ``Int8Cache``: ``int8_paged_attention``."""
+    if isinstance(kv_cache, Int8Cache):
+        return int8_paged_attention(q, kv_cache, meta, scale, window)
     _need(q, "q", None, 3)
     _need(kv_cache, "kv_cache", q.dtype, 5)
     t, hq, d = q.shape
@@ -744,7 +749,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out_dtype=None) -> torch.Tenso
     accumulation on the tensor cores, and ``weight`` is a constant: a kernel of this package that is still running
     when the product is launched must not write it; ``out_dtype=torch.float32`` returns the
     accumulator unrounded (used for the logits).  With few rows and a split of k the
-    bfloat16 product comes back as a ``SplitSum`` (see there)."""
+    bfloat16 product comes back as a ``SplitSum`` (see there).  ``weight`` may be an ``Int8Weight``: ``int8_linear``."""
+    if isinstance(weight, Int8Weight):
+        return int8_linear(x, weight, out_dtype)
     if isinstance(x, (GatedSplit, SplitAttention)) and weight.dtype == torch.bfloat16 \
             and tuple(x.shape)[1] == weight.shape[1]:
         from . import gemm_bf16
@@ -776,6 +783,8 @@ def gated_linear(x: torch.Tensor, w_gate_up: torch.Tensor):
     product's epilogue, or, when the product comes back as split-k partials, left to the
     reader (a ``GatedSplit``); otherwise this is ``silu_mul(linear(x, w_gate_up))``."""
     x = as_tensor(x)
+    if isinstance(w_gate_up, Int8Weight):
+        return silu_mul(int8_linear(x, w_gate_up))
     if x.dtype == torch.bfloat16 and x.is_cuda:
         _need(x, "x", None, 2)
         _need(w_gate_up, "w_gate_up", x.dtype, 2)
@@ -2073,3 +2082,9 @@ def masked_attention(q: torch.Tensor, kv_cache: torch.Tensor, meta, scale: float
         _stream())
     _check(st, "masked_attention", f"heads {hq}/{num_kv_heads}, sizes {dk}/{v_head_dim}")
     return out
+
+
+# ---------------------------------------------------------------- 8-bit integers
+
+from .int8 import (Int8Cache, Int8Rows, Int8Weight, int8_cache_read, int8_cache_write, int8_linear,  # noqa: E402,F401
+                   int8_paged_attention, quantize_rows)
