@@ -233,6 +233,69 @@ def int8_cache_read(cache: Int8Cache, slots: torch.Tensor, dtype: torch.dtype = 
     return k, v
 
 
+# ---- the split form's work: one launch for the sequences with one new token, one for those with more
+
+def _pages_fit(page_size: int) -> bool:
+    """Page sizes whose rows the split form copies: a block of 32 keys is whole pages, or lies in one."""
+    return page_size % 32 == 0 or (page_size >= 4 and 32 % page_size == 0)
+
+
+def _most_runs(kv_len: int) -> int:
+    """The most runs of a sequence of at most ``kv_len`` keys (the length on the device may be less than the host's)."""
+    runs, keys = 1, _lib().dib_int8_attention_split_keys
+    for n in {min(kv_len, 2048), min(kv_len, 4096), min(kv_len, 16384), kv_len}:
+        runs = max(runs, -(-n // keys(n, 1)))
+    return runs
+
+
+def _lib():
+    return _ops()._lib("attention_int8")
+
+
+class _SplitPart:
+    """The sequences of one launch: their number, the most rows of one, rows a tile, the most work items of one."""
+
+    def __init__(self, seqs: list, q_lens: list, kv_lens: list, group: int, hkv: int, device):
+        first, count = seqs[0], len(seqs)
+        self.first, self.count, self.list = first, count, None
+        if seqs != list(range(first, first + count)):
+            self.list = torch.tensor(seqs, dtype=torch.int32).to(device, non_blocking=True)
+        self.max_rows = max(q_lens[s] for s in seqs) * group
+        self.tile_rows = 8 if self.max_rows <= 8 else 16
+        runs = _most_runs(max(kv_lens[s] for s in seqs))
+        tiles, per32 = -(-self.max_rows // self.tile_rows), 32 // self.tile_rows
+        # (runs get longer with the rows: tiles * runs is largest at 64 rows, or the tiles' own number is)
+        self.items = hkv * min(tiles * runs, max(2 * per32 * runs, per32 * (runs + 1) + tiles))
+        self.merge = runs > 1
+
+
+def _split_parts(meta, group: int, hkv: int, device) -> list:
+    key = ("int8_split", group, hkv)
+    parts = meta.scratch.get(key)
+    if parts is None:
+        q_lens, kv_lens = meta.q_lens, meta.kv_lens
+        one = [s for s, n in enumerate(q_lens) if n == 1]
+        more = [s for s, n in enumerate(q_lens) if n > 1]
+        parts = [_SplitPart(x, q_lens, kv_lens, group, hkv, device) for x in (one, more) if x]
+        meta.scratch[key] = parts
+    return parts
+
+
+def _split(q, out, cache: Int8Cache, meta, part: _SplitPart, scale: float, window: int) -> None:
+    ops = _ops()
+    pages, _, hkv, page_size, d = cache.shape
+    rows = part.count * part.items * part.tile_rows if part.merge else 0
+    partial = torch.empty(rows * (d + 2), dtype=torch.float32, device=q.device)      # outputs, then (maximum, sum)
+    st = _lib().dib_int8_attention_split(
+        ops._ptr(q), ops._ptr(out), ops._ptr(cache.data), ops._ptr(cache.scales), c_longlong(pages),
+        ops._ptr(meta.block_table), c_int(meta.block_table.shape[1]), ops._ptr(meta.cu_q_lens), ops._ptr(meta.seq_lens),
+        ops._ptr(part.list), c_int(part.first), c_int(part.count), c_int(part.max_rows), c_int(part.tile_rows),
+        ops._ptr(partial), ops._ptr(partial[rows * d:]), c_int(part.items), c_int(1 if part.merge else 0), c_int(q.shape[1]), c_int(hkv),
+        c_int(d), c_int(page_size), c_float(scale), c_int(window), c_int(ops._dt(q, "q")), c_int(_sms(q.device)),
+        ops._stream())
+    ops._check(st, "int8_paged_attention", f"head_dim {d}, heads {q.shape[1]}/{hkv}", kernels=2 if part.merge else 1)
+
+
 def int8_paged_attention(q: torch.Tensor, cache: Int8Cache, meta, scale: float, window=None) -> torch.Tensor:
     """Causal attention of every token of the step over its sequence's keys in the cache, as ``ops.paged_attention``: q
     [T, Hq, D] float32 or bfloat16, ``meta`` the step's ``AttentionMeta``.  A sequence's new tokens are its last ones
@@ -258,6 +321,10 @@ def int8_paged_attention(q: torch.Tensor, cache: Int8Cache, meta, scale: float, 
     _same_device("int8_paged_attention", q, cache.data, meta.block_table, meta.token_seq, meta.cu_q_lens, meta.seq_lens)
     out = torch.empty_like(q)
     if t == 0:
+        return out
+    if d <= 128 and _pages_fit(page_size) and q.data_ptr() % 16 == 0 and pages * 2 * hkv * page_size < 1 << 31:
+        for part in _split_parts(meta, hq // hkv, hkv, q.device):
+            _split(q, out, cache, meta, part, float(scale), win)
         return out
     st = ops._lib("attention_int8").dib_int8_attention_any(
         ops._ptr(q), ops._ptr(out), ops._ptr(cache.data), ops._ptr(cache.scales), ops._ptr(meta.block_table),

@@ -109,6 +109,7 @@ _STATUS_FUNCTIONS = {
     "gemm_fp32": ("dib_gemm_fp32_status", "dib_gemm_fp32_status_clear"),
     "attention_bf16": ("dib_attention_bf16_status", "dib_attention_bf16_status_clear"),
     "attention_prefill_tc": ("dib_attention_prefill_tc_status", "dib_attention_prefill_tc_status_clear"),
+    "attention_int8": ("dib_attention_int8_status", "dib_attention_int8_status_clear"),
 }
 _extra_status: dict = {}
 
