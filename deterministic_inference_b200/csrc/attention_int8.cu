@@ -39,15 +39,18 @@ __device__ __forceinline__ float fast_exp2(float x) {
 // values (TMA, swizzled, a copy a page) and their scales (cp.async), all counted by one mbarrier a stage; the next blocks,
 // of the next work item too, are under way meanwhile.
 //
-// Products by mma.sync m16n8k16 on float16, transposed so that 16 KEYS (or 16 dimensions) are the rows and 8 query rows
-// the columns: S^T = K Q^T, O^T = V^T P^T.  Eight rows fill the instruction, where a decoded token of a group of 2 to 8
-// heads would leave half of it or more empty.  Codes become float16 numbers in registers, exactly: a byte under the
-// exponent byte 0x64 is 1024 + byte.  The k index of a product may be permuted as long as both operands agree: a thread
-// takes 32 (16) consecutive bytes of a key as its share of S's k, and of V 16 (8) consecutive dimensions of the keys
-// that its part of P^T belongs to, so nothing is shuffled but P, by movmatrix.
-// Queries enter scaled by a power of two per row (so that float16 holds them), as one float16 number (bfloat16 queries:
-// exact but for elements below 2^-14 of the row's largest, 2^-25 of it off) or as the sum of two (float32, 22 bits).
-// Probabilities times value scale likewise, against a power of two per row that follows their largest.
+// Products by mma.sync, transposed so that 16 KEYS (or 16 dimensions) are the rows and 8 query rows the columns:
+// S^T = K Q^T, O^T = V^T P^T.  Eight rows fill the instruction, where a decoded token of a group of 2 to 8 heads would
+// leave half of it or more empty.
+//   S: m16n8k32 on the keys' bytes as they are.  A query row enters as integers against its largest element, of 15 bits
+//   (bfloat16) or 22 (float32), as the sum of two or three bytes: an element is off by 2^-15 (2^-22) of the row's largest
+//   at most, and the dot product of the integers is exact.
+//   O: m16n8k16 on float16.  Codes become float16 numbers in registers, exactly: a byte under the exponent byte 0x64 is
+//   1024 + byte.  Probabilities times value scale enter as one float16 number (bfloat16 queries) or the sum of two
+//   (float32), against a power of two per row that follows their largest.
+// The k index of a product may be permuted as long as both operands agree: a thread takes 32 (16) consecutive bytes of a
+// key as its share of S's k, and of V 16 (8) consecutive dimensions of the keys that its part of P^T belongs to, so
+// nothing is shuffled but P, by movmatrix.
 //
 // What bounds it: the bytes of keys and values.  The row's running maximum and its power of two are touched only when a
 // score has passed them by 2^8 (2^12): one vote of the warp a block, no reductions.
@@ -74,6 +77,13 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], unsigned a0, unsigned a1,
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8(int (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
+                                       unsigned b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ unsigned transpose8(unsigned x) {
@@ -111,7 +121,7 @@ struct SplitArgs {
   const int* seq_lens;
   const int* seq_list;          // the sequences of this launch, or null: seq_first ..
   int seq_first, seq_count, max_blocks;
-  int Hq, Hkv, D, page_size, window, box_rows;
+  int Hq, Hkv, D, page_shift, window, box_rows;
   int num_pages;
   float scale;
   float* part_o;                // [seq_count, max_items, 8 NT, D]
@@ -127,7 +137,7 @@ template <int ROWS> __device__ __forceinline__ SplitSeq split_seq(const SplitArg
   s.seq = a.seq_list != nullptr ? a.seq_list[i] : a.seq_first + i;
   s.q_begin = a.cu_q_lens[s.seq];
   s.n = a.cu_q_lens[s.seq + 1] - s.q_begin;
-  s.kv_len = min(a.seq_lens[s.seq], (int)min((long long)a.max_blocks * a.page_size, 0x7fffffc0ll));
+  s.kv_len = min(a.seq_lens[s.seq], (int)min((long long)a.max_blocks << a.page_shift, 0x7fffffc0ll));
   const int rows = s.n * (a.Hq / a.Hkv);
   s.tiles = (rows + ROWS - 1) / ROWS;
   s.split = split_keys(s.kv_len, rows);
@@ -137,13 +147,22 @@ template <int ROWS> __device__ __forceinline__ SplitSeq split_seq(const SplitArg
 
 template <typename T, int DP, int NT> struct SplitShape {
   static constexpr int ROWS = 8 * NT;
-  static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;       // float16 numbers a query or probability is the sum of
-  static constexpr int STAGES = 2;
-  static constexpr int TILE = SP_BLOCK * DP, STAGE = 2 * TILE + 256;      // keys, values, their scales
-  static constexpr int RING = (STAGES * STAGE + 1023) / 1024 * 1024;
-  // (a stage's tiles lie on 1,024 bytes: all stages' tiles first, then the scales)
+  static constexpr int Q_PARTS = sizeof(T) == 4 ? 3 : 2;     // bytes a query's element is the sum of
+  static constexpr int P_PARTS = sizeof(T) == 4 ? 2 : 1;     // float16 numbers a probability is the sum of
+  static constexpr int STAGES = 2, QUEUE = 4;
+  static constexpr int TILE = SP_BLOCK * DP;                 // a block's keys, or values
+  // a warp's ring: the stages' tiles (each on 1,024 bytes), then the stages' scales
   static constexpr int SCALES = STAGES * 2 * TILE;
-  static constexpr size_t fixed = (size_t)SP_WARPS * RING + SP_WARPS * STAGES * 8 + 1024;
+  static constexpr int RING = (SCALES + STAGES * 256 + 1023) / 1024 * 1024;
+  static constexpr size_t fixed = (size_t)SP_WARPS * (RING + STAGES * 8 + QUEUE * 32) + 1024;
+};
+
+// A work item as it is handed from the end of a warp's pipe that fetches to the one that computes.
+struct __align__(16) SplitItem {
+  int i, kvh, tile;             // sequence of the launch, kv head, tile of rows
+  int lo;                       // first key of the run
+  int at, end;                  // its keys [at, end), `at` a multiple of 32 and perhaps below the first one seen
+  int out_item, unused;         // number of the item among its sequence's
 };
 
 template <typename T, int DP, int NT>
@@ -151,14 +170,16 @@ __global__ void __launch_bounds__(SP_WARPS * 32)
 attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restrict__ q, T* __restrict__ out,
                        const __grid_constant__ SplitArgs a) {
   using SH = SplitShape<T, DP, NT>;
-  constexpr int ROWS = SH::ROWS, PARTS = SH::PARTS, STAGES = SH::STAGES, KS = DP / 16, MT = DP / 16;
-  constexpr int WORDS = DP / 16;            // 32-bit words of a thread's share of a key, and twice that of a value's
+  constexpr int ROWS = SH::ROWS, Q_PARTS = SH::Q_PARTS, P_PARTS = SH::P_PARTS, STAGES = SH::STAGES, QUEUE = SH::QUEUE;
+  constexpr int MT = DP / 16, WORDS = DP / 16;      // 32-bit words of a thread's share of a key
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   unsigned char* ring = smem + warp * SH::RING;
-  unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + SP_WARPS * SH::RING) + warp * STAGES;
-  int* first = reinterpret_cast<int*>(smem + SP_WARPS * SH::RING + SP_WARPS * STAGES * 8);    // [seq_count + 1]
+  SplitItem* queue = reinterpret_cast<SplitItem*>(smem + SP_WARPS * SH::RING) + warp * QUEUE;
+  unsigned long long* bars =
+      reinterpret_cast<unsigned long long*>(smem + SP_WARPS * (SH::RING + QUEUE * 32)) + warp * STAGES;
+  int* first = reinterpret_cast<int*>(smem + SP_WARPS * (SH::RING + QUEUE * 32 + STAGES * 8));    // [seq_count + 1]
   if (threadIdx.x == 0) prefetch_tensormap(&map);
   pdl_trigger();
   // ---- the items before each sequence (metadata alone, which no kernel of a step writes)
@@ -189,111 +210,126 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
   const int total = first[a.seq_count];
   const int G = a.Hq / a.Hkv;
   const int stride = gridDim.x * SP_WARPS;
+  const int page_mask = (1 << a.page_shift) - 1;
 
-  // ---- a cursor over this warp's items and their blocks of keys
-  struct Cursor {
-    int item, at, end;          // item number; the next block's first key; the end of the item's keys
-    int i, kvh, tile, run;      // sequence of the launch, kv head, tile of rows, run of keys
-    SplitSeq s;
-  };
-  // the item's keys that some row of the tile sees: [at, end), at a multiple of 32 from key 0
-  auto open = [&](Cursor& c) {
-    for (; c.item < total; c.item += stride) {
+  // ---- the end that fetches: its item, the block of keys to be sent for next, this lane's page of it
+  int f_item = warp * gridDim.x + blockIdx.x, f_at = 0, f_end = 0, f_head = 0, f_page = -1, opened = 0;
+  const int* f_table = nullptr;
+  // the item f_item, or the first one behind it that has keys (on this warp's list); f_item >= total: none is left
+  auto open = [&]() {
+    for (; f_item < total; f_item += stride) {
       int lo = 0, hi = a.seq_count - 1;          // the sequence whose items hold this one
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (first[mid] <= c.item) lo = mid; else hi = mid - 1;
+        if (first[mid] <= f_item) lo = mid; else hi = mid - 1;
       }
-      c.i = lo;
-      c.s = split_seq<ROWS>(a, lo);
-      int r = c.item - first[lo];
-      c.tile = r % c.s.tiles;
-      r /= c.s.tiles;
-      c.run = r % c.s.splits;
-      c.kvh = r / c.s.splits;
-      const int p0 = c.s.kv_len - c.s.n;
-      const int tok0 = c.tile * ROWS / G, tok1 = min((c.tile + 1) * ROWS - 1, c.s.n * G - 1) / G;
-      const int k_lo = max(c.run * c.s.split, first_visible_key(p0 + tok0, a.window));
-      const int k_hi = min((c.run + 1) * c.s.split, p0 + tok1 + 1);
-      c.at = k_lo & ~(SP_BLOCK - 1);
-      c.end = k_hi;
-      if (k_hi > k_lo || c.s.splits == 1) return;      // (a sequence of one run: its rows are written here, even as zeros)
+      const SplitSeq s = split_seq<ROWS>(a, lo);
+      const int local = f_item - first[lo];
+      int r = local, tile = 0;
+      if (s.tiles > 1) {
+        tile = r % s.tiles;
+        r /= s.tiles;
+      }
+      const int kvh = r / s.splits, run_at = (r - kvh * s.splits) * s.split;
+      const int p0 = s.kv_len - s.n, n_rows = s.n * G;
+      int tok0 = 0, tok1 = s.n - 1;
+      if (s.tiles > 1) {
+        tok0 = tile * ROWS / G;
+        tok1 = min((tile + 1) * ROWS, n_rows) - 1;
+        tok1 /= G;
+      }
+      const int k_lo = max(run_at, first_visible_key(p0 + tok0, a.window)), k_hi = min(run_at + s.split, p0 + tok1 + 1);
+      if (k_hi > k_lo) {
+        f_at = k_lo & ~(SP_BLOCK - 1);
+        f_end = k_hi;
+        f_table = a.block_table + (long long)s.seq * a.max_blocks;
+        f_head = kvh << a.page_shift;
+        __syncwarp();
+        if (lane == 0) {
+          SplitItem it;
+          it.i = lo; it.kvh = kvh; it.tile = tile; it.lo = run_at;
+          it.at = f_at; it.end = f_end; it.out_item = local; it.unused = 0;
+          queue[opened % QUEUE] = it;
+        }
+        __syncwarp();
+        ++opened;
+        return;
+      }
+      if (s.splits == 1)                         // a sequence of one run: rows that see no key are zeros, from here
+        for (int e = lane; e < min(ROWS, n_rows - tile * ROWS) * a.D; e += 32) {
+          const int row = tile * ROWS + e / a.D;
+          Elem<T>::store(out + ((long long)(s.q_begin + row / G) * a.Hq + kvh * G + row % G) * a.D + e % a.D, 0.f);
+        }
     }
   };
-  auto page_of = [&](const Cursor& c) {               // this lane's page of the cursor's block, or -1
-    const int key = c.at + lane;
+  auto look_up = [&]() {                         // this lane's page of the block at f_at, or -1
+    const int key = f_at + lane;
     int page = -1;
-    if (c.item < total && key < c.end) page = a.block_table[(long long)c.s.seq * a.max_blocks + key / a.page_size];
-    return page < a.num_pages ? page : -1;
+    if (key < f_end) page = f_table[key >> a.page_shift];
+    f_page = page < a.num_pages ? page : -1;
   };
-  // the block at the cursor -> stage: lane l's key is at + l; the first lane of each page sends for its rows
-  auto fetch = [&](const Cursor& c, int page, int stage) {
-    unsigned char* tiles = ring + stage * 2 * SH::TILE;
-    float* sc = reinterpret_cast<float*>(ring + SH::SCALES) + stage * 64;
-    const int key = c.at + lane, off = key % a.page_size;
-    const bool have = page >= 0;
+  // the block -> stage: lane l's key is f_at + l; the first lane of each page sends for its rows
+  auto fetch = [&](int stage) {
+    const unsigned tiles = smem_u32(ring) + stage * 2 * SH::TILE;
+    const unsigned sc = smem_u32(ring) + SH::SCALES + stage * 256 + lane * 4;
+    const int off = (f_at + lane) & page_mask;
+    const bool have = f_page >= 0;
     const bool sends = have && (lane == 0 || off == 0);
     const unsigned senders = __ballot_sync(0xffffffffu, sends);
     if (lane == 0) mbar_expect_tx(&bars[stage], __popc(senders) * 2 * a.box_rows * DP);
     __syncwarp();
-    const long long row = ((long long)page * 2 * a.Hkv + c.kvh) * a.page_size + off;
-    const long long vrow = row + (long long)a.Hkv * a.page_size;
+    const int half = a.Hkv << a.page_shift;      // rows of a page's keys
+    const int row = f_page * 2 * half + f_head + off;
     if (sends) {
-      tma_load_2d(smem_u32(tiles) + lane * DP, &map, 0, (int)row, &bars[stage]);
-      tma_load_2d(smem_u32(tiles) + SH::TILE + lane * DP, &map, 0, (int)vrow, &bars[stage]);
+      tma_load_2d(tiles + lane * DP, &map, 0, row, &bars[stage]);
+      tma_load_2d(tiles + SH::TILE + lane * DP, &map, 0, row + half, &bars[stage]);
     }
     if (have) {
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(sc + lane)), "l"(a.scales + row) : "memory");
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(sc + 32 + lane)), "l"(a.scales + vrow) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc), "l"(a.scales + row) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc + 128), "l"(a.scales + row + half) : "memory");
     }
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bars[stage])) : "memory");
+    f_at += SP_BLOCK;
+    if (f_at >= f_end) {
+      f_item += stride;
+      open();
+    }
+    if (f_item < total) look_up();
   };
 
-  Cursor f;                                            // what is fetched next
-  f.item = warp * gridDim.x + blockIdx.x;
-  open(f);
-  int f_page = page_of(f);
-  auto step = [&]() {                                  // the fetch cursor to the next block that holds keys
-    if (f.item >= total) return;
-    f.at += SP_BLOCK;
-    while (f.at >= f.end) {
-      f.item += stride;
-      open(f);
-      if (f.item >= total) return;
-      if (f.at < f.end) break;
-    }
-    f_page = page_of(f);
-  };
   pdl_wait(q);
-  // (an item without keys has no block: skip it here as `step` does)
-  if (f.item < total && f.at >= f.end) {
-    f.at -= SP_BLOCK;
-    step();
-  }
-  int sent = 0;                                        // blocks sent for
-  for (int s = 0; s < STAGES; ++s) {
-    if (f.item < total) {
-      fetch(f, f_page, s);
-      ++sent;
-      step();
-    }
+  open();
+  if (f_item < total) look_up();
+  int sent = 0, used = 0;                          // blocks sent for, consumed
+  for (; sent < STAGES && f_item < total; ++sent) fetch(sent);
+
+  // where a lane finds its pieces of a tile (the copy's swizzle: bits 4.. of the address joined by bits 7..)
+  constexpr int SWIZZLE = DP == 128 ? 7 : 3, LINE = DP == 128 ? 1 : 2;      // rows of 128 bytes hold LINE keys
+  int k_off[WORDS / 4], v_off[2];
+#pragma unroll
+  for (int p = 0; p < WORDS / 4; ++p)
+    k_off[p] = g * DP + (((t * (WORDS / 4) + p) ^ ((g / LINE) & SWIZZLE)) << 4);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int r = 2 * t + e;
+    v_off[e] = DP == 128 ? r * DP + ((g ^ (r & 7)) << 4) : r * DP + (((g >> 1) ^ ((r >> 1) & 3)) << 4) + (g & 1) * 8;
   }
 
   bool ok = true;
-  int used = 0;                                        // blocks consumed
-  Cursor c;
-  c.item = warp * gridDim.x + blockIdx.x;
-  for (open(c); c.item < total && ok; c.item += stride, open(c)) {
-    const int p0 = c.s.kv_len - c.s.n, row0 = c.tile * ROWS, rows = min(ROWS, c.s.n * G - row0);
-    // ---- queries: row g of tile nt as the B operand; this thread's share of the dimensions
-    unsigned qf[NT][PARTS][KS][2];
+  for (int taken = 0; ok && taken < opened; ++taken) {
+    const SplitItem it = queue[taken % QUEUE];
+    const SplitSeq s_ = split_seq<ROWS>(a, it.i);
+    const int p0 = s_.kv_len - s_.n, row0 = it.tile * ROWS, rows = min(ROWS, s_.n * G - row0);
+    // ---- queries: row g of tile nt as the B operand, this thread's share of the dimensions, as the sum of Q_PARTS bytes
+    // of 7 bits each against the row's largest element
+    unsigned qf[NT][Q_PARTS][WORDS];
     float q_unit[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = nt * 8 + g;
       const bool in = r < rows;
-      const int tok = in ? (row0 + r) / G : 0, h = c.kvh * G + (in ? (row0 + r) % G : 0);
-      const T* src = q + ((long long)(c.s.q_begin + tok) * a.Hq + h) * a.D + t * (DP / 4);
+      const int tok = in ? (row0 + r) / G : 0, h = in ? row0 + r - tok * G : 0;
+      const T* src = q + ((long long)(s_.q_begin + tok) * a.Hq + it.kvh * G + h) * a.D + t * (DP / 4);
       float x[DP / 4];
 #pragma unroll
       for (int v = 0; v < DP / 4; v += 16 / (int)sizeof(T)) {
@@ -310,27 +346,38 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
           }
         }
       }
-      float top = 0.f;
+      unsigned bits = 0;
 #pragma unroll
-      for (int d = 0; d < DP / 4; ++d) top = fmaxf(top, fabsf(x[d]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);      // 2^(e - 127) <= top
-      const float down = __uint_as_float((unsigned)(254 - e) << 23);
-      q_unit[nt] = a.scale * LOG2E * __uint_as_float((unsigned)e << 23);
+      for (int d = 0; d < DP / 4; ++d) bits = max(bits, __float_as_uint(x[d]) & 0x7fffffffu);
+      bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
+      bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
+      const float top = fmaxf(__uint_as_float(bits), 0x1p-100f);
+      constexpr float MOST = Q_PARTS == 3 ? 127.f * 16384.f : 127.f * 128.f;
+      const float up = MOST / top;
+      // (a row that holds an infinity or a NaN: its unit is NaN, and so is all that comes of it)
+      q_unit[nt] = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.scale * LOG2E * (top / MOST);
 #pragma unroll
-      for (int j = 0; j < KS; ++j)
+      for (int j = 0; j < WORDS; ++j) {
+        int part[4][3];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const float y0 = x[4 * j + 2 * b] * down, y1 = x[4 * j + 2 * b + 1] * down;
-          qf[nt][0][j][b] = pack_f16(y0, y1);
-          if (PARTS == 2)
-            qf[nt][PARTS - 1][j][b] = pack_f16(y0 - low_of(qf[nt][0][j][b]), y1 - high_of(qf[nt][0][j][b]));
+        for (int b = 0; b < 4; ++b) {
+          int v = __float2int_rn(x[4 * j + b] * up);
+          if (Q_PARTS == 3) {
+            const int above = (v + 64) >> 7;
+            part[b][2] = v - above * 128;
+            v = above;
+          }
+          part[b][0] = (v + 64) >> 7;
+          part[b][1] = v - part[b][0] * 128;
         }
+#pragma unroll
+        for (int p = 0; p < Q_PARTS; ++p)
+          qf[nt][p][j] = __byte_perm(__byte_perm(part[0][p], part[1][p], 0x0040), __byte_perm(part[2][p], part[3][p], 0x0040), 0x5410);
+      }
     }
     // ---- what belongs to the rows this thread has scores of: 2t and 2t + 1 of each tile
     float unit[NT][2], m[NT][2], l[NT][2], w_unit[NT][2];
-    int k_lo[NT][2], k_hi[NT][2], lo_all = 0, hi_all = 0x7fffffff;
+    int k_lo[NT][2], k_hi[NT][2], lo_all = it.lo, hi_all = it.end - 1;
     float o[NT][MT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -340,9 +387,9 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
         const bool in = r < rows;
         const int p = p0 + (in ? (row0 + r) / G : 0);
         unit[nt][e] = __shfl_sync(0xffffffffu, q_unit[nt], (2 * t + e) * 4);
-        k_lo[nt][e] = first_visible_key(p, a.window);
-        k_hi[nt][e] = in ? p : -1;
-        if (in) {
+        k_lo[nt][e] = max(first_visible_key(p, a.window), it.lo);
+        k_hi[nt][e] = in ? min(p, it.end - 1) : -1;
+        if (in) {        // (rows of the tile beyond the sequence's last one: their scores are never looked at)
           lo_all = max(lo_all, k_lo[nt][e]);
           hi_all = min(hi_all, p);
         }
@@ -355,9 +402,6 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       lo_all = max(lo_all, __shfl_xor_sync(0xffffffffu, lo_all, o_));
       hi_all = min(hi_all, __shfl_xor_sync(0xffffffffu, hi_all, o_));
     }
-    // (rows of the tile beyond the sequence's last one count for nothing: their scores are never looked at)
-    lo_all = max(lo_all, c.run * c.s.split);
-    hi_all = min(hi_all, c.end - 1);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -365,7 +409,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
 
-    for (int kb = c.at; kb < c.end; kb += SP_BLOCK, ++used) {
+    for (int kb = it.at; kb < it.end; kb += SP_BLOCK, ++used) {
       const int stage = used % STAGES;
       ok = mbar_wait(&bars[stage], (used / STAGES) & 1);
       ok = __all_sync(0xffffffffu, ok);
@@ -373,40 +417,39 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       const unsigned char* kt = ring + stage * 2 * SH::TILE;
       const unsigned char* vt = kt + SH::TILE;
       const float* sc = reinterpret_cast<const float*>(ring + SH::SCALES) + stage * 64;
-      // 16-byte piece p of row r of a tile (the swizzle of the copy: the address' bits 7.. join bits 4..)
-      auto piece = [&](const unsigned char* tile, int r, int p) {
-        const int at = r * DP + p * 16;
-        return *reinterpret_cast<const uint4*>(tile + (at ^ ((at >> 3) & (DP == 128 ? 0x70 : 0x30))));
-      };
-      // ---- S^T
+      // ---- S^T, an exact integer
       float s[2][NT][4];
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
-        unsigned kw[2][WORDS];
+        uint4 kw[2][WORDS / 4];
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int p = 0; p < WORDS / 4; ++p) {
-            const uint4 v = piece(kt, mt * 16 + half * 8 + g, t * (WORDS / 4) + p);
-            kw[half][p * 4] = v.x ^ 0x80808080u;
-            kw[half][p * 4 + 1] = v.y ^ 0x80808080u;
-            kw[half][p * 4 + 2] = v.z ^ 0x80808080u;
-            kw[half][p * 4 + 3] = v.w ^ 0x80808080u;
-          }
+          for (int p = 0; p < WORDS / 4; ++p)
+            kw[half][p] = *reinterpret_cast<const uint4*>(kt + (mt * 16 + half * 8) * DP + k_off[p]);
+        int acc[NT][Q_PARTS][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
+          for (int p = 0; p < Q_PARTS; ++p)
 #pragma unroll
-        for (int j = 0; j < KS; ++j) {
-          const unsigned a0 = half2_of(kw[0][j], 0x4140), a1 = half2_of(kw[1][j], 0x4140);
-          const unsigned a2 = half2_of(kw[0][j], 0x4342), a3 = half2_of(kw[1][j], 0x4342);
+            for (int e = 0; e < 4; ++e) acc[nt][p][e] = 0;
+#pragma unroll
+        for (int p4 = 0; p4 < WORDS / 4; ++p4)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int p = PARTS - 1; p >= 0; --p)       // the small part first
-              mma_f16(s[mt][nt], a0, a1, a2, a3, qf[nt][p][j][0], qf[nt][p][j][1]);
-        }
+            for (int p = 0; p < Q_PARTS; ++p) {
+              mma_s8(acc[nt][p], kw[0][p4].x, kw[1][p4].x, kw[0][p4].y, kw[1][p4].y, qf[nt][p][p4 * 4], qf[nt][p][p4 * 4 + 1]);
+              mma_s8(acc[nt][p], kw[0][p4].z, kw[1][p4].z, kw[0][p4].w, kw[1][p4].w, qf[nt][p][p4 * 4 + 2], qf[nt][p][p4 * 4 + 3]);
+            }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float high = (float)(acc[nt][0][e] * 128 + acc[nt][1][e]);
+            s[mt][nt][e] = Q_PARTS == 3 ? fmaf(high, 128.f, (float)acc[nt][Q_PARTS - 1][e]) : high;
+          }
       }
       float ks[2][2], vs[2][2];
 #pragma unroll
@@ -417,35 +460,37 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
           vs[mt][half] = sc[32 + mt * 16 + half * 8 + g];
         }
       const bool plain = kb >= lo_all && kb + SP_BLOCK - 1 <= hi_all;      // every row sees every key
+      float top[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          top[nt][e] = -INFINITY;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) s[mt][nt][2 * half + e] *= ks[mt][half] * unit[nt][e];
+        }
       if (!plain) {
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int half = 0; half < 2; ++half)         // a row of the cache that is not there may hold anything
-            if (kb + mt * 16 + half * 8 + g >= c.end || kb + mt * 16 + half * 8 + g < c.run * c.s.split) {
-              ks[mt][half] = 0.f;
-              vs[mt][half] = 0.f;
-            }
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                const int key = kb + mt * 16 + half * 8 + g;
+                if (key < k_lo[nt][e] || key > k_hi[nt][e]) s[mt][nt][2 * half + e] = -INFINITY;
+              }
       }
       bool high = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float top = -INFINITY;
-#pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              float& x = s[mt][nt][2 * half + e];
-              x *= ks[mt][half] * unit[nt][e];
-              if (!plain) {
-                const int key = kb + mt * 16 + half * 8 + g;
-                if (key < max(k_lo[nt][e], c.run * c.s.split) || key > k_hi[nt][e] || key >= c.end) x = -INFINITY;
-              }
-              top = fmaxf(top, x);
-            }
-          high |= top > m[nt][e] + 8.f;
+          top[nt][e] = fmaxf(fmaxf(s[0][nt][e], s[0][nt][2 + e]), fmaxf(s[1][nt][e], s[1][nt][2 + e]));
+          high |= top[nt][e] > m[nt][e] + 8.f;
         }
       if (__any_sync(0xffffffffu, high)) {
         // some row's reference maximum rises (each row by its own scores alone)
@@ -453,23 +498,22 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(fmaxf(s[0][nt][e], s[0][nt][2 + e]), fmaxf(s[1][nt][e], s[1][nt][2 + e]));
+            float best = top[nt][e];
 #pragma unroll
-            for (int o_ = 4; o_ < 32; o_ <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o_));
+            for (int o_ = 4; o_ < 32; o_ <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o_));
             float factor = 1.f;
-            if (top > m[nt][e] + 8.f) {
-              factor = fast_exp2(m[nt][e] - top);      // (zero from minus infinity)
-              m[nt][e] = top;
+            if (best > m[nt][e] + 8.f) {
+              factor = fast_exp2(m[nt][e] - best);     // (zero from minus infinity)
+              m[nt][e] = best;
               l[nt][e] *= factor;
-              // the probabilities' power of two is chosen anew: 1 / the largest probability * scale of the block
+              // the probabilities' power of two is chosen anew: by the block's largest probability * scale
               float wt = 0.f;
 #pragma unroll
               for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                 for (int half = 0; half < 2; ++half)
-                  wt = fmaxf(wt, fast_exp2(s[mt][nt][2 * half + e] - top) * vs[mt][half]);
-              // (every lane of a row takes this branch)
-              const unsigned lanes = 0x11111111u << t;
+                  wt = fmaxf(wt, fast_exp2(s[mt][nt][2 * half + e] - best) * vs[mt][half]);
+              const unsigned lanes = 0x11111111u << t;      // (every lane of a row takes this branch)
 #pragma unroll
               for (int o_ = 4; o_ < 32; o_ <<= 1) wt = fmaxf(wt, __shfl_xor_sync(lanes, wt, o_));
               const float now = unit_of(wt);
@@ -493,18 +537,27 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float ref = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
+          float most = 0.f;
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              const float x = s[mt][nt][2 * half + e];
-              const float p = fast_exp2(x - ref);
+              const float p = fast_exp2(s[mt][nt][2 * half + e] - ref);
               l[nt][e] += p;
-              // (a key that the row does not see may have a value that is no number)
-              w[mt][nt][2 * half + e] = x == -INFINITY ? 0.f : p * vs[mt][half];
-              large |= w[mt][nt][2 * half + e] * w_unit[nt][e] > 4096.f;
+              w[mt][nt][2 * half + e] = p * (vs[mt][half] * w_unit[nt][e]);
+              most = fmaxf(most, w[mt][nt][2 * half + e]);
             }
+          large |= most > 4096.f;
         }
+      if (!plain) {        // a key that the row does not see may have a value that is no number
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (s[mt][nt][e] == -INFINITY) w[mt][nt][e] = 0.f;
+      }
       if (__any_sync(0xffffffffu, large)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -514,10 +567,12 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
 #pragma unroll
             for (int o_ = 4; o_ < 32; o_ <<= 1) wt = fmaxf(wt, __shfl_xor_sync(0xffffffffu, wt, o_));
             float factor = 1.f;
-            if (wt * w_unit[nt][e] > 4096.f) {
-              const float now = unit_of(wt);
-              factor = now / w_unit[nt][e];
-              w_unit[nt][e] = now;
+            if (wt > 4096.f) factor = unit_of(wt);      // (of the product with the old unit)
+            w_unit[nt][e] *= factor;
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+              w[mt][nt][e] *= factor;
+              w[mt][nt][2 + e] *= factor;
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
@@ -529,30 +584,29 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       // ---- O^T += V^T P^T, 16 keys at a time
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
-        unsigned pf[NT][PARTS][2];
+        unsigned pf[NT][P_PARTS][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const float w0 = w[mt][nt][2 * half] * w_unit[nt][0], w1 = w[mt][nt][2 * half + 1] * w_unit[nt][1];
+            const float w0 = w[mt][nt][2 * half], w1 = w[mt][nt][2 * half + 1];
             const unsigned hi = pack_f16(w0, w1);
             pf[nt][0][half] = transpose8(hi);
-            if (PARTS == 2) pf[nt][PARTS - 1][half] = transpose8(pack_f16(w0 - low_of(hi), w1 - high_of(hi)));
+            if (P_PARTS == 2) pf[nt][P_PARTS - 1][half] = transpose8(pack_f16(w0 - low_of(hi), w1 - high_of(hi)));
           }
         // the thread's 16 (8) dimensions of the keys 2t, 2t + 1, 2t + 8, 2t + 9
         unsigned vw[4][DP / 32];
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
-          const int r = mt * 16 + 2 * t + (kk & 1) + (kk >> 1) * 8;
+          const unsigned char* src = vt + (mt * 16 + (kk >> 1) * 8) * DP + v_off[kk & 1];
           if (DP == 128) {
-            const uint4 v = piece(vt, r, g);
+            const uint4 v = *reinterpret_cast<const uint4*>(src);
             vw[kk][0] = v.x ^ 0x80808080u;
             vw[kk][1] = v.y ^ 0x80808080u;
             vw[kk][DP / 32 - 2] = v.z ^ 0x80808080u;
             vw[kk][DP / 32 - 1] = v.w ^ 0x80808080u;
           } else {
-            const int at = r * DP + g * 8;
-            const uint2 v = *reinterpret_cast<const uint2*>(vt + (at ^ ((at >> 3) & 0x30)));
+            const uint2 v = *reinterpret_cast<const uint2*>(src);
             vw[kk][0] = v.x ^ 0x80808080u;
             vw[kk][1] = v.y ^ 0x80808080u;
           }
@@ -566,17 +620,16 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int p = PARTS - 1; p >= 0; --p) {
+            for (int p = P_PARTS - 1; p >= 0; --p) {       // the small part first
               mma_f16(o[nt][2 * c4], a0, a1, a2, a3, pf[nt][p][0], pf[nt][p][1]);
               mma_f16(o[nt][2 * c4 + 1], b0, b1, b2, b3, pf[nt][p][0], pf[nt][p][1]);
             }
         }
       }
       __syncwarp();                                    // every lane has read the stage
-      if (f.item < total) {
-        fetch(f, f_page, stage);
+      if (f_item < total) {
+        fetch(stage);
         ++sent;
-        step();
       }
     }
     if (!ok) break;
@@ -593,9 +646,10 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
         const float back = 1.f / w_unit[nt][e];
         const int d0 = g * (DP / 8);
         if (d0 >= a.D) continue;
-        if (c.s.splits == 1) {
+        if (s_.splits == 1) {
           const float inv = sum == 0.f ? 0.f : back / sum;
-          T* dst = out + ((long long)(c.s.q_begin + (row0 + r) / G) * a.Hq + c.kvh * G + (row0 + r) % G) * a.D + d0;
+          const int tok = (row0 + r) / G;
+          T* dst = out + ((long long)(s_.q_begin + tok) * a.Hq + it.kvh * G + row0 + r - tok * G) * a.D + d0;
 #pragma unroll
           for (int i = 0; i < MT; i += 2) {
             if (d0 + 2 * i >= a.D) break;
@@ -608,9 +662,8 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
               *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(y0, y1, y2, y3);
             }
           }
-        } else {
-          if (c.item - first[c.i] >= a.max_items) continue;
-          const long long at = ((long long)c.i * a.max_items + (c.item - first[c.i])) * ROWS + r;
+        } else if (it.out_item < a.max_items) {
+          const long long at = ((long long)it.i * a.max_items + it.out_item) * ROWS + r;
           float* dst = a.part_o + at * a.D + d0;
 #pragma unroll
           for (int i = 0; i < MT; i += 2) {
@@ -837,8 +890,8 @@ int dib_attention_int8_status_clear() {
 // Keys of a run of the split form, for a sequence of kv_len keys and `rows` rows (new tokens x query heads of a kv head).
 int dib_int8_attention_split_keys(int kv_len, int rows) { return split_keys(kv_len, rows); }
 
-// The split form, for the sequences seq_list[0 .. seq_count) or (null) seq_first ...: heads up to 128, pages of 4, 8, 16
-// or a multiple of 32 rows.  max_rows: the most rows (new tokens x query heads of a kv head) of one of them; tile_rows: 8
+// The split form, for the sequences seq_list[0 .. seq_count) or (null) seq_first ...: heads up to 128, pages of a
+// power of two of rows, 4 at least.  max_rows: the most rows (new tokens x query heads of a kv head) of one of them; tile_rows: 8
 // or 16 rows a tile; max_items: the most (tiles x runs x kv heads) of one; part_o float32 [seq_count, max_items,
 // tile_rows, D] and part_ml [.., 2] take partial results where merge is not 0 (some sequence may have two runs).
 int dib_int8_attention_split(const void* q, void* out, const void* data, const void* scales, long long num_pages,
@@ -847,7 +900,7 @@ int dib_int8_attention_split(const void* q, void* out, const void* data, const v
                              void* part_ml, int max_items, int merge, int Hq, int Hkv, int D, int page_size, float scale,
                              int window, int dtype, int sm_count, cudaStream_t st) {
   if (dtype != 0 && dtype != 1) return DIB_BAD_DTYPE;
-  const bool pages_fit = page_size % 32 == 0 || (page_size >= 4 && 32 % page_size == 0);
+  const bool pages_fit = page_size >= 4 && (page_size & (page_size - 1)) == 0;
   if (seq_count < 0 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || D < 16 || D > 128 || D % 16 != 0 || page_size < 1 || !pages_fit ||
       num_pages * 2 * Hkv * page_size >= (1ll << 31) || seq_count > 65535 || max_items < 1 || sm_count < 1 ||
       (tile_rows != 8 && tile_rows != 16))
@@ -864,7 +917,9 @@ int dib_int8_attention_split(const void* q, void* out, const void* data, const v
   a.seq_first = seq_first;
   a.seq_count = seq_count;
   a.max_blocks = max_blocks;
-  a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.page_size = page_size; a.window = window;
+  a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.window = window;
+  a.page_shift = 0;
+  while ((1 << a.page_shift) < page_size) ++a.page_shift;
   a.box_rows = page_size < SP_BLOCK ? page_size : SP_BLOCK;
   a.scale = scale;
   a.part_o = reinterpret_cast<float*>(part_o);

@@ -236,8 +236,8 @@ def int8_cache_read(cache: Int8Cache, slots: torch.Tensor, dtype: torch.dtype = 
 # ---- the split form's work: one launch for the sequences with one new token, one for those with more
 
 def _pages_fit(page_size: int) -> bool:
-    """Page sizes whose rows the split form copies: a block of 32 keys is whole pages, or lies in one."""
-    return page_size % 32 == 0 or (page_size >= 4 and 32 % page_size == 0)
+    """Page sizes that the split form takes: a block of 32 keys is whole pages, or lies in one."""
+    return page_size >= 4 and page_size & (page_size - 1) == 0
 
 
 def _most_runs(kv_len: int) -> int:
