@@ -34,84 +34,113 @@ __device__ __forceinline__ float fast_exp2(float x) {
 }
 
 // ---------------------------------------------------------------- split form
-// A sequence's rows (new token, query head of the kv group), 8 NT at a time, against a run of its keys, by ONE warp: no
-// warp waits for another.  Per block of 32 keys a warp holds, in its own ring of shared memory, the codes of the keys and
-// values (TMA, swizzled, a copy a page) and their scales (cp.async), all counted by one mbarrier a stage; the next blocks,
-// of the next work item too, are under way meanwhile.
+// A sequence's rows (new token, query head of the kv group), ROWS at a time, against a run of its keys, by one CTA, in
+// tiles of 128 keys.  Both products run on the tensor cores' 8-bit integers (tcgen05.mma kind::i8) and read keys and
+// values from shared memory as the copies left them: nothing is converted, whatever the number of rows.
+//   S^T = K Q^T:  A = the keys' tile (128 keys x 128 bytes, K-major), B = the query rows as integers against their largest
+//     element, each the sum of PARTS bytes of 7 bits (2 for bfloat16 queries, 4 for float32), a column of B a byte.
+//     Lane k of the accumulator holds key k's exact integer dot products with all rows.
+//   O^T = V^T P^T: A = the values' tile read MN-major (128 dimensions), B = the weights w = p vs, p = 2^(s - L), as
+//     integers against the tile's largest one of the row, again PARTS bytes each (MN-major, a thread writes its key's).
+//     Lane d holds dimension d's integers for all rows.
+// An integer of 15 (28) bits against the largest weight of 128 keys: what the others lose is 2^-16 (2^-29) of it each at
+// most, 0.2 % of a tile's sum in the worst case and 2^-9 of a weight that matters, like a bfloat16 probability's.  The
+// integers are then scaled and added up in float32.  L, the reference of a row's probabilities, follows the tiles'
+// largest weights and is raised only when they have left it by 2^20: float32 holds what lies between.
 //
-// Products by mma.sync, transposed so that 16 KEYS (or 16 dimensions) are the rows and 8 query rows the columns:
-// S^T = K Q^T, O^T = V^T P^T.  Eight rows fill the instruction, where a decoded token of a group of 2 to 8 heads would
-// leave half of it or more empty.
-//   S: m16n8k32 on the keys' bytes as they are.  A query row enters as integers against its largest element, of 15 bits
-//   (bfloat16) or 22 (float32), as the sum of two or three bytes: an element is off by 2^-15 (2^-22) of the row's largest
-//   at most, and the dot product of the integers is exact.
-//   O: m16n8k16 on float16.  Codes become float16 numbers in registers, exactly: a byte under the exponent byte 0x64 is
-//   1024 + byte.  Probabilities times value scale enter as one float16 number (bfloat16 queries) or the sum of two
-//   (float32), against a power of two per row that follows their largest.
-// The k index of a product may be permuted as long as both operands agree: a thread takes 32 (16) consecutive bytes of a
-// key as its share of S's k, and of V 16 (8) consecutive dimensions of the keys that its part of P^T belongs to, so
-// nothing is shuffled but P, by movmatrix.
+// What bounds it: the bytes of keys and values.  A thread has a key (then a dimension) and ROWS rows: some 20
+// instructions a key and row, a quarter of what mma.sync on converted codes takes.  Three CTAs an SM, each with a tile
+// on its way and one in use, cover the trips between copy, tensor core and threads.
 //
-// What bounds it: the bytes of keys and values.  The row's running maximum and its power of two are touched only when a
-// score has passed them by 2^8 (2^12): one vote of the warp a block, no reductions.
-//
-// Work items: (sequence, run of keys, kv head, tile of rows).  The length of a run follows from the sequence's own
-// lengths, so a row's bits do not depend on the rest of the step, nor on NT.
-constexpr int SP_WARPS = 4, SP_BLOCK = 32;
+// Roles in a CTA: warps 0-3 softmax (TMEM lane = key, dimension), warp 4 copies (TMA, a box a page; scales by cp.async),
+// warp 5 issues the scores' products, warp 7 the outputs', warp 6 finds the next work items and makes their query rows.
+// Registers are handed out to groups of four warps: the second group gives a part of its own to the first (setmaxnreg).
+// Work items: (sequence, kv head, tile of rows,
+// run of keys), a CTA takes a contiguous range of them.  The length of a run follows from the sequence's own lengths, so a
+// row's bits do not depend on the rest of the step.
+constexpr int SP_TILE = 128, SP_THREADS = 256, SP_STAGES = 2, SP_ITEMS = 4;
+constexpr int SP_COPY_WARP = 4, SP_SCORE_WARP = 5, SP_OUTPUT_WARP = 7;      // and 6: items and query rows
 
-// Keys of a run: short runs where a sequence has few keys (its warps then share them), longer ones where the partial
-// results would grow; with many rows a run gets longer still, as their partial results do with the rows.
+// Keys of a run: two tiles (one: 72 -> 77 us for 64 decoding requests of up to 4,096 keys, as an item's beginning and end
+// cost about a tile, and no gain for one request of 2,048), longer ones where the partial results would grow; with many
+// rows a run gets longer still, as their partial results do with the rows.
 __host__ __device__ __forceinline__ int split_keys(int kv_len, int rows) {
-  const int base = kv_len <= 2048 ? 64 : kv_len <= 4096 ? 128 : kv_len <= 16384 ? 256 : 512;
+  const int base = kv_len <= 16384 ? 256 : 512;
   const int tiles = (rows + 31) / 32;
   return tiles <= 2 ? base : base * tiles;
 }
 
-__device__ __forceinline__ unsigned half2_of(unsigned w, unsigned sel) {     // two code bytes (offset by 128) -> float16 x 2
-  unsigned h = __byte_perm(w, 0x64646464u, sel), r;
-  asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x64806480u));         // 1024 + 128
-  return r;
-}
-__device__ __forceinline__ void mma_f16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
-                                        unsigned b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_s8(int (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
-                                       unsigned b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ unsigned transpose8(unsigned x) {
-  unsigned y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-__device__ __forceinline__ unsigned pack_f16(float lo, float hi) {
-  unsigned r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float low_of(unsigned h) {
-  float f;
-  asm("{ .reg .b16 a, b; mov.b32 {a, b}, %1; cvt.f32.f16 %0, a; }" : "=f"(f) : "r"(h));
-  return f;
-}
-__device__ __forceinline__ float high_of(unsigned h) {
-  float f;
-  asm("{ .reg .b16 a, b; mov.b32 {a, b}, %1; cvt.f32.f16 %0, b; }" : "=f"(f) : "r"(h));
-  return f;
-}
+// What a work item takes, in tiles of 128 keys: its own, and one for its beginning and end.
+__device__ __forceinline__ int item_work(int split) { return split / SP_TILE + 1; }
 
-// 1 over the power of two below w, between 2^-67 and 2^60: the quotient of two of them is finite.  (Values above 2^83 so
-// leave float16's range.)
-__device__ __forceinline__ float unit_of(float w) {
-  const int e = min(max((int)(__float_as_uint(w) >> 23), 67), 194);
-  return __uint_as_float((unsigned)(254 - e) << 23);
+__device__ __forceinline__ void mbar_arrive(unsigned long long* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(unsigned long long* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_mma_i8(unsigned tmem_d, unsigned long long desc_a, unsigned long long desc_b, unsigned idesc,
+                                          unsigned accum) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t"
+      "}\n" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accum), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// 8 consecutive columns of this thread's lane; valid after tc_wait_ld()
+__device__ __forceinline__ void tc_ld8(unsigned taddr, int (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+// Matrix descriptors: rows of 128 bytes, 128-byte swizzle, 8-row groups 1,024 bytes apart (K-major: a row is a key or a
+// query byte column; MN-major: a row is a key, its bytes the dimensions); and MN-major without swizzle: 16 columns x 8 keys
+// in 128 bytes, the next 8 keys 128 bytes on, the next 16 columns 2,048.
+__device__ __forceinline__ unsigned long long desc_sw128(unsigned addr) {
+  return (unsigned long long)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((unsigned long long)(1024u >> 4) << 32) | (1ull << 46) |
+         (2ull << 61);
+}
+__device__ __forceinline__ unsigned long long desc_columns16(unsigned addr) {
+  return (unsigned long long)((addr & 0x3FFFFu) >> 4) | ((unsigned long long)(128u >> 4) << 16) |
+         ((unsigned long long)(2048u >> 4) << 32) | (1ull << 46);
+}
+// kind::i8: 32-bit integer accumulator, signed bytes; A and B MN-major or not
+constexpr unsigned idesc_i8(int m, int n, int mn_major) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((unsigned)mn_major << 15) | ((unsigned)mn_major << 16) |
+         ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24);
+}
+__device__ __forceinline__ float warp_top(float v) {      // the largest of the warp's values, NaN aside
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+// An integer y, |y| <= 127 * 128^(PARTS - 1) and rounded here, as the sum of part[i] * 128^(PARTS - 1 - i), a signed byte
+// each (in the low byte of a word): adding 1.5 * 2^23 rounds to an integer and leaves it in the low bits.
+template <int PARTS> __device__ __forceinline__ void split7(float y, unsigned (&part)[PARTS]) {
+  constexpr float MAGIC = 12582912.f;
+  float unit = PARTS == 4 ? 2097152.f : 128.f;
+#pragma unroll
+  for (int i = 0; i < PARTS - 1; ++i) {
+    const float z = fmaf(y, 1.f / unit, MAGIC);
+    part[i] = __float_as_uint(z);
+    y = fmaf(z - MAGIC, -unit, y);
+    unit *= 0.0078125f;
+  }
+  part[PARTS - 1] = __float_as_uint(y + MAGIC);
+}
+__device__ __forceinline__ unsigned low_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+// the number that PARTS exact sums of part products stand for
+template <int PARTS, int STRIDE> __device__ __forceinline__ float join7(const int* acc) {
+  const float high = (float)(acc[0] * 128 + acc[STRIDE]);
+  return PARTS == 4 ? fmaf(high, 16384.f, (float)(acc[2 * STRIDE] * 128 + acc[3 * STRIDE])) : high;
 }
 
 struct SplitArgs {
@@ -124,9 +153,10 @@ struct SplitArgs {
   int Hq, Hkv, D, page_shift, window, box_rows;
   int num_pages;
   float scale;
-  float* part_o;                // [seq_count, max_items, 8 NT, D]
-  float2* part_ml;              // [seq_count, max_items, 8 NT]: reference maximum (log 2), sum
+  float* part_o;                // [seq_count, max_items, ROWS, D]
+  float2* part_ml;              // [seq_count, max_items, ROWS]: reference (log 2), sum
   int max_items;
+  int late;                     // the grid fills the GPU: the kernel that follows waits for its end
 };
 // A sequence of the launch and how it is cut.
 struct SplitSeq {
@@ -145,52 +175,106 @@ template <int ROWS> __device__ __forceinline__ SplitSeq split_seq(const SplitArg
   return s;
 }
 
-template <typename T, int DP, int NT> struct SplitShape {
-  static constexpr int ROWS = 8 * NT;
-  static constexpr int Q_PARTS = sizeof(T) == 4 ? 3 : 2;     // bytes a query's element is the sum of
-  static constexpr int P_PARTS = sizeof(T) == 4 ? 2 : 1;     // float16 numbers a probability is the sum of
-  static constexpr int STAGES = 2, QUEUE = 4;
-  static constexpr int TILE = SP_BLOCK * DP;                 // a block's keys, or values
-  // a warp's ring: the stages' tiles (each on 1,024 bytes), then the stages' scales
-  static constexpr int SCALES = STAGES * 2 * TILE;
-  static constexpr int RING = (SCALES + STAGES * 256 + 1023) / 1024 * 1024;
-  static constexpr size_t fixed = (size_t)SP_WARPS * (RING + STAGES * 8 + QUEUE * 32) + 1024;
-};
-
-// A work item as it is handed from the end of a warp's pipe that fetches to the one that computes.
+// A work item as it is handed from the warp that walks the CTA's items to the others.
 struct __align__(16) SplitItem {
-  int i, kvh, tile;             // sequence of the launch, kv head, tile of rows
-  int lo;                       // first key of the run
-  int at, end;                  // its keys [at, end), `at` a multiple of 32 and perhaps below the first one seen
-  int out_item, unused;         // number of the item among its sequence's
+  int seq, q_begin, n, kv_len;      // the sequence: index, first token, new tokens, keys
+  int i, kvh, tile, local;          // sequence of the launch, kv head, tile of rows, number of the item in its sequence
+  int run_at, at, end, splits;      // first key of the run; its keys [at, end), `at` a multiple of 128 and perhaps before the
+                                    // first one seen; runs of the sequence
+  int fresh, tiles, unused0, unused1;      // other query rows than the item before; tiles of keys, 0: there are no more items
 };
 
-template <typename T, int DP, int NT>
-__global__ void __launch_bounds__(SP_WARPS * 32)
+__device__ __forceinline__ float4 four_floats(const float4& v) { return v; }
+__device__ __forceinline__ float4 four_floats(const uint2& v) {      // four bfloat16
+  return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
+                     __uint_as_float(v.y & 0xffff0000u));
+}
+template <typename T> struct FourOf { using type = uint2; };
+template <> struct FourOf<float> { using type = float4; };
+
+template <typename T, int ROWS> struct SplitShape {
+  using Four = typename FourOf<T>::type;
+  static constexpr int PARTS = sizeof(T) == 4 ? 4 : 2;
+  static constexpr int N = ROWS * PARTS < 16 ? 16 : ROWS * PARTS;      // byte columns of a product's B (16 at least)
+  static constexpr int TMEM = N == 16 ? 64 : N == 32 ? 128 : 256;      // S twice, O; a power of two
+  static constexpr int STAGE = 2 * SP_TILE * 128;              // keys, values
+  static constexpr int SCALES = SP_STAGES * STAGE;             // [stages][2][128] float32
+  static constexpr int QUERIES = SCALES + SP_STAGES * 1024;    // [2][N][128], swizzled
+  static constexpr int WEIGHTS = QUERIES + 2 * N * 128;        // [N / 16][128 keys][16]
+  static constexpr int ROWDATA = WEIGHTS + N * 128;            // [2][3][ROWS]: unit, first and last key seen
+  static constexpr int TOPS = ROWDATA + 2 * 3 * ROWS * 4;      // [2][4 warps][ROWS + 4]
+  static constexpr int SUMS = TOPS + 2 * 4 * (ROWS + 4) * 4;   // [4 warps][ROWS]
+  static constexpr int ITEMS = SUMS + 4 * ROWS * 4;            // [SP_ITEMS]
+  static constexpr int BARS = ITEMS + SP_ITEMS * 64;
+  static constexpr int FIRST = BARS + 32 * 8;
+  static constexpr size_t fixed = FIRST + 16 + 1024;
+  // CTAs an SM (what shared memory allows); they are launched with 80 (128) registers a thread, and the groups' shares
+  // add up to twice that
+  static constexpr int CTAS = N == 16 ? 3 : 2, REGS_MANY = N == 16 ? 112 : 200, REGS_FEW = N == 16 ? 48 : 56;
+};
+
+template <int N> __device__ __forceinline__ void regs_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(SP_THREADS, SplitShape<T, ROWS>::CTAS)
 attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restrict__ q, T* __restrict__ out,
                        const __grid_constant__ SplitArgs a) {
-  using SH = SplitShape<T, DP, NT>;
-  constexpr int ROWS = SH::ROWS, Q_PARTS = SH::Q_PARTS, P_PARTS = SH::P_PARTS, STAGES = SH::STAGES, QUEUE = SH::QUEUE;
-  constexpr int MT = DP / 16, WORDS = DP / 16;      // 32-bit words of a thread's share of a key
+  using SH = SplitShape<T, ROWS>;
+  constexpr int PARTS = SH::PARTS, N = SH::N;
+  constexpr float MOST = PARTS == 4 ? 127.f * 2097152.f : 127.f * 128.f;      // of the integers
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  unsigned char* ring = smem + warp * SH::RING;
-  SplitItem* queue = reinterpret_cast<SplitItem*>(smem + SP_WARPS * SH::RING) + warp * QUEUE;
-  unsigned long long* bars =
-      reinterpret_cast<unsigned long long*>(smem + SP_WARPS * (SH::RING + QUEUE * 32)) + warp * STAGES;
-  int* first = reinterpret_cast<int*>(smem + SP_WARPS * (SH::RING + QUEUE * 32 + STAGES * 8));    // [seq_count + 1]
+  float* scales = reinterpret_cast<float*>(smem + SH::SCALES);
+  float* row_data = reinterpret_cast<float*>(smem + SH::ROWDATA);
+  float* tops = reinterpret_cast<float*>(smem + SH::TOPS);
+  float* sums = reinterpret_cast<float*>(smem + SH::SUMS);
+  SplitItem* items = reinterpret_cast<SplitItem*>(smem + SH::ITEMS);
+  unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + SH::BARS);
+  unsigned long long* k_full = bars;           // [2] a tile's keys and both kinds of scales have arrived
+  unsigned long long* v_full = bars + 2;       // [2] its values have
+  unsigned long long* s_full = bars + 4;       // [2] its scores are in tensor memory, its keys have been read
+  unsigned long long* s_empty = bars + 6;      // [2] its scores and scales have been read
+  unsigned long long* p_full = bars + 8;       // its weights are in shared memory, and O has been read
+  unsigned long long* o_full = bars + 9;       // its outputs are in tensor memory, its values and weights have been read
+  unsigned long long* v_empty = bars + 10;     // [2] its values have been read
+  unsigned long long* q_full = bars + 12;      // [2] an item's query rows are in shared memory
+  unsigned long long* q_empty = bars + 14;     // [2] they have been read
+  unsigned long long* item_full = bars + 16;   // [SP_ITEMS] an item's record is there
+  unsigned long long* item_empty = bars + 16 + SP_ITEMS;      // [SP_ITEMS] it has been read by every role
+  unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 16 + 2 * SP_ITEMS);
+  int* first = reinterpret_cast<int*>(smem + SH::FIRST);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) prefetch_tensormap(&map);
-  pdl_trigger();
-  // ---- the items before each sequence (metadata alone, which no kernel of a step writes)
-  for (int i = threadIdx.x; i < a.seq_count; i += blockDim.x) {
+  if (!a.late) pdl_trigger();
+  // ---- the work before each sequence (metadata alone, which no kernel of a step writes)
+  for (int i = threadIdx.x; i < a.seq_count; i += SP_THREADS) {
     const SplitSeq s = split_seq<ROWS>(a, i);
-    first[i + 1] = s.tiles * s.splits * a.Hkv;
+    first[i + 1] = s.tiles * s.splits * a.Hkv * item_work(s.split);
   }
   if (threadIdx.x == 0) first[0] = 0;
-  if (lane == 0) {
-    for (int s = 0; s < STAGES; ++s) mbar_init(&bars[s], 33);
+  if (threadIdx.x == 32) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 33);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 4);
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 5);
+    }
+    mbar_init(p_full, 4);
+    mbar_init(o_full, 1);
+    for (int i = 0; i < SP_ITEMS; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 7);      // copy, scores, outputs, four softmax warps
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == SP_SCORE_WARP) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"((unsigned)SH::TMEM));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
   __syncthreads();
   if (warp == 0) {
@@ -206,547 +290,592 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       base += __shfl_sync(0xffffffffu, v, 31);
     }
   }
+  tc_fence_before();
   __syncthreads();
-  const int total = first[a.seq_count];
+  tc_fence_after();
+  const unsigned tmem = *tmem_slot;
   const int G = a.Hq / a.Hkv;
-  const int stride = gridDim.x * SP_WARPS;
-  const int page_mask = (1 << a.page_shift) - 1;
-
-  // ---- the end that fetches: its item, the block of keys to be sent for next, this lane's page of it
-  int f_item = warp * gridDim.x + blockIdx.x, f_at = 0, f_end = 0, f_head = 0, f_page = -1, opened = 0;
-  const int* f_table = nullptr;
-  // the item f_item, or the first one behind it that has keys (on this warp's list); f_item >= total: none is left
-  auto open = [&]() {
-    for (; f_item < total; f_item += stride) {
-      int lo = 0, hi = a.seq_count - 1;          // the sequence whose items hold this one
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (first[mid] <= f_item) lo = mid; else hi = mid - 1;
-      }
-      const SplitSeq s = split_seq<ROWS>(a, lo);
-      const int local = f_item - first[lo];
-      int r = local, tile = 0;
-      if (s.tiles > 1) {
-        tile = r % s.tiles;
-        r /= s.tiles;
-      }
-      const int kvh = r / s.splits, run_at = (r - kvh * s.splits) * s.split;
-      const int p0 = s.kv_len - s.n, n_rows = s.n * G;
-      int tok0 = 0, tok1 = s.n - 1;
-      if (s.tiles > 1) {
-        tok0 = tile * ROWS / G;
-        tok1 = min((tile + 1) * ROWS, n_rows) - 1;
-        tok1 /= G;
-      }
-      const int k_lo = max(run_at, first_visible_key(p0 + tok0, a.window)), k_hi = min(run_at + s.split, p0 + tok1 + 1);
-      if (k_hi > k_lo) {
-        f_at = k_lo & ~(SP_BLOCK - 1);
-        f_end = k_hi;
-        f_table = a.block_table + (long long)s.seq * a.max_blocks;
-        f_head = kvh << a.page_shift;
-        __syncwarp();
-        if (lane == 0) {
-          SplitItem it;
-          it.i = lo; it.kvh = kvh; it.tile = tile; it.lo = run_at;
-          it.at = f_at; it.end = f_end; it.out_item = local; it.unused = 0;
-          queue[opened % QUEUE] = it;
-        }
-        __syncwarp();
-        ++opened;
-        return;
-      }
-      if (s.splits == 1)                         // a sequence of one run: rows that see no key are zeros, from here
-        for (int e = lane; e < min(ROWS, n_rows - tile * ROWS) * a.D; e += 32) {
-          const int row = tile * ROWS + e / a.D;
-          Elem<T>::store(out + ((long long)(s.q_begin + row / G) * a.Hq + kvh * G + row % G) * a.D + e % a.D, 0.f);
-        }
-    }
-  };
-  auto look_up = [&]() {                         // this lane's page of the block at f_at, or -1
-    const int key = f_at + lane;
-    int page = -1;
-    if (key < f_end) page = f_table[key >> a.page_shift];
-    f_page = page < a.num_pages ? page : -1;
-  };
-  // the block -> stage: lane l's key is f_at + l; the first lane of each page sends for its rows
-  auto fetch = [&](int stage) {
-    const unsigned tiles = smem_u32(ring) + stage * 2 * SH::TILE;
-    const unsigned sc = smem_u32(ring) + SH::SCALES + stage * 256 + lane * 4;
-    const int off = (f_at + lane) & page_mask;
-    const bool have = f_page >= 0;
-    const bool sends = have && (lane == 0 || off == 0);
-    const unsigned senders = __ballot_sync(0xffffffffu, sends);
-    if (lane == 0) mbar_expect_tx(&bars[stage], __popc(senders) * 2 * a.box_rows * DP);
-    __syncwarp();
-    const int half = a.Hkv << a.page_shift;      // rows of a page's keys
-    const int row = f_page * 2 * half + f_head + off;
-    if (sends) {
-      tma_load_2d(tiles + lane * DP, &map, 0, row, &bars[stage]);
-      tma_load_2d(tiles + SH::TILE + lane * DP, &map, 0, row + half, &bars[stage]);
-    }
-    if (have) {
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc), "l"(a.scales + row) : "memory");
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc + 128), "l"(a.scales + row + half) : "memory");
-    }
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bars[stage])) : "memory");
-    f_at += SP_BLOCK;
-    if (f_at >= f_end) {
-      f_item += stride;
-      open();
-    }
-    if (f_item < total) look_up();
-  };
-
   pdl_wait(q);
-  open();
-  if (f_item < total) look_up();
-  int sent = 0, used = 0;                          // blocks sent for, consumed
-  for (; sent < STAGES && f_item < total; ++sent) fetch(sent);
-
-  // where a lane finds its pieces of a tile (the copy's swizzle: bits 4.. of the address joined by bits 7..)
-  constexpr int SWIZZLE = DP == 128 ? 7 : 3, LINE = DP == 128 ? 1 : 2;      // rows of 128 bytes hold LINE keys
-  int k_off[WORDS / 4], v_off[2];
-#pragma unroll
-  for (int p = 0; p < WORDS / 4; ++p)
-    k_off[p] = g * DP + (((t * (WORDS / 4) + p) ^ ((g / LINE) & SWIZZLE)) << 4);
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int r = 2 * t + e;
-    v_off[e] = DP == 128 ? r * DP + ((g ^ (r & 7)) << 4) : r * DP + (((g >> 1) ^ ((r >> 1) & 3)) << 4) + (g & 1) * 8;
-  }
-
   bool ok = true;
-  for (int taken = 0; ok && taken < opened; ++taken) {
-    const SplitItem it = queue[taken % QUEUE];
-    const SplitSeq s_ = split_seq<ROWS>(a, it.i);
-    const int p0 = s_.kv_len - s_.n, row0 = it.tile * ROWS, rows = min(ROWS, s_.n * G - row0);
-    // ---- queries: row g of tile nt as the B operand, this thread's share of the dimensions, as the sum of Q_PARTS bytes
-    // of 7 bits each against the row's largest element
-    unsigned qf[NT][Q_PARTS][WORDS];
-    float q_unit[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int r = nt * 8 + g;
-      const bool in = r < rows;
-      const int tok = in ? (row0 + r) / G : 0, h = in ? row0 + r - tok * G : 0;
-      const T* src = q + ((long long)(s_.q_begin + tok) * a.Hq + it.kvh * G + h) * a.D + t * (DP / 4);
-      float x[DP / 4];
-#pragma unroll
-      for (int v = 0; v < DP / 4; v += 16 / (int)sizeof(T)) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (in && t * (DP / 4) + v < a.D) w = *reinterpret_cast<const uint4*>(src + v);
-        const unsigned u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (sizeof(T) == 2) {
-            x[v + 2 * e] = __uint_as_float(u[e] << 16);
-            x[v + 2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u);
-          } else {
-            x[v + e] = __uint_as_float(u[e]);
-          }
-        }
-      }
-      unsigned bits = 0;
-#pragma unroll
-      for (int d = 0; d < DP / 4; ++d) bits = max(bits, __float_as_uint(x[d]) & 0x7fffffffu);
-      bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
-      bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
-      const float top = fmaxf(__uint_as_float(bits), 0x1p-100f);
-      constexpr float MOST = Q_PARTS == 3 ? 127.f * 16384.f : 127.f * 128.f;
-      const float up = MOST / top;
-      // (a row that holds an infinity or a NaN: its unit is NaN, and so is all that comes of it)
-      q_unit[nt] = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.scale * LOG2E * (top / MOST);
-#pragma unroll
-      for (int j = 0; j < WORDS; ++j) {
-        int part[4][3];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          int v = __float2int_rn(x[4 * j + b] * up);
-          if (Q_PARTS == 3) {
-            const int above = (v + 64) >> 7;
-            part[b][2] = v - above * 128;
-            v = above;
-          }
-          part[b][0] = (v + 64) >> 7;
-          part[b][1] = v - part[b][0] * 128;
-        }
-#pragma unroll
-        for (int p = 0; p < Q_PARTS; ++p)
-          qf[nt][p][j] = __byte_perm(__byte_perm(part[0][p], part[1][p], 0x0040), __byte_perm(part[2][p], part[3][p], 0x0040), 0x5410);
-      }
-    }
-    // ---- what belongs to the rows this thread has scores of: 2t and 2t + 1 of each tile
-    float unit[NT][2], m[NT][2], l[NT][2], w_unit[NT][2];
-    int k_lo[NT][2], k_hi[NT][2], lo_all = it.lo, hi_all = it.end - 1;
-    float o[NT][MT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = nt * 8 + 2 * t + e;
-        const bool in = r < rows;
-        const int p = p0 + (in ? (row0 + r) / G : 0);
-        unit[nt][e] = __shfl_sync(0xffffffffu, q_unit[nt], (2 * t + e) * 4);
-        k_lo[nt][e] = max(first_visible_key(p, a.window), it.lo);
-        k_hi[nt][e] = in ? min(p, it.end - 1) : -1;
-        if (in) {        // (rows of the tile beyond the sequence's last one: their scores are never looked at)
-          lo_all = max(lo_all, k_lo[nt][e]);
-          hi_all = min(hi_all, p);
-        }
-        m[nt][e] = -INFINITY;
-        l[nt][e] = 0.f;
-        w_unit[nt][e] = 1.f;
-      }
-#pragma unroll
-    for (int o_ = 1; o_ < 4; o_ <<= 1) {
-      lo_all = max(lo_all, __shfl_xor_sync(0xffffffffu, lo_all, o_));
-      hi_all = min(hi_all, __shfl_xor_sync(0xffffffffu, hi_all, o_));
-    }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
 
-    for (int kb = it.at; kb < it.end; kb += SP_BLOCK, ++used) {
-      const int stage = used % STAGES;
-      ok = mbar_wait(&bars[stage], (used / STAGES) & 1);
+  if (warp >= 4) {
+  regs_give<SH::REGS_FEW>();
+  if (warp == SP_COPY_WARP) {
+    // ---- copies: lane l has the keys 4l .. 4l + 3 of a tile; the first lane of each page sends for its rows.  Keys are
+    // free again once the scores are made, long before the values: keys go a tile ahead of them.
+    const int page_mask = (1 << a.page_shift) - 1, half = a.Hkv << a.page_shift;      // rows of a page's keys
+    int n = 0, v_row = 0;                  // tiles sent for; the values' row of the tile before
+    unsigned v_senders = 0;
+    auto send_values = [&](int m) {        // of tile m
+      if (m >= SP_STAGES) ok = mbar_wait(&v_empty[m & 1], ((m >> 1) - 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      if (lane == 0) mbar_expect_tx(&v_full[m & 1], __popc(v_senders) * a.box_rows * 128);
+      __syncwarp();
+      if (v_senders >> lane & 1)
+        tma_load_2d(smem_u32(smem) + (m & 1) * SH::STAGE + SP_TILE * 128 + lane * 512, &map, 0, v_row, &v_full[m & 1]);
+    };
+    for (int k = 0; ok; ++k) {
+      const int slot = k % SP_ITEMS;
+      ok = mbar_wait(&item_full[slot], (k / SP_ITEMS) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      const unsigned char* kt = ring + stage * 2 * SH::TILE;
-      const unsigned char* vt = kt + SH::TILE;
-      const float* sc = reinterpret_cast<const float*>(ring + SH::SCALES) + stage * 64;
-      // ---- S^T, an exact integer
-      float s[2][NT][4];
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        uint4 kw[2][WORDS / 4];
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int p = 0; p < WORDS / 4; ++p)
-            kw[half][p] = *reinterpret_cast<const uint4*>(kt + (mt * 16 + half * 8) * DP + k_off[p]);
-        int acc[NT][Q_PARTS][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int p = 0; p < Q_PARTS; ++p)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[nt][p][e] = 0;
-#pragma unroll
-        for (int p4 = 0; p4 < WORDS / 4; ++p4)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int p = 0; p < Q_PARTS; ++p) {
-              mma_s8(acc[nt][p], kw[0][p4].x, kw[1][p4].x, kw[0][p4].y, kw[1][p4].y, qf[nt][p][p4 * 4], qf[nt][p][p4 * 4 + 1]);
-              mma_s8(acc[nt][p], kw[0][p4].z, kw[1][p4].z, kw[0][p4].w, kw[1][p4].w, qf[nt][p][p4 * 4 + 2], qf[nt][p][p4 * 4 + 3]);
-            }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float high = (float)(acc[nt][0][e] * 128 + acc[nt][1][e]);
-            s[mt][nt][e] = Q_PARTS == 3 ? fmaf(high, 128.f, (float)acc[nt][Q_PARTS - 1][e]) : high;
-          }
-      }
-      float ks[2][2], vs[2][2];
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          ks[mt][half] = sc[mt * 16 + half * 8 + g];
-          vs[mt][half] = sc[32 + mt * 16 + half * 8 + g];
+      const int seq = items[slot].seq, kvh = items[slot].kvh, at = items[slot].at, end = items[slot].end, tiles = items[slot].tiles;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[slot]);
+      if (tiles == 0) break;
+      const int* table = a.block_table + (long long)seq * a.max_blocks;
+      for (int kb = at; kb < end; kb += SP_TILE, ++n) {
+        const int key = kb + lane * 4, off = key & page_mask, stage = n & 1;
+        int page = -1;
+        if (key < end) page = table[key >> a.page_shift];
+        const bool have = page >= 0 && page < a.num_pages;
+        const unsigned senders = __ballot_sync(0xffffffffu, have && (lane == 0 || off == 0));
+        if (n >= SP_STAGES)       // (the scores made, and the scales read: those of the tile two before this one)
+          ok = mbar_wait(&s_full[stage], ((n >> 1) - 1) & 1) && mbar_wait(&s_empty[stage], ((n >> 1) - 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(&k_full[stage], __popc(senders) * a.box_rows * 128);
+        __syncwarp();
+        const int row = page * 2 * half + (kvh << a.page_shift) + off;
+        if (senders >> lane & 1) tma_load_2d(smem_u32(smem) + stage * SH::STAGE + lane * 512, &map, 0, row, &k_full[stage]);
+        if (have) {
+          const unsigned sc = smem_u32(scales) + stage * 1024 + lane * 16;
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(sc), "l"(a.scales + row) : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(sc + 512), "l"(a.scales + row + half) : "memory");
         }
-      const bool plain = kb >= lo_all && kb + SP_BLOCK - 1 <= hi_all;      // every row sees every key
-      float top[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          top[nt][e] = -INFINITY;
-#pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) s[mt][nt][2 * half + e] *= ks[mt][half] * unit[nt][e];
-        }
-      if (!plain) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                const int key = kb + mt * 16 + half * 8 + g;
-                if (key < k_lo[nt][e] || key > k_hi[nt][e]) s[mt][nt][2 * half + e] = -INFINITY;
-              }
-      }
-      bool high = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          top[nt][e] = fmaxf(fmaxf(s[0][nt][e], s[0][nt][2 + e]), fmaxf(s[1][nt][e], s[1][nt][2 + e]));
-          high |= top[nt][e] > m[nt][e] + 8.f;
-        }
-      if (__any_sync(0xffffffffu, high)) {
-        // some row's reference maximum rises (each row by its own scores alone)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float best = top[nt][e];
-#pragma unroll
-            for (int o_ = 4; o_ < 32; o_ <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o_));
-            float factor = 1.f;
-            if (best > m[nt][e] + 8.f) {
-              factor = fast_exp2(m[nt][e] - best);     // (zero from minus infinity)
-              m[nt][e] = best;
-              l[nt][e] *= factor;
-              // the probabilities' power of two is chosen anew: by the block's largest probability * scale
-              float wt = 0.f;
-#pragma unroll
-              for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-                for (int half = 0; half < 2; ++half)
-                  wt = fmaxf(wt, fast_exp2(s[mt][nt][2 * half + e] - best) * vs[mt][half]);
-              const unsigned lanes = 0x11111111u << t;      // (every lane of a row takes this branch)
-#pragma unroll
-              for (int o_ = 4; o_ < 32; o_ <<= 1) wt = fmaxf(wt, __shfl_xor_sync(lanes, wt, o_));
-              const float now = unit_of(wt);
-              if (factor * (now / w_unit[nt][e]) <= 0x1p40f) {      // (else what O holds outweighs the block by far)
-                factor *= now / w_unit[nt][e];
-                w_unit[nt][e] = now;
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              o[nt][i][e] *= factor;
-              o[nt][i][2 + e] *= factor;
-            }
-          }
-      }
-      // ---- probabilities, times the value's scale and the row's power of two
-      bool large = false;
-      float w[2][NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float ref = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
-          float most = 0.f;
-#pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const float p = fast_exp2(s[mt][nt][2 * half + e] - ref);
-              l[nt][e] += p;
-              w[mt][nt][2 * half + e] = p * (vs[mt][half] * w_unit[nt][e]);
-              most = fmaxf(most, w[mt][nt][2 * half + e]);
-            }
-          large |= most > 4096.f;
-        }
-      if (!plain) {        // a key that the row does not see may have a value that is no number
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (s[mt][nt][e] == -INFINITY) w[mt][nt][e] = 0.f;
-      }
-      if (__any_sync(0xffffffffu, large)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float wt = fmaxf(fmaxf(w[0][nt][e], w[0][nt][2 + e]), fmaxf(w[1][nt][e], w[1][nt][2 + e]));
-#pragma unroll
-            for (int o_ = 4; o_ < 32; o_ <<= 1) wt = fmaxf(wt, __shfl_xor_sync(0xffffffffu, wt, o_));
-            float factor = 1.f;
-            if (wt > 4096.f) factor = unit_of(wt);      // (of the product with the old unit)
-            w_unit[nt][e] *= factor;
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
-              w[mt][nt][e] *= factor;
-              w[mt][nt][2 + e] *= factor;
-            }
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              o[nt][i][e] *= factor;
-              o[nt][i][2 + e] *= factor;
-            }
-          }
-      }
-      // ---- O^T += V^T P^T, 16 keys at a time
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        unsigned pf[NT][P_PARTS][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const float w0 = w[mt][nt][2 * half], w1 = w[mt][nt][2 * half + 1];
-            const unsigned hi = pack_f16(w0, w1);
-            pf[nt][0][half] = transpose8(hi);
-            if (P_PARTS == 2) pf[nt][P_PARTS - 1][half] = transpose8(pack_f16(w0 - low_of(hi), w1 - high_of(hi)));
-          }
-        // the thread's 16 (8) dimensions of the keys 2t, 2t + 1, 2t + 8, 2t + 9
-        unsigned vw[4][DP / 32];
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          const unsigned char* src = vt + (mt * 16 + (kk >> 1) * 8) * DP + v_off[kk & 1];
-          if (DP == 128) {
-            const uint4 v = *reinterpret_cast<const uint4*>(src);
-            vw[kk][0] = v.x ^ 0x80808080u;
-            vw[kk][1] = v.y ^ 0x80808080u;
-            vw[kk][DP / 32 - 2] = v.z ^ 0x80808080u;
-            vw[kk][DP / 32 - 1] = v.w ^ 0x80808080u;
-          } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(src);
-            vw[kk][0] = v.x ^ 0x80808080u;
-            vw[kk][1] = v.y ^ 0x80808080u;
-          }
-        }
-#pragma unroll
-        for (int c4 = 0; c4 < DP / 32; ++c4) {
-          const unsigned x = __byte_perm(vw[0][c4], vw[1][c4], 0x5140), y = __byte_perm(vw[0][c4], vw[1][c4], 0x7362);
-          const unsigned u = __byte_perm(vw[2][c4], vw[3][c4], 0x5140), z = __byte_perm(vw[2][c4], vw[3][c4], 0x7362);
-          const unsigned a0 = half2_of(x, 0x4140), a1 = half2_of(x, 0x4342), a2 = half2_of(u, 0x4140), a3 = half2_of(u, 0x4342);
-          const unsigned b0 = half2_of(y, 0x4140), b1 = half2_of(y, 0x4342), b2 = half2_of(z, 0x4140), b3 = half2_of(z, 0x4342);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int p = P_PARTS - 1; p >= 0; --p) {       // the small part first
-              mma_f16(o[nt][2 * c4], a0, a1, a2, a3, pf[nt][p][0], pf[nt][p][1]);
-              mma_f16(o[nt][2 * c4 + 1], b0, b1, b2, b3, pf[nt][p][0], pf[nt][p][1]);
-            }
-        }
-      }
-      __syncwarp();                                    // every lane has read the stage
-      if (f_item < total) {
-        fetch(stage);
-        ++sent;
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&k_full[stage])) : "memory");
+        if (n > 0) send_values(n - 1);
+        v_row = row + half;
+        v_senders = senders;
       }
     }
-    if (!ok) break;
-    // ---- the item's rows: finished where the sequence has one run, else partial results for the merge
+    if (ok && n > 0) send_values(n - 1);
+  } else if (warp == SP_SCORE_WARP) {
+    // ---- scores: a tile ahead of the softmax
+    if (lane == 0) {
+      constexpr unsigned idesc = idesc_i8(128, N, 0);
+      const unsigned base = smem_u32(smem);
+      int n = 0, q_used = -1;
+      for (int k = 0; ok; ++k) {
+        const int slot = k % SP_ITEMS;
+        ok = mbar_wait(&item_full[slot], (k / SP_ITEMS) & 1);
+        if (!ok) break;
+        const int tiles = items[slot].tiles, fresh = items[slot].fresh;
+        mbar_arrive(&item_empty[slot]);
+        if (tiles == 0) break;
+        if (fresh) {
+          if (q_used >= 0) tc_commit(&q_empty[q_used & 1]);
+          ++q_used;
+          ok = mbar_wait(&q_full[q_used & 1], (q_used >> 1) & 1);
+          if (!ok) break;
+        }
+        const unsigned long long qd = desc_sw128(base + SH::QUERIES + (q_used & 1) * N * 128);
+        for (int t = tiles; t > 0 && ok; --t, ++n) {
+          ok = mbar_wait(&k_full[n & 1], (n >> 1) & 1) && (n < 2 || mbar_wait(&s_empty[n & 1], ((n >> 1) - 1) & 1));
+          if (!ok) break;
+          tc_fence_after();
+          const unsigned long long kd = desc_sw128(base + (n & 1) * SH::STAGE);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float sum = l[nt][e];
-#pragma unroll
-        for (int o_ = 4; o_ < 32; o_ <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o_);
-        const int r = nt * 8 + 2 * t + e;
-        if (r >= rows) continue;
-        const float back = 1.f / w_unit[nt][e];
-        const int d0 = g * (DP / 8);
-        if (d0 >= a.D) continue;
-        if (s_.splits == 1) {
-          const float inv = sum == 0.f ? 0.f : back / sum;
-          const int tok = (row0 + r) / G;
-          T* dst = out + ((long long)(s_.q_begin + tok) * a.Hq + it.kvh * G + row0 + r - tok * G) * a.D + d0;
-#pragma unroll
-          for (int i = 0; i < MT; i += 2) {
-            if (d0 + 2 * i >= a.D) break;
-            const float y0 = o[nt][i][e] * inv, y1 = o[nt][i][2 + e] * inv, y2 = o[nt][i + 1][e] * inv, y3 = o[nt][i + 1][2 + e] * inv;
-            if (sizeof(T) == 2) {
-              const __nv_bfloat162 lo2 = __floats2bfloat162_rn(y0, y1), hi2 = __floats2bfloat162_rn(y2, y3);
-              *reinterpret_cast<uint2*>(dst + 2 * i) =
-                  make_uint2(*reinterpret_cast<const unsigned*>(&lo2), *reinterpret_cast<const unsigned*>(&hi2));
-            } else {
-              *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(y0, y1, y2, y3);
-            }
-          }
-        } else if (it.out_item < a.max_items) {
-          const long long at = ((long long)it.i * a.max_items + it.out_item) * ROWS + r;
-          float* dst = a.part_o + at * a.D + d0;
-#pragma unroll
-          for (int i = 0; i < MT; i += 2) {
-            if (d0 + 2 * i >= a.D) break;
-            *reinterpret_cast<float4*>(dst + 2 * i) =
-                make_float4(o[nt][i][e] * back, o[nt][i][2 + e] * back, o[nt][i + 1][e] * back, o[nt][i + 1][2 + e] * back);
-          }
-          if (g == 0) a.part_ml[at] = make_float2(m[nt][e], sum);
+          for (int ks = 0; ks < 4; ++ks) tc_mma_i8(tmem + (n & 1) * N, kd + ks * 2, qd + ks * 2, idesc, ks > 0);
+          tc_commit(&s_full[n & 1]);
         }
       }
+    }
+  } else if (warp == SP_OUTPUT_WARP) {
+    // ---- outputs, as soon as a tile's weights are there
+    if (lane == 0) {
+      constexpr unsigned idesc = idesc_i8(128, N, 1);
+      const unsigned base = smem_u32(smem);
+      const unsigned long long weights = desc_columns16(base + SH::WEIGHTS);
+      int n = 0;
+      for (int k = 0; ok; ++k) {
+        const int slot = k % SP_ITEMS;
+        ok = mbar_wait(&item_full[slot], (k / SP_ITEMS) & 1);
+        if (!ok) break;
+        const int tiles = items[slot].tiles;
+        mbar_arrive(&item_empty[slot]);
+        if (tiles == 0) break;
+        for (int t = tiles; t > 0 && ok; --t, ++n) {
+          ok = mbar_wait(&v_full[n & 1], (n >> 1) & 1) && mbar_wait(p_full, n & 1);
+          if (!ok) break;
+          tc_fence_after();
+          const unsigned long long vd = desc_sw128(base + (n & 1) * SH::STAGE + SP_TILE * 128);
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            tc_mma_i8(tmem + 2 * N, vd + ks * (4096 >> 4), weights + ks * (512 >> 4), idesc, ks > 0);
+          tc_commit(o_full);
+          tc_commit(&v_empty[n & 1]);
+        }
+      }
+    }
+  } else {
+    // ---- the walk over this CTA's items, a contiguous range of equal work, and the query rows: a lane has 4 of a row's
+    // dimensions
+    const long long total = first[a.seq_count];
+    const int from_work = (int)(total * blockIdx.x / gridDim.x), to_work = (int)(total * (blockIdx.x + 1) / gridDim.x);
+    int i = 0, item = 0, old_i = -1, old_kvh = -1, old_tile = -1, made = 0;
+    for (int hi = a.seq_count - 1; i < hi;) {      // the sequence in which the range begins
+      const int mid = (i + hi + 1) >> 1;
+      if (first[mid] <= from_work) i = mid; else hi = mid - 1;
+    }
+    if (total > 0) {
+      const int each = item_work(split_seq<ROWS>(a, i).split);
+      item = (from_work - first[i] + each - 1) / each;       // the first item that begins in it
+    }
+    for (int k = 0; ok; ++item) {
+      SplitItem it = {};              // (as it is: no more items)
+      bool more = false;
+      SplitSeq s;
+      for (; i < a.seq_count; ++i, item = 0) {
+        s = split_seq<ROWS>(a, i);
+        if (item < s.tiles * s.splits * a.Hkv) {
+          more = first[i] + item * item_work(s.split) < to_work;
+          break;
+        }
+      }
+      if (more) {
+        const int local = item;
+        const int unit = s.splits > 1 ? local / s.splits : local;
+        it.seq = s.seq; it.q_begin = s.q_begin; it.n = s.n; it.kv_len = s.kv_len;
+        it.i = i; it.local = local; it.splits = s.splits;
+        it.run_at = (local - unit * s.splits) * s.split;
+        it.kvh = s.tiles > 1 ? unit / s.tiles : unit;
+        it.tile = unit - it.kvh * s.tiles;
+        const int p0 = s.kv_len - s.n;
+        int tok0 = 0, tok1 = s.n - 1;
+        if (s.tiles > 1) {
+          tok0 = it.tile * ROWS / G;
+          tok1 = (min((it.tile + 1) * ROWS, s.n * G) - 1) / G;
+        }
+        const int k_lo = max(it.run_at, first_visible_key(p0 + tok0, a.window));
+        it.end = min(it.run_at + s.split, p0 + tok1 + 1);
+        it.at = k_lo & ~(SP_TILE - 1);
+        if (it.end <= k_lo) {
+          if (s.splits == 1) {             // a sequence of one run: rows that see no key are zeros, from here
+            const int rows = min(ROWS, s.n * G - it.tile * ROWS);
+            for (int e = lane; e < rows * a.D; e += 32) {
+              const int row = it.tile * ROWS + e / a.D, tok = row / G;
+              Elem<T>::store(out + ((long long)(s.q_begin + tok) * a.Hq + it.kvh * G + row - tok * G) * a.D + e % a.D, 0.f);
+            }
+          }
+          continue;
+        }
+        it.tiles = (it.end - it.at + SP_TILE - 1) / SP_TILE;
+        it.fresh = i != old_i || it.kvh != old_kvh || it.tile != old_tile;
+        old_i = i; old_kvh = it.kvh; old_tile = it.tile;
+      }
+      // the query rows' loads, some rows at a time, go out ahead of the copies that the record sets off
+      const int row0 = it.tile * ROWS, rows = min(ROWS, it.n * G - row0);
+      constexpr int AHEAD = PARTS == 4 || ROWS < 8 ? 4 : 8;
+      typename SH::Four raw[AHEAD];        // 4 elements of a row
+      int tok = row0 / G, head = row0 - tok * G;      // of the next row to be loaded
+      const T* src = q + ((long long)(it.q_begin + tok) * a.Hq + it.kvh * G + head) * a.D + lane * 4;
+      auto load_rows = [&](int from) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          raw[u] = typename SH::Four();
+          if (from + u < rows && lane * 4 < a.D) raw[u] = *reinterpret_cast<const typename SH::Four*>(src);
+          src += a.D;
+          if (++head == G) {
+            head = 0;
+            src += (long long)(a.Hq - G) * a.D;
+          }
+        }
+      };
+      if (it.fresh) load_rows(0);
+      const int slot = k % SP_ITEMS;
+      if (k >= SP_ITEMS) ok = mbar_wait(&item_empty[slot], ((k / SP_ITEMS) - 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (lane == 0) {
+        items[slot] = it;
+        mbar_arrive(&item_full[slot]);
+      }
+      ++k;
+      if (it.tiles == 0) break;
+      if (!it.fresh) continue;
+      const int buf = made & 1;
+      if (made >= 2) ok = mbar_wait(&q_empty[buf], ((made >> 1) - 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      unsigned char* dst = smem + SH::QUERIES + buf * N * 128;
+      float* data = row_data + buf * 3 * ROWS;
+      int pos = it.kv_len - it.n + tok, pos_head = row0 - tok * G;      // of the next row to be made
+#pragma unroll
+      for (int from = 0; from < ROWS; from += AHEAD) {
+        if (from > 0) load_rows(from);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          const int r = from + u;
+          const float4 x4 = four_floats(raw[u]);
+          const float x[4] = {x4.x, x4.y, x4.z, x4.w};
+          unsigned bits = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) bits = max(bits, __float_as_uint(x[e]) & 0x7fffffffu);
+          bits = __reduce_max_sync(0xffffffffu, bits);
+          const float top = fmaxf(__uint_as_float(bits), 0x1p-100f), up = __fdividef(MOST * (1.f - 0x1p-20f), top);
+          unsigned part[4][PARTS];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) split7<PARTS>(x[e] * up, part[e]);
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) {
+            const int col = p * ROWS + r;
+            *reinterpret_cast<unsigned*>(dst + col * 128 + (((lane >> 2) ^ (col & 7)) << 4) + (lane & 3) * 4) =
+                low_bytes(part[0][p], part[1][p], part[2][p], part[3][p]);
+          }
+          if (lane == 0) {
+            // (a row that holds an infinity or a NaN: its unit is NaN, and so is all that comes of it)
+            data[r] = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __fdiv_rn(a.scale * LOG2E, up);
+            data[ROWS + r] = __int_as_float(first_visible_key(pos, a.window));
+            data[2 * ROWS + r] = __int_as_float(r < rows ? pos : -1);
+          }
+          if (++pos_head == G) {
+            pos_head = 0;
+            ++pos;
+          }
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the rows are read by the tensor core
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[buf]);
+      ++made;
+    }
   }
-  if (!ok) {
-    atomicExch(&dib_attention_int8_error_word, 1);
-    for (int u = used + 1; u < sent; ++u) mbar_wait(&bars[u % STAGES], (u / STAGES) & 1);      // no copy outlives the warp
+  } else {
+    regs_take<SH::REGS_MANY>();
+    // ---- softmax: thread = key of the tile, then dimension
+    constexpr float UNSET = -1e30f;      // the reference of a row that has seen no key
+    constexpr int R8 = ROWS < 8 ? ROWS : 8;
+    const int key_of = threadIdx.x;
+    const unsigned tm = tmem + ((unsigned)(warp * 32) << 16);
+    float L[ROWS], l[ROWS], o[ROWS], f[ROWS];      // f: what the pending tile's integers are multiplied by
+    int n = 0, q_used = -1;
+    // PARTS x R8 columns from `col` on, as numbers: rows r8 .. of an accumulator
+    auto load_rows = [&](unsigned acc_col, int r8, float (&y)[R8]) {
+      if (ROWS == 4 && PARTS == 2) {
+        int acc[8];
+        tc_ld8(tm + acc_col, acc);
+        tc_wait_ld();
+#pragma unroll
+        for (int r = 0; r < R8; ++r) y[r] = join7<2, 4>(&acc[r]);
+      } else {
+        int acc[PARTS][8];
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) tc_ld8(tm + acc_col + p * ROWS + r8, acc[p]);
+        tc_wait_ld();
+#pragma unroll
+        for (int r = 0; r < R8; ++r) y[r] = join7<PARTS, 8>(&acc[0][r]);
+      }
+    };
+    auto add_outputs = [&](int m) {      // tile m's integers
+      ok = mbar_wait(o_full, m & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      tc_fence_after();
+#pragma unroll
+      for (int r8 = 0; r8 < ROWS; r8 += R8) {
+        float y[R8];
+        load_rows(2 * N, r8, y);
+#pragma unroll
+        for (int r = 0; r < R8; ++r) o[r8 + r] = fmaf(y[r], f[r8 + r], o[r8 + r]);
+      }
+    };
+    // The rows of the item whose tiles have all been added: finished where the sequence has one run, else partial
+    // results for the merge.  (Done under the next item's first tile, whose scores do not wait for it.)
+    int d_rows = 0, d_splits = 0, d_local = 0, d_head = 0, d_row0 = 0, d_begin = 0;
+    long long d_at = 0;
+    auto finish = [&]() {
+#pragma unroll
+      for (int r8 = 0; r8 < ROWS; r8 += R8) {
+        // sums of R8 rows over a warp: exchanges that halve the rows a lane has, then whole sums
+        float v[R8];
+#pragma unroll
+        for (int r = 0; r < R8; ++r) v[r] = l[r8 + r];
+        int of = 16;
+#pragma unroll
+        for (int h = R8 / 2; h > 0; h >>= 1, of >>= 1) {
+          const bool up = lane & of;
+#pragma unroll
+          for (int r = 0; r < h; ++r) {
+            const float give = up ? v[r] : v[r + h], keep = up ? v[r + h] : v[r];
+            v[r] = keep + __shfl_xor_sync(0xffffffffu, give, of);
+          }
+        }
+#pragma unroll
+        for (int x = 16 / R8; x > 0; x >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], x);
+        if ((lane & (32 / R8 - 1)) == 0) sums[warp * ROWS + r8 + lane / (32 / R8)] = v[0];
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      float sum[ROWS];
+#pragma unroll
+      for (int r = 0; r < ROWS; r += 4) {
+        const float4 w0 = *reinterpret_cast<const float4*>(sums + r), w1 = *reinterpret_cast<const float4*>(sums + ROWS + r);
+        const float4 w2 = *reinterpret_cast<const float4*>(sums + 2 * ROWS + r), w3 = *reinterpret_cast<const float4*>(sums + 3 * ROWS + r);
+        sum[r] = (w0.x + w1.x) + (w2.x + w3.x); sum[r + 1] = (w0.y + w1.y) + (w2.y + w3.y);
+        sum[r + 2] = (w0.z + w1.z) + (w2.z + w3.z); sum[r + 3] = (w0.w + w1.w) + (w2.w + w3.w);
+      }
+      if (d_splits == 1) {
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+          if (r >= d_rows) break;
+          const int row = d_row0 + r, tok = row / G;
+          if (key_of < a.D)
+            Elem<T>::store(out + ((long long)(d_begin + tok) * a.Hq + d_head + row - tok * G) * a.D + key_of,
+                           sum[r] == 0.f ? 0.f : o[r] / sum[r]);
+        }
+      } else if (d_local < a.max_items) {
+        float* dst = a.part_o + d_at * a.D + key_of;
+        if (key_of < a.D) {
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r, dst += a.D)
+            if (r < d_rows) *dst = o[r];
+        }
+        if (key_of == 0) {
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r)
+            if (r < d_rows) a.part_ml[d_at + r] = make_float2(L[r], sum[r]);
+        }
+      }
+    };
+    for (int k = 0; ok; ++k) {
+      const int slot = k % SP_ITEMS;
+      ok = mbar_wait(&item_full[slot], (k / SP_ITEMS) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const SplitItem it = items[slot];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[slot]);
+      if (it.tiles == 0) break;
+      const int row0 = it.tile * ROWS, rows = min(ROWS, it.n * G - row0), p0 = it.kv_len - it.n;
+      if (it.fresh) {
+        if (q_used >= 0 && lane == 0) mbar_arrive(&q_empty[q_used & 1]);
+        ++q_used;
+        ok = mbar_wait(&q_full[q_used & 1], (q_used >> 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+      }
+      const float* data = row_data + (q_used & 1) * 3 * ROWS;
+      // the keys that every row sees
+      const int lo_all = max(it.run_at, first_visible_key(p0 + (row0 + rows - 1) / G, a.window));
+      const int hi_all = min(it.end - 1, p0 + row0 / G);
+      for (int kb = it.at; kb < it.end; kb += SP_TILE, ++n) {
+        const int buf = n & 1;
+        ok = mbar_wait(&k_full[buf], (n >> 1) & 1) && mbar_wait(&s_full[buf], (n >> 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        // scores, in units of log 2
+        const float vs_raw = scales[buf * 256 + 128 + key_of];
+        const float ks = scales[buf * 256 + key_of] + (vs_raw - vs_raw);      // NaN if either is
+        const int key = kb + key_of;
+        const bool plain = kb >= lo_all && kb + SP_TILE - 1 <= hi_all;        // every row sees every key
+        const bool there = key >= it.run_at && key < it.end;
+        const float vs = there ? vs_raw : 0.f, lv = there ? fmaxf(__log2f(vs), -120.f) : -INFINITY;
+        float s[ROWS];
+#pragma unroll
+        for (int r8 = 0; r8 < ROWS; r8 += R8) {
+          float y[R8];
+          load_rows(buf * N, r8, y);
+#pragma unroll
+          for (int r = 0; r < R8; r += 4) {
+            const float4 unit = *reinterpret_cast<const float4*>(data + r8 + r);
+            s[r8 + r] = y[r] * (ks * unit.x); s[r8 + r + 1] = y[r + 1] * (ks * unit.y);
+            s[r8 + r + 2] = y[r + 2] * (ks * unit.z); s[r8 + r + 3] = y[r + 3] * (ks * unit.w);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_empty[buf]);
+        if (!plain) {
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r)
+            if (!there || key < __float_as_int(data[ROWS + r]) || key > __float_as_int(data[2 * ROWS + r])) s[r] = -INFINITY;
+        }
+        // the tile's largest weight of each row, and its largest value scale
+        float top[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) top[r] = warp_top(s[r] + lv);
+        float size = warp_top(lv);
+        float* mine = tops + (buf * 4) * (ROWS + 4);
+        if (lane == 0) {
+#pragma unroll
+          for (int r = 0; r < ROWS; r += 4)
+            *reinterpret_cast<float4*>(mine + warp * (ROWS + 4) + r) = make_float4(top[r], top[r + 1], top[r + 2], top[r + 3]);
+          mine[warp * (ROWS + 4) + ROWS] = size;
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll
+        for (int w = 0; w < 4; ++w) size = fmaxf(size, mine[w * (ROWS + 4) + ROWS]);
+#pragma unroll
+        for (int r = 0; r < ROWS; r += 4) {
+          float4 v = *reinterpret_cast<const float4*>(mine + r);
+#pragma unroll
+          for (int w = 1; w < 4; ++w) {
+            const float4 u = *reinterpret_cast<const float4*>(mine + w * (ROWS + 4) + r);
+            v.x = fmaxf(v.x, u.x); v.y = fmaxf(v.y, u.y); v.z = fmaxf(v.z, u.z); v.w = fmaxf(v.w, u.w);
+          }
+          top[r] = v.x; top[r + 1] = v.y; top[r + 2] = v.z; top[r + 3] = v.w;
+        }
+        // the tile before this one: its outputs are there as a rule
+        if (n > 0) add_outputs(n - 1);
+        if (!ok) break;
+        if (kb == it.at) {
+          if (n > 0) finish();
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r) {
+            L[r] = UNSET;
+            l[r] = o[r] = 0.f;
+          }
+          d_rows = rows; d_splits = it.splits; d_local = it.local; d_head = it.kvh * G; d_row0 = row0; d_begin = it.q_begin;
+          d_at = ((long long)it.i * a.max_items + it.local) * ROWS;
+        }
+        bool rises = false;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) rises |= top[r] - size > L[r] + 20.f;
+        if (rises) {      // (the same in every thread)
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r) {
+            const float about = top[r] - size;        // near the largest score: below it by the scales' spread at most
+            if (about > L[r] + 20.f) {
+              const float factor = fast_exp2(L[r] - about);
+              L[r] = about;
+              l[r] *= factor;
+              o[r] *= factor;
+            }
+          }
+        }
+        // weights
+        unsigned pw[N / 4];
+#pragma unroll
+        for (int c = 0; c < N / 4; ++c) pw[c] = 0;
+#pragma unroll
+        for (int r4 = 0; r4 < ROWS; r4 += 4) {
+          unsigned part[4][PARTS];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = r4 + e;
+            // a power of two that brings the row's largest weight near the integers' largest, and back: 2^floor(L - top)
+            const float x = floorf(fminf(L[r] - top[r], 96.f));
+            const int ex = (int)(__float_as_uint(x + 12582912.f) << 23);
+            const float up = __int_as_float(ex + (127 << 23));
+            f[r] = __int_as_float((127 << 23) - ex) * (1.f / MOST);
+            const float p = fast_exp2(s[r] - L[r]);
+            l[r] += p;
+            split7<PARTS>((p * (up * MOST)) * vs, part[e]);
+          }
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) pw[(p * ROWS + r4) / 4] = low_bytes(part[0][p], part[1][p], part[2][p], part[3][p]);
+        }
+#pragma unroll
+        for (int c = 0; c < N / 16; ++c)
+          *reinterpret_cast<uint4*>(smem + SH::WEIGHTS + c * 2048 + key_of * 16) =
+              make_uint4(pw[c * 4], pw[c * 4 + 1], pw[c * 4 + 2], pw[c * 4 + 3]);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full);
+      }
+    }
+    if (ok && n > 0) {
+      add_outputs(n - 1);
+      if (ok) finish();
+    }
   }
+  if (!ok) atomicExch(&dib_attention_int8_error_word, 1);
+  // A grid that fills the GPU lets the kernel that follows come from here on, not earlier: a block of it that lies between
+  // two of this grid's CTAs, or of the next step's, leaves an SM's shared memory in pieces that hold two CTAs instead of
+  // three, and the CTAs that find no place start when others end (four contexts of 32,000 keys: 75 us instead of 64; but
+  // one of 2,048, which does not fill it, 9.9 us instead of 9.0).
+  if (a.late) pdl_trigger();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == SP_SCORE_WARP)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((unsigned)SH::TMEM));
 }
 
-// The runs' results of a row, in the order of the runs: a warp a row, a lane 4 dimensions.
+// The runs' results of a row: out = sum_r 2^(L_r - top) O_r / sum_r 2^(L_r - top) l_r.  A block a row: warp w takes the
+// runs w, w + 4, ... in their order, a lane 4 dimensions; the four warps' sums are added in the order of the warps.
 constexpr int SM_WARPS = 4;
-template <typename T, int NT>
+template <typename T, int ROWS>
 __global__ void __launch_bounds__(SM_WARPS * 32)
 attention_split_merge_kernel(T* __restrict__ out, const __grid_constant__ SplitArgs a) {
-  constexpr int ROWS = 8 * NT;
   const float* part_o = a.part_o;
   const float2* part_ml = a.part_ml;
-  pdl_trigger();
+  __shared__ float4 s_o[SM_WARPS][32];
+  __shared__ float s_top[SM_WARPS], s_sum[SM_WARPS];
+  if (!a.late) pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int i = blockIdx.y, G = a.Hq / a.Hkv;
   const SplitSeq s = split_seq<ROWS>(a, i);
-  const int n_rows = s.n * G;                      // of a kv head
-  const int id = blockIdx.x * SM_WARPS + warp;
-  pdl_wait(part_o, part_ml);
+  const int n_rows = s.n * G, id = blockIdx.x;     // rows of a kv head
   if (s.splits <= 1 || id >= n_rows * a.Hkv || s.splits * s.tiles * a.Hkv > a.max_items) return;
-  const int kvh = id / n_rows, row = id % n_rows, tile = row / ROWS, r = row % ROWS;
+  const int kvh = id / n_rows, row = id - kvh * n_rows, tile = row / ROWS, r = row % ROWS;
   const int p0 = s.kv_len - s.n;
   const int tok0 = tile * ROWS / G, tok1 = min((tile + 1) * ROWS - 1, n_rows - 1) / G;
   // the runs that hold keys which some row of the tile sees
   const int k_lo = first_visible_key(p0 + tok0, a.window), k_hi = p0 + tok1;
   const int s0 = k_lo / s.split, s1 = k_hi < k_lo ? s0 - 1 : min(k_hi / s.split, s.splits - 1);
-  const long long base = (long long)i * a.max_items + (long long)kvh * s.splits * s.tiles + tile;
-  auto at = [&](int run) { return (base + (long long)run * s.tiles) * ROWS + r; };
-  float top = -INFINITY;
-  for (int run = s0 + lane; run <= s1; run += 32) top = fmaxf(top, part_ml[at(run)].x);
-  top = warp_max(top);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f), o2 = o;
-  float sum = 0.f;
+  const long long base = ((long long)i * a.max_items + (long long)(kvh * s.tiles + tile) * s.splits) * ROWS + r;
   const bool in = lane * 4 < a.D;
-  for (int run0 = s0; run0 <= s1; run0 += 32) {
-    float w = 0.f, ws = 0.f;
-    if (run0 + lane <= s1) {
-      const float2 ml = part_ml[at(run0 + lane)];
-      w = fast_exp2(ml.x - ref);
-      ws = w * ml.y;
-    }
-    sum += warp_sum(ws);
-    const int n = min(32, s1 - run0 + 1);
-    int j = 0;
-    for (; j + 8 <= n; j += 8) {
-      float4 v[8];
+  pdl_wait(part_o, part_ml);
+  float top = -INFINITY;
+  for (int run = s0 + (int)threadIdx.x; run <= s1; run += SM_WARPS * 32) top = fmaxf(top, part_ml[base + (long long)run * ROWS].x);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  constexpr int AHEAD = 8;
+  // the first results are on their way while the references are compared
+  float4 v[AHEAD];
+  float2 ml[AHEAD];
+  auto load = [&](int from) {
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        v[u] = in ? *reinterpret_cast<const float4*>(part_o + at(run0 + j + u) * a.D + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float wj = __shfl_sync(0xffffffffu, w, j + u);
-        float4& d = u & 1 ? o2 : o;
-        d.x = fmaf(wj, v[u].x, d.x); d.y = fmaf(wj, v[u].y, d.y);
-        d.z = fmaf(wj, v[u].z, d.z); d.w = fmaf(wj, v[u].w, d.w);
+    for (int u = 0; u < AHEAD; ++u) {
+      const int run = from + u * SM_WARPS;
+      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      ml[u] = make_float2(-INFINITY, 0.f);
+      if (run <= s1) {
+        const long long at = base + (long long)run * ROWS;
+        ml[u] = part_ml[at];
+        if (in) v[u] = *reinterpret_cast<const float4*>(part_o + at * a.D + lane * 4);
       }
     }
-    for (; j < n; ++j) {
-      const float wj = __shfl_sync(0xffffffffu, w, j);
-      const float4 v = in ? *reinterpret_cast<const float4*>(part_o + at(run0 + j) * a.D + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-      o.x = fmaf(wj, v.x, o.x); o.y = fmaf(wj, v.y, o.y); o.z = fmaf(wj, v.z, o.z); o.w = fmaf(wj, v.w, o.w);
+  };
+  load(s0 + warp);
+  top = warp_max(top);
+  if (lane == 0) s_top[warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+  const float ref = top == -INFINITY ? 0.f : top;
+  for (int from = s0 + warp; from <= s1; from += AHEAD * SM_WARPS) {
+    if (from != s0 + warp) load(from);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const float w = fast_exp2(ml[u].x - ref);
+      sum = fmaf(w, ml[u].y, sum);
+      o.x = fmaf(w, v[u].x, o.x); o.y = fmaf(w, v[u].y, o.y);
+      o.z = fmaf(w, v[u].z, o.z); o.w = fmaf(w, v[u].w, o.w);
     }
   }
-  if (!in) return;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const float y[4] = {(o.x + o2.x) * inv, (o.y + o2.y) * inv, (o.z + o2.z) * inv, (o.w + o2.w) * inv};
-  T* dst = out + ((long long)(s.q_begin + row / G) * a.Hq + kvh * G + row % G) * a.D + lane * 4;
+  s_o[warp][lane] = o;
+  if (lane == 0) s_sum[warp] = sum;
+  if (a.late) pdl_trigger();       // (as in the split kernel)
+  __syncthreads();
+  if (warp != 0 || !in) return;
+  float4 y = s_o[0][lane];
+  sum = s_sum[0];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) Elem<T>::store(dst + e, y[e]);
+  for (int k = 1; k < SM_WARPS; ++k) {
+    const float4 z = s_o[k][lane];
+    y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+    sum += s_sum[k];
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int tok = row / G;
+  T* dst = out + ((long long)(s.q_begin + tok) * a.Hq + kvh * G + row - tok * G) * a.D + lane * 4;
+  Elem<T>::store(dst, y.x * inv);
+  Elem<T>::store(dst + 1, y.y * inv);
+  Elem<T>::store(dst + 2, y.z * inv);
+  Elem<T>::store(dst + 3, y.w * inv);
 }
 
 // ---------------------------------------------------------------- the form for every shape
@@ -832,41 +961,50 @@ EncodeTiledFn encode_tiled() {
   }
   return fn;
 }
-// The cache as rows of D bytes; boxes of box_rows x DP bytes (what lies beyond D reads as zero), swizzled.
-bool make_cache_map(CUtensorMap* map, const void* data, long long rows, int D, int DP, int box_rows) {
+// The cache as rows of D bytes; boxes of box_rows x 128 bytes (what lies beyond D reads as zero), swizzled.
+bool make_cache_map(CUtensorMap* map, const void* data, long long rows, int D, int box_rows) {
   EncodeTiledFn enc = encode_tiled();
   if (enc == nullptr) return false;
   const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)D};
-  const cuuint32_t box[2] = {(cuuint32_t)DP, (cuuint32_t)box_rows};
+  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
   return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(data), dims, strides, box, estr,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, DP == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int DP, int NT>
-int launch_split(const CUtensorMap& map, const void* q, void* out, const SplitArgs& a, int max_rows, int merge, int sm_count,
+template <typename T, int ROWS>
+int launch_split(const CUtensorMap& map, const void* q, void* out, SplitArgs a, int max_rows, int merge, int sm_count,
                  cudaStream_t st) {
-  using SH = SplitShape<T, DP, NT>;
-  auto kern = attention_split_kernel<T, DP, NT>;
+  using SH = SplitShape<T, ROWS>;
+  auto kern = attention_split_kernel<T, ROWS>;
   const size_t smem = SH::fixed + ((size_t)a.seq_count + 1) * 4;
   if (smem > 200 * 1024) return DIB_BAD_SIZE;
   static DeviceOnce attr_set;
   if (!attr_set.done()) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess)
+    // (All of an SM's memory as shared memory for both kernels: an SM that is set up otherwise, by the merge of the layer
+    // before, would take two CTAs until it is empty, and a CTA that starts late ends late.)
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess ||
+        cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess ||
+        cudaFuncSetAttribute(attention_split_merge_kernel<T, ROWS>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                             cudaSharedmemCarveoutMaxShared) != cudaSuccess)
       return DIB_LAUNCH_FAILED;
     attr_set.mark();
   }
-  int per_sm = 0;      // the grid is what runs at a time
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, SP_WARPS * 32, smem) != cudaSuccess || per_sm < 1)
-    return DIB_LAUNCH_FAILED;
-  dib_launch(kern, dim3(sm_count * per_sm), dim3(SP_WARPS * 32), smem, st, map, reinterpret_cast<const T*>(q), reinterpret_cast<T*>(out), a);
+  // the grid is what runs at a time: by shared memory (228 KB an SM, 1 KB of each block's own), registers, tensor memory
+  const int by_smem = (int)(228 * 1024 / (smem + 1024)), by_regs = SH::CTAS, by_tmem = 512 / SH::TMEM;
+  int per_sm = by_smem < by_regs ? by_smem : by_regs;
+  per_sm = per_sm < by_tmem ? per_sm : by_tmem;
+  const long long most = (long long)a.max_items * a.seq_count, grid = (long long)sm_count * (per_sm < 1 ? 1 : per_sm);
+  a.late = most >= grid;
+  dib_launch(kern, dim3((unsigned)(grid < most ? grid : most)), dim3(SP_THREADS), smem, st, map, reinterpret_cast<const T*>(q),
+             reinterpret_cast<T*>(out), a);
   DIB_CHECK_LAUNCH();
   if (merge) {
-    const long long blocks = ((long long)max_rows * a.Hkv + SM_WARPS - 1) / SM_WARPS;
+    const long long blocks = (long long)max_rows * a.Hkv;
     if (blocks > 0x7fffffffll) return DIB_BAD_SIZE;
-    dib_launch(attention_split_merge_kernel<T, NT>, dim3((unsigned)blocks, a.seq_count), dim3(SM_WARPS * 32), 0, st,
+    dib_launch(attention_split_merge_kernel<T, ROWS>, dim3((unsigned)blocks, a.seq_count), dim3(SM_WARPS * 32), 0, st,
                reinterpret_cast<T*>(out), a);
     DIB_CHECK_LAUNCH();
   }
@@ -891,8 +1029,8 @@ int dib_attention_int8_status_clear() {
 int dib_int8_attention_split_keys(int kv_len, int rows) { return split_keys(kv_len, rows); }
 
 // The split form, for the sequences seq_list[0 .. seq_count) or (null) seq_first ...: heads up to 128, pages of a
-// power of two of rows, 4 at least.  max_rows: the most rows (new tokens x query heads of a kv head) of one of them; tile_rows: 8
-// or 16 rows a tile; max_items: the most (tiles x runs x kv heads) of one; part_o float32 [seq_count, max_items,
+// power of two of rows, 4 at least.  max_rows: the most rows (new tokens x query heads of a kv head) of one of them; tile_rows: 8,
+// 16 or (bfloat16) 4 or 32 rows a tile; max_items: the most (tiles x runs x kv heads) of one; part_o float32 [seq_count, max_items,
 // tile_rows, D] and part_ml [.., 2] take partial results where merge is not 0 (some sequence may have two runs).
 int dib_int8_attention_split(const void* q, void* out, const void* data, const void* scales, long long num_pages,
                              const void* block_table, int max_blocks, const void* cu_q_lens, const void* seq_lens,
@@ -903,9 +1041,10 @@ int dib_int8_attention_split(const void* q, void* out, const void* data, const v
   const bool pages_fit = page_size >= 4 && (page_size & (page_size - 1)) == 0;
   if (seq_count < 0 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || D < 16 || D > 128 || D % 16 != 0 || page_size < 1 || !pages_fit ||
       num_pages * 2 * Hkv * page_size >= (1ll << 31) || seq_count > 65535 || max_items < 1 || sm_count < 1 ||
-      (tile_rows != 8 && tile_rows != 16))
+      (tile_rows != 8 && tile_rows != 16 && ((tile_rows != 4 && tile_rows != 32) || dtype != 1)))
     return DIB_BAD_SIZE;
-  if (((reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) != 0)
+  if (((reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(q) |
+        reinterpret_cast<uintptr_t>(out)) & 15) != 0)
     return DIB_BAD_ALIGN;
   if (seq_count == 0 || max_rows == 0) return DIB_OK;
   SplitArgs a;
@@ -920,26 +1059,23 @@ int dib_int8_attention_split(const void* q, void* out, const void* data, const v
   a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.window = window;
   a.page_shift = 0;
   while ((1 << a.page_shift) < page_size) ++a.page_shift;
-  a.box_rows = page_size < SP_BLOCK ? page_size : SP_BLOCK;
+  a.box_rows = page_size < SP_TILE ? page_size : SP_TILE;
   a.scale = scale;
   a.part_o = reinterpret_cast<float*>(part_o);
   a.part_ml = reinterpret_cast<float2*>(part_ml);
   a.max_items = max_items;
   a.num_pages = (int)num_pages;
-  const int DP = D <= 64 ? 64 : 128;
   CUtensorMap map;
-  if (!make_cache_map(&map, data, num_pages * 2 * Hkv * page_size, D, DP, a.box_rows)) return DIB_LAUNCH_FAILED;
+  if (!make_cache_map(&map, data, num_pages * 2 * Hkv * page_size, D, a.box_rows)) return DIB_LAUNCH_FAILED;
   using B = __nv_bfloat16;
   if (dtype == 1) {
-    if (DP == 128) return tile_rows == 8 ? launch_split<B, 128, 1>(map, q, out, a, max_rows, merge, sm_count, st)
-                                         : launch_split<B, 128, 2>(map, q, out, a, max_rows, merge, sm_count, st);
-    return tile_rows == 8 ? launch_split<B, 64, 1>(map, q, out, a, max_rows, merge, sm_count, st)
-                          : launch_split<B, 64, 2>(map, q, out, a, max_rows, merge, sm_count, st);
+    if (tile_rows == 4) return launch_split<B, 4>(map, q, out, a, max_rows, merge, sm_count, st);
+    if (tile_rows == 8) return launch_split<B, 8>(map, q, out, a, max_rows, merge, sm_count, st);
+    if (tile_rows == 16) return launch_split<B, 16>(map, q, out, a, max_rows, merge, sm_count, st);
+    return launch_split<B, 32>(map, q, out, a, max_rows, merge, sm_count, st);
   }
-  if (DP == 128) return tile_rows == 8 ? launch_split<float, 128, 1>(map, q, out, a, max_rows, merge, sm_count, st)
-                                       : launch_split<float, 128, 2>(map, q, out, a, max_rows, merge, sm_count, st);
-  return tile_rows == 8 ? launch_split<float, 64, 1>(map, q, out, a, max_rows, merge, sm_count, st)
-                        : launch_split<float, 64, 2>(map, q, out, a, max_rows, merge, sm_count, st);
+  if (tile_rows == 8) return launch_split<float, 8>(map, q, out, a, max_rows, merge, sm_count, st);
+  return launch_split<float, 16>(map, q, out, a, max_rows, merge, sm_count, st);
 }
 
 int dib_int8_attention_any(const void* q, void* out, const void* data, const void* scales, const void* block_table,

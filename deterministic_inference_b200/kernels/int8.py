@@ -255,13 +255,13 @@ def _lib():
 class _SplitPart:
     """The sequences of one launch: their number, the most rows of one, rows a tile, the most work items of one."""
 
-    def __init__(self, seqs: list, q_lens: list, kv_lens: list, group: int, hkv: int, device):
+    def __init__(self, seqs: list, q_lens: list, kv_lens: list, group: int, hkv: int, wide: bool, device):
         first, count = seqs[0], len(seqs)
         self.first, self.count, self.list = first, count, None
         if seqs != list(range(first, first + count)):
             self.list = torch.tensor(seqs, dtype=torch.int32).to(device, non_blocking=True)
         self.max_rows = max(q_lens[s] for s in seqs) * group
-        self.tile_rows = 8 if self.max_rows <= 8 else 16
+        self.tile_rows = next(r for r in ((8, 16) if wide else (4, 8, 16, 32)) if self.max_rows <= r or r == (16 if wide else 32))
         runs = _most_runs(max(kv_lens[s] for s in seqs))
         tiles, per32 = -(-self.max_rows // self.tile_rows), 32 // self.tile_rows
         # (runs get longer with the rows: tiles * runs is largest at 64 rows, or the tiles' own number is)
@@ -269,14 +269,14 @@ class _SplitPart:
         self.merge = runs > 1
 
 
-def _split_parts(meta, group: int, hkv: int, device) -> list:
-    key = ("int8_split", group, hkv)
+def _split_parts(meta, group: int, hkv: int, wide: bool, device) -> list:
+    key = ("int8_split", group, hkv, wide)
     parts = meta.scratch.get(key)
     if parts is None:
         q_lens, kv_lens = meta.q_lens, meta.kv_lens
         one = [s for s, n in enumerate(q_lens) if n == 1]
         more = [s for s, n in enumerate(q_lens) if n > 1]
-        parts = [_SplitPart(x, q_lens, kv_lens, group, hkv, device) for x in (one, more) if x]
+        parts = [_SplitPart(x, q_lens, kv_lens, group, hkv, wide, device) for x in (one, more) if x]
         meta.scratch[key] = parts
     return parts
 
@@ -322,8 +322,8 @@ def int8_paged_attention(q: torch.Tensor, cache: Int8Cache, meta, scale: float, 
     out = torch.empty_like(q)
     if t == 0:
         return out
-    if d <= 128 and _pages_fit(page_size) and q.data_ptr() % 16 == 0 and pages * 2 * hkv * page_size < 1 << 31:
-        for part in _split_parts(meta, hq // hkv, hkv, q.device):
+    if d <= 128 and _pages_fit(page_size) and q.data_ptr() % 16 == 0 and cache.scales.data_ptr() % 16 == 0 and pages * 2 * hkv * page_size < 1 << 31:
+        for part in _split_parts(meta, hq // hkv, hkv, q.dtype == torch.float32, q.device):
             _split(q, out, cache, meta, part, float(scale), win)
         return out
     st = ops._lib("attention_int8").dib_int8_attention_any(

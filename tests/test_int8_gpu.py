@@ -10,6 +10,8 @@ Tolerances, before any run:
                                of the output, relative to the largest value seen, probabilities of 22 bits or more
                                (float32) another 2^-20, those rounded to bfloat16 (bfloat16) 2^-8 and the exponential's
                                2^-12; the bfloat16 output's rounding is 2^-8 of itself.
+                               (The kernels keep bfloat16 queries to 15 bits of a row's largest element and their
+                               probabilities to 15 bits of a tile's largest weight: the 2^-8 holds both.)
 """
 
 from __future__ import annotations
