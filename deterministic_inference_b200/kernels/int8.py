@@ -79,6 +79,8 @@ class Int8Weight:
             padded = torch.zeros(n, _padded(k), dtype=torch.int8, device=codes.device)
             padded[:, :k] = codes
             codes = padded
+        if scales.data_ptr() % 16:
+            scales = scales.clone()
         self.codes, self.scales = codes, scales
 
     @classmethod
@@ -147,6 +149,12 @@ def int8_linear(x, weight: Int8Weight, out_dtype=None) -> torch.Tensor:
         c_int(n), c_int(x.codes.shape[1]), c_int(ops._dt(out, "out")), c_int(_sms(x.device)), ops._stream())
     ops._check(st, "int8_linear", f"M={m} N={n} K={x.k}")
     return out
+
+
+def force_product_form(form: int) -> None:
+    """Measurement and test switch of the product: mma.sync on a streamed weight (0), tiles of 128 x 64, 128 x 128 or
+    128 x 256 (1, 2, 3), the pair of CTAs (4), whatever the sizes; -1: the library's own choice.  All give the same bits."""
+    _ops()._lib("gemm_int8").dib_gemm_int8_force_form(c_int(form))
 
 
 def _sms(device) -> int:

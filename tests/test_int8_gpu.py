@@ -137,6 +137,23 @@ def test_a_row_of_a_product_does_not_depend_on_the_others(n, k):
         assert torch.equal(ops.int8_linear(x[:m], w, F32), all_rows[:m])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m,n,k", [(1, 17, 40), (129, 257, 130), (300, 1000, 520), (513, 513, 1040), (256, 24, 16)])
+def test_every_form_of_a_product_gives_the_same_bits(m, n, k, dtype):
+    from deterministic_inference_b200.kernels import int8
+    x, w = _rand(m, k, seed=m, dtype=dtype), ops.Int8Weight.of(_rand(n, k, seed=n))
+    want = ops.int8_linear(x, w)
+    _check_product(want, x, w.codes[:, :k], w.scales, dtype)
+    try:
+        for form in range(5):
+            int8.force_product_form(form)
+            got = ops.int8_linear(x, w)
+            ops.check_kernel_status()
+            assert torch.equal(got, want), f"form {form}"
+    finally:
+        int8.force_product_form(-1)
+
+
 def test_product_with_no_rows():
     w = ops.Int8Weight.of(_rand(32, 64))
     assert ops.int8_linear(torch.empty(0, 64, device="cuda"), w).shape == (0, 32)
