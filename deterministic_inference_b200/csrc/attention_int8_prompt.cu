@@ -1,0 +1,815 @@
+// Attention of a prompt's portion over a paged cache in 8-bit integers (cache_int8.cu; formulas in attention_int8.cu), for
+// bfloat16 queries and many rows: S = Q K^T and O = P V by tcgen05.mma kind::f16 on bfloat16, accumulators in tensor memory,
+// a thread a query row for the softmax.
+//
+// The codes are exact in bfloat16, so they enter both products as they are: three warps turn a key tile's bytes (fetched by
+// TMA, a box a page) into swizzled bfloat16 tiles, once for the 256 rows of the two query tiles that share them.  A key's
+// scale (times the softmax's) joins its column of the scores, a value's the probabilities before they are rounded to
+// bfloat16 for the second product; the sum of probabilities is taken before that.
+//
+// Two query tiles A and B of 128 rows (tokens x heads of a kv group) of one sequence a CTA.  Roles: warps 0-3 softmax of A,
+// 4-7 of B (a row's 128 scores in registers; probabilities go back to tensor memory over the scores and are the second
+// product's operand from there), warp 9 issues the products, warps 8, 10, 11 convert, and warp 8 sends for the next bytes.
+// The products of the two tiles are staggered, each tile's softmax runs under the other's products.  Once a tile has had
+// its last key tile (or there is no B) the other runs alone and takes its score columns as a second buffer.
+// Tensor memory: S/P of A columns 0.., of B 128.., O of A 256.., of B 384...
+//
+// Keys are cut at multiples of 4,096 (chunks of constant size from key 0); a query tile that reaches over a cut has a CTA a
+// chunk, and a second kernel adds the partial results in chunk order.  Key tiles are anchored at key 0 and cuts depend on
+// positions alone, so a row's bits do not depend on the step.
+//
+// What bounds it: the softmax threads' instructions (a score's scale, maximum, exponential, sum, value scale and packing),
+// with the conversion beside them; the products take half of that time.
+#include <cuda.h>
+
+#include "common.cuh"
+
+namespace {
+
+constexpr int TILE = 128, THREADS = 384, COPY_WARP = 8, MMA_WARP = 9;
+constexpr int REGS_FEW = 80, REGS_MANY = 208;         // 128 * 80 + 256 * 208 <= 384 * 168
+constexpr int TILE_BYTES = 128 * 128 * 2, HALF_BYTES = 128 * 64 * 2;      // a bfloat16 tile: two halves of 64 columns
+constexpr int RAW_BYTES = 128 * 128;
+constexpr float NEG_BIG = -1e30f;
+constexpr float LOG2E = 1.4426950408889634f;
+
+// shared memory: queries of A and B, two stages of keys and values, the bytes of a tile's keys and values, scales
+constexpr int S_KV = 2 * TILE_BYTES, S_RAW = 6 * TILE_BYTES, S_SCALES = S_RAW + 2 * RAW_BYTES, S_BARS = S_SCALES + 2 * 1024;
+constexpr int S_TOTAL = S_BARS + 24 * 8, S_DYNAMIC = 232448;
+
+__device__ int dib_attention_int8_prompt_error_word = 0;
+
+template <int N> __device__ __forceinline__ void regs_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(unsigned long long* bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(unsigned long long* bar, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(unsigned long long* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(unsigned dst, const CUtensorMap* map, int c0, int c1, unsigned long long* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<unsigned long long>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&v);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x for x <= ~8, two values at once on the FMA and integer pipes: the nearest integer by its exponent bits, the rest by a
+// cubic (relative error 1e-4, below the bfloat16 step of the probabilities).
+__device__ __forceinline__ float2 exp2_fma2(float2 x) {
+  x.x = fmaxf(x.x, -125.0f);
+  x.y = fmaxf(x.y, -125.0f);
+  const float2 magic = make_float2(12582912.0f, 12582912.0f);
+  const float2 xf = __fadd2_rn(x, magic);
+  const float2 t = __fadd2_rn(xf, make_float2(-12582912.0f, -12582912.0f));
+  const float2 f = __ffma2_rn(t, make_float2(-1.0f, -1.0f), x);
+  float2 p = __ffma2_rn(f, make_float2(0.05500893f, 0.05500893f), make_float2(0.24221095f, 0.24221095f));
+  p = __ffma2_rn(p, f, make_float2(0.6932829f, 0.6932829f));
+  p = __ffma2_rn(p, f, make_float2(1.0f, 1.0f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(xf.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(xf.y) << 23)));
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(unsigned long long* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_mma(unsigned tmem_d, unsigned long long desc_a, unsigned long long desc_b, unsigned idesc,
+                                       unsigned accum) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accum)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(unsigned tmem_d, unsigned tmem_a, unsigned long long desc_b, unsigned idesc,
+                                          unsigned accum) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "}\n" ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accum)
+      : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_ld32(unsigned taddr, unsigned (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tc_st32(unsigned taddr, const unsigned (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31, %32};\n" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+// Descriptors (rows of 128 bytes, 128-byte swizzle, 8-row groups 1,024 bytes apart): K-major; MN-major, the next 64 columns
+// half a tile on.
+__device__ __forceinline__ unsigned long long desc_k_major(unsigned addr) {
+  return (unsigned long long)((addr & 0x3FFFFu) >> 4) | ((unsigned long long)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ unsigned long long desc_mn_major(unsigned addr) {
+  return desc_k_major(addr) | ((unsigned long long)(HALF_BYTES >> 4) << 16);
+}
+// kind::f16: float32 accumulator, bfloat16 A and B
+constexpr unsigned idesc_f16(int m, int n, int b_mn_major) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)b_mn_major << 16) | ((unsigned)(n >> 3) << 17) |
+         ((unsigned)(m >> 4) << 24);
+}
+// byte offset of (row, 16-byte piece c of the row's 128 elements) in a bfloat16 tile
+__device__ __forceinline__ int piece_off(int row, int c) {
+  return (c >> 3) * HALF_BYTES + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+}
+// Two codes of a word as bfloat16, exactly: low 7 bits and sign bit of a byte under the exponent byte 0x43 are 128 + low and
+// 128 + 128 sign, and a code is the first minus the second.
+__device__ __forceinline__ unsigned codes_bf16(unsigned low7, unsigned sign, unsigned sel) {
+  const unsigned a = __byte_perm(low7, 0x43434343u, sel), b = __byte_perm(sign, 0x43434343u, sel);
+  const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const unsigned*>(&d);
+}
+
+struct PromptArgs {
+  const float* scales;          // [pages, 2, Hkv, page_size]
+  const int* block_table;       // [B, max_blocks]
+  const int* cu_q_lens;
+  const int* seq_lens;
+  const int* units;             // [4][count]: sequence, first token of A, of B (or -1), chunk
+  int count, max_blocks, Hq, Hkv, D, page_shift, num_pages, window, chunk_tiles, max_chunks;
+  float scale;
+  float* part_o;                // [T, Hq, max_chunks, 128]
+  float2* part_ml;              // [T, Hq, max_chunks]: reference (log 2), sum
+};
+
+__global__ void __launch_bounds__(THREADS, 1)
+attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __restrict__ q,
+                        __nv_bfloat16* __restrict__ out, const __grid_constant__ PromptArgs a) {
+  extern __shared__ unsigned char smem_dyn[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~(uintptr_t)1023);
+  unsigned char* sQ = smem;
+  unsigned char* sKV = smem + S_KV;
+  unsigned char* raw = smem + S_RAW;
+  float* scales = reinterpret_cast<float*>(smem + S_SCALES);          // [2][keys', values' of 128]
+  unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + S_BARS);
+  unsigned long long* raw_full = bars;            // [keys, values] a tile's bytes have arrived
+  unsigned long long* k_full = bars + 2;          // [2] the keys of a tile are there as bfloat16
+  unsigned long long* k_empty = bars + 4;         // [2] both score products have read them
+  unsigned long long* v_full = bars + 6;          // [2] the values likewise
+  unsigned long long* v_empty = bars + 8;         // [2]
+  unsigned long long* sc_full = bars + 10;        // [2] the scales of a tile are there
+  unsigned long long* s_full = bars + 12;         // [A, B] the query tile's scores are in tensor memory
+  unsigned long long* p_full = bars + 14;         // [2] its probabilities are, and O is rescaled (128)
+  unsigned long long* o_final = bars + 16;        // [2] its last product has completed
+  unsigned long long* pv_done = bars + 18;        // an output product of the tile that runs alone has completed
+  unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 19);
+  if (threadIdx.x == 0) prefetch_tensormap(&map);
+  pdl_trigger();
+  if (smem - smem_dyn + S_TOTAL > S_DYNAMIC) {      // (the memory is aligned to 1,024 as a rule)
+    if (threadIdx.x == 0) atomicExch(&dib_attention_int8_prompt_error_word, 2);
+    return;
+  }
+  const int unit = a.count - 1 - blockIdx.y, kvh = blockIdx.x;        // the longest first
+  const int G = a.Hq / a.Hkv, npt = TILE / G;                         // tokens of a query tile
+  const int seq = a.units[unit];
+  const int tokx[2] = {a.units[a.count + unit], a.units[2 * a.count + unit]};
+  const int chunk = a.chunk_tiles > 0 ? a.units[3 * a.count + unit] : 0;
+  const int q_begin = a.cu_q_lens[seq], q_len = a.cu_q_lens[seq + 1] - q_begin;
+  const int kv_len = min(a.seq_lens[seq], (int)min((long long)a.max_blocks << a.page_shift, 0x7fffff00ll));
+  const int prefix = kv_len - q_len;
+  const int* bt = a.block_table + (long long)seq * a.max_blocks;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // Per query tile: its tokens and the key tiles of this chunk that it needs.
+  int ntok[2], jf[2], jl[2];
+  bool whole[2];
+  const int c_lo = chunk * a.chunk_tiles, c_hi = a.chunk_tiles > 0 ? c_lo + a.chunk_tiles - 1 : 0x7fffffff;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int t0 = tokx[x];
+    ntok[x] = t0 >= 0 ? max(0, min(npt, q_len - t0)) : 0;
+    const int last_pos = prefix + t0 + ntok[x] - 1;
+    const int f = first_visible_key(prefix + t0, a.window) / TILE;
+    const int l = ntok[x] > 0 && last_pos >= 0 ? last_pos / TILE : -1;      // an empty tile is never active
+    whole[x] = a.chunk_tiles <= 0 || f / a.chunk_tiles == l / a.chunk_tiles;
+    jf[x] = max(f, c_lo);
+    jl[x] = min(l, c_hi);
+    if (l < 0 && ntok[x] > 0 && chunk == 0) {      // its rows lie before the first key: zeros
+      pdl_wait();
+      for (int e = threadIdx.x; e < ntok[x] * G * a.D; e += THREADS) {
+        const int row = e / a.D;
+        out[((long long)(q_begin + t0 + row / G) * a.Hq + kvh * G + row % G) * a.D + e % a.D] = __float2bfloat16_rn(0.f);
+      }
+    }
+  }
+  const bool any0 = jl[0] >= jf[0], any1 = jl[1] >= jf[1];
+  if (!any0 && !any1) return;     // nothing of this chunk concerns the pair
+  const int j0 = any0 && any1 ? min(jf[0], jf[1]) : (any0 ? jf[0] : jf[1]);
+  const int ntiles = max(any0 ? jl[0] : -1, any1 ? jl[1] : -1) - j0 + 1;
+  auto active = [&](int x, int i) { return j0 + i >= jf[x] && j0 + i <= jl[x]; };
+  // From key tile solo_from on query tile solo_x is alone; the other one has had n_other key tiles.
+  const int solo_x = (any1 && (!any0 || jl[1] >= jl[0])) ? 1 : 0;
+  const int n_other = (solo_x ? any0 : any1) ? jl[1 - solo_x] - jf[1 - solo_x] + 1 : 0;
+  const int solo_from = max((solo_x ? any0 : any1) ? jl[1 - solo_x] - j0 + 1 : 0, jf[solo_x] - j0);
+
+  bool ok = true;
+  // ---- bytes of key tile i (0 keys, 1 values): lane l has the keys 4l .. 4l + 3, the first lane of each page sends
+  const int page_mask = (1 << a.page_shift) - 1, half_rows = a.Hkv << a.page_shift, box_rows = min(1 << a.page_shift, TILE);
+  auto row_of = [&](int i) {      // this lane's row of the cache for its keys of key tile i, or -1
+    const int key = (j0 + i) * TILE + lane * 4;
+    if (i >= ntiles || key >= kv_len) return -1;
+    const int page = bt[key >> a.page_shift];
+    return page >= 0 && page < a.num_pages ? page * 2 * half_rows + (kvh << a.page_shift) + (key & page_mask) : -1;
+  };
+  auto send = [&](int kv, int row) {
+    const bool sends = row >= 0 && (lane == 0 || (lane * 4 & page_mask) == 0);
+    const unsigned senders = __ballot_sync(0xffffffffu, sends);
+    if (lane == 0) mbar_expect_tx(&raw_full[kv], __popc(senders) * box_rows * 128);
+    __syncwarp();
+    if (sends) tma_load_2d(smem_u32(raw) + kv * RAW_BYTES + lane * 512, &map, 0, row + kv * half_rows, &raw_full[kv]);
+  };
+  int row_next = -1;
+  if (warp == COPY_WARP) {
+    if (lane == 0) {
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&raw_full[i], 1);
+        mbar_init(&k_full[i], 1);
+        mbar_init(&k_empty[i], 1);
+        mbar_init(&v_full[i], 1);
+        mbar_init(&v_empty[i], 1);
+        mbar_init(&sc_full[i], 2);
+        mbar_init(&s_full[i], 1);
+        mbar_init(&p_full[i], 128);
+        mbar_init(&o_final[i], 1);
+      }
+      mbar_init(pv_done, 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    row_next = row_of(0);
+  }
+  const __nv_bfloat16* qp = q;
+  pdl_wait(qp);
+  if (warp == COPY_WARP) {
+    send(0, row_next);
+    send(1, row_next);
+    row_next = row_of(1);
+  }
+  if (warp == MMA_WARP) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  // both query tiles -> shared memory, swizzled; rows beyond a tile's tokens and dimensions beyond D are zero
+  {
+    constexpr int LOADERS = 256, PER_THREAD = 2 * TILE * 16 / LOADERS;
+    uint4 v[PER_THREAD];
+#pragma unroll
+    for (int it = 0; it < PER_THREAD; ++it) {
+      const int c = threadIdx.x + it * LOADERS;
+      const int x = c >> 11, r = (c >> 4) & 127, ch = c & 15;
+      const int tl = r / G, g = r - tl * G;
+      v[it] = make_uint4(0, 0, 0, 0);
+      if (threadIdx.x < LOADERS && tl < ntok[x] && ch * 8 < a.D)
+        v[it] = *reinterpret_cast<const uint4*>(qp + ((long long)(q_begin + tokx[x] + tl) * a.Hq + kvh * G + g) * a.D + ch * 8);
+    }
+#pragma unroll
+    for (int it = 0; it < PER_THREAD; ++it) {
+      const int c = threadIdx.x + it * LOADERS;
+      const int x = c >> 11, r = (c >> 4) & 127, ch = c & 15;
+      if (threadIdx.x < LOADERS) *reinterpret_cast<uint4*>(sQ + x * TILE_BYTES + piece_off(r, ch)) = v[it];
+    }
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the queries are read by the tensor core
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const unsigned tmem = *tmem_slot;
+
+  if (warp >= COPY_WARP) {
+  regs_give<REGS_FEW>();
+  if (warp == MMA_WARP) {
+    if (lane == 0) {
+      constexpr unsigned idesc_s = idesc_f16(TILE, TILE, 0), idesc_o = idesc_f16(TILE, TILE, 1);
+      // Descriptors are made once: a step inside a tile is an addition to the low bits, which hold the address.
+      const unsigned long long q_desc[2] = {desc_k_major(smem_u32(sQ)), desc_k_major(smem_u32(sQ + TILE_BYTES))};
+      unsigned long long k_desc[2], v_desc[2];
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        k_desc[st] = desc_k_major(smem_u32(sKV + st * 2 * TILE_BYTES));
+        v_desc[st] = desc_mn_major(smem_u32(sKV + st * 2 * TILE_BYTES + TILE_BYTES));
+      }
+      auto issue_s = [&](int x, int buf, int i) {      // scores of query tile x, key tile i -> columns of buf
+        const unsigned long long qd = x ? q_desc[1] : q_desc[0], kd = i & 1 ? k_desc[1] : k_desc[0];
+#pragma unroll
+        for (int ks = 0; ks < TILE / 16; ++ks) {
+          const unsigned long long at = (unsigned long long)(((ks >> 2) * HALF_BYTES + (ks & 3) * 32) >> 4);
+          tc_mma(tmem + buf * 128, qd + at, kd + at, idesc_s, ks > 0);
+        }
+        tc_commit(&s_full[buf]);
+      };
+      auto issue_o = [&](int x, int buf, int i) {      // outputs of query tile x from the probabilities in buf
+        const unsigned long long vd = i & 1 ? v_desc[1] : v_desc[0];
+        const bool first = j0 + i == jf[x];
+#pragma unroll
+        for (int ks = 0; ks < TILE / 16; ++ks)
+          tc_mma_ts(tmem + 256 + x * 128, tmem + buf * 128 + ks * 8, vd + (unsigned long long)((ks * 16 * 128) >> 4), idesc_o,
+                    !first || ks > 0);
+      };
+      int uses[2] = {0, 0};     // completed phases of p_full
+      int have_k = 0, have_v = -1;
+      auto want_k = [&](int i) {
+        if (have_k < i) {
+          ok = mbar_wait(&k_full[i & 1], (i >> 1) & 1);
+          have_k = i;
+        }
+        return ok;
+      };
+      auto want_v = [&](int i) {
+        if (have_v < i) {
+          ok = mbar_wait(&v_full[i & 1], (i >> 1) & 1);
+          have_v = i;
+        }
+        return ok;
+      };
+      ok = mbar_wait(&k_full[0], 0);
+      if (ok) {
+        tc_fence_after();
+        if (active(0, 0)) issue_s(0, 0, 0);
+        if (active(1, 0)) issue_s(1, 1, 0);
+        tc_commit(&k_empty[0]);
+      }
+      const int paired_end = min(ntiles, solo_from);
+      for (int i = 0; i < paired_end && ok; ++i) {
+        if (!want_v(i) || (i + 1 < ntiles && !want_k(i + 1))) break;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (active(x, i)) {
+            ok = mbar_wait(&p_full[x], uses[x] & 1);
+            if (!ok) break;
+            ++uses[x];
+            tc_fence_after();
+            issue_o(x, x, i);
+            if (j0 + i == jl[x]) tc_commit(&o_final[x]);
+          }
+          if (x == 1) tc_commit(&v_empty[i & 1]);
+          if (i + 1 < ntiles && active(x, i + 1)) issue_s(x, x, i + 1);
+          if (x == 1 && i + 1 < ntiles) tc_commit(&k_empty[(i + 1) & 1]);
+        }
+      }
+      // ---- one query tile alone: its scores of key tile i are in buffer (i - solo_from) & 1 (0: its own columns); those of
+      // i + 1 go to the other one before the probabilities of i are waited for
+      for (int i = solo_from; i < ntiles && ok; ++i) {
+        const int x = solo_x, buf = ((i - solo_from) & 1) ? 1 - x : x;
+        if (i + 1 < ntiles) {
+          if (!want_k(i + 1)) break;
+          issue_s(x, 1 - buf, i + 1);
+          tc_commit(&k_empty[(i + 1) & 1]);
+        }
+        if (!want_v(i)) break;
+        ok = mbar_wait(&p_full[buf], uses[buf] & 1);
+        if (!ok) break;
+        ++uses[buf];
+        tc_fence_after();
+        issue_o(x, buf, i);
+        tc_commit(&v_empty[i & 1]);
+        tc_commit(pv_done);
+        if (i == ntiles - 1) tc_commit(&o_final[x]);
+      }
+    }
+  } else {
+    // ---- conversion.  A warp takes 8 rows x 64 codes at a time: eight lanes a pair of rows r, r ^ 5, whose pieces lie in
+    // different banks in the bytes' swizzle and in the bfloat16 tile's.
+    const int part = warp == COPY_WARP ? 0 : warp - 9;        // 0, 1, 2
+    const int r8 = lane & 4 ? (lane >> 3) ^ 5 : lane >> 3, p4 = lane & 3;
+    auto convert = [&](const unsigned char* src, unsigned char* dst) {
+#pragma unroll 2
+      for (int u = part; u < 32; u += 3) {
+        const int row = (u >> 1) * 8 + r8, p = (u & 1) * 4 + p4;
+        const uint4 w = *reinterpret_cast<const uint4*>(src + row * 128 + ((p ^ (row & 7)) << 4));
+        const unsigned word[4] = {w.x, w.y, w.z, w.w};
+        unsigned y[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned low7 = word[e] & 0x7f7f7f7fu, sign = word[e] & 0x80808080u;
+          y[2 * e] = codes_bf16(low7, sign, 0x4140);
+          y[2 * e + 1] = codes_bf16(low7, sign, 0x4342);
+        }
+        *reinterpret_cast<uint4*>(dst + piece_off(row, 2 * p)) = make_uint4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<uint4*>(dst + piece_off(row, 2 * p + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the tile is read by the tensor core, the bytes are
+      asm volatile("bar.sync 1, 96;" ::: "memory");                    // written by the next copy
+    };
+    for (int i = 0; i < ntiles && ok; ++i) {
+      unsigned char* stage = sKV + (i & 1) * 2 * TILE_BYTES;
+      // the scales of this lane's keys: warp part 0 the keys', 1 the values'; zero for keys the sequence does not have
+      float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (part < 2) {
+        const int row = row_of(i);
+        const int left = kv_len - ((j0 + i) * TILE + lane * 4);
+        if (row >= 0) {
+          sc = *reinterpret_cast<const float4*>(a.scales + row + part * half_rows);
+          if (part == 1) {      // a key that is no number shows through its value (the scores' maximum does not see it)
+            const float4 k = *reinterpret_cast<const float4*>(a.scales + row);
+            sc.x += k.x - k.x; sc.y += k.y - k.y; sc.z += k.z - k.z; sc.w += k.w - k.w;
+          }
+          if (left < 2) sc.y = 0.f;
+          if (left < 3) sc.z = 0.f;
+          if (left < 4) sc.w = 0.f;
+        }
+        if (part == 0) {
+          const float unit = a.scale * LOG2E;
+          sc.x *= unit; sc.y *= unit; sc.z *= unit; sc.w *= unit;
+        }
+      }
+      ok = mbar_wait(&raw_full[0], i & 1) && (i < 2 || mbar_wait(&k_empty[i & 1], ((i >> 1) - 1) & 1));
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      convert(raw, stage);
+      if (warp == COPY_WARP) {
+        if (lane == 0) mbar_arrive(&k_full[i & 1]);
+        if (i + 1 < ntiles) send(0, row_next);
+      }
+      ok = mbar_wait(&raw_full[1], i & 1) && (i < 2 || mbar_wait(&v_empty[i & 1], ((i >> 1) - 1) & 1));
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (part < 2) {      // (the softmax has read those of the tile two before this one: its outputs have been made)
+        *reinterpret_cast<float4*>(scales + (i & 1) * 256 + part * 128 + lane * 4) = sc;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sc_full[i & 1]);
+      }
+      convert(raw + RAW_BYTES, stage + TILE_BYTES);
+      if (warp == COPY_WARP) {
+        if (lane == 0) mbar_arrive(&v_full[i & 1]);
+        if (i + 1 < ntiles) {
+          send(1, row_next);
+          row_next = row_of(i + 2);
+        }
+      }
+    }
+  }
+  } else {
+    regs_take<REGS_MANY>();
+    // ---- softmax: thread r of group x owns row r of query tile x
+    const int x = threadIdx.x >> 7, r = threadIdx.x & 127;
+    const int tl = r / G, g = r - tl * G;
+    const bool valid = tl < ntok[x];
+    // (rows behind the sequence's last token see what a token there would see: no warp goes through the tests for masked
+    // keys for their sake)
+    const int hi = prefix + tokx[x] + tl, lo = first_visible_key(hi, a.window);
+    const unsigned lane_base = (unsigned)((warp & 3) * 32) << 16;
+    const unsigned tmem_o = tmem + lane_base + 256 + x * 128;
+    float m_ref = NEG_BIG, l = 0.f;
+    int uses_own = 0, uses_other = n_other;      // completed phases of s_full of the own columns and of the other's
+    const int my_solo = x == solo_x ? solo_from : 0x7fffffff;
+    for (int i = 0; i < ntiles && ok; ++i) {
+      if (!active(x, i)) continue;
+      const bool borrowed = i >= my_solo && ((i - my_solo) & 1);
+      const int buf = borrowed ? 1 - x : x;
+      const unsigned tmem_s = tmem + lane_base + buf * 128;
+      ok = mbar_wait(&sc_full[i & 1], (i >> 1) & 1) && mbar_wait(&s_full[buf], (borrowed ? uses_other : uses_own) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (borrowed) ++uses_other; else ++uses_own;
+      tc_fence_after();
+      const int kbase = (j0 + i) * TILE;
+      const bool full = kbase >= lo && kbase + TILE - 1 <= hi;   // no key of the tile is masked
+      const float* ks = scales + (i & 1) * 256;
+      const float* vs = ks + 128;
+      unsigned v[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tc_ld32(tmem_s + c * 32, v[c]);
+      tc_wait_ld();
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          const float4 w = *reinterpret_cast<const float4*>(ks + c * 32 + k);
+          const float2 y0 = __fmul2_rn(make_float2(__uint_as_float(v[c][k]), __uint_as_float(v[c][k + 1])), make_float2(w.x, w.y));
+          const float2 y1 = __fmul2_rn(make_float2(__uint_as_float(v[c][k + 2]), __uint_as_float(v[c][k + 3])), make_float2(w.z, w.w));
+          v[c][k] = __float_as_uint(y0.x); v[c][k + 1] = __float_as_uint(y0.y);
+          v[c][k + 2] = __float_as_uint(y1.x); v[c][k + 3] = __float_as_uint(y1.y);
+        }
+      if (!full) {
+        // keys outside [lo, hi] get NEG_BIG: one subtraction and one unsigned comparison each
+        const int first = lo - kbase, last = hi - kbase;
+        const int first_vis = last >= first ? first : (1 << 20);
+        const unsigned span = last >= first ? (unsigned)(last - first) : 0u;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if ((unsigned)(c * 32 + k - first_vis) > span) v[c][k] = __float_as_uint(NEG_BIG);
+      }
+      float m4[4] = {NEG_BIG, NEG_BIG, NEG_BIG, NEG_BIG};
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int k = 0; k < 32; k += 8)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            m4[j] = max3(m4[j], __uint_as_float(v[c][k + 2 * j]), __uint_as_float(v[c][k + 2 * j + 1]));
+      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+      // the reference rises only when it must (or at the first visible key)
+      float factor = 1.0f;
+      bool rescale = false;
+      if (mx > m_ref + 8.0f) {
+        rescale = m_ref > -1e29f;
+        factor = rescale ? fast_exp2(m_ref - mx) : 0.f;
+        m_ref = mx;
+        l *= factor;
+      }
+      const float m_use = m_ref <= -1e29f ? 0.f : m_ref;
+      // Two keys in eight take their exponentials on the FMA pipe, the others on the special-function unit.
+      float2 s8[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      const float2 nm2 = make_float2(-m_use, -m_use);
+      if (full) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            float2 p[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              p[j] = __fadd2_rn(make_float2(__uint_as_float(v[c][k + 2 * j]), __uint_as_float(v[c][k + 2 * j + 1])), nm2);
+#pragma unroll
+            for (int j = 0; j < 3; ++j) p[j] = make_float2(fast_exp2(p[j].x), fast_exp2(p[j].y));
+            p[3] = exp2_fma2(p[3]);
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+              const float4 w = *reinterpret_cast<const float4*>(vs + c * 32 + k + 2 * j);
+              s8[j] = __fadd2_rn(s8[j], p[j]);
+              s8[j + 1] = __fadd2_rn(s8[j + 1], p[j + 1]);
+              const float2 y0 = __fmul2_rn(p[j], make_float2(w.x, w.y)), y1 = __fmul2_rn(p[j + 1], make_float2(w.z, w.w));
+              v[c >> 1][(c & 1) * 16 + (k >> 1) + j] = pack_bf16(y0.x, y0.y);      // 64 packed pairs in v[0], v[1]
+              v[c >> 1][(c & 1) * 16 + (k >> 1) + j + 1] = pack_bf16(y1.x, y1.y);
+            }
+          }
+      } else {
+        // a tile with masked keys: every exponential on the special-function unit, whose result for a masked score is
+        // exactly zero; the scale of a masked key may be no number
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) {
+            const float4 w = *reinterpret_cast<const float4*>(vs + c * 32 + k);
+            const float wk[4] = {w.x, w.y, w.z, w.w};
+            float pj[4], y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              pj[j] = fast_exp2(__uint_as_float(v[c][k + j]) - m_use);
+              y[j] = __uint_as_float(v[c][k + j]) == NEG_BIG ? 0.f : pj[j] * wk[j];
+            }
+            s8[(k >> 1) & 2] = __fadd2_rn(s8[(k >> 1) & 2], make_float2(pj[0], pj[1]));
+            s8[((k >> 1) & 2) + 1] = __fadd2_rn(s8[((k >> 1) & 2) + 1], make_float2(pj[2], pj[3]));
+            v[c >> 1][(c & 1) * 16 + (k >> 1)] = pack_bf16(y[0], y[1]);
+            v[c >> 1][(c & 1) * 16 + (k >> 1) + 1] = pack_bf16(y[2], y[3]);
+          }
+      }
+      l += ((s8[0].x + s8[0].y) + (s8[1].x + s8[1].y)) + ((s8[2].x + s8[2].y) + (s8[3].x + s8[3].y));
+      // O of this tile is rescaled when a row of the warp raised its reference.  Its last product completed before these
+      // scores did, except where the tile runs alone: the product of i - 1 is waited for there.
+      if (__any_sync(0xffffffffu, rescale)) {
+        if (i > my_solo) {
+          ok = mbar_wait(pv_done, (i - 1 - my_solo) & 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tc_ld32(tmem_o + c * 32, v[2]);
+          tc_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            v[2][k] = __float_as_uint(__uint_as_float(v[2][k]) * (rescale ? factor : 1.0f));
+          tc_st32(tmem_o + c * 32, v[2]);
+        }
+      }
+      tc_st32(tmem_s, v[0]);          // probabilities over the scores they came from
+      tc_st32(tmem_s + 32, v[1]);
+      tc_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_full[buf]);
+    }
+    if (ok && jl[x] >= jf[x]) {
+      ok = mbar_wait(&o_final[x], 0);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      const long long row = (long long)(q_begin + tokx[x] + tl) * a.Hq + kvh * G + g;
+      if (ok && !whole[x]) {
+        // a partial result of this chunk: O as accumulated (against m_ref), m_ref, l
+        const long long at = row * a.max_chunks + chunk;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          unsigned o[32];
+          tc_ld32(tmem_o + c * 32, o);
+          tc_wait_ld();
+          if (valid) {
+#pragma unroll
+            for (int ch = 0; ch < 8; ++ch)
+              *reinterpret_cast<uint4*>(a.part_o + at * TILE + c * 32 + ch * 4) =
+                  make_uint4(o[ch * 4], o[ch * 4 + 1], o[ch * 4 + 2], o[ch * 4 + 3]);
+          }
+        }
+        if (valid) a.part_ml[at] = make_float2(m_ref, l);
+      } else if (ok) {
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          unsigned o[32];
+          tc_ld32(tmem_o + c * 32, o);
+          tc_wait_ld();
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch)
+            if (valid && c * 32 + ch * 8 < a.D)
+              *reinterpret_cast<uint4*>(out + row * a.D + c * 32 + ch * 8) =
+                  make_uint4(pack_bf16(__uint_as_float(o[ch * 8]) * inv, __uint_as_float(o[ch * 8 + 1]) * inv),
+                             pack_bf16(__uint_as_float(o[ch * 8 + 2]) * inv, __uint_as_float(o[ch * 8 + 3]) * inv),
+                             pack_bf16(__uint_as_float(o[ch * 8 + 4]) * inv, __uint_as_float(o[ch * 8 + 5]) * inv),
+                             pack_bf16(__uint_as_float(o[ch * 8 + 6]) * inv, __uint_as_float(o[ch * 8 + 7]) * inv));
+        }
+      }
+    }
+  }
+  if (!ok) atomicExch(&dib_attention_int8_prompt_error_word, 1);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+}
+
+// Rows whose keys span several chunks: out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c in chunk order, over the chunks of
+// the row's query tile.  A warp a (token, head), a lane four dimensions; rows that the attention finished cost a look at
+// their lengths.
+constexpr int MERGE_MAX = 16;
+__global__ void __launch_bounds__(256)
+attention_prompt_merge_kernel(__nv_bfloat16* __restrict__ out, const __grid_constant__ PromptArgs a,
+                              const int* __restrict__ seq_list) {
+  const float* part_o = a.part_o;
+  const float2* part_ml = a.part_ml;
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int seq = seq_list[blockIdx.y];
+  const int q_begin = a.cu_q_lens[seq], q_len = a.cu_q_lens[seq + 1] - q_begin;
+  const int id = blockIdx.x * 8 + (threadIdx.x >> 5), tok = id / a.Hq, h = id - tok * a.Hq;
+  pdl_wait(part_o, part_ml);
+  if (tok >= q_len) return;
+  const int kv_len = min(a.seq_lens[seq], (int)min((long long)a.max_blocks << a.page_shift, 0x7fffff00ll));
+  const int npt = TILE / (a.Hq / a.Hkv), tok0 = tok / npt * npt;
+  const int first_pos = kv_len - q_len + tok0, last_pos = first_pos + min(npt, q_len - tok0) - 1;
+  if (last_pos < 0) return;
+  const int c0 = first_visible_key(first_pos, a.window) / TILE / a.chunk_tiles, c1 = last_pos / TILE / a.chunk_tiles;
+  if (c0 >= c1) return;     // finished by the attention itself
+  const long long row = (long long)(q_begin + tok) * a.Hq + h;
+  float m[MERGE_MAX], l[MERGE_MAX], top = NEG_BIG;
+#pragma unroll
+  for (int c = 0; c < MERGE_MAX; ++c) {
+    m[c] = NEG_BIG;
+    l[c] = 0.f;
+    if (c0 + c <= c1) {
+      const float2 ml = part_ml[row * a.max_chunks + c0 + c];
+      m[c] = ml.x;
+      l[c] = ml.y;
+    }
+    top = fmaxf(top, m[c]);
+  }
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+#pragma unroll
+  for (int c = 0; c < MERGE_MAX; ++c) {
+    if (c0 + c > c1) break;
+    const float w = fast_exp2(m[c] - top);
+    const float4 v = *reinterpret_cast<const float4*>(part_o + (row * a.max_chunks + c0 + c) * TILE + lane * 4);
+    sum = fmaf(w, l[c], sum);
+    o.x = fmaf(w, v.x, o.x); o.y = fmaf(w, v.y, o.y); o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
+  }
+  if (lane * 4 >= a.D) return;
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  *reinterpret_cast<uint2*>(out + row * a.D + lane * 4) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+}
+
+// ---- host side
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled() {
+  static EncodeTiledFn fn = nullptr;
+  if (fn == nullptr) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) == cudaSuccess &&
+        r == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  }
+  return fn;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dib_attention_int8_prompt_status() {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, dib_attention_int8_prompt_error_word, sizeof(int)) != cudaSuccess) return -1;
+  return v;
+}
+int dib_attention_int8_prompt_status_clear() {
+  const int v = 0;
+  return cudaMemcpyToSymbol(dib_attention_int8_prompt_error_word, &v, sizeof(int)) == cudaSuccess ? 0 : -1;
+}
+
+// q, out bfloat16 [T, Hq, D], heads up to 128, up to 128 query heads a kv head, pages of a power of two of rows, 4 at least.
+// units int32 [4, count]: sequence, first tokens of A and B (128 / (Hq / Hkv) tokens each; -1: no B), chunk; the longest last.
+// chunk_tiles: 0, or the key tiles of a chunk: then part_o float32 [T, Hq, max_chunks, 128] and part_ml [.., 2] take partial
+// results (at most 16 chunks of a row), which are added up for the tokens of the seq_count sequences in seq_list
+// (max_tokens: the most of one).
+int dib_int8_attention_prompt(const void* q, void* out, const void* data, const void* scales, long long num_pages,
+                              const void* block_table, int max_blocks, const void* cu_q_lens, const void* seq_lens,
+                              const void* units, int count, const void* seq_list, int seq_count, int max_tokens, void* part_o,
+                              void* part_ml, int chunk_tiles, int max_chunks, int Hq, int Hkv, int D, int page_size,
+                              float scale, int window, cudaStream_t st) {
+  if (count < 0 || count > 65535 || seq_count < 0 || seq_count > 65535 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 ||
+      Hq / Hkv > TILE || D < 16 || D > 128 || D % 16 != 0 || page_size < 4 || (page_size & (page_size - 1)) != 0 ||
+      num_pages * 2 * Hkv * page_size >= (1ll << 31) || chunk_tiles < 0 || (chunk_tiles > 0 && max_chunks > MERGE_MAX))
+    return DIB_BAD_SIZE;
+  if (((reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(q) |
+        reinterpret_cast<uintptr_t>(out)) & 15) != 0)
+    return DIB_BAD_ALIGN;
+  if (count == 0) return DIB_OK;
+  PromptArgs a;
+  a.scales = reinterpret_cast<const float*>(scales);
+  a.block_table = reinterpret_cast<const int*>(block_table);
+  a.cu_q_lens = reinterpret_cast<const int*>(cu_q_lens);
+  a.seq_lens = reinterpret_cast<const int*>(seq_lens);
+  a.units = reinterpret_cast<const int*>(units);
+  a.count = count; a.max_blocks = max_blocks; a.Hq = Hq; a.Hkv = Hkv; a.D = D;
+  a.page_shift = 0;
+  while ((1 << a.page_shift) < page_size) ++a.page_shift;
+  a.num_pages = (int)num_pages;
+  a.window = window; a.chunk_tiles = chunk_tiles; a.max_chunks = max_chunks;
+  a.scale = scale;
+  a.part_o = reinterpret_cast<float*>(part_o);
+  a.part_ml = reinterpret_cast<float2*>(part_ml);
+  CUtensorMap map;
+  EncodeTiledFn enc = encode_tiled();
+  if (enc == nullptr) return DIB_LAUNCH_FAILED;
+  const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)(num_pages * 2 * Hkv * page_size)};
+  const cuuint64_t strides[1] = {(cuuint64_t)D};
+  const cuuint32_t box[2] = {128, (cuuint32_t)(page_size < TILE ? page_size : TILE)};
+  const cuuint32_t estr[2] = {1, 1};
+  if (enc(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(data), dims, strides, box, estr,
+          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return DIB_LAUNCH_FAILED;
+  static_assert(S_TOTAL + 512 <= S_DYNAMIC, "shared memory");
+  static DeviceOnce attr_set;
+  if (!attr_set.done()) {
+    if (cudaFuncSetAttribute(attention_prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S_DYNAMIC) != cudaSuccess)
+      return DIB_LAUNCH_FAILED;
+    attr_set.mark();
+  }
+  dib_launch(attention_prompt_kernel, dim3(Hkv, count), dim3(THREADS), S_DYNAMIC, st, map,
+             reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<__nv_bfloat16*>(out), a);
+  DIB_CHECK_LAUNCH();
+  if (chunk_tiles > 0) {
+    const long long blocks = ((long long)max_tokens * Hq + 7) / 8;
+    if (blocks > 0x7fffffffll) return DIB_BAD_SIZE;
+    dib_launch(attention_prompt_merge_kernel, dim3((unsigned)blocks, seq_count), dim3(256), 0, st,
+               reinterpret_cast<__nv_bfloat16*>(out), a, reinterpret_cast<const int*>(seq_list));
+    DIB_CHECK_LAUNCH();
+  }
+  return DIB_OK;
+}
+
+}  // extern "C"

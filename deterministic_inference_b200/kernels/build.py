@@ -51,6 +51,7 @@ SOURCES = {
     "gated_linear_attention": "gated_linear_attention.cu",
     "cache_int8": "cache_int8.cu",
     "attention_int8": "attention_int8.cu",
+    "attention_int8_prompt": "attention_int8_prompt.cu",
     "gemm_int8": "gemm_int8.cu",
 }
 HEADERS = ("common.cuh", "attention_merge.cuh")

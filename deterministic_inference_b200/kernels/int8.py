@@ -241,7 +241,8 @@ def int8_cache_read(cache: Int8Cache, slots: torch.Tensor, dtype: torch.dtype = 
     return k, v
 
 
-# ---- the split form's work: one launch for the sequences with one new token, one for those with more
+# ---- a step's work: one launch of the split form for the sequences with one new token, one for those with a few, one of the
+# prompt form for those with many
 
 def _pages_fit(page_size: int) -> bool:
     """Page sizes that the split form takes: a block of 32 keys is whole pages, or lies in one."""
@@ -277,16 +278,68 @@ class _SplitPart:
         self.merge = runs > 1
 
 
-def _split_parts(meta, group: int, hkv: int, wide: bool, device) -> list:
-    key = ("int8_split", group, hkv, wide)
+# Rows (new tokens x query heads of a kv head) of a sequence above which its bfloat16 tokens take the prompt form, whose
+# query tiles have 128 rows.
+PROMPT_ROWS = 64
+MAX_CHUNKS = 16        # chunks of 4,096 keys that the prompt form adds up for a row
+
+
+class _PromptPart:
+    """The sequences of the prompt form's launch: its list of query-tile pairs (and chunks of keys), longest last."""
+
+    def __init__(self, seqs: list, q_lens: list, kv_lens: list, group: int, hkv: int, window: int, device):
+        from . import attention_bf16
+        chosen = set(seqs)
+        new = [n if s in chosen else 0 for s, n in enumerate(q_lens)]
+        keys = [max(n, kv) for n, kv in zip(new, kv_lens)]
+        tokens = 128 // group
+        self.chunks = -(-max(keys[s] for s in seqs) // (attention_bf16.CHUNK_TILES * 128))
+        self.chunk_tiles = attention_bf16.CHUNK_TILES if self.chunks > 1 else 0
+        if self.chunks > 1:
+            seq, a, b, chunk = attention_bf16.extend_chunk_units(new, keys, 0, tokens, attention_bf16.CHUNK_TILES)
+        else:
+            # how tiles are paired depends on the step, the arithmetic of a tile does not (see ``extend_tile_pairs``)
+            ctas = (sum(-(-n // tokens) for n in new) + 1) // 2 * hkv
+            sms = attention_bf16._sm_count(device)
+            seq, a, b = attention_bf16.extend_tile_pairs(new, keys, 0, tokens, window, alone=2 * ctas <= sms,
+                                                         neighbours=ctas > sms)
+            chunk = [0] * len(seq)
+        self.count, self.seqs, self.max_tokens = len(seq), len(seqs), max(new)
+        lists = torch.tensor(seq + a + b + chunk + list(seqs), dtype=torch.int32).to(device, non_blocking=True)
+        self.units, self.seq_list = lists[:4 * self.count], lists[4 * self.count:]
+
+
+def _parts(meta, group: int, hkv: int, wide: bool, window: int, device) -> list:
+    """The step's launches: the sequences with one new token, those with a few, those with many (bfloat16)."""
+    key = ("int8", group, hkv, wide, window)
     parts = meta.scratch.get(key)
     if parts is None:
         q_lens, kv_lens = meta.q_lens, meta.kv_lens
         one = [s for s, n in enumerate(q_lens) if n == 1]
         more = [s for s, n in enumerate(q_lens) if n > 1]
-        parts = [_SplitPart(x, q_lens, kv_lens, group, hkv, wide, device) for x in (one, more) if x]
+        many = [s for s in more if not wide and q_lens[s] * group > PROMPT_ROWS and group <= 128
+                and kv_lens[s] <= MAX_CHUNKS * 4096]
+        few = [s for s in more if s not in set(many)]
+        parts = [_SplitPart(x, q_lens, kv_lens, group, hkv, wide, device) for x in (one, few) if x]
+        if many:
+            parts.append(_PromptPart(many, q_lens, kv_lens, group, hkv, window, device))
         meta.scratch[key] = parts
     return parts
+
+
+def _prompt(q, out, cache: Int8Cache, meta, part: _PromptPart, scale: float, window: int) -> None:
+    ops = _ops()
+    pages, _, hkv, page_size, d = cache.shape
+    t, hq, _ = q.shape
+    rows = t * hq * part.chunks if part.chunks > 1 else 0
+    partial = torch.empty(rows * 130, dtype=torch.float32, device=q.device)          # outputs, then (maximum, sum)
+    st = ops._lib("attention_int8_prompt").dib_int8_attention_prompt(
+        ops._ptr(q), ops._ptr(out), ops._ptr(cache.data), ops._ptr(cache.scales), c_longlong(pages),
+        ops._ptr(meta.block_table), c_int(meta.block_table.shape[1]), ops._ptr(meta.cu_q_lens), ops._ptr(meta.seq_lens),
+        ops._ptr(part.units), c_int(part.count), ops._ptr(part.seq_list), c_int(part.seqs), c_int(part.max_tokens),
+        ops._ptr(partial), ops._ptr(partial[rows * 128:]), c_int(part.chunk_tiles), c_int(part.chunks), c_int(hq), c_int(hkv),
+        c_int(d), c_int(page_size), c_float(scale), c_int(window), ops._stream())
+    ops._check(st, "int8_paged_attention", f"head_dim {d}, heads {hq}/{hkv}", kernels=2 if part.chunks > 1 else 1)
 
 
 def _split(q, out, cache: Int8Cache, meta, part: _SplitPart, scale: float, window: int) -> None:
@@ -331,8 +384,9 @@ def int8_paged_attention(q: torch.Tensor, cache: Int8Cache, meta, scale: float, 
     if t == 0:
         return out
     if d <= 128 and _pages_fit(page_size) and q.data_ptr() % 16 == 0 and cache.scales.data_ptr() % 16 == 0 and pages * 2 * hkv * page_size < 1 << 31:
-        for part in _split_parts(meta, hq // hkv, hkv, q.dtype == torch.float32, q.device):
-            _split(q, out, cache, meta, part, float(scale), win)
+        for part in _parts(meta, hq // hkv, hkv, q.dtype == torch.float32, win, q.device):
+            run = _prompt if isinstance(part, _PromptPart) else _split
+            run(q, out, cache, meta, part, float(scale), win)
         return out
     st = ops._lib("attention_int8").dib_int8_attention_any(
         ops._ptr(q), ops._ptr(out), ops._ptr(cache.data), ops._ptr(cache.scales), ops._ptr(meta.block_table),

@@ -110,6 +110,7 @@ _STATUS_FUNCTIONS = {
     "attention_bf16": ("dib_attention_bf16_status", "dib_attention_bf16_status_clear"),
     "attention_prefill_tc": ("dib_attention_prefill_tc_status", "dib_attention_prefill_tc_status_clear"),
     "attention_int8": ("dib_attention_int8_status", "dib_attention_int8_status_clear"),
+    "attention_int8_prompt": ("dib_attention_int8_prompt_status", "dib_attention_int8_prompt_status_clear"),
     "gemm_int8": ("dib_gemm_int8_status", "dib_gemm_int8_status_clear"),
 }
 _extra_status: dict = {}
