@@ -27,7 +27,7 @@ def _cmd_generate(a) -> int:
     if (a.model is None) == (a.preset is None):
         print("give exactly one of --model DIR or --preset NAME", file=sys.stderr)
         return 2
-    kw = dict(dtype=a.dtype, kv_pool_tokens=a.kv_pool_tokens, page_size=a.page_size,
+    kw = dict(dtype=a.dtype, weight_dtype=a.weight_dtype, cache_dtype=a.cache_dtype, kv_pool_tokens=a.kv_pool_tokens, page_size=a.page_size,
               max_reqs=a.max_reqs, max_seq_len=a.max_seq_len,
               max_prefill_tokens=a.max_prefill_tokens, max_decode_batch=a.max_decode_batch,
               cuda_graphs=not a.no_cuda_graphs, async_scheduling=not a.no_async_scheduling,
@@ -109,6 +109,8 @@ def main(argv=None) -> int:
     g.add_argument("--preset", help="a named shape with random weights instead of a folder")
     g.add_argument("--random-seed", type=int, default=0)
     g.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    g.add_argument("--weight-dtype", choices=["int8"], help="the layers' matrices in 8 bits")
+    g.add_argument("--cache-dtype", choices=["int8"], help="keys and values in 8 bits")
     g.add_argument("--prompt-ids", action="append", help='"1,2,3"; may be repeated')
     g.add_argument("--prompt-lens", help='"5,17,33": random prompts of these lengths')
     g.add_argument("--prompt-seed", type=int, default=1)

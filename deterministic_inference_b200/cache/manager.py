@@ -50,7 +50,8 @@ class CacheView:
 
     kv: Optional[torch.Tensor] = None            # [pages, 2, Hkv, page_size, D] of this cache; with
                                                  # values of another size than keys [pages, Hkv *
-                                                 # page_size * (D + Dv)]: a page's keys, then its values
+                                                 # page_size * (D + Dv)]: a page's keys, then its values;
+                                                 # in 8 bits an ``ops.Int8Cache``
     page_size: int = 0
     slot_mapping: Optional[torch.Tensor] = None  # int32 [T]: page * page_size + offset
     attention_meta: object = None                # the group's AttentionMeta of this step
@@ -78,7 +79,7 @@ class PageGroup:
         # per slot: the pages before this index (the kept first ones aside) have been given back, so the
         # next look starts there instead of walking the released run again every step
         self.first_live: list[int] = [0] * max_reqs
-        self.pool: Optional[torch.Tensor] = None
+        self.pool = None               # a tensor of all the group's caches; in 8 bits a list, one ``ops.Int8Cache`` each
 
     @property
     def num_free(self) -> int:
@@ -144,18 +145,21 @@ def _element_size(dtype: torch.dtype) -> int:
     return torch.empty(0, dtype=dtype).element_size()
 
 
+def _row_bytes(spec: PagedKVSpec, dtype: torch.dtype) -> int:
+    """Bytes of a token's key and value of one head (int8: with their float32 scales)."""
+    return (spec.head_dim + spec.value_dim) * _element_size(dtype) + (8 if dtype == torch.int8 else 0)
+
+
 def group_page_bytes(cache_specs: dict, page_size: int, dtype: torch.dtype) -> dict:
     """group key -> (spec, bytes of one page over all caches of the group), for the groups
-    of paged caches among ``cache_specs`` (cache id -> need)."""
+    of paged caches among ``cache_specs`` (cache id -> need); ``dtype`` is the pages'."""
     count: dict = {}
     specs: dict = {}
     for spec in flatten_cache_specs(cache_specs).values():
         if isinstance(spec, PagedKVSpec):
             count[spec.group_key()] = count.get(spec.group_key(), 0) + 1
             specs[spec.group_key()] = spec
-    item = _element_size(dtype)
-    return {k: (specs[k], n * specs[k].num_kv_heads * page_size
-                * (specs[k].head_dim + specs[k].value_dim) * item)
+    return {k: (specs[k], n * specs[k].num_kv_heads * page_size * _row_bytes(specs[k], dtype))
             for k, n in count.items()}
 
 
@@ -199,7 +203,8 @@ class CacheManager:
                  max_seq_len: int, dtype: torch.dtype = torch.bfloat16, device="cuda",
                  allocate_device: bool = True):
         """``num_pages``: pages of every group's pool (page 0 included), or a dict from
-        group key to the pages of that group (``pages_for_budget``)."""
+        group key to the pages of that group (``pages_for_budget``).  ``dtype``: the pages' type;
+        torch.int8: pools of ``ops.Int8Cache``."""
         self.page_size, self.max_reqs = int(page_size), int(max_reqs)
         self.max_seq_len = int(max_seq_len)
         self.max_blocks = -(-self.max_seq_len // self.page_size)
@@ -241,13 +246,18 @@ class CacheManager:
 
     def bytes_per_page(self) -> int:
         """Bytes of one page over all groups and caches (for sizing the pool)."""
-        item = _element_size(self.dtype)
-        return sum(len(g.cache_ids) * g.spec.num_kv_heads * g.page_size
-                   * (g.spec.head_dim + g.spec.value_dim) * item for g in self.page_groups.values())
+        return sum(len(g.cache_ids) * g.spec.num_kv_heads * g.page_size * _row_bytes(g.spec, self.dtype)
+                   for g in self.page_groups.values())
 
     def allocate_device_memory(self) -> None:
         for g in self.page_groups.values():
-            if g.spec.value_dim == g.spec.head_dim:
+            if self.dtype == torch.int8:
+                if g.spec.value_dim != g.spec.head_dim:
+                    raise CacheError(f"group {g.key}: values of another size than keys have no pages in 8 bits")
+                from ..kernels import ops
+                g.pool = [ops.Int8Cache.zeros(g.num_pages, g.spec.num_kv_heads, g.page_size, g.spec.head_dim, self.device)
+                          for _ in g.cache_ids]
+            elif g.spec.value_dim == g.spec.head_dim:
                 g.pool = torch.zeros(len(g.cache_ids), g.num_pages, 2, g.spec.num_kv_heads, g.page_size,
                                      g.spec.head_dim, dtype=self.dtype, device=self.device)
             else:     # a page: its keys [Hkv, page_size, D], then its values [Hkv, page_size, Dv]

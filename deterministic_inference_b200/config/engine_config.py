@@ -23,6 +23,13 @@ class EngineConfig:
 
     dtype: str = "bfloat16"              # "bfloat16" | "float32" (the true 32-bit path)
 
+    # "int8": the layers' matrices in 8 bits with a scale per output channel, activations quantised
+    # per token in front of every product, whose sums are exact integers (embedding and head stay in
+    # ``dtype``).  "int8" for the cache: keys and values in 8 bits with a scale per token and head;
+    # half the memory and half of what a decode step reads.  None: ``dtype``.
+    weight_dtype: Optional[str] = None
+    cache_dtype: Optional[str] = None
+
     # cache (sid/config.py:66-70)
     kv_pool_tokens: int = 256 * 1024     # tokens the page pool of each layer group holds
     # If set (0 < f <= 1): the pools are sized instead from the device memory that is free
@@ -66,6 +73,9 @@ class EngineConfig:
         if self.dtype not in _DTYPES:
             raise ValueError(f"dtype must be one of {sorted(set(_DTYPES))}, got {self.dtype!r}")
         self.dtype = _DTYPES[self.dtype]
+        for name in ("weight_dtype", "cache_dtype"):
+            if getattr(self, name) not in (None, "int8"):
+                raise ValueError(f"{name} must be None or 'int8', got {getattr(self, name)!r}")
         if self.model_path is None and self.model_config is None:
             raise ValueError("EngineConfig needs model_path (a folder) or model_config")
         if self.model_path is None and self.random_seed is None:

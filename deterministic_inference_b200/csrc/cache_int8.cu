@@ -77,6 +77,25 @@ template <> __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16*
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+template <typename T> __device__ __forceinline__ void load4(const T* p, float (&x)[4]);
+template <> __device__ __forceinline__ void load4<float>(const float* p, float (&x)[4]) {
+  const float4 v = *reinterpret_cast<const float4*>(p);
+  x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+}
+template <> __device__ __forceinline__ void load4<__nv_bfloat16>(const __nv_bfloat16* p, float (&x)[4]) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
+  x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
+}
+template <typename T> __device__ __forceinline__ void store4(T* p, const float (&x)[4]);
+template <> __device__ __forceinline__ void store4<float>(float* p, const float (&x)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+template <> __device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16* p, const float (&x)[4]) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+}
+
 constexpr int CACHE_THREADS = 256, ROW_LANES = 16;       // half a warp a row: 8 values a lane, twice for heads above 128
 
 // Row r = (token, key or value, kv head).  Memory bound: a row is read once into registers.
@@ -148,6 +167,100 @@ cache_read_kernel(const signed char* __restrict__ data, const float* __restrict_
     for (int j = 0; j < 8; ++j) x[j] = scale * (float)(signed char)((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
     store8<T>(dst + d, x);
   }
+}
+
+// The step's fused projection rows [q heads | k heads | v heads]: q and k normed (RMS) and rotated, q to its output, k and v
+// rounded to T, quantised and written to the token's slot; the norm's sum and the rotation are those of the kernels that
+// write an unquantised cache.  A warp a (token, head), a lane 4 consecutive elements of 128 at a time; the rotation's pairs
+// meet in shared memory.
+constexpr int QKV_WARPS = 4;
+template <typename T>
+__global__ void __launch_bounds__(QKV_WARPS * 32)
+qk_norm_rope_cache_int8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, signed char* __restrict__ data,
+                               float* __restrict__ scales, const float* __restrict__ q_norm_w,
+                               const float* __restrict__ k_norm_w, float eps, const float* __restrict__ cos_sin, int rotary_dim,
+                               int max_pos, const int* __restrict__ positions, const int* __restrict__ slots, int T_tokens,
+                               int Hq, int Hkv, int D, int page_size, long long num_pages) {
+  pdl_prologue(qkv, q_norm_w, k_norm_w);
+  __shared__ float row[QKV_WARPS][256];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = Hq + 2 * Hkv;
+  const long long item = (long long)blockIdx.x * QKV_WARPS + warp;
+  if (item >= (long long)T_tokens * heads) return;
+  const int t = (int)(item / heads), head = (int)(item - (long long)t * heads);
+  const bool is_q = head < Hq, is_k = !is_q && head < Hq + Hkv;
+  const float* nw = is_q ? q_norm_w : is_k ? k_norm_w : nullptr;
+  const int slot = is_q ? 0 : slots[t];
+  const long long page = slot < 0 ? -1 : slot / page_size;
+  if (!is_q && (page < 0 || page >= num_pages)) return;
+  const T* src = qkv + item * D;
+  float* s = row[warp];
+  float x[2][4], squares[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int d = i * 128 + lane * 4;
+    x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
+    if (d < D) load4<T>(src + d, x[i]);
+    squares[i] = sumsq4(x[i][0], x[i][1], x[i][2], x[i][3]);
+  }
+  if (nw != nullptr) {
+    float total = warp_sum(squares[0]);
+    if (D > 128) total = __fadd_rn(total, warp_sum(squares[1]));
+    const float rstd = rms_rstd(total, D, eps);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int d = i * 128 + lane * 4;
+      if (d < D)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][e] = norm_scale(x[i][e], rstd, nw[d + e]);
+    }
+  }
+  if (cos_sin != nullptr && (is_q || is_k)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int d = i * 128 + lane * 4;
+      if (d < D) *reinterpret_cast<float4*>(s + d) = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
+    }
+    __syncwarp();
+    int pos = positions[t];
+    pos = pos < 0 ? 0 : pos >= max_pos ? max_pos - 1 : pos;
+    const float* tab = cos_sin + (long long)pos * rotary_dim;
+    const int half = rotary_dim >> 1;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = i * 128 + lane * 4 + e;
+        if (d < half) x[i][e] = rope_first(x[i][e], s[d + half], tab[d], tab[half + d]);
+        else if (d < rotary_dim) x[i][e] = rope_second(s[d - half], x[i][e], tab[d - half], tab[d]);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[i][e] = round_to<T>(x[i][e]);
+  if (is_q) {
+    T* dst = q_out + ((long long)t * Hq + head) * D;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int d = i * 128 + lane * 4;
+      if (d < D) store4<T>(dst + d, x[i]);
+    }
+    return;
+  }
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = max(top, magnitude_bits(x[i][e]));
+  const RowScale scale = row_scale(__reduce_max_sync(0xffffffffu, top));
+  const int kv = !is_k, h = is_k ? head - Hq : head - Hq - Hkv;
+  const long long at = ((page * 2 + kv) * Hkv + h) * page_size + (slot - page * page_size);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int d = i * 128 + lane * 4;
+    if (d < D) *reinterpret_cast<unsigned*>(data + at * D + d) = pack4(x[i], scale.inv);
+  }
+  if (lane == 0) scales[at] = scale.scale;
 }
 
 // ---- rows of a matrix [M, K] (row stride `stride`) -> codes [M, Kp], Kp = K rounded up to 16 with zeros, scales [M].
@@ -250,6 +363,38 @@ int dib_int8_cache_write(const void* k, const void* v, long long k_stride, long 
     dib_launch(kern, dim3((unsigned)blocks), dim3(CACHE_THREADS), 0, st, reinterpret_cast<const float*>(k),
                reinterpret_cast<const float*>(v), k_stride, v_stride, d, s, sl, rows, Hkv, D, page_size, num_pages);
   }
+  DIB_CHECK_LAUNCH();
+  return DIB_OK;
+}
+
+// qkv [T, (Hq + 2 Hkv) D] -> q_out [T, Hq, D] and the cache; q_norm_w, k_norm_w float32 [D] or null; cos_sin float32
+// [max_pos, rotary_dim] = [cos | sin] or null; a token whose slot is none of the pool's keeps no key.
+int dib_int8_qk_norm_rope_cache(const void* qkv, void* q_out, void* data, void* scales, const void* q_norm_w,
+                                const void* k_norm_w, float eps, const void* cos_sin, int rotary_dim, int max_pos,
+                                const void* positions, const void* slots, int T, int Hq, int Hkv, int D, int page_size,
+                                long long num_pages, int dtype, cudaStream_t st) {
+  if (dtype != 0 && dtype != 1) return DIB_BAD_DTYPE;
+  if (T < 0 || Hq < 1 || Hkv < 1 || D < 16 || D > 256 || D % 16 != 0 || page_size < 1 || rotary_dim < 0 || rotary_dim > D ||
+      rotary_dim % 2 != 0 || (cos_sin != nullptr && max_pos < 1))
+    return DIB_BAD_SIZE;
+  if (((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(data)) & 15) != 0)
+    return DIB_BAD_ALIGN;
+  if (T == 0) return DIB_OK;
+  const long long blocks = ((long long)T * (Hq + 2 * Hkv) + QKV_WARPS - 1) / QKV_WARPS;
+  if (blocks > 0x7fffffffll) return DIB_BAD_SIZE;
+  const float *qw = reinterpret_cast<const float*>(q_norm_w), *kw = reinterpret_cast<const float*>(k_norm_w),
+              *tab = reinterpret_cast<const float*>(cos_sin);
+  const int *ps = reinterpret_cast<const int*>(positions), *sl = reinterpret_cast<const int*>(slots);
+  signed char* d = reinterpret_cast<signed char*>(data);
+  float* sc = reinterpret_cast<float*>(scales);
+  if (dtype == 1)
+    dib_launch(qk_norm_rope_cache_int8_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(QKV_WARPS * 32), 0, st,
+               reinterpret_cast<const __nv_bfloat16*>(qkv), reinterpret_cast<__nv_bfloat16*>(q_out), d, sc, qw, kw, eps, tab,
+               rotary_dim, max_pos, ps, sl, T, Hq, Hkv, D, page_size, num_pages);
+  else
+    dib_launch(qk_norm_rope_cache_int8_kernel<float>, dim3((unsigned)blocks), dim3(QKV_WARPS * 32), 0, st,
+               reinterpret_cast<const float*>(qkv), reinterpret_cast<float*>(q_out), d, sc, qw, kw, eps, tab, rotary_dim, max_pos,
+               ps, sl, T, Hq, Hkv, D, page_size, num_pages);
   DIB_CHECK_LAUNCH();
   return DIB_OK;
 }

@@ -49,6 +49,13 @@ class ModelRunner:
             else:
                 tensors = random_tensors_on_device(specs, cfg.random_seed, self.dtype, self.device)
             self.model.load(tensors)
+            if cfg.weight_dtype == "int8":
+                del tensors
+                self.model.quantize_weights()
+        cache_dtype = self.dtype
+        if cfg.cache_dtype == "int8":
+            self.model.check_int8_cache()
+            cache_dtype = torch.int8
         self.max_positions = self.model.plan.max_positions
         if self.dtype == torch.bfloat16 and self.device.type == "cuda":
             from ..kernels import gemm_bf16
@@ -59,12 +66,12 @@ class ModelRunner:
         if cfg.gpu_memory_fraction is not None and self.device.type == "cuda":
             free, _ = torch.cuda.mem_get_info(self.device)
             num_pages = pages_for_budget(self.model.cache_specs(), int(free * cfg.gpu_memory_fraction),
-                                         cfg.page_size, self.dtype, cfg.max_reqs + 1,
+                                         cfg.page_size, cache_dtype, cfg.max_reqs + 1,
                                          cfg.max_prefill_tokens)
         self.cache = CacheManager(self.model.cache_specs(), num_pages=num_pages,
                                   page_size=cfg.page_size, max_reqs=cfg.max_reqs + 1,
                                   max_seq_len=min(cfg.max_seq_len, self.max_positions),
-                                  dtype=self.dtype, device=self.device)
+                                  dtype=cache_dtype, device=self.device)
         self.steps_run = 0
         self.tokens_run = 0
         # pure-decode steps, and steps of any other shape that come again, are replayed as

@@ -12,6 +12,7 @@ in float32, whatever the row's type.  A row that holds an infinity or a NaN has 
 ``int8_linear``         y = x @ weight^T: an exact 32-bit sum of products of codes, times the two scales
 ``Int8Cache``           the cache of one layer: data int8 [pages, 2, Hkv, page_size, D], scales float32 [.., page_size]
 ``int8_cache_write``    keys and values into their slots
+``int8_qk_norm_rope_cache``  the same from the fused projection's rows, q and k normed and rotated on the way
 ``int8_cache_read``     what the rows of given slots stand for
 ``int8_paged_attention``  attention of a step's new tokens over the cache
 """
@@ -223,6 +224,42 @@ def int8_cache_write(k: torch.Tensor, v: torch.Tensor, cache: Int8Cache, slot_ma
         ops._ptr(slot_mapping), c_int(t), c_int(hkv), c_int(d), c_int(page_size), c_longlong(pages), c_int(ops._dt(k, "k")),
         ops._stream())
     ops._check(st, "int8_cache_write", f"heads {hkv} x {d}")
+
+
+def int8_qk_norm_rope_cache(qkv, num_heads: int, num_kv_heads: int, head_dim: int, q_norm_weight, k_norm_weight, eps: float,
+                            cos_sin, positions: torch.Tensor, cache: Int8Cache, slot_mapping: torch.Tensor) -> torch.Tensor:
+    """``ops.qk_norm_rope_cache`` with an 8-bit cache: q [T, Hq, D] normed and rotated; k, treated alike, and v are rounded to
+    the activations' type, quantised and written to the tokens' slots."""
+    ops = _ops()
+    qkv = ops.as_tensor(qkv)
+    ops._need(qkv, "qkv", None, 2)
+    t, width = qkv.shape
+    pages, _, hkv, page_size, d = cache.shape
+    if (hkv, d) != (num_kv_heads, head_dim) or width != (num_heads + 2 * hkv) * d:
+        raise ops.KernelError(f"int8_qk_norm_rope_cache: rows of {width} for heads {num_heads}/{num_kv_heads} x {head_dim}, "
+                              f"cache {tuple(cache.shape)}")
+    for x, name in ((positions, "positions"), (slot_mapping, "slot_mapping")):
+        ops._need(x, name, torch.int32, 1)
+        if x.shape[0] < t:
+            raise ops.KernelError(f"int8_qk_norm_rope_cache: {x.shape[0]} {name} for {t} tokens")
+    for w, name in ((q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight")):
+        if w is not None:
+            ops._need(w, name, torch.float32, 1)
+            if w.shape[0] != d:
+                raise ops.KernelError(f"{name} has {w.shape[0]} elements, head_dim is {d}")
+    rotary_dim, max_pos = 0, 0
+    if cos_sin is not None:
+        ops._need(cos_sin, "cos_sin", torch.float32, 2)
+        max_pos, rotary_dim = cos_sin.shape
+    _same_device("int8_qk_norm_rope_cache", qkv, cache.data, positions, slot_mapping)
+    q = torch.empty(t, num_heads, d, dtype=qkv.dtype, device=qkv.device)
+    st = ops._lib("cache_int8").dib_int8_qk_norm_rope_cache(
+        ops._ptr(qkv), ops._ptr(q), ops._ptr(cache.data), ops._ptr(cache.scales), ops._ptr(q_norm_weight),
+        ops._ptr(k_norm_weight), c_float(eps), ops._ptr(cos_sin), c_int(rotary_dim), c_int(max_pos), ops._ptr(positions),
+        ops._ptr(slot_mapping), c_int(t), c_int(num_heads), c_int(hkv), c_int(d), c_int(page_size), c_longlong(pages),
+        c_int(ops._dt(qkv, "qkv")), ops._stream())
+    ops._check(st, "int8_qk_norm_rope_cache", f"head_dim {d}, rotary_dim {rotary_dim}")
+    return q
 
 
 def int8_cache_read(cache: Int8Cache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16):

@@ -569,7 +569,11 @@ def qk_norm_rope_cache(qkv: torch.Tensor, num_heads: int, num_kv_heads: int, hea
     given), q to the returned tensor [T, Hq, D], k and v into the token's slot of
     the paged cache [pages, 2, Hkv, page_size, D] (when a cache is given;
     slot = page * page_size + offset, negative = skip).  ``cos_sin``, ``positions`` and ``slot_mapping`` are the
-    step's constants: no kernel of this package that is still running when this one is launched may write them."""
+    step's constants: no kernel of this package that is still running when this one is launched may write them.
+    ``kv_cache`` may be an ``Int8Cache``: ``int8_qk_norm_rope_cache``."""
+    if isinstance(kv_cache, Int8Cache):
+        return int8_qk_norm_rope_cache(qkv, num_heads, num_kv_heads, head_dim, q_norm_weight, k_norm_weight, eps, cos_sin,
+                                       positions, kv_cache, slot_mapping)
     parts = None
     if isinstance(qkv, SplitSum):
         if head_dim in (64, 128, 256) and (cos_sin is None or cos_sin.shape[1] == head_dim):
@@ -630,7 +634,7 @@ def qkv_project(x: torch.Tensor, w_qkv: torch.Tensor, num_heads: int, num_kv_hea
     the two kernels."""
     x = as_tensor(x)
     if x.dtype == torch.bfloat16 and x.is_cuda and head_dim == 128 and kv_cache is not None \
-            and (cos_sin is None or cos_sin.shape[1] == head_dim):
+            and not isinstance(kv_cache, Int8Cache) and not isinstance(w_qkv, Int8Weight) and (cos_sin is None or cos_sin.shape[1] == head_dim):
         from . import gemm_bf16
         q = gemm_bf16.qkv_large(x, w_qkv, num_heads, num_kv_heads, q_norm_weight, k_norm_weight, eps,
                                 cos_sin, positions, kv_cache, slot_mapping, page_size)
@@ -2090,4 +2094,4 @@ def masked_attention(q: torch.Tensor, kv_cache: torch.Tensor, meta, scale: float
 # ---------------------------------------------------------------- 8-bit integers
 
 from .int8 import (Int8Cache, Int8Rows, Int8Weight, int8_cache_read, int8_cache_write, int8_linear,  # noqa: E402,F401
-                   int8_paged_attention, quantize_rows)
+                   int8_paged_attention, int8_qk_norm_rope_cache, quantize_rows)

@@ -22,6 +22,9 @@ from .spec import PagedKVSpec, PartSpec, TensorSpec
 
 @register_mixer("gqa_attention")
 class GQAAttention(Mixer):
+    int8_weights = ("w_qkv", "w_o")
+    int8_cache = True
+
     def __init__(self, ctx, prefix: str, hidden_size: int, num_heads: int, num_kv_heads: int,
                  head_dim: int, scale: float, position_encoding: PartSpec,
                  qk_norm_eps: Optional[float] = None, window: Optional[int] = None):

@@ -36,12 +36,20 @@ from .spec import TensorSpec
 
 class Part:
     kind = "?"
+    # attributes that hold a weight [out, in] whose products may run in 8-bit integers
+    int8_weights: tuple = ()
 
     def tensor_specs(self) -> list[TensorSpec]:
         return []
 
     def load(self, tensors: dict[str, torch.Tensor]) -> None:
         pass
+
+    def quantize_weights(self) -> None:
+        """After ``load``: the weights named in ``int8_weights`` in 8 bits."""
+        from ..kernels import ops
+        for name in self.int8_weights:
+            setattr(self, name, ops.Int8Weight.of(getattr(self, name)))
 
 
 class TokenEmbedding(Part):
@@ -80,6 +88,8 @@ class PositionEncoding(Part):
 
 
 class Mixer(Part):
+    int8_cache = False       # whether it takes its pages as an ``ops.Int8Cache``
+
     def cache_spec(self):
         return None
 

@@ -19,6 +19,8 @@ class GatedMLP(FeedForward):
     accumulator where it is at hand.  ``names``: the checkpoint names of gate, up and down after the
     prefix."""
 
+    int8_weights = ("w_gate_up", "w_down")
+
     def __init__(self, ctx, prefix: str, hidden_size: int, intermediate_size: int,
                  activation: str = "silu", limit: float = None, alpha: float = 1.702, names=None):
         if activation not in ("silu", "limited_swish"):

@@ -1,0 +1,59 @@
+"""What serving in 8 bits settles on the host: options, page sizes in bytes, the work lists, refusals without a GPU."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from deterministic_inference_b200 import EngineConfig, preset
+from deterministic_inference_b200.cache.manager import CacheManager, group_page_bytes
+from deterministic_inference_b200.kernels import int8, ops
+from deterministic_inference_b200.parts.spec import PagedKVSpec
+
+
+def test_options():
+    ok = EngineConfig(model_config=preset("tiny_a"), random_seed=0, weight_dtype="int8", cache_dtype="int8")
+    assert ok.weight_dtype == ok.cache_dtype == "int8"
+    for name in ("weight_dtype", "cache_dtype"):
+        with pytest.raises(ValueError, match=name):
+            EngineConfig(model_config=preset("tiny_a"), random_seed=0, **{name: "fp8"})
+
+
+def test_page_bytes():
+    specs = {0: PagedKVSpec(8, 128), 1: PagedKVSpec(8, 128)}
+    (_, wide), = group_page_bytes(specs, 16, torch.bfloat16).values()
+    (_, narrow), = group_page_bytes(specs, 16, torch.int8).values()
+    assert wide == 2 * 8 * 16 * 512 and narrow == 2 * 8 * 16 * (256 + 8)
+    manager = CacheManager(specs, 4, 16, 2, 64, dtype=torch.int8, device="cpu", allocate_device=False)
+    assert manager.bytes_per_page() == narrow
+
+
+def test_there_is_no_cpu_path():
+    x = torch.zeros(2, 64)
+    for call in (lambda: ops.quantize_rows(x), lambda: ops.Int8Weight.of(x),
+                 lambda: ops.Int8Weight(x.to(torch.int8), torch.ones(2)), lambda: ops.Int8Cache.zeros(2, 1, 16, 64, device="cpu")):
+        with pytest.raises(ops.KernelError, match="CUDA"):
+            call()
+
+
+def test_prompt_units_cover_every_token_once():
+    """Every token of a sequence of the prompt form is in one query tile, with the chunks of keys up to its own position."""
+    for q_lens, kv_lens in (([1, 3, 200, 70, 500], [9, 50, 200, 4500, 9000]), ([130, 129], [130, 700])):
+        many = [s for s, n in enumerate(q_lens) if n * 2 > int8.PROMPT_ROWS]
+        part = int8._PromptPart.__new__(int8._PromptPart)
+        from deterministic_inference_b200.kernels import attention_bf16
+        attention_bf16._sms[torch.device("cpu")] = 148
+        part.__init__(many, q_lens, kv_lens, 2, 8, 0, torch.device("cpu"))
+        seq, a, b, chunk = part.units.view(4, part.count).tolist()
+        seen = {}
+        for s, t0, t1, c in zip(seq, a, b, chunk):
+            for t in (t0, t1):
+                if t >= 0:
+                    for tok in range(t, min(t + 64, q_lens[s])):
+                        assert (s, tok, c) not in seen
+                        seen[s, tok, c] = True
+        for s in many:
+            for tok in range(q_lens[s]):
+                last = (kv_lens[s] - q_lens[s] + tok) // 4096 if part.chunk_tiles else 0
+                assert all((s, tok, c) in seen for c in range(last + 1))
+        assert part.seq_list.tolist() == many and part.max_tokens == max(q_lens[s] for s in many)
