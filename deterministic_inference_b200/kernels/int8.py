@@ -19,7 +19,8 @@ in float32, whatever the row's type.  A row that holds an infinity or a NaN has 
 
 from __future__ import annotations
 
-from ctypes import c_float, c_int, c_longlong
+import ctypes
+from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import torch
 
@@ -27,14 +28,76 @@ MAX_K = 133144          # 127^2 * K stays below 2^31
 MAX_HEAD_DIM = 256
 
 
+# A decoded token's operators take the GPU a few microseconds: what the host does in front of a launch is kept short.  The C
+# functions are looked up once, with their argument types (pointers and numbers are passed as Python integers); an argument
+# is looked at in one expression, and the check that words the error runs only where that fails.
+_P, _I, _L, _F = c_void_p, c_int, c_longlong, c_float
+_SIGNATURES = {
+    "dib_quantize_rows": ("cache_int8", (_P, _L, _P, _P, _L, _I, _I, _I, _P)),
+    "dib_int8_cache_write": ("cache_int8", (_P, _P, _L, _L, _P, _P, _P, _I, _I, _I, _I, _L, _I, _P)),
+    "dib_int8_cache_read": ("cache_int8", (_P, _P, _P, _P, _P, _I, _I, _I, _I, _L, _I, _P)),
+    "dib_int8_qk_norm_rope_cache": ("cache_int8", (_P, _P, _P, _P, _P, _P, _F, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _L, _I, _P)),
+    "dib_gemm_int8": ("gemm_int8", (_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P)),
+    "dib_int8_linear": ("gemm_int8", (_P, _P, _L, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P)),
+    "dib_int8_attention_split": ("attention_int8", (_P, _P, _P, _P, _L, _P, _I, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _I, _I,
+                                                    _I, _I, _F, _I, _I, _I, _P)),
+    "dib_int8_attention_any": ("attention_int8", (_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _P)),
+    "dib_int8_attention_prompt": ("attention_int8_prompt", (_P, _P, _P, _P, _L, _P, _I, _P, _P, _P, _I, _P, _I, _I, _P, _P, _I, _I,
+                                                            _I, _I, _I, _I, _F, _I, _P)),
+}
+_functions: dict = {}
+_ops_module = None
+
+
 def _ops():
-    from . import ops
-    return ops
+    global _ops_module
+    if _ops_module is None:
+        from . import ops
+        _ops_module = ops
+    return _ops_module
 
 
-def _same_device(what: str, *tensors) -> None:
-    if len({t.device for t in tensors}) > 1:
-        raise _ops().KernelError(f"{what}: tensors on different devices ({sorted({str(t.device) for t in tensors})})")
+def _fn(name: str):
+    fn = _functions.get(name)
+    if fn is None:
+        library, types = _SIGNATURES[name]
+        fn = getattr(_ops()._lib(library), name)
+        fn.argtypes, fn.restype = types, c_int
+        _functions[name] = fn
+    return fn
+
+
+def _stream() -> int:
+    raw = _ops()._raw_stream
+    return raw(torch.cuda.current_device()) if raw is not None else torch.cuda.current_stream().cuda_stream
+
+
+def _done(status: int, what: str, detail, kernels: int = 1) -> None:
+    """``detail``: called for the error's text."""
+    if status == 0:
+        _ops()._launched(kernels)
+    else:
+        _ops()._check(status, what, detail(), kernels)
+
+
+def _require(t, name: str, dtype, ndim: int) -> None:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.dim() == ndim and t.is_contiguous()):
+        _ops()._need(t, name, dtype, ndim)
+
+
+def _code(dtype, name: str) -> int:
+    code = _ops()._DT.get(dtype)
+    if code is None:
+        raise _ops().KernelError(f"{name}: dtype {dtype} is not supported (float32 or bfloat16)")
+    return code
+
+
+def _same_device(what: str, first, *others) -> None:
+    device = first.device
+    for t in others:
+        if t.device != device:
+            raise _ops().KernelError(f"{what}: tensors on different devices "
+                                     f"({sorted({str(x.device) for x in (first, *others)})})")
 
 
 def _padded(k: int) -> int:
@@ -105,21 +168,26 @@ class Int8Weight:
         return self.codes[:, :self.k].float() * self.scales[:, None]
 
 
-def _quantize(x: torch.Tensor, name: str, early: bool) -> Int8Rows:
+def _check_rows(x, name: str) -> int:
+    """The type's code of a matrix whose rows are consecutive values, at any distance from one another."""
     ops = _ops()
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ops.KernelError(f"{name} must be a CUDA tensor: this package has no CPU path")
     if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
         raise ops.KernelError(f"{name} must be rows of consecutive values (shape {tuple(x.shape)}, stride {x.stride()})")
+    if not 1 <= x.shape[1] <= MAX_K:
+        raise ops.KernelError(f"{name} has rows of {x.shape[1]} values (1 to {MAX_K})")
+    return _code(x.dtype, name)
+
+
+def _quantize(x: torch.Tensor, name: str, early: bool) -> Int8Rows:
+    code = _check_rows(x, name)
     m, k = x.shape
-    if k < 1 or k > MAX_K:
-        raise ops.KernelError(f"{name} has rows of {k} values (1 to {MAX_K})")
     codes = torch.empty(m, _padded(k), dtype=torch.int8, device=x.device)
     scales = torch.empty(m, dtype=torch.float32, device=x.device)
-    st = ops._lib("cache_int8").dib_quantize_rows(
-        ops._ptr(x), c_longlong(x.stride(0)), ops._ptr(codes), ops._ptr(scales), c_longlong(m), c_int(k),
-        c_int(ops._dt(x, name)), c_int(1 if early else 0), ops._stream())
-    ops._check(st, "quantize_rows", f"rows {m} x {k}")
+    st = _fn("dib_quantize_rows")(x.data_ptr(), x.stride(0), codes.data_ptr(), scales.data_ptr(), m, k, code,
+                                  1 if early else 0, _stream())
+    _done(st, "quantize_rows", lambda: f"rows {m} x {k}")
     return Int8Rows(codes, scales, k, x.dtype)
 
 
@@ -132,24 +200,43 @@ def int8_linear(x, weight: Int8Weight, out_dtype=None) -> torch.Tensor:
     """y = x @ weight^T, [M, N]: ``x`` [M, K] is quantised row by row (or is an ``Int8Rows``); the sum of the codes'
     products is exact in 32 bits, so a row's bits depend on the row and the weight alone; times the token's and the
     channel's scale in float32, rounded once to ``out_dtype`` (float32 or bfloat16; x's type if not given)."""
-    ops = _ops()
     if not isinstance(weight, Int8Weight):
-        raise ops.KernelError("int8_linear: weight must be an Int8Weight")
-    if not isinstance(x, Int8Rows):
-        x = ops.as_tensor(x)
-        if x.dim() == 2 and x.shape[1] != weight.k:
-            raise ops.KernelError(f"int8_linear: x {tuple(x.shape)} against weight {tuple(weight.shape)}")
-        x = quantize_rows(x)
-    if x.k != weight.k:
-        raise ops.KernelError(f"int8_linear: x {tuple(x.shape)} against weight {tuple(weight.shape)}")
-    _same_device("int8_linear", x.codes, weight.codes)
-    m, n = x.codes.shape[0], weight.codes.shape[0]
-    out = torch.empty(m, n, dtype=out_dtype or x.dtype, device=x.device)
-    st = ops._lib("gemm_int8").dib_gemm_int8(
-        ops._ptr(x.codes), ops._ptr(x.scales), ops._ptr(weight.codes), ops._ptr(weight.scales), ops._ptr(out), c_int(m),
-        c_int(n), c_int(x.codes.shape[1]), c_int(ops._dt(out, "out")), c_int(_sms(x.device)), ops._stream())
-    ops._check(st, "int8_linear", f"M={m} N={n} K={x.k}")
+        raise _ops().KernelError("int8_linear: weight must be an Int8Weight")
+    rows = isinstance(x, Int8Rows)
+    if not rows:
+        if not isinstance(x, torch.Tensor):
+            x = _ops().as_tensor(x)
+        code = _check_rows(x, "x")
+    m, k = x.shape
+    if k != weight.k:
+        raise _ops().KernelError(f"int8_linear: x {tuple(x.shape)} against weight {tuple(weight.shape)}")
+    device = weight.codes.device
+    if x.device != device:
+        _same_device("int8_linear", x, weight)
+    n = weight.codes.shape[0]
+    out_dtype = out_dtype or x.dtype
+    out_code = _code(out_dtype, "out")
+    out = torch.empty(m, n, dtype=out_dtype, device=device)
+    if rows:
+        st = _fn("dib_gemm_int8")(x.codes.data_ptr(), x.scales.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(),
+                                  out.data_ptr(), m, n, x.codes.shape[1], out_code, _sms(device), _stream())
+    else:
+        work = torch.empty(m * (_padded(k) + 4), dtype=torch.int8, device=device)      # codes, then scales
+        st = _fn("dib_int8_linear")(_address("dib_quantize_rows"), x.data_ptr(), x.stride(0), code, k, work.data_ptr(),
+                                    weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(), m, n, out_code,
+                                    _sms(device), _stream())
+    _done(st, "int8_linear", lambda: f"M={m} N={n} K={k}", 1 if rows else 2)
     return out
+
+
+_addresses: dict = {}
+
+
+def _address(name: str) -> int:
+    got = _addresses.get(name)
+    if got is None:
+        got = _addresses[name] = ctypes.cast(_fn(name), c_void_p).value
+    return got
 
 
 def force_product_form(form: int) -> None:
@@ -158,9 +245,14 @@ def force_product_form(form: int) -> None:
     _ops()._lib("gemm_int8").dib_gemm_int8_force_form(c_int(form))
 
 
+_sm_counts: dict = {}
+
+
 def _sms(device) -> int:
-    from . import gemm_bf16
-    return gemm_bf16._sms(device)
+    n = _sm_counts.get(device)
+    if n is None:
+        n = _sm_counts[device] = torch.cuda.get_device_properties(device).multi_processor_count
+    return n
 
 
 class Int8Cache:
@@ -195,35 +287,34 @@ class Int8Cache:
         return self.data.device
 
 
-def _row_stride(x: torch.Tensor, name: str, hkv: int, d: int) -> int:
+def _row_stride(x, name: str, hkv: int, d: int) -> int:
     """Distance of a token's rows [Hkv, D], which lie together (a column range of a fused projection, say)."""
     ops = _ops()
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ops.KernelError(f"{name} must be a CUDA tensor: this package has no CPU path")
-    if x.dim() != 3 or tuple(x.shape[1:]) != (hkv, d):
+    if x.dim() != 3 or x.shape[1] != hkv or x.shape[2] != d:
         raise ops.KernelError(f"{name} has shape {tuple(x.shape)}, the cache's heads are [{hkv}, {d}]")
-    if x.stride(2) != 1 or (hkv > 1 and x.stride(1) != d):
-        raise ops.KernelError(f"{name}: a token's heads must lie together (stride {x.stride()})")
-    return x.stride(0) if x.shape[0] > 1 else hkv * d
+    stride = x.stride()
+    if stride[2] != 1 or (hkv > 1 and stride[1] != d):
+        raise ops.KernelError(f"{name}: a token's heads must lie together (stride {stride})")
+    return stride[0]
 
 
 def int8_cache_write(k: torch.Tensor, v: torch.Tensor, cache: Int8Cache, slot_mapping: torch.Tensor) -> None:
     """k, v [T, Hkv, D] (float32 or bfloat16; column ranges of wider rows too) into the rows ``slot_mapping`` (int32 [T],
     page * page_size + offset) of the cache; a negative slot is skipped.  Slots are distinct."""
-    ops = _ops()
-    pages, _, hkv, page_size, d = cache.shape
+    data = cache.data
+    pages, _, hkv, page_size, d = data.shape
     ks, vs = _row_stride(k, "k", hkv, d), _row_stride(v, "v", hkv, d)
-    ops._need(slot_mapping, "slot_mapping", torch.int32, 1)
+    _require(slot_mapping, "slot_mapping", torch.int32, 1)
     t = k.shape[0]
-    if v.shape[0] != t or v.dtype != k.dtype or slot_mapping.shape[0] < t:
-        raise ops.KernelError(f"int8_cache_write: k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}, "
-                              f"{slot_mapping.shape[0]} slots")
-    _same_device("int8_cache_write", k, v, cache.data, slot_mapping)
-    st = ops._lib("cache_int8").dib_int8_cache_write(
-        ops._ptr(k), ops._ptr(v), c_longlong(ks), c_longlong(vs), ops._ptr(cache.data), ops._ptr(cache.scales),
-        ops._ptr(slot_mapping), c_int(t), c_int(hkv), c_int(d), c_int(page_size), c_longlong(pages), c_int(ops._dt(k, "k")),
-        ops._stream())
-    ops._check(st, "int8_cache_write", f"heads {hkv} x {d}")
+    if v.shape[0] != t or v.dtype is not k.dtype or slot_mapping.shape[0] < t:
+        raise _ops().KernelError(f"int8_cache_write: k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}, "
+                                 f"{slot_mapping.shape[0]} slots")
+    _same_device("int8_cache_write", data, k, v, slot_mapping)
+    st = _fn("dib_int8_cache_write")(k.data_ptr(), v.data_ptr(), ks, vs, data.data_ptr(), cache.scales.data_ptr(),
+                                     slot_mapping.data_ptr(), t, hkv, d, page_size, pages, _code(k.dtype, "k"), _stream())
+    _done(st, "int8_cache_write", lambda: f"heads {hkv} x {d}")
 
 
 def int8_qk_norm_rope_cache(qkv, num_heads: int, num_kv_heads: int, head_dim: int, q_norm_weight, k_norm_weight, eps: float,
@@ -253,28 +344,31 @@ def int8_qk_norm_rope_cache(qkv, num_heads: int, num_kv_heads: int, head_dim: in
         max_pos, rotary_dim = cos_sin.shape
     _same_device("int8_qk_norm_rope_cache", qkv, cache.data, positions, slot_mapping)
     q = torch.empty(t, num_heads, d, dtype=qkv.dtype, device=qkv.device)
-    st = ops._lib("cache_int8").dib_int8_qk_norm_rope_cache(
-        ops._ptr(qkv), ops._ptr(q), ops._ptr(cache.data), ops._ptr(cache.scales), ops._ptr(q_norm_weight),
-        ops._ptr(k_norm_weight), c_float(eps), ops._ptr(cos_sin), c_int(rotary_dim), c_int(max_pos), ops._ptr(positions),
-        ops._ptr(slot_mapping), c_int(t), c_int(num_heads), c_int(hkv), c_int(d), c_int(page_size), c_longlong(pages),
-        c_int(ops._dt(qkv, "qkv")), ops._stream())
-    ops._check(st, "int8_qk_norm_rope_cache", f"head_dim {d}, rotary_dim {rotary_dim}")
+    st = _fn("dib_int8_qk_norm_rope_cache")(
+        qkv.data_ptr(), q.data_ptr(), cache.data.data_ptr(), cache.scales.data_ptr(), _pointer(q_norm_weight),
+        _pointer(k_norm_weight), float(eps), _pointer(cos_sin), rotary_dim, max_pos, positions.data_ptr(),
+        slot_mapping.data_ptr(), t, num_heads, hkv, d, page_size, pages, _code(qkv.dtype, "qkv"), _stream())
+    _done(st, "int8_qk_norm_rope_cache", lambda: f"head_dim {d}, rotary_dim {rotary_dim}")
     return q
+
+
+def _pointer(t) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def int8_cache_read(cache: Int8Cache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
     """(k, v) [T, Hkv, D] in ``dtype``: what the rows ``slots`` (int32 [T]) of the cache stand for; zeros for a negative
     slot."""
-    ops = _ops()
-    pages, _, hkv, page_size, d = cache.shape
-    ops._need(slots, "slots", torch.int32, 1)
-    _same_device("int8_cache_read", cache.data, slots)
-    k = torch.empty(slots.shape[0], hkv, d, dtype=dtype, device=cache.device)
-    v = torch.empty_like(k)
-    st = ops._lib("cache_int8").dib_int8_cache_read(
-        ops._ptr(cache.data), ops._ptr(cache.scales), ops._ptr(slots), ops._ptr(k), ops._ptr(v), c_int(slots.shape[0]),
-        c_int(hkv), c_int(d), c_int(page_size), c_longlong(pages), c_int(ops._dt(k, "out")), ops._stream())
-    ops._check(st, "int8_cache_read", f"heads {hkv} x {d}")
+    data = cache.data
+    pages, _, hkv, page_size, d = data.shape
+    _require(slots, "slots", torch.int32, 1)
+    _same_device("int8_cache_read", data, slots)
+    code = _code(dtype, "out")
+    t = slots.shape[0]
+    k, v = torch.empty(2, t, hkv, d, dtype=dtype, device=data.device).unbind(0)
+    st = _fn("dib_int8_cache_read")(data.data_ptr(), cache.scales.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), t,
+                                    hkv, d, page_size, pages, code, _stream())
+    _done(st, "int8_cache_read", lambda: f"heads {hkv} x {d}")
     return k, v
 
 
@@ -312,7 +406,9 @@ class _SplitPart:
         tiles, per32 = -(-self.max_rows // self.tile_rows), 32 // self.tile_rows
         # (runs get longer with the rows: tiles * runs is largest at 64 rows, or the tiles' own number is)
         self.items = hkv * min(tiles * runs, max(2 * per32 * runs, per32 * (runs + 1) + tiles))
-        self.merge = runs > 1
+        # (rows of partial results: none where every sequence has one run)
+        self.rows = count * self.items * self.tile_rows if runs > 1 else 0
+        self.list_pointer = _pointer(self.list)
 
 
 # Rows (new tokens x query heads of a kv head) of a sequence above which its bfloat16 tokens take the prompt form, whose
@@ -337,7 +433,7 @@ class _PromptPart:
         else:
             # how tiles are paired depends on the step, the arithmetic of a tile does not (see ``extend_tile_pairs``)
             ctas = (sum(-(-n // tokens) for n in new) + 1) // 2 * hkv
-            sms = attention_bf16._sm_count(device)
+            sms = _sms(device)
             seq, a, b = attention_bf16.extend_tile_pairs(new, keys, 0, tokens, window, alone=2 * ctas <= sms,
                                                          neighbours=ctas > sms)
             chunk = [0] * len(seq)
@@ -365,33 +461,31 @@ def _parts(meta, group: int, hkv: int, wide: bool, window: int, device) -> list:
 
 
 def _prompt(q, out, cache: Int8Cache, meta, part: _PromptPart, scale: float, window: int) -> None:
-    ops = _ops()
-    pages, _, hkv, page_size, d = cache.shape
+    pages, _, hkv, page_size, d = cache.data.shape
     t, hq, _ = q.shape
     rows = t * hq * part.chunks if part.chunks > 1 else 0
-    partial = torch.empty(rows * 130, dtype=torch.float32, device=q.device)          # outputs, then (maximum, sum)
-    st = ops._lib("attention_int8_prompt").dib_int8_attention_prompt(
-        ops._ptr(q), ops._ptr(out), ops._ptr(cache.data), ops._ptr(cache.scales), c_longlong(pages),
-        ops._ptr(meta.block_table), c_int(meta.block_table.shape[1]), ops._ptr(meta.cu_q_lens), ops._ptr(meta.seq_lens),
-        ops._ptr(part.units), c_int(part.count), ops._ptr(part.seq_list), c_int(part.seqs), c_int(part.max_tokens),
-        ops._ptr(partial), ops._ptr(partial[rows * 128:]), c_int(part.chunk_tiles), c_int(part.chunks), c_int(hq), c_int(hkv),
-        c_int(d), c_int(page_size), c_float(scale), c_int(window), ops._stream())
-    ops._check(st, "int8_paged_attention", f"head_dim {d}, heads {hq}/{hkv}", kernels=2 if part.chunks > 1 else 1)
+    held = torch.empty(rows * 130, dtype=torch.float32, device=q.device) if rows else None      # outputs, then (maximum, sum)
+    partial = _pointer(held)
+    st = _fn("dib_int8_attention_prompt")(
+        q.data_ptr(), out.data_ptr(), cache.data.data_ptr(), cache.scales.data_ptr(), pages, meta.block_table.data_ptr(),
+        meta.block_table.shape[1], meta.cu_q_lens.data_ptr(), meta.seq_lens.data_ptr(), part.units.data_ptr(), part.count,
+        part.seq_list.data_ptr(), part.seqs, part.max_tokens, partial, partial + rows * 512, part.chunk_tiles, part.chunks, hq,
+        hkv, d, page_size, scale, window, _stream())
+    _done(st, "int8_paged_attention", lambda: f"head_dim {d}, heads {hq}/{hkv}", 2 if part.chunks > 1 else 1)
 
 
 def _split(q, out, cache: Int8Cache, meta, part: _SplitPart, scale: float, window: int) -> None:
-    ops = _ops()
-    pages, _, hkv, page_size, d = cache.shape
-    rows = part.count * part.items * part.tile_rows if part.merge else 0
-    partial = torch.empty(rows * (d + 2), dtype=torch.float32, device=q.device)      # outputs, then (maximum, sum)
-    st = _lib().dib_int8_attention_split(
-        ops._ptr(q), ops._ptr(out), ops._ptr(cache.data), ops._ptr(cache.scales), c_longlong(pages),
-        ops._ptr(meta.block_table), c_int(meta.block_table.shape[1]), ops._ptr(meta.cu_q_lens), ops._ptr(meta.seq_lens),
-        ops._ptr(part.list), c_int(part.first), c_int(part.count), c_int(part.max_rows), c_int(part.tile_rows),
-        ops._ptr(partial), ops._ptr(partial[rows * d:]), c_int(part.items), c_int(1 if part.merge else 0), c_int(q.shape[1]), c_int(hkv),
-        c_int(d), c_int(page_size), c_float(scale), c_int(window), c_int(ops._dt(q, "q")), c_int(_sms(q.device)),
-        ops._stream())
-    ops._check(st, "int8_paged_attention", f"head_dim {d}, heads {q.shape[1]}/{hkv}", kernels=2 if part.merge else 1)
+    pages, _, hkv, page_size, d = cache.data.shape
+    hq = q.shape[1]
+    rows = part.rows
+    held = torch.empty(rows * (d + 2), dtype=torch.float32, device=q.device) if rows else None      # outputs, (maximum, sum)
+    partial = _pointer(held)
+    st = _fn("dib_int8_attention_split")(
+        q.data_ptr(), out.data_ptr(), cache.data.data_ptr(), cache.scales.data_ptr(), pages, meta.block_table.data_ptr(),
+        meta.block_table.shape[1], meta.cu_q_lens.data_ptr(), meta.seq_lens.data_ptr(), part.list_pointer, part.first, part.count,
+        part.max_rows, part.tile_rows, partial, partial + rows * d * 4, part.items, 1 if rows else 0, hq, hkv, d, page_size, scale,
+        window, _ops()._DT[q.dtype], _sms(q.device), _stream())
+    _done(st, "int8_paged_attention", lambda: f"head_dim {d}, heads {hq}/{hkv}", 2 if rows else 1)
 
 
 def int8_paged_attention(q: torch.Tensor, cache: Int8Cache, meta, scale: float, window=None) -> torch.Tensor:
@@ -401,34 +495,36 @@ def int8_paged_attention(q: torch.Tensor, cache: Int8Cache, meta, scale: float, 
     codes of keys and values enter the products as they are, the scales join scores and probabilities in float32.  A
     token that sees no key gives zeros."""
     ops = _ops()
-    ops._need(q, "q", None, 3)
+    if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dim() == 3 and q.is_contiguous()):
+        ops._need(q, "q", None, 3)
+    code = _code(q.dtype, "q")
     t, hq, d = q.shape
-    pages, _, hkv, page_size, d2 = cache.shape
+    data = cache.data
+    pages, _, hkv, page_size, d2 = data.shape
     if d2 != d or hq < 1 or hq % hkv:
         raise ops.KernelError(f"int8_paged_attention: q {tuple(q.shape)} vs cache {tuple(cache.shape)}")
-    b = meta.block_table.shape[0] if meta.block_table.dim() == 2 else -1
-    ops._need(meta.block_table, "block_table", torch.int32, 2)
-    for x, name, n in ((meta.token_seq, "token_seq", t), (meta.cu_q_lens, "cu_q_lens", b + 1),
-                       (meta.seq_lens, "seq_lens", b)):
-        ops._need(x, name, torch.int32, 1)
+    table, token_seq, cu, lens = meta.block_table, meta.token_seq, meta.cu_q_lens, meta.seq_lens
+    _require(table, "block_table", torch.int32, 2)
+    b = table.shape[0]
+    for x, name, n in ((token_seq, "token_seq", t), (cu, "cu_q_lens", b + 1), (lens, "seq_lens", b)):
+        _require(x, name, torch.int32, 1)
         if x.shape[0] < n:
             raise ops.KernelError(f"int8_paged_attention: {name} has {x.shape[0]} entries, the step needs {n}")
     win = int(window) if window else 0
     if win < 0:
         raise ops.KernelError(f"int8_paged_attention: a window of {win} keys")
-    _same_device("int8_paged_attention", q, cache.data, meta.block_table, meta.token_seq, meta.cu_q_lens, meta.seq_lens)
+    _same_device("int8_paged_attention", data, q, table, token_seq, cu, lens)
     out = torch.empty_like(q)
     if t == 0:
         return out
-    if d <= 128 and _pages_fit(page_size) and q.data_ptr() % 16 == 0 and cache.scales.data_ptr() % 16 == 0 and pages * 2 * hkv * page_size < 1 << 31:
-        for part in _parts(meta, hq // hkv, hkv, q.dtype == torch.float32, win, q.device):
+    if d <= 128 and _pages_fit(page_size) and q.data_ptr() % 16 == 0 and cache.scales.data_ptr() % 16 == 0 \
+            and pages * 2 * hkv * page_size < 1 << 31:
+        for part in _parts(meta, hq // hkv, hkv, code == 0, win, q.device):
             run = _prompt if isinstance(part, _PromptPart) else _split
             run(q, out, cache, meta, part, float(scale), win)
         return out
-    st = ops._lib("attention_int8").dib_int8_attention_any(
-        ops._ptr(q), ops._ptr(out), ops._ptr(cache.data), ops._ptr(cache.scales), ops._ptr(meta.block_table),
-        c_int(meta.block_table.shape[1]), ops._ptr(meta.token_seq), ops._ptr(meta.cu_q_lens), ops._ptr(meta.seq_lens),
-        c_int(t), c_int(hq), c_int(hkv), c_int(d), c_int(page_size), c_float(scale), c_int(win), c_int(ops._dt(q, "q")),
-        ops._stream())
-    ops._check(st, "int8_paged_attention", f"head_dim {d}, heads {hq}/{hkv}")
+    st = _fn("dib_int8_attention_any")(
+        q.data_ptr(), out.data_ptr(), data.data_ptr(), cache.scales.data_ptr(), table.data_ptr(), table.shape[1],
+        token_seq.data_ptr(), cu.data_ptr(), lens.data_ptr(), t, hq, hkv, d, page_size, float(scale), win, code, _stream())
+    _done(st, "int8_paged_attention", lambda: f"head_dim {d}, heads {hq}/{hkv}")
     return out

@@ -41,8 +41,7 @@ def test_prompt_units_cover_every_token_once():
     for q_lens, kv_lens in (([1, 3, 200, 70, 500], [9, 50, 200, 4500, 9000]), ([130, 129], [130, 700])):
         many = [s for s, n in enumerate(q_lens) if n * 2 > int8.PROMPT_ROWS]
         part = int8._PromptPart.__new__(int8._PromptPart)
-        from deterministic_inference_b200.kernels import attention_bf16
-        attention_bf16._sms[torch.device("cpu")] = 148
+        int8._sm_counts[torch.device("cpu")] = 148
         part.__init__(many, q_lens, kv_lens, 2, 8, 0, torch.device("cpu"))
         seq, a, b, chunk = part.units.view(4, part.count).tolist()
         seen = {}
