@@ -32,15 +32,33 @@ __device__ __forceinline__ RowScale row_scale(unsigned bits) {
   return r;
 }
 __device__ __forceinline__ unsigned magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-// four codes in a word, x0's in the low byte (a row with scale NaN: 0 * infinity is NaN, whose integer is 0)
+// the larger magnitude, a NaN if either is one
+__device__ __forceinline__ float larger(float top, float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(top), "f"(fabsf(x)));
+  return r;
+}
+// The codes in the low bytes: adding 1.5 * 2^23 to the product rounds it to an integer, ties to even, and leaves that in
+// the low bits (a row with scale NaN has inv 0; what 0 * infinity gives there is cleared).
+__device__ __forceinline__ unsigned code_bits(float x, float inv) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.f));
+}
+// four codes in a word, x0's in the low byte
 __device__ __forceinline__ unsigned pack4(const float* x, float inv) {
-  const int c0 = __float2int_rn(__fmul_rn(x[0], inv)), c1 = __float2int_rn(__fmul_rn(x[1], inv));
-  const int c2 = __float2int_rn(__fmul_rn(x[2], inv)), c3 = __float2int_rn(__fmul_rn(x[3], inv));
-  return (unsigned)(c0 & 0xff) | (unsigned)(c1 & 0xff) << 8 | (unsigned)(c2 & 0xff) << 16 | (unsigned)c3 << 24;
+  if (inv == 0.f) return 0;
+  return __byte_perm(__byte_perm(code_bits(x[0], inv), code_bits(x[1], inv), 0x0040),
+                     __byte_perm(code_bits(x[2], inv), code_bits(x[3], inv), 0x0040), 0x5410);
+}
+// four codes as numbers: a byte with its sign turned, under the exponent of 2^23, is 2^23 + 128 + code
+__device__ __forceinline__ void unpack4(unsigned w, float scale, float* x) {
+  w ^= 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    x[i] = __fmul_rn(__fadd_rn(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 + i)), -8388736.f), scale);
 }
 
-template <typename T, bool ALIGNED> __device__ __forceinline__ void load8(const T* p, float (&x)[8]);
-template <> __device__ __forceinline__ void load8<__nv_bfloat16, true>(const __nv_bfloat16* p, float (&x)[8]) {
+template <typename T> __device__ __forceinline__ void load8(const T* p, float (&x)[8]);
+template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&x)[8]) {
   const uint4 v = *reinterpret_cast<const uint4*>(p);
   const unsigned w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -49,32 +67,10 @@ template <> __device__ __forceinline__ void load8<__nv_bfloat16, true>(const __n
     x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
 }
-template <> __device__ __forceinline__ void load8<float, true>(const float* p, float (&x)[8]) {
+template <> __device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
   const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
   x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
   x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-template <> __device__ __forceinline__ void load8<__nv_bfloat16, false>(const __nv_bfloat16* p, float (&x)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = __bfloat162float(p[i]);
-}
-template <> __device__ __forceinline__ void load8<float, false>(const float* p, float (&x)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = p[i];
-}
-template <typename T> __device__ __forceinline__ void store8(T* p, const float (&x)[8]);
-template <> __device__ __forceinline__ void store8<float>(float* p, const float (&x)[8]) {
-  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
-}
-template <> __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* p, const float (&x)[8]) {
-  unsigned w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-    w[i] = *reinterpret_cast<const unsigned*>(&v);
-  }
-  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <typename T> __device__ __forceinline__ void load4(const T* p, float (&x)[4]);
@@ -96,76 +92,172 @@ template <> __device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16*
   *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
 }
 
-constexpr int CACHE_THREADS = 256, ROW_LANES = 16;       // half a warp a row: 8 values a lane, twice for heads above 128
+// 32 bytes of a row at once
+template <typename T> struct Piece {
+  static constexpr int N = 32 / (int)sizeof(T);        // values
+  unsigned w[8];
+  __device__ __forceinline__ void load(const T* p) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p));
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  }
+  __device__ __forceinline__ float get(int e) const {
+    if (sizeof(T) == 4) return __uint_as_float(w[e & 7]);
+    return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+  }
+};
+// n / d for n < 2^31 by a product: d's reciprocal rounded up, with as many bits as make that exact
+struct Divisor {
+  unsigned mul, shift, d;
+};
+__device__ __forceinline__ unsigned quotient(unsigned n, const Divisor& v) {
+  return v.mul == 0 ? n >> v.shift : __umulhi(n, v.mul) >> v.shift;
+}
+static inline Divisor make_divisor(unsigned d) {
+  Divisor v;
+  v.d = d;
+  unsigned log = 0;
+  while ((1ull << log) < d) ++log;
+  if ((1u << log) == d) {
+    v.mul = 0;
+    v.shift = log;
+  } else {      // n < 2^31: floor(n m / 2^(31 + log)) with m = ceil(2^(31 + log) / d) < 2^32 is exact
+    v.mul = (unsigned)(((1ull << (31 + log)) + d - 1) / d);
+    v.shift = log - 1;
+  }
+  return v;
+}
 
-// Row r = (token, key or value, kv head).  Memory bound: a row is read once into registers.
-template <typename T, bool ALIGNED>
+// A row of the cache: 128 values are LANES lanes, 32 bytes of the unquantised row each.  Memory bound: many warps of few
+// registers and few instructions, a row a group of lanes (several rows a group, all asked for first: 25 us where this
+// takes 12, 8,000 tokens of 8 heads of 128 written).
+constexpr int CACHE_THREADS = 256;
+template <typename T> struct Rows {
+  static constexpr int N = Piece<T>::N, LANES = 128 / N, GROUPS = CACHE_THREADS / LANES;
+};
+struct CacheShape {
+  Divisor per_token, page;      // 2 Hkv rows a token, rows a page
+  unsigned rows;
+  int Hkv, D;
+  unsigned num_pages;
+};
+struct CacheRow {
+  long long at;      // row of the cache, or -1
+  int token, kv, h;
+};
+// row r = (token, key or value, kv head)
+__device__ __forceinline__ CacheRow cache_row(unsigned r, const CacheShape& s, const int* slots) {
+  CacheRow c;
+  c.at = -1;
+  c.token = (int)quotient(r, s.per_token);
+  const int rest = (int)(r - (unsigned)c.token * s.per_token.d);
+  c.kv = rest >= s.Hkv;
+  c.h = rest - c.kv * s.Hkv;
+  if (r >= s.rows) return c;
+  const int slot = slots[c.token];
+  if (slot < 0) return c;
+  const unsigned page = quotient((unsigned)slot, s.page);
+  if (page < s.num_pages) c.at = ((long long)page * s.per_token.d + rest) * s.page.d + (slot - (int)(page * s.page.d));
+  return c;
+}
+
+template <typename T, bool ALIGNED, int HALVES>
 __global__ void __launch_bounds__(CACHE_THREADS)
 cache_write_kernel(const T* __restrict__ k, const T* __restrict__ v, long long k_stride, long long v_stride,
                    signed char* __restrict__ data, float* __restrict__ scales, const int* __restrict__ slots,
-                   long long rows, int Hkv, int D, int page_size, long long num_pages) {
+                   const __grid_constant__ CacheShape s) {
+  using R = Rows<T>;
   pdl_prologue(k, v, slots);
-  const long long r = ((long long)blockIdx.x * CACHE_THREADS + threadIdx.x) / ROW_LANES;
-  const int l = threadIdx.x & (ROW_LANES - 1);
-  const bool in = r < rows;
-  const long long token = in ? r / (2 * Hkv) : 0;
-  const int rest = in ? (int)(r - token * 2 * Hkv) : 0;
-  const int kv = rest >= Hkv, h = rest - kv * Hkv;
-  const T* src = (kv ? v + token * v_stride : k + token * k_stride) + (long long)h * D;
-  const int slot = in ? slots[token] : -1;
-  float x[2][8];
-  unsigned top = 0;
+  const int l = threadIdx.x & (R::LANES - 1);
+  const CacheRow c = cache_row(blockIdx.x * R::GROUPS + threadIdx.x / R::LANES, s, slots);
+  const T* src = (c.kv ? v + c.token * v_stride : k + c.token * k_stride) + c.h * s.D;
+  Piece<T> x[HALVES];
+  float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int d = (i * ROW_LANES + l) * 8;
-    if (in && d < D) {
-      load8<T, ALIGNED>(src + d, x[i]);
+  for (int i = 0; i < HALVES; ++i) {
+    const int d = i * 128 + l * R::N;
+    const bool in = c.at >= 0 && d < s.D;
+    if (ALIGNED) {
+      if (in) x[i].load(src + d);
+    } else if (in) {
+      T* to = reinterpret_cast<T*>(x[i].w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, magnitude_bits(x[i][j]));
+      for (int e = 0; e < R::N; ++e) to[e] = src[d + e];
     }
+    if (in)
+#pragma unroll
+      for (int e = 0; e < R::N; ++e) top = larger(top, x[i].get(e));
   }
 #pragma unroll
-  for (int o = ROW_LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (slot < 0) return;
-  const long long page = slot / page_size;
-  if (page >= num_pages) return;
-  const long long at = ((page * 2 + kv) * Hkv + h) * page_size + (slot - page * page_size);
-  const RowScale s = row_scale(top);
+  for (int o = R::LANES / 2; o > 0; o >>= 1) top = larger(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (c.at < 0) return;
+  const RowScale scale = row_scale(__float_as_uint(top));
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int d = (i * ROW_LANES + l) * 8;
-    if (d < D) *reinterpret_cast<uint2*>(data + at * D + d) = make_uint2(pack4(x[i], s.inv), pack4(x[i] + 4, s.inv));
+  for (int i = 0; i < HALVES; ++i) {
+    const int d = i * 128 + l * R::N;
+    if (d >= s.D) break;
+    unsigned y[R::N / 4];
+#pragma unroll
+    for (int e = 0; e < R::N; e += 4) {
+      const float four[4] = {x[i].get(e), x[i].get(e + 1), x[i].get(e + 2), x[i].get(e + 3)};
+      y[e / 4] = pack4(four, scale.inv);
+    }
+    signed char* dst = data + c.at * s.D + d;
+    if (R::N == 16) *reinterpret_cast<uint4*>(dst) = make_uint4(y[0], y[1], y[R::N / 4 - 2], y[R::N / 4 - 1]);
+    else *reinterpret_cast<uint2*>(dst) = make_uint2(y[0], y[1]);
   }
-  if (l == 0) scales[at] = s.scale;
+  if (l == 0) scales[c.at] = scale.scale;
 }
 
-template <typename T>
+template <typename T, int HALVES>
 __global__ void __launch_bounds__(CACHE_THREADS)
 cache_read_kernel(const signed char* __restrict__ data, const float* __restrict__ scales, const int* __restrict__ slots,
-                  T* __restrict__ k, T* __restrict__ v, long long rows, int Hkv, int D, int page_size,
-                  long long num_pages) {
+                  T* __restrict__ k, T* __restrict__ v, const __grid_constant__ CacheShape s) {
+  using R = Rows<T>;
   pdl_prologue(data, scales, slots);
-  const long long r = ((long long)blockIdx.x * CACHE_THREADS + threadIdx.x) / ROW_LANES;
-  const int l = threadIdx.x & (ROW_LANES - 1);
-  if (r >= rows) return;
-  const long long token = r / (2 * Hkv);
-  const int rest = (int)(r - token * 2 * Hkv);
-  const int kv = rest >= Hkv, h = rest - kv * Hkv;
-  const int slot = slots[token];
-  const long long page = slot < 0 ? -1 : slot / page_size;
-  const bool there = page >= 0 && page < num_pages;
-  const long long at = there ? ((page * 2 + kv) * Hkv + h) * page_size + (slot - page * page_size) : 0;
-  const float scale = there ? scales[at] : 0.f;
-  T* dst = (kv ? v : k) + (token * Hkv + h) * D;
+  const int l = threadIdx.x & (R::LANES - 1);
+  const unsigned r = blockIdx.x * R::GROUPS + threadIdx.x / R::LANES;
+  const CacheRow c = cache_row(r, s, slots);
+  if (r >= s.rows) return;
+  const float scale = c.at >= 0 ? scales[c.at] : 0.f;
+  T* dst = (c.kv ? v : k) + ((long long)c.token * s.Hkv + c.h) * s.D;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int d = (i * ROW_LANES + l) * 8;
-    if (d >= D) break;
-    const uint2 c = there ? *reinterpret_cast<const uint2*>(data + at * D + d) : make_uint2(0, 0);
-    float x[8];
+  for (int i = 0; i < HALVES; ++i) {
+    const int d = i * 128 + l * R::N;
+    if (d >= s.D) break;
+    unsigned w[R::N / 4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = scale * (float)(signed char)((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
-    store8<T>(dst + d, x);
+    for (int e = 0; e < R::N / 4; ++e) w[e] = 0;
+    if (c.at >= 0) {
+      const signed char* src = data + c.at * s.D + d;
+      if (R::N == 16) {
+        const uint4 q = *reinterpret_cast<const uint4*>(src);
+        w[0] = q.x; w[1] = q.y; w[R::N / 4 - 2] = q.z; w[R::N / 4 - 1] = q.w;
+      } else {
+        const uint2 q = *reinterpret_cast<const uint2*>(src);
+        w[0] = q.x; w[1] = q.y;
+      }
+    }
+    Piece<T> y;
+#pragma unroll
+    for (int e = 0; e < R::N / 4; ++e) {
+      float x[4];
+      unpack4(w[e], scale, x);
+      if (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y.w[(e * 4 + j) & 7] = __float_as_uint(x[j]);
+      } else {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+        y.w[(e * 2) & 7] = *reinterpret_cast<const unsigned*>(&a);
+        y.w[(e * 2 + 1) & 7] = *reinterpret_cast<const unsigned*>(&b);
+      }
+    }
+    y.store(dst + d);
   }
 }
 
@@ -284,7 +376,7 @@ quantize_rows_kernel(const T* __restrict__ x, long long stride, signed char* __r
     for (int i = 0; i < VECTORS; ++i) {
       const int at = (i * ROWS_THREADS + threadIdx.x) * 8;
       if (at < K) {
-        load8<T, true>(src + at, v[i]);
+        load8<T>(src + at, v[i]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = max(top, magnitude_bits(v[i][j]));
       }
@@ -312,6 +404,40 @@ quantize_rows_kernel(const T* __restrict__ x, long long stride, signed char* __r
     for (int at = threadIdx.x; at < Kp; at += ROWS_THREADS)
       dst[at] = at < K ? (signed char)__float2int_rn(__fmul_rn(Elem<T>::load(src + at), s.inv)) : 0;
   }
+}
+
+CacheShape make_shape(long long rows, int Hkv, int D, int page_size, long long num_pages) {
+  CacheShape s;
+  s.per_token = make_divisor(2u * Hkv);
+  s.page = make_divisor((unsigned)page_size);
+  s.rows = (unsigned)rows;
+  s.Hkv = Hkv; s.D = D;
+  s.num_pages = (unsigned)num_pages;
+  return s;
+}
+template <typename T>
+int launch_write(const void* k, const void* v, long long k_stride, long long v_stride, signed char* data, float* scales,
+                 const int* slots, const CacheShape& s, cudaStream_t st) {
+  constexpr int GROUPS = Rows<T>::GROUPS;
+  const bool wide = s.D > 128;
+  const bool aligned = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 31) == 0 &&
+                       (k_stride * sizeof(T)) % 32 == 0 && (v_stride * sizeof(T)) % 32 == 0 && (s.D * sizeof(T)) % 32 == 0;
+  auto kern = wide ? (aligned ? cache_write_kernel<T, true, 2> : cache_write_kernel<T, false, 2>)
+                   : (aligned ? cache_write_kernel<T, true, 1> : cache_write_kernel<T, false, 1>);
+  dib_launch(kern, dim3((s.rows + GROUPS - 1) / GROUPS), dim3(CACHE_THREADS), 0, st, reinterpret_cast<const T*>(k),
+             reinterpret_cast<const T*>(v), k_stride, v_stride, data, scales, slots, s);
+  DIB_CHECK_LAUNCH();
+  return DIB_OK;
+}
+template <typename T>
+int launch_read(const signed char* data, const float* scales, const int* slots, void* k, void* v, const CacheShape& s,
+                cudaStream_t st) {
+  constexpr int GROUPS = Rows<T>::GROUPS;
+  if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 31) != 0) return DIB_BAD_ALIGN;
+  dib_launch(s.D > 128 ? cache_read_kernel<T, 2> : cache_read_kernel<T, 1>, dim3((s.rows + GROUPS - 1) / GROUPS),
+             dim3(CACHE_THREADS), 0, st, data, scales, slots, reinterpret_cast<T*>(k), reinterpret_cast<T*>(v), s);
+  DIB_CHECK_LAUNCH();
+  return DIB_OK;
 }
 
 template <typename T>
@@ -346,25 +472,14 @@ int dib_int8_cache_write(const void* k, const void* v, long long k_stride, long 
   if ((reinterpret_cast<uintptr_t>(data) & 15) != 0) return DIB_BAD_ALIGN;
   if (T == 0) return DIB_OK;
   const long long rows = (long long)T * 2 * Hkv;
-  const long long blocks = (rows * ROW_LANES + CACHE_THREADS - 1) / CACHE_THREADS;
-  if (blocks > 0x7fffffffll) return DIB_BAD_SIZE;
-  const int per16 = dtype == 1 ? 8 : 4;
-  const bool aligned = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0 &&
-                       k_stride % per16 == 0 && v_stride % per16 == 0;
+  if (rows > 0x7fffff00ll || num_pages > 0x7fffffffll) return DIB_BAD_SIZE;
+  const CacheShape shape = make_shape(rows, Hkv, D, page_size, num_pages);
   signed char* d = reinterpret_cast<signed char*>(data);
   float* s = reinterpret_cast<float*>(scales);
   const int* sl = reinterpret_cast<const int*>(slots);
-  if (dtype == 1) {
-    auto kern = aligned ? cache_write_kernel<__nv_bfloat16, true> : cache_write_kernel<__nv_bfloat16, false>;
-    dib_launch(kern, dim3((unsigned)blocks), dim3(CACHE_THREADS), 0, st, reinterpret_cast<const __nv_bfloat16*>(k),
-               reinterpret_cast<const __nv_bfloat16*>(v), k_stride, v_stride, d, s, sl, rows, Hkv, D, page_size, num_pages);
-  } else {
-    auto kern = aligned ? cache_write_kernel<float, true> : cache_write_kernel<float, false>;
-    dib_launch(kern, dim3((unsigned)blocks), dim3(CACHE_THREADS), 0, st, reinterpret_cast<const float*>(k),
-               reinterpret_cast<const float*>(v), k_stride, v_stride, d, s, sl, rows, Hkv, D, page_size, num_pages);
-  }
-  DIB_CHECK_LAUNCH();
-  return DIB_OK;
+  if (dtype == 1)
+    return launch_write<__nv_bfloat16>(k, v, k_stride, v_stride, d, s, sl, shape, st);
+  return launch_write<float>(k, v, k_stride, v_stride, d, s, sl, shape, st);
 }
 
 // qkv [T, (Hq + 2 Hkv) D] -> q_out [T, Hq, D] and the cache; q_norm_w, k_norm_w float32 [D] or null; cos_sin float32
@@ -408,19 +523,13 @@ int dib_int8_cache_read(const void* data, const void* scales, const void* slots,
     return DIB_BAD_ALIGN;
   if (T == 0) return DIB_OK;
   const long long rows = (long long)T * 2 * Hkv;
-  const long long blocks = (rows * ROW_LANES + CACHE_THREADS - 1) / CACHE_THREADS;
-  if (blocks > 0x7fffffffll) return DIB_BAD_SIZE;
+  if (rows > 0x7fffff00ll || num_pages > 0x7fffffffll) return DIB_BAD_SIZE;
   const signed char* d = reinterpret_cast<const signed char*>(data);
   const float* s = reinterpret_cast<const float*>(scales);
   const int* sl = reinterpret_cast<const int*>(slots);
-  if (dtype == 1)
-    dib_launch(cache_read_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(CACHE_THREADS), 0, st, d, s, sl,
-               reinterpret_cast<__nv_bfloat16*>(k), reinterpret_cast<__nv_bfloat16*>(v), rows, Hkv, D, page_size, num_pages);
-  else
-    dib_launch(cache_read_kernel<float>, dim3((unsigned)blocks), dim3(CACHE_THREADS), 0, st, d, s, sl,
-               reinterpret_cast<float*>(k), reinterpret_cast<float*>(v), rows, Hkv, D, page_size, num_pages);
-  DIB_CHECK_LAUNCH();
-  return DIB_OK;
+  const CacheShape shape = make_shape(rows, Hkv, D, page_size, num_pages);
+  if (dtype == 1) return launch_read<__nv_bfloat16>(d, s, sl, k, v, shape, st);
+  return launch_read<float>(d, s, sl, k, v, shape, st);
 }
 
 // codes int8 [M, Kp] (Kp = K rounded up to 16, zeros behind K) and scales [M] of x [M, K], rows `stride` values apart.
