@@ -2,14 +2,15 @@
 // bfloat16 queries and many rows: S = Q K^T and O = P V by tcgen05.mma kind::f16 on bfloat16, accumulators in tensor memory,
 // a thread a query row for the softmax.
 //
-// The codes are exact in bfloat16, so they enter both products as they are: three warps turn a key tile's bytes (fetched by
+// The codes are exact in bfloat16, so they enter both products as they are: six warps turn a key tile's bytes (fetched by
 // TMA, a box a page) into swizzled bfloat16 tiles, once for the 256 rows of the two query tiles that share them.  A key's
 // scale (times the softmax's) joins its column of the scores, a value's the probabilities before they are rounded to
 // bfloat16 for the second product; the sum of probabilities is taken before that.
 //
 // Two query tiles A and B of 128 rows (tokens x heads of a kv group) of one sequence a CTA.  Roles: warps 0-3 softmax of A,
 // 4-7 of B (a row's 128 scores in registers; probabilities go back to tensor memory over the scores and are the second
-// product's operand from there), warp 9 issues the products, warps 8, 10, 11 convert, and warp 8 sends for the next bytes.
+// product's operand from there), warp 9 issues the products, warp 8 sends for bytes and scales, warps 10-12 convert
+// keys, 13-15 values.
 // The products of the two tiles are staggered, each tile's softmax runs under the other's products.  Once a tile has had
 // its last key tile (or there is no B) the other runs alone and takes its score columns as a second buffer.
 // Tensor memory: S/P of A columns 0.., of B 128.., O of A 256.., of B 384...
@@ -21,21 +22,27 @@
 // What bounds it: the softmax threads' instructions (a score's scale, maximum, exponential, sum, value scale and packing),
 // with the conversion beside them; the products take half of that time.
 #include <cuda.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 
 namespace {
 
-constexpr int TILE = 128, THREADS = 384, COPY_WARP = 8, MMA_WARP = 9;
-constexpr int REGS_FEW = 80, REGS_MANY = 208;         // 128 * 80 + 256 * 208 <= 384 * 168
+constexpr int TILE = 128, SOFTMAX_WARPS = 8, COPY_WARP = 8, MMA_WARP = 9, CONVERT_WARP = 10, CONVERTERS = 6;
+constexpr int THREADS = 512, SOFTMAX = SOFTMAX_WARPS * 32;
+constexpr int REGS_FEW = 56, REGS_MANY = 200;         // 256 * 56 + 256 * 200 = 512 * 128
 constexpr int TILE_BYTES = 128 * 128 * 2, HALF_BYTES = 128 * 64 * 2;      // a bfloat16 tile: two halves of 64 columns
 constexpr int RAW_BYTES = 128 * 128;
 constexpr float NEG_BIG = -1e30f;
 constexpr float LOG2E = 1.4426950408889634f;
 
-// shared memory: queries of A and B, two stages of keys and values, the bytes of a tile's keys and values, scales
-constexpr int S_KV = 2 * TILE_BYTES, S_RAW = 6 * TILE_BYTES, S_SCALES = S_RAW + 2 * RAW_BYTES, S_BARS = S_SCALES + 2 * 1024;
-constexpr int S_TOTAL = S_BARS + 24 * 8, S_DYNAMIC = 232448;
+// shared memory: queries of A and B; a ring of 16-bit tiles and one of bytes, keys and values in turn; scales
+constexpr int RING = 3, SLOTS = 4;
+constexpr int S_KV = 2 * TILE_BYTES, S_RAW = S_KV + RING * TILE_BYTES, S_SCALES = S_RAW + RING * RAW_BYTES;
+constexpr int S_NAN = S_SCALES + SLOTS * 1024, S_BARS = S_NAN + SLOTS * 32, S_TOTAL = S_BARS + 32 * 8;
+constexpr int S_DYNAMIC = S_TOTAL + 1024;
 
 __device__ int dib_attention_int8_prompt_error_word = 0;
 
@@ -61,6 +68,11 @@ __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float two_to(int n) { return __int_as_float((n + 127) << 23); }      // -126 <= n <= 127
+__device__ __forceinline__ unsigned pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&v);
 }
 __device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -88,27 +100,46 @@ __device__ __forceinline__ float2 exp2_fma2(float2 x) {
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(unsigned long long* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void tc_mma(unsigned tmem_d, unsigned long long desc_a, unsigned long long desc_b, unsigned idesc,
-                                       unsigned accum) {
+// Issued by one lane, in code that the whole warp runs: what they are given stays in uniform registers.
+__device__ __forceinline__ unsigned elect_one() {
+  unsigned is;
   asm volatile(
       "{\n\t"
       ".reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
-      "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accum)
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t"
+      "}\n" : "=r"(is));
+  return is;
+}
+__device__ __forceinline__ void tc_commit(unsigned elected, unsigned long long* bar) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred e;\n\t"
+      "setp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t"
+      "}\n" ::"r"(smem_u32(bar)), "r"(elected)
       : "memory");
 }
-__device__ __forceinline__ void tc_mma_ts(unsigned tmem_d, unsigned tmem_a, unsigned long long desc_b, unsigned idesc,
-                                          unsigned accum) {
+__device__ __forceinline__ void tc_mma(unsigned elected, unsigned tmem_d, unsigned long long desc_a, unsigned long long desc_b,
+                                       unsigned idesc, unsigned accum) {
   asm volatile(
       "{\n\t"
-      ".reg .pred p;\n\t"
+      ".reg .pred p, e;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
-      "}\n" ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accum)
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accum), "r"(elected)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(unsigned elected, unsigned tmem_d, unsigned tmem_a, unsigned long long desc_b,
+                                          unsigned idesc, unsigned accum) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "}\n" ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accum), "r"(elected)
       : "memory");
 }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -144,22 +175,34 @@ __device__ __forceinline__ unsigned long long desc_k_major(unsigned addr) {
 __device__ __forceinline__ unsigned long long desc_mn_major(unsigned addr) {
   return desc_k_major(addr) | ((unsigned long long)(HALF_BYTES >> 4) << 16);
 }
-// kind::f16: float32 accumulator, bfloat16 A and B
-constexpr unsigned idesc_f16(int m, int n, int b_mn_major) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)b_mn_major << 16) | ((unsigned)(n >> 3) << 17) |
+// kind::f16: float32 accumulator, A and B both float16 or both bfloat16
+constexpr unsigned idesc_f16(int m, int n, bool bf16, int b_mn_major) {
+  return (1u << 4) | ((unsigned)bf16 << 7) | ((unsigned)bf16 << 10) | ((unsigned)b_mn_major << 16) | ((unsigned)(n >> 3) << 17) |
          ((unsigned)(m >> 4) << 24);
 }
-// byte offset of (row, 16-byte piece c of the row's 128 elements) in a bfloat16 tile
+// byte offset of (row, 16-byte piece c of the row's 128 elements) in a tile of 16-bit numbers
 __device__ __forceinline__ int piece_off(int row, int c) {
   return (c >> 3) * HALF_BYTES + row * 128 + (((c & 7) ^ (row & 7)) << 4);
 }
-// Two codes of a word as bfloat16, exactly: low 7 bits and sign bit of a byte under the exponent byte 0x43 are 128 + low and
-// 128 + 128 sign, and a code is the first minus the second.
-__device__ __forceinline__ unsigned codes_bf16(unsigned low7, unsigned sign, unsigned sel) {
-  const unsigned a = __byte_perm(low7, 0x43434343u, sel), b = __byte_perm(sign, 0x43434343u, sel);
-  const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-  return *reinterpret_cast<const unsigned*>(&d);
+// Two codes of a word as float16, exactly: a byte with its sign turned, under the exponent byte 0x64, is 1024 + 128 + code.
+__device__ __forceinline__ unsigned codes_f16(unsigned turned, unsigned sel) {
+  const unsigned a = __byte_perm(turned, 0x64646464u, sel);
+  const __half2 c = __hsub2(*reinterpret_cast<const __half2*>(&a), __half2half2(__ushort_as_half(0x6480)));      // 1152
+  return *reinterpret_cast<const unsigned*>(&c);
 }
+// Two codes of a word times a scale as bfloat16, rounded once: a byte with its sign turned, under the exponent of 2^23, is
+// 2^23 + 128 + code.
+__device__ __forceinline__ unsigned codes_bf16(unsigned turned, unsigned sel, float2 scale) {
+  const float2 u = make_float2(__uint_as_float(__byte_perm(turned, 0x4b000000u, sel)),
+                               __uint_as_float(__byte_perm(turned, 0x4b000000u, sel + 1)));
+  const float2 y = __fmul2_rn(__fadd2_rn(u, make_float2(-8388736.f, -8388736.f)), scale);
+  return pack_bf16(y.x, y.y);
+}
+
+// The keys of a tile that are no numbers: bit l of word j, key 4 l + j.
+struct NanKeys {
+  unsigned key[4], any, pad[3];
+};
 
 struct PromptArgs {
   const float* scales;          // [pages, 2, Hkv, page_size]
@@ -181,19 +224,20 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
   unsigned char* sQ = smem;
   unsigned char* sKV = smem + S_KV;
   unsigned char* raw = smem + S_RAW;
-  float* scales = reinterpret_cast<float*>(smem + S_SCALES);          // [2][keys', values' of 128]
+  float* scales = reinterpret_cast<float*>(smem + S_SCALES);          // [SLOTS][keys', values' of 128]
+  NanKeys* nan_keys = reinterpret_cast<NanKeys*>(smem + S_NAN);       // [SLOTS]
   unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + S_BARS);
-  unsigned long long* raw_full = bars;            // [keys, values] a tile's bytes have arrived
-  unsigned long long* k_full = bars + 2;          // [2] the keys of a tile are there as bfloat16
-  unsigned long long* k_empty = bars + 4;         // [2] both score products have read them
-  unsigned long long* v_full = bars + 6;          // [2] the values likewise
-  unsigned long long* v_empty = bars + 8;         // [2]
-  unsigned long long* sc_full = bars + 10;        // [2] the scales of a tile are there
-  unsigned long long* s_full = bars + 12;         // [A, B] the query tile's scores are in tensor memory
-  unsigned long long* p_full = bars + 14;         // [2] its probabilities are, and O is rescaled (128)
-  unsigned long long* o_final = bars + 16;        // [2] its last product has completed
-  unsigned long long* pv_done = bars + 18;        // an output product of the tile that runs alone has completed
-  unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 19);
+  unsigned long long* raw_full = bars;            // [RING] a tile's bytes have arrived
+  unsigned long long* raw_empty = bars + 3;       // [RING] they have been converted (a warp each)
+  unsigned long long* full = bars + 6;            // [RING] a tile is there in 16 bits (a warp each)
+  unsigned long long* empty = bars + 9;           // [RING] both products have read it
+  unsigned long long* sc_full = bars + 12;        // [SLOTS] the scales of a key tile are there
+  unsigned long long* sc_empty = bars + 16;       // [SLOTS] its outputs have been made
+  unsigned long long* s_full = bars + 20;         // [A, B] the query tile's scores are in tensor memory
+  unsigned long long* p_full = bars + 22;         // [2] its probabilities are, and O is rescaled (a warp each)
+  unsigned long long* o_final = bars + 24;        // [2] its last product has completed
+  unsigned long long* pv_done = bars + 26;        // an output product of the tile that runs alone has completed
+  unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 30);
   if (threadIdx.x == 0) prefetch_tensormap(&map);
   pdl_trigger();
   if (smem - smem_dyn + S_TOTAL > S_DYNAMIC) {      // (the memory is aligned to 1,024 as a rule)
@@ -209,7 +253,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
   const int kv_len = min(a.seq_lens[seq], (int)min((long long)a.max_blocks << a.page_shift, 0x7fffff00ll));
   const int prefix = kv_len - q_len;
   const int* bt = a.block_table + (long long)seq * a.max_blocks;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   // Per query tile: its tokens and the key tiles of this chunk that it needs.
   int ntok[2], jf[2], jl[2];
@@ -237,14 +281,16 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
   if (!any0 && !any1) return;     // nothing of this chunk concerns the pair
   const int j0 = any0 && any1 ? min(jf[0], jf[1]) : (any0 ? jf[0] : jf[1]);
   const int ntiles = max(any0 ? jl[0] : -1, any1 ? jl[1] : -1) - j0 + 1;
-  auto active = [&](int x, int i) { return j0 + i >= jf[x] && j0 + i <= jl[x]; };
+  // (arrays indexed by a running x would live in local memory)
+  auto active = [&](int x, int i) { return j0 + i >= (x ? jf[1] : jf[0]) && j0 + i <= (x ? jl[1] : jl[0]); };
   // From key tile solo_from on query tile solo_x is alone; the other one has had n_other key tiles.
   const int solo_x = (any1 && (!any0 || jl[1] >= jl[0])) ? 1 : 0;
   const int n_other = (solo_x ? any0 : any1) ? jl[1 - solo_x] - jf[1 - solo_x] + 1 : 0;
   const int solo_from = max((solo_x ? any0 : any1) ? jl[1 - solo_x] - j0 + 1 : 0, jf[solo_x] - j0);
 
   bool ok = true;
-  // ---- bytes of key tile i (0 keys, 1 values): lane l has the keys 4l .. 4l + 3, the first lane of each page sends
+  // ---- bytes of key tile i: lane l has the keys 4l .. 4l + 3, the first lane of each page sends.  Item 2i is the keys,
+  // 2i + 1 the values.
   const int page_mask = (1 << a.page_shift) - 1, half_rows = a.Hkv << a.page_shift, box_rows = min(1 << a.page_shift, TILE);
   auto row_of = [&](int i) {      // this lane's row of the cache for its keys of key tile i, or -1
     const int key = (j0 + i) * TILE + lane * 4;
@@ -252,139 +298,149 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
     const int page = bt[key >> a.page_shift];
     return page >= 0 && page < a.num_pages ? page * 2 * half_rows + (kvh << a.page_shift) + (key & page_mask) : -1;
   };
-  auto send = [&](int kv, int row) {
+  auto send = [&](int item, int row) {
     const bool sends = row >= 0 && (lane == 0 || (lane * 4 & page_mask) == 0);
     const unsigned senders = __ballot_sync(0xffffffffu, sends);
-    if (lane == 0) mbar_expect_tx(&raw_full[kv], __popc(senders) * box_rows * 128);
+    const int at = item % RING;
+    if (lane == 0) mbar_expect_tx(&raw_full[at], __popc(senders) * box_rows * 128);
     __syncwarp();
-    if (sends) tma_load_2d(smem_u32(raw) + kv * RAW_BYTES + lane * 512, &map, 0, row + kv * half_rows, &raw_full[kv]);
+    if (sends)
+      tma_load_2d(smem_u32(raw) + at * RAW_BYTES + lane * 512, &map, 0, row + (item & 1) * half_rows, &raw_full[at]);
   };
-  int row_next = -1;
+  int row_now = -1;
   if (warp == COPY_WARP) {
     if (lane == 0) {
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < RING; ++i) {
         mbar_init(&raw_full[i], 1);
-        mbar_init(&k_full[i], 1);
-        mbar_init(&k_empty[i], 1);
-        mbar_init(&v_full[i], 1);
-        mbar_init(&v_empty[i], 1);
-        mbar_init(&sc_full[i], 2);
+        mbar_init(&raw_empty[i], CONVERTERS);
+        mbar_init(&full[i], CONVERTERS);
+        mbar_init(&empty[i], 1);
+      }
+      for (int i = 0; i < SLOTS; ++i) {
+        mbar_init(&sc_full[i], 1);
+        mbar_init(&sc_empty[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
         mbar_init(&s_full[i], 1);
-        mbar_init(&p_full[i], 128);
+        mbar_init(&p_full[i], SOFTMAX_WARPS / 2);
         mbar_init(&o_final[i], 1);
       }
       mbar_init(pv_done, 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
-    row_next = row_of(0);
+    row_now = row_of(0);
   }
   const __nv_bfloat16* qp = q;
   pdl_wait(qp);
   if (warp == COPY_WARP) {
-    send(0, row_next);
-    send(1, row_next);
-    row_next = row_of(1);
+    send(0, row_now);
+    send(1, row_now);
   }
   if (warp == MMA_WARP) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
-  // both query tiles -> shared memory, swizzled; rows beyond a tile's tokens and dimensions beyond D are zero
-  {
-    constexpr int LOADERS = 256, PER_THREAD = 2 * TILE * 16 / LOADERS;
-    uint4 v[PER_THREAD];
+  // Both query tiles -> shared memory, swizzled, a thread a row: times the power of two that takes the row's largest value
+  // to 2^4 (exact in float16 down to 2^-21 of that); rows beyond a tile's tokens and dimensions beyond D are zero.
+  float row_unit = 1.f, row_sum = 0.f;
+  const int x = threadIdx.x >> 7, r = threadIdx.x & 127;
+  if (threadIdx.x < SOFTMAX) {
+    const int tl = r / G, g = r - tl * G, my_ntok = x ? ntok[1] : ntok[0];
+    uint4 v[16];
+    const __nv_bfloat16* src = qp + ((long long)(q_begin + (x ? tokx[1] : tokx[0]) + tl) * a.Hq + kvh * G + g) * a.D;
 #pragma unroll
-    for (int it = 0; it < PER_THREAD; ++it) {
-      const int c = threadIdx.x + it * LOADERS;
-      const int x = c >> 11, r = (c >> 4) & 127, ch = c & 15;
-      const int tl = r / G, g = r - tl * G;
-      v[it] = make_uint4(0, 0, 0, 0);
-      if (threadIdx.x < LOADERS && tl < ntok[x] && ch * 8 < a.D)
-        v[it] = *reinterpret_cast<const uint4*>(qp + ((long long)(q_begin + tokx[x] + tl) * a.Hq + kvh * G + g) * a.D + ch * 8);
+    for (int ch = 0; ch < 16; ++ch) {
+      v[ch] = make_uint4(0, 0, 0, 0);
+      if (tl < my_ntok && ch * 8 < a.D) v[ch] = *reinterpret_cast<const uint4*>(src + ch * 8);
+    }
+    unsigned top = 0;      // the largest magnitude, in the high half
+#pragma unroll
+    for (int ch = 0; ch < 16; ++ch) {
+      const unsigned w[4] = {v[ch].x, v[ch].y, v[ch].z, v[ch].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7fff0000u, w[e] << 16 & 0x7fff0000u));
+    }
+    const int expo = max((int)(top >> 23), 5);                    // (2^126 at most below)
+    float to_unit = two_to(131 - expo);
+    row_unit = two_to(expo - 131);
+    if (top >= 0x7f800000u) {                                     // an infinity or a NaN: so is what the row gets
+      to_unit = 0.f;
+      row_sum = __int_as_float(0x7fc00000);
     }
 #pragma unroll
-    for (int it = 0; it < PER_THREAD; ++it) {
-      const int c = threadIdx.x + it * LOADERS;
-      const int x = c >> 11, r = (c >> 4) & 127, ch = c & 15;
-      if (threadIdx.x < LOADERS) *reinterpret_cast<uint4*>(sQ + x * TILE_BYTES + piece_off(r, ch)) = v[it];
+    for (int ch = 0; ch < 16; ++ch) {
+      const unsigned w[4] = {v[ch].x, v[ch].y, v[ch].z, v[ch].w};
+      unsigned y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        y[e] = to_unit == 0.f ? 0u
+                              : pack_f16(__uint_as_float(w[e] << 16) * to_unit, __uint_as_float(w[e] & 0xffff0000u) * to_unit);
+      *reinterpret_cast<uint4*>(sQ + x * TILE_BYTES + piece_off(r, ch)) = make_uint4(y[0], y[1], y[2], y[3]);
     }
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the queries are read by the tensor core
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const unsigned tmem = *tmem_slot;
+  const unsigned tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp >= COPY_WARP) {
   regs_give<REGS_FEW>();
   if (warp == MMA_WARP) {
-    if (lane == 0) {
-      constexpr unsigned idesc_s = idesc_f16(TILE, TILE, 0), idesc_o = idesc_f16(TILE, TILE, 1);
+    {
+      const unsigned elected = elect_one();
+      constexpr unsigned idesc_s = idesc_f16(TILE, TILE, false, 0), idesc_o = idesc_f16(TILE, TILE, true, 1);
       // Descriptors are made once: a step inside a tile is an addition to the low bits, which hold the address.
-      const unsigned long long q_desc[2] = {desc_k_major(smem_u32(sQ)), desc_k_major(smem_u32(sQ + TILE_BYTES))};
-      unsigned long long k_desc[2], v_desc[2];
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        k_desc[st] = desc_k_major(smem_u32(sKV + st * 2 * TILE_BYTES));
-        v_desc[st] = desc_mn_major(smem_u32(sKV + st * 2 * TILE_BYTES + TILE_BYTES));
-      }
+      const unsigned long long q_desc = desc_k_major(smem_u32(sQ)), k_desc = desc_k_major(smem_u32(sKV)),
+                               v_desc = desc_mn_major(smem_u32(sKV));
       auto issue_s = [&](int x, int buf, int i) {      // scores of query tile x, key tile i -> columns of buf
-        const unsigned long long qd = x ? q_desc[1] : q_desc[0], kd = i & 1 ? k_desc[1] : k_desc[0];
+        const unsigned long long qd = q_desc + x * (TILE_BYTES >> 4), kd = k_desc + (2 * i % RING) * (TILE_BYTES >> 4);
 #pragma unroll
         for (int ks = 0; ks < TILE / 16; ++ks) {
           const unsigned long long at = (unsigned long long)(((ks >> 2) * HALF_BYTES + (ks & 3) * 32) >> 4);
-          tc_mma(tmem + buf * 128, qd + at, kd + at, idesc_s, ks > 0);
+          tc_mma(elected, tmem + buf * 128, qd + at, kd + at, idesc_s, ks > 0);
         }
-        tc_commit(&s_full[buf]);
+        tc_commit(elected, &s_full[buf]);
       };
       auto issue_o = [&](int x, int buf, int i) {      // outputs of query tile x from the probabilities in buf
-        const unsigned long long vd = i & 1 ? v_desc[1] : v_desc[0];
-        const bool first = j0 + i == jf[x];
+        const unsigned long long vd = v_desc + ((2 * i + 1) % RING) * (TILE_BYTES >> 4);
+        const bool first = j0 + i == (x ? jf[1] : jf[0]);
 #pragma unroll
         for (int ks = 0; ks < TILE / 16; ++ks)
-          tc_mma_ts(tmem + 256 + x * 128, tmem + buf * 128 + ks * 8, vd + (unsigned long long)((ks * 16 * 128) >> 4), idesc_o,
+          tc_mma_ts(elected, tmem + 256 + x * 128, tmem + buf * 128 + ks * 8, vd + (unsigned long long)((ks * 16 * 128) >> 4), idesc_o,
                     !first || ks > 0);
       };
       int uses[2] = {0, 0};     // completed phases of p_full
-      int have_k = 0, have_v = -1;
-      auto want_k = [&](int i) {
-        if (have_k < i) {
-          ok = mbar_wait(&k_full[i & 1], (i >> 1) & 1);
-          have_k = i;
-        }
-        return ok;
-      };
-      auto want_v = [&](int i) {
-        if (have_v < i) {
-          ok = mbar_wait(&v_full[i & 1], (i >> 1) & 1);
-          have_v = i;
-        }
-        return ok;
-      };
-      ok = mbar_wait(&k_full[0], 0);
-      if (ok) {
+      auto want = [&](int item) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&full[item % RING], (item / RING) & 1));
         tc_fence_after();
+        return ok;
+      };
+      if (want(0)) {
         if (active(0, 0)) issue_s(0, 0, 0);
         if (active(1, 0)) issue_s(1, 1, 0);
-        tc_commit(&k_empty[0]);
+        tc_commit(elected, &empty[0]);
       }
       const int paired_end = min(ntiles, solo_from);
       for (int i = 0; i < paired_end && ok; ++i) {
-        if (!want_v(i) || (i + 1 < ntiles && !want_k(i + 1))) break;
+        if (!want(2 * i + 1) || (i + 1 < ntiles && !want(2 * i + 2))) break;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           if (active(x, i)) {
-            ok = mbar_wait(&p_full[x], uses[x] & 1);
+            ok = __all_sync(0xffffffffu, mbar_wait(&p_full[x], uses[x] & 1));
             if (!ok) break;
             ++uses[x];
             tc_fence_after();
             issue_o(x, x, i);
-            if (j0 + i == jl[x]) tc_commit(&o_final[x]);
+            if (j0 + i == jl[x]) tc_commit(elected, &o_final[x]);
           }
-          if (x == 1) tc_commit(&v_empty[i & 1]);
+          if (x == 1) {
+            tc_commit(elected, &empty[(2 * i + 1) % RING]);
+            tc_commit(elected, &sc_empty[i % SLOTS]);
+          }
           if (i + 1 < ntiles && active(x, i + 1)) issue_s(x, x, i + 1);
-          if (x == 1 && i + 1 < ntiles) tc_commit(&k_empty[(i + 1) & 1]);
+          if (x == 1 && i + 1 < ntiles) tc_commit(elected, &empty[(2 * i + 2) % RING]);
         }
       }
       // ---- one query tile alone: its scores of key tile i are in buffer (i - solo_from) & 1 (0: its own columns); those of
@@ -392,121 +448,155 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
       for (int i = solo_from; i < ntiles && ok; ++i) {
         const int x = solo_x, buf = ((i - solo_from) & 1) ? 1 - x : x;
         if (i + 1 < ntiles) {
-          if (!want_k(i + 1)) break;
+          if (!want(2 * i + 2)) break;
           issue_s(x, 1 - buf, i + 1);
-          tc_commit(&k_empty[(i + 1) & 1]);
+          tc_commit(elected, &empty[(2 * i + 2) % RING]);
         }
-        if (!want_v(i)) break;
-        ok = mbar_wait(&p_full[buf], uses[buf] & 1);
+        if (!want(2 * i + 1)) break;
+        ok = __all_sync(0xffffffffu, mbar_wait(&p_full[buf], (buf ? uses[1] : uses[0]) & 1));
         if (!ok) break;
-        ++uses[buf];
+        if (buf) ++uses[1]; else ++uses[0];
         tc_fence_after();
         issue_o(x, buf, i);
-        tc_commit(&v_empty[i & 1]);
-        tc_commit(pv_done);
-        if (i == ntiles - 1) tc_commit(&o_final[x]);
+        tc_commit(elected, &empty[(2 * i + 1) % RING]);
+        tc_commit(elected, &sc_empty[i % SLOTS]);
+        tc_commit(elected, pv_done);
+        if (i == ntiles - 1) tc_commit(elected, &o_final[x]);
       }
     }
+  } else if (warp == COPY_WARP) {
+    // ---- bytes, and the scales of this lane's keys (zero for keys that the sequence does not have), which are asked for a
+    // tile ahead
+    int sent = 2;
+    float ks[4], vs[4];
+    auto load_scales = [&](int row) {
+      float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+      if (row >= 0) {
+        k = *reinterpret_cast<const float4*>(a.scales + row);
+        v = *reinterpret_cast<const float4*>(a.scales + row + half_rows);
+      }
+      ks[0] = k.x; ks[1] = k.y; ks[2] = k.z; ks[3] = k.w;
+      vs[0] = v.x; vs[1] = v.y; vs[2] = v.z; vs[3] = v.w;
+    };
+    load_scales(row_now);
+    int row_next = row_of(1);
+    const float unit = a.scale * LOG2E;
+    for (int i = 0; i < ntiles && ok; ++i) {
+      if (i >= SLOTS) ok = mbar_wait(&sc_empty[i % SLOTS], (i / SLOTS - 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const int left = kv_len - ((j0 + i) * TILE + lane * 4);
+      unsigned bad[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // a key or a value that is no number shows in the sums of the rows that see it
+        const float both = (ks[j] - ks[j]) + (vs[j] - vs[j]);
+        const bool is_nan = left > j && both != both;
+        bad[j] = __ballot_sync(0xffffffffu, is_nan);
+        ks[j] *= unit;
+        if (left <= j || is_nan) ks[j] = vs[j] = 0.f;
+      }
+      float* slot = scales + (i % SLOTS) * 256 + lane * 4;
+      *reinterpret_cast<float4*>(slot) = make_float4(ks[0], ks[1], ks[2], ks[3]);
+      *reinterpret_cast<float4*>(slot + 128) = make_float4(vs[0], vs[1], vs[2], vs[3]);
+      if (lane == 0) {
+        NanKeys n;
+        n.any = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) n.any |= n.key[j] = bad[j];
+        n.pad[0] = n.pad[1] = n.pad[2] = 0;
+        nan_keys[i % SLOTS] = n;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sc_full[i % SLOTS]);
+      if (i + 1 < ntiles) {
+        load_scales(row_next);
+        row_now = row_next;
+        row_next = row_of(i + 2);
+        for (int item = 2 * i + 2; item < 2 * i + 4 && ok; ++item) {
+          if (item >= RING) ok = mbar_wait(&raw_empty[item % RING], (item / RING - 1) & 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (ok) {
+            send(item, row_now);
+            sent = item + 1;
+          }
+        }
+      }
+    }
+    // the last bytes that were sent for have arrived before this block's memory is another's
+    for (int item = max(0, sent - RING); item < sent; ++item)
+      if (!mbar_wait(&raw_full[item % RING], (item / RING) & 1)) ok = false;
   } else {
     // ---- conversion.  A warp takes 8 rows x 64 codes at a time: eight lanes a pair of rows r, r ^ 5, whose pieces lie in
-    // different banks in the bytes' swizzle and in the bfloat16 tile's.
-    const int part = warp == COPY_WARP ? 0 : warp - 9;        // 0, 1, 2
+    // different banks in the bytes' swizzle and in the 16-bit tile's.
     const int r8 = lane & 4 ? (lane >> 3) ^ 5 : lane >> 3, p4 = lane & 3;
-    auto convert = [&](const unsigned char* src, unsigned char* dst) {
+    auto convert = [&](const unsigned char* src, unsigned char* dst, const float* vs, auto keys) {
 #pragma unroll 2
-      for (int u = part; u < 32; u += 3) {
+      for (int u = warp - CONVERT_WARP; u < 32; u += CONVERTERS) {
         const int row = (u >> 1) * 8 + r8, p = (u & 1) * 4 + p4;
         const uint4 w = *reinterpret_cast<const uint4*>(src + row * 128 + ((p ^ (row & 7)) << 4));
-        const unsigned word[4] = {w.x, w.y, w.z, w.w};
+        const unsigned turned[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+        const float scale = keys.value ? 0.f : vs[row];
+        const float2 scale2 = make_float2(scale, scale);
         unsigned y[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const unsigned low7 = word[e] & 0x7f7f7f7fu, sign = word[e] & 0x80808080u;
-          y[2 * e] = codes_bf16(low7, sign, 0x4140);
-          y[2 * e + 1] = codes_bf16(low7, sign, 0x4342);
+          y[2 * e] = keys.value ? codes_f16(turned[e], 0x4140) : codes_bf16(turned[e], 0x7540, scale2);
+          y[2 * e + 1] = keys.value ? codes_f16(turned[e], 0x4342) : codes_bf16(turned[e], 0x7542, scale2);
         }
         *reinterpret_cast<uint4*>(dst + piece_off(row, 2 * p)) = make_uint4(y[0], y[1], y[2], y[3]);
         *reinterpret_cast<uint4*>(dst + piece_off(row, 2 * p + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the tile is read by the tensor core, the bytes are
-      asm volatile("bar.sync 1, 96;" ::: "memory");                    // written by the next copy
     };
-    for (int i = 0; i < ntiles && ok; ++i) {
-      unsigned char* stage = sKV + (i & 1) * 2 * TILE_BYTES;
-      // the scales of this lane's keys: warp part 0 the keys', 1 the values'; zero for keys the sequence does not have
-      float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (part < 2) {
-        const int row = row_of(i);
-        const int left = kv_len - ((j0 + i) * TILE + lane * 4);
-        if (row >= 0) {
-          sc = *reinterpret_cast<const float4*>(a.scales + row + part * half_rows);
-          if (part == 1) {      // a key that is no number shows through its value (the scores' maximum does not see it)
-            const float4 k = *reinterpret_cast<const float4*>(a.scales + row);
-            sc.x += k.x - k.x; sc.y += k.y - k.y; sc.z += k.z - k.z; sc.w += k.w - k.w;
-          }
-          if (left < 2) sc.y = 0.f;
-          if (left < 3) sc.z = 0.f;
-          if (left < 4) sc.w = 0.f;
-        }
-        if (part == 0) {
-          const float unit = a.scale * LOG2E;
-          sc.x *= unit; sc.y *= unit; sc.z *= unit; sc.w *= unit;
-        }
-      }
-      ok = mbar_wait(&raw_full[0], i & 1) && (i < 2 || mbar_wait(&k_empty[i & 1], ((i >> 1) - 1) & 1));
+    for (int item = 0, at = 0, turn = 0; item < 2 * ntiles && ok; ++item) {
+      const int slot = (item >> 1) % SLOTS;
+      ok = (!(item & 1) || mbar_wait(&sc_full[slot], ((item >> 1) / SLOTS) & 1)) && mbar_wait(&raw_full[at], turn) &&
+           (item < RING || mbar_wait(&empty[at], turn ^ 1));
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      convert(raw, stage);
-      if (warp == COPY_WARP) {
-        if (lane == 0) mbar_arrive(&k_full[i & 1]);
-        if (i + 1 < ntiles) send(0, row_next);
+      const float* vs = scales + slot * 256 + 128;
+      if (item & 1) convert(raw + at * RAW_BYTES, sKV + at * TILE_BYTES, vs, std::false_type());
+      else convert(raw + at * RAW_BYTES, sKV + at * TILE_BYTES, vs, std::true_type());
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the tile is read by the tensor core, the bytes are
+      __syncwarp();                                                    // written by the next copy
+      if (lane == 0) {
+        mbar_arrive(&full[at]);
+        mbar_arrive(&raw_empty[at]);
       }
-      ok = mbar_wait(&raw_full[1], i & 1) && (i < 2 || mbar_wait(&v_empty[i & 1], ((i >> 1) - 1) & 1));
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      if (part < 2) {      // (the softmax has read those of the tile two before this one: its outputs have been made)
-        *reinterpret_cast<float4*>(scales + (i & 1) * 256 + part * 128 + lane * 4) = sc;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sc_full[i & 1]);
-      }
-      convert(raw + RAW_BYTES, stage + TILE_BYTES);
-      if (warp == COPY_WARP) {
-        if (lane == 0) mbar_arrive(&v_full[i & 1]);
-        if (i + 1 < ntiles) {
-          send(1, row_next);
-          row_next = row_of(i + 2);
-        }
+      if (++at == RING) {
+        at = 0;
+        turn ^= 1;
       }
     }
   }
   } else {
     regs_take<REGS_MANY>();
     // ---- softmax: thread r of group x owns row r of query tile x
-    const int x = threadIdx.x >> 7, r = threadIdx.x & 127;
     const int tl = r / G, g = r - tl * G;
-    const bool valid = tl < ntok[x];
+    const int tok0 = x ? tokx[1] : tokx[0], i_first = (x ? jf[1] : jf[0]) - j0, i_last = (x ? jl[1] : jl[0]) - j0;
+    const bool valid = tl < (x ? ntok[1] : ntok[0]);
     // (rows behind the sequence's last token see what a token there would see: no warp goes through the tests for masked
     // keys for their sake)
-    const int hi = prefix + tokx[x] + tl, lo = first_visible_key(hi, a.window);
+    const int hi = prefix + tok0 + tl, lo = first_visible_key(hi, a.window);
     const unsigned lane_base = (unsigned)((warp & 3) * 32) << 16;
     const unsigned tmem_o = tmem + lane_base + 256 + x * 128;
-    float m_ref = NEG_BIG, l = 0.f;
+    float m_ref = NEG_BIG, l = row_sum;
     int uses_own = 0, uses_other = n_other;      // completed phases of s_full of the own columns and of the other's
     const int my_solo = x == solo_x ? solo_from : 0x7fffffff;
-    for (int i = 0; i < ntiles && ok; ++i) {
-      if (!active(x, i)) continue;
+    const float2 unit2 = make_float2(row_unit, row_unit);
+    for (int i = i_first; i <= i_last && ok; ++i) {
       const bool borrowed = i >= my_solo && ((i - my_solo) & 1);
       const int buf = borrowed ? 1 - x : x;
       const unsigned tmem_s = tmem + lane_base + buf * 128;
-      ok = mbar_wait(&sc_full[i & 1], (i >> 1) & 1) && mbar_wait(&s_full[buf], (borrowed ? uses_other : uses_own) & 1);
+      ok = mbar_wait(&sc_full[i % SLOTS], (i / SLOTS) & 1) && mbar_wait(&s_full[buf], (borrowed ? uses_other : uses_own) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (borrowed) ++uses_other; else ++uses_own;
       tc_fence_after();
-      const int kbase = (j0 + i) * TILE;
-      const bool full = kbase >= lo && kbase + TILE - 1 <= hi;   // no key of the tile is masked
-      const float* ks = scales + (i & 1) * 256;
-      const float* vs = ks + 128;
+      const int kbase = (j0 + i) * TILE, first = lo - kbase, last = hi - kbase;      // visible: [first, last]
+      const bool unmasked = first <= 0 && last >= TILE - 1;
+      const float* ks = scales + (i % SLOTS) * 256;
+      const NanKeys* nan = nan_keys + i % SLOTS;
       unsigned v[4][32];
 #pragma unroll
       for (int c = 0; c < 4; ++c) tc_ld32(tmem_s + c * 32, v[c]);
@@ -521,26 +611,24 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
           v[c][k] = __float_as_uint(y0.x); v[c][k + 1] = __float_as_uint(y0.y);
           v[c][k + 2] = __float_as_uint(y1.x); v[c][k + 3] = __float_as_uint(y1.y);
         }
-      if (!full) {
-        // keys outside [lo, hi] get NEG_BIG: one subtraction and one unsigned comparison each
-        const int first = lo - kbase, last = hi - kbase;
+      if (!unmasked) {
+        // keys outside [first, last]: one subtraction and one unsigned comparison each
         const int first_vis = last >= first ? first : (1 << 20);
         const unsigned span = last >= first ? (unsigned)(last - first) : 0u;
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int k = 0; k < 32; ++k)
-            if ((unsigned)(c * 32 + k - first_vis) > span) v[c][k] = __float_as_uint(NEG_BIG);
+            if ((unsigned)(c * 32 + k - first_vis) > span) v[c][k] = 0xff800000u;
       }
-      float m4[4] = {NEG_BIG, NEG_BIG, NEG_BIG, NEG_BIG};
+      float m4[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < 4; ++c) m4[c] = fmaxf(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]));
 #pragma unroll
-        for (int k = 0; k < 32; k += 8)
+      for (int k = 2; k < 32; k += 2)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            m4[j] = max3(m4[j], __uint_as_float(v[c][k + 2 * j]), __uint_as_float(v[c][k + 2 * j + 1]));
-      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        for (int c = 0; c < 4; ++c) m4[c] = max3(m4[c], __uint_as_float(v[c][k]), __uint_as_float(v[c][k + 1]));
+      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * row_unit;
       // the reference rises only when it must (or at the first visible key)
       float factor = 1.0f;
       bool rescale = false;
@@ -550,11 +638,12 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         m_ref = mx;
         l *= factor;
       }
-      const float m_use = m_ref <= -1e29f ? 0.f : m_ref;
-      // Two keys in eight take their exponentials on the FMA pipe, the others on the special-function unit.
+      const float offset = m_ref <= -1e29f ? 0.f : -m_ref;
+      const float2 off2 = make_float2(offset, offset);
+      // Two keys in eight take their exponentials on the FMA pipe, the others on the special-function unit; in a tile with
+      // masked keys all do, for whose scores its result is exactly zero.
       float2 s8[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      const float2 nm2 = make_float2(-m_use, -m_use);
-      if (full) {
+      auto exponentials = [&](auto all_sfu) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -562,42 +651,23 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
             float2 p[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              p[j] = __fadd2_rn(make_float2(__uint_as_float(v[c][k + 2 * j]), __uint_as_float(v[c][k + 2 * j + 1])), nm2);
+              p[j] = __ffma2_rn(make_float2(__uint_as_float(v[c][k + 2 * j]), __uint_as_float(v[c][k + 2 * j + 1])), unit2, off2);
 #pragma unroll
-            for (int j = 0; j < 3; ++j) p[j] = make_float2(fast_exp2(p[j].x), fast_exp2(p[j].y));
-            p[3] = exp2_fma2(p[3]);
-#pragma unroll
-            for (int j = 0; j < 4; j += 2) {
-              const float4 w = *reinterpret_cast<const float4*>(vs + c * 32 + k + 2 * j);
-              s8[j] = __fadd2_rn(s8[j], p[j]);
-              s8[j + 1] = __fadd2_rn(s8[j + 1], p[j + 1]);
-              const float2 y0 = __fmul2_rn(p[j], make_float2(w.x, w.y)), y1 = __fmul2_rn(p[j + 1], make_float2(w.z, w.w));
-              v[c >> 1][(c & 1) * 16 + (k >> 1) + j] = pack_bf16(y0.x, y0.y);      // 64 packed pairs in v[0], v[1]
-              v[c >> 1][(c & 1) * 16 + (k >> 1) + j + 1] = pack_bf16(y1.x, y1.y);
-            }
-          }
-      } else {
-        // a tile with masked keys: every exponential on the special-function unit, whose result for a masked score is
-        // exactly zero; the scale of a masked key may be no number
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            const float4 w = *reinterpret_cast<const float4*>(vs + c * 32 + k);
-            const float wk[4] = {w.x, w.y, w.z, w.w};
-            float pj[4], y[4];
+            for (int j = 0; j < 4; ++j)
+              p[j] = j == 3 && !all_sfu.value ? exp2_fma2(p[j]) : make_float2(fast_exp2(p[j].x), fast_exp2(p[j].y));
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              pj[j] = fast_exp2(__uint_as_float(v[c][k + j]) - m_use);
-              y[j] = __uint_as_float(v[c][k + j]) == NEG_BIG ? 0.f : pj[j] * wk[j];
+              s8[j] = __fadd2_rn(s8[j], p[j]);
+              v[c >> 1][(c & 1) * 16 + (k >> 1) + j] = pack_bf16(p[j].x, p[j].y);      // 64 packed pairs in v[0], v[1]
             }
-            s8[(k >> 1) & 2] = __fadd2_rn(s8[(k >> 1) & 2], make_float2(pj[0], pj[1]));
-            s8[((k >> 1) & 2) + 1] = __fadd2_rn(s8[((k >> 1) & 2) + 1], make_float2(pj[2], pj[3]));
-            v[c >> 1][(c & 1) * 16 + (k >> 1)] = pack_bf16(y[0], y[1]);
-            v[c >> 1][(c & 1) * 16 + (k >> 1) + 1] = pack_bf16(y[2], y[3]);
           }
-      }
+      };
+      if (unmasked) exponentials(std::false_type()); else exponentials(std::true_type());
       l += ((s8[0].x + s8[0].y) + (s8[1].x + s8[1].y)) + ((s8[2].x + s8[2].y) + (s8[3].x + s8[3].y));
+      if (nan->any) {      // a visible key that is no number: so is the row's result
+        for (int k = max(first, 0); k <= min(last, TILE - 1); ++k)
+          if (nan->key[k & 3] >> (k >> 2) & 1) l = __int_as_float(0x7fc00000);
+      }
       // O of this tile is rescaled when a row of the warp raised its reference.  Its last product completed before these
       // scores did, except where the tile runs alone: the product of i - 1 is waited for there.
       if (__any_sync(0xffffffffu, rescale)) {
@@ -621,14 +691,15 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
       tc_st32(tmem_s + 32, v[1]);
       tc_wait_st();
       tc_fence_before();
-      mbar_arrive(&p_full[buf]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[buf]);
     }
-    if (ok && jl[x] >= jf[x]) {
+    if (ok && i_last >= i_first) {
       ok = mbar_wait(&o_final[x], 0);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
-      const long long row = (long long)(q_begin + tokx[x] + tl) * a.Hq + kvh * G + g;
-      if (ok && !whole[x]) {
+      const long long row = (long long)(q_begin + tok0 + tl) * a.Hq + kvh * G + g;
+      if (ok && !(x ? whole[1] : whole[0])) {
         // a partial result of this chunk: O as accumulated (against m_ref), m_ref, l
         const long long at = row * a.max_chunks + chunk;
 #pragma unroll
@@ -651,14 +722,13 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
           unsigned o[32];
           tc_ld32(tmem_o + c * 32, o);
           tc_wait_ld();
+          auto value = [&](int e) { return __uint_as_float(o[e]) * inv; };
 #pragma unroll
           for (int ch = 0; ch < 4; ++ch)
             if (valid && c * 32 + ch * 8 < a.D)
               *reinterpret_cast<uint4*>(out + row * a.D + c * 32 + ch * 8) =
-                  make_uint4(pack_bf16(__uint_as_float(o[ch * 8]) * inv, __uint_as_float(o[ch * 8 + 1]) * inv),
-                             pack_bf16(__uint_as_float(o[ch * 8 + 2]) * inv, __uint_as_float(o[ch * 8 + 3]) * inv),
-                             pack_bf16(__uint_as_float(o[ch * 8 + 4]) * inv, __uint_as_float(o[ch * 8 + 5]) * inv),
-                             pack_bf16(__uint_as_float(o[ch * 8 + 6]) * inv, __uint_as_float(o[ch * 8 + 7]) * inv));
+                  make_uint4(pack_bf16(value(ch * 8), value(ch * 8 + 1)), pack_bf16(value(ch * 8 + 2), value(ch * 8 + 3)),
+                             pack_bf16(value(ch * 8 + 4), value(ch * 8 + 5)), pack_bf16(value(ch * 8 + 6), value(ch * 8 + 7)));
         }
       }
     }
@@ -792,7 +862,7 @@ int dib_int8_attention_prompt(const void* q, void* out, const void* data, const 
           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return DIB_LAUNCH_FAILED;
-  static_assert(S_TOTAL + 512 <= S_DYNAMIC, "shared memory");
+  static_assert(S_DYNAMIC <= 232448, "shared memory");
   static DeviceOnce attr_set;
   if (!attr_set.done()) {
     if (cudaFuncSetAttribute(attention_prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S_DYNAMIC) != cudaSuccess)
