@@ -30,9 +30,9 @@
 
 namespace {
 
-constexpr int TILE = 128, SOFTMAX_WARPS = 8, COPY_WARP = 8, MMA_WARP = 9, CONVERT_WARP = 10, CONVERTERS = 6;
+constexpr int TILE = 128, SOFTMAX_WARPS = 8, COPY_WARP = 8, MMA_WARP = 9, CONVERTERS = 6;
 constexpr int THREADS = 512, SOFTMAX = SOFTMAX_WARPS * 32;
-constexpr int REGS_FEW = 56, REGS_MANY = 200;         // 256 * 56 + 256 * 200 = 512 * 128
+constexpr int REGS_FEW = 64, REGS_MANY = 192;         // 256 * 64 + 256 * 192 = 512 * 128
 constexpr int TILE_BYTES = 128 * 128 * 2, HALF_BYTES = 128 * 64 * 2;      // a bfloat16 tile: two halves of 64 columns
 constexpr int RAW_BYTES = 128 * 128;
 constexpr float NEG_BIG = -1e30f;
@@ -82,21 +82,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
-}
-// 2^x for x <= ~8, two values at once on the FMA and integer pipes: the nearest integer by its exponent bits, the rest by a
-// cubic (relative error 1e-4, below the bfloat16 step of the probabilities).
-__device__ __forceinline__ float2 exp2_fma2(float2 x) {
-  x.x = fmaxf(x.x, -125.0f);
-  x.y = fmaxf(x.y, -125.0f);
-  const float2 magic = make_float2(12582912.0f, 12582912.0f);
-  const float2 xf = __fadd2_rn(x, magic);
-  const float2 t = __fadd2_rn(xf, make_float2(-12582912.0f, -12582912.0f));
-  const float2 f = __ffma2_rn(t, make_float2(-1.0f, -1.0f), x);
-  float2 p = __ffma2_rn(f, make_float2(0.05500893f, 0.05500893f), make_float2(0.24221095f, 0.24221095f));
-  p = __ffma2_rn(p, f, make_float2(0.6932829f, 0.6932829f));
-  p = __ffma2_rn(p, f, make_float2(1.0f, 1.0f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(xf.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (__float_as_int(xf.y) << 23)));
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -167,6 +152,16 @@ __device__ __forceinline__ void tc_st32(unsigned taddr, const unsigned (&r)[32])
       "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tc_ld8(unsigned taddr, unsigned (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tc_st8(unsigned taddr, const unsigned (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 // Descriptors (rows of 128 bytes, 128-byte swizzle, 8-row groups 1,024 bytes apart): K-major; MN-major, the next 64 columns
 // half a tile on.
 __device__ __forceinline__ unsigned long long desc_k_major(unsigned addr) {
@@ -234,9 +229,9 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
   unsigned long long* sc_full = bars + 12;        // [SLOTS] the scales of a key tile are there
   unsigned long long* sc_empty = bars + 16;       // [SLOTS] its outputs have been made
   unsigned long long* s_full = bars + 20;         // [A, B] the query tile's scores are in tensor memory
-  unsigned long long* p_full = bars + 22;         // [2] its probabilities are, and O is rescaled (a warp each)
-  unsigned long long* o_final = bars + 24;        // [2] its last product has completed
-  unsigned long long* pv_done = bars + 26;        // an output product of the tile that runs alone has completed
+  unsigned long long* p_full = bars + 22;         // [2][2] half of its probabilities are, and O is rescaled (a warp each)
+  unsigned long long* o_final = bars + 26;        // [2] its last product has completed
+  unsigned long long* pv_done = bars + 28;        // an output product of the tile that runs alone has completed
   unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 30);
   if (threadIdx.x == 0) prefetch_tensormap(&map);
   pdl_trigger();
@@ -322,7 +317,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&s_full[i], 1);
-        mbar_init(&p_full[i], SOFTMAX_WARPS / 2);
+        mbar_init(&p_full[2 * i], SOFTMAX_WARPS / 2);
+        mbar_init(&p_full[2 * i + 1], SOFTMAX_WARPS / 2);
         mbar_init(&o_final[i], 1);
       }
       mbar_init(pv_done, 1);
@@ -403,15 +399,23 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         }
         tc_commit(elected, &s_full[buf]);
       };
-      auto issue_o = [&](int x, int buf, int i) {      // outputs of query tile x from the probabilities in buf
+      int uses[2] = {0, 0};     // completed phases of p_full
+      // outputs of query tile x from the probabilities in buf, each half as soon as it is there
+      auto issue_o = [&](int x, int buf, int i) {
         const unsigned long long vd = v_desc + ((2 * i + 1) % RING) * (TILE_BYTES >> 4);
         const bool first = j0 + i == (x ? jf[1] : jf[0]);
+        const int turn = (buf ? uses[1]++ : uses[0]++) & 1;
 #pragma unroll
-        for (int ks = 0; ks < TILE / 16; ++ks)
-          tc_mma_ts(elected, tmem + 256 + x * 128, tmem + buf * 128 + ks * 8, vd + (unsigned long long)((ks * 16 * 128) >> 4), idesc_o,
-                    !first || ks > 0);
+        for (int half = 0; half < 2; ++half) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&p_full[2 * buf + half], turn));
+          if (!ok) return;
+          tc_fence_after();
+#pragma unroll
+          for (int ks = half * 4; ks < half * 4 + 4; ++ks)
+            tc_mma_ts(elected, tmem + 256 + x * 128, tmem + buf * 128 + ks * 8, vd + (unsigned long long)((ks * 16 * 128) >> 4),
+                      idesc_o, !first || ks > 0);
+        }
       };
-      int uses[2] = {0, 0};     // completed phases of p_full
       auto want = [&](int item) {
         ok = __all_sync(0xffffffffu, mbar_wait(&full[item % RING], (item / RING) & 1));
         tc_fence_after();
@@ -428,11 +432,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           if (active(x, i)) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&p_full[x], uses[x] & 1));
-            if (!ok) break;
-            ++uses[x];
-            tc_fence_after();
             issue_o(x, x, i);
+            if (!ok) break;
             if (j0 + i == jl[x]) tc_commit(elected, &o_final[x]);
           }
           if (x == 1) {
@@ -453,11 +454,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
           tc_commit(elected, &empty[(2 * i + 2) % RING]);
         }
         if (!want(2 * i + 1)) break;
-        ok = __all_sync(0xffffffffu, mbar_wait(&p_full[buf], (buf ? uses[1] : uses[0]) & 1));
-        if (!ok) break;
-        if (buf) ++uses[1]; else ++uses[0];
-        tc_fence_after();
         issue_o(x, buf, i);
+        if (!ok) break;
         tc_commit(elected, &empty[(2 * i + 1) % RING]);
         tc_commit(elected, &sc_empty[i % SLOTS]);
         tc_commit(elected, pv_done);
@@ -527,16 +525,18 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
     for (int item = max(0, sent - RING); item < sent; ++item)
       if (!mbar_wait(&raw_full[item % RING], (item / RING) & 1)) ok = false;
   } else {
-    // ---- conversion.  A warp takes 8 rows x 64 codes at a time: eight lanes a pair of rows r, r ^ 5, whose pieces lie in
-    // different banks in the bytes' swizzle and in the 16-bit tile's.
-    const int r8 = lane & 4 ? (lane >> 3) ^ 5 : lane >> 3, p4 = lane & 3;
+    // ---- conversion.  A warp has the even or the odd 64 codes of some groups of 8 rows; eight lanes a pair of rows r, r ^ 5,
+    // whose pieces lie in different banks in the bytes' swizzle and in the 16-bit tile's.  Warps 12 and 13 have half of the
+    // groups: the others are two to a scheduler.
+    const int r8 = lane & 4 ? (lane >> 3) ^ 5 : lane >> 3, p = (warp & 1) * 4 + (lane & 3);
+    const int g_from = warp < 12 ? 0 : warp < 14 ? 4 : 12, g_to = warp < 12 ? 4 : warp < 14 ? 12 : 16;
+    const int src_off = r8 * 128 + ((p ^ r8) << 4), dst_off0 = piece_off(r8, 2 * p), dst_off1 = piece_off(r8, 2 * p + 1);
     auto convert = [&](const unsigned char* src, unsigned char* dst, const float* vs, auto keys) {
 #pragma unroll 2
-      for (int u = warp - CONVERT_WARP; u < 32; u += CONVERTERS) {
-        const int row = (u >> 1) * 8 + r8, p = (u & 1) * 4 + p4;
-        const uint4 w = *reinterpret_cast<const uint4*>(src + row * 128 + ((p ^ (row & 7)) << 4));
+      for (int g8 = g_from; g8 < g_to; ++g8) {
+        const uint4 w = *reinterpret_cast<const uint4*>(src + src_off + g8 * 1024);
         const unsigned turned[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
-        const float scale = keys.value ? 0.f : vs[row];
+        const float scale = keys.value ? 0.f : vs[g8 * 8 + r8];
         const float2 scale2 = make_float2(scale, scale);
         unsigned y[8];
 #pragma unroll
@@ -544,8 +544,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
           y[2 * e] = keys.value ? codes_f16(turned[e], 0x4140) : codes_bf16(turned[e], 0x7540, scale2);
           y[2 * e + 1] = keys.value ? codes_f16(turned[e], 0x4342) : codes_bf16(turned[e], 0x7542, scale2);
         }
-        *reinterpret_cast<uint4*>(dst + piece_off(row, 2 * p)) = make_uint4(y[0], y[1], y[2], y[3]);
-        *reinterpret_cast<uint4*>(dst + piece_off(row, 2 * p + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+        *reinterpret_cast<uint4*>(dst + dst_off0 + g8 * 1024) = make_uint4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<uint4*>(dst + dst_off1 + g8 * 1024) = make_uint4(y[4], y[5], y[6], y[7]);
       }
     };
     for (int item = 0, at = 0, turn = 0; item < 2 * ntiles && ok; ++item) {
@@ -594,7 +594,6 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
       if (borrowed) ++uses_other; else ++uses_own;
       tc_fence_after();
       const int kbase = (j0 + i) * TILE, first = lo - kbase, last = hi - kbase;      // visible: [first, last]
-      const bool unmasked = first <= 0 && last >= TILE - 1;
       const float* ks = scales + (i % SLOTS) * 256;
       const NanKeys* nan = nan_keys + i % SLOTS;
       unsigned v[4][32];
@@ -611,7 +610,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
           v[c][k] = __float_as_uint(y0.x); v[c][k + 1] = __float_as_uint(y0.y);
           v[c][k + 2] = __float_as_uint(y1.x); v[c][k + 3] = __float_as_uint(y1.y);
         }
-      if (!unmasked) {
+      if (first > 0 || last < TILE - 1) {
         // keys outside [first, last]: one subtraction and one unsigned comparison each
         const int first_vis = last >= first ? first : (1 << 20);
         const unsigned span = last >= first ? (unsigned)(last - first) : 0u;
@@ -629,6 +628,10 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
 #pragma unroll
         for (int c = 0; c < 4; ++c) m4[c] = max3(m4[c], __uint_as_float(v[c][k]), __uint_as_float(v[c][k + 1]));
       const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * row_unit;
+      if (nan->any) {      // a visible key that is no number: so is the row's result
+        for (int k = max(first, 0); k <= min(last, TILE - 1); ++k)
+          if (nan->key[k & 3] >> (k >> 2) & 1) l = __int_as_float(0x7fc00000);
+      }
       // the reference rises only when it must (or at the first visible key)
       float factor = 1.0f;
       bool rescale = false;
@@ -637,36 +640,6 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         factor = rescale ? fast_exp2(m_ref - mx) : 0.f;
         m_ref = mx;
         l *= factor;
-      }
-      const float offset = m_ref <= -1e29f ? 0.f : -m_ref;
-      const float2 off2 = make_float2(offset, offset);
-      // Two keys in eight take their exponentials on the FMA pipe, the others on the special-function unit; in a tile with
-      // masked keys all do, for whose scores its result is exactly zero.
-      float2 s8[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      auto exponentials = [&](auto all_sfu) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int k = 0; k < 32; k += 8) {
-            float2 p[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              p[j] = __ffma2_rn(make_float2(__uint_as_float(v[c][k + 2 * j]), __uint_as_float(v[c][k + 2 * j + 1])), unit2, off2);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              p[j] = j == 3 && !all_sfu.value ? exp2_fma2(p[j]) : make_float2(fast_exp2(p[j].x), fast_exp2(p[j].y));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              s8[j] = __fadd2_rn(s8[j], p[j]);
-              v[c >> 1][(c & 1) * 16 + (k >> 1) + j] = pack_bf16(p[j].x, p[j].y);      // 64 packed pairs in v[0], v[1]
-            }
-          }
-      };
-      if (unmasked) exponentials(std::false_type()); else exponentials(std::true_type());
-      l += ((s8[0].x + s8[0].y) + (s8[1].x + s8[1].y)) + ((s8[2].x + s8[2].y) + (s8[3].x + s8[3].y));
-      if (nan->any) {      // a visible key that is no number: so is the row's result
-        for (int k = max(first, 0); k <= min(last, TILE - 1); ++k)
-          if (nan->key[k & 3] >> (k >> 2) & 1) l = __int_as_float(0x7fc00000);
       }
       // O of this tile is rescaled when a row of the warp raised its reference.  Its last product completed before these
       // scores did, except where the tile runs alone: the product of i - 1 is waited for there.
@@ -678,21 +651,35 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
           tc_fence_after();
         }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tc_ld32(tmem_o + c * 32, v[2]);
+        for (int c = 0; c < 16; ++c) {
+          unsigned o[8];
+          tc_ld8(tmem_o + c * 8, o);
           tc_wait_ld();
 #pragma unroll
-          for (int k = 0; k < 32; ++k)
-            v[2][k] = __float_as_uint(__uint_as_float(v[2][k]) * (rescale ? factor : 1.0f));
-          tc_st32(tmem_o + c * 32, v[2]);
+          for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * (rescale ? factor : 1.0f));
+          tc_st8(tmem_o + c * 8, o);
         }
       }
-      tc_st32(tmem_s, v[0]);          // probabilities over the scores they came from
-      tc_st32(tmem_s + 32, v[1]);
-      tc_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[buf]);
+      const float offset = m_ref <= -1e29f ? 0.f : -m_ref;
+      const float2 off2 = make_float2(offset, offset);
+      float2 s8[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int k = 0; k < 64; k += 2) {
+          const int c = half * 2 + (k >> 5);
+          const float2 y = __ffma2_rn(make_float2(__uint_as_float(v[c][k & 31]), __uint_as_float(v[c][(k & 31) + 1])), unit2, off2);
+          const float2 p = make_float2(fast_exp2(y.x), fast_exp2(y.y));      // (exactly zero for a masked score)
+          s8[(k >> 1) & 3] = __fadd2_rn(s8[(k >> 1) & 3], p);
+          v[half][k >> 1] = pack_bf16(p.x, p.y);
+        }
+        tc_st32(tmem_s + half * 32, v[half]);      // probabilities over the scores they came from
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * buf + half]);
+      }
+      l += ((s8[0].x + s8[0].y) + (s8[1].x + s8[1].y)) + ((s8[2].x + s8[2].y) + (s8[3].x + s8[3].y));
     }
     if (ok && i_last >= i_first) {
       ok = mbar_wait(&o_final[x], 0);
