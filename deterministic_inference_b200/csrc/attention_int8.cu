@@ -78,18 +78,35 @@ __device__ __forceinline__ void mbar_arrive(unsigned long long* bar) {
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(unsigned long long* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void tc_mma_i8(unsigned tmem_d, unsigned long long desc_a, unsigned long long desc_b, unsigned idesc,
-                                          unsigned accum) {
+// Issued by one lane, in code that the whole warp runs: what they are given stays in uniform registers.
+__device__ __forceinline__ unsigned elect_one() {
+  unsigned is;
   asm volatile(
       "{\n\t"
       ".reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t"
+      "}\n" : "=r"(is));
+  return is;
+}
+__device__ __forceinline__ void tc_commit(unsigned elected, unsigned long long* bar) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred e;\n\t"
+      "setp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t"
+      "}\n" ::"r"(smem_u32(bar)), "r"(elected)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_i8(unsigned elected, unsigned tmem_d, unsigned long long desc_a, unsigned long long desc_b,
+                                          unsigned idesc, unsigned accum) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, e;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t"
-      "}\n" ::"r"(tmem_d),
-      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accum), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
+      "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accum), "r"(elected)
       : "memory");
 }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -244,7 +261,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
   unsigned long long* item_empty = bars + 16 + SP_ITEMS;      // [SP_ITEMS] it has been read by every role
   unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 16 + 2 * SP_ITEMS);
   int* first = reinterpret_cast<int*>(smem + SH::FIRST);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) prefetch_tensormap(&map);
   if (!a.late) pdl_trigger();
   // ---- the work before each sequence (metadata alone, which no kernel of a step writes)
@@ -293,7 +310,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const unsigned tmem = *tmem_slot;
+  const unsigned tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const int G = a.Hq / a.Hkv;
   pdl_wait(q);
   bool ok = true;
@@ -353,59 +370,63 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
     if (ok && n > 0) send_values(n - 1);
   } else if (warp == SP_SCORE_WARP) {
     // ---- scores: a tile ahead of the softmax
-    if (lane == 0) {
+    {
+      const unsigned elected = elect_one();
       constexpr unsigned idesc = idesc_i8(128, N, 0);
       const unsigned base = smem_u32(smem);
       int n = 0, q_used = -1;
       for (int k = 0; ok; ++k) {
         const int slot = k % SP_ITEMS;
-        ok = mbar_wait(&item_full[slot], (k / SP_ITEMS) & 1);
+        ok = __all_sync(0xffffffffu, mbar_wait(&item_full[slot], (k / SP_ITEMS) & 1));
         if (!ok) break;
         const int tiles = items[slot].tiles, fresh = items[slot].fresh;
-        mbar_arrive(&item_empty[slot]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[slot]);
         if (tiles == 0) break;
         if (fresh) {
-          if (q_used >= 0) tc_commit(&q_empty[q_used & 1]);
+          if (q_used >= 0) tc_commit(elected, &q_empty[q_used & 1]);
           ++q_used;
-          ok = mbar_wait(&q_full[q_used & 1], (q_used >> 1) & 1);
+          ok = __all_sync(0xffffffffu, mbar_wait(&q_full[q_used & 1], (q_used >> 1) & 1));
           if (!ok) break;
         }
         const unsigned long long qd = desc_sw128(base + SH::QUERIES + (q_used & 1) * N * 128);
         for (int t = tiles; t > 0 && ok; --t, ++n) {
-          ok = mbar_wait(&k_full[n & 1], (n >> 1) & 1) && (n < 2 || mbar_wait(&s_empty[n & 1], ((n >> 1) - 1) & 1));
+          ok = __all_sync(0xffffffffu, mbar_wait(&k_full[n & 1], (n >> 1) & 1) && (n < 2 || mbar_wait(&s_empty[n & 1], ((n >> 1) - 1) & 1)));
           if (!ok) break;
           tc_fence_after();
           const unsigned long long kd = desc_sw128(base + (n & 1) * SH::STAGE);
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) tc_mma_i8(tmem + (n & 1) * N, kd + ks * 2, qd + ks * 2, idesc, ks > 0);
-          tc_commit(&s_full[n & 1]);
+          for (int ks = 0; ks < 4; ++ks) tc_mma_i8(elected, tmem + (n & 1) * N, kd + ks * 2, qd + ks * 2, idesc, ks > 0);
+          tc_commit(elected, &s_full[n & 1]);
         }
       }
     }
   } else if (warp == SP_OUTPUT_WARP) {
     // ---- outputs, as soon as a tile's weights are there
-    if (lane == 0) {
+    {
+      const unsigned elected = elect_one();
       constexpr unsigned idesc = idesc_i8(128, N, 1);
       const unsigned base = smem_u32(smem);
       const unsigned long long weights = desc_columns16(base + SH::WEIGHTS);
       int n = 0;
       for (int k = 0; ok; ++k) {
         const int slot = k % SP_ITEMS;
-        ok = mbar_wait(&item_full[slot], (k / SP_ITEMS) & 1);
+        ok = __all_sync(0xffffffffu, mbar_wait(&item_full[slot], (k / SP_ITEMS) & 1));
         if (!ok) break;
         const int tiles = items[slot].tiles;
-        mbar_arrive(&item_empty[slot]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[slot]);
         if (tiles == 0) break;
         for (int t = tiles; t > 0 && ok; --t, ++n) {
-          ok = mbar_wait(&v_full[n & 1], (n >> 1) & 1) && mbar_wait(p_full, n & 1);
+          ok = __all_sync(0xffffffffu, mbar_wait(&v_full[n & 1], (n >> 1) & 1) && mbar_wait(p_full, n & 1));
           if (!ok) break;
           tc_fence_after();
           const unsigned long long vd = desc_sw128(base + (n & 1) * SH::STAGE + SP_TILE * 128);
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
-            tc_mma_i8(tmem + 2 * N, vd + ks * (4096 >> 4), weights + ks * (512 >> 4), idesc, ks > 0);
-          tc_commit(o_full);
-          tc_commit(&v_empty[n & 1]);
+            tc_mma_i8(elected, tmem + 2 * N, vd + ks * (4096 >> 4), weights + ks * (512 >> 4), idesc, ks > 0);
+          tc_commit(elected, o_full);
+          tc_commit(elected, &v_empty[n & 1]);
         }
       }
     }

@@ -160,33 +160,55 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-template <bool PAIR> __device__ __forceinline__ void tc_commit(unsigned long long* bar) {
+// Issued by one lane, in code that the whole warp runs: what they are given stays in uniform registers.
+__device__ __forceinline__ unsigned elect_one() {
+  unsigned is;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t"
+      "}\n" : "=r"(is));
+  return is;
+}
+template <bool PAIR> __device__ __forceinline__ void tc_commit(unsigned elected, unsigned long long* bar) {
   if (PAIR)
     asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-        ::"r"(smem_u32(bar)), "h"((unsigned short)3)
+        "{\n\t"
+        ".reg .pred e;\n\t"
+        "setp.ne.b32 e, %2, 0;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t"
+        "}\n" ::"r"(smem_u32(bar)), "h"((unsigned short)3), "r"(elected)
         : "memory");
   else
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    asm volatile(
+        "{\n\t"
+        ".reg .pred e;\n\t"
+        "setp.ne.b32 e, %1, 0;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t"
+        "}\n" ::"r"(smem_u32(bar)), "r"(elected)
+        : "memory");
 }
 template <bool PAIR>
-__device__ __forceinline__ void tc_mma(unsigned tmem_d, unsigned long long desc_a, unsigned long long desc_b, unsigned idesc,
-                                       unsigned accum) {
+__device__ __forceinline__ void tc_mma(unsigned elected, unsigned tmem_d, unsigned long long desc_a, unsigned long long desc_b,
+                                       unsigned idesc, unsigned accum) {
   if (PAIR)
     asm volatile(
         "{\n\t"
-        ".reg .pred p;\n\t"
+        ".reg .pred p, e;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
-        "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accum)
+        "setp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
+        "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accum), "r"(elected)
         : "memory");
   else
     asm volatile(
         "{\n\t"
-        ".reg .pred p;\n\t"
+        ".reg .pred p, e;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
-        "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accum)
+        "setp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
+        "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accum), "r"(elected)
         : "memory");
 }
 __device__ __forceinline__ void tc_ld32(unsigned taddr, unsigned (&r)[32]) {
@@ -325,7 +347,7 @@ gemm_large_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     prefetch_tensormap(&map_w);
     prefetch_tensormap(&map_out);
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = PAIR ? (int)cluster_rank() : 0;
   const int group = blockIdx.x / CTAS, groups = gridDim.x / CTAS;
   const int tiles = a.m_tiles * a.n_tiles;
@@ -353,7 +375,7 @@ gemm_large_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
   __syncthreads();
   if (PAIR) cluster_sync_all();       // both CTAs' barriers and tensor memory exist before either is used
   tc_fence_after();
-  const unsigned tmem = *tmem_slot;
+  const unsigned tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   bool ok = true;
 
   if (warp == 0) {
@@ -390,29 +412,30 @@ gemm_large_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       // ---- products
+      const unsigned elected = elect_one();
       constexpr unsigned idesc = make_idesc(CTAS * BM, BNL);
       int count = 0, local = 0;
       for (int t = group; t < tiles && ok; t += groups, ++local) {
         const int buf = local & 1;
         if (local >= 2) {      // the epilogue must have read this buffer's earlier tile
-          ok = mbar_wait(&acc_empty[buf], ((local >> 1) - 1) & 1);
+          ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((local >> 1) - 1) & 1));
           if (!ok) break;
           tc_fence_after();
         }
         for (int kb = 0; kb < a.num_kb && ok; ++kb, ++count) {
           const int s = count % STAGES;
-          ok = mbar_wait(&full[s], (count / STAGES) & 1);
+          ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (count / STAGES) & 1));
           if (!ok) break;
           tc_fence_after();
           const unsigned long long da = smem_desc(smem_u32(smem + s * STAGE)), db = smem_desc(smem_u32(smem + s * STAGE) + A_BYTES);
 #pragma unroll
           for (int k = 0; k < BK / UMMA_K; ++k)
-            tc_mma<PAIR>(tmem + buf * BNL, da + k * (UMMA_K >> 4), db + k * (UMMA_K >> 4), idesc, (kb > 0 || k > 0) ? 1u : 0u);
-          tc_commit<PAIR>(&empty[s]);
+            tc_mma<PAIR>(elected, tmem + buf * BNL, da + k * (UMMA_K >> 4), db + k * (UMMA_K >> 4), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+          tc_commit<PAIR>(elected, &empty[s]);
         }
-        if (ok) tc_commit<PAIR>(&acc_full[buf]);
+        if (ok) tc_commit<PAIR>(elected, &acc_full[buf]);
       }
     }
   } else if (warp >= EPI_WARP0) {
