@@ -12,10 +12,13 @@
 // Many rows: persistent kernels on the 5th-generation tensor cores (tcgen05.mma kind::i8), one CTA an SM on tiles of 128
 // tokens x BNL channels, or a pair of CTAs (cta_group::2) on tiles of 256 x 256: each then fetches its own 128 token rows
 // and half of the channels, a third less for the same products, and the rate at which L2 feeds the SMs bounds them.
+// Some rows: clusters of up to eight CTAs share a tile's k (see gemm_split_kernel).
 // Operands by TMA (128 k a stage: rows of 128 bytes, 128-byte swizzle) through a ring of mbarrier-guarded stages, the
 // accumulator twice in tensor memory, so that a tile's epilogue (integers to float32, the two scales, one rounding) runs
 // under the products of the next.  Roles: warp 0 copies, warp 1 issues the products, warps 4-11 are the epilogue.
 #include <cuda.h>
+
+#include <atomic>
 
 #include "common.cuh"
 
@@ -248,6 +251,14 @@ __device__ __forceinline__ unsigned cluster_addr(unsigned local, unsigned rank) 
   return r;
 }
 
+__device__ __forceinline__ int cluster_size() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return (int)r;
+}
+__device__ __forceinline__ void store_as(float& to, float x) { to = x; }
+__device__ __forceinline__ void store_as(__nv_bfloat16& to, float x) { to = __float2bfloat16_rn(x); }
+
 struct LargeArgs {
   const float* sx;      // [M]
   const float* sw;      // [N]
@@ -476,6 +487,155 @@ gemm_large_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
   }
 }
 
+// Some rows (more than the streamed weight likes, fewer than fill the GPU with tiles): a cluster of S CTAs has a tile of 128
+// tokens x BNL channels, each a run of the k-blocks; then each adds up the S integers of some of the columns (a thread a
+// token's 8 columns) from the others' shared memory and writes them.  Only the token rows that there are, rounded up to
+// a_rows, are fetched; what the products make of the rows behind them is never read.
+constexpr int SPLIT_THREADS = 256, SPLIT_MAX = 8, SPLIT_RING = 192 * 1024;
+struct SplitArgs {
+  const float* sx;
+  const float* sw;
+  void* out;
+  int M, N, num_kb, a_rows, stages;
+  int by_lines;
+};
+template <int BNL> struct SplitShape {
+  static constexpr int SUM_ROW = BNL * 4 + 16;      // a token's integers, 16 bytes off: no two of a warp's rows share banks
+};
+__device__ __forceinline__ int4 load_cluster(unsigned addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+template <typename OutT, int BNL>
+__global__ void __launch_bounds__(SPLIT_THREADS)
+gemm_split_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                  const __grid_constant__ SplitArgs a) {
+  constexpr int SUM_ROW = SplitShape<BNL>::SUM_ROW;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ unsigned long long full[16], empty[16], acc_full;
+  __shared__ unsigned tmem_slot;
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&map_x);
+    prefetch_tensormap(&map_w);
+  }
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = (int)cluster_rank(), split = cluster_size();
+  const int n0 = blockIdx.x / split * BNL, m0 = blockIdx.y * BM;
+  const int kb0 = rank * a.num_kb / split, count = (rank + 1) * a.num_kb / split - kb0;
+  const int b_bytes = BNL * BK, stage = b_bytes + a.a_rows * BK;
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&acc_full, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"((unsigned)BNL));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const unsigned tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
+  bool ok = true;
+  if (warp == 0) {
+    if (lane == 0) {
+      auto load_w = [&](int c) {
+        const int s = c % a.stages;
+        mbar_expect_tx(&full[s], stage);
+        tma_load_2d<false>(smem + s * stage, &map_w, (kb0 + c) * BK, n0, smem_u32(&full[s]));
+      };
+      auto load_x = [&](int c) {
+        const int s = c % a.stages;
+        tma_load_2d<false>(smem + s * stage + b_bytes, &map_x, (kb0 + c) * BK, m0, smem_u32(&full[s]));
+      };
+      const int pre = count < a.stages ? count : a.stages;
+      for (int c = 0; c < pre; ++c) load_w(c);      // weights are constants: the first stages' go out before the wait
+      pdl_wait();
+      for (int c = 0; c < pre; ++c) load_x(c);
+      for (int c = pre; c < count; ++c) {
+        ok = mbar_wait(&empty[c % a.stages], ((c / a.stages) - 1) & 1);
+        if (!ok) break;
+        load_w(c);
+        load_x(c);
+      }
+    }
+  } else if (warp == 1) {
+    const unsigned elected = elect_one();
+    constexpr unsigned idesc = make_idesc(BM, BNL);
+    for (int c = 0; c < count; ++c) {
+      const int s = c % a.stages;
+      ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (c / a.stages) & 1));
+      if (!ok) break;
+      tc_fence_after();
+      const unsigned long long db = smem_desc(smem_u32(smem) + s * stage), da = smem_desc(smem_u32(smem) + s * stage + b_bytes);
+#pragma unroll
+      for (int k = 0; k < BK / UMMA_K; ++k)
+        tc_mma<false>(elected, tmem, da + k * (UMMA_K >> 4), db + k * (UMMA_K >> 4), idesc, (c > 0 || k > 0) ? 1u : 0u);
+      tc_commit<false>(elected, &empty[s]);
+    }
+    if (ok) tc_commit<false>(elected, &acc_full);
+  } else if (warp >= 4) {
+    // ---- integers to shared memory, over the ring: all of its copies have been read
+    const int row = (warp - 4) * 32 + lane;
+    if ((warp - 4) * 32 < a.a_rows) {
+      ok = mbar_wait(&acc_full, 0);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      if (ok)
+#pragma unroll
+        for (int c = 0; c < BNL; c += 32) {
+          unsigned v[32];
+          tc_ld32(tmem + ((unsigned)((warp - 4) * 32) << 16) + c, v);
+          tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<uint4*>(smem + row * SUM_ROW + (c + j) * 4) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        }
+    }
+  }
+  if (!ok) atomicExch(&dib_gemm_int8_error_word, 1);
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync_all();
+  pdl_wait();
+  const unsigned base = smem_u32(smem);
+  const int rows = a.M - m0 < BM ? a.M - m0 : BM, groups = (BNL / 8 - rank + split - 1) / split;
+  for (int e = threadIdx.x; e < rows * groups; e += SPLIT_THREADS) {
+    const int group = e / rows, row = e - group * rows, col = (rank + group * split) * 8;
+    if (n0 + col >= a.N) continue;
+    int sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int r = 0; r < split; ++r) {
+      const unsigned from = cluster_addr(base + row * SUM_ROW + col * 4, r);
+      const int4 lo = load_cluster(from), hi = load_cluster(from + 16);
+      sum[0] += lo.x; sum[1] += lo.y; sum[2] += lo.z; sum[3] += lo.w;
+      sum[4] += hi.x; sum[5] += hi.y; sum[6] += hi.z; sum[7] += hi.w;
+    }
+    const float sx = a.sx[m0 + row];
+    alignas(16) OutT y[8];
+    const int left = a.N - (n0 + col);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < left) store_as(y[j], (float)sum[j] * sx * a.sw[n0 + col + j]);
+    OutT* out = reinterpret_cast<OutT*>(a.out) + (long long)(m0 + row) * a.N + n0 + col;
+    if (!a.by_lines && left >= 8) {
+#pragma unroll
+      for (int j = 0; j < 8 * (int)sizeof(OutT) / 16; ++j) reinterpret_cast<uint4*>(out)[j] = reinterpret_cast<const uint4*>(y)[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < left) out[j] = y[j];
+    }
+  }
+  cluster_sync_all();       // the others may still read this one's integers
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((unsigned)BNL));
+}
+
 // ---- host side
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -552,33 +712,137 @@ int launch_large(const void* x, const void* sx, const void* w, const void* sw, v
   return DIB_OK;
 }
 
+// (the products read 128 token rows whatever was fetched: the last stage's lie in the memory behind it)
+constexpr int SPLIT_SMEM = 1024 + SPLIT_RING + BM * BK;
+// A launch of clusters of `split` CTAs.
+struct SplitLaunch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  SplitLaunch(int split, int n_tiles, int m_tiles, cudaStream_t st) {
+    cfg.gridDim = dim3(split * n_tiles, m_tiles);
+    cfg.blockDim = dim3(SPLIT_THREADS);
+    cfg.dynamicSmemBytes = SPLIT_SMEM;
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = dib_pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = split;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+  }
+};
+// The CTAs that a tile's k is shared among: as many as leave all tiles running at once, two k-blocks for each at least.  A
+// cluster lies within a part of the GPU, so that 148 SMs hold fewer than 49 clusters of three: the driver is asked once.
+template <typename OutT, int BNL>
+int split_of(int tiles, int num_kb) {
+  auto kern = gemm_split_kernel<OutT, BNL>;
+  static DeviceOnce attr_set;
+  if (!attr_set.done()) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SPLIT_SMEM) != cudaSuccess) return 0;
+    attr_set.mark();
+  }
+  static std::atomic<int> resident[SPLIT_MAX + 1];
+  int split = num_kb / 2 < SPLIT_MAX ? num_kb / 2 : SPLIT_MAX;
+  for (; split > 1; --split) {
+    int n = resident[split].load(std::memory_order_relaxed);
+    if (n == 0) {
+      SplitLaunch launch(split, 1, 1, nullptr);
+      if (cudaOccupancyMaxActiveClusters(&n, kern, &launch.cfg) != cudaSuccess) return 0;
+      if (n < 1) n = 1;
+      resident[split].store(n, std::memory_order_relaxed);
+    }
+    if (n >= tiles) break;
+  }
+  return split < 1 ? 1 : split;
+}
+template <typename OutT, int BNL>
+int launch_split(const void* x, const void* sx, const void* w, const void* sw, void* out, int M, int N, int Kp, cudaStream_t st) {
+  SplitArgs a;
+  a.sx = reinterpret_cast<const float*>(sx);
+  a.sw = reinterpret_cast<const float*>(sw);
+  a.out = out;
+  a.M = M; a.N = N;
+  a.num_kb = (Kp + BK - 1) / BK;
+  a.a_rows = M <= 32 ? 32 : M <= 64 ? 64 : BM;
+  a.by_lines = ((long long)N * sizeof(OutT)) % 16 != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0;
+  const int m_tiles = (M + BM - 1) / BM, n_tiles = (N + BNL - 1) / BNL;
+  if (m_tiles > 65535 || n_tiles > 0x7fffffff / SPLIT_MAX) return DIB_BAD_SIZE;
+  const int stage = (BNL + a.a_rows) * BK;
+  a.stages = SPLIT_RING / stage < 16 ? SPLIT_RING / stage : 16;
+  static_assert(BM * SplitShape<BNL>::SUM_ROW <= SPLIT_RING && SPLIT_SMEM + 1024 <= 232448, "shared memory");
+  CUtensorMap mx, mw;
+  if (!make_map(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, M, Kp, a.a_rows) ||
+      !make_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, N, Kp, BNL))
+    return DIB_LAUNCH_FAILED;
+  const long long tiles = (long long)m_tiles * n_tiles;
+  const int split = split_of<OutT, BNL>(tiles < 0x7fffffff ? (int)tiles : 0x7fffffff, a.num_kb);
+  if (split < 1) return DIB_LAUNCH_FAILED;
+  SplitLaunch launch(split, n_tiles, m_tiles, st);
+  if (cudaLaunchKernelEx(&launch.cfg, gemm_split_kernel<OutT, BNL>, mx, mw, a) != cudaSuccess) return DIB_LAUNCH_FAILED;
+  DIB_CHECK_LAUNCH();
+  return DIB_OK;
+}
+
 // Form forced for measurements and tests (-1: the choice of `form`): 0 few rows, 1 tiles of 128 x 64, 2 of 128 x 128, 3 of
-// 128 x 256, 4 the pair.
+// 128 x 256, 4 the pair, 5 clusters on tiles of 128 x 64, 6 of 128 x 128.
 int& forced_form() {
   static int v = -1;
   return v;
 }
-// A function of the sizes and the SM count; the form never changes a bit of the result.
-int form(int M, int N, int sm_count) {
-  if (forced_form() >= 0) return forced_form();
-  // the streamed weight up to 16 rows, and up to 32 where its blocks of 16 channels are a few waves at most: its tokens come
-  // from L2 again for every block (4,096 x 4,096: 12.4 against 13.0 us at 32 rows; 24,576 x 4,096: 36.9 against 23.7)
-  if (M <= 16 || (M <= 32 && N <= 48 * sm_count)) return 0;
+// A function of the sizes and the GPU; the form never changes a bit of the result.
+int large_form(int M, int N, int sm_count) {
   const long long pair_tiles = (long long)((M + 2 * BM - 1) / (2 * BM)) * ((N + 255) / 256);
   if (sm_count >= 2 && M > BM && 3 * pair_tiles >= sm_count) return 4;
   const long long m_tiles = (M + BM - 1) / BM;
   if (m_tiles * ((N + 127) / 128) <= sm_count / 2) return 1;
   return 2 * m_tiles * ((N + 255) / 256) <= sm_count ? 2 : 3;
 }
+// Up to 256 rows the times of the forms are estimated, in us, from lines through measured ones (K-blocks of 128):
+//   streamed weight, 8 rows     1,024 x 1,024 1.8, 4,096 x 4,096 6.4, 24,576 x 4,096 20, 4,096 x 12,288 15, 5,120 x 25,600 30;
+//                               16, 24, 32 rows take 1.3, 1.85, 2 times that, as a block fetches its tokens from L2
+//   clusters, 128 wide          32 rows: 4,096 x 4,096 8.4, 6,144 x 4,096 9.6, 4,096 x 12,288 13.3, 5,120 x 25,600 26.5
+//                               128 rows: 13.5, 14.1, 18.4, 32.3
+//   clusters, 64 wide           32 rows: 2,560 x 4,096 8.0, 4,096 x 4,096 9.3; 128 rows: 10.1, 10.6
+//   a tile a CTA                4,096 x 4,096 12.7, 4,096 x 12,288 32, 5,120 x 25,600 65
+template <typename OutT>
+int form(int M, int N, int Kp, int sm_count) {
+  if (forced_form() >= 0) return forced_form();
+  const int large = large_form(M, N, sm_count);
+  if (M > 2 * BM) return large;
+  const int num_kb = (Kp + BK - 1) / BK, m_tiles = (M + BM - 1) / BM;
+  float best = 1e30f;
+  int choice = large;
+  auto consider = [&](int form, float us) {
+    if (us < best) {
+      best = us;
+      choice = form;
+    }
+  };
+  if (M <= 16 || (M <= 32 && N <= 48 * sm_count))
+    consider(0, (0.8f + 0.75e-3f * Kp + (float)N * Kp / 6.5e6f) * (M <= 8 ? 1.f : M <= 16 ? 1.3f : M <= 24 ? 1.85f : 2.f));
+  if (M > 16) {
+    const int width = large == 1 ? 64 : large == 2 ? 128 : 256, tiles = m_tiles * ((N + width - 1) / width);
+    consider(large, 2.8f + 0.31f * num_kb * ((tiles + sm_count - 1) / sm_count));
+  }
+  const int tiles64 = m_tiles * ((N + 63) / 64), tiles128 = m_tiles * ((N + 127) / 128);
+  const int s64 = 2 * tiles64 <= sm_count ? split_of<OutT, 64>(tiles64, num_kb) : 1;
+  const int s128 = 2 * tiles128 <= sm_count ? split_of<OutT, 128>(tiles128, num_kb) : 1;
+  if (s64 > 1) consider(5, 4.f + 0.33f * ((num_kb + s64 - 1) / s64) + (M > 64 ? 1.5f : M > 32 ? 0.5f : 0.f));
+  if (s128 > 1) consider(6, 4.f + 0.40f * ((num_kb + s128 - 1) / s128) + (M > 64 ? 5.f : M > 32 ? 1.7f : 0.f));
+  return choice;
+}
 
 template <typename OutT>
 int launch(const void* x, const void* sx, const void* w, const void* sw, void* out, int M, int N, int Kp, int sm_count,
            cudaStream_t st) {
-  switch (form(M, N, sm_count)) {
+  switch (form<OutT>(M, N, Kp, sm_count)) {
     case 0: return launch_few<OutT>(x, sx, w, sw, out, M, N, Kp, st);
     case 1: return launch_large<OutT, 64, false>(x, sx, w, sw, out, M, N, Kp, sm_count, st);
     case 2: return launch_large<OutT, 128, false>(x, sx, w, sw, out, M, N, Kp, sm_count, st);
     case 3: return launch_large<OutT, 256, false>(x, sx, w, sw, out, M, N, Kp, sm_count, st);
+    case 5: return launch_split<OutT, 64>(x, sx, w, sw, out, M, N, Kp, st);
+    case 6: return launch_split<OutT, 128>(x, sx, w, sw, out, M, N, Kp, st);
     default: return launch_large<OutT, 256, true>(x, sx, w, sw, out, M, N, Kp, sm_count, st);
   }
 }

@@ -241,7 +241,8 @@ def _address(name: str) -> int:
 
 def force_product_form(form: int) -> None:
     """Measurement and test switch of the product: mma.sync on a streamed weight (0), tiles of 128 x 64, 128 x 128 or
-    128 x 256 (1, 2, 3), the pair of CTAs (4), whatever the sizes; -1: the library's own choice.  All give the same bits."""
+    128 x 256 (1, 2, 3), the pair of CTAs (4), clusters that share k on tiles of 128 x 64 or 128 x 128 (5, 6), whatever the
+    sizes; -1: the library's own choice.  All give the same bits."""
     _ops()._lib("gemm_int8").dib_gemm_int8_force_form(c_int(form))
 
 

@@ -154,6 +154,25 @@ def test_every_form_of_a_product_gives_the_same_bits(m, n, k, dtype):
         int8.force_product_form(-1)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m,n,k", [(1, 17, 40), (16, 1024, 1024), (33, 1000, 2064), (65, 130, 4112), (128, 2048, 300),
+                                   (129, 257, 1300), (256, 200, 8192), (40, 4096, 1056)])
+def test_clusters_that_share_k_give_the_same_bits(m, n, k, dtype):
+    from deterministic_inference_b200.kernels import int8
+    x, w = _rand(m, k, seed=m + 1, dtype=dtype), ops.Int8Weight.of(_rand(n, k, seed=n + 1))
+    try:
+        int8.force_product_form(2)
+        want = ops.int8_linear(x, w)
+        for form in (5, 6):
+            int8.force_product_form(form)
+            got = ops.int8_linear(x, w)
+            ops.check_kernel_status()
+            assert torch.equal(got, want), f"form {form}"
+    finally:
+        int8.force_product_form(-1)
+    _check_product(ops.int8_linear(x, w), x, w.codes[:, :k], w.scales, dtype)
+
+
 def test_product_with_no_rows():
     w = ops.Int8Weight.of(_rand(32, 64))
     assert ops.int8_linear(torch.empty(0, 64, device="cuda"), w).shape == (0, 32)
