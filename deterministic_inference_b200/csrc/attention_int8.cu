@@ -1051,7 +1051,7 @@ int dib_int8_attention_split_keys(int kv_len, int rows) { return split_keys(kv_l
 
 // The split form, for the sequences seq_list[0 .. seq_count) or (null) seq_first ...: heads up to 128, pages of a
 // power of two of rows, 4 at least.  max_rows: the most rows (new tokens x query heads of a kv head) of one of them; tile_rows: 8,
-// 16 or (bfloat16) 4 or 32 rows a tile; max_items: the most (tiles x runs x kv heads) of one; part_o float32 [seq_count, max_items,
+// 16 or (bfloat16) 4, 24 or 32 rows a tile; max_items: the most (tiles x runs x kv heads) of one; part_o float32 [seq_count, max_items,
 // tile_rows, D] and part_ml [.., 2] take partial results where merge is not 0 (some sequence may have two runs).
 int dib_int8_attention_split(const void* q, void* out, const void* data, const void* scales, long long num_pages,
                              const void* block_table, int max_blocks, const void* cu_q_lens, const void* seq_lens,
@@ -1062,7 +1062,7 @@ int dib_int8_attention_split(const void* q, void* out, const void* data, const v
   const bool pages_fit = page_size >= 4 && (page_size & (page_size - 1)) == 0;
   if (seq_count < 0 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || D < 16 || D > 128 || D % 16 != 0 || page_size < 1 || !pages_fit ||
       num_pages * 2 * Hkv * page_size >= (1ll << 31) || seq_count > 65535 || max_items < 1 || sm_count < 1 ||
-      (tile_rows != 8 && tile_rows != 16 && ((tile_rows != 4 && tile_rows != 32) || dtype != 1)))
+      (tile_rows != 8 && tile_rows != 16 && ((tile_rows != 4 && tile_rows != 24 && tile_rows != 32) || dtype != 1)))
     return DIB_BAD_SIZE;
   if (((reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(q) |
         reinterpret_cast<uintptr_t>(out)) & 15) != 0)
@@ -1093,6 +1093,7 @@ int dib_int8_attention_split(const void* q, void* out, const void* data, const v
     if (tile_rows == 4) return launch_split<B, 4>(map, q, out, a, max_rows, merge, sm_count, st);
     if (tile_rows == 8) return launch_split<B, 8>(map, q, out, a, max_rows, merge, sm_count, st);
     if (tile_rows == 16) return launch_split<B, 16>(map, q, out, a, max_rows, merge, sm_count, st);
+    if (tile_rows == 24) return launch_split<B, 24>(map, q, out, a, max_rows, merge, sm_count, st);
     return launch_split<B, 32>(map, q, out, a, max_rows, merge, sm_count, st);
   }
   if (tile_rows == 8) return launch_split<float, 8>(map, q, out, a, max_rows, merge, sm_count, st);

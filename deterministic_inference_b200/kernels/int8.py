@@ -402,7 +402,7 @@ class _SplitPart:
         if seqs != list(range(first, first + count)):
             self.list = torch.tensor(seqs, dtype=torch.int32).to(device, non_blocking=True)
         self.max_rows = max(q_lens[s] for s in seqs) * group
-        self.tile_rows = next(r for r in ((8, 16) if wide else (4, 8, 16, 32)) if self.max_rows <= r or r == (16 if wide else 32))
+        self.tile_rows = next(r for r in ((8, 16) if wide else (4, 8, 16, 24, 32)) if self.max_rows <= r or r == (16 if wide else 32))
         runs = _most_runs(max(kv_lens[s] for s in seqs))
         tiles, per32 = -(-self.max_rows // self.tile_rows), 32 // self.tile_rows
         # (runs get longer with the rows: tiles * runs is largest at 64 rows, or the tiles' own number is)
