@@ -62,10 +62,12 @@ constexpr int SP_TILE = 128, SP_THREADS = 256, SP_STAGES = 2, SP_ITEMS = 4;
 constexpr int SP_COPY_WARP = 4, SP_SCORE_WARP = 5, SP_OUTPUT_WARP = 7;      // and 6: items and query rows
 
 // Keys of a run: two tiles (one: 72 -> 77 us for 64 decoding requests of up to 4,096 keys, as an item's beginning and end
-// cost about a tile, and no gain for one request of 2,048), longer ones where the partial results would grow; with many
-// rows a run gets longer still, as their partial results do with the rows.
+// cost about a tile, and no gain for one request of 2,048), four for more than 4 rows, whose beginning and end cost more (32
+// requests of 4,096 keys and 64 heads: 69 -> 62 us, sixteen of 1,500 with five drafted tokens 32 -> 29; but one of those
+// 15.5 -> 17.7), and for long sequences, where the partial results would grow; with many rows a run gets longer still, as
+// their partial results do with the rows.
 __host__ __device__ __forceinline__ int split_keys(int kv_len, int rows) {
-  const int base = kv_len <= 16384 ? 256 : 512;
+  const int base = kv_len <= 16384 && rows <= 4 ? 256 : 512;
   const int tiles = (rows + 31) / 32;
   return tiles <= 2 ? base : base * tiles;
 }
