@@ -38,10 +38,12 @@ constexpr int RAW_BYTES = 128 * 128;
 constexpr float NEG_BIG = -1e30f;
 constexpr float LOG2E = 1.4426950408889634f;
 
-// shared memory: queries of A and B; a ring of 16-bit tiles and one of bytes, keys and values in turn; scales
+// shared memory: queries of A and B (later their outputs); a ring of 16-bit tiles and one of bytes, keys and values in turn;
+// scales; the query rows' units
 constexpr int RING = 3, SLOTS = 4;
 constexpr int S_KV = 2 * TILE_BYTES, S_RAW = S_KV + RING * TILE_BYTES, S_SCALES = S_RAW + RING * RAW_BYTES;
-constexpr int S_NAN = S_SCALES + SLOTS * 1024, S_BARS = S_NAN + SLOTS * 32, S_TOTAL = S_BARS + 32 * 8;
+constexpr int S_NAN = S_SCALES + SLOTS * 1024, S_ROWS = S_NAN + SLOTS * 32;
+constexpr int S_BARS = S_ROWS + 2 * TILE * 4, S_TOTAL = S_BARS + 32 * 8;
 constexpr int S_DYNAMIC = S_TOTAL + 1024;
 
 __device__ int dib_attention_int8_prompt_error_word = 0;
@@ -226,6 +228,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
   unsigned char* sKV = smem + S_KV;
   unsigned char* raw = smem + S_RAW;
   float* scales = reinterpret_cast<float*>(smem + S_SCALES);          // [SLOTS][keys', values' of 128]
+  float* row_units = reinterpret_cast<float*>(smem + S_ROWS);         // [2][TILE]; NaN: the row holds an infinity or a NaN
   NanKeys* nan_keys = reinterpret_cast<NanKeys*>(smem + S_NAN);       // [SLOTS]
   unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + S_BARS);
   unsigned long long* raw_full = bars;            // [RING] a tile's bytes have arrived
@@ -343,42 +346,40 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
-  // Both query tiles -> shared memory, swizzled, a thread a row: times the power of two that takes the row's largest value
-  // to 2^4 (exact in float16 down to 2^-21 of that); rows beyond a tile's tokens and dimensions beyond D are zero.
-  float row_unit = 1.f, row_sum = 0.f;
-  const int x = threadIdx.x >> 7, r = threadIdx.x & 127;
-  if (threadIdx.x < SOFTMAX) {
-    const int tl = r / G, g = r - tl * G, my_ntok = x ? ntok[1] : ntok[0];
-    uint4 v[16];
-    const __nv_bfloat16* src = qp + ((long long)(q_begin + (x ? tokx[1] : tokx[0]) + tl) * a.Hq + kvh * G + g) * a.D;
+  // Both query tiles -> shared memory, swizzled, 16 lanes a row: times the power of two that takes the row's largest value to
+  // 2^4 .. 2^5 (exact in float16 down to 2^-21 of that); rows beyond a tile's tokens and dimensions beyond D are zero.  (A
+  // thread a row took 5 us: the lines do not stay in what L1 has left.)
+  {
+    constexpr int PER_THREAD = 2 * TILE * 16 / THREADS;
+    const int ch = threadIdx.x & 15;
+    uint4 v[PER_THREAD];
 #pragma unroll
-    for (int ch = 0; ch < 16; ++ch) {
-      v[ch] = make_uint4(0, 0, 0, 0);
-      if (tl < my_ntok && ch * 8 < a.D) v[ch] = *reinterpret_cast<const uint4*>(src + ch * 8);
+    for (int it = 0; it < PER_THREAD; ++it) {
+      const int row = it * (THREADS / 16) + (threadIdx.x >> 4), x = row >> 7;
+      const int tl = (row & 127) / G, g = (row & 127) - tl * G;
+      v[it] = make_uint4(0, 0, 0, 0);
+      if (tl < (x ? ntok[1] : ntok[0]) && ch * 8 < a.D)
+        v[it] = *reinterpret_cast<const uint4*>(
+            qp + ((long long)(q_begin + (x ? tokx[1] : tokx[0]) + tl) * a.Hq + kvh * G + g) * a.D + ch * 8);
     }
-    unsigned top = 0;      // the largest magnitude, in the high half
 #pragma unroll
-    for (int ch = 0; ch < 16; ++ch) {
-      const unsigned w[4] = {v[ch].x, v[ch].y, v[ch].z, v[ch].w};
+    for (int it = 0; it < PER_THREAD; ++it) {
+      const int row = it * (THREADS / 16) + (threadIdx.x >> 4), x = row >> 7;
+      const unsigned w[4] = {v[it].x, v[it].y, v[it].z, v[it].w};
+      unsigned top = 0;      // the largest magnitude, in the high half
 #pragma unroll
       for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7fff0000u, w[e] << 16 & 0x7fff0000u));
-    }
-    const int expo = max((int)(top >> 23), 5);                    // (2^126 at most below)
-    float to_unit = two_to(131 - expo);
-    row_unit = two_to(expo - 131);
-    if (top >= 0x7f800000u) {                                     // an infinity or a NaN: so is what the row gets
-      to_unit = 0.f;
-      row_sum = __int_as_float(0x7fc00000);
-    }
 #pragma unroll
-    for (int ch = 0; ch < 16; ++ch) {
-      const unsigned w[4] = {v[ch].x, v[ch].y, v[ch].z, v[ch].w};
+      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const int expo = max((int)(top >> 23), 5);                    // (2^126 at most below)
+      const bool finite = top < 0x7f800000u;
+      const float to_unit = two_to(131 - expo);
       unsigned y[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        y[e] = to_unit == 0.f ? 0u
-                              : pack_f16(__uint_as_float(w[e] << 16) * to_unit, __uint_as_float(w[e] & 0xffff0000u) * to_unit);
-      *reinterpret_cast<uint4*>(sQ + x * TILE_BYTES + piece_off(r, ch)) = make_uint4(y[0], y[1], y[2], y[3]);
+        y[e] = finite ? pack_f16(__uint_as_float(w[e] << 16) * to_unit, __uint_as_float(w[e] & 0xffff0000u) * to_unit) : 0u;
+      *reinterpret_cast<uint4*>(sQ + x * TILE_BYTES + piece_off(row & 127, ch)) = make_uint4(y[0], y[1], y[2], y[3]);
+      if (ch == 0) row_units[row] = finite ? two_to(expo - 131) : __int_as_float(0x7fc00000);
     }
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the queries are read by the tensor core
@@ -578,6 +579,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
   } else {
     regs_take<REGS_MANY>();
     // ---- softmax: thread r of group x owns row r of query tile x
+    const int x = threadIdx.x >> 7, r = threadIdx.x & 127;
     const int tl = r / G, g = r - tl * G;
     const int tok0 = x ? tokx[1] : tokx[0], i_first = (x ? jf[1] : jf[0]) - j0, i_last = (x ? jl[1] : jl[0]) - j0;
     const bool valid = tl < (x ? ntok[1] : ntok[0]);
@@ -586,7 +588,11 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
     const int hi = prefix + tok0 + tl, lo = first_visible_key(hi, a.window);
     const unsigned lane_base = (unsigned)((warp & 3) * 32) << 16;
     const unsigned tmem_o = tmem + lane_base + 256 + x * 128;
-    float m_ref = NEG_BIG, l = row_sum;
+    float row_unit = row_units[threadIdx.x], m_ref = NEG_BIG, l = 0.f;
+    if (row_unit != row_unit) {      // its queries are zeros: the sum makes its result NaN
+      l = row_unit;
+      row_unit = 1.f;
+    }
     int uses_own = 0, uses_other = n_other;      // completed phases of s_full of the own columns and of the other's
     const int my_solo = x == solo_x ? solo_from : 0x7fffffff;
     const float2 unit2 = make_float2(row_unit, row_unit);
@@ -690,25 +696,40 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
       ok = mbar_wait(&o_final[x], 0);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
-      const long long row = (long long)(q_begin + tok0 + tl) * a.Hq + kvh * G + g;
-      if (ok && !(x ? whole[1] : whole[0])) {
-        // a partial result of this chunk: O as accumulated (against m_ref), m_ref, l
-        const long long at = row * a.max_chunks + chunk;
+      // Outputs by way of the query tile, which nobody reads any more: a warp's 32 rows, then whole rows to memory.
+      unsigned char* stage = sQ + x * TILE_BYTES + (warp & 3) * 8192;
+      const bool partial = !(x ? whole[1] : whole[0]);      // this chunk's: O as accumulated (against m_ref), m_ref, l
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      const int my_ntok = x ? ntok[1] : ntok[0], row0 = (warp & 3) * 32;
+      auto row_of_lane = [&](int rr) {      // the row of the output that is row rr of this tile, or -1
+        const int t = rr / G;
+        return t < my_ntok ? (long long)(q_begin + tok0 + t) * a.Hq + kvh * G + rr - t * G : -1ll;
+      };
+      if (ok && partial) {
+        if (valid) a.part_ml[((long long)(q_begin + tok0 + tl) * a.Hq + kvh * G + g) * a.max_chunks + chunk] = make_float2(m_ref, l);
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {      // 64 dimensions at a time
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          unsigned o[32];
-          tc_ld32(tmem_o + c * 32, o);
-          tc_wait_ld();
-          if (valid) {
+          for (int c = 0; c < 2; ++c) {
+            unsigned o[32];
+            tc_ld32(tmem_o + half * 64 + c * 32, o);
+            tc_wait_ld();
 #pragma unroll
             for (int ch = 0; ch < 8; ++ch)
-              *reinterpret_cast<uint4*>(a.part_o + at * TILE + c * 32 + ch * 4) =
+              *reinterpret_cast<uint4*>(stage + lane * 256 + ((c * 8 + ch) ^ (lane & 7)) * 16) =
                   make_uint4(o[ch * 4], o[ch * 4 + 1], o[ch * 4 + 2], o[ch * 4 + 3]);
           }
+          __syncwarp();
+#pragma unroll 4
+          for (int rr = lane >> 4; rr < 32; rr += 2) {
+            const long long row = row_of_lane(row0 + rr);
+            if (row >= 0)
+              *reinterpret_cast<uint4*>(a.part_o + (row * a.max_chunks + chunk) * TILE + half * 64 + (lane & 15) * 4) =
+                  *reinterpret_cast<const uint4*>(stage + rr * 256 + ((lane & 15) ^ (rr & 7)) * 16);
+          }
+          __syncwarp();
         }
-        if (valid) a.part_ml[at] = make_float2(m_ref, l);
       } else if (ok) {
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           unsigned o[32];
@@ -717,10 +738,17 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
           auto value = [&](int e) { return __uint_as_float(o[e]) * inv; };
 #pragma unroll
           for (int ch = 0; ch < 4; ++ch)
-            if (valid && c * 32 + ch * 8 < a.D)
-              *reinterpret_cast<uint4*>(out + row * a.D + c * 32 + ch * 8) =
-                  make_uint4(pack_bf16(value(ch * 8), value(ch * 8 + 1)), pack_bf16(value(ch * 8 + 2), value(ch * 8 + 3)),
-                             pack_bf16(value(ch * 8 + 4), value(ch * 8 + 5)), pack_bf16(value(ch * 8 + 6), value(ch * 8 + 7)));
+            *reinterpret_cast<uint4*>(stage + lane * 256 + ((c * 4 + ch) ^ (lane & 7)) * 16) =
+                make_uint4(pack_bf16(value(ch * 8), value(ch * 8 + 1)), pack_bf16(value(ch * 8 + 2), value(ch * 8 + 3)),
+                           pack_bf16(value(ch * 8 + 4), value(ch * 8 + 5)), pack_bf16(value(ch * 8 + 6), value(ch * 8 + 7)));
+        }
+        __syncwarp();
+#pragma unroll 4
+        for (int rr = lane >> 4; rr < 32; rr += 2) {
+          const long long row = row_of_lane(row0 + rr);
+          if (row >= 0 && (lane & 15) * 8 < a.D)
+            *reinterpret_cast<uint4*>(out + row * a.D + (lane & 15) * 8) =
+                *reinterpret_cast<const uint4*>(stage + rr * 256 + ((lane & 15) ^ (rr & 7)) * 16);
         }
       }
     }
