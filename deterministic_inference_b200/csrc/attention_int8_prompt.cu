@@ -31,7 +31,7 @@
 namespace {
 
 constexpr int TILE = 128, SOFTMAX_WARPS = 8, COPY_WARP = 8, MMA_WARP = 9, CONVERTERS = 6;
-constexpr int THREADS = 512, SOFTMAX = SOFTMAX_WARPS * 32;
+constexpr int THREADS = 512;
 constexpr int REGS_FEW = 64, REGS_MANY = 192;         // 256 * 64 + 256 * 192 = 512 * 128
 constexpr int TILE_BYTES = 128 * 128 * 2, HALF_BYTES = 128 * 64 * 2;      // a bfloat16 tile: two halves of 64 columns
 constexpr int RAW_BYTES = 128 * 128;
@@ -250,6 +250,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
   }
   const int unit = a.count - 1 - blockIdx.y, kvh = blockIdx.x;        // the longest first
   const int G = a.Hq / a.Hkv, npt = TILE / G;                         // tokens of a query tile
+  const unsigned g_up = 65536u / G + 1;      // r / G for r < 128, exactly: 128 G < 65536
+  auto token_of = [&](int r) { return (int)(r * g_up >> 16); };
   const int seq = a.units[unit];
   const int tokx[2] = {a.units[a.count + unit], a.units[2 * a.count + unit]};
   const int chunk = a.chunk_tiles > 0 ? a.units[3 * a.count + unit] : 0;
@@ -356,7 +358,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
 #pragma unroll
     for (int it = 0; it < PER_THREAD; ++it) {
       const int row = it * (THREADS / 16) + (threadIdx.x >> 4), x = row >> 7;
-      const int tl = (row & 127) / G, g = (row & 127) - tl * G;
+      const int tl = token_of(row & 127), g = (row & 127) - tl * G;
       v[it] = make_uint4(0, 0, 0, 0);
       if (tl < (x ? ntok[1] : ntok[0]) && ch * 8 < a.D)
         v[it] = *reinterpret_cast<const uint4*>(
@@ -580,7 +582,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
     regs_take<REGS_MANY>();
     // ---- softmax: thread r of group x owns row r of query tile x
     const int x = threadIdx.x >> 7, r = threadIdx.x & 127;
-    const int tl = r / G, g = r - tl * G;
+    const int tl = token_of(r), g = r - tl * G;
     const int tok0 = x ? tokx[1] : tokx[0], i_first = (x ? jf[1] : jf[0]) - j0, i_last = (x ? jl[1] : jl[0]) - j0;
     const bool valid = tl < (x ? ntok[1] : ntok[0]);
     // (rows behind the sequence's last token see what a token there would see: no warp goes through the tests for masked
@@ -702,7 +704,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
       const float inv = l == 0.f ? 0.f : 1.0f / l;
       const int my_ntok = x ? ntok[1] : ntok[0], row0 = (warp & 3) * 32;
       auto row_of_lane = [&](int rr) {      // the row of the output that is row rr of this tile, or -1
-        const int t = rr / G;
+        const int t = token_of(rr);
         return t < my_ntok ? (long long)(q_begin + tok0 + t) * a.Hq + kvh * G + rr - t * G : -1ll;
       };
       if (ok && partial) {
