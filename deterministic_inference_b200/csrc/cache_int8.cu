@@ -2,10 +2,11 @@
 // of quantised keys and values, and reading it back.
 //
 // A row (a token's activations, an output channel of a weight, a token's key or value of one head) of values x:
-//   a = max(max |x|, 2^-100),  code = rint(x * (127 / a)) (ties to even),  scale = a / 127,  value = scale * code.
-// 127 / a and a / 127 are the correctly rounded quotients and x * (127 / a) one rounded product, so the codes are the
-// same on every path that makes them.  |x * (127 / a)| <= 127 (1 + 2^-23), which rounds to 127: no clamp.  The floor
-// 2^-100 keeps 127 / a finite; rows below it read back as zeros, 2^-100 off at most.  A row that holds an infinity or
+//   a = max(max |x|, 2^-100),  code = rint(x * (127 * (1 / a))) (ties to even),  scale = a * (1 / 127),
+//   value = scale * code,
+// every operation rounded to float32 by itself (what a division by, or of, a plain number is in torch), so the codes are
+// the same on every path that makes them.  |x * (127 * (1 / a))| <= 127 (1 + 2^-22), which rounds to 127: no clamp.  The
+// floor 2^-100 keeps 127 / a finite; rows below it read back as zeros, 2^-100 off at most.  A row that holds an infinity or
 // a NaN has the scale NaN, so whatever reads it gets NaN and not a number that looks right.
 //
 // Cache: data int8 [pages, 2, Hkv, page_size, D], scales float32 [pages, 2, Hkv, page_size].
@@ -26,8 +27,8 @@ __device__ __forceinline__ RowScale row_scale(unsigned bits) {
     r.scale = __uint_as_float(0x7fc00000u);
   } else {
     const float a = fmaxf(__uint_as_float(bits), ROW_FLOOR);
-    r.inv = __fdiv_rn(127.f, a);
-    r.scale = __fdiv_rn(a, 127.f);
+    r.inv = __fmul_rn(__frcp_rn(a), 127.f);
+    r.scale = __fmul_rn(a, 1.f / 127.f);
   }
   return r;
 }

@@ -3,7 +3,7 @@ cache of keys and values with a scale for each token and head.  ``ops`` exports 
 
 One rule quantises every row (a token's activations, an output channel of a weight, a token's key or value of one head):
 
-    a = max(max |x|, 2^-100),  code = rint(x * (127 / a)) (ties to even),  scale = a / 127,  value = scale * code
+    a = max(max |x|, 2^-100),  code = rint(x * (127 * (1 / a))) (ties to even),  scale = a * (1 / 127),  value = scale * code
 
 in float32, whatever the row's type.  A row that holds an infinity or a NaN has the scale NaN and reads back as NaN.
 

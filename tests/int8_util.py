@@ -15,10 +15,10 @@ def codes_of(x: torch.Tensor):
     a = x.abs().amax(-1)
     bad = ~torch.isfinite(a)
     a = torch.where(bad, torch.ones_like(a), a).clamp(min=FLOOR)
-    seven = torch.full_like(a, 127.0)            # (a tensor: a division by a Python number is a product in torch)
-    codes = torch.round(x * (seven / a)[..., None])
+    one = torch.ones_like(a)                     # (a tensor: the quotients are rounded, and so are the products)
+    codes = torch.round(x * ((one / a) * 127.0)[..., None])
     codes = torch.where(bad[..., None], torch.zeros_like(codes), codes).to(torch.int8)
-    return codes, torch.where(bad, torch.full_like(a, float("nan")), a / seven)
+    return codes, torch.where(bad, torch.full_like(a, float("nan")), a * (one / (127.0 * one)))
 
 
 class Int8Case:
