@@ -326,7 +326,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
     int n = 0, v_row = 0;                  // tiles sent for; the values' row of the tile before
     unsigned v_senders = 0;
     auto send_values = [&](int m) {        // of tile m
-      if (m >= SP_STAGES) ok = mbar_wait(&v_empty[m & 1], ((m >> 1) - 1) & 1);
+      if (m >= SP_STAGES) ok = mbar_wait_brief(&v_empty[m & 1], ((m >> 1) - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       if (lane == 0) mbar_expect_tx(&v_full[m & 1], __popc(v_senders) * a.box_rows * 128);
@@ -336,7 +336,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
     };
     for (int k = 0; ok; ++k) {
       const int slot = k % SP_ITEMS;
-      ok = mbar_wait(&item_full[slot], (k / SP_ITEMS) & 1);
+      ok = mbar_wait_brief(&item_full[slot], (k / SP_ITEMS) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       const int seq = items[slot].seq, kvh = items[slot].kvh, at = items[slot].at, end = items[slot].end, tiles = items[slot].tiles;
@@ -351,7 +351,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
         const bool have = page >= 0 && page < a.num_pages;
         const unsigned senders = __ballot_sync(0xffffffffu, have && (lane == 0 || off == 0));
         if (n >= SP_STAGES)       // (the scores made, and the scales read: those of the tile two before this one)
-          ok = mbar_wait(&s_full[stage], ((n >> 1) - 1) & 1) && mbar_wait(&s_empty[stage], ((n >> 1) - 1) & 1);
+          ok = mbar_wait_brief(&s_full[stage], ((n >> 1) - 1) & 1) && mbar_wait_brief(&s_empty[stage], ((n >> 1) - 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (lane == 0) mbar_expect_tx(&k_full[stage], __popc(senders) * a.box_rows * 128);
@@ -379,7 +379,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       int n = 0, q_used = -1;
       for (int k = 0; ok; ++k) {
         const int slot = k % SP_ITEMS;
-        ok = __all_sync(0xffffffffu, mbar_wait(&item_full[slot], (k / SP_ITEMS) & 1));
+        ok = __all_sync(0xffffffffu, mbar_wait_brief(&item_full[slot], (k / SP_ITEMS) & 1));
         if (!ok) break;
         const int tiles = items[slot].tiles, fresh = items[slot].fresh;
         __syncwarp();
@@ -388,12 +388,12 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
         if (fresh) {
           if (q_used >= 0) tc_commit(elected, &q_empty[q_used & 1]);
           ++q_used;
-          ok = __all_sync(0xffffffffu, mbar_wait(&q_full[q_used & 1], (q_used >> 1) & 1));
+          ok = __all_sync(0xffffffffu, mbar_wait_brief(&q_full[q_used & 1], (q_used >> 1) & 1));
           if (!ok) break;
         }
         const unsigned long long qd = desc_sw128(base + SH::QUERIES + (q_used & 1) * N * 128);
         for (int t = tiles; t > 0 && ok; --t, ++n) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&k_full[n & 1], (n >> 1) & 1) && (n < 2 || mbar_wait(&s_empty[n & 1], ((n >> 1) - 1) & 1)));
+          ok = __all_sync(0xffffffffu, mbar_wait_brief(&k_full[n & 1], (n >> 1) & 1) && (n < 2 || mbar_wait_brief(&s_empty[n & 1], ((n >> 1) - 1) & 1)));
           if (!ok) break;
           tc_fence_after();
           const unsigned long long kd = desc_sw128(base + (n & 1) * SH::STAGE);
@@ -413,14 +413,14 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       int n = 0;
       for (int k = 0; ok; ++k) {
         const int slot = k % SP_ITEMS;
-        ok = __all_sync(0xffffffffu, mbar_wait(&item_full[slot], (k / SP_ITEMS) & 1));
+        ok = __all_sync(0xffffffffu, mbar_wait_brief(&item_full[slot], (k / SP_ITEMS) & 1));
         if (!ok) break;
         const int tiles = items[slot].tiles;
         __syncwarp();
         if (lane == 0) mbar_arrive(&item_empty[slot]);
         if (tiles == 0) break;
         for (int t = tiles; t > 0 && ok; --t, ++n) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&v_full[n & 1], (n >> 1) & 1) && mbar_wait(p_full, n & 1));
+          ok = __all_sync(0xffffffffu, mbar_wait_brief(&v_full[n & 1], (n >> 1) & 1) && mbar_wait_brief(p_full, n & 1));
           if (!ok) break;
           tc_fence_after();
           const unsigned long long vd = desc_sw128(base + (n & 1) * SH::STAGE + SP_TILE * 128);
@@ -508,7 +508,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       };
       if (it.fresh) load_rows(0);
       const int slot = k % SP_ITEMS;
-      if (k >= SP_ITEMS) ok = mbar_wait(&item_empty[slot], ((k / SP_ITEMS) - 1) & 1);
+      if (k >= SP_ITEMS) ok = mbar_wait_brief(&item_empty[slot], ((k / SP_ITEMS) - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (lane == 0) {
@@ -519,7 +519,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       if (it.tiles == 0) break;
       if (!it.fresh) continue;
       const int buf = made & 1;
-      if (made >= 2) ok = mbar_wait(&q_empty[buf], ((made >> 1) - 1) & 1);
+      if (made >= 2) ok = mbar_wait_brief(&q_empty[buf], ((made >> 1) - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       unsigned char* dst = smem + SH::QUERIES + buf * N * 128;
@@ -592,7 +592,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       }
     };
     auto add_outputs = [&](int m) {      // tile m's integers
-      ok = mbar_wait(o_full, m & 1);
+      ok = mbar_wait_brief(o_full, m & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       tc_fence_after();
@@ -663,7 +663,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
     };
     for (int k = 0; ok; ++k) {
       const int slot = k % SP_ITEMS;
-      ok = mbar_wait(&item_full[slot], (k / SP_ITEMS) & 1);
+      ok = mbar_wait_brief(&item_full[slot], (k / SP_ITEMS) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       const SplitItem it = items[slot];
@@ -674,7 +674,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       if (it.fresh) {
         if (q_used >= 0 && lane == 0) mbar_arrive(&q_empty[q_used & 1]);
         ++q_used;
-        ok = mbar_wait(&q_full[q_used & 1], (q_used >> 1) & 1);
+        ok = mbar_wait_brief(&q_full[q_used & 1], (q_used >> 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
       }
@@ -684,7 +684,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       const int hi_all = min(it.end - 1, p0 + row0 / G);
       for (int kb = it.at; kb < it.end; kb += SP_TILE, ++n) {
         const int buf = n & 1;
-        ok = mbar_wait(&k_full[buf], (n >> 1) & 1) && mbar_wait(&s_full[buf], (n >> 1) & 1);
+        ok = mbar_wait_brief(&k_full[buf], (n >> 1) & 1) && mbar_wait_brief(&s_full[buf], (n >> 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();

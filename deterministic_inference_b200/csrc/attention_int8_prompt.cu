@@ -42,7 +42,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 // scales; the query rows' units
 constexpr int RING = 3, SLOTS = 4;
 constexpr int S_KV = 2 * TILE_BYTES, S_RAW = S_KV + RING * TILE_BYTES, S_SCALES = S_RAW + RING * RAW_BYTES;
-constexpr int S_NAN = S_SCALES + SLOTS * 1024, S_ROWS = S_NAN + SLOTS * 32;
+constexpr int S_INFO = S_SCALES + SLOTS * 1024, S_ROWS = S_INFO + SLOTS * 32;
 constexpr int S_BARS = S_ROWS + 2 * TILE * 4, S_TOTAL = S_BARS + 32 * 8;
 constexpr int S_DYNAMIC = S_TOTAL + 1024;
 
@@ -193,18 +193,23 @@ __device__ __forceinline__ unsigned codes_f16(unsigned turned, unsigned sel) {
   const __half2 c = __hsub2(*reinterpret_cast<const __half2*>(&a), __half2half2(__ushort_as_half(0x6480)));      // 1152
   return *reinterpret_cast<const unsigned*>(&c);
 }
-// Two codes of a word times a scale as bfloat16, rounded once: a byte with its sign turned, under the exponent of 2^23, is
-// 2^23 + 128 + code.
-__device__ __forceinline__ unsigned codes_bf16(unsigned turned, unsigned sel, float2 scale) {
-  const float2 u = make_float2(__uint_as_float(__byte_perm(turned, 0x4b000000u, sel)),
-                               __uint_as_float(__byte_perm(turned, 0x4b000000u, sel + 1)));
-  const float2 y = __fmul2_rn(__fadd2_rn(u, make_float2(-8388736.f, -8388736.f)), scale);
-  return pack_bf16(y.x, y.y);
+// Two codes of a word as bfloat16, exactly: low 7 bits and sign bit of a byte under the exponent byte 0x43 are 128 + low and
+// 128 + 128 sign, and a code is the first minus the second.
+__device__ __forceinline__ unsigned codes_bf16(unsigned word, unsigned sel) {
+  const unsigned a = __byte_perm(word & 0x7f7f7f7fu, 0x43434343u, sel), b = __byte_perm(word & 0x80808080u, 0x43434343u, sel);
+  const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const unsigned*>(&d);
+}
+__device__ __forceinline__ unsigned times_f16(unsigned codes, __half2 scale) {
+  const __half2 y = __hmul2_rn(*reinterpret_cast<const __half2*>(&codes), scale);
+  return *reinterpret_cast<const unsigned*>(&y);
 }
 
-// The keys of a tile that are no numbers: bit l of word j, key 4 l + j.
-struct NanKeys {
-  unsigned key[4], any, pad[3];
+// What the keys of a tile have in common.  value_exp: the values' scales are in units of 2^value_exp, the outputs too.
+// wide: some scale lies outside float16's range then.  nan: the keys that are no numbers, bit l of word j key 4 l + j.
+struct TileInfo {
+  unsigned nan[4], any_nan;
+  int wide, value_exp, pad;
 };
 
 struct PromptArgs {
@@ -229,7 +234,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
   unsigned char* raw = smem + S_RAW;
   float* scales = reinterpret_cast<float*>(smem + S_SCALES);          // [SLOTS][keys', values' of 128]
   float* row_units = reinterpret_cast<float*>(smem + S_ROWS);         // [2][TILE]; NaN: the row holds an infinity or a NaN
-  NanKeys* nan_keys = reinterpret_cast<NanKeys*>(smem + S_NAN);       // [SLOTS]
+  TileInfo* infos = reinterpret_cast<TileInfo*>(smem + S_INFO);       // [SLOTS]
   unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + S_BARS);
   unsigned long long* raw_full = bars;            // [RING] a tile's bytes have arrived
   unsigned long long* raw_empty = bars + 3;       // [RING] they have been converted (a warp each)
@@ -395,7 +400,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
   if (warp == MMA_WARP) {
     {
       const unsigned elected = elect_one();
-      constexpr unsigned idesc_s = idesc_f16(TILE, TILE, false, 0), idesc_o = idesc_f16(TILE, TILE, true, 1);
+      constexpr unsigned idesc_s = idesc_f16(TILE, TILE, false, 0);
       // Descriptors are made once: a step inside a tile is an addition to the low bits, which hold the address.
       const unsigned long long q_desc = desc_k_major(smem_u32(sQ)), k_desc = desc_k_major(smem_u32(sKV)),
                                v_desc = desc_mn_major(smem_u32(sKV));
@@ -413,10 +418,11 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
       auto issue_o = [&](int x, int buf, int i) {
         const unsigned long long vd = v_desc + ((2 * i + 1) % RING) * (TILE_BYTES >> 4);
         const bool first = j0 + i == (x ? jf[1] : jf[0]);
+        const unsigned idesc_o = infos[i % SLOTS].wide ? idesc_f16(TILE, TILE, true, 1) : idesc_f16(TILE, TILE, false, 1);
         const int turn = (buf ? uses[1]++ : uses[0]++) & 1;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&p_full[2 * buf + half], turn));
+          ok = __all_sync(0xffffffffu, mbar_wait_brief(&p_full[2 * buf + half], turn));
           if (!ok) return;
           tc_fence_after();
 #pragma unroll
@@ -426,7 +432,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         }
       };
       auto want = [&](int item) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&full[item % RING], (item / RING) & 1));
+        ok = __all_sync(0xffffffffu, mbar_wait_brief(&full[item % RING], (item / RING) & 1));
         tc_fence_after();
         return ok;
       };
@@ -488,8 +494,9 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
     load_scales(row_now);
     int row_next = row_of(1);
     const float unit = a.scale * LOG2E;
+    int value_exp = -1000;      // (not known before a scale that is not zero)
     for (int i = 0; i < ntiles && ok; ++i) {
-      if (i >= SLOTS) ok = mbar_wait(&sc_empty[i % SLOTS], (i / SLOTS - 1) & 1);
+      if (i >= SLOTS) ok = mbar_wait_brief(&sc_empty[i % SLOTS], (i / SLOTS - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       const int left = kv_len - ((j0 + i) * TILE + lane * 4);
@@ -503,16 +510,30 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         ks[j] *= unit;
         if (left <= j || is_nan) ks[j] = vs[j] = 0.f;
       }
+      // The values' unit takes the largest scale of the first tile to 2^4 .. 2^5; scales of 2^-13 .. 2^8 leave float16 all of
+      // its bits for the values.
+      float top = 0.f, bottom = INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        top = fmaxf(top, fabsf(vs[j]));
+        if (vs[j] != 0.f) bottom = fminf(bottom, fabsf(vs[j]));
+      }
+      top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+      bottom = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(bottom)));
+      if (value_exp == -1000 && top > 0.f) value_exp = max((int)(__float_as_uint(top) >> 23), 5) - 131;
+      const float to_unit = value_exp == -1000 ? 0.f : two_to(-value_exp);
       float* slot = scales + (i % SLOTS) * 256 + lane * 4;
       *reinterpret_cast<float4*>(slot) = make_float4(ks[0], ks[1], ks[2], ks[3]);
-      *reinterpret_cast<float4*>(slot + 128) = make_float4(vs[0], vs[1], vs[2], vs[3]);
+      *reinterpret_cast<float4*>(slot + 128) = make_float4(vs[0] * to_unit, vs[1] * to_unit, vs[2] * to_unit, vs[3] * to_unit);
       if (lane == 0) {
-        NanKeys n;
-        n.any = 0;
+        TileInfo n;
+        n.any_nan = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) n.any |= n.key[j] = bad[j];
-        n.pad[0] = n.pad[1] = n.pad[2] = 0;
-        nan_keys[i % SLOTS] = n;
+        for (int j = 0; j < 4; ++j) n.any_nan |= n.nan[j] = bad[j];
+        n.wide = top * to_unit > 256.f || bottom * to_unit < 0x1p-13f;
+        n.value_exp = value_exp == -1000 ? 0 : value_exp;
+        n.pad = 0;
+        infos[i % SLOTS] = n;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sc_full[i % SLOTS]);
@@ -521,7 +542,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         row_now = row_next;
         row_next = row_of(i + 2);
         for (int item = 2 * i + 2; item < 2 * i + 4 && ok; ++item) {
-          if (item >= RING) ok = mbar_wait(&raw_empty[item % RING], (item / RING - 1) & 1);
+          if (item >= RING) ok = mbar_wait_brief(&raw_empty[item % RING], (item / RING - 1) & 1);
           ok = __all_sync(0xffffffffu, ok);
           if (ok) {
             send(item, row_now);
@@ -532,7 +553,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
     }
     // the last bytes that were sent for have arrived before this block's memory is another's
     for (int item = max(0, sent - RING); item < sent; ++item)
-      if (!mbar_wait(&raw_full[item % RING], (item / RING) & 1)) ok = false;
+      if (!mbar_wait_brief(&raw_full[item % RING], (item / RING) & 1)) ok = false;
   } else {
     // ---- conversion.  A warp has the even or the odd 64 codes of some groups of 8 rows; eight lanes a pair of rows r, r ^ 5,
     // whose pieces lie in different banks in the bytes' swizzle and in the 16-bit tile's.  Warps 12 and 13 have half of the
@@ -540,32 +561,40 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
     const int r8 = lane & 4 ? (lane >> 3) ^ 5 : lane >> 3, p = (warp & 1) * 4 + (lane & 3);
     const int g_from = warp < 12 ? 0 : warp < 14 ? 4 : 12, g_to = warp < 12 ? 4 : warp < 14 ? 12 : 16;
     const int src_off = r8 * 128 + ((p ^ r8) << 4), dst_off0 = piece_off(r8, 2 * p), dst_off1 = piece_off(r8, 2 * p + 1);
-    auto convert = [&](const unsigned char* src, unsigned char* dst, const float* vs, auto keys) {
-#pragma unroll 2
-      for (int g8 = g_from; g8 < g_to; ++g8) {
-        const uint4 w = *reinterpret_cast<const uint4*>(src + src_off + g8 * 1024);
-        const unsigned turned[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
-        const float scale = keys.value ? 0.f : vs[g8 * 8 + r8];
-        const float2 scale2 = make_float2(scale, scale);
-        unsigned y[8];
+    // codes times a scale (keys': 1, exactly) in float16; wide: codes in bfloat16
+    auto convert8 = [&](const unsigned char* src, unsigned char* dst, __half2 scale, int g8, auto wide) {
+      const uint4 w = *reinterpret_cast<const uint4*>(src + src_off + g8 * 1024);
+      const unsigned word[4] = {w.x, w.y, w.z, w.w};
+      unsigned y[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          y[2 * e] = keys.value ? codes_f16(turned[e], 0x4140) : codes_bf16(turned[e], 0x7540, scale2);
-          y[2 * e + 1] = keys.value ? codes_f16(turned[e], 0x4342) : codes_bf16(turned[e], 0x7542, scale2);
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const unsigned sel = half ? 0x4342 : 0x4140;
+          y[2 * e + half] = wide.value ? codes_bf16(word[e], sel) : times_f16(codes_f16(word[e] ^ 0x80808080u, sel), scale);
         }
-        *reinterpret_cast<uint4*>(dst + dst_off0 + g8 * 1024) = make_uint4(y[0], y[1], y[2], y[3]);
-        *reinterpret_cast<uint4*>(dst + dst_off1 + g8 * 1024) = make_uint4(y[4], y[5], y[6], y[7]);
-      }
+      *reinterpret_cast<uint4*>(dst + dst_off0 + g8 * 1024) = make_uint4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<uint4*>(dst + dst_off1 + g8 * 1024) = make_uint4(y[4], y[5], y[6], y[7]);
     };
     for (int item = 0, at = 0, turn = 0; item < 2 * ntiles && ok; ++item) {
       const int slot = (item >> 1) % SLOTS;
-      ok = (!(item & 1) || mbar_wait(&sc_full[slot], ((item >> 1) / SLOTS) & 1)) && mbar_wait(&raw_full[at], turn) &&
-           (item < RING || mbar_wait(&empty[at], turn ^ 1));
+      ok = (!(item & 1) || mbar_wait_brief(&sc_full[slot], ((item >> 1) / SLOTS) & 1)) && mbar_wait_brief(&raw_full[at], turn) &&
+           (item < RING || mbar_wait_brief(&empty[at], turn ^ 1));
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       const float* vs = scales + slot * 256 + 128;
-      if (item & 1) convert(raw + at * RAW_BYTES, sKV + at * TILE_BYTES, vs, std::false_type());
-      else convert(raw + at * RAW_BYTES, sKV + at * TILE_BYTES, vs, std::true_type());
+      const unsigned char* src = raw + at * RAW_BYTES;
+      unsigned char* dst = sKV + at * TILE_BYTES;
+      // (loops as short as they can be: what a warp runs seldom costs the others their instructions)
+      const bool values = item & 1;
+      if (__builtin_expect(values && infos[slot].wide, 0)) {
+#pragma unroll 1
+        for (int g8 = g_from; g8 < g_to; ++g8) convert8(src, dst, __half2(), g8, std::true_type());
+      } else {
+#pragma unroll 1
+        for (int g8 = g_from; g8 < g_to; ++g8)
+          convert8(src, dst, __float2half2_rn(values ? vs[g8 * 8 + r8] : 1.f), g8, std::false_type());
+      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the tile is read by the tensor core, the bytes are
       __syncwarp();                                                    // written by the next copy
       if (lane == 0) {
@@ -598,18 +627,19 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
     int uses_own = 0, uses_other = n_other;      // completed phases of s_full of the own columns and of the other's
     const int my_solo = x == solo_x ? solo_from : 0x7fffffff;
     const float2 unit2 = make_float2(row_unit, row_unit);
+    int value_exp = 0;
     for (int i = i_first; i <= i_last && ok; ++i) {
       const bool borrowed = i >= my_solo && ((i - my_solo) & 1);
       const int buf = borrowed ? 1 - x : x;
       const unsigned tmem_s = tmem + lane_base + buf * 128;
-      ok = mbar_wait(&sc_full[i % SLOTS], (i / SLOTS) & 1) && mbar_wait(&s_full[buf], (borrowed ? uses_other : uses_own) & 1);
+      ok = mbar_wait_brief(&sc_full[i % SLOTS], (i / SLOTS) & 1) && mbar_wait_brief(&s_full[buf], (borrowed ? uses_other : uses_own) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (borrowed) ++uses_other; else ++uses_own;
       tc_fence_after();
       const int kbase = (j0 + i) * TILE, first = lo - kbase, last = hi - kbase;      // visible: [first, last]
       const unsigned ks = smem_u32(scales + (i % SLOTS) * 256);
-      const NanKeys* nan = nan_keys + i % SLOTS;
+      const TileInfo* info = infos + i % SLOTS;
       unsigned v[4][32];
 #pragma unroll
       for (int c = 0; c < 4; ++c) tc_ld32(tmem_s + c * 32, v[c]);
@@ -623,7 +653,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
           v[c][k] = __float_as_uint(y.x);
           v[c][k + 1] = __float_as_uint(y.y);
         }
-      if (first > 0 || last < TILE - 1) {
+      if (__builtin_expect(first > 0 || last < TILE - 1, 0)) {
         // keys outside [first, last]: one subtraction and one unsigned comparison each
         const int first_vis = last >= first ? first : (1 << 20);
         const unsigned span = last >= first ? (unsigned)(last - first) : 0u;
@@ -641,10 +671,12 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
 #pragma unroll
         for (int c = 0; c < 4; ++c) m4[c] = max3(m4[c], __uint_as_float(v[c][k]), __uint_as_float(v[c][k + 1]));
       const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * row_unit;
-      if (nan->any) {      // a visible key that is no number: so is the row's result
+      if (__builtin_expect(info->any_nan, 0)) {      // a visible key that is no number: so is the row's result
         for (int k = max(first, 0); k <= min(last, TILE - 1); ++k)
-          if (nan->key[k & 3] >> (k >> 2) & 1) l = __int_as_float(0x7fc00000);
+          if (info->nan[k & 3] >> (k >> 2) & 1) l = __int_as_float(0x7fc00000);
       }
+      value_exp = info->value_exp;
+      const bool wide_tile = info->wide != 0;
       // the reference rises only when it must (or at the first visible key)
       float factor = 1.0f;
       bool rescale = false;
@@ -656,9 +688,9 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
       }
       // O of this tile is rescaled when a row of the warp raised its reference.  Its last product completed before these
       // scores did, except where the tile runs alone: the product of i - 1 is waited for there.
-      if (__any_sync(0xffffffffu, rescale)) {
+      if (__builtin_expect(__any_sync(0xffffffffu, rescale), 0)) {
         if (i > my_solo) {
-          ok = mbar_wait(pv_done, (i - 1 - my_solo) & 1);
+          ok = mbar_wait_brief(pv_done, (i - 1 - my_solo) & 1);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
@@ -676,32 +708,48 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
       const float offset = m_ref <= -1e29f ? 0.f : -m_ref;
       const float2 off2 = make_float2(offset, offset);
       float2 s8[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      auto weights = [&](int half, auto wide) {      // (wide: the values' scales join the probabilities)
 #pragma unroll
         for (int k = 0; k < 64; k += 2) {
           const int c = half * 2 + (k >> 5);
           const float2 y = __ffma2_rn(make_float2(__uint_as_float(v[c][k & 31]), __uint_as_float(v[c][(k & 31) + 1])), unit2, off2);
           const float2 p = make_float2(fast_exp2(y.x), fast_exp2(y.y));      // (exactly zero for a masked score)
           s8[(k >> 1) & 3] = __fadd2_rn(s8[(k >> 1) & 3], p);
-          v[half][k >> 1] = pack_bf16(p.x, p.y);
+          if (wide.value) {
+            const float2 w = __fmul2_rn(p, load_shared2(ks + (128 + half * 64 + k) * 4));
+            v[half][k >> 1] = pack_bf16(w.x, w.y);
+          } else {
+            v[half][k >> 1] = pack_f16(p.x, p.y);
+          }
         }
+      };
+      auto hand_over = [&](int half) {
         tc_st32(tmem_s + half * 32, v[half]);      // probabilities over the scores they came from
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * buf + half]);
+      };
+      if (__builtin_expect(wide_tile, 0)) {
+        weights(0, std::true_type());
+        hand_over(0);
+        weights(1, std::true_type());
+      } else {
+        weights(0, std::false_type());
+        hand_over(0);
+        weights(1, std::false_type());
       }
+      hand_over(1);
       l += ((s8[0].x + s8[0].y) + (s8[1].x + s8[1].y)) + ((s8[2].x + s8[2].y) + (s8[3].x + s8[3].y));
     }
     if (ok && i_last >= i_first) {
-      ok = mbar_wait(&o_final[x], 0);
+      ok = mbar_wait_brief(&o_final[x], 0);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
       // Outputs by way of the query tile, which nobody reads any more: a warp's 32 rows, then whole rows to memory.
       unsigned char* stage = sQ + x * TILE_BYTES + (warp & 3) * 8192;
       const bool partial = !(x ? whole[1] : whole[0]);      // this chunk's: O as accumulated (against m_ref), m_ref, l
-      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      const float inv = l == 0.f ? 0.f : 1.0f / l, value_unit = two_to(value_exp);
       const int my_ntok = x ? ntok[1] : ntok[0], row0 = (warp & 3) * 32;
       auto row_of_lane = [&](int rr) {      // the row of the output that is row rr of this tile, or -1
         const int t = token_of(rr);
@@ -716,10 +764,11 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
             unsigned o[32];
             tc_ld32(tmem_o + half * 64 + c * 32, o);
             tc_wait_ld();
+            auto value = [&](int e) { return __float_as_uint(__uint_as_float(o[e]) * value_unit); };
 #pragma unroll
             for (int ch = 0; ch < 8; ++ch)
               *reinterpret_cast<uint4*>(stage + lane * 256 + ((c * 8 + ch) ^ (lane & 7)) * 16) =
-                  make_uint4(o[ch * 4], o[ch * 4 + 1], o[ch * 4 + 2], o[ch * 4 + 3]);
+                  make_uint4(value(ch * 4), value(ch * 4 + 1), value(ch * 4 + 2), value(ch * 4 + 3));
           }
           __syncwarp();
 #pragma unroll 4
@@ -737,7 +786,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
           unsigned o[32];
           tc_ld32(tmem_o + c * 32, o);
           tc_wait_ld();
-          auto value = [&](int e) { return __uint_as_float(o[e]) * inv; };
+          auto value = [&](int e) { return __uint_as_float(o[e]) * inv * value_unit; };
 #pragma unroll
           for (int ch = 0; ch < 4; ++ch)
             *reinterpret_cast<uint4*>(stage + lane * 256 + ((c * 4 + ch) ^ (lane & 7)) * 16) =

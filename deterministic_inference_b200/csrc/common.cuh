@@ -358,3 +358,20 @@ __device__ __forceinline__ bool mbar_wait(unsigned long long* bar, unsigned pari
     }
   }
 }
+// The same in as few instructions as it takes, for kernels whose roles share the instruction cache: the limit is a number of
+// tries, each of which may sleep 256 ns (a second in all, or so).
+__device__ __forceinline__ bool mbar_wait_brief(unsigned long long* bar, unsigned parity) {
+  const unsigned addr = (unsigned)__cvta_generic_to_shared(bar);
+#pragma unroll 1
+  for (unsigned i = 0; i < (1u << 22); ++i) {
+    unsigned ok;
+    asm volatile(
+        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 256; "
+        "selp.u32 %0, 1, 0, p; }"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  }
+  return false;
+}

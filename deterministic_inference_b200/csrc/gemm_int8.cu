@@ -415,7 +415,7 @@ gemm_large_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       pdl_wait();
       for (int c = 0; c < pre; ++c) load_x(c);
       for (int c = pre; c < total && ok; ++c) {
-        ok = mbar_wait(&empty[c % STAGES], ((c / STAGES) - 1) & 1);
+        ok = mbar_wait_brief(&empty[c % STAGES], ((c / STAGES) - 1) & 1);
         if (!ok) break;
         if (rank == 0) mbar_expect_tx(&full[c % STAGES], CTAS * STAGE);
         load_w(c);
@@ -431,13 +431,13 @@ gemm_large_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       for (int t = group; t < tiles && ok; t += groups, ++local) {
         const int buf = local & 1;
         if (local >= 2) {      // the epilogue must have read this buffer's earlier tile
-          ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((local >> 1) - 1) & 1));
+          ok = __all_sync(0xffffffffu, mbar_wait_brief(&acc_empty[buf], ((local >> 1) - 1) & 1));
           if (!ok) break;
           tc_fence_after();
         }
         for (int kb = 0; kb < a.num_kb && ok; ++kb, ++count) {
           const int s = count % STAGES;
-          ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (count / STAGES) & 1));
+          ok = __all_sync(0xffffffffu, mbar_wait_brief(&full[s], (count / STAGES) & 1));
           if (!ok) break;
           tc_fence_after();
           const unsigned long long da = smem_desc(smem_u32(smem + s * STAGE)), db = smem_desc(smem_u32(smem + s * STAGE) + A_BYTES);
@@ -458,7 +458,7 @@ gemm_large_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     int local = 0;
     for (int t = group; t < tiles; t += groups, ++local) {
       const int buf = local & 1;
-      bool got = ok && mbar_wait(&acc_full[buf], (local >> 1) & 1);
+      bool got = ok && mbar_wait_brief(&acc_full[buf], (local >> 1) & 1);
       got = __all_sync(0xffffffffu, got);      // tcgen05.ld below is warp-wide
       if (!got) {
         ok = false;
@@ -559,7 +559,7 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       pdl_wait();
       for (int c = 0; c < pre; ++c) load_x(c);
       for (int c = pre; c < count; ++c) {
-        ok = mbar_wait(&empty[c % a.stages], ((c / a.stages) - 1) & 1);
+        ok = mbar_wait_brief(&empty[c % a.stages], ((c / a.stages) - 1) & 1);
         if (!ok) break;
         load_w(c);
         load_x(c);
@@ -570,7 +570,7 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     constexpr unsigned idesc = make_idesc(BM, BNL);
     for (int c = 0; c < count; ++c) {
       const int s = c % a.stages;
-      ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (c / a.stages) & 1));
+      ok = __all_sync(0xffffffffu, mbar_wait_brief(&full[s], (c / a.stages) & 1));
       if (!ok) break;
       tc_fence_after();
       const unsigned long long db = smem_desc(smem_u32(smem) + s * stage), da = smem_desc(smem_u32(smem) + s * stage + b_bytes);
@@ -584,7 +584,7 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     // ---- integers to shared memory, over the ring: all of its copies have been read
     const int row = (warp - 4) * 32 + lane;
     if ((warp - 4) * 32 < a.a_rows) {
-      ok = mbar_wait(&acc_full, 0);
+      ok = mbar_wait_brief(&acc_full, 0);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
       if (ok)
