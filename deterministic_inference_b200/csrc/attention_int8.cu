@@ -200,7 +200,8 @@ struct __align__(16) SplitItem {
   int i, kvh, tile, local;          // sequence of the launch, kv head, tile of rows, number of the item in its sequence
   int run_at, at, end, splits;      // first key of the run; its keys [at, end), `at` a multiple of 128 and perhaps before the
                                     // first one seen; runs of the sequence
-  int fresh, tiles, unused0, unused1;      // other query rows than the item before; tiles of keys, 0: there are no more items
+  int fresh, tiles, lo_all, hi_all;        // other query rows than the item before; tiles of keys, 0: there are no more
+                                           // items; the keys that every row sees
 };
 
 __device__ __forceinline__ float4 four_floats(const float4& v) { return v; }
@@ -485,6 +486,8 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
           continue;
         }
         it.tiles = (it.end - it.at + SP_TILE - 1) / SP_TILE;
+        it.lo_all = max(it.run_at, first_visible_key(p0 + tok1, a.window));
+        it.hi_all = min(it.end - 1, p0 + tok0);
         it.fresh = i != old_i || it.kvh != old_kvh || it.tile != old_tile;
         old_i = i; old_kvh = it.kvh; old_tile = it.tile;
       }
@@ -670,7 +673,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[slot]);
       if (it.tiles == 0) break;
-      const int row0 = it.tile * ROWS, rows = min(ROWS, it.n * G - row0), p0 = it.kv_len - it.n;
+      const int row0 = it.tile * ROWS, rows = min(ROWS, it.n * G - row0);
       if (it.fresh) {
         if (q_used >= 0 && lane == 0) mbar_arrive(&q_empty[q_used & 1]);
         ++q_used;
@@ -679,9 +682,6 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
         if (!ok) break;
       }
       const float* data = row_data + (q_used & 1) * 3 * ROWS;
-      // the keys that every row sees
-      const int lo_all = max(it.run_at, first_visible_key(p0 + (row0 + rows - 1) / G, a.window));
-      const int hi_all = min(it.end - 1, p0 + row0 / G);
       for (int kb = it.at; kb < it.end; kb += SP_TILE, ++n) {
         const int buf = n & 1;
         ok = mbar_wait_brief(&k_full[buf], (n >> 1) & 1) && mbar_wait_brief(&s_full[buf], (n >> 1) & 1);
@@ -692,7 +692,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
         const float vs_raw = scales[buf * 256 + 128 + key_of];
         const float ks = scales[buf * 256 + key_of] + (vs_raw - vs_raw);      // NaN if either is
         const int key = kb + key_of;
-        const bool plain = kb >= lo_all && kb + SP_TILE - 1 <= hi_all;        // every row sees every key
+        const bool plain = kb >= it.lo_all && kb + SP_TILE - 1 <= it.hi_all;        // every row sees every key
         const bool there = key >= it.run_at && key < it.end;
         const float vs = there ? vs_raw : 0.f, lv = there ? fmaxf(__log2f(vs), -120.f) : -INFINITY;
         float s[ROWS];
