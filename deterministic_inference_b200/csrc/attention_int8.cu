@@ -493,7 +493,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       }
       // the query rows' loads, some rows at a time, go out ahead of the copies that the record sets off
       const int row0 = it.tile * ROWS, rows = min(ROWS, it.n * G - row0);
-      constexpr int AHEAD = PARTS == 4 || ROWS < 8 ? 4 : 8;
+      constexpr int AHEAD = 4;      // (few, and not unrolled further: instructions that a warp runs seldom cost the others theirs)
       typename SH::Four raw[AHEAD];        // 4 elements of a row
       int tok = row0 / G, head = row0 - tok * G;      // of the next row to be loaded
       const T* src = q + ((long long)(it.q_begin + tok) * a.Hq + it.kvh * G + head) * a.D + lane * 4;
@@ -527,8 +527,9 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       if (!ok) break;
       unsigned char* dst = smem + SH::QUERIES + buf * N * 128;
       float* data = row_data + buf * 3 * ROWS;
-      int pos = it.kv_len - it.n + tok, pos_head = row0 - tok * G;      // of the next row to be made
-#pragma unroll
+      unsigned my_bits = 0;      // of the row that is this lane's number
+      float my_up = 1.f;
+#pragma unroll 1
       for (int from = 0; from < ROWS; from += AHEAD) {
         if (from > 0) load_rows(from);
 #pragma unroll
@@ -550,17 +551,18 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
             *reinterpret_cast<unsigned*>(dst + col * 128 + (((lane >> 2) ^ (col & 7)) << 4) + (lane & 3) * 4) =
                 low_bytes(part[0][p], part[1][p], part[2][p], part[3][p]);
           }
-          if (lane == 0) {
-            // (a row that holds an infinity or a NaN: its unit is NaN, and so is all that comes of it)
-            data[r] = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __fdiv_rn(a.scale * LOG2E, up);
-            data[ROWS + r] = __int_as_float(first_visible_key(pos, a.window));
-            data[2 * ROWS + r] = __int_as_float(r < rows ? pos : -1);
-          }
-          if (++pos_head == G) {
-            pos_head = 0;
-            ++pos;
+          if (lane == r) {
+            my_bits = bits;
+            my_up = up;
           }
         }
+      }
+      if (lane < ROWS) {      // lane r: what belongs to row r
+        // (a row that holds an infinity or a NaN: its unit is NaN, and so is all that comes of it)
+        const int pos = it.kv_len - it.n + (row0 + lane) / G;
+        data[lane] = my_bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __fdiv_rn(a.scale * LOG2E, my_up);
+        data[ROWS + lane] = __int_as_float(first_visible_key(pos, a.window));
+        data[2 * ROWS + lane] = __int_as_float(lane < rows ? pos : -1);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the rows are read by the tensor core
       __syncwarp();
