@@ -4,7 +4,8 @@
 // kc, vc the codes of a key and a value, ks, vs their scales.  The scales never touch the codes: a key's joins its score,
 // a value's the probability.  A row that sees no key is zeros.  A sequence's new tokens are its last ones.
 //
-// Forms: split (one to a few new tokens: the cache is streamed once and bounds it), and one for every shape.
+// Forms: split (one to a few new tokens, and every float32 portion: the cache is streamed once), one for every shape (heads
+// above 128, pages that are not a power of two), and attention_int8_prompt.cu for bfloat16 portions of many rows.
 #include <cuda.h>
 
 #include "common.cuh"
@@ -48,9 +49,13 @@ __device__ __forceinline__ float fast_exp2(float x) {
 // integers are then scaled and added up in float32.  L, the reference of a row's probabilities, follows the tiles'
 // largest weights and is raised only when they have left it by 2^20: float32 holds what lies between.
 //
-// What bounds it: the bytes of keys and values.  A thread has a key (then a dimension) and ROWS rows: some 20
-// instructions a key and row, a quarter of what mma.sync on converted codes takes.  Three CTAs an SM, each with a tile
-// on its way and one in use, cover the trips between copy, tensor core and threads.
+// What bounds it: the bytes of keys and values for up to 4 rows, the threads above.  A thread has a key (then a dimension)
+// and ROWS rows: some 20 instructions a key and row, a quarter of what mma.sync on converted codes takes.  Three CTAs an SM
+// (two above 8 rows), each with a tile on its way and one in use, cover the trips between copy, tensor core and threads.  An
+// item's beginning and end cost as much as a tile or two, through instructions that are not in the cache any more: they are
+// kept few.  Heads of 128, 8 kv heads: 64 requests of up to 4,096 keys, 4 rows each, 67.5 us (312 MB at 4.6 TB/s); four of
+// 32,000, 8 rows, 58.9 us (270 MB at 4.6 TB/s), of which the last CTA is 7 us behind the median and the merge takes 6; sixteen of up to 1,500
+// with 10 rows 25.1 us (31 MB), with 20 rows at 4,096 keys 75 us (tiles of 24 rows; 104 us in tiles of 32); one of 2,048, 8.7 us.
 //
 // Roles in a CTA: warps 0-3 softmax (TMEM lane = key, dimension), warp 4 copies (TMA, a box a page; scales by cp.async),
 // warp 5 issues the scores' products, warp 7 the outputs', warp 6 finds the next work items and makes their query rows.

@@ -1,26 +1,37 @@
 // Attention of a prompt's portion over a paged cache in 8-bit integers (cache_int8.cu; formulas in attention_int8.cu), for
-// bfloat16 queries and many rows: S = Q K^T and O = P V by tcgen05.mma kind::f16 on bfloat16, accumulators in tensor memory,
-// a thread a query row for the softmax.
+// bfloat16 queries and many rows: S = Q K^T and O = P V by tcgen05.mma kind::f16, accumulators in tensor memory, a thread a
+// query row for the softmax.
 //
-// The codes are exact in bfloat16, so they enter both products as they are: six warps turn a key tile's bytes (fetched by
-// TMA, a box a page) into swizzled bfloat16 tiles, once for the 256 rows of the two query tiles that share them.  A key's
-// scale (times the softmax's) joins its column of the scores, a value's the probabilities before they are rounded to
-// bfloat16 for the second product; the sum of probabilities is taken before that.
+// Numbers.  Keys enter the first product as their codes, which float16 holds exactly, queries in float16 times a power of
+// two of their row (exact: bfloat16 has fewer bits); a key's scale (times the softmax's) joins its column of the scores in
+// float32.  Values enter the second product as code times scale in float16 (11 bits, two roundings of 2^-12), in units of a
+// power of two, the probabilities in float16; their sum is taken in float32 before that.  Against 64 bits the output is off by
+// its own rounding to bfloat16, 0.0017 of its norm (with bfloat16 probabilities it was 0.0024, with bfloat16 values too
+// 0.0028).  A tile with a value's scale outside 2^-17 .. 2^3 of the first tile's largest is "wide": codes in bfloat16, exactly,
+// and the scales joined to probabilities in bfloat16, whose range is float32's.
+//
+// Six warps turn a key tile's bytes (fetched by TMA, a box a page) into swizzled 16-bit tiles, once for the 256 rows of the
+// two query tiles that share them.
 //
 // Two query tiles A and B of 128 rows (tokens x heads of a kv group) of one sequence a CTA.  Roles: warps 0-3 softmax of A,
-// 4-7 of B (a row's 128 scores in registers; probabilities go back to tensor memory over the scores and are the second
-// product's operand from there), warp 9 issues the products, warp 8 sends for bytes and scales, warps 10-12 convert
-// keys, 13-15 values.
+// 4-7 of B (a row's 128 scores in registers; probabilities go back to tensor memory over the scores, half a tile at a time, and
+// are the second product's operand from there), warp 9 issues the products (in code that all its lanes run, which keeps
+// descriptors in uniform registers: 641 -> 566 us at 3,000 tokens on 4,096), warp 8 sends for bytes and scales, warps 10-15 convert.
 // The products of the two tiles are staggered, each tile's softmax runs under the other's products.  Once a tile has had
 // its last key tile (or there is no B) the other runs alone and takes its score columns as a second buffer.
 // Tensor memory: S/P of A columns 0.., of B 128.., O of A 256.., of B 384...
 //
 // Keys are cut at multiples of 4,096 (chunks of constant size from key 0); a query tile that reaches over a cut has a CTA a
-// chunk, and a second kernel adds the partial results in chunk order.  Key tiles are anchored at key 0 and cuts depend on
-// positions alone, so a row's bits do not depend on the step.
+// chunk, and a second kernel adds the partial results in chunk order.  Key tiles are anchored at key 0, cuts depend on
+// positions alone and units are powers of two, so a row's bits do not depend on the step (but for wide tiles, which a
+// portion's first tile and the keys there are decide).
 //
-// What bounds it: the softmax threads' instructions (a score's scale, maximum, exponential, sum, value scale and packing),
-// with the conversion beside them; the products take half of that time.
+// What bounds it: 2.5 us a key tile for both query tiles, of which the products need 1.1.  A query tile's chain is its
+// scores' way out of tensor memory, scales, maximum, exponentials, packing (some 700 instructions a warp) and the next
+// products; the schedulers are shared with the conversion, and with the instruction cache: what a warp runs seldom is kept
+// short or out of the way.  A CTA's beginning and end cost 9 us more.  One CTA an SM (213 KB).  Two threads a row were
+// slower (635 -> 852 us: registers spilled), as were exponentials shared with the FMA pipe (506 -> 518).
+// 2,048 tokens, 32 / 8 heads of 128: 56.7 us, 606 TFLOP/s.  3,000 tokens on 4,096 keys: 455 us.
 #include <cuda.h>
 #include <cuda_fp16.h>
 

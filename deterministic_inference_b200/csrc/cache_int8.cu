@@ -135,8 +135,8 @@ static inline Divisor make_divisor(unsigned d) {
 }
 
 // A row of the cache: 128 values are LANES lanes, 32 bytes of the unquantised row each.  Memory bound: many warps of few
-// registers and few instructions.  16 values a lane of several rows a group took 93 registers and 37 us where this takes
-// 20 us: 8,000 tokens of 8 heads of 128 written from bfloat16, 99 MB at 5.0 TB/s.
+// registers and few instructions: 8,000 tokens of 8 heads of 128 written from bfloat16 and read back in 19.4 us, 99 MB at
+// 5.1 TB/s (16 values a lane of several rows a group: 93 registers, 37 us).
 constexpr int CACHE_THREADS = 256;
 template <typename T> struct Rows {
   static constexpr int N = Piece<T>::N, LANES = 128 / N, GROUPS = CACHE_THREADS / LANES;
@@ -215,8 +215,8 @@ cache_write_kernel(const T* __restrict__ k, const T* __restrict__ v, long long k
   if (l == 0) scales[c.at] = scale.scale;
 }
 
-// ROWS rows a group, all asked for before the first is used: 193 MB of float32 read back in 36.8 us (5.3 TB/s) at 2, 42.0 at
-// 1, 40.6 at 4.
+// ROWS rows a group, all asked for before the first is used: 194 MB of float32, most of it read back, in 36.0 us (5.4 TB/s) at
+// 2, 42.0 at 1, 40.6 at 4.
 template <typename T, int HALVES, int ROWS>
 __global__ void __launch_bounds__(CACHE_THREADS)
 cache_read_kernel(const signed char* __restrict__ data, const float* __restrict__ scales, const int* __restrict__ slots,

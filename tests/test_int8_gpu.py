@@ -320,6 +320,35 @@ def test_attention_of_uneven_value_scales(q_len, dtype):
     _check_attention(case, [q_len, q_len], 4, dtype, window=1)
 
 
+@pytest.mark.parametrize("step", [1 / 24, -1 / 24, 1 / 400])
+@pytest.mark.parametrize("keys,q_len", [(700, 1), (700, 300), (4500, 200)])
+def test_attention_of_value_scales_that_drift(keys, q_len, step):
+    """Scales that leave the first keys' range along the sequence, within it and across its chunks."""
+    scales = lambda n, hkv, g: (2.0 ** (torch.arange(n) * step).clamp(-40, 40))[:, None].expand(n, hkv).contiguous()
+    case = Int8Case([keys, keys // 2], 2, 128, 16, seed=q_len, value_scales=scales)
+    _check_attention(case, [q_len, q_len], 4, BF16)
+    _check_attention(case, [q_len, q_len], 4, BF16, window=64)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("scale", [0.0, -0.07])
+def test_attention_of_zero_and_negative_scales(scale, dtype):
+    case = Int8Case([500, 300, 77], 2, 128, 16, seed=8)
+    _check_attention(case, [200, 4, 1], 8, dtype, scale=scale)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (6, 2, 64)])
+def test_a_prompt_attends_the_same_in_any_portion(hq, hkv, d):
+    """The bits of a prompt's rows do not depend on where its portions begin."""
+    case = Int8Case([900], hkv, d, 16, seed=6)
+    q = _rand(500, hq, d, seed=7, dtype=BF16)
+    cache = ops.Int8Cache(case.data, case.scales)
+    whole = ops.int8_paged_attention(q, cache, case.meta([500]), 0.1)
+    for n in (450, 333, 128, 70):
+        got = ops.int8_paged_attention(q[500 - n:].contiguous(), cache, case.meta([n]), 0.1)
+        assert torch.equal(got, whole[500 - n:])
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("q_len", [1, 150])
 @pytest.mark.parametrize("q_scale", [1e-30, 3e4, 1e8])
