@@ -57,8 +57,27 @@ template <bool STREAM> __device__ __forceinline__ void load32(const signed char*
   }
 }
 
+// The same for rows that lie on 32 bytes (WIDE): one load, so that no sector is asked for twice.
+template <bool STREAM, bool WIDE>
+__device__ __forceinline__ void load_row(const signed char* row, bool in, int k, int Kp, uint4 (&v)[2]) {
+  if (!WIDE) {
+    load32<STREAM>(row, in, k, Kp, v);
+    return;
+  }
+  v[0] = v[1] = make_uint4(0, 0, 0, 0);
+  if (!in || k >= Kp) return;
+  if (STREAM)
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0].x), "=r"(v[0].y), "=r"(v[0].z), "=r"(v[0].w), "=r"(v[1].x), "=r"(v[1].y), "=r"(v[1].z), "=r"(v[1].w)
+                 : "l"(row + k));
+  else
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0].x), "=r"(v[0].y), "=r"(v[0].z), "=r"(v[0].w), "=r"(v[1].x), "=r"(v[1].y), "=r"(v[1].z), "=r"(v[1].w)
+                 : "l"(row + k));
+}
+
 // NT tiles of 8 tokens
-template <typename OutT, int NT>
+template <typename OutT, int NT, bool WIDE>
 __global__ void __launch_bounds__(FEW_WARPS * 32)
 gemm_few_kernel(const signed char* __restrict__ x, const float* __restrict__ sx, const signed char* __restrict__ w,
                 const float* __restrict__ sw, OutT* __restrict__ out, int M, int N, int Kp) {
@@ -73,18 +92,18 @@ gemm_few_kernel(const signed char* __restrict__ x, const float* __restrict__ sx,
   int k = warp * CHUNK + t * 32;
   uint4 a[2], b[2];
   // the weights are constants: the first step's are on their way before the wait for the kernel in front
-  load32<true>(w0, in0, k, Kp, a);
-  load32<true>(w1, in1, k, Kp, b);
+  load_row<true, WIDE>(w0, in0, k, Kp, a);
+  load_row<true, WIDE>(w1, in1, k, Kp, b);
   pdl_wait(x, sx);
   for (; k - t * 32 < Kp; k += FEW_WARPS * CHUNK) {
     const uint4 ca[2] = {a[0], a[1]}, cb[2] = {b[0], b[1]};
-    load32<true>(w0, in0, k + FEW_WARPS * CHUNK, Kp, a);
-    load32<true>(w1, in1, k + FEW_WARPS * CHUNK, Kp, b);
+    load_row<true, WIDE>(w0, in0, k + FEW_WARPS * CHUNK, Kp, a);
+    load_row<true, WIDE>(w1, in1, k + FEW_WARPS * CHUNK, Kp, b);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int m = m0 + nt * 8 + g;
       uint4 c[2];
-      load32<false>(x + (long long)m * Kp, m < M, k, Kp, c);
+      load_row<false, WIDE>(x + (long long)m * Kp, m < M, k, Kp, c);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         mma_s8(acc[nt], ca[i].x, cb[i].x, ca[i].y, cb[i].y, c[i].x, c[i].y);
@@ -116,7 +135,9 @@ int launch_few(const void* x, const void* sx, const void* w, const void* sw, voi
   const int nt = M <= 8 ? 1 : M <= 16 ? 2 : 4;
   const dim3 grid((N + FEW_ROWS - 1) / FEW_ROWS, (M + nt * 8 - 1) / (nt * 8));
   if (grid.y > 65535) return DIB_BAD_SIZE;
-  auto kern = nt == 1 ? gemm_few_kernel<OutT, 1> : nt == 2 ? gemm_few_kernel<OutT, 2> : gemm_few_kernel<OutT, 4>;
+  auto kern = nt == 1 ? gemm_few_kernel<OutT, 1, false> : nt == 2 ? gemm_few_kernel<OutT, 2, false> : gemm_few_kernel<OutT, 4, false>;
+  if (Kp % 32 == 0 && (reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(x)) % 32 == 0)
+    kern = nt == 1 ? gemm_few_kernel<OutT, 1, true> : nt == 2 ? gemm_few_kernel<OutT, 2, true> : gemm_few_kernel<OutT, 4, true>;
   dib_launch(kern, grid, dim3(FEW_WARPS * 32), 0, st, reinterpret_cast<const signed char*>(x),
              reinterpret_cast<const float*>(sx), reinterpret_cast<const signed char*>(w),
              reinterpret_cast<const float*>(sw), reinterpret_cast<OutT*>(out), M, N, Kp);
