@@ -8,10 +8,11 @@
 // operands agree, so a thread takes 32 consecutive bytes of its two weight rows (two 16-byte loads each) and calls them
 // the k it needs; the tokens' rows are read the same way, from L2.  A block of eight warps takes 16 channels; the warps
 // share the row's k among them and add their integers up in shared memory.  Bound by memory: 8 tokens on 24,576 x 4,096
-// 20 us (5.0 TB/s), on 4,096 x 4,096 6.4 us, where the launch and one trip to memory are most of it.
+// 19 us (5.3 TB/s), on 4,096 x 4,096 5.8 us, where the launch and a few trips to memory are most of it (two or four steps of
+// the weight on their way instead of one: 6.9 and 7.4 us, 22 and 34, for want of warps).
 //
 // Some rows, or few against long channels: clusters of up to eight CTAs share a tile's k (gemm_split_kernel), so that all SMs
-// fetch a weight whose tiles are fewer than they are: 32 tokens on 4,096 x 12,288 13.3 us (3.8 TB/s; 30.5 us streamed, 32 on a
+// fetch a weight whose tiles are fewer than they are: 32 tokens on 4,096 x 12,288 13.8 us (3.7 TB/s; 19.6 us streamed, 32 on a
 // CTA a tile).
 //
 // Many rows: persistent kernels on the 5th-generation tensor cores (tcgen05.mma kind::i8), one CTA an SM on tiles of 128
@@ -825,12 +826,12 @@ int large_form(int M, int N, int sm_count) {
   if (m_tiles * ((N + 127) / 128) <= sm_count / 2) return 1;
   return 2 * m_tiles * ((N + 255) / 256) <= sm_count ? 2 : 3;
 }
-// Up to 256 rows the times of the forms are estimated, in us, from lines through measured ones (K-blocks of 128):
-//   streamed weight, 8 rows     1,024 x 1,024 1.8, 4,096 x 4,096 6.4, 24,576 x 4,096 20, 4,096 x 12,288 15, 5,120 x 25,600 30;
-//                               16, 24, 32 rows take 1.3, 1.85, 2 times that, as a block fetches its tokens from L2
-//   clusters, 128 wide          32 rows: 4,096 x 4,096 8.4, 6,144 x 4,096 9.6, 4,096 x 12,288 13.3, 5,120 x 25,600 26.5
+// Up to 256 rows the times of the forms are estimated, in us, from lines through measured ones (k-blocks of 128):
+//   streamed weight, 8 rows     1,024 x 1,024 1.6, 4,096 x 4,096 5.8, 24,576 x 4,096 18.7, 4,096 x 12,288 12.6, 5,120 x 25,600 26;
+//                               16, 24, 32 rows take some 1.2, 1.4, 1.55 times that, as a block fetches its tokens from L2
+//   clusters, 128 wide          32 rows: 4,096 x 4,096 8.8, 6,144 x 4,096 9.8, 4,096 x 12,288 13.8, 5,120 x 25,600 26.5
 //                               128 rows: 13.5, 14.1, 18.4, 32.3
-//   clusters, 64 wide           32 rows: 2,560 x 4,096 8.0, 4,096 x 4,096 9.3; 128 rows: 10.1, 10.6
+//   clusters, 64 wide           32 rows: 2,560 x 4,096 8.0, 4,096 x 4,096 9.5; 128 rows: 10.1, 10.6
 //   a tile a CTA                4,096 x 4,096 12.7, 4,096 x 12,288 32, 5,120 x 25,600 65
 template <typename OutT>
 int form(int M, int N, int Kp, int sm_count) {
@@ -847,7 +848,7 @@ int form(int M, int N, int Kp, int sm_count) {
     }
   };
   if (M <= 16 || (M <= 32 && N <= 48 * sm_count))
-    consider(0, (0.8f + 0.75e-3f * Kp + (float)N * Kp / 6.5e6f) * (M <= 8 ? 1.f : M <= 16 ? 1.3f : M <= 24 ? 1.85f : 2.f));
+    consider(0, (1.2f + 0.5e-3f * Kp + (float)N * Kp / 6.8e6f) * (M <= 8 ? 1.f : M <= 16 ? 1.2f : M <= 24 ? 1.42f : 1.55f));
   if (M > 16) {
     const int width = large == 1 ? 64 : large == 2 ? 128 : 256, tiles = m_tiles * ((N + width - 1) / width);
     consider(large, 2.8f + 0.31f * num_kb * ((tiles + sm_count - 1) / sm_count));
@@ -855,8 +856,8 @@ int form(int M, int N, int Kp, int sm_count) {
   const int tiles64 = m_tiles * ((N + 63) / 64), tiles128 = m_tiles * ((N + 127) / 128);
   const int s64 = 2 * tiles64 <= sm_count ? split_of<OutT, 64>(tiles64, num_kb) : 1;
   const int s128 = 2 * tiles128 <= sm_count ? split_of<OutT, 128>(tiles128, num_kb) : 1;
-  if (s64 > 1) consider(5, 4.f + 0.33f * ((num_kb + s64 - 1) / s64) + (M > 64 ? 1.5f : M > 32 ? 0.5f : 0.f));
-  if (s128 > 1) consider(6, 4.f + 0.40f * ((num_kb + s128 - 1) / s128) + (M > 64 ? 5.f : M > 32 ? 1.7f : 0.f));
+  if (s64 > 1) consider(5, 4.6f + 0.33f * ((num_kb + s64 - 1) / s64) + (M > 64 ? 1.2f : M > 32 ? 0.3f : 0.f));
+  if (s128 > 1) consider(6, 5.f + 0.35f * ((num_kb + s128 - 1) / s128) + (M > 64 ? 4.5f : M > 32 ? 1.7f : 0.f));
   return choice;
 }
 
