@@ -8,8 +8,8 @@
 // operands agree, so a thread takes 32 consecutive bytes of its two weight rows (two 16-byte loads each) and calls them
 // the k it needs; the tokens' rows are read the same way, from L2.  A block of eight warps takes 16 channels; the warps
 // share the row's k among them and add their integers up in shared memory.  Bound by memory: 8 tokens on 24,576 x 4,096
-// 19 us (5.3 TB/s), on 4,096 x 4,096 5.8 us, where the launch and a few trips to memory are most of it (two or four steps of
-// the weight on their way instead of one: 6.9 and 7.4 us, 22 and 34, for want of warps).
+// 19 us (5.3 TB/s), on 4,096 x 4,096 5.8 us, where the launch and a few trips to memory are most of it (with two to four steps
+// of the weight on their way instead of one no faster, and 21 to 23 us for the former, for want of warps).
 //
 // Some rows, or few against long channels: clusters of up to eight CTAs share a tile's k (gemm_split_kernel), so that all SMs
 // fetch a weight whose tiles are fewer than they are: 32 tokens on 4,096 x 12,288 13.8 us (3.7 TB/s; 19.6 us streamed, 32 on a
@@ -77,9 +77,9 @@ __device__ __forceinline__ void load_row(const signed char* row, bool in, int k,
                  : "l"(row + k));
 }
 
-// NT tiles of 8 tokens
+// NT tiles of 8 tokens.  (Three blocks an SM with two tiles and more: 16 tokens on 6,144 x 4,096 7.1 us, with two 9.1.)
 template <typename OutT, int NT, bool WIDE>
-__global__ void __launch_bounds__(FEW_WARPS * 32)
+__global__ void __launch_bounds__(FEW_WARPS * 32, NT == 1 ? 4 : 3)
 gemm_few_kernel(const signed char* __restrict__ x, const float* __restrict__ sx, const signed char* __restrict__ w,
                 const float* __restrict__ sw, OutT* __restrict__ out, int M, int N, int Kp) {
   pdl_trigger();
@@ -96,19 +96,29 @@ gemm_few_kernel(const signed char* __restrict__ x, const float* __restrict__ sx,
   load_row<true, WIDE>(w0, in0, k, Kp, a);
   load_row<true, WIDE>(w1, in1, k, Kp, b);
   pdl_wait(x, sx);
+  // (the tokens a step ahead too, where there are tiles enough for it to show: 16 of them on 4,096 x 4,096 6.7 -> 6.2 us, but 8
+  // on 24,576 x 4,096 19.4 -> 19.9)
+  constexpr bool AHEAD = NT > 1;
+  uint4 c[NT][2];
+  auto load_tokens = [&](int nt, int at) {
+    load_row<false, WIDE>(x + (long long)(m0 + nt * 8 + g) * Kp, m0 + nt * 8 + g < M, at, Kp, c[nt]);
+  };
+  if (AHEAD)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) load_tokens(nt, k);
   for (; k - t * 32 < Kp; k += FEW_WARPS * CHUNK) {
     const uint4 ca[2] = {a[0], a[1]}, cb[2] = {b[0], b[1]};
     load_row<true, WIDE>(w0, in0, k + FEW_WARPS * CHUNK, Kp, a);
     load_row<true, WIDE>(w1, in1, k + FEW_WARPS * CHUNK, Kp, b);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int m = m0 + nt * 8 + g;
-      uint4 c[2];
-      load_row<false, WIDE>(x + (long long)m * Kp, m < M, k, Kp, c);
+      if (!AHEAD) load_tokens(nt, k);
+      const uint4 cc[2] = {c[nt][0], c[nt][1]};
+      if (AHEAD) load_tokens(nt, k + FEW_WARPS * CHUNK);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        mma_s8(acc[nt], ca[i].x, cb[i].x, ca[i].y, cb[i].y, c[i].x, c[i].y);
-        mma_s8(acc[nt], ca[i].z, cb[i].z, ca[i].w, cb[i].w, c[i].z, c[i].w);
+        mma_s8(acc[nt], ca[i].x, cb[i].x, ca[i].y, cb[i].y, cc[i].x, cc[i].y);
+        mma_s8(acc[nt], ca[i].z, cb[i].z, ca[i].w, cb[i].w, cc[i].z, cc[i].w);
       }
     }
   }
@@ -828,7 +838,7 @@ int large_form(int M, int N, int sm_count) {
 }
 // Up to 256 rows the times of the forms are estimated, in us, from lines through measured ones (k-blocks of 128):
 //   streamed weight, 8 rows     1,024 x 1,024 1.6, 4,096 x 4,096 5.8, 24,576 x 4,096 18.7, 4,096 x 12,288 12.6, 5,120 x 25,600 26;
-//                               16, 24, 32 rows take some 1.2, 1.4, 1.55 times that, as a block fetches its tokens from L2
+//                               16, 24, 32 rows take some 1.15, 1.4, 1.5 times that, as a block fetches its tokens from L2
 //   clusters, 128 wide          32 rows: 4,096 x 4,096 8.8, 6,144 x 4,096 9.8, 4,096 x 12,288 13.8, 5,120 x 25,600 26.5
 //                               128 rows: 13.5, 14.1, 18.4, 32.3
 //   clusters, 64 wide           32 rows: 2,560 x 4,096 8.0, 4,096 x 4,096 9.5; 128 rows: 10.1, 10.6
@@ -848,7 +858,7 @@ int form(int M, int N, int Kp, int sm_count) {
     }
   };
   if (M <= 16 || (M <= 32 && N <= 48 * sm_count))
-    consider(0, (1.2f + 0.5e-3f * Kp + (float)N * Kp / 6.8e6f) * (M <= 8 ? 1.f : M <= 16 ? 1.2f : M <= 24 ? 1.42f : 1.55f));
+    consider(0, (1.2f + 0.5e-3f * Kp + (float)N * Kp / 6.8e6f) * (M <= 8 ? 1.f : M <= 16 ? 1.15f : M <= 24 ? 1.4f : 1.5f));
   if (M > 16) {
     const int width = large == 1 ? 64 : large == 2 ? 128 : 256, tiles = m_tiles * ((N + width - 1) / width);
     consider(large, 2.8f + 0.31f * num_kb * ((tiles + sm_count - 1) / sm_count));

@@ -68,8 +68,9 @@ def _fn(name: str):
 
 
 def _stream() -> int:
+    """The current stream.  (There are tensors on the GPU: torch has been set up.)"""
     raw = _ops()._raw_stream
-    return raw(torch.cuda.current_device()) if raw is not None else torch.cuda.current_stream().cuda_stream
+    return raw(torch._C._cuda_getDevice()) if raw is not None else torch.cuda.current_stream().cuda_stream
 
 
 def _done(status: int, what: str, detail, kernels: int = 1) -> None:
@@ -81,8 +82,14 @@ def _done(status: int, what: str, detail, kernels: int = 1) -> None:
 
 
 def _require(t, name: str, dtype, ndim: int) -> None:
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.dim() == ndim and t.is_contiguous()):
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_cuda and t.dim() == ndim and t.is_contiguous()):
         _ops()._need(t, name, dtype, ndim)
+
+
+def _require_entries(t, name: str, n: int) -> None:
+    _require(t, name, torch.int32, 1)
+    if t.shape[0] < n:
+        raise _ops().KernelError(f"int8_paged_attention: {name} has {t.shape[0]} entries, the step needs {n}")
 
 
 def _code(dtype, name: str) -> int:
@@ -210,20 +217,21 @@ def int8_linear(x, weight: Int8Weight, out_dtype=None) -> torch.Tensor:
     m, k = x.shape
     if k != weight.k:
         raise _ops().KernelError(f"int8_linear: x {tuple(x.shape)} against weight {tuple(weight.shape)}")
-    device = weight.codes.device
+    codes = weight.codes
+    device = codes.device
     if x.device != device:
         _same_device("int8_linear", x, weight)
-    n = weight.codes.shape[0]
+    n = codes.shape[0]
     out_dtype = out_dtype or x.dtype
     out_code = _code(out_dtype, "out")
     out = torch.empty(m, n, dtype=out_dtype, device=device)
     if rows:
-        st = _fn("dib_gemm_int8")(x.codes.data_ptr(), x.scales.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(),
+        st = _fn("dib_gemm_int8")(x.codes.data_ptr(), x.scales.data_ptr(), codes.data_ptr(), weight.scales.data_ptr(),
                                   out.data_ptr(), m, n, x.codes.shape[1], out_code, _sms(device), _stream())
     else:
         work = torch.empty(m * (_padded(k) + 4), dtype=torch.int8, device=device)      # codes, then scales
         st = _fn("dib_int8_linear")(_address("dib_quantize_rows"), x.data_ptr(), x.stride(0), code, k, work.data_ptr(),
-                                    weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(), m, n, out_code,
+                                    codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(), m, n, out_code,
                                     _sms(device), _stream())
     _done(st, "int8_linear", lambda: f"M={m} N={n} K={k}", 1 if rows else 2)
     return out
@@ -290,14 +298,13 @@ class Int8Cache:
 
 def _row_stride(x, name: str, hkv: int, d: int) -> int:
     """Distance of a token's rows [Hkv, D], which lie together (a column range of a fused projection, say)."""
-    ops = _ops()
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
-        raise ops.KernelError(f"{name} must be a CUDA tensor: this package has no CPU path")
-    if x.dim() != 3 or x.shape[1] != hkv or x.shape[2] != d:
-        raise ops.KernelError(f"{name} has shape {tuple(x.shape)}, the cache's heads are [{hkv}, {d}]")
-    stride = x.stride()
+        raise _ops().KernelError(f"{name} must be a CUDA tensor: this package has no CPU path")
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 3 or shape[1] != hkv or shape[2] != d:
+        raise _ops().KernelError(f"{name} has shape {tuple(shape)}, the cache's heads are [{hkv}, {d}]")
     if stride[2] != 1 or (hkv > 1 and stride[1] != d):
-        raise ops.KernelError(f"{name}: a token's heads must lie together (stride {stride})")
+        raise _ops().KernelError(f"{name}: a token's heads must lie together (stride {stride})")
     return stride[0]
 
 
@@ -312,7 +319,9 @@ def int8_cache_write(k: torch.Tensor, v: torch.Tensor, cache: Int8Cache, slot_ma
     if v.shape[0] != t or v.dtype is not k.dtype or slot_mapping.shape[0] < t:
         raise _ops().KernelError(f"int8_cache_write: k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}, "
                                  f"{slot_mapping.shape[0]} slots")
-    _same_device("int8_cache_write", data, k, v, slot_mapping)
+    device = data.get_device()
+    if k.get_device() != device or v.get_device() != device or slot_mapping.get_device() != device:
+        _same_device("int8_cache_write", data, k, v, slot_mapping)
     st = _fn("dib_int8_cache_write")(k.data_ptr(), v.data_ptr(), ks, vs, data.data_ptr(), cache.scales.data_ptr(),
                                      slot_mapping.data_ptr(), t, hkv, d, page_size, pages, _code(k.dtype, "k"), _stream())
     _done(st, "int8_cache_write", lambda: f"heads {hkv} x {d}")
@@ -363,7 +372,8 @@ def int8_cache_read(cache: Int8Cache, slots: torch.Tensor, dtype: torch.dtype = 
     data = cache.data
     pages, _, hkv, page_size, d = data.shape
     _require(slots, "slots", torch.int32, 1)
-    _same_device("int8_cache_read", data, slots)
+    if slots.get_device() != data.get_device():
+        _same_device("int8_cache_read", data, slots)
     code = _code(dtype, "out")
     t = slots.shape[0]
     k, v = torch.empty(2, t, hkv, d, dtype=dtype, device=data.device).unbind(0)
@@ -507,14 +517,16 @@ def int8_paged_attention(q: torch.Tensor, cache: Int8Cache, meta, scale: float, 
     table, token_seq, cu, lens = meta.block_table, meta.token_seq, meta.cu_q_lens, meta.seq_lens
     _require(table, "block_table", torch.int32, 2)
     b = table.shape[0]
-    for x, name, n in ((token_seq, "token_seq", t), (cu, "cu_q_lens", b + 1), (lens, "seq_lens", b)):
-        _require(x, name, torch.int32, 1)
-        if x.shape[0] < n:
-            raise ops.KernelError(f"int8_paged_attention: {name} has {x.shape[0]} entries, the step needs {n}")
+    _require_entries(token_seq, "token_seq", t)
+    _require_entries(cu, "cu_q_lens", b + 1)
+    _require_entries(lens, "seq_lens", b)
     win = int(window) if window else 0
     if win < 0:
         raise ops.KernelError(f"int8_paged_attention: a window of {win} keys")
-    _same_device("int8_paged_attention", data, q, table, token_seq, cu, lens)
+    device = data.get_device()
+    if q.get_device() != device or table.get_device() != device or token_seq.get_device() != device \
+            or cu.get_device() != device or lens.get_device() != device:
+        _same_device("int8_paged_attention", data, q, table, token_seq, cu, lens)
     out = torch.empty_like(q)
     if t == 0:
         return out
