@@ -423,8 +423,9 @@ class _SplitPart:
 
 
 # Rows (new tokens x query heads of a kv head) of a sequence above which its bfloat16 tokens take the prompt form, whose
-# query tiles have 128 rows.
-PROMPT_ROWS = 64
+# query tiles have 128 rows.  By the sequence's own rows, so that its bits do not depend on the step: 16 sequences of 4,096
+# keys and 48 rows take 76 us there and 210 in the split form, of 1,500 keys and 64 rows 36 and 111, one of 4,096 keys 72 and 37.
+PROMPT_ROWS = 32
 MAX_CHUNKS = 16        # chunks of 4,096 keys that the prompt form adds up for a row
 
 
