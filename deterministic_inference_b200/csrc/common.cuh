@@ -359,11 +359,11 @@ __device__ __forceinline__ bool mbar_wait(unsigned long long* bar, unsigned pari
   }
 }
 // The same in as few instructions as it takes, for kernels whose roles share the instruction cache: the limit is a number of
-// tries, each of which may sleep 256 ns (a second in all, or so).
+// tries, each of which sleeps 4 us where nothing arrives (a second in all).
 __device__ __forceinline__ bool mbar_wait_brief(unsigned long long* bar, unsigned parity) {
   const unsigned addr = (unsigned)__cvta_generic_to_shared(bar);
 #pragma unroll 1
-  for (unsigned i = 0; i < (1u << 22); ++i) {
+  for (unsigned i = 0; i < (1u << 18); ++i) {
     unsigned ok;
     asm volatile(
         "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 256; "
