@@ -839,7 +839,12 @@ attention_split_merge_kernel(T* __restrict__ out, const __grid_constant__ SplitA
   const int i = blockIdx.y, G = a.Hq / a.Hkv;
   const SplitSeq s = split_seq<ROWS>(a, i);
   const int n_rows = s.n * G, id = blockIdx.x;     // rows of a kv head
-  if (s.splits <= 1 || id >= n_rows * a.Hkv || s.splits * s.tiles * a.Hkv > a.max_items) return;
+  // (every block waits, the one without work too: a grid none of whose blocks has waited ends ahead of the attention, and the
+  // kernel that follows takes this one's end for the attention's)
+  if (s.splits <= 1 || id >= n_rows * a.Hkv || s.splits * s.tiles * a.Hkv > a.max_items) {
+    pdl_wait();
+    return;
+  }
   const int kvh = id / n_rows, row = id - kvh * n_rows, tile = row / ROWS, r = row % ROWS;
   const int p0 = s.kv_len - s.n;
   const int tok0 = tile * ROWS / G, tok1 = min((tile + 1) * ROWS - 1, n_rows - 1) / G;

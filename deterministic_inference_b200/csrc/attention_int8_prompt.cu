@@ -262,6 +262,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
   pdl_trigger();
   if (smem - smem_dyn + S_TOTAL > S_DYNAMIC) {      // (the memory is aligned to 1,024 as a rule)
     if (threadIdx.x == 0) atomicExch(&dib_attention_int8_prompt_error_word, 2);
+    pdl_wait();
     return;
   }
   const int unit = a.count - 1 - blockIdx.y, kvh = blockIdx.x;        // the longest first
@@ -300,7 +301,10 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
     }
   }
   const bool any0 = jl[0] >= jf[0], any1 = jl[1] >= jf[1];
-  if (!any0 && !any1) return;     // nothing of this chunk concerns the pair
+  if (!any0 && !any1) {           // nothing of this chunk concerns the pair
+    pdl_wait();                   // (a grid none of whose blocks has waited would end ahead of the kernel in front)
+    return;
+  }
   const int j0 = any0 && any1 ? min(jf[0], jf[1]) : (any0 ? jf[0] : jf[1]);
   const int ntiles = max(any0 ? jl[0] : -1, any1 ? jl[1] : -1) - j0 + 1;
   // (arrays indexed by a running x would live in local memory)

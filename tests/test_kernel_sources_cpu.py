@@ -99,3 +99,58 @@ def test_arrays_in_shared_memory_that_are_read_as_vectors_start_on_them():
                     need = WIDTH.get(use.group(1), 16)
                     assert align % need == 0, f"{path.name}: {name} is read as {use.group(1)}, aligned to {align}"
     assert seen >= 2
+
+
+# ---- waits for the kernel in front
+
+GLOBAL = re.compile(r"__global__\s+void\s+(?:__launch_bounds__\s*\((?:[^()]|\([^()]*\))*\)\s*)?(\w+)\s*\(")
+LAMBDA = re.compile(r"\[[&=\w, ]*\]\s*\([^()]*\)\s*\{")
+
+
+def _blank(text: str, a: int, b: int) -> str:
+    return text[:a] + re.sub(r"[^\n]", " ", text[a:b]) + text[b:]
+
+
+def _kernels(name: str) -> list:
+    """(kernel, its body without comments and without the bodies of its lambdas) of a source."""
+    text = re.sub(r"//[^\n]*", "", (CSRC / name).read_text())
+    found = []
+    for m in GLOBAL.finditer(text):
+        at, depth = m.end(), 1
+        while depth:
+            depth += {"(": 1, ")": -1}.get(text[at], 0)
+            at += 1
+        if text[at:].lstrip()[0] != "{":
+            continue                          # (a declaration)
+        a, b = _braced(text, at)
+        body = text[a:b]
+        for x in list(LAMBDA.finditer(body)):
+            c, d = _braced(body, x.end() - 1)
+            body = _blank(body, c, d)
+        found.append((m.group(1), body))
+    return found
+
+
+INT8_SOURCES = ("cache_int8.cu", "gemm_int8.cu", "attention_int8.cu", "attention_int8_prompt.cu")
+
+
+@pytest.mark.parametrize("name", INT8_SOURCES)
+def test_no_block_leaves_without_having_waited_for_the_kernel_in_front(name):
+    """A grid all of whose blocks leave without the wait ends ahead of the kernel in front of it, and the kernel behind
+    waits for that grid alone: it would read what the one in front has not written."""
+    kernels = _kernels(name)
+    assert kernels
+    for kernel, body in kernels:
+        blocks, waited = [False], None        # by depth of braces: whether the block has waited
+        for m in re.finditer(r"[{}]|\bpdl_(?:wait|prologue)\s*\(|\breturn\b", body):
+            what = m.group()
+            if what == "{":
+                blocks.append(blocks[-1])
+            elif what == "}":
+                blocks.pop()
+            elif what == "return":
+                assert blocks[-1], f"{name}: {kernel} returns before its wait: {body[max(0, m.start() - 120):m.end()]}"
+            else:
+                blocks[-1] = True
+                waited = True
+        assert waited, f"{name}: {kernel} never waits"
