@@ -391,11 +391,12 @@ def _pages_fit(page_size: int) -> bool:
     return page_size >= 4 and page_size & (page_size - 1) == 0
 
 
-def _most_runs(kv_len: int) -> int:
-    """The most runs of a sequence of at most ``kv_len`` keys (the length on the device may be less than the host's)."""
+def _most_runs(kv_len: int, group: int) -> int:
+    """The most runs of a sequence of at most ``kv_len`` keys and ``group`` rows or more (the lengths on the device may be less
+    than the host's, so a token's rows are all that is certain)."""
     runs, keys = 1, _lib().dib_int8_attention_split_keys
     for n in {min(kv_len, 2048), min(kv_len, 4096), min(kv_len, 16384), kv_len}:
-        runs = max(runs, -(-n // keys(n, 1)))
+        runs = max(runs, -(-n // keys(n, group)))
     return runs
 
 
@@ -413,7 +414,7 @@ class _SplitPart:
             self.list = torch.tensor(seqs, dtype=torch.int32).to(device, non_blocking=True)
         self.max_rows = max(q_lens[s] for s in seqs) * group
         self.tile_rows = next(r for r in ((8, 16) if wide else (4, 8, 16, 24, 32)) if self.max_rows <= r or r == (16 if wide else 32))
-        runs = _most_runs(max(kv_lens[s] for s in seqs))
+        runs = _most_runs(max(kv_lens[s] for s in seqs), group)
         tiles, per32 = -(-self.max_rows // self.tile_rows), 32 // self.tile_rows
         # (runs get longer with the rows: tiles * runs is largest at 64 rows, or the tiles' own number is)
         self.items = hkv * min(tiles * runs, max(2 * per32 * runs, per32 * (runs + 1) + tiles))

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import random
+
 import pytest
 import torch
 
@@ -56,3 +58,29 @@ def test_prompt_units_cover_every_token_once():
                 last = (kv_lens[s] - q_lens[s] + tok) // 4096 if part.chunk_tiles else 0
                 assert all((s, tok, c) in seen for c in range(last + 1))
         assert part.seq_list.tolist() == many and part.max_tokens == max(q_lens[s] for s in many)
+
+
+def _runs(keys: int, rows: int) -> int:
+    return max(1, -(-keys // int8._lib().dib_int8_attention_split_keys(keys, rows)))
+
+
+@pytest.mark.parametrize("group", [1, 2, 4, 5, 8, 40])
+@pytest.mark.parametrize("wide", [False, True])
+def test_split_work_covers_the_steps_that_the_lengths_allow(group, wide):
+    """Work items and partial results are sized for every step that the host's lengths, upper bounds in a captured step, allow;
+    and where none of those has a second run of keys, there are no partial results and no merge."""
+    rng = random.Random(group)
+    for _ in range(300):
+        n = rng.randrange(1, 5)
+        q_lens = [rng.choice([1, 1, 2, 3, 7, 32 // group + 1, 200]) for _ in range(n)]
+        kv_lens = [rng.choice([1, 100, 256, 257, 300, 512, 513, 4096, 16384, 16385, rng.randrange(1, 40000)]) for _ in range(n)]
+        part = int8._SplitPart(list(range(n)), q_lens, kv_lens, group, 8, wide, torch.device("cpu"))
+        two = False
+        for q, kv in zip(q_lens, kv_lens):
+            for _ in range(20):
+                q1, kv1 = rng.choice([q, rng.randrange(1, q + 1)]), rng.choice([kv, rng.randrange(1, kv + 1)])
+                runs = _runs(kv1, q1 * group)
+                assert 8 * -(-q1 * group // part.tile_rows) * runs <= part.items
+                two |= runs > 1
+            two |= _runs(min(kv, 16384), group) > 1
+        assert (part.rows > 0) == two
