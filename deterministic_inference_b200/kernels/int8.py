@@ -423,9 +423,11 @@ class _SplitPart:
         self.list_pointer = _pointer(self.list)
 
 
-# Rows (new tokens x query heads of a kv head) of a sequence above which its bfloat16 tokens take the prompt form, whose
-# query tiles have 128 rows.  By the sequence's own rows, so that its bits do not depend on the step: 16 sequences of 4,096
+# Rows (new tokens x query heads of a kv head) of a sequence of drafted tokens above which they take the prompt form (bfloat16),
+# whose query tiles have 128 rows.  By the sequence's own rows, so that its bits do not depend on the step: 16 sequences of 4,096
 # keys and 48 rows take 76 us there and 210 in the split form, of 1,500 keys and 64 rows 36 and 111, one of 4,096 keys 72 and 37.
+# A prompt's portions take it whatever their rows: the scheduler cuts a prompt where the step has room, and in a captured step
+# the host knows a portion's bucket only, so a line between two forms would show in a request's bits.
 PROMPT_ROWS = 32
 MAX_CHUNKS = 16        # chunks of 4,096 keys that the prompt form adds up for a row
 
@@ -455,15 +457,16 @@ class _PromptPart:
         self.units, self.seq_list = lists[:4 * self.count], lists[4 * self.count:]
 
 
-def _parts(meta, group: int, hkv: int, wide: bool, window: int, device) -> list:
-    """The step's launches: the sequences with one new token, those with a few, those with many (bfloat16)."""
-    key = ("int8", group, hkv, wide, window)
+def _parts(meta, group: int, hkv: int, wide: bool, window: int, portions: bool, device) -> list:
+    """The step's launches: the sequences with one new token, those of the prompt form (bfloat16: all others that are portions
+    of prompts, or those with many drafted tokens), the rest."""
+    key = ("int8", group, hkv, wide, window, portions)
     parts = meta.scratch.get(key)
     if parts is None:
         q_lens, kv_lens = meta.q_lens, meta.kv_lens
         one = [s for s, n in enumerate(q_lens) if n == 1]
         more = [s for s, n in enumerate(q_lens) if n > 1]
-        many = [s for s in more if not wide and q_lens[s] * group > PROMPT_ROWS and group <= 128
+        many = [s for s in more if not wide and (portions or q_lens[s] * group > PROMPT_ROWS) and group <= 128
                 and kv_lens[s] <= MAX_CHUNKS * 4096]
         few = [s for s in more if s not in set(many)]
         parts = [_SplitPart(x, q_lens, kv_lens, group, hkv, wide, device) for x in (one, few) if x]
@@ -501,12 +504,18 @@ def _split(q, out, cache: Int8Cache, meta, part: _SplitPart, scale: float, windo
     _done(st, "int8_paged_attention", lambda: f"head_dim {d}, heads {hq}/{hkv}", 2 if rows else 1)
 
 
-def int8_paged_attention(q: torch.Tensor, cache: Int8Cache, meta, scale: float, window=None) -> torch.Tensor:
+def int8_paged_attention(q: torch.Tensor, cache: Int8Cache, meta, scale: float, window=None,
+                         portions: bool = False) -> torch.Tensor:
     """Causal attention of every token of the step over its sequence's keys in the cache, as ``ops.paged_attention``: q
     [T, Hq, D] float32 or bfloat16, ``meta`` the step's ``AttentionMeta``.  A sequence's new tokens are its last ones
     (``seq_lens`` counts them); each sees the keys up to its own position, the last ``window`` of them if given.  The
     codes of keys and values enter the products as they are, the scales join scores and probabilities in float32.  A
-    token that sees no key gives zeros."""
+    token that sees no key gives zeros.
+
+    ``portions``: the sequences with more than one new token bring portions of prompts.  In bfloat16 they then all take one
+    form, so that a token's bits depend neither on where its prompt was cut (a portion of one token aside) nor on whether
+    ``meta`` holds the lengths or upper bounds of them.  Otherwise they count as drafted tokens, few of which are faster in
+    another form, chosen by their number."""
     ops = _ops()
     if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dim() == 3 and q.is_contiguous()):
         ops._need(q, "q", None, 3)
@@ -534,7 +543,7 @@ def int8_paged_attention(q: torch.Tensor, cache: Int8Cache, meta, scale: float, 
         return out
     if d <= 128 and _pages_fit(page_size) and q.data_ptr() % 16 == 0 and cache.scales.data_ptr() % 16 == 0 \
             and pages * 2 * hkv * page_size < 1 << 31:
-        for part in _parts(meta, hq // hkv, hkv, code == 0, win, q.device):
+        for part in _parts(meta, hq // hkv, hkv, code == 0, win, bool(portions), q.device):
             run = _prompt if isinstance(part, _PromptPart) else _split
             run(q, out, cache, meta, part, float(scale), win)
         return out

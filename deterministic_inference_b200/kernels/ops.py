@@ -675,9 +675,9 @@ def paged_attention(q: torch.Tensor, kv_cache: torch.Tensor, meta, scale: float,
     sequences).  A query at position p sees keys max(0, p-window+1) .. p.
     ``defer``: a step of one-token sequences only may come back as a ``SplitAttention``
     (its splits not yet merged) for the matrix product that follows to merge.  ``kv_cache`` may be an
-    ``Int8Cache``: ``int8_paged_attention``."""
+    ``Int8Cache``: ``int8_paged_attention`` of portions of prompts."""
     if isinstance(kv_cache, Int8Cache):
-        return int8_paged_attention(q, kv_cache, meta, scale, window)
+        return int8_paged_attention(q, kv_cache, meta, scale, window, portions=True)
     _need(q, "q", None, 3)
     _need(kv_cache, "kv_cache", q.dtype, 5)
     t, hq, d = q.shape

@@ -1,0 +1,75 @@
+"""What a token's bits over a cache in 8 bits do not depend on: whether its step was launched or replayed, where its prompt was
+cut, the other sequences of the step, and keys that it does not see."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from deterministic_inference_b200 import EngineConfig
+from deterministic_inference_b200.engine.batch import SequenceInput
+from deterministic_inference_b200.engine.graphs import token_bucket
+from deterministic_inference_b200.engine.runner import ModelRunner
+from deterministic_inference_b200.kernels import ops
+from tests.int8_util import Int8Case
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def _rand(*shape, seed=0, dtype=F32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).cuda().to(dtype)
+
+
+# ---- portions
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 5, 8])
+def test_a_portion_attends_the_same_launched_and_captured(group, dtype):
+    """``meta`` with a portion's own lengths, and with its bucket's, which are all that the host knows of a captured step."""
+    case = Int8Case([700], 2, 128, 16, seed=group)
+    cache = ops.Int8Cache(case.data, case.scales)
+    for n in (2, 3, 4, 5, 7, 8, 11, 16, 17, 33):
+        q = _rand(n, 2 * group, 128, seed=n, dtype=dtype)
+        own, bucket = case.meta([n]), case.meta([n])
+        upper, least = token_bucket(n)
+        bucket.q_lens, bucket.kv_lens = [upper], [1024 + upper - least]
+        want = ops.paged_attention(q, cache, own, 0.1)
+        assert torch.equal(ops.paged_attention(q, cache, bucket, 0.1), want), n
+
+
+@pytest.mark.parametrize("window", [None, 100])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (2, 2, 128), (6, 2, 64)])
+def test_a_prompt_attends_the_same_in_short_portions(hq, hkv, d, window):
+    """Down to two tokens."""
+    case = Int8Case([400], hkv, d, 16, seed=6)
+    q = _rand(200, hq, d, seed=7, dtype=BF16)
+    cache = ops.Int8Cache(case.data, case.scales)
+    whole = ops.paged_attention(q, cache, case.meta([200]), 0.1, window)
+    for n in (33, 17, 16, 9, 4, 3, 2):
+        got = ops.paged_attention(q[200 - n:].contiguous(), cache, case.meta([n]), 0.1, window)
+        assert torch.equal(got, whole[200 - n:]), n
+
+
+@pytest.mark.parametrize("name", ["d", "e"])
+def test_short_portions_replayed_give_the_bits_of_launched_ones(name, tiny_model_dirs):
+    """Portions of 3 to 7 tokens behind different prompts, one bucket: from the third on they are replayed."""
+    g = torch.Generator().manual_seed(5)
+    prompts = [torch.randint(0, 300, (40 + i,), generator=g).tolist() for i in range(6)]
+    outs = []
+    for graphs in (True, False):
+        r = ModelRunner(EngineConfig(model_path=str(tiny_model_dirs[name]), dtype="bfloat16", weight_dtype="int8",
+                                     cache_dtype="int8", kv_pool_tokens=4096, page_size=32, max_reqs=16, max_seq_len=512,
+                                     cuda_graphs=graphs))
+        rows = []
+        for p, n in zip(prompts, (5, 3, 7, 4, 6, 3)):
+            slot = r.cache.allocate_slot()
+            for at, m in ((0, len(p) - n), (len(p) - n, n)):
+                rows.append(r.step([SequenceInput(slot, p[at:at + m], at, [m - 1])])[0].clone())
+                torch.cuda.synchronize()
+        if graphs:
+            assert r.step_graphs.replays >= 2
+        outs.append(rows)
+    ops.check_kernel_status()
+    for i, (a, b) in enumerate(zip(*outs)):
+        assert torch.equal(a, b), i
