@@ -228,11 +228,12 @@ struct PromptArgs {
   const int* block_table;       // [B, max_blocks]
   const int* cu_q_lens;
   const int* seq_lens;
-  const int* units;             // [4][count]: sequence, first token of A, of B (or -1), chunk
-  int count, max_blocks, Hq, Hkv, D, page_shift, num_pages, window, chunk_tiles, max_chunks;
+  const int* units;             // [5][unit_stride], of which `count`: sequence, first token of A, of B (or -1), chunk, place of
+                                // A's first token in the partial results
+  int count, unit_stride, max_blocks, Hq, Hkv, D, page_shift, num_pages, window, chunk_tiles, max_chunks;
   float scale;
-  float* part_o;                // [T, Hq, max_chunks, 128]
-  float2* part_ml;              // [T, Hq, max_chunks]: reference (log 2), sum
+  float* part_o;                // [places, Hq, max_chunks, 128]
+  float2* part_ml;              // [places, Hq, max_chunks]: reference (log 2), sum
 };
 
 __global__ void __launch_bounds__(THREADS, 1)
@@ -270,8 +271,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
   const unsigned g_up = 65536u / G + 1;      // r / G for r < 128, exactly: 128 G < 65536
   auto token_of = [&](int r) { return (int)(r * g_up >> 16); };
   const int seq = a.units[unit];
-  const int tokx[2] = {a.units[a.count + unit], a.units[2 * a.count + unit]};
-  const int chunk = a.chunk_tiles > 0 ? a.units[3 * a.count + unit] : 0;
+  const int tokx[2] = {a.units[a.unit_stride + unit], a.units[2 * a.unit_stride + unit]};
+  const int chunk = a.chunk_tiles > 0 ? a.units[3 * a.unit_stride + unit] : 0;
   const int q_begin = a.cu_q_lens[seq], q_len = a.cu_q_lens[seq + 1] - q_begin;
   const int kv_len = min(a.seq_lens[seq], (int)min((long long)a.max_blocks << a.page_shift, 0x7fffff00ll));
   const int prefix = kv_len - q_len;
@@ -766,12 +767,14 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
       const bool partial = !(x ? whole[1] : whole[0]);      // this chunk's: O as accumulated (against m_ref), m_ref, l
       const float inv = l == 0.f ? 0.f : 1.0f / l, value_unit = two_to(value_exp);
       const int my_ntok = x ? ntok[1] : ntok[0], row0 = (warp & 3) * 32;
-      auto row_of_lane = [&](int rr) {      // the row of the output that is row rr of this tile, or -1
+      // row rr of this tile as a row of the output, or of the partial results, whose first token is `first`; -1: none
+      auto row_of_lane = [&](int first, int rr) {
         const int t = token_of(rr);
-        return t < my_ntok ? (long long)(q_begin + tok0 + t) * a.Hq + kvh * G + rr - t * G : -1ll;
+        return t < my_ntok ? (long long)(first + t) * a.Hq + kvh * G + rr - t * G : -1ll;
       };
       if (ok && partial) {
-        if (valid) a.part_ml[((long long)(q_begin + tok0 + tl) * a.Hq + kvh * G + g) * a.max_chunks + chunk] = make_float2(m_ref, l);
+        const int place0 = a.units[4 * a.unit_stride + unit] + tok0 - tokx[0];      // of this tile's first token
+        if (valid) a.part_ml[((long long)(place0 + tl) * a.Hq + kvh * G + g) * a.max_chunks + chunk] = make_float2(m_ref, l);
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {      // 64 dimensions at a time
 #pragma unroll
@@ -788,7 +791,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
           __syncwarp();
 #pragma unroll 4
           for (int rr = lane >> 4; rr < 32; rr += 2) {
-            const long long row = row_of_lane(row0 + rr);
+            const long long row = row_of_lane(place0, row0 + rr);
             if (row >= 0)
               *reinterpret_cast<uint4*>(a.part_o + (row * a.max_chunks + chunk) * TILE + half * 64 + (lane & 15) * 4) =
                   *reinterpret_cast<const uint4*>(stage + rr * 256 + ((lane & 15) ^ (rr & 7)) * 16);
@@ -811,7 +814,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         __syncwarp();
 #pragma unroll 4
         for (int rr = lane >> 4; rr < 32; rr += 2) {
-          const long long row = row_of_lane(row0 + rr);
+          const long long row = row_of_lane(q_begin + tok0, row0 + rr);
           if (row >= 0 && (lane & 15) * 8 < a.D)
             *reinterpret_cast<uint4*>(out + row * a.D + (lane & 15) * 8) =
                 *reinterpret_cast<const uint4*>(stage + rr * 256 + ((lane & 15) ^ (rr & 7)) * 16);
@@ -827,52 +830,46 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
 
 // Rows whose keys span several chunks: out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c in chunk order, over the chunks of
 // the row's query tile.  A warp a (token, head), a lane four dimensions; rows that the attention finished cost a look at
-// their lengths.
-constexpr int MERGE_MAX = 16;
+// their lengths.  entries [4][entry_stride]: sequence, first token, end, place of the first token's partial results.
 __global__ void __launch_bounds__(256)
 attention_prompt_merge_kernel(__nv_bfloat16* __restrict__ out, const __grid_constant__ PromptArgs a,
-                              const int* __restrict__ seq_list) {
+                              const int* __restrict__ entries, int entry_stride) {
   const float* part_o = a.part_o;
   const float2* part_ml = a.part_ml;
   pdl_trigger();
   const int lane = threadIdx.x & 31;
-  const int seq = seq_list[blockIdx.y];
+  const int seq = entries[blockIdx.y], tok_begin = entries[entry_stride + blockIdx.y], tok_end = entries[2 * entry_stride + blockIdx.y];
   const int q_begin = a.cu_q_lens[seq], q_len = a.cu_q_lens[seq + 1] - q_begin;
-  const int id = blockIdx.x * 8 + (threadIdx.x >> 5), tok = id / a.Hq, h = id - tok * a.Hq;
+  const int id = blockIdx.x * 8 + (threadIdx.x >> 5), h = id % a.Hq, tok = tok_begin + id / a.Hq;
   pdl_wait(part_o, part_ml);
-  if (tok >= q_len) return;
+  if (tok >= min(tok_end, q_len)) return;
   const int kv_len = min(a.seq_lens[seq], (int)min((long long)a.max_blocks << a.page_shift, 0x7fffff00ll));
   const int npt = TILE / (a.Hq / a.Hkv), tok0 = tok / npt * npt;
   const int first_pos = kv_len - q_len + tok0, last_pos = first_pos + min(npt, q_len - tok0) - 1;
   if (last_pos < 0) return;
-  const int c0 = first_visible_key(first_pos, a.window) / TILE / a.chunk_tiles, c1 = last_pos / TILE / a.chunk_tiles;
+  const int c0 = first_visible_key(first_pos, a.window) / TILE / a.chunk_tiles;
+  const int c1 = min(last_pos / TILE / a.chunk_tiles, a.max_chunks - 1);
   if (c0 >= c1) return;     // finished by the attention itself
-  const long long row = (long long)(q_begin + tok) * a.Hq + h;
-  float m[MERGE_MAX], l[MERGE_MAX], top = NEG_BIG;
-#pragma unroll
-  for (int c = 0; c < MERGE_MAX; ++c) {
-    m[c] = NEG_BIG;
-    l[c] = 0.f;
-    if (c0 + c <= c1) {
-      const float2 ml = part_ml[row * a.max_chunks + c0 + c];
-      m[c] = ml.x;
-      l[c] = ml.y;
-    }
-    top = fmaxf(top, m[c]);
-  }
+  const long long row = (long long)(entries[3 * entry_stride + blockIdx.y] + tok - tok_begin) * a.Hq + h;
+  part_o += row * a.max_chunks * TILE + lane * 4;
+  part_ml += row * a.max_chunks;
+  float top = NEG_BIG;
+  for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, part_ml[c].x);
+  top = warp_max(top);
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
-#pragma unroll
-  for (int c = 0; c < MERGE_MAX; ++c) {
-    if (c0 + c > c1) break;
-    const float w = fast_exp2(m[c] - top);
-    const float4 v = *reinterpret_cast<const float4*>(part_o + (row * a.max_chunks + c0 + c) * TILE + lane * 4);
-    sum = fmaf(w, l[c], sum);
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c) {
+    const float2 ml = part_ml[c];
+    const float4 v = *reinterpret_cast<const float4*>(part_o + (long long)c * TILE);
+    const float w = fast_exp2(ml.x - top);
+    sum = fmaf(w, ml.y, sum);
     o.x = fmaf(w, v.x, o.x); o.y = fmaf(w, v.y, o.y); o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
   }
   if (lane * 4 >= a.D) return;
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  *reinterpret_cast<uint2*>(out + row * a.D + lane * 4) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+  *reinterpret_cast<uint2*>(out + ((long long)(q_begin + tok) * a.Hq + h) * a.D + lane * 4) =
+      make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
 }
 
 // ---- host side
@@ -906,18 +903,19 @@ int dib_attention_int8_prompt_status_clear() {
 }
 
 // q, out bfloat16 [T, Hq, D], heads up to 128, up to 128 query heads a kv head, pages of a power of two of rows, 4 at least.
-// units int32 [4, count]: sequence, first tokens of A and B (128 / (Hq / Hkv) tokens each; -1: no B), chunk; the longest last.
-// chunk_tiles: 0, or the key tiles of a chunk: then part_o float32 [T, Hq, max_chunks, 128] and part_ml [.., 2] take partial
-// results (at most 16 chunks of a row), which are added up for the tokens of the seq_count sequences in seq_list
-// (max_tokens: the most of one).
+// units int32 [5, unit_stride], `count` of each row: sequence, first tokens of A and B (128 / (Hq / Hkv) tokens each; -1: no B),
+// chunk, place of A's first token in the partial results (B follows A); the longest last.
+// chunk_tiles: 0, or the key tiles of a chunk: then part_o float32 [places, Hq, max_chunks, 128] and part_ml [.., 2] take partial
+// results, which are added up for entry_count entries, int32 [4, entry_stride]: sequence, first token, end, place of the first
+// token (max_tokens: the most of one).
 int dib_int8_attention_prompt(const void* q, void* out, const void* data, const void* scales, long long num_pages,
                               const void* block_table, int max_blocks, const void* cu_q_lens, const void* seq_lens,
-                              const void* units, int count, const void* seq_list, int seq_count, int max_tokens, void* part_o,
-                              void* part_ml, int chunk_tiles, int max_chunks, int Hq, int Hkv, int D, int page_size,
-                              float scale, int window, cudaStream_t st) {
-  if (count < 0 || count > 65535 || seq_count < 0 || seq_count > 65535 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 ||
-      Hq / Hkv > TILE || D < 16 || D > 128 || D % 16 != 0 || page_size < 4 || (page_size & (page_size - 1)) != 0 ||
-      num_pages * 2 * Hkv * page_size >= (1ll << 31) || chunk_tiles < 0 || (chunk_tiles > 0 && max_chunks > MERGE_MAX))
+                              const void* units, int count, int unit_stride, const void* entries, int entry_count,
+                              int entry_stride, int max_tokens, void* part_o, void* part_ml, int chunk_tiles, int max_chunks,
+                              int Hq, int Hkv, int D, int page_size, float scale, int window, cudaStream_t st) {
+  if (count < 0 || count > 65535 || unit_stride < count || entry_count < 0 || entry_count > 65535 || entry_stride < entry_count ||
+      Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || Hq / Hkv > TILE || D < 16 || D > 128 || D % 16 != 0 || page_size < 4 || (page_size & (page_size - 1)) != 0 ||
+      num_pages * 2 * Hkv * page_size >= (1ll << 31) || chunk_tiles < 0 || max_chunks < 1)
     return DIB_BAD_SIZE;
   if (((reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(q) |
         reinterpret_cast<uintptr_t>(out)) & 15) != 0)
@@ -929,7 +927,7 @@ int dib_int8_attention_prompt(const void* q, void* out, const void* data, const 
   a.cu_q_lens = reinterpret_cast<const int*>(cu_q_lens);
   a.seq_lens = reinterpret_cast<const int*>(seq_lens);
   a.units = reinterpret_cast<const int*>(units);
-  a.count = count; a.max_blocks = max_blocks; a.Hq = Hq; a.Hkv = Hkv; a.D = D;
+  a.count = count; a.unit_stride = unit_stride; a.max_blocks = max_blocks; a.Hq = Hq; a.Hkv = Hkv; a.D = D;
   a.page_shift = 0;
   while ((1 << a.page_shift) < page_size) ++a.page_shift;
   a.num_pages = (int)num_pages;
@@ -961,8 +959,8 @@ int dib_int8_attention_prompt(const void* q, void* out, const void* data, const 
   if (chunk_tiles > 0) {
     const long long blocks = ((long long)max_tokens * Hq + 7) / 8;
     if (blocks > 0x7fffffffll) return DIB_BAD_SIZE;
-    dib_launch(attention_prompt_merge_kernel, dim3((unsigned)blocks, seq_count), dim3(256), 0, st,
-               reinterpret_cast<__nv_bfloat16*>(out), a, reinterpret_cast<const int*>(seq_list));
+    dib_launch(attention_prompt_merge_kernel, dim3((unsigned)blocks, entry_count), dim3(256), 0, st,
+               reinterpret_cast<__nv_bfloat16*>(out), a, reinterpret_cast<const int*>(entries), entry_stride);
     DIB_CHECK_LAUNCH();
   }
   return DIB_OK;

@@ -42,8 +42,8 @@ _SIGNATURES = {
     "dib_int8_attention_split": ("attention_int8", (_P, _P, _P, _P, _L, _P, _I, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _I, _I,
                                                     _I, _I, _F, _I, _I, _I, _P)),
     "dib_int8_attention_any": ("attention_int8", (_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _P)),
-    "dib_int8_attention_prompt": ("attention_int8_prompt", (_P, _P, _P, _P, _L, _P, _I, _P, _P, _P, _I, _P, _I, _I, _P, _P, _I, _I,
-                                                            _I, _I, _I, _I, _F, _I, _P)),
+    "dib_int8_attention_prompt": ("attention_int8_prompt", (_P, _P, _P, _P, _L, _P, _I, _P, _P, _P, _I, _I, _P, _I, _I, _I, _P, _P,
+                                                            _I, _I, _I, _I, _I, _I, _F, _I, _P)),
 }
 _functions: dict = {}
 _ops_module = None
@@ -429,11 +429,15 @@ class _SplitPart:
 # A prompt's portions take it whatever their rows: the scheduler cuts a prompt where the step has room, and in a captured step
 # the host knows a portion's bucket only, so a line between two forms would show in a request's bits.
 PROMPT_ROWS = 32
-MAX_CHUNKS = 16        # chunks of 4,096 keys that the prompt form adds up for a row
+# Bytes of partial results that a launch of the prompt form may take, where rows have several chunks of keys: 8,192 tokens of 64
+# heads on 65,536 keys would take 4.4 GB at once; those of a few thousand rows fill the GPU.
+SCRATCH_BYTES = 1 << 30
 
 
 class _PromptPart:
-    """The sequences of the prompt form's launch: its list of query-tile pairs (and chunks of keys), longest last."""
+    """The sequences of the prompt form's launches: the list of query-tile pairs (and chunks of keys, and places of partial
+    results), longest last in a launch; ``launches``: (first unit, units, first entry, entries, tokens of the longest entry),
+    an entry being tokens of a sequence whose chunks are added up; ``rows``: tokens that partial results are held of."""
 
     def __init__(self, seqs: list, q_lens: list, kv_lens: list, group: int, hkv: int, window: int, device):
         from . import attention_bf16
@@ -443,18 +447,50 @@ class _PromptPart:
         tokens = 128 // group
         self.chunks = -(-max(keys[s] for s in seqs) // (attention_bf16.CHUNK_TILES * 128))
         self.chunk_tiles = attention_bf16.CHUNK_TILES if self.chunks > 1 else 0
+        self.max_tokens, self.rows = max(new), 0
         if self.chunks > 1:
-            seq, a, b, chunk = attention_bf16.extend_chunk_units(new, keys, 0, tokens, attention_bf16.CHUNK_TILES)
+            units = list(zip(*attention_bf16.extend_chunk_units(new, keys, 0, tokens, attention_bf16.CHUNK_TILES)))
+            entries, place = self._entries(seqs, new, 2 * tokens, group * hkv * self.chunks * 520)
         else:
             # how tiles are paired depends on the step, the arithmetic of a tile does not (see ``extend_tile_pairs``)
             ctas = (sum(-(-n // tokens) for n in new) + 1) // 2 * hkv
             sms = _sms(device)
-            seq, a, b = attention_bf16.extend_tile_pairs(new, keys, 0, tokens, window, alone=2 * ctas <= sms,
-                                                         neighbours=ctas > sms)
-            chunk = [0] * len(seq)
-        self.count, self.seqs, self.max_tokens = len(seq), len(seqs), max(new)
-        lists = torch.tensor(seq + a + b + chunk + list(seqs), dtype=torch.int32).to(device, non_blocking=True)
-        self.units, self.seq_list = lists[:4 * self.count], lists[4 * self.count:]
+            units = [(*u, 0) for u in zip(*attention_bf16.extend_tile_pairs(new, keys, 0, tokens, window, alone=2 * ctas <= sms,
+                                                                            neighbours=ctas > sms))]
+            entries, place = [[(s, 0, new[s], 0) for s in seqs]], lambda s, t: (0, 0)
+        units = [(*place(s, a), s, a, b, c) for s, a, b, c in units]
+        units.sort(key=lambda u: u[0])          # by launch, in their order
+        self.count, self.launches, at = len(units), [], 0
+        for i, own in enumerate(entries):
+            count = sum(1 for u in units if u[0] == i)
+            self.launches.append((sum(n for _, n, *_ in self.launches), count, at, len(own), max(hi - lo for _, lo, hi, _ in own)))
+            at += len(own)
+        flat = [e for own in entries for e in own]
+        lists = torch.tensor([u[i] for i in (2, 3, 4, 5, 1) for u in units] + [e[i] for i in range(4) for e in flat],
+                             dtype=torch.int32).to(device, non_blocking=True)
+        self.units, self.entries = lists[:4 * self.count], lists[5 * self.count:]
+        self.entry_count = len(flat)
+        self.seq_list = self.entries[:self.entry_count]
+
+    def _entries(self, seqs: list, new: list, pair: int, token_bytes: int):
+        """The launches' entries (sequence, first token, end, place of its first token's partial results), cut between pairs of
+        query tiles where a launch's partial results are full, and the launch and place of a pair."""
+        room = max(1, SCRATCH_BYTES // (token_bytes * pair)) * pair
+        entries, where, used = [[]], {}, 0
+        for s in seqs:
+            at = 0
+            while at < new[s]:
+                if used >= room:
+                    entries.append([])
+                    used = 0
+                end = min(new[s], at + room - used)
+                entries[-1].append((s, at, end, used))
+                for t in range(at, end, pair):
+                    where[s, t] = (len(entries) - 1, used + t - at)
+                used += -(-(end - at) // pair) * pair
+                self.rows = max(self.rows, used)
+                at = end
+        return entries, lambda s, t: where[s, t]
 
 
 def _parts(meta, group: int, hkv: int, wide: bool, window: int, portions: bool, device) -> list:
@@ -466,8 +502,7 @@ def _parts(meta, group: int, hkv: int, wide: bool, window: int, portions: bool, 
         q_lens, kv_lens = meta.q_lens, meta.kv_lens
         one = [s for s, n in enumerate(q_lens) if n == 1]
         more = [s for s, n in enumerate(q_lens) if n > 1]
-        many = [s for s in more if not wide and (portions or q_lens[s] * group > PROMPT_ROWS) and group <= 128
-                and kv_lens[s] <= MAX_CHUNKS * 4096]
+        many = [s for s in more if not wide and (portions or q_lens[s] * group > PROMPT_ROWS) and group <= 128]
         few = [s for s in more if s not in set(many)]
         parts = [_SplitPart(x, q_lens, kv_lens, group, hkv, wide, device) for x in (one, few) if x]
         if many:
@@ -478,16 +513,18 @@ def _parts(meta, group: int, hkv: int, wide: bool, window: int, portions: bool, 
 
 def _prompt(q, out, cache: Int8Cache, meta, part: _PromptPart, scale: float, window: int) -> None:
     pages, _, hkv, page_size, d = cache.data.shape
-    t, hq, _ = q.shape
-    rows = t * hq * part.chunks if part.chunks > 1 else 0
+    hq = q.shape[1]
+    rows = part.rows * hq * part.chunks
     held = torch.empty(rows * 130, dtype=torch.float32, device=q.device) if rows else None      # outputs, then (maximum, sum)
     partial = _pointer(held)
-    st = _fn("dib_int8_attention_prompt")(
-        q.data_ptr(), out.data_ptr(), cache.data.data_ptr(), cache.scales.data_ptr(), pages, meta.block_table.data_ptr(),
-        meta.block_table.shape[1], meta.cu_q_lens.data_ptr(), meta.seq_lens.data_ptr(), part.units.data_ptr(), part.count,
-        part.seq_list.data_ptr(), part.seqs, part.max_tokens, partial, partial + rows * 512, part.chunk_tiles, part.chunks, hq,
-        hkv, d, page_size, scale, window, _stream())
-    _done(st, "int8_paged_attention", lambda: f"head_dim {d}, heads {hq}/{hkv}", 2 if part.chunks > 1 else 1)
+    units, entries = part.units.data_ptr(), part.entries.data_ptr()
+    for first, count, first_entry, num_entries, max_tokens in part.launches:
+        st = _fn("dib_int8_attention_prompt")(
+            q.data_ptr(), out.data_ptr(), cache.data.data_ptr(), cache.scales.data_ptr(), pages, meta.block_table.data_ptr(),
+            meta.block_table.shape[1], meta.cu_q_lens.data_ptr(), meta.seq_lens.data_ptr(), units + 4 * first, count, part.count,
+            entries + 4 * first_entry, num_entries, part.entry_count, max_tokens, partial, partial + rows * 512, part.chunk_tiles,
+            part.chunks, hq, hkv, d, page_size, scale, window, _stream())
+        _done(st, "int8_paged_attention", lambda: f"head_dim {d}, heads {hq}/{hkv}", 2 if part.chunks > 1 else 1)
 
 
 def _split(q, out, cache: Int8Cache, meta, part: _SplitPart, scale: float, window: int) -> None:

@@ -51,6 +51,43 @@ def test_a_prompt_attends_the_same_in_short_portions(hq, hkv, d, window):
         assert torch.equal(got, whole[200 - n:]), n
 
 
+def test_a_portion_attends_the_same_at_any_number_of_keys():
+    """Around 65,536 keys, where a captured step reckons with more keys than a launched one."""
+    case = Int8Case([70000], 1, 128, 64, seed=3)
+    cache = ops.Int8Cache(case.data, case.scales)
+    for n, keys in ((40, 65530), (5, 65536), (200, 65600), (40, 70000)):
+        q = _rand(n, 4, 128, seed=n, dtype=BF16)
+        own, bucket = case.meta([n], [keys]), case.meta([n], [keys])
+        upper, least = token_bucket(n)
+        bucket.q_lens, bucket.kv_lens = [upper], [70000 + upper - least]
+        want = ops.paged_attention(q, cache, own, 0.1)
+        assert torch.equal(ops.paged_attention(q, cache, bucket, 0.1), want), (n, keys)
+        exact, _, _ = case.attention(q, [n], 0.1, kv_lens=[keys])
+        # float16 probabilities and values: 2^-12 each and 2^-12 again for the value's scale, the output 2^-9, of each of many
+        # terms of one size and either sign; four times their root mean square, 2^-8
+        off = (want.double() - exact).norm(dim=-1) / exact.norm(dim=-1)
+        assert off.max() < 2.0 ** -8
+        part = ops.paged_attention(q[n // 2:].contiguous(), cache, case.meta([n - n // 2], [keys]), 0.1)
+        assert torch.equal(part, want[n // 2:])
+
+
+@pytest.mark.parametrize("window", [None, 5000])
+def test_partial_results_in_several_launches(window, monkeypatch):
+    """The prompt form's partial results limited to a few pairs of query tiles a launch: the same bits."""
+    from deterministic_inference_b200.kernels import int8
+    case = Int8Case([9000, 300, 4500, 14000], 2, 128, 16, seed=2)
+    cache, q_lens = ops.Int8Cache(case.data, case.scales), [700, 1, 90, 333]
+    q = _rand(sum(q_lens), 8, 128, seed=1, dtype=BF16)
+    want = ops.paged_attention(q, cache, case.meta(q_lens), 0.1, window)
+    for pairs in (1, 3, 8):
+        monkeypatch.setattr(int8, "SCRATCH_BYTES", pairs * 64 * 8 * 4 * 520)
+        meta = case.meta(q_lens)
+        assert torch.equal(ops.paged_attention(q, cache, meta, 0.1, window), want)
+        part = next(p for p in meta.scratch[next(iter(meta.scratch))] if isinstance(p, int8._PromptPart))
+        assert len(part.launches) == -(-(11 + 2 + 6) // pairs) and part.rows <= pairs * 64
+    ops.check_kernel_status()
+
+
 @pytest.mark.parametrize("name", ["d", "e"])
 def test_short_portions_replayed_give_the_bits_of_launched_ones(name, tiny_model_dirs):
     """Portions of 3 to 7 tokens behind different prompts, one bucket: from the third on they are replayed."""
