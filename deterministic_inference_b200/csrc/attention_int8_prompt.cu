@@ -7,8 +7,9 @@
 // float32.  Values enter the second product as code times scale in float16 (11 bits, two roundings of 2^-12), in units of a
 // power of two, the probabilities in float16; their sum is taken in float32 before that.  Against 64 bits the output is off by
 // its own rounding to bfloat16, 0.0017 of its norm (with bfloat16 probabilities it was 0.0024, with bfloat16 values too
-// 0.0028).  A tile with a value's scale outside 2^-17 .. 2^3 of the first tile's largest is "wide": codes in bfloat16, exactly,
-// and the scales joined to probabilities in bfloat16, whose range is float32's.
+// 0.0028).  The unit stays while a tile's scales lie within 2^-13 .. 2^8 of it and is the tile's own otherwise; the outputs so far
+// are then multiplied by a power of two, so that no bit depends on it.  A tile whose own scales lie more than 2^17 apart is
+// "wide": codes in bfloat16, exactly, and the scales joined to probabilities in bfloat16, whose range is float32's.
 //
 // Six warps turn a key tile's bytes (fetched by TMA, a box a page) into swizzled 16-bit tiles, once for the 256 rows of the
 // two query tiles that share them.
@@ -23,8 +24,8 @@
 //
 // Keys are cut at multiples of 4,096 (chunks of constant size from key 0); a query tile that reaches over a cut has a CTA a
 // chunk, and a second kernel adds the partial results in chunk order.  Key tiles are anchored at key 0, cuts depend on
-// positions alone and units are powers of two, so a row's bits do not depend on the step (but for wide tiles, which a
-// portion's first tile and the keys there are decide).
+// positions alone and units are powers of two, so a row's bits do not depend on the step (but for a tile of which it does not
+// see all keys and some that it does not see make the tile wide).
 //
 // What bounds it: 2.5 us a key tile for both query tiles, of which the products need 1.1.  A query tile's chain is its
 // scores' way out of tensor memory, scales, maximum, exponentials, packing (some 700 instructions a warp) and the next
@@ -217,7 +218,7 @@ __device__ __forceinline__ unsigned times_f16(unsigned codes, __half2 scale) {
 }
 
 // What the keys of a tile have in common.  value_exp: the values' scales are in units of 2^value_exp, the outputs too.
-// wide: some scale lies outside float16's range then.  nan: the keys that are no numbers, bit l of word j key 4 l + j.
+// wide: they are too far apart for float16.  nan: the keys that are no numbers, bit l of word j key 4 l + j.
 struct TileInfo {
   unsigned nan[4], any_nan;
   int wide, value_exp, pad;
@@ -510,34 +511,46 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
     load_scales(row_now);
     int row_next = row_of(1);
     const float unit = a.scale * LOG2E;
-    int value_exp = -1000;      // (not known before a scale that is not zero)
+    constexpr int UNSET = -1000;
+    int value_exp = UNSET;      // (not known before a scale that is not zero)
+    // what some row sees; the other keys of a tile are somebody else's, or not there yet
+    const int seen_from = first_visible_key(prefix + (any0 ? tokx[0] : tokx[1]), a.window);
+    const int seen_to = prefix + (any1 ? tokx[1] + ntok[1] : tokx[0] + ntok[0]);
     for (int i = 0; i < ntiles && ok; ++i) {
       if (i >= SLOTS) ok = mbar_wait_brief(&sc_empty[i % SLOTS], (i / SLOTS - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      const int left = kv_len - ((j0 + i) * TILE + lane * 4);
+      const int key = (j0 + i) * TILE + lane * 4;
       unsigned bad[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         // a key or a value that is no number shows in the sums of the rows that see it
         const float both = (ks[j] - ks[j]) + (vs[j] - vs[j]);
-        const bool is_nan = left > j && both != both;
+        const bool seen = key + j >= seen_from && key + j < seen_to, is_nan = seen && both != both;
         bad[j] = __ballot_sync(0xffffffffu, is_nan);
         ks[j] *= unit;
-        if (left <= j || is_nan) ks[j] = vs[j] = 0.f;
+        if (!seen || is_nan) ks[j] = vs[j] = 0.f;
+        if (fabsf(vs[j]) < 0x1p-106f) vs[j] = 0.f;      // (a row of values below 2^-99, such as zeros: it reads back as zeros)
       }
-      // The values' unit takes the largest scale of the first tile to 2^4 .. 2^5; scales of 2^-13 .. 2^8 leave float16 all of
-      // its bits for the values.
       float top = 0.f, bottom = INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         top = fmaxf(top, fabsf(vs[j]));
         if (vs[j] != 0.f) bottom = fminf(bottom, fabsf(vs[j]));
       }
-      top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-      bottom = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(bottom)));
-      if (value_exp == -1000 && top > 0.f) value_exp = max((int)(__float_as_uint(top) >> 23), 5) - 131;
-      const float to_unit = value_exp == -1000 ? 0.f : two_to(-value_exp);
+      const int top_exp = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 127;
+      const int bottom_exp = (int)(__reduce_min_sync(0xffffffffu, __float_as_uint(bottom)) >> 23) - 127;
+      // A unit takes the largest scale to 2^4 .. 2^5; scales of 2^-13 .. 2^8 leave float16 all of its bits for the values.
+      bool wide = false;
+      if (top_exp > -127) {
+        wide = top_exp - bottom_exp > 17;
+        if (value_exp == UNSET || top_exp - value_exp > (wide ? 40 : 7)) value_exp = top_exp - 4;
+        if (!wide && bottom_exp - value_exp < -13) {
+          // (float32 holds the outputs so far in a unit up to 2^80 smaller)
+          if (value_exp - (top_exp - 4) > 80) wide = true; else value_exp = top_exp - 4;
+        }
+      }
+      const float to_unit = value_exp == UNSET ? 0.f : two_to(-value_exp);
       float* slot = scales + (i % SLOTS) * 256 + lane * 4;
       *reinterpret_cast<float4*>(slot) = make_float4(ks[0], ks[1], ks[2], ks[3]);
       *reinterpret_cast<float4*>(slot + 128) = make_float4(vs[0] * to_unit, vs[1] * to_unit, vs[2] * to_unit, vs[3] * to_unit);
@@ -546,8 +559,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         n.any_nan = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) n.any_nan |= n.nan[j] = bad[j];
-        n.wide = top * to_unit > 256.f || bottom * to_unit < 0x1p-13f;
-        n.value_exp = value_exp == -1000 ? 0 : value_exp;
+        n.wide = wide;
+        n.value_exp = value_exp == UNSET ? 0 : value_exp;
         n.pad = 0;
         infos[i % SLOTS] = n;
       }
@@ -691,8 +704,9 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         for (int k = max(first, 0); k <= min(last, TILE - 1); ++k)
           if (info->nan[k & 3] >> (k >> 2) & 1) l = __int_as_float(0x7fc00000);
       }
+      const int old_exp = value_exp;
       value_exp = info->value_exp;
-      const bool wide_tile = info->wide != 0;
+      const bool wide_tile = info->wide != 0, moved = i > i_first && value_exp != old_exp;
       // the reference rises only when it must (or at the first visible key)
       float factor = 1.0f;
       bool rescale = false;
@@ -702,9 +716,10 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         m_ref = mx;
         l *= factor;
       }
-      // O of this tile is rescaled when a row of the warp raised its reference.  Its last product completed before these
-      // scores did, except where the tile runs alone: the product of i - 1 is waited for there.
-      if (__builtin_expect(__any_sync(0xffffffffu, rescale), 0)) {
+      // O of this tile is rescaled when a row of the warp raised its reference, or the values' unit moved.  Its last product
+      // completed before these scores did, except where the tile runs alone: the product of i - 1 is waited for there.
+      if (__builtin_expect(__any_sync(0xffffffffu, rescale) || moved, 0)) {
+        const float by = (rescale ? factor : 1.f) * (moved ? two_to(max(old_exp - value_exp, -126)) : 1.f);
         if (i > my_solo) {
           ok = mbar_wait_brief(pv_done, (i - 1 - my_solo) & 1);
           ok = __all_sync(0xffffffffu, ok);
@@ -717,7 +732,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
           tc_ld8(tmem_o + c * 8, o);
           tc_wait_ld();
 #pragma unroll
-          for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * (rescale ? factor : 1.0f));
+          for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
           tc_st8(tmem_o + c * 8, o);
         }
       }

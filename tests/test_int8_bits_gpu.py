@@ -88,6 +88,56 @@ def test_partial_results_in_several_launches(window, monkeypatch):
     ops.check_kernel_status()
 
 
+# ---- the other sequences of a step, and keys that a row does not see
+
+def _alone(case, s):
+    """Sequence s of a case by itself."""
+    alone = Int8Case.__new__(Int8Case)
+    alone.__dict__.update(case.__dict__)
+    alone.tables, alone.lens = [case.tables[s]], [case.lens[s]]
+    return alone
+
+
+@pytest.mark.parametrize("window", [None, 60, 150])
+@pytest.mark.parametrize("step", [4, -4, 13, -13])
+def test_a_prompt_with_moving_value_scales_attends_the_same_in_any_step(window, step):
+    """Value scales 2^step times larger from each tile of 128 keys to the next; alone, in portions, and beside prompts that make
+    query tiles share their keys in another way."""
+    scales = lambda n, hkv, g: (2.0 ** (torch.arange(n) // 128 * step) * (1 + torch.arange(n) % 7))[:, None].expand(n, hkv).contiguous()
+    case = Int8Case([900, 900, 900, 800], 2, 128, 16, seed=6, value_scales=scales)
+    cache, q_lens = ops.Int8Cache(case.data, case.scales), [300, 900, 900, 800]
+    q = _rand(sum(q_lens), 8, 128, seed=7, dtype=BF16)
+    whole = ops.paged_attention(q, cache, case.meta(q_lens), 0.1, window)
+    alone = _alone(case, 0)
+    assert torch.equal(ops.paged_attention(q[:300].contiguous(), cache, alone.meta([300]), 0.1, window), whole[:300])
+    for n in (200, 131, 33, 2):
+        assert torch.equal(ops.paged_attention(q[300 - n:300].contiguous(), cache, alone.meta([n]), 0.1, window), whole[300 - n:300])
+    exact, _, _ = alone.attention(q[:300], [300], 0.1, window)
+    # (of a row's norm, as above)
+    assert ((whole[:300].double() - exact).norm(dim=-1) <= 2.0 ** -8 * exact.norm(dim=-1)).all()
+
+
+def _with_scales(case, s, keys, kv, scale):
+    """The case's cache with the scales of some keys of sequence s set."""
+    scales = case.scales.clone()
+    at = torch.tensor(keys)
+    page = torch.tensor(case.tables[s])[at // case.page_size].cuda()
+    scales[page, kv, :, (at % case.page_size).cuda()] = scale
+    return ops.Int8Cache(case.data, scales)
+
+
+@pytest.mark.parametrize("kv", [0, 1])
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), 2.0 ** 20, 2.0 ** -40, 0.0])
+def test_prompt_rows_do_not_depend_on_keys_before_the_window(kv, scale):
+    """Pages that a window has left may be anybody's."""
+    case = Int8Case([700], 2, 128, 16, seed=3)
+    q = _rand(300, 8, 128, seed=4, dtype=BF16)
+    run = lambda cache: ops.paged_attention(q, cache, case.meta([300]), 0.1, 70)
+    want = run(ops.Int8Cache(case.data, case.scales))
+    assert torch.equal(run(_with_scales(case, 0, range(400 - 69), kv, scale)), want)
+    ops.check_kernel_status()
+
+
 @pytest.mark.parametrize("name", ["d", "e"])
 def test_short_portions_replayed_give_the_bits_of_launched_ones(name, tiny_model_dirs):
     """Portions of 3 to 7 tokens behind different prompts, one bucket: from the third on they are replayed."""
