@@ -203,8 +203,8 @@ template <int ROWS> __device__ __forceinline__ SplitSeq split_seq(const SplitArg
 struct __align__(16) SplitItem {
   int seq, q_begin, n, kv_len;      // the sequence: index, first token, new tokens, keys
   int i, kvh, tile, local;          // sequence of the launch, kv head, tile of rows, number of the item in its sequence
-  int run_at, at, end, splits;      // first key of the run; its keys [at, end), `at` a multiple of 128 and perhaps before the
-                                    // first one seen; runs of the sequence
+  int seen, at, end, splits;        // its keys: [seen, end), those of the run that some row sees; its tiles from `at` on, a multiple
+                                    // of 128; runs of the sequence
   int fresh, tiles, lo_all, hi_all;        // other query rows than the item before; tiles of keys, 0: there are no more
                                            // items; the keys that every row sees
 };
@@ -364,11 +364,11 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
         __syncwarp();
         const int row = page * 2 * half + (kvh << a.page_shift) + off;
         if (senders >> lane & 1) tma_load_2d(smem_u32(smem) + stage * SH::STAGE + lane * 512, &map, 0, row, &k_full[stage]);
-        if (have) {
-          const unsigned sc = smem_u32(scales) + stage * 1024 + lane * 16;
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(sc), "l"(a.scales + row) : "memory");
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(sc + 512), "l"(a.scales + row + half) : "memory");
-        }
+        // (keys that are not there, and those on a page that is none of the pool's: scales of zero)
+        const unsigned sc = smem_u32(scales) + stage * 1024 + lane * 16, bytes = have ? 16 : 0;
+        const float* from = a.scales + (have ? row : 0);
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(sc), "l"(from), "r"(bytes) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(sc + 512), "l"(from + half), "r"(bytes) : "memory");
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&k_full[stage])) : "memory");
         if (n > 0) send_values(n - 1);
         v_row = row + half;
@@ -468,7 +468,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
         const int unit = s.splits > 1 ? local / s.splits : local;
         it.seq = s.seq; it.q_begin = s.q_begin; it.n = s.n; it.kv_len = s.kv_len;
         it.i = i; it.local = local; it.splits = s.splits;
-        it.run_at = (local - unit * s.splits) * s.split;
+        const int run_at = (local - unit * s.splits) * s.split;
         it.kvh = s.tiles > 1 ? unit / s.tiles : unit;
         it.tile = unit - it.kvh * s.tiles;
         const int p0 = s.kv_len - s.n;
@@ -477,10 +477,10 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
           tok0 = it.tile * ROWS / G;
           tok1 = (min((it.tile + 1) * ROWS, s.n * G) - 1) / G;
         }
-        const int k_lo = max(it.run_at, first_visible_key(p0 + tok0, a.window));
-        it.end = min(it.run_at + s.split, p0 + tok1 + 1);
-        it.at = k_lo & ~(SP_TILE - 1);
-        if (it.end <= k_lo) {
+        it.seen = max(run_at, first_visible_key(p0 + tok0, a.window));
+        it.end = min(run_at + s.split, p0 + tok1 + 1);
+        it.at = it.seen & ~(SP_TILE - 1);
+        if (it.end <= it.seen) {
           if (s.splits == 1) {             // a sequence of one run: rows that see no key are zeros, from here
             const int rows = min(ROWS, s.n * G - it.tile * ROWS);
             for (int e = lane; e < rows * a.D; e += 32) {
@@ -491,7 +491,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
           continue;
         }
         it.tiles = (it.end - it.at + SP_TILE - 1) / SP_TILE;
-        it.lo_all = max(it.run_at, first_visible_key(p0 + tok1, a.window));
+        it.lo_all = max(run_at, first_visible_key(p0 + tok1, a.window));
         it.hi_all = min(it.end - 1, p0 + tok0);
         it.fresh = i != old_i || it.kvh != old_kvh || it.tile != old_tile;
         old_i = i; old_kvh = it.kvh; old_tile = it.tile;
@@ -695,13 +695,14 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        // scores, in units of log 2
-        const float vs_raw = scales[buf * 256 + 128 + key_of];
-        const float ks = scales[buf * 256 + key_of] + (vs_raw - vs_raw);      // NaN if either is
+        // scores, in units of log 2.  A scale that is no finite number, the key's or the value's, makes the key's scores NaN in
+        // the rows that see it, and the value's is zero then: a row that does not see it multiplies it by a probability of zero.
+        const float vs_raw = scales[buf * 256 + 128 + key_of], ks_raw = scales[buf * 256 + key_of];
+        const float no_number = (ks_raw - ks_raw) + (vs_raw - vs_raw), ks = ks_raw + no_number;
         const int key = kb + key_of;
         const bool plain = kb >= it.lo_all && kb + SP_TILE - 1 <= it.hi_all;        // every row sees every key
-        const bool there = key >= it.run_at && key < it.end;
-        const float vs = there ? vs_raw : 0.f, lv = there ? fmaxf(__log2f(vs), -120.f) : -INFINITY;
+        const bool there = key >= it.seen && key < it.end;
+        const float vs = there && no_number == 0.f ? vs_raw : 0.f, lv = there ? fmaxf(__log2f(vs), -120.f) : -INFINITY;
         float s[ROWS];
 #pragma unroll
         for (int r8 = 0; r8 < ROWS; r8 += R8) {
@@ -722,11 +723,12 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
           for (int r = 0; r < ROWS; ++r)
             if (!there || key < __float_as_int(data[ROWS + r]) || key > __float_as_int(data[2 * ROWS + r])) s[r] = -INFINITY;
         }
-        // the tile's largest weight of each row, and its largest value scale
+        // the tile's largest weight of each row, and the largest value scale of the keys that all rows see: what one row sees
+        // has no part in another's reference
         float top[ROWS];
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) top[r] = warp_top(s[r] + lv);
-        float size = warp_top(lv);
+        float size = warp_top(key >= it.lo_all && key <= it.hi_all ? lv : -INFINITY);
         float* mine = tops + (buf * 4) * (ROWS + 4);
         if (lane == 0) {
 #pragma unroll
@@ -737,6 +739,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
         asm volatile("bar.sync 1, 128;" ::: "memory");
 #pragma unroll
         for (int w = 0; w < 4; ++w) size = fmaxf(size, mine[w * (ROWS + 4) + ROWS]);
+        if (size == -INFINITY) size = 0.f;
 #pragma unroll
         for (int r = 0; r < ROWS; r += 4) {
           float4 v = *reinterpret_cast<const float4*>(mine + r);

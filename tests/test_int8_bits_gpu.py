@@ -138,6 +138,53 @@ def test_prompt_rows_do_not_depend_on_keys_before_the_window(kv, scale):
     ops.check_kernel_status()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kv", [0, 1])
+@pytest.mark.parametrize("q_len", [1, 5])
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), 2.0 ** 20, 2.0 ** -40, 0.0])
+def test_few_rows_do_not_depend_on_keys_before_the_window(q_len, kv, scale, dtype):
+    case = Int8Case([700, 300], 2, 128, 16, seed=3)
+    q = _rand(2 * q_len, 4, 128, seed=4, dtype=dtype)
+    run = lambda cache: ops.int8_paged_attention(q, cache, case.meta([q_len] * 2), 0.1, 70)
+    want = run(ops.Int8Cache(case.data, case.scales))
+    assert want.isfinite().all()
+    assert torch.equal(run(_with_scales(case, 0, range(700 - q_len - 69), kv, scale)), want)
+    ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kv", [0, 1])
+@pytest.mark.parametrize("portions", [False, True])
+@pytest.mark.parametrize("scale", [float("nan"), -float("inf"), 2.0 ** 10, 2.0 ** -5])
+def test_rows_do_not_depend_on_later_keys(portions, kv, scale, dtype):
+    """The last two of six tokens have another scale: the rows in front keep their bits, and a scale that is no number shows in
+    every row that sees it."""
+    case = Int8Case([300], 2, 128, 16, seed=5)
+    q = _rand(6, 4, 128, seed=4, dtype=dtype)
+    run = lambda cache: ops.int8_paged_attention(q, cache, case.meta([6]), 0.1, portions=portions)
+    want, got = run(ops.Int8Cache(case.data, case.scales)), run(_with_scales(case, 0, [298, 299], kv, scale))
+    assert want.isfinite().all() and torch.equal(got[:4], want[:4])
+    assert (got[4:].isnan().all() if scale != scale or abs(scale) == float("inf") else (got[4:] != want[4:]).any())
+    ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("q_len", [1, 4, 40])
+def test_a_page_that_is_none_of_the_pools_is_a_page_of_zeros(q_len, dtype):
+    """Not what was read before it, and nothing beyond the pool."""
+    case = Int8Case([300, 300], 2, 128, 16, seed=5)
+    q = _rand(2 * q_len, 4, 128, seed=4, dtype=dtype)
+    zeros = ops.Int8Cache(case.data.clone(), case.scales.clone())
+    page = case.tables[0][7]
+    zeros.scales[page] = 0
+    want = ops.int8_paged_attention(q, zeros, case.meta([q_len] * 2), 0.1)
+    for entry in (-1, case.data.shape[0], 2 ** 31 - 1):
+        meta = case.meta([q_len] * 2)
+        meta.block_table[0, 7] = entry
+        assert torch.equal(ops.int8_paged_attention(q, ops.Int8Cache(case.data, case.scales), meta, 0.1), want)
+    ops.check_kernel_status()
+
+
 @pytest.mark.parametrize("name", ["d", "e"])
 def test_short_portions_replayed_give_the_bits_of_launched_ones(name, tiny_model_dirs):
     """Portions of 3 to 7 tokens behind different prompts, one bucket: from the third on they are replayed."""
