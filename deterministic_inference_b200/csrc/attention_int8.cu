@@ -77,8 +77,12 @@ __host__ __device__ __forceinline__ int split_keys(int kv_len, int rows) {
   return tiles <= 2 ? base : base * tiles;
 }
 
-// What a work item takes, in tiles of 128 keys: its own, and one for its beginning and end.
-__device__ __forceinline__ int item_work(int split) { return split / SP_TILE + 1; }
+// What a work item takes, in tiles of 128 keys: its own, and one for its beginning and end.  (Of a run longer than the sequence
+// those of the sequence, as a run grows with the rows; but not below 512, so that short sequences' items do not share a CTA
+// while others have none.)
+__device__ __forceinline__ int item_work(int split, int kv_len) {
+  return (min(split, max(kv_len, 512)) + SP_TILE - 1) / SP_TILE + 1;
+}
 
 __device__ __forceinline__ void mbar_arrive(unsigned long long* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -272,10 +276,11 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) prefetch_tensormap(&map);
   if (!a.late) pdl_trigger();
-  // ---- the work before each sequence (metadata alone, which no kernel of a step writes)
+  // ---- the work before each sequence (metadata alone, which no kernel of a step writes); all of it stays below 2^31, which the
+  // host sees to
   for (int i = threadIdx.x; i < a.seq_count; i += SP_THREADS) {
     const SplitSeq s = split_seq<ROWS>(a, i);
-    first[i + 1] = s.tiles * s.splits * a.Hkv * item_work(s.split);
+    first[i + 1] = s.tiles * s.splits * a.Hkv * item_work(s.split, s.kv_len);
   }
   if (threadIdx.x == 0) first[0] = 0;
   if (threadIdx.x == 32) {
@@ -449,7 +454,8 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       if (first[mid] <= from_work) i = mid; else hi = mid - 1;
     }
     if (total > 0) {
-      const int each = item_work(split_seq<ROWS>(a, i).split);
+      const SplitSeq s = split_seq<ROWS>(a, i);
+      const int each = item_work(s.split, s.kv_len);
       item = (from_work - first[i] + each - 1) / each;       // the first item that begins in it
     }
     for (int k = 0; ok; ++item) {
@@ -459,7 +465,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       for (; i < a.seq_count; ++i, item = 0) {
         s = split_seq<ROWS>(a, i);
         if (item < s.tiles * s.splits * a.Hkv) {
-          more = first[i] + item * item_work(s.split) < to_work;
+          more = first[i] + item * item_work(s.split, s.kv_len) < to_work;
           break;
         }
       }
@@ -1069,7 +1075,8 @@ int dib_int8_attention_split_keys(int kv_len, int rows) { return split_keys(kv_l
 // The split form, for the sequences seq_list[0 .. seq_count) or (null) seq_first ...: heads up to 128, pages of a
 // power of two of rows, 4 at least.  max_rows: the most rows (new tokens x query heads of a kv head) of one of them; tile_rows: 8,
 // 16 or (bfloat16) 4, 24 or 32 rows a tile; max_items: the most (tiles x runs x kv heads) of one; part_o float32 [seq_count, max_items,
-// tile_rows, D] and part_ml [.., 2] take partial results where merge is not 0 (some sequence may have two runs).
+// tile_rows, D] and part_ml [.., 2] take partial results where merge is not 0 (some sequence may have two runs).  The work
+// of all of them, (tiles of rows) x (kv heads) x (runs) x (tiles of keys of a run, and one), is below 2^31.
 int dib_int8_attention_split(const void* q, void* out, const void* data, const void* scales, long long num_pages,
                              const void* block_table, int max_blocks, const void* cu_q_lens, const void* seq_lens,
                              const void* seq_list, int seq_first, int seq_count, int max_rows, int tile_rows, void* part_o,

@@ -404,6 +404,12 @@ def _lib():
     return _ops()._lib("attention_int8")
 
 
+def _split_work(seqs: list, q_lens: list, kv_lens: list, group: int, hkv: int, tile_rows: int, runs: int) -> int:
+    """The most work that the split form's kernel counts, in tiles of 128 keys (a work item: its run's, the last run counted as
+    a whole one, and one; of 512 keys at least)."""
+    return sum(hkv * -(-q_lens[s] * group // tile_rows) * (2 * (kv_lens[s] // 128 + 3) + runs) for s in seqs)
+
+
 class _SplitPart:
     """The sequences of one launch: their number, the most rows of one, rows a tile, the most work items of one."""
 
@@ -416,6 +422,11 @@ class _SplitPart:
         self.tile_rows = next(r for r in ((8, 16) if wide else (4, 8, 16, 24, 32)) if self.max_rows <= r or r == (16 if wide else 32))
         runs = _most_runs(max(kv_lens[s] for s in seqs), group)
         tiles, per32 = -(-self.max_rows // self.tile_rows), 32 // self.tile_rows
+        longest = max(kv_lens[s] for s in seqs)
+        if count * hkv * tiles * (2 * (longest // 128 + 3) + runs) >= 1 << 31 \
+                and _split_work(seqs, q_lens, kv_lens, group, hkv, self.tile_rows, runs) >= 1 << 31:
+            raise _ops().KernelError(f"int8_paged_attention: {sum(q_lens[s] for s in seqs)} new tokens of up to {longest} keys, "
+                                     f"{group} heads a kv head, are more than a launch counts: smaller portions")
         # (runs get longer with the rows: tiles * runs is largest at 64 rows, or the tiles' own number is)
         self.items = hkv * min(tiles * runs, max(2 * per32 * runs, per32 * (runs + 1) + tiles))
         # (rows of partial results: none where every sequence has one run)

@@ -207,3 +207,15 @@ def test_short_portions_replayed_give_the_bits_of_launched_ones(name, tiny_model
     ops.check_kernel_status()
     for i, (a, b) in enumerate(zip(*outs)):
         assert torch.equal(a, b), i
+
+
+def test_a_portion_whose_work_is_large():
+    """1,024 float32 tokens of 512 heads on one kv head: the count of work items once went beyond 31 bits, and rows were left
+    out."""
+    case = Int8Case([1024], 1, 16, 16, seed=1)
+    cache, q = ops.Int8Cache(case.data, case.scales), _rand(1024, 512, 16, seed=2)
+    out = ops.int8_paged_attention(q, cache, case.meta([1024]), 0.25)
+    ops.check_kernel_status()
+    exact, vmax, smax = case.attention(q, [1024], 0.25)
+    tol = (2 * smax * (2.0 ** -21 + 4 * 2.0 ** -23) + 2.0 ** -20) * vmax      # as for every float32 case
+    assert ((out.double() - exact).abs() <= tol).all()

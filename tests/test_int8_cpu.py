@@ -84,3 +84,28 @@ def test_split_work_covers_the_steps_that_the_lengths_allow(group, wide):
                 two |= runs > 1
             two |= _runs(min(kv, 16384), group) > 1
         assert (part.rows > 0) == two
+
+
+def _device_work(q: int, kv: int, group: int, hkv: int, tile_rows: int) -> int:
+    """What the split form's kernel counts for a sequence."""
+    split = int8._lib().dib_int8_attention_split_keys(kv, q * group)
+    return -(-q * group // tile_rows) * max(1, -(-kv // split)) * hkv * (-(-min(split, max(kv, 512)) // 128) + 1)
+
+
+def test_the_work_of_a_step_is_counted_without_overflow():
+    """A long float32 portion's work, and that of several, stays below 2^31; a step beyond it is refused."""
+    for q, kv, group, hkv in ((23171, 23171, 8, 8), (100000, 100000, 8, 8), (1024, 1024, 512, 1), (8192, 65536, 8, 8)):
+        part = int8._SplitPart([0], [q], [kv], group, hkv, True, torch.device("cpu"))
+        assert _device_work(q, kv, group, hkv, part.tile_rows) < 1 << 31
+    for group in (1, 8):
+        int8._SplitPart(list(range(64)), [8192] * 64, [8192] * 64, group, 8, True, torch.device("cpu"))
+        with pytest.raises(ops.KernelError, match="smaller portions"):
+            int8._SplitPart([0], [1 << 21], [1 << 21], group, 8, True, torch.device("cpu"))
+    rng = random.Random(3)
+    for _ in range(3000):
+        group, tile_rows = rng.choice([1, 2, 5, 8, 64]), rng.choice([4, 8, 16, 24, 32])
+        q, kv = int(2 ** rng.uniform(0, 15)), int(2 ** rng.uniform(0, 18))
+        runs = int8._most_runs(kv, group)
+        most = int8._split_work([0], [q], [kv], group, 8, tile_rows, runs)
+        for _ in range(5):
+            assert _device_work(rng.randrange(1, q + 1), rng.randrange(1, kv + 1), group, 8, tile_rows) <= most
