@@ -116,7 +116,21 @@ class Int8Rows:
     the type of the tensor they were made from, which a product's output takes."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, k: int, dtype: torch.dtype):
-        self.codes, self.scales, self.k, self.dtype = codes, scales, int(k), dtype
+        ops = _ops()
+        ops._need(codes, "codes", torch.int8, 2)
+        ops._need(scales, "scales", torch.float32, 1)
+        if not 1 <= k <= MAX_K or codes.shape[1] != _padded(k) or scales.shape[0] != codes.shape[0]:
+            raise ops.KernelError(f"Int8Rows: codes {tuple(codes.shape)}, scales {tuple(scales.shape)} for rows of {k} values "
+                                  f"(K from 1 to {MAX_K}, codes of K rounded up to 16)")
+        if codes.data_ptr() % 16:
+            raise ops.KernelError("Int8Rows: codes must lie on 16 bytes")
+        _same_device("Int8Rows", codes, scales)
+        _code(dtype, "Int8Rows")
+        self._set(codes, scales, int(k), dtype)
+
+    def _set(self, codes, scales, k, dtype) -> "Int8Rows":
+        self.codes, self.scales, self.k, self.dtype = codes, scales, k, dtype
+        return self
 
     @property
     def shape(self):
@@ -195,7 +209,7 @@ def _quantize(x: torch.Tensor, name: str, early: bool) -> Int8Rows:
     st = _fn("dib_quantize_rows")(x.data_ptr(), x.stride(0), codes.data_ptr(), scales.data_ptr(), m, k, code,
                                   1 if early else 0, _stream())
     _done(st, "quantize_rows", lambda: f"rows {m} x {k}")
-    return Int8Rows(codes, scales, k, x.dtype)
+    return Int8Rows.__new__(Int8Rows)._set(codes, scales, k, x.dtype)
 
 
 def quantize_rows(x) -> Int8Rows:
@@ -226,6 +240,8 @@ def int8_linear(x, weight: Int8Weight, out_dtype=None) -> torch.Tensor:
     out_code = _code(out_dtype, "out")
     out = torch.empty(m, n, dtype=out_dtype, device=device)
     if rows:
+        if x.codes.shape[1] != codes.shape[1]:
+            raise _ops().KernelError(f"int8_linear: codes {tuple(x.codes.shape)} against the weight's {tuple(codes.shape)}")
         st = _fn("dib_gemm_int8")(x.codes.data_ptr(), x.scales.data_ptr(), codes.data_ptr(), weight.scales.data_ptr(),
                                   out.data_ptr(), m, n, x.codes.shape[1], out_code, _sms(device), _stream())
     else:

@@ -1,0 +1,46 @@
+"""What the 8-bit operators refuse, or take in good order, beyond the shapes of their calls."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from deterministic_inference_b200.kernels import ops
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def _rand(*shape, seed=0, dtype=F32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).cuda().to(dtype)
+
+
+def _refused(call, *words):
+    with pytest.raises(ops.KernelError) as e:
+        call()
+    for word in words:
+        assert word in str(e.value)
+
+
+def test_rows_that_are_not_laid_out_as_rows():
+    codes, scales = torch.zeros(4, 64, dtype=torch.int8, device="cuda"), torch.ones(4, device="cuda")
+    good = ops.Int8Rows(codes, scales, 50, BF16)
+    assert good.shape == (4, 50) and ops.int8_linear(good, ops.Int8Weight.of(_rand(8, 50))).dtype == BF16
+    _refused(lambda: ops.Int8Rows(codes, scales, 40, BF16), "rounded up")         # a pitch that is another K's
+    _refused(lambda: ops.Int8Rows(codes, scales, 65, BF16), "rounded up")
+    _refused(lambda: ops.Int8Rows(codes, scales, 0, BF16), "K from 1")
+    _refused(lambda: ops.Int8Rows(codes, scales[:3], 64, BF16), "scales")
+    _refused(lambda: ops.Int8Rows(codes, scales.double(), 64, BF16), "float32")
+    _refused(lambda: ops.Int8Rows(codes.float(), scales, 64, BF16), "int8")
+    _refused(lambda: ops.Int8Rows(codes.t(), scales, 4, BF16), "contiguous")
+    _refused(lambda: ops.Int8Rows(codes.cpu(), scales, 64, BF16), "CUDA")
+    _refused(lambda: ops.Int8Rows(codes, scales, 64, torch.float16), "float16")
+    odd = torch.zeros(4 * 64 + 1, dtype=torch.int8, device="cuda")[1:].view(4, 64)
+    _refused(lambda: ops.Int8Rows(odd, scales, 64, BF16), "16 bytes")
+
+
+def test_a_product_refuses_rows_of_another_pitch():
+    rows, weight = ops.quantize_rows(_rand(4, 40)), ops.Int8Weight.of(_rand(8, 40))
+    assert ops.int8_linear(rows, weight).shape == (4, 8)
+    rows.codes = torch.zeros(4, 64, dtype=torch.int8, device="cuda")
+    _refused(lambda: ops.int8_linear(rows, weight), "against the weight's")
