@@ -932,8 +932,8 @@ __global__ void __launch_bounds__(ANY_WARPS * 32)
 attention_any_kernel(const T* __restrict__ q, T* __restrict__ out, const signed char* __restrict__ data,
                      const float* __restrict__ scales, const int* __restrict__ block_table, int max_blocks,
                      const int* __restrict__ token_seq, const int* __restrict__ cu_q_lens,
-                     const int* __restrict__ seq_lens, int T_, int Hq, int Hkv, int D, int page_size, float scale,
-                     int window) {
+                     const int* __restrict__ seq_lens, int T_, int Hq, int Hkv, int D, int page_size, long long num_pages,
+                     float scale, int window) {
   pdl_prologue(q, data, scales);
   __shared__ float sq[ANY_WARPS][256];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -952,11 +952,12 @@ attention_any_kernel(const T* __restrict__ q, T* __restrict__ out, const signed 
   for (int k0 = lo; k0 <= hi; k0 += 32) {
     const int key = k0 + lane;
     const bool seen = key <= hi;
-    const long long page = seen ? bt[key / page_size] : 0;
-    const long long krow = ((page * 2) * Hkv + kvh) * page_size + (seen ? key % page_size : 0);
-    const long long vrow = krow + (long long)Hkv * page_size;
-    float s = -INFINITY;
-    if (seen) {
+    const long long page = seen ? bt[key / page_size] : -1;
+    const bool have = page >= 0 && page < num_pages;      // (a page that is none of the pool's: keys and values of zeros)
+    const long long krow = ((page * 2) * Hkv + kvh) * page_size + key % page_size;
+    const long long vrow = have ? krow + (long long)Hkv * page_size : -1;
+    float s = seen ? 0.f : -INFINITY;
+    if (have) {
       float dot = 0.f;
       const uint4* p = reinterpret_cast<const uint4*>(data + krow * D);
       for (int c = 0; c < D / 16; ++c) {
@@ -970,7 +971,7 @@ attention_any_kernel(const T* __restrict__ q, T* __restrict__ out, const signed 
     const float top = fmaxf(m, warp_max(s));
     const float p = seen ? exp2f(s - (top == -INFINITY ? 0.f : top)) : 0.f;
     const float alpha = m == -INFINITY ? 0.f : exp2f(m - top);
-    const float vs = seen ? scales[vrow] : 0.f;
+    const float vs = have ? scales[vrow] : 0.f;
     l = l * alpha + warp_sum(p);
     m = top;
 #pragma unroll
@@ -978,7 +979,9 @@ attention_any_kernel(const T* __restrict__ q, T* __restrict__ out, const signed 
     const int n = min(32, hi - k0 + 1);
     for (int j = 0; j < n; ++j) {
       const float pj = __shfl_sync(0xffffffffu, p, j) * __shfl_sync(0xffffffffu, vs, j);
-      const signed char* vp = data + __shfl_sync(0xffffffffu, vrow, j) * D;
+      const long long row = __shfl_sync(0xffffffffu, vrow, j);
+      if (row < 0) continue;
+      const signed char* vp = data + row * D;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (i * 32 + lane < D) o[i] = fmaf(pj, (float)vp[i * 32 + lane], o[i]);
@@ -1126,7 +1129,8 @@ int dib_int8_attention_split(const void* q, void* out, const void* data, const v
 
 int dib_int8_attention_any(const void* q, void* out, const void* data, const void* scales, const void* block_table,
                            int max_blocks, const void* token_seq, const void* cu_q_lens, const void* seq_lens, int T,
-                           int Hq, int Hkv, int D, int page_size, float scale, int window, int dtype, cudaStream_t st) {
+                           int Hq, int Hkv, int D, int page_size, long long num_pages, float scale, int window, int dtype,
+                           cudaStream_t st) {
   if (dtype != 0 && dtype != 1) return DIB_BAD_DTYPE;
   if (T < 0 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || D < 16 || D > 256 || D % 16 != 0 || page_size < 1) return DIB_BAD_SIZE;
   if ((reinterpret_cast<uintptr_t>(data) & 15) != 0) return DIB_BAD_ALIGN;
@@ -1141,11 +1145,11 @@ int dib_int8_attention_any(const void* q, void* out, const void* data, const voi
   if (dtype == 1)
     dib_launch(attention_any_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(ANY_WARPS * 32), 0, st,
                reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<__nv_bfloat16*>(out), d, s, bt, max_blocks, ts,
-               cu, sl, T, Hq, Hkv, D, page_size, scale, window);
+               cu, sl, T, Hq, Hkv, D, page_size, num_pages, scale, window);
   else
     dib_launch(attention_any_kernel<float>, dim3((unsigned)blocks), dim3(ANY_WARPS * 32), 0, st,
                reinterpret_cast<const float*>(q), reinterpret_cast<float*>(out), d, s, bt, max_blocks, ts, cu, sl, T, Hq,
-               Hkv, D, page_size, scale, window);
+               Hkv, D, page_size, num_pages, scale, window);
   DIB_CHECK_LAUNCH();
   return DIB_OK;
 }

@@ -41,7 +41,7 @@ _SIGNATURES = {
     "dib_int8_linear": ("gemm_int8", (_P, _P, _L, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P)),
     "dib_int8_attention_split": ("attention_int8", (_P, _P, _P, _P, _L, _P, _I, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _I, _I,
                                                     _I, _I, _F, _I, _I, _I, _P)),
-    "dib_int8_attention_any": ("attention_int8", (_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _P)),
+    "dib_int8_attention_any": ("attention_int8", (_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _L, _F, _I, _I, _P)),
     "dib_int8_attention_prompt": ("attention_int8_prompt", (_P, _P, _P, _P, _L, _P, _I, _P, _P, _P, _I, _I, _P, _I, _I, _I, _P, _P,
                                                             _I, _I, _I, _I, _I, _I, _F, _I, _P)),
 }
@@ -613,6 +613,6 @@ def int8_paged_attention(q: torch.Tensor, cache: Int8Cache, meta, scale: float, 
         return out
     st = _fn("dib_int8_attention_any")(
         q.data_ptr(), out.data_ptr(), data.data_ptr(), cache.scales.data_ptr(), table.data_ptr(), table.shape[1],
-        token_seq.data_ptr(), cu.data_ptr(), lens.data_ptr(), t, hq, hkv, d, page_size, float(scale), win, code, _stream())
+        token_seq.data_ptr(), cu.data_ptr(), lens.data_ptr(), t, hq, hkv, d, page_size, pages, float(scale), win, code, _stream())
     _done(st, "int8_paged_attention", lambda: f"head_dim {d}, heads {hq}/{hkv}")
     return out

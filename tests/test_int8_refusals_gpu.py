@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from deterministic_inference_b200.kernels import ops
+from tests.int8_util import Int8Case
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
@@ -44,3 +45,19 @@ def test_a_product_refuses_rows_of_another_pitch():
     assert ops.int8_linear(rows, weight).shape == (4, 8)
     rows.codes = torch.zeros(4, 64, dtype=torch.int8, device="cuda")
     _refused(lambda: ops.int8_linear(rows, weight), "against the weight's")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("q_len", [1, 5])
+@pytest.mark.parametrize("hkv,d,page", [(2, 144, 16), (1, 256, 32), (2, 64, 24), (1, 32, 1)])
+def test_pages_that_are_none_of_the_pools_in_the_form_for_every_shape(hkv, d, page, q_len, dtype):
+    """Heads above 128 and pages that are no power of two: such pages are pages of zeros there too."""
+    case = Int8Case([200, 100], hkv, d, page, seed=5)
+    q = _rand(2 * q_len, 2 * hkv, d, seed=4, dtype=dtype)
+    zeros = ops.Int8Cache(case.data.clone(), case.scales.clone())
+    zeros.scales[case.tables[0][2]] = 0
+    want = ops.int8_paged_attention(q, zeros, case.meta([q_len] * 2), 0.1)
+    for entry in (-1, case.data.shape[0], 2 ** 31 - 1):
+        meta = case.meta([q_len] * 2)
+        meta.block_table[0, 2] = entry
+        assert torch.equal(ops.int8_paged_attention(q, ops.Int8Cache(case.data, case.scales), meta, 0.1), want)
