@@ -164,9 +164,9 @@ class Int8Weight:
             padded = torch.zeros(n, _padded(k), dtype=torch.int8, device=codes.device)
             padded[:, :k] = codes
             codes = padded
-        if scales.data_ptr() % 16:
-            scales = scales.clone()
-        self.codes, self.scales = codes, scales
+        # The copy stands between a kernel of this package that may have made the codes (``quantize_rows``), and that lets the
+        # next one start beside it, and a product, which reads its weight ahead of its wait: a copy waits for all of it.
+        self.codes, self.scales = codes, scales.clone()
 
     @classmethod
     def of(cls, weight: torch.Tensor) -> "Int8Weight":

@@ -64,3 +64,21 @@ def test_a_product_behind_attention_in_a_graph_of_longer_sequences(hq, hkv):
         graph.replay()
         assert torch.equal(y, want[i & 1]), f"replay {i}"
     ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("m,n,k", [(4, 4096, 4096), (40, 8192, 2048), (700, 2048, 4096)])
+def test_a_weight_made_of_rows_that_are_still_being_quantised(m, n, k):
+    """The product reads its weight ahead of its wait for the kernel in front; one made of ``quantize_rows``' codes, and used at
+    once, is read when they are there."""
+    x = ops.quantize_rows(_rand(m, k, seed=1, dtype=BF16))
+    sources = [_rand(n, k, seed=s, dtype=BF16) for s in (2, 3)]
+    want = [ops.int8_linear(x, ops.Int8Weight.of(w)) for w in sources]
+    torch.cuda.synchronize()
+    for i in range(30):
+        rows = ops.quantize_rows(sources[i & 1])
+        weight = ops.Int8Weight(rows.codes, rows.scales)
+        y = ops.int8_linear(x, weight)
+        assert weight.scales.data_ptr() != rows.scales.data_ptr()      # (the copy that stands between)
+        del rows, weight
+        assert torch.equal(y, want[i & 1]), f"pass {i}"
+    ops.check_kernel_status()
