@@ -334,7 +334,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
     // ---- copies: lane l has the keys 4l .. 4l + 3 of a tile; the first lane of each page sends for its rows.  Keys are
     // free again once the scores are made, long before the values: keys go a tile ahead of them.
     const int page_mask = (1 << a.page_shift) - 1, half = a.Hkv << a.page_shift;      // rows of a page's keys
-    int n = 0, v_row = 0;                  // tiles sent for; the values' row of the tile before
+    int n = 0, v_sent = 0, v_row = 0;      // tiles whose keys, whose values were sent for; the values' row of the tile before
     unsigned v_senders = 0;
     auto send_values = [&](int m) {        // of tile m
       if (m >= SP_STAGES) ok = mbar_wait_brief(&v_empty[m & 1], ((m >> 1) - 1) & 1);
@@ -344,6 +344,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       __syncwarp();
       if (v_senders >> lane & 1)
         tma_load_2d(smem_u32(smem) + (m & 1) * SH::STAGE + SP_TILE * 128 + lane * 512, &map, 0, v_row, &v_full[m & 1]);
+      v_sent = m + 1;
     };
     for (int k = 0; ok; ++k) {
       const int slot = k % SP_ITEMS;
@@ -381,6 +382,10 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
       }
     }
     if (ok && n > 0) send_values(n - 1);
+    if (!ok) {      // given up: what was sent for arrives before this memory is another's
+      for (int m = max(n - SP_STAGES, 0); m < n; ++m) mbar_wait_brief(&k_full[m & 1], (m >> 1) & 1);
+      for (int m = max(v_sent - SP_STAGES, 0); m < v_sent; ++m) mbar_wait_brief(&v_full[m & 1], (m >> 1) & 1);
+    }
   } else if (warp == SP_SCORE_WARP) {
     // ---- scores: a tile ahead of the softmax
     {

@@ -452,13 +452,18 @@ gemm_large_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       }
       pdl_wait();
       for (int c = 0; c < pre; ++c) load_x(c);
-      for (int c = pre; c < total && ok; ++c) {
+      int c = pre;
+      for (; c < total; ++c) {
         ok = mbar_wait_brief(&empty[c % STAGES], ((c / STAGES) - 1) & 1);
         if (!ok) break;
         if (rank == 0) mbar_expect_tx(&full[c % STAGES], CTAS * STAGE);
         load_w(c);
         load_x(c);
       }
+      // given up: what was sent for arrives before this memory is another's (the pair's second CTA stays until the first, whose
+      // barriers count for both, has waited)
+      if (!ok && rank == 0)
+        for (int s = c - STAGES; s < c; ++s) mbar_wait_brief(&full[s % STAGES], (s / STAGES) & 1);
     }
   } else if (warp == 1) {
     if (rank == 0) {
@@ -596,12 +601,15 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       for (int c = 0; c < pre; ++c) load_w(c);      // weights are constants: the first stages' go out before the wait
       pdl_wait();
       for (int c = 0; c < pre; ++c) load_x(c);
-      for (int c = pre; c < count; ++c) {
+      int c = pre;
+      for (; c < count; ++c) {
         ok = mbar_wait_brief(&empty[c % a.stages], ((c / a.stages) - 1) & 1);
         if (!ok) break;
         load_w(c);
         load_x(c);
       }
+      if (!ok)      // (as in the kernel above)
+        for (int s = c - a.stages; s < c; ++s) mbar_wait_brief(&full[s % a.stages], (s / a.stages) & 1);
     }
   } else if (warp == 1) {
     const unsigned elected = elect_one();

@@ -154,3 +154,25 @@ def test_no_block_leaves_without_having_waited_for_the_kernel_in_front(name):
                 blocks[-1] = True
                 waited = True
         assert waited, f"{name}: {kernel} never waits"
+
+
+# ---- kernels that give up
+
+def _limited(name: str) -> list:
+    """(kernel, body) of the kernels whose waits may give up, lambdas and all."""
+    text = re.sub(r"//[^\n]*", "", (CSRC / name).read_text())
+    starts = [m.start() for m in GLOBAL.finditer(text)] + [len(text)]
+    parts = [(GLOBAL.match(text, a).group(1), text[a:b]) for a, b in zip(starts, starts[1:])]
+    return [(k, body) for k, body in parts if "mbar_wait_brief" in body]
+
+
+@pytest.mark.parametrize("name", ["gemm_int8.cu", "attention_int8.cu", "attention_int8_prompt.cu"])
+def test_a_kernel_that_gives_up_waits_for_its_copies(name):
+    """After a wait that ran out a kernel waits for the copies it has sent for, with a limit again."""
+    kernels = _limited(name)
+    assert kernels
+    for kernel, body in kernels:
+        assert re.search(r"tma_load_2d", body), kernel
+        copies = re.search(r"for \(int \w+ = [^;]*(?:- a?\.?stages|- STAGES|- SP_STAGES|sent - RING)[^;]*; [^;]*; \+\+\w+\)\s*"
+                           r"(?:if \(!)?mbar_wait_brief\(&\w*full\[", body)
+        assert copies, f"{name}: {kernel} leaves with copies in flight"
