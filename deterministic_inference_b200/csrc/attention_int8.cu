@@ -272,6 +272,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
   unsigned long long* item_full = bars + 16;   // [SP_ITEMS] an item's record is there
   unsigned long long* item_empty = bars + 16 + SP_ITEMS;      // [SP_ITEMS] it has been read by every role
   unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + 16 + 2 * SP_ITEMS);
+  int* softmax_left = reinterpret_cast<int*>(tmem_slot + 1);      // softmax warps that have ended
   int* first = reinterpret_cast<int*>(smem + SH::FIRST);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) prefetch_tensormap(&map);
@@ -284,6 +285,7 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
   }
   if (threadIdx.x == 0) first[0] = 0;
   if (threadIdx.x == 32) {
+    *softmax_left = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 33);
       mbar_init(&v_full[i], 1);
@@ -824,6 +826,17 @@ attention_split_kernel(const __grid_constant__ CUtensorMap map, const T* __restr
     if (ok && n > 0) {
       add_outputs(n - 1);
       if (ok) finish();
+    }
+    // A warp that has given up arrives at the four warps' barrier, which has no limit of its own, until the others have left it:
+    // they come to the end of their item, or to a wait for what this warp no longer does.
+    if (lane == 0) atomicAdd(softmax_left, 1);
+    if (!ok) {
+      for (int i = 0; i < 4096; ++i) {
+        const int left = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile int*>(softmax_left), 0);
+        if (left == 4) break;
+        asm volatile("bar.arrive 1, 128;" ::: "memory");
+        __nanosleep(1000000);
+      }
     }
   }
   if (!ok) atomicExch(&dib_attention_int8_error_word, 1);

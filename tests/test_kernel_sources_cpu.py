@@ -176,3 +176,12 @@ def test_a_kernel_that_gives_up_waits_for_its_copies(name):
         copies = re.search(r"for \(int \w+ = [^;]*(?:- a?\.?stages|- STAGES|- SP_STAGES|sent - RING)[^;]*; [^;]*; \+\+\w+\)\s*"
                            r"(?:if \(!)?mbar_wait_brief\(&\w*full\[", body)
         assert copies, f"{name}: {kernel} leaves with copies in flight"
+
+
+@pytest.mark.parametrize("name", ["gemm_int8.cu", "attention_int8.cu", "attention_int8_prompt.cu"])
+def test_a_warp_that_gives_up_leaves_nobody_at_a_barrier(name):
+    """A named barrier has no limit: a warp that leaves after a wait that ran out arrives at those at which others may wait."""
+    for kernel, body in _limited(name):
+        for barrier in set(re.findall(r"bar\.sync (\d+),", body)):
+            given_up = [body[slice(*_braced(body, m.end()))] for m in re.finditer(r"if \(!ok\) (?=\{)", body)]
+            assert any(f"bar.arrive {barrier}," in x for x in given_up), f"{name}: {kernel}, barrier {barrier}"
