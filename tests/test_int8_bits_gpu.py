@@ -63,8 +63,8 @@ def test_a_portion_attends_the_same_at_any_number_of_keys():
         want = ops.paged_attention(q, cache, own, 0.1)
         assert torch.equal(ops.paged_attention(q, cache, bucket, 0.1), want), (n, keys)
         exact, _, _ = case.attention(q, [n], 0.1, kv_lens=[keys])
-        # float16 probabilities and values: 2^-12 each and 2^-12 again for the value's scale, the output 2^-9, of each of many
-        # terms of one size and either sign; four times their root mean square, 2^-8
+        # the output's rounding to bfloat16: 2^-8 of an element at most, 0.0017 in the root mean square; of 128 elements, with
+        # the roundings to float16 in front of it, well below 2^-8
         off = (want.double() - exact).norm(dim=-1) / exact.norm(dim=-1)
         assert off.max() < 2.0 ** -8
         part = ops.paged_attention(q[n // 2:].contiguous(), cache, case.meta([n - n // 2], [keys]), 0.1)
@@ -113,8 +113,25 @@ def test_a_prompt_with_moving_value_scales_attends_the_same_in_any_step(window, 
     for n in (200, 131, 33, 2):
         assert torch.equal(ops.paged_attention(q[300 - n:300].contiguous(), cache, alone.meta([n]), 0.1, window), whole[300 - n:300])
     exact, _, _ = alone.attention(q[:300], [300], 0.1, window)
-    # (of a row's norm, as above)
+    # (as above)
     assert ((whole[:300].double() - exact).norm(dim=-1) <= 2.0 ** -8 * exact.norm(dim=-1)).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hq,hkv,d", [(16, 8, 128), (4, 2, 64), (6, 2, 128), (8, 1, 128)])
+@pytest.mark.parametrize("window", [None, 100])
+def test_drafted_tokens_attend_the_same_in_any_step(hq, hkv, d, window, dtype):
+    """Steps whose tiles have 4 to 32 rows, by their longest draft."""
+    case = Int8Case([900, 333, 1500, 40, 700, 513], hkv, d, 16, seed=6)
+    cache = ops.Int8Cache(case.data, case.scales)
+    for q_lens in ([1, 1, 2, 2, 3, 1], [1, 2, 4, 3, 2, 5], [1, 1, 8, 2, 16, 3], [2, 1, 5, 20, 2, 2]):
+        q = _rand(sum(q_lens), hq, d, seed=7, dtype=dtype)
+        whole = ops.int8_paged_attention(q, cache, case.meta(q_lens), 0.1, window)
+        at = 0
+        for s, n in enumerate(q_lens):
+            got = ops.int8_paged_attention(q[at:at + n].contiguous(), cache, _alone(case, s).meta([n]), 0.1, window)
+            assert torch.equal(got, whole[at:at + n]), (q_lens, s)
+            at += n
 
 
 def _with_scales(case, s, keys, kv, scale):
