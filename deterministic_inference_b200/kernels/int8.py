@@ -527,6 +527,9 @@ def _parts(meta, group: int, hkv: int, wide: bool, window: int, portions: bool, 
     parts = meta.scratch.get(key)
     if parts is None:
         q_lens, kv_lens = meta.q_lens, meta.kv_lens
+        if not len(q_lens) == len(kv_lens) <= meta.block_table.shape[0]:
+            raise _ops().KernelError(f"int8_paged_attention: {len(q_lens)} q_lens and {len(kv_lens)} kv_lens for a block table "
+                                     f"of {meta.block_table.shape[0]} sequences")
         one = [s for s, n in enumerate(q_lens) if n == 1]
         more = [s for s, n in enumerate(q_lens) if n > 1]
         many = [s for s in more if not wide and (portions or q_lens[s] * group > PROMPT_ROWS) and group <= 128]

@@ -61,3 +61,12 @@ def test_pages_that_are_none_of_the_pools_in_the_form_for_every_shape(hkv, d, pa
         meta = case.meta([q_len] * 2)
         meta.block_table[0, 2] = entry
         assert torch.equal(ops.int8_paged_attention(q, ops.Int8Cache(case.data, case.scales), meta, 0.1), want)
+
+
+def test_lengths_of_more_sequences_than_there_are_tables():
+    case = Int8Case([200, 100], 2, 64, 16, seed=5)
+    q, cache = _rand(2, 4, 64), ops.Int8Cache(case.data, case.scales)
+    for q_lens, kv_lens in (([1, 1, 1], [200, 100, 100]), ([1, 1], [200]), ([1], [200, 100])):
+        meta = case.meta([1, 1])
+        meta.q_lens, meta.kv_lens = q_lens, kv_lens
+        _refused(lambda: ops.int8_paged_attention(q, cache, meta, 0.1), "block table")
