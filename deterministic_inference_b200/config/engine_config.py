@@ -26,7 +26,9 @@ class EngineConfig:
     # "int8": the layers' matrices in 8 bits with a scale per output channel, activations quantised
     # per token in front of every product, whose sums are exact integers (embedding and head stay in
     # ``dtype``).  "int8" for the cache: keys and values in 8 bits with a scale per token and head;
-    # half the memory and half of what a decode step reads.  None: ``dtype``.
+    # half the memory, and half of the cached bytes that a decode step reads.  None: ``dtype``.  (A
+    # decode step of qwen3_8b, 8 / 64 requests of 2,100 tokens: 3.92 / 7.73 ms in bfloat16, with 8-bit
+    # weights 3.34 / 6.74, cache 3.99 / 6.92, both 2.97 / 5.26.)
     weight_dtype: Optional[str] = None
     cache_dtype: Optional[str] = None
 

@@ -4,8 +4,8 @@
 // kc, vc the codes of a key and a value, ks, vs their scales.  The scales never touch the codes: a key's joins its score,
 // a value's the probability.  A row that sees no key is zeros.  A sequence's new tokens are its last ones.
 //
-// Forms: split (one to a few new tokens, and every float32 portion: the cache is streamed once), one for every shape (heads
-// above 128, pages that are not a power of two), and attention_int8_prompt.cu for bfloat16 portions of many rows.
+// Forms: split (one new token, a few drafted ones, and every float32 portion: the cache is streamed once), one for every shape
+// (heads above 128, pages that are not a power of two), and attention_int8_prompt.cu for bfloat16 portions of prompts.
 #include <cuda.h>
 
 #include "common.cuh"
@@ -44,8 +44,9 @@ __device__ __forceinline__ float fast_exp2(float x) {
 //   O^T = V^T P^T: A = the values' tile read MN-major (128 dimensions), B = the weights w = p vs, p = 2^(s - L), as
 //     integers against the tile's largest one of the row, again PARTS bytes each (MN-major, a thread writes its key's).
 //     Lane d holds dimension d's integers for all rows.
-// An integer of 15 (28) bits against the largest weight of 128 keys: what the others lose is 2^-16 (2^-29) of it each at
-// most, 0.2 % of a tile's sum in the worst case and 2^-9 of a weight that matters, like a bfloat16 probability's.  The
+// The largest weight of 128 keys becomes an integer between 2^13 and 2^14 (2^27 and 2^28): each is off by 2^-14 (2^-28) of it at
+// most, 0.8 % of a tile's sum if all erred alike, in either sense 2^-10 of one in which many matter.  A query's elements are off by
+// 2^-15 of the row's largest, which is more than bfloat16's own step for those below 2^-7 of it.  The
 // integers are then scaled and added up in float32.  L, the reference of a row's probabilities, follows the tiles'
 // largest weights and is raised only when they have left it by 2^20: float32 holds what lies between.
 //
@@ -53,16 +54,16 @@ __device__ __forceinline__ float fast_exp2(float x) {
 // and ROWS rows: some 20 instructions a key and row, a quarter of what mma.sync on converted codes takes.  Three CTAs an SM
 // (two above 8 rows), each with a tile on its way and one in use, cover the trips between copy, tensor core and threads.  An
 // item's beginning and end cost as much as a tile or two, through instructions that are not in the cache any more: they are
-// kept few.  Heads of 128, 8 kv heads: 64 requests of up to 4,096 keys, 4 rows each, 67.5 us (312 MB at 4.6 TB/s); four of
-// 32,000, 8 rows, 58.9 us (270 MB at 4.6 TB/s), of which the last CTA is 7 us behind the median and the merge takes 6; sixteen of up to 1,500
-// with 10 rows 25.1 us (31 MB), with 20 rows at 4,096 keys 75 us (tiles of 24 rows; 104 us in tiles of 32); one of 2,048, 8.7 us.
+// kept few.  Heads of 128, 8 kv heads: 64 requests of up to 4,096 keys, 4 rows each, 67.3 us (312 MB at 4.6 TB/s); four of
+// 32,000, 8 rows, 58.7 us (270 MB at 4.6 TB/s), of which the last CTA is 7 us behind the median and the merge takes 6; sixteen of up to 1,500
+// with 10 rows 26.0 us (31 MB), with 20 rows at 4,096 keys 73 us (tiles of 24 rows; 104 us in tiles of 32); one of 2,048, 8.8 us.
 //
 // Roles in a CTA: warps 0-3 softmax (TMEM lane = key, dimension), warp 4 copies (TMA, a box a page; scales by cp.async),
 // warp 5 issues the scores' products, warp 7 the outputs', warp 6 finds the next work items and makes their query rows.
 // Registers are handed out to groups of four warps: the second group gives a part of its own to the first (setmaxnreg).
 // Work items: (sequence, kv head, tile of rows,
 // run of keys), a CTA takes a contiguous range of them.  The length of a run follows from the sequence's own lengths, so a
-// row's bits do not depend on the rest of the step.
+// row's bits do not depend on the rest of the step (those of a float32 portion do on its own rows: where its prompt was cut).
 constexpr int SP_TILE = 128, SP_THREADS = 256, SP_STAGES = 2, SP_ITEMS = 4;
 constexpr int SP_COPY_WARP = 4, SP_SCORE_WARP = 5, SP_OUTPUT_WARP = 7;      // and 6: items and query rows
 
@@ -942,7 +943,8 @@ attention_split_merge_kernel(T* __restrict__ out, const __grid_constant__ SplitA
 
 // ---------------------------------------------------------------- the form for every shape
 // Head sizes up to 256, any page size and group ratio: a warp takes a (token, head), a lane a key of 32 at a time for
-// the scores, then a lane D / 32 dimensions for the values.
+// the scores, then a lane D / 32 dimensions for the values.  Bound by a warp's chain over the keys: 2,048 keys of heads of 256
+// 1.3 ms, for one request as for sixteen.
 constexpr int ANY_WARPS = 4;
 
 template <typename T>

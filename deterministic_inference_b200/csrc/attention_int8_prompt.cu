@@ -1,5 +1,5 @@
 // Attention of a prompt's portion over a paged cache in 8-bit integers (cache_int8.cu; formulas in attention_int8.cu), for
-// bfloat16 queries and many rows: S = Q K^T and O = P V by tcgen05.mma kind::f16, accumulators in tensor memory, a thread a
+// bfloat16 queries, whatever a portion's rows (and drafted tokens of many): S = Q K^T and O = P V by tcgen05.mma kind::f16, accumulators in tensor memory, a thread a
 // query row for the softmax.
 //
 // Numbers.  Keys enter the first product as their codes, which float16 holds exactly, queries in float16 times a power of
@@ -32,7 +32,7 @@
 // products; the schedulers are shared with the conversion, and with the instruction cache: what a warp runs seldom is kept
 // short or out of the way.  A CTA's beginning and end cost 9 us more.  One CTA an SM (213 KB).  Two threads a row were
 // slower (635 -> 852 us: registers spilled), as were exponentials shared with the FMA pipe (506 -> 518).
-// 2,048 tokens, 32 / 8 heads of 128: 56.7 us, 606 TFLOP/s.  3,000 tokens on 4,096 keys: 455 us.
+// 2,048 tokens, 32 / 8 heads of 128: 56.4 us, 610 TFLOP/s.  3,000 tokens on 5,000 keys beside 24 decodes: 471 us.
 #include <cuda.h>
 #include <cuda_fp16.h>
 
