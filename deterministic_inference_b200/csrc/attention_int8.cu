@@ -45,7 +45,7 @@ __device__ __forceinline__ float fast_exp2(float x) {
 //     integers against the tile's largest one of the row, again PARTS bytes each (MN-major, a thread writes its key's).
 //     Lane d holds dimension d's integers for all rows.
 // The largest weight of 128 keys becomes an integer between 2^13 and 2^14 (2^27 and 2^28): each is off by 2^-14 (2^-28) of it at
-// most, 0.8 % of a tile's sum if all erred alike, in either sense 2^-10 of one in which many matter.  A query's elements are off by
+// most, 0.8 % of a tile's sum if all erred alike; errors of either sign in a sum of many that matter are 2^-10 of it.  A query's elements are off by
 // 2^-15 of the row's largest, which is more than bfloat16's own step for those below 2^-7 of it.  The
 // integers are then scaled and added up in float32.  L, the reference of a row's probabilities, follows the tiles'
 // largest weights and is raised only when they have left it by 2^20: float32 holds what lies between.

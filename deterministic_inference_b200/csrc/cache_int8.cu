@@ -377,9 +377,8 @@ qk_norm_rope_cache_int8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out,
 template <typename T, int VECTORS, int THREADS>
 __global__ void __launch_bounds__(THREADS)
 quantize_rows_kernel(const T* __restrict__ x, long long stride, signed char* __restrict__ codes,
-                     float* __restrict__ scales, int K, int Kp, int early) {
-  if (early) pdl_trigger();
-  pdl_wait(x);
+                     float* __restrict__ scales, int K, int Kp) {
+  pdl_prologue(x);
   __shared__ unsigned tops[THREADS / 32];
   const long long row = blockIdx.x;
   const T* src = x + row * stride;
@@ -457,8 +456,7 @@ int launch_read(const signed char* data, const float* scales, const int* slots, 
 }
 
 template <typename T>
-int launch_rows(const void* x, long long stride, void* codes, void* scales, long long M, int K, int Kp, int early,
-                cudaStream_t st) {
+int launch_rows(const void* x, long long stride, void* codes, void* scales, long long M, int K, int Kp, cudaStream_t st) {
   const T* p = reinterpret_cast<const T*>(x);
   signed char* c = reinterpret_cast<signed char*>(codes);
   float* s = reinterpret_cast<float*>(scales);
@@ -473,7 +471,7 @@ int launch_rows(const void* x, long long stride, void* codes, void* scales, long
     kern = need <= 4 ? quantize_rows_kernel<T, 4, 512> : quantize_rows_kernel<T, 8, 512>;
     wide = true;
   }
-  dib_launch(kern, dim3((unsigned)M), dim3(wide ? 512 : 256), 0, st, p, stride, c, s, K, Kp, early);
+  dib_launch(kern, dim3((unsigned)M), dim3(wide ? 512 : 256), 0, st, p, stride, c, s, K, Kp);
   DIB_CHECK_LAUNCH();
   return DIB_OK;
 }
@@ -553,17 +551,15 @@ int dib_int8_cache_read(const void* data, const void* scales, const void* slots,
 }
 
 // codes int8 [M, Kp] (Kp = K rounded up to 16, zeros behind K) and scales [M] of x [M, K], rows `stride` values apart.
-// early: the kernel that follows may set itself up beside this one; 0 for a weight, which products read ahead of their
-// wait for the kernel in front of them.
 int dib_quantize_rows(const void* x, long long stride, void* codes, void* scales, long long M, int K, int dtype,
-                      int early, cudaStream_t st) {
+                      cudaStream_t st) {
   if (dtype != 0 && dtype != 1) return DIB_BAD_DTYPE;
   if (M < 0 || M > 0x7fffffffll || K < 1 || K > (1 << 30)) return DIB_BAD_SIZE;
   if ((reinterpret_cast<uintptr_t>(codes) & 15) != 0) return DIB_BAD_ALIGN;
   if (M == 0) return DIB_OK;
   const int Kp = (K + 15) / 16 * 16;
-  if (dtype == 1) return launch_rows<__nv_bfloat16>(x, stride, codes, scales, M, K, Kp, early, st);
-  return launch_rows<float>(x, stride, codes, scales, M, K, Kp, early, st);
+  if (dtype == 1) return launch_rows<__nv_bfloat16>(x, stride, codes, scales, M, K, Kp, st);
+  return launch_rows<float>(x, stride, codes, scales, M, K, Kp, st);
 }
 
 }  // extern "C"

@@ -913,12 +913,12 @@ int dib_gemm_int8(const void* x, const void* sx, const void* w, const void* sw, 
 // The same with x [M, K] of values (x_dtype 0 float32, 1 bfloat16; rows `stride` values apart), which `quantize`
 // (dib_quantize_rows of the cache's library) first turns into codes and scales in `work` (M Kp + 4 M bytes, the scales
 // behind the codes).
-int dib_int8_linear(int (*quantize)(const void*, long long, void*, void*, long long, int, int, int, cudaStream_t),
+int dib_int8_linear(int (*quantize)(const void*, long long, void*, void*, long long, int, int, cudaStream_t),
                     const void* x, long long stride, int x_dtype, int K, void* work, const void* w, const void* sw, void* out,
                     int M, int N, int out_dtype, int sm_count, cudaStream_t st) {
   const int Kp = (K + 15) / 16 * 16;
   void* scales = reinterpret_cast<char*>(work) + (long long)M * Kp;
-  const int rc = quantize(x, stride, work, scales, M, K, x_dtype, 1, st);
+  const int rc = quantize(x, stride, work, scales, M, K, x_dtype, st);
   if (rc != DIB_OK) return rc;
   return dib_gemm_int8(work, scales, w, sw, out, M, N, Kp, out_dtype, sm_count, st);
 }

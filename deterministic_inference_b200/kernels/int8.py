@@ -33,7 +33,7 @@ MAX_HEAD_DIM = 256
 # is looked at in one expression, and the check that words the error runs only where that fails.
 _P, _I, _L, _F = c_void_p, c_int, c_longlong, c_float
 _SIGNATURES = {
-    "dib_quantize_rows": ("cache_int8", (_P, _L, _P, _P, _L, _I, _I, _I, _P)),
+    "dib_quantize_rows": ("cache_int8", (_P, _L, _P, _P, _L, _I, _I, _P)),
     "dib_int8_cache_write": ("cache_int8", (_P, _P, _L, _L, _P, _P, _P, _I, _I, _I, _I, _L, _I, _P)),
     "dib_int8_cache_read": ("cache_int8", (_P, _P, _P, _P, _P, _I, _I, _I, _I, _L, _I, _P)),
     "dib_int8_qk_norm_rope_cache": ("cache_int8", (_P, _P, _P, _P, _P, _P, _F, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _L, _I, _P)),
@@ -159,22 +159,23 @@ class Int8Weight:
             raise ops.KernelError(f"Int8Weight: codes {tuple(codes.shape)}, scales {tuple(scales.shape)} "
                                   f"(K from 1 to {MAX_K})")
         _same_device("Int8Weight", codes, scales)
-        self.k = k
         if _padded(k) != k or codes.data_ptr() % 16:
             padded = torch.zeros(n, _padded(k), dtype=torch.int8, device=codes.device)
             padded[:, :k] = codes
             codes = padded
-        # The copy stands between a kernel of this package that may have made the codes (``quantize_rows``), and that lets the
-        # next one start beside it, and a product, which reads its weight ahead of its wait: a copy waits for all of it.
-        self.codes, self.scales = codes, scales.clone()
+        self._set(codes, scales, k)
 
     @classmethod
     def of(cls, weight: torch.Tensor) -> "Int8Weight":
         """Quantises a float32 or bfloat16 weight [N, K]."""
-        rows = _quantize(weight, "weight", early=False)
-        out = cls.__new__(cls)
-        out.codes, out.scales, out.k = rows.codes, rows.scales, rows.k
-        return out
+        rows = _quantize(weight, "weight")
+        return cls.__new__(cls)._set(rows.codes, rows.scales, rows.k)
+
+    def _set(self, codes, scales, k) -> "Int8Weight":
+        # The copy stands between the kernel of this package that may have made the codes, which lets the next one start beside
+        # it, and a product, which reads its weight ahead of its wait for the kernel in front: a copy waits for all of it.
+        self.codes, self.scales, self.k = codes, scales.clone(), k
+        return self
 
     @property
     def shape(self):
@@ -201,20 +202,19 @@ def _check_rows(x, name: str) -> int:
     return _code(x.dtype, name)
 
 
-def _quantize(x: torch.Tensor, name: str, early: bool) -> Int8Rows:
+def _quantize(x: torch.Tensor, name: str) -> Int8Rows:
     code = _check_rows(x, name)
     m, k = x.shape
     codes = torch.empty(m, _padded(k), dtype=torch.int8, device=x.device)
     scales = torch.empty(m, dtype=torch.float32, device=x.device)
-    st = _fn("dib_quantize_rows")(x.data_ptr(), x.stride(0), codes.data_ptr(), scales.data_ptr(), m, k, code,
-                                  1 if early else 0, _stream())
+    st = _fn("dib_quantize_rows")(x.data_ptr(), x.stride(0), codes.data_ptr(), scales.data_ptr(), m, k, code, _stream())
     _done(st, "quantize_rows", lambda: f"rows {m} x {k}")
     return Int8Rows.__new__(Int8Rows)._set(codes, scales, k, x.dtype)
 
 
 def quantize_rows(x) -> Int8Rows:
     """Rows [M, K] (float32 or bfloat16, any distance between rows; or the partial sums of a product) in 8 bits."""
-    return _quantize(_ops().as_tensor(x), "x", early=True)
+    return _quantize(_ops().as_tensor(x), "x")
 
 
 def int8_linear(x, weight: Int8Weight, out_dtype=None) -> torch.Tensor:

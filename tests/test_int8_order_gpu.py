@@ -82,3 +82,19 @@ def test_a_weight_made_of_rows_that_are_still_being_quantised(m, n, k):
         del rows, weight
         assert torch.equal(y, want[i & 1]), f"pass {i}"
     ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("m,n,k", [(4, 4096, 4096), (40, 8192, 2048), (700, 2048, 4096)])
+def test_a_weight_used_as_soon_as_it_is_quantised(m, n, k):
+    x = ops.quantize_rows(_rand(m, k, seed=1, dtype=BF16))
+    sources = [_rand(n, k, seed=s, dtype=BF16) for s in (2, 3)]
+    want = []
+    for w in sources:
+        weight = ops.Int8Weight.of(w)
+        torch.cuda.synchronize()
+        want.append(ops.int8_linear(x, weight))
+    del weight
+    for i in range(30):
+        y = ops.int8_linear(x, ops.Int8Weight.of(sources[i & 1]))
+        assert torch.equal(y, want[i & 1]), f"pass {i}"
+    ops.check_kernel_status()
