@@ -1,0 +1,251 @@
+// Rows of a matrix in 4-bit floating point (fp4.cuh has the rule): quantising activations and weights, laying out codes that were
+// made elsewhere, and reading rows back.
+//
+// Kept: codes [M, Kp / 2] (two a byte, the first in the low half; Kp = K rounded up to 32, zeros behind K), block scales in
+// tiles (fp4_scale_at; zeros behind K), units float32 [M] = 2^E.
+//
+// A thread has a block of 16 values: its largest is the thread's own, its scale a byte, its codes 8 bytes.  Bound by memory.
+#include "fp4.cuh"
+
+namespace {
+
+// 16 values of a row from `at` on, zeros behind K; kept as they came (bfloat16 two a word).
+template <typename T> struct Block16 {
+  static constexpr int WORDS = 16 * (int)sizeof(T) / 4;
+  unsigned w[WORDS];
+  template <bool WIDE> __device__ __forceinline__ void load(const T* row, int at, int K) {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = 0;
+    if (at >= K) return;
+    if (WIDE) {      // rows on 32 bytes, K a multiple of 16
+#pragma unroll
+      for (int i = 0; i < WORDS / 8; ++i)
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(w[8 * i]), "=r"(w[8 * i + 1]), "=r"(w[8 * i + 2]), "=r"(w[8 * i + 3]), "=r"(w[8 * i + 4]),
+                       "=r"(w[8 * i + 5]), "=r"(w[8 * i + 6]), "=r"(w[8 * i + 7])
+                     : "l"(reinterpret_cast<const char*>(row + at) + 32 * i));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (at + e < K) {
+          if (sizeof(T) == 4) w[e % WORDS] = __float_as_uint(Elem<T>::load(row + at + e));
+          else w[e >> 1] |= (unsigned)*reinterpret_cast<const unsigned short*>(row + at + e) << (16 * (e & 1));
+        }
+    }
+  }
+  __device__ __forceinline__ float get(int e) const {
+    if (sizeof(T) == 4) return __uint_as_float(w[e % WORDS]);
+    return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+  }
+  __device__ __forceinline__ unsigned top() const {
+    unsigned t = 0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) t = max(t, fp4_magnitude(get(e)));
+    return t;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void write_block(const Block16<T>& x, unsigned top, float down, unsigned char* codes, unsigned char* tiles,
+                                            long long row, int block, int Kp, int k_tiles) {
+  const unsigned scale = fp4_block_scale(top, down);
+  const Fp4Scaler s = fp4_scaler(scale, down);
+  float v[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) v[e] = x.get(e);
+  if (block * 16 < Kp)
+    *reinterpret_cast<uint2*>(codes + row * (Kp / 2) + block * 8) = make_uint2(fp4_codes8(v, s), fp4_codes8(v + 8, s));
+  tiles[fp4_scale_at(row, block, k_tiles)] = (unsigned char)scale;
+}
+
+// A block of threads a row.  BLOCKS > 0: each thread keeps that many blocks of 16 in registers; 0: the row is read twice.
+template <typename T, int BLOCKS, bool WIDE>
+__global__ void __launch_bounds__(512)
+quantize_rows_kernel(const T* __restrict__ x, long long stride, unsigned char* __restrict__ codes, unsigned char* __restrict__ tiles,
+                     float* __restrict__ units, int K, int Kp, int k_tiles) {
+  pdl_prologue(x);
+  __shared__ unsigned tops[16];
+  const long long row = blockIdx.x;
+  const T* src = x + row * stride;
+  const int blocks = k_tiles * 4;
+  constexpr int KEPT = BLOCKS > 0 ? BLOCKS : 1;
+  Block16<T> v[KEPT];
+  unsigned own[KEPT], top = 0;
+  if (BLOCKS > 0) {
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) v[i].template load<WIDE>(src, (i * blockDim.x + threadIdx.x) * 16, K);
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) {
+      own[i] = v[i].top();
+      top = max(top, own[i]);
+    }
+  } else {
+    for (int b = threadIdx.x; b < blocks; b += blockDim.x) {
+      v[0].template load<WIDE>(src, b * 16, K);
+      top = max(top, v[0].top());
+    }
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+  for (int w = 0; w < (int)blockDim.x / 32; ++w) top = max(top, tops[w]);
+  const unsigned exponent = fp4_row_exponent(top);
+  const float down = fp4_down(exponent);
+  if (threadIdx.x == 0) units[row] = fp4_unit(exponent);
+  if (BLOCKS > 0) {
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) {
+      const int b = i * blockDim.x + threadIdx.x;
+      if (b < blocks) write_block(v[i], own[i], down, codes, tiles, row, b, Kp, k_tiles);
+    }
+  } else {
+    for (int b = threadIdx.x; b < blocks; b += blockDim.x) {
+      v[0].template load<WIDE>(src, b * 16, K);
+      write_block(v[0], v[0].top(), down, codes, tiles, row, b, Kp, k_tiles);
+    }
+  }
+}
+
+template <typename T>
+int launch_rows(const void* x, long long stride, void* codes, void* tiles, void* units, long long M, int K, cudaStream_t st) {
+  const int Kp = (K + 31) / 32 * 32, k_tiles = fp4_k_tiles(K), blocks = k_tiles * 4;
+  const bool wide = K % 16 == 0 && (stride * sizeof(T)) % 32 == 0 && reinterpret_cast<uintptr_t>(x) % 32 == 0;
+  const int per = blocks <= 512 ? 1 : blocks <= 1024 ? 2 : blocks <= 2048 ? 4 : 0;
+  const int threads = per == 0 ? 512 : ((blocks + per - 1) / per + 31) / 32 * 32;
+  auto kern = per == 1 ? (wide ? quantize_rows_kernel<T, 1, true> : quantize_rows_kernel<T, 1, false>)
+              : per == 2 ? (wide ? quantize_rows_kernel<T, 2, true> : quantize_rows_kernel<T, 2, false>)
+              : per == 4 ? (wide ? quantize_rows_kernel<T, 4, true> : quantize_rows_kernel<T, 4, false>)
+                         : (wide ? quantize_rows_kernel<T, 0, true> : quantize_rows_kernel<T, 0, false>);
+  dib_launch(kern, dim3((unsigned)M), dim3(threads), 0, st, reinterpret_cast<const T*>(x), stride,
+             reinterpret_cast<unsigned char*>(codes), reinterpret_cast<unsigned char*>(tiles), reinterpret_cast<float*>(units), K, Kp,
+             k_tiles);
+  DIB_CHECK_LAUNCH();
+  return DIB_OK;
+}
+
+// A thread a block of 16: out[row, 16 b ..] = codes * scale * unit.
+constexpr int READ_THREADS = 256;
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(READ_THREADS)
+read_rows_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ tiles, const float* __restrict__ units,
+                 T* __restrict__ out, long long M, int K, int Kp, int k_tiles, int blocks) {
+  pdl_prologue(codes, tiles, units);
+  const long long i = (long long)blockIdx.x * READ_THREADS + threadIdx.x;
+  const long long row = i / blocks;
+  const int b = (int)(i - row * blocks);
+  if (row >= M) return;
+  const uint2 w = *reinterpret_cast<const uint2*>(codes + row * (Kp / 2) + b * 8);
+  const float scale = fp4_scale_value(tiles[fp4_scale_at(row, b, k_tiles)]), unit = units[row];
+  float x[16];
+  fp4_values8(w.x, scale, x);
+  fp4_values8(w.y, scale, x + 8);
+  T* dst = out + row * K + b * 16;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] *= unit;
+  if (WIDE) {
+    unsigned y[16];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (sizeof(T) == 4) {
+        y[2 * e] = __float_as_uint(x[2 * e]);
+        y[2 * e + 1] = __float_as_uint(x[2 * e + 1]);
+      } else {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+        y[e] = *reinterpret_cast<const unsigned*>(&p);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < (int)sizeof(T) / 2; ++h)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<char*>(dst) + 32 * h),
+                   "r"(y[8 * h]), "r"(y[8 * h + 1]), "r"(y[8 * h + 2]), "r"(y[8 * h + 3]), "r"(y[8 * h + 4]), "r"(y[8 * h + 5]),
+                   "r"(y[8 * h + 6]), "r"(y[8 * h + 7])
+                   : "memory");
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (b * 16 + e < K) Elem<T>::store(dst + e, x[e]);
+  }
+}
+
+template <typename T>
+int launch_read(const void* codes, const void* tiles, const void* units, void* out, long long M, int K, cudaStream_t st) {
+  const int blocks = (K + 15) / 16;
+  const long long grid = (M * blocks + READ_THREADS - 1) / READ_THREADS;
+  if (grid > 0x7fffffffll) return DIB_BAD_SIZE;
+  const bool wide = K % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 32 == 0;
+  dib_launch(wide ? read_rows_kernel<T, true> : read_rows_kernel<T, false>, dim3((unsigned)grid), dim3(READ_THREADS), 0, st,
+             reinterpret_cast<const unsigned char*>(codes), reinterpret_cast<const unsigned char*>(tiles),
+             reinterpret_cast<const float*>(units), reinterpret_cast<T*>(out), M, K, (K + 31) / 32 * 32, fp4_k_tiles(K), blocks);
+  DIB_CHECK_LAUNCH();
+  return DIB_OK;
+}
+
+// Codes, block scales and exponent bytes as rows [M, code_bytes], [M, scale_bytes], [M] -> the layout above.  A thread a block
+// of 16.  (Codes behind K are dropped, a scale's sign is: a block scale is not negative.)
+__global__ void __launch_bounds__(READ_THREADS)
+layout_rows_kernel(const unsigned char* __restrict__ in_codes, const unsigned char* __restrict__ in_scales,
+                   const unsigned char* __restrict__ in_exponents, unsigned char* __restrict__ codes, unsigned char* __restrict__ tiles,
+                   float* __restrict__ units, long long M, int K, int Kp, int k_tiles) {
+  pdl_prologue(in_codes, in_scales, in_exponents);
+  const int blocks = k_tiles * 4, code_bytes = (K + 1) / 2, scale_bytes = (K + 15) / 16;
+  const long long i = (long long)blockIdx.x * READ_THREADS + threadIdx.x;
+  const long long row = i / blocks;
+  const int b = (int)(i - row * blocks);
+  if (row >= M) return;
+  if (b * 16 < Kp) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int at = b * 8 + j;
+      unsigned c = at < code_bytes ? in_codes[row * code_bytes + at] : 0;
+      if (2 * at + 1 >= K) c &= 15;
+      codes[row * (Kp / 2) + at] = (unsigned char)c;
+    }
+  }
+  tiles[fp4_scale_at(row, b, k_tiles)] = b < scale_bytes ? in_scales[row * scale_bytes + b] & 127 : 0;
+  if (b == 0) units[row] = fp4_unit(in_exponents[row]);
+}
+
+}  // namespace
+
+extern "C" {
+
+// codes [M, Kp / 2], tiles [ceil(M / 128), fp4_k_tiles(K), 512], units float32 [M] of x [M, K] (dtype 0 float32, 1 bfloat16),
+// rows `stride` values apart.
+int dib_fp4_quantize_rows(const void* x, long long stride, void* codes, void* tiles, void* units, long long M, int K, int dtype,
+                          cudaStream_t st) {
+  if (dtype != 0 && dtype != 1) return DIB_BAD_DTYPE;
+  if (M < 0 || M > 0x7fffffffll || K < 1 || K > (1 << 30)) return DIB_BAD_SIZE;
+  if (((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(tiles)) & 15) != 0) return DIB_BAD_ALIGN;
+  if (M == 0) return DIB_OK;
+  if (dtype == 1) return launch_rows<__nv_bfloat16>(x, stride, codes, tiles, units, M, K, st);
+  return launch_rows<float>(x, stride, codes, tiles, units, M, K, st);
+}
+
+// out [M, K] (dtype 0 float32, 1 bfloat16): what the rows stand for.
+int dib_fp4_read_rows(const void* codes, const void* tiles, const void* units, void* out, long long M, int K, int dtype,
+                      cudaStream_t st) {
+  if (dtype != 0 && dtype != 1) return DIB_BAD_DTYPE;
+  if (M < 0 || K < 1 || K > (1 << 30)) return DIB_BAD_SIZE;
+  if ((reinterpret_cast<uintptr_t>(codes) & 15) != 0) return DIB_BAD_ALIGN;
+  if (M == 0) return DIB_OK;
+  if (dtype == 1) return launch_read<__nv_bfloat16>(codes, tiles, units, out, M, K, st);
+  return launch_read<float>(codes, tiles, units, out, M, K, st);
+}
+
+// The layout of rows that were quantised elsewhere: in_codes [M, ceil(K / 2)], in_scales [M, ceil(K / 16)] (e4m3), in_exponents [M].
+int dib_fp4_layout_rows(const void* in_codes, const void* in_scales, const void* in_exponents, void* codes, void* tiles, void* units,
+                        long long M, int K, cudaStream_t st) {
+  if (M < 0 || K < 1 || K > (1 << 30)) return DIB_BAD_SIZE;
+  if (M == 0) return DIB_OK;
+  const int k_tiles = fp4_k_tiles(K);
+  const long long grid = (M * k_tiles * 4 + READ_THREADS - 1) / READ_THREADS;
+  if (grid > 0x7fffffffll) return DIB_BAD_SIZE;
+  dib_launch(layout_rows_kernel, dim3((unsigned)grid), dim3(READ_THREADS), 0, st, reinterpret_cast<const unsigned char*>(in_codes),
+             reinterpret_cast<const unsigned char*>(in_scales), reinterpret_cast<const unsigned char*>(in_exponents),
+             reinterpret_cast<unsigned char*>(codes), reinterpret_cast<unsigned char*>(tiles), reinterpret_cast<float*>(units), M, K,
+             (K + 31) / 32 * 32, k_tiles);
+  DIB_CHECK_LAUNCH();
+  return DIB_OK;
+}
+
+}  // extern "C"

@@ -53,6 +53,8 @@ SOURCES = {
     "attention_int8": "attention_int8.cu",
     "attention_int8_prompt": "attention_int8_prompt.cu",
     "gemm_int8": "gemm_int8.cu",
+    "rows_fp4": "rows_fp4.cu",
+    "gemm_fp4": "gemm_fp4.cu",
 }
 HEADERS = ("common.cuh", "attention_merge.cuh")
 # further headers a library includes
@@ -69,6 +71,8 @@ EXTRA_HEADERS = {
     "routed_experts": ("source.cuh",),
     "retention": ("source.cuh", "sigmoid_attention_mma.cuh", "linear_chunks.cuh"),
     "gated_linear_attention": ("source.cuh", "sigmoid_attention_mma.cuh", "linear_chunks.cuh"),
+    "rows_fp4": ("fp4.cuh",),
+    "gemm_fp4": ("fp4.cuh",),
 }
 
 NVCC_FLAGS = [

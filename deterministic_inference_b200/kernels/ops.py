@@ -112,6 +112,7 @@ _STATUS_FUNCTIONS = {
     "attention_int8": ("dib_attention_int8_status", "dib_attention_int8_status_clear"),
     "attention_int8_prompt": ("dib_attention_int8_prompt_status", "dib_attention_int8_prompt_status_clear"),
     "gemm_int8": ("dib_gemm_int8_status", "dib_gemm_int8_status_clear"),
+    "gemm_fp4": ("dib_gemm_fp4_status", "dib_gemm_fp4_status_clear"),
 }
 _extra_status: dict = {}
 
@@ -2095,3 +2096,4 @@ def masked_attention(q: torch.Tensor, kv_cache: torch.Tensor, meta, scale: float
 
 from .int8 import (Int8Cache, Int8Rows, Int8Weight, int8_cache_read, int8_cache_write, int8_linear,  # noqa: E402,F401
                    int8_paged_attention, int8_qk_norm_rope_cache, quantize_rows)
+from .fp4 import Fp4Rows, Fp4Weight, fp4_linear, fp4_quantize_rows  # noqa: E402,F401
