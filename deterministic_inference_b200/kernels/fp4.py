@@ -250,9 +250,8 @@ def fp4_quantize_rows(x) -> Fp4Rows:
 
 def fp4_linear(x, weight: Fp4Weight, out_dtype=None) -> torch.Tensor:
     """y = x @ weight^T, [M, N]: ``x`` [M, K] is quantised row by row (or is an ``Fp4Rows``); the products of codes and block
-    scales are added up in float32, 64 values at a time in the order of k whatever the sizes, so a row's bits depend on the row
-    and the weight alone; times the two rows' powers of two, rounded once to ``out_dtype`` (float32 or bfloat16; x's type if
-    not given)."""
+    scales are added up in float32 in one order of k whatever the other sizes, so a row's bits depend on the row and the
+    weight alone; times the two rows' powers of two, rounded once to ``out_dtype`` (float32 or bfloat16; x's type if not given)."""
     if not isinstance(weight, Fp4Weight):
         raise _ops().KernelError("fp4_linear: weight must be an Fp4Weight")
     rows = isinstance(x, Fp4Rows)
@@ -287,5 +286,5 @@ def fp4_linear(x, weight: Fp4Weight, out_dtype=None) -> torch.Tensor:
 
 def force_product_form(form: int) -> None:
     """Measurement and test switch of the product: tiles of 128 x 64, 128 x 128 or 128 x 192 (0, 1, 2), the pair of CTAs (3),
-    whatever the sizes; -1: the library's own choice.  All give the same bits."""
+    clusters that share k (4, up to 128 rows), whatever the sizes; -1: the library's own choice.  All give the same bits."""
     _ops()._lib("gemm_fp4").dib_gemm_fp4_force_form(c_int(form))
