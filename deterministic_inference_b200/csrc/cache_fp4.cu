@@ -1,0 +1,338 @@
+// A paged cache of keys and values in 4-bit floating point (fp4.cuh has the rule; a row is a token's key or value of one head): writing
+// it, from keys and values or from the step's fused projection, and reading it back, by slots or as bfloat16 pages for the
+// prompt attention.
+//
+// Cache: data [pages, 2, Hkv, page_size, D / 2] (two codes a byte, the first in the low half), scales e4m3
+// [pages, 2, Hkv, page_size, D / 16], exponents [pages, 2, Hkv, page_size] (E + 127).  128 values take 73 bytes.
+//
+// A lane has a block of 16 values: 32 (64) bytes of the unquantised row, 8 bytes of codes, a scale.  Bound by memory.
+#include "cache_rows.cuh"
+#include "fp4.cuh"
+
+namespace {
+
+constexpr int CACHE_THREADS = 256;
+struct Cache4 {
+  unsigned char* data;
+  unsigned char* scales;
+  unsigned char* exponents;
+};
+
+// LANES: 8 for rows up to 128, 16 up to 256
+template <typename T, bool WIDE, int LANES>
+__global__ void __launch_bounds__(CACHE_THREADS)
+cache_write_kernel(const T* __restrict__ k, const T* __restrict__ v, long long k_stride, long long v_stride,
+                   const __grid_constant__ Cache4 cache, const int* __restrict__ slots, const __grid_constant__ CacheShape s) {
+  pdl_prologue(k, v, slots);
+  const int l = threadIdx.x & (LANES - 1);
+  const CacheRow c = cache_row(blockIdx.x * (CACHE_THREADS / LANES) + threadIdx.x / LANES, s, slots);
+  const T* src = (c.kv ? v + c.token * v_stride : k + c.token * k_stride) + c.h * s.D;
+  Block16<T> x;
+  x.template load<WIDE>(src, c.at >= 0 ? l * 16 : s.D, s.D);
+  const unsigned own = x.top();
+  unsigned top = own;
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (c.at < 0 || l * 16 >= s.D) return;
+  const unsigned exponent = fp4_row_exponent(top);
+  const float down = fp4_down(exponent);
+  const unsigned scale = fp4_block_scale(own, down);
+  const Fp4Scaler q = fp4_scaler(scale, down);
+  float y[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) y[e] = x.get(e);
+  *reinterpret_cast<uint2*>(cache.data + c.at * (s.D / 2) + l * 8) = make_uint2(fp4_codes8(y, q), fp4_codes8(y + 8, q));
+  cache.scales[c.at * (s.D / 16) + l] = (unsigned char)scale;
+  if (l == 0) cache.exponents[c.at] = (unsigned char)exponent;
+}
+
+// a block of 16 of the row at `at` as numbers; zeros for a row that is not there
+struct Held16 {
+  uint2 w;
+  unsigned scale, exponent;
+  __device__ __forceinline__ void load(const Cache4& cache, long long at, int l, int D) {
+    w = make_uint2(0, 0);
+    scale = exponent = 0;
+    if (at >= 0 && l * 16 < D) {
+      w = *reinterpret_cast<const uint2*>(cache.data + at * (D / 2) + l * 8);
+      scale = cache.scales[at * (D / 16) + l];
+      exponent = cache.exponents[at];
+    }
+  }
+  __device__ __forceinline__ void values(float (&x)[16]) const {
+    const float b = fp4_scale_value(scale), unit = fp4_unit(exponent);
+    fp4_values8(w.x, b, x);
+    fp4_values8(w.y, b, x + 8);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] *= unit;
+  }
+};
+
+// ROWS rows a group, all asked for before the first is used
+template <typename T, int LANES, int ROWS>
+__global__ void __launch_bounds__(CACHE_THREADS)
+cache_read_kernel(const __grid_constant__ Cache4 cache, const int* __restrict__ slots, T* __restrict__ k, T* __restrict__ v,
+                  const __grid_constant__ CacheShape s) {
+  constexpr int GROUPS = CACHE_THREADS / LANES;
+  Cache4 held = cache;
+  pdl_prologue(held.data, held.scales, held.exponents, slots);
+  const int l = threadIdx.x & (LANES - 1);
+  const unsigned r0 = blockIdx.x * (GROUPS * ROWS) + threadIdx.x / LANES;
+  CacheRow c[ROWS];
+  Held16 x[ROWS];
+#pragma unroll
+  for (int g = 0; g < ROWS; ++g) c[g] = cache_row(r0 + g * GROUPS, s, slots);
+#pragma unroll
+  for (int g = 0; g < ROWS; ++g) x[g].load(held, c[g].at, l, s.D);
+#pragma unroll
+  for (int g = 0; g < ROWS; ++g) {
+    if (r0 + g * GROUPS >= s.rows || l * 16 >= s.D) return;
+    float y[16];
+    x[g].values(y);
+    store16((c[g].kv ? v : k) + ((long long)c[g].token * s.Hkv + c[g].h) * s.D + l * 16, y);
+  }
+}
+
+// The step's fused projection rows [q heads | k heads | v heads]: q and k normed and rotated, q to its output, k and v rounded to T,
+// quantised and written to the token's slot.  A warp a (token, head), a lane 4 consecutive elements of 128 at a time: a block
+// of 16 is four lanes.
+constexpr int QKV_WARPS = 4;
+template <typename T>
+__global__ void __launch_bounds__(QKV_WARPS * 32)
+qk_norm_rope_cache_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const __grid_constant__ Cache4 cache,
+                          const float* __restrict__ q_norm_w, const float* __restrict__ k_norm_w, float eps,
+                          const float* __restrict__ cos_sin, int rotary_dim, int max_pos, const int* __restrict__ positions,
+                          const int* __restrict__ slots, int T_tokens, int Hq, int Hkv, int D, int page_size, long long num_pages) {
+  pdl_prologue(qkv, q_norm_w, k_norm_w);
+  __shared__ float row[QKV_WARPS][256];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = Hq + 2 * Hkv;
+  const long long item = (long long)blockIdx.x * QKV_WARPS + warp;
+  if (item >= (long long)T_tokens * heads) return;
+  const int t = (int)(item / heads), head = (int)(item - (long long)t * heads);
+  const bool is_q = head < Hq, is_k = !is_q && head < Hq + Hkv;
+  const int slot = is_q ? 0 : slots[t];
+  const long long page = slot < 0 ? -1 : slot / page_size;
+  if (!is_q && (page < 0 || page >= num_pages)) return;
+  float x[2][4];
+  norm_rope_row<T>(qkv + item * D, row[warp], is_q ? q_norm_w : is_k ? k_norm_w : nullptr, eps, cos_sin != nullptr && (is_q || is_k),
+                   cos_sin, rotary_dim, max_pos, positions, t, D, x);
+  if (is_q) {
+    T* dst = q_out + ((long long)t * Hq + head) * D;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int d = i * 128 + lane * 4;
+      if (d < D) store4<T>(dst + d, x[i]);
+    }
+    return;
+  }
+  unsigned own[2] = {0, 0};      // of the lane's blocks
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) own[i] = max(own[i], fp4_magnitude(x[i][e]));
+    own[i] = max(own[i], __shfl_xor_sync(0xffffffffu, own[i], 1));
+    own[i] = max(own[i], __shfl_xor_sync(0xffffffffu, own[i], 2));
+  }
+  const unsigned exponent = fp4_row_exponent(__reduce_max_sync(0xffffffffu, max(own[0], own[1])));
+  const float down = fp4_down(exponent);
+  const int kv = !is_k, h = is_k ? head - Hq : head - Hq - Hkv;
+  const long long at = ((page * 2 + kv) * Hkv + h) * page_size + (slot - page * page_size);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int d = i * 128 + lane * 4;
+    if (d >= D) break;
+    const unsigned scale = fp4_block_scale(own[i], down);
+    const Fp4Scaler q = fp4_scaler(scale, down);
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = fp4_quotient(x[i][e], q);
+    *reinterpret_cast<unsigned short*>(cache.data + at * (D / 2) + d / 2) = (unsigned short)(q.inv == 0.f ? 0 : fp4_pack4(y));
+    if ((lane & 3) == 0) cache.scales[at * (D / 16) + d / 16] = (unsigned char)scale;
+  }
+  if (lane == 0) cache.exponents[at] = (unsigned char)exponent;
+}
+
+// ---- the keys and values of some sequences as bfloat16 pages of their own, [pages, 2, Hkv, PAGE, D], for attention over an unquantised
+// cache: what 4 bits stand for has 6 digits, so that bfloat16 holds it exactly.  Sequence number i of the launch, seq_list[i],
+// has its pages from first_page[i] on, one for every PAGE keys up to the host's bound of its length.  Keys behind its real length,
+// and those that are on no page of the pool, are zeros up to the page's end; pages wholly behind the last key, or ahead of the
+// window of the first new token, are left as they are.  (The new block table follows from the bounds: the host makes it.)
+constexpr int UNPACK_PAGE = 128;
+struct UnpackArgs {
+  Cache4 cache;
+  const int* block_table;
+  const int* cu_q_lens;
+  const int* seq_lens;
+  const int* seq_list;      // [count]
+  const int* first_page;    // [count + 1]
+  __nv_bfloat16* out;
+  int max_blocks, Hkv, D, page_size, window;
+  long long num_pages;
+};
+template <int LANES>
+__global__ void __launch_bounds__(CACHE_THREADS)
+unpack_pages_kernel(const __grid_constant__ UnpackArgs a) {
+  Cache4 held = a.cache;
+  pdl_prologue(held.data, held.scales, held.exponents);
+  const int seq = a.seq_list[blockIdx.z], page = blockIdx.x, rows = blockIdx.y;      // rows: (keys or values, head)
+  const int first_page = a.first_page[blockIdx.z], bound = a.first_page[blockIdx.z + 1] - first_page;
+  if (page >= bound) return;
+  const int kv_len = (int)min((long long)a.seq_lens[seq], (long long)a.max_blocks * a.page_size);
+  const int first = first_visible_key(max(kv_len - (a.cu_q_lens[seq + 1] - a.cu_q_lens[seq]), 0), a.window);
+  const int key0 = page * UNPACK_PAGE;
+  if (key0 >= kv_len || key0 + UNPACK_PAGE <= first) return;
+  constexpr int GROUPS = CACHE_THREADS / LANES, ROWS = 2;
+  const int l = threadIdx.x % LANES;
+  if (l * 16 >= a.D) return;
+  const int* table = a.block_table + (long long)seq * a.max_blocks;
+  __nv_bfloat16* out = a.out + ((long long)(first_page + page) * 2 * a.Hkv + rows) * UNPACK_PAGE * a.D + l * 16;
+#pragma unroll 1
+  for (int r0 = threadIdx.x / LANES; r0 < UNPACK_PAGE; r0 += GROUPS * ROWS) {
+    Held16 x[ROWS];
+#pragma unroll
+    for (int g = 0; g < ROWS; ++g) {
+      const int key = key0 + r0 + g * GROUPS;
+      long long at = -1;
+      if (key < kv_len) {
+        const int of = key / a.page_size, p = table[of];
+        if (p >= 0 && p < a.num_pages) at = ((long long)p * 2 * a.Hkv + rows) * a.page_size + (key - of * a.page_size);
+      }
+      x[g].load(held, at, l, a.D);
+    }
+#pragma unroll
+    for (int g = 0; g < ROWS; ++g) {
+      float y[16];
+      x[g].values(y);
+      store16(out + (long long)(r0 + g * GROUPS) * a.D, y);
+    }
+  }
+}
+
+template <typename T>
+int launch_write(const void* k, const void* v, long long k_stride, long long v_stride, const Cache4& cache, const int* slots,
+                 const CacheShape& s, cudaStream_t st) {
+  const bool wide = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 31) == 0 &&
+                    (k_stride * sizeof(T)) % 32 == 0 && (v_stride * sizeof(T)) % 32 == 0;
+  const int groups = CACHE_THREADS / (s.D > 128 ? 16 : 8);
+  auto kern = s.D > 128 ? (wide ? cache_write_kernel<T, true, 16> : cache_write_kernel<T, false, 16>)
+                        : (wide ? cache_write_kernel<T, true, 8> : cache_write_kernel<T, false, 8>);
+  dib_launch(kern, dim3((s.rows + groups - 1) / groups), dim3(CACHE_THREADS), 0, st, reinterpret_cast<const T*>(k),
+             reinterpret_cast<const T*>(v), k_stride, v_stride, cache, slots, s);
+  DIB_CHECK_LAUNCH();
+  return DIB_OK;
+}
+template <typename T>
+int launch_read(const Cache4& cache, const int* slots, void* k, void* v, const CacheShape& s, cudaStream_t st) {
+  if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 31) != 0) return DIB_BAD_ALIGN;
+  constexpr int ROWS = 2;
+  const int per = CACHE_THREADS / (s.D > 128 ? 16 : 8) * ROWS;
+  dib_launch(s.D > 128 ? cache_read_kernel<T, 16, ROWS> : cache_read_kernel<T, 8, ROWS>, dim3((s.rows + per - 1) / per),
+             dim3(CACHE_THREADS), 0, st, cache, slots, reinterpret_cast<T*>(k), reinterpret_cast<T*>(v), s);
+  DIB_CHECK_LAUNCH();
+  return DIB_OK;
+}
+bool shape_fits(int T, int Hkv, int D, int page_size, long long num_pages) {
+  return T >= 0 && Hkv >= 1 && D >= 16 && D <= 256 && D % 16 == 0 && page_size >= 1 && (long long)T * 2 * Hkv <= 0x7fffff00ll &&
+         num_pages <= 0x7fffffffll;
+}
+Cache4 make_cache(const void* data, const void* scales, const void* exponents) {
+  Cache4 c;
+  c.data = reinterpret_cast<unsigned char*>(const_cast<void*>(data));
+  c.scales = reinterpret_cast<unsigned char*>(const_cast<void*>(scales));
+  c.exponents = reinterpret_cast<unsigned char*>(const_cast<void*>(exponents));
+  return c;
+}
+
+}  // namespace
+
+extern "C" {
+
+// k, v: rows [T] of Hkv * D values, `k_stride`, `v_stride` values apart (dtype 0 float32, 1 bfloat16); slots int32 [T]
+// (page * page_size + offset; a negative one, or one beyond the pool, is skipped).
+int dib_fp4_cache_write(const void* k, const void* v, long long k_stride, long long v_stride, void* data, void* scales, void* exponents,
+                        const void* slots, int T, int Hkv, int D, int page_size, long long num_pages, int dtype, cudaStream_t st) {
+  if (dtype != 0 && dtype != 1) return DIB_BAD_DTYPE;
+  if (!shape_fits(T, Hkv, D, page_size, num_pages)) return DIB_BAD_SIZE;
+  if ((reinterpret_cast<uintptr_t>(data) & 15) != 0) return DIB_BAD_ALIGN;
+  if (T == 0) return DIB_OK;
+  const CacheShape shape = make_shape((long long)T * 2 * Hkv, Hkv, D, page_size, num_pages);
+  const Cache4 cache = make_cache(data, scales, exponents);
+  const int* sl = reinterpret_cast<const int*>(slots);
+  if (dtype == 1) return launch_write<__nv_bfloat16>(k, v, k_stride, v_stride, cache, sl, shape, st);
+  return launch_write<float>(k, v, k_stride, v_stride, cache, sl, shape, st);
+}
+
+// qkv [T, (Hq + 2 Hkv) D] -> q_out [T, Hq, D] and the cache; q_norm_w, k_norm_w float32 [D] or null; cos_sin float32
+// [max_pos, rotary_dim] = [cos | sin] or null; a token whose slot is none of the pool's keeps no key.
+int dib_fp4_qk_norm_rope_cache(const void* qkv, void* q_out, void* data, void* scales, void* exponents, const void* q_norm_w,
+                               const void* k_norm_w, float eps, const void* cos_sin, int rotary_dim, int max_pos,
+                               const void* positions, const void* slots, int T, int Hq, int Hkv, int D, int page_size,
+                               long long num_pages, int dtype, cudaStream_t st) {
+  if (dtype != 0 && dtype != 1) return DIB_BAD_DTYPE;
+  if (!shape_fits(T, Hkv, D, page_size, num_pages) || Hq < 1 || rotary_dim < 0 || rotary_dim > D || rotary_dim % 2 != 0 ||
+      (cos_sin != nullptr && max_pos < 1))
+    return DIB_BAD_SIZE;
+  if (((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(data)) & 15) != 0)
+    return DIB_BAD_ALIGN;
+  if (T == 0) return DIB_OK;
+  const long long blocks = ((long long)T * (Hq + 2 * Hkv) + QKV_WARPS - 1) / QKV_WARPS;
+  if (blocks > 0x7fffffffll) return DIB_BAD_SIZE;
+  const float *qw = reinterpret_cast<const float*>(q_norm_w), *kw = reinterpret_cast<const float*>(k_norm_w),
+              *tab = reinterpret_cast<const float*>(cos_sin);
+  const int *ps = reinterpret_cast<const int*>(positions), *sl = reinterpret_cast<const int*>(slots);
+  const Cache4 cache = make_cache(data, scales, exponents);
+  if (dtype == 1)
+    dib_launch(qk_norm_rope_cache_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(QKV_WARPS * 32), 0, st,
+               reinterpret_cast<const __nv_bfloat16*>(qkv), reinterpret_cast<__nv_bfloat16*>(q_out), cache, qw, kw, eps, tab,
+               rotary_dim, max_pos, ps, sl, T, Hq, Hkv, D, page_size, num_pages);
+  else
+    dib_launch(qk_norm_rope_cache_kernel<float>, dim3((unsigned)blocks), dim3(QKV_WARPS * 32), 0, st,
+               reinterpret_cast<const float*>(qkv), reinterpret_cast<float*>(q_out), cache, qw, kw, eps, tab, rotary_dim, max_pos, ps, sl,
+               T, Hq, Hkv, D, page_size, num_pages);
+  DIB_CHECK_LAUNCH();
+  return DIB_OK;
+}
+
+// k, v [T, Hkv, D] = the values that the rows in `slots` stand for; zeros for a slot that is none of the pool's.
+int dib_fp4_cache_read(const void* data, const void* scales, const void* exponents, const void* slots, void* k, void* v, int T, int Hkv,
+                       int D, int page_size, long long num_pages, int dtype, cudaStream_t st) {
+  if (dtype != 0 && dtype != 1) return DIB_BAD_DTYPE;
+  if (!shape_fits(T, Hkv, D, page_size, num_pages)) return DIB_BAD_SIZE;
+  if ((reinterpret_cast<uintptr_t>(data) & 15) != 0) return DIB_BAD_ALIGN;
+  if (T == 0) return DIB_OK;
+  const CacheShape shape = make_shape((long long)T * 2 * Hkv, Hkv, D, page_size, num_pages);
+  const Cache4 cache = make_cache(data, scales, exponents);
+  const int* sl = reinterpret_cast<const int*>(slots);
+  if (dtype == 1) return launch_read<__nv_bfloat16>(cache, sl, k, v, shape, st);
+  return launch_read<float>(cache, sl, k, v, shape, st);
+}
+
+int dib_fp4_unpack_page() { return UNPACK_PAGE; }
+
+// The keys and values of the sequences seq_list [count] as bfloat16 pages [first_page[count], 2, Hkv, 128, D] (see
+// unpack_pages_kernel); first_page int32 [count + 1], max_pages the most pages of one of them.
+int dib_fp4_unpack_pages(const void* data, const void* scales, const void* exponents, long long num_pages, const void* block_table,
+                         int max_blocks, const void* cu_q_lens, const void* seq_lens, const void* seq_list, const void* first_page,
+                         int count, int max_pages, void* out, int Hkv, int D, int page_size, int window, cudaStream_t st) {
+  if (!shape_fits(0, Hkv, D, page_size, num_pages) || count < 0 || count > 65535 || max_pages < 1 || 2 * Hkv > 65535 || max_blocks < 1)
+    return DIB_BAD_SIZE;
+  if ((reinterpret_cast<uintptr_t>(data) & 15) != 0 || (reinterpret_cast<uintptr_t>(out) & 31) != 0) return DIB_BAD_ALIGN;
+  if (count == 0) return DIB_OK;
+  UnpackArgs a;
+  a.cache = make_cache(data, scales, exponents);
+  a.block_table = reinterpret_cast<const int*>(block_table);
+  a.cu_q_lens = reinterpret_cast<const int*>(cu_q_lens);
+  a.seq_lens = reinterpret_cast<const int*>(seq_lens);
+  a.seq_list = reinterpret_cast<const int*>(seq_list);
+  a.first_page = reinterpret_cast<const int*>(first_page);
+  a.out = reinterpret_cast<__nv_bfloat16*>(out);
+  a.max_blocks = max_blocks;
+  a.Hkv = Hkv; a.D = D; a.page_size = page_size; a.window = window;
+  a.num_pages = num_pages;
+  dib_launch(D > 128 ? unpack_pages_kernel<16> : unpack_pages_kernel<8>, dim3((unsigned)max_pages, 2u * Hkv, (unsigned)count),
+             dim3(CACHE_THREADS), 0, st, a);
+  DIB_CHECK_LAUNCH();
+  return DIB_OK;
+}
+
+}  // extern "C"

@@ -10,7 +10,7 @@
 // a NaN has the scale NaN, so whatever reads it gets NaN and not a number that looks right.
 //
 // Cache: data int8 [pages, 2, Hkv, page_size, D], scales float32 [pages, 2, Hkv, page_size].
-#include "common.cuh"
+#include "cache_rows.cuh"
 
 namespace {
 
@@ -74,25 +74,6 @@ template <> __device__ __forceinline__ void load8<float>(const float* p, float (
   x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
 }
 
-template <typename T> __device__ __forceinline__ void load4(const T* p, float (&x)[4]);
-template <> __device__ __forceinline__ void load4<float>(const float* p, float (&x)[4]) {
-  const float4 v = *reinterpret_cast<const float4*>(p);
-  x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-}
-template <> __device__ __forceinline__ void load4<__nv_bfloat16>(const __nv_bfloat16* p, float (&x)[4]) {
-  const uint2 v = *reinterpret_cast<const uint2*>(p);
-  x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
-  x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
-}
-template <typename T> __device__ __forceinline__ void store4(T* p, const float (&x)[4]);
-template <> __device__ __forceinline__ void store4<float>(float* p, const float (&x)[4]) {
-  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-}
-template <> __device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16* p, const float (&x)[4]) {
-  const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
-  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
-}
-
 // 32 bytes of a row at once
 template <typename T> struct Piece {
   static constexpr int N = 32 / (int)sizeof(T);        // values
@@ -112,28 +93,6 @@ template <typename T> struct Piece {
     return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
   }
 };
-// n / d for n < 2^31 by a product: d's reciprocal rounded up, with as many bits as make that exact
-struct Divisor {
-  unsigned mul, shift, d;
-};
-__device__ __forceinline__ unsigned quotient(unsigned n, const Divisor& v) {
-  return v.mul == 0 ? n >> v.shift : __umulhi(n, v.mul) >> v.shift;
-}
-static inline Divisor make_divisor(unsigned d) {
-  Divisor v;
-  v.d = d;
-  unsigned log = 0;
-  while ((1ull << log) < d) ++log;
-  if ((1u << log) == d) {
-    v.mul = 0;
-    v.shift = log;
-  } else {      // n < 2^31: floor(n m / 2^(31 + log)) with m = ceil(2^(31 + log) / d) < 2^32 is exact
-    v.mul = (unsigned)(((1ull << (31 + log)) + d - 1) / d);
-    v.shift = log - 1;
-  }
-  return v;
-}
-
 // A row of the cache: 128 values are LANES lanes, 32 bytes of the unquantised row each.  Memory bound: many warps of few
 // registers and few instructions: 8,000 tokens of 8 heads of 128 written from bfloat16 and read back in 19.4 us, 99 MB at
 // 5.1 TB/s (16 values a lane of several rows a group: 93 registers, 37 us).
@@ -141,32 +100,6 @@ constexpr int CACHE_THREADS = 256;
 template <typename T> struct Rows {
   static constexpr int N = Piece<T>::N, LANES = 128 / N, GROUPS = CACHE_THREADS / LANES;
 };
-struct CacheShape {
-  Divisor per_token, page;      // 2 Hkv rows a token, rows a page
-  unsigned rows;
-  int Hkv, D;
-  unsigned num_pages;
-};
-struct CacheRow {
-  long long at;      // row of the cache, or -1
-  int token, kv, h;
-};
-// row r = (token, key or value, kv head)
-__device__ __forceinline__ CacheRow cache_row(unsigned r, const CacheShape& s, const int* slots) {
-  CacheRow c;
-  c.at = -1;
-  c.token = (int)quotient(r, s.per_token);
-  const int rest = (int)(r - (unsigned)c.token * s.per_token.d);
-  c.kv = rest >= s.Hkv;
-  c.h = rest - c.kv * s.Hkv;
-  if (r >= s.rows) return c;
-  const int slot = slots[c.token];
-  if (slot < 0) return c;
-  const unsigned page = quotient((unsigned)slot, s.page);
-  if (page < s.num_pages) c.at = ((long long)page * s.per_token.d + rest) * s.page.d + (slot - (int)(page * s.page.d));
-  return c;
-}
-
 template <typename T, bool ALIGNED, int HALVES>
 __global__ void __launch_bounds__(CACHE_THREADS)
 cache_write_kernel(const T* __restrict__ k, const T* __restrict__ v, long long k_stride, long long v_stride,
@@ -300,52 +233,9 @@ qk_norm_rope_cache_int8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out,
   const int slot = is_q ? 0 : slots[t];
   const long long page = slot < 0 ? -1 : slot / page_size;
   if (!is_q && (page < 0 || page >= num_pages)) return;
-  const T* src = qkv + item * D;
-  float* s = row[warp];
-  float x[2][4], squares[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int d = i * 128 + lane * 4;
-    x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
-    if (d < D) load4<T>(src + d, x[i]);
-    squares[i] = sumsq4(x[i][0], x[i][1], x[i][2], x[i][3]);
-  }
-  if (nw != nullptr) {
-    float total = warp_sum(squares[0]);
-    if (D > 128) total = __fadd_rn(total, warp_sum(squares[1]));
-    const float rstd = rms_rstd(total, D, eps);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int d = i * 128 + lane * 4;
-      if (d < D)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[i][e] = norm_scale(x[i][e], rstd, nw[d + e]);
-    }
-  }
-  if (cos_sin != nullptr && (is_q || is_k)) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int d = i * 128 + lane * 4;
-      if (d < D) *reinterpret_cast<float4*>(s + d) = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
-    }
-    __syncwarp();
-    int pos = positions[t];
-    pos = pos < 0 ? 0 : pos >= max_pos ? max_pos - 1 : pos;
-    const float* tab = cos_sin + (long long)pos * rotary_dim;
-    const int half = rotary_dim >> 1;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d = i * 128 + lane * 4 + e;
-        if (d < half) x[i][e] = rope_first(x[i][e], s[d + half], tab[d], tab[half + d]);
-        else if (d < rotary_dim) x[i][e] = rope_second(s[d - half], x[i][e], tab[d - half], tab[d]);
-      }
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[i][e] = round_to<T>(x[i][e]);
+  float x[2][4];
+  norm_rope_row<T>(qkv + item * D, row[warp], nw, eps, cos_sin != nullptr && (is_q || is_k), cos_sin, rotary_dim, max_pos, positions,
+                   t, D, x);
   if (is_q) {
     T* dst = q_out + ((long long)t * Hq + head) * D;
 #pragma unroll
@@ -420,15 +310,6 @@ quantize_rows_kernel(const T* __restrict__ x, long long stride, signed char* __r
   }
 }
 
-CacheShape make_shape(long long rows, int Hkv, int D, int page_size, long long num_pages) {
-  CacheShape s;
-  s.per_token = make_divisor(2u * Hkv);
-  s.page = make_divisor((unsigned)page_size);
-  s.rows = (unsigned)rows;
-  s.Hkv = Hkv; s.D = D;
-  s.num_pages = (unsigned)num_pages;
-  return s;
-}
 template <typename T>
 int launch_write(const void* k, const void* v, long long k_stride, long long v_stride, signed char* data, float* scales,
                  const int* slots, const CacheShape& s, cudaStream_t st) {

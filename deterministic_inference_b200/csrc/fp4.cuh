@@ -64,6 +64,11 @@ __device__ __forceinline__ unsigned fp4_pack8(const float* y) {
       "}" : "=r"(r) : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
   return r;
 }
+// four values' codes in the low 16 bits
+__device__ __forceinline__ unsigned fp4_pack4(const float* y) {
+  const float x[8] = {y[0], y[1], y[2], y[3], 0.f, 0.f, 0.f, 0.f};
+  return fp4_pack8(x) & 0xffffu;
+}
 // What the values of a block are multiplied with: 2^-E, and the block scale with its reciprocal (0 and 0: all codes are 0).
 struct Fp4Scaler {
   float down, b, inv;
@@ -107,6 +112,62 @@ __device__ __forceinline__ void fp4_values8(unsigned w, float scale, float* x) {
     x[2 * i] = lo * scale;
     x[2 * i + 1] = hi * scale;
   }
+}
+
+// 16 values of a row from `at` on, zeros behind K; kept as they came (bfloat16 two a word).
+template <typename T> struct Block16 {
+  static constexpr int WORDS = 16 * (int)sizeof(T) / 4;
+  unsigned w[WORDS];
+  template <bool WIDE> __device__ __forceinline__ void load(const T* row, int at, int K) {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = 0;
+    if (at >= K) return;
+    if (WIDE) {      // rows on 32 bytes, K a multiple of 16
+#pragma unroll
+      for (int i = 0; i < WORDS / 8; ++i)
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(w[8 * i]), "=r"(w[8 * i + 1]), "=r"(w[8 * i + 2]), "=r"(w[8 * i + 3]), "=r"(w[8 * i + 4]),
+                       "=r"(w[8 * i + 5]), "=r"(w[8 * i + 6]), "=r"(w[8 * i + 7])
+                     : "l"(reinterpret_cast<const char*>(row + at) + 32 * i));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (at + e < K) {
+          if (sizeof(T) == 4) w[e % WORDS] = __float_as_uint(Elem<T>::load(row + at + e));
+          else w[e >> 1] |= (unsigned)*reinterpret_cast<const unsigned short*>(row + at + e) << (16 * (e & 1));
+        }
+    }
+  }
+  __device__ __forceinline__ float get(int e) const {
+    if (sizeof(T) == 4) return __uint_as_float(w[e % WORDS]);
+    return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+  }
+  __device__ __forceinline__ unsigned top() const {
+    unsigned t = 0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) t = max(t, fp4_magnitude(get(e)));
+    return t;
+  }
+};
+// 16 values, on 32 bytes
+template <typename T> __device__ __forceinline__ void store16(T* dst, const float (&x)[16]) {
+  constexpr int WORDS = 16 * (int)sizeof(T) / 4;
+  unsigned y[16];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (sizeof(T) == 4) {
+      y[2 * e] = __float_as_uint(x[2 * e]);
+      y[2 * e + 1] = __float_as_uint(x[2 * e + 1]);
+    } else {
+      const __nv_bfloat162 p = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+      y[e] = *reinterpret_cast<const unsigned*>(&p);
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < WORDS; w += 8)
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<unsigned*>(dst) + w), "r"(y[w]),
+                 "r"(y[w + 1]), "r"(y[w + 2]), "r"(y[w + 3]), "r"(y[w + 4]), "r"(y[w + 5]), "r"(y[w + 6]), "r"(y[w + 7])
+                 : "memory");
 }
 
 // ---- block scales of a matrix's rows as the tensor cores' block-scaled products take them: tiles of 128 rows x 64 values, 512

@@ -9,42 +9,6 @@
 
 namespace {
 
-// 16 values of a row from `at` on, zeros behind K; kept as they came (bfloat16 two a word).
-template <typename T> struct Block16 {
-  static constexpr int WORDS = 16 * (int)sizeof(T) / 4;
-  unsigned w[WORDS];
-  template <bool WIDE> __device__ __forceinline__ void load(const T* row, int at, int K) {
-#pragma unroll
-    for (int i = 0; i < WORDS; ++i) w[i] = 0;
-    if (at >= K) return;
-    if (WIDE) {      // rows on 32 bytes, K a multiple of 16
-#pragma unroll
-      for (int i = 0; i < WORDS / 8; ++i)
-        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                     : "=r"(w[8 * i]), "=r"(w[8 * i + 1]), "=r"(w[8 * i + 2]), "=r"(w[8 * i + 3]), "=r"(w[8 * i + 4]),
-                       "=r"(w[8 * i + 5]), "=r"(w[8 * i + 6]), "=r"(w[8 * i + 7])
-                     : "l"(reinterpret_cast<const char*>(row + at) + 32 * i));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (at + e < K) {
-          if (sizeof(T) == 4) w[e % WORDS] = __float_as_uint(Elem<T>::load(row + at + e));
-          else w[e >> 1] |= (unsigned)*reinterpret_cast<const unsigned short*>(row + at + e) << (16 * (e & 1));
-        }
-    }
-  }
-  __device__ __forceinline__ float get(int e) const {
-    if (sizeof(T) == 4) return __uint_as_float(w[e % WORDS]);
-    return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
-  }
-  __device__ __forceinline__ unsigned top() const {
-    unsigned t = 0;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) t = max(t, fp4_magnitude(get(e)));
-    return t;
-  }
-};
-
 template <typename T>
 __device__ __forceinline__ void write_block(const Block16<T>& x, unsigned top, float down, unsigned char* codes, unsigned char* tiles,
                                             long long row, int block, int Kp, int k_tiles) {
@@ -143,23 +107,7 @@ read_rows_kernel(const unsigned char* __restrict__ codes, const unsigned char* _
 #pragma unroll
   for (int e = 0; e < 16; ++e) x[e] *= unit;
   if (WIDE) {
-    unsigned y[16];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (sizeof(T) == 4) {
-        y[2 * e] = __float_as_uint(x[2 * e]);
-        y[2 * e + 1] = __float_as_uint(x[2 * e + 1]);
-      } else {
-        const __nv_bfloat162 p = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
-        y[e] = *reinterpret_cast<const unsigned*>(&p);
-      }
-    }
-#pragma unroll
-    for (int h = 0; h < (int)sizeof(T) / 2; ++h)
-      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<char*>(dst) + 32 * h),
-                   "r"(y[8 * h]), "r"(y[8 * h + 1]), "r"(y[8 * h + 2]), "r"(y[8 * h + 3]), "r"(y[8 * h + 4]), "r"(y[8 * h + 5]),
-                   "r"(y[8 * h + 6]), "r"(y[8 * h + 7])
-                   : "memory");
+    store16(dst, x);
   } else {
 #pragma unroll
     for (int e = 0; e < 16; ++e)

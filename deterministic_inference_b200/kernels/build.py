@@ -55,6 +55,8 @@ SOURCES = {
     "gemm_int8": "gemm_int8.cu",
     "rows_fp4": "rows_fp4.cu",
     "gemm_fp4": "gemm_fp4.cu",
+    "cache_fp4": "cache_fp4.cu",
+    "attention_fp4": "attention_fp4.cu",
 }
 HEADERS = ("common.cuh", "attention_merge.cuh")
 # further headers a library includes
@@ -73,6 +75,9 @@ EXTRA_HEADERS = {
     "gated_linear_attention": ("source.cuh", "sigmoid_attention_mma.cuh", "linear_chunks.cuh"),
     "rows_fp4": ("fp4.cuh",),
     "gemm_fp4": ("fp4.cuh",),
+    "cache_int8": ("cache_rows.cuh",),
+    "cache_fp4": ("cache_rows.cuh", "fp4.cuh"),
+    "attention_fp4": ("fp4.cuh",),
 }
 
 NVCC_FLAGS = [

@@ -26,6 +26,7 @@ from __future__ import annotations
 
 import ctypes
 from ctypes import c_float, c_int, c_longlong, c_void_p
+from types import SimpleNamespace
 
 import torch
 
@@ -43,6 +44,13 @@ _SIGNATURES = {
     "dib_fp4_layout_rows": ("rows_fp4", (_P, _P, _P, _P, _P, _P, _L, _I, _P)),
     "dib_gemm_fp4": ("gemm_fp4", (_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P)),
     "dib_fp4_linear": ("gemm_fp4", (_P, _P, _L, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P)),
+    "dib_fp4_cache_write": ("cache_fp4", (_P, _P, _L, _L, _P, _P, _P, _P, _I, _I, _I, _I, _L, _I, _P)),
+    "dib_fp4_cache_read": ("cache_fp4", (_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _L, _I, _P)),
+    "dib_fp4_qk_norm_rope_cache": ("cache_fp4", (_P, _P, _P, _P, _P, _P, _P, _F, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _L, _I, _P)),
+    "dib_fp4_unpack_pages": ("cache_fp4", (_P, _P, _P, _L, _P, _I, _P, _P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _P)),
+    "dib_fp4_attention_split": ("attention_fp4", (_P, _P, _P, _P, _P, _L, _P, _I, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _I, _I,
+                                                  _I, _I, _F, _I, _I, _I, _P)),
+    "dib_fp4_attention_any": ("attention_fp4", (_P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _L, _F, _I, _I, _P)),
 }
 _functions: dict = {}
 _ops_module = None
@@ -288,3 +296,309 @@ def force_product_form(form: int) -> None:
     """Measurement and test switch of the product: tiles of 128 x 64, 128 x 128 or 128 x 192 (0, 1, 2), the pair of CTAs (3),
     clusters that share k (4, up to 128 rows), whatever the sizes; -1: the library's own choice.  All give the same bits."""
     _ops()._lib("gemm_fp4").dib_gemm_fp4_force_form(c_int(form))
+
+
+# ---- the cache
+
+class Fp4Cache:
+    """One layer's paged cache in 4 bits: ``data`` uint8 [pages, 2, Hkv, page_size, D / 2], ``scales`` float8_e4m3fn
+    [pages, 2, Hkv, page_size, D / 16], finite and not negative in the rows that are read, ``exponents`` uint8
+    [pages, 2, Hkv, page_size]; [:, 0] are keys, [:, 1] values.  D a multiple of 16, at most 256."""
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor, exponents: torch.Tensor):
+        ops = _ops()
+        ops._need(data, "data", torch.uint8, 5)
+        ops._need(scales, "scales", torch.float8_e4m3fn, 5)
+        ops._need(exponents, "exponents", torch.uint8, 4)
+        pages, two, hkv, page_size, half = data.shape
+        d = 2 * half
+        if tuple(exponents.shape) != (pages, two, hkv, page_size) or tuple(scales.shape) != (pages, two, hkv, page_size, d // BLOCK) \
+                or two != 2 or hkv < 1 or page_size < 1:
+            raise ops.KernelError(f"Fp4Cache: data {tuple(data.shape)}, scales {tuple(scales.shape)}, exponents "
+                                  f"{tuple(exponents.shape)}")
+        if d < 16 or d > MAX_HEAD_DIM or d % 16:
+            raise ops.KernelError(f"Fp4Cache: heads of {d} (a multiple of 16, at most {MAX_HEAD_DIM})")
+        if data.data_ptr() % 16:
+            raise ops.KernelError("Fp4Cache: data must lie on 16 bytes")
+        _same_device("Fp4Cache", data, scales, exponents)
+        self.data, self.scales, self.exponents = data, scales, exponents
+        self.shape = torch.Size((pages, 2, hkv, page_size, d))
+
+    @classmethod
+    def zeros(cls, num_pages: int, num_kv_heads: int, page_size: int, head_dim: int, device="cuda") -> "Fp4Cache":
+        rows = (num_pages, 2, num_kv_heads, page_size)
+        return cls(torch.zeros(*rows, head_dim // 2, dtype=torch.uint8, device=device),
+                   torch.zeros(*rows, head_dim // BLOCK, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn),
+                   torch.zeros(rows, dtype=torch.uint8, device=device))
+
+    @property
+    def device(self):
+        return self.data.device
+
+    def _pointers(self) -> tuple:
+        return self.data.data_ptr(), self.scales.data_ptr(), self.exponents.data_ptr()
+
+
+def _row_stride(x, name: str, hkv: int, d: int) -> int:
+    """Distance of a token's rows [Hkv, D], which lie together (a column range of a fused projection, say)."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise _ops().KernelError(f"{name} must be a CUDA tensor: this package has no CPU path")
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 3 or shape[1] != hkv or shape[2] != d:
+        raise _ops().KernelError(f"{name} has shape {tuple(shape)}, the cache's heads are [{hkv}, {d}]")
+    if stride[2] != 1 or (hkv > 1 and stride[1] != d):
+        raise _ops().KernelError(f"{name}: a token's heads must lie together (stride {stride})")
+    return stride[0]
+
+
+def fp4_cache_write(k: torch.Tensor, v: torch.Tensor, cache: Fp4Cache, slot_mapping: torch.Tensor) -> None:
+    """k, v [T, Hkv, D] (float32 or bfloat16; column ranges of wider rows too) into the rows ``slot_mapping`` (int32 [T],
+    page * page_size + offset) of the cache; a negative slot is skipped.  Slots are distinct."""
+    pages, _, hkv, page_size, d = cache.shape
+    ks, vs = _row_stride(k, "k", hkv, d), _row_stride(v, "v", hkv, d)
+    _require(slot_mapping, "slot_mapping", torch.int32, 1)
+    t = k.shape[0]
+    if v.shape[0] != t or v.dtype is not k.dtype or slot_mapping.shape[0] < t:
+        raise _ops().KernelError(f"fp4_cache_write: k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}, "
+                                 f"{slot_mapping.shape[0]} slots")
+    device = cache.device
+    if k.device != device or v.device != device or slot_mapping.device != device:
+        _same_device("fp4_cache_write", cache.data, k, v, slot_mapping)
+    st = _fn("dib_fp4_cache_write")(k.data_ptr(), v.data_ptr(), ks, vs, *cache._pointers(), slot_mapping.data_ptr(), t, hkv, d,
+                                    page_size, pages, _code(k.dtype, "k"), _stream("fp4_cache_write", device))
+    _done(st, "fp4_cache_write", lambda: f"heads {hkv} x {d}")
+
+
+def fp4_qk_norm_rope_cache(qkv, num_heads: int, num_kv_heads: int, head_dim: int, q_norm_weight, k_norm_weight, eps: float,
+                           cos_sin, positions: torch.Tensor, cache: Fp4Cache, slot_mapping: torch.Tensor) -> torch.Tensor:
+    """``ops.qk_norm_rope_cache`` with a 4-bit cache: q [T, Hq, D] normed and rotated; k, treated alike, and v are rounded to
+    the activations' type, quantised and written to the tokens' slots."""
+    ops = _ops()
+    qkv = ops.as_tensor(qkv)
+    ops._need(qkv, "qkv", None, 2)
+    t, width = qkv.shape
+    pages, _, hkv, page_size, d = cache.shape
+    if (hkv, d) != (num_kv_heads, head_dim) or width != (num_heads + 2 * hkv) * d:
+        raise ops.KernelError(f"fp4_qk_norm_rope_cache: rows of {width} for heads {num_heads}/{num_kv_heads} x {head_dim}, "
+                              f"cache {tuple(cache.shape)}")
+    for x, name in ((positions, "positions"), (slot_mapping, "slot_mapping")):
+        ops._need(x, name, torch.int32, 1)
+        if x.shape[0] < t:
+            raise ops.KernelError(f"fp4_qk_norm_rope_cache: {x.shape[0]} {name} for {t} tokens")
+    for w, name in ((q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight")):
+        if w is not None:
+            ops._need(w, name, torch.float32, 1)
+            if w.shape[0] != d:
+                raise ops.KernelError(f"{name} has {w.shape[0]} elements, head_dim is {d}")
+    rotary_dim, max_pos = 0, 0
+    if cos_sin is not None:
+        ops._need(cos_sin, "cos_sin", torch.float32, 2)
+        max_pos, rotary_dim = cos_sin.shape
+    _same_device("fp4_qk_norm_rope_cache", qkv, cache.data, positions, slot_mapping,
+                 *(x for x in (q_norm_weight, k_norm_weight, cos_sin) if x is not None))
+    q = torch.empty(t, num_heads, d, dtype=qkv.dtype, device=qkv.device)
+    st = _fn("dib_fp4_qk_norm_rope_cache")(
+        qkv.data_ptr(), q.data_ptr(), *cache._pointers(), _pointer(q_norm_weight), _pointer(k_norm_weight), float(eps),
+        _pointer(cos_sin), rotary_dim, max_pos, positions.data_ptr(), slot_mapping.data_ptr(), t, num_heads, hkv, d, page_size,
+        pages, _code(qkv.dtype, "qkv"), _stream("fp4_qk_norm_rope_cache", qkv.device))
+    _done(st, "fp4_qk_norm_rope_cache", lambda: f"head_dim {d}, rotary_dim {rotary_dim}")
+    return q
+
+
+def fp4_cache_read(cache: Fp4Cache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
+    """(k, v) [T, Hkv, D] in ``dtype``: what the rows ``slots`` (int32 [T]) of the cache stand for; zeros for a negative
+    slot."""
+    pages, _, hkv, page_size, d = cache.shape
+    _require(slots, "slots", torch.int32, 1)
+    device = cache.device
+    if slots.device != device:
+        _same_device("fp4_cache_read", cache.data, slots)
+    code = _code(dtype, "out")
+    t = slots.shape[0]
+    k, v = torch.empty(2, t, hkv, d, dtype=dtype, device=device).unbind(0)
+    st = _fn("dib_fp4_cache_read")(*cache._pointers(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), t, hkv, d, page_size, pages,
+                                   code, _stream("fp4_cache_read", device))
+    _done(st, "fp4_cache_read", lambda: f"heads {hkv} x {d}")
+    return k, v
+
+
+# ---- attention: a step's work is one launch of the split form for the sequences with one new token, one for those with a
+# few, and the prompt form for those with many
+
+# Rows (new tokens x query heads of a kv head) of a sequence of drafted tokens above which they take the prompt form (bfloat16).  By
+# the sequence's own rows, so that its bits do not depend on the step; a prompt's portions take it whatever their rows.
+PROMPT_ROWS = 32
+# Bytes of bfloat16 pages that a launch of the prompt form makes of its sequences' keys and values, one sequence at least.
+PAGES_BYTES = 1 << 30
+PAGE = 128
+
+
+def _split_fits(d: int, page_size: int) -> bool:
+    """Shapes that the split form takes: four keys lie in one page, their block scales on 8 bytes."""
+    return d <= 128 and d % 32 == 0 and page_size >= 4 and page_size & (page_size - 1) == 0
+
+
+def _most_runs(kv_len: int) -> int:
+    """The most runs of a sequence of at most ``kv_len`` keys, whatever its rows (the lengths on the device may be less than the
+    host's)."""
+    keys = _ops()._lib("attention_fp4").dib_fp4_attention_split_keys
+    return max(1, max(-(-n // keys(n, 1)) for n in (min(kv_len, 4096), kv_len)))
+
+
+class _SplitPart:
+    """The sequences of one launch: their number, the most rows of one, rows a tile, the most work items of one."""
+
+    def __init__(self, seqs: list, q_lens: list, kv_lens: list, group: int, hkv: int, device):
+        self.first, self.count, self.list = seqs[0], len(seqs), None
+        if seqs != list(range(seqs[0], seqs[0] + len(seqs))):
+            self.list = torch.tensor(seqs, dtype=torch.int32).to(device, non_blocking=True)
+        self.list_pointer = _pointer(self.list)
+        self.max_rows = max(q_lens[s] for s in seqs) * group
+        self.tile_rows = 8 if self.max_rows <= 8 else 16
+        runs, tiles = _most_runs(max(kv_lens[s] for s in seqs)), -(-self.max_rows // self.tile_rows)
+        # (runs get longer with the rows: tiles times runs is at most the tiles' number and twice that of the shortest runs)
+        self.items = hkv * min(tiles * runs, tiles + 2 * runs)
+        self.rows = self.count * self.items * self.tile_rows if runs > 1 else 0
+
+
+class _PromptPart:
+    """The sequences of one launch of the prompt form: the pages that hold their keys and values in bfloat16, and what the
+    attention over them needs to know of the step."""
+
+    def __init__(self, seqs: list, q_lens: list, kv_lens: list, meta, device):
+        pages = [-(-max(kv_lens[s], 1) // PAGE) for s in seqs]
+        first = [0]
+        for n in pages:
+            first.append(first[-1] + n)
+        self.count, self.most, self.pages = len(seqs), max(pages), first[-1]
+        b = len(q_lens)
+        table = torch.zeros(b, self.most, dtype=torch.int32)
+        for s, at, n in zip(seqs, first, pages):
+            table[s, :n] = torch.arange(at, at + n, dtype=torch.int32)
+        chosen = set(seqs)
+        own = [n if s in chosen else 0 for s, n in enumerate(q_lens)]
+        ints = torch.cat([torch.tensor(seqs + first, dtype=torch.int32), table.flatten(),
+                          torch.tensor([s in chosen for s in range(b)], dtype=torch.int32)]).to(device, non_blocking=True)
+        self.ints, n = ints, len(seqs)
+        self.seqs, self.first = ints[:n].data_ptr(), ints[n:2 * n + 1].data_ptr()
+        # The attention adds up the chunks of long rows of every token that has some: those of other sequences must not, so
+        # their lengths are 0 there.
+        self.mask = None if len(chosen) == b else ints[2 * n + 1 + b * self.most:]
+        self.meta = SimpleNamespace(block_table=ints[2 * n + 1:2 * n + 1 + b * self.most].view(b, self.most), q_lens=own,
+                                    kv_lens=[n if s in chosen else 0 for s, n in enumerate(kv_lens)], num_decode=0, scratch={})
+
+
+def _parts(meta, group: int, hkv: int, d: int, page_size: int, wide: bool, portions: bool, device) -> list:
+    """The step's launches: the sequences with one new token, those with a few, those of the prompt form (bfloat16: all others
+    that are portions of prompts, or those with many drafted tokens)."""
+    key = ("fp4", group, hkv, d, page_size, wide, portions)
+    parts = meta.scratch.get(key)
+    if parts is None:
+        from . import attention_bf16
+        q_lens, kv_lens = list(meta.q_lens), [max(a, b) for a, b in zip(meta.q_lens, meta.kv_lens)]
+        if not len(q_lens) == len(meta.kv_lens) <= meta.block_table.shape[0]:
+            raise _ops().KernelError(f"fp4_paged_attention: {len(q_lens)} q_lens and {len(meta.kv_lens)} kv_lens for a block table "
+                                     f"of {meta.block_table.shape[0]} sequences")
+        prompts = not wide and attention_bf16.supports(group * hkv, hkv, d, PAGE)
+        one = [s for s, n in enumerate(q_lens) if n == 1]
+        many = [s for s, n in enumerate(q_lens) if n > 1 and prompts and (portions or n * group > PROMPT_ROWS)]
+        few = sorted({s for s, n in enumerate(q_lens) if n > 1} - set(many))
+        parts, some, used = [], [], 0
+        room = max(1, PAGES_BYTES // (4 * hkv * PAGE * d))
+        for s in many:
+            n = -(-kv_lens[s] // PAGE)
+            if some and used + n > room:
+                parts.append(_PromptPart(some, q_lens, kv_lens, meta, device))
+                some, used = [], 0
+            some.append(s)
+            used += n
+        if some:
+            parts.append(_PromptPart(some, q_lens, kv_lens, meta, device))
+        parts += [_SplitPart(x, q_lens, kv_lens, group, hkv, device) for x in (one, few) if x]
+        meta.scratch[key] = parts
+    return parts
+
+
+def _prompt(q, out, cache: Fp4Cache, meta, part: _PromptPart, scale: float, window: int, stream: int) -> None:
+    from . import attention_bf16
+    pages, _, hkv, page_size, d = cache.shape
+    held = torch.empty(part.pages, 2, hkv, PAGE, d, dtype=torch.bfloat16, device=q.device)
+    own = part.meta
+    own.cu_q_lens, own.token_seq = meta.cu_q_lens, meta.token_seq
+    own.seq_lens = meta.seq_lens
+    if part.mask is not None and max(own.kv_lens) > attention_bf16.CHUNK_TILES * PAGE:
+        own.seq_lens = meta.seq_lens[:len(own.q_lens)] * part.mask
+    st = _fn("dib_fp4_unpack_pages")(*cache._pointers(), pages, meta.block_table.data_ptr(), meta.block_table.shape[1],
+                                     meta.cu_q_lens.data_ptr(), meta.seq_lens.data_ptr(), part.seqs, part.first, part.count, part.most,
+                                     held.data_ptr(), hkv, d, page_size, window, stream)
+    _done(st, "fp4_paged_attention", lambda: f"head_dim {d}, kv heads {hkv}, {part.pages} pages")
+    attention_bf16.run(q, out, held, own, scale, window)
+
+
+def _split(q, out, cache: Fp4Cache, meta, part: _SplitPart, scale: float, window: int, stream: int) -> None:
+    pages, _, hkv, page_size, d = cache.shape
+    hq, rows = q.shape[1], part.rows
+    held = torch.empty(rows * 130, dtype=torch.float32, device=q.device) if rows else None      # sums, (reference, sum)
+    partial = _pointer(held)
+    st = _fn("dib_fp4_attention_split")(
+        q.data_ptr(), out.data_ptr(), *cache._pointers(), pages, meta.block_table.data_ptr(), meta.block_table.shape[1],
+        meta.cu_q_lens.data_ptr(), meta.seq_lens.data_ptr(), part.list_pointer, part.first, part.count, part.max_rows, part.tile_rows,
+        partial, partial + rows * 512, part.items, 1 if rows else 0, hq, hkv, d, page_size, scale, window, _ops()._DT[q.dtype],
+        _sms(q.device), stream)
+    _done(st, "fp4_paged_attention", lambda: f"head_dim {d}, heads {hq}/{hkv}, {part.count} sequences", 2 if rows else 1)
+
+
+def _require_entries(t, name: str, n: int) -> None:
+    _require(t, name, torch.int32, 1)
+    if t.shape[0] < n:
+        raise _ops().KernelError(f"fp4_paged_attention: {name} has {t.shape[0]} entries, the step needs {n}")
+
+
+def fp4_paged_attention(q: torch.Tensor, cache: Fp4Cache, meta, scale: float, window=None,
+                        portions: bool = False) -> torch.Tensor:
+    """Causal attention of every token of the step over its sequence's keys in the cache, as ``ops.paged_attention``: q
+    [T, Hq, D] float32 or bfloat16, ``meta`` the step's ``AttentionMeta``.  A sequence's new tokens are its last ones
+    (``seq_lens`` counts them); each sees the keys up to its own position, the last ``window`` of them if given.  Keys and
+    values enter the products as what their codes and block scales stand for, exactly; the rows' powers of two join scores and
+    probabilities in float32.  A token that sees no key gives zeros.
+
+    ``portions``: the sequences with more than one new token bring portions of prompts.  In bfloat16 they then all take one
+    form, which makes bfloat16 pages of their keys and values and runs the prompt attention of the unquantised cache over
+    them.  Otherwise they count as drafted tokens, few of which are faster in another form, chosen by their number."""
+    ops = _ops()
+    if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dim() == 3 and q.is_contiguous()):
+        ops._need(q, "q", None, 3)
+    if not isinstance(cache, Fp4Cache):
+        raise ops.KernelError("fp4_paged_attention: cache must be an Fp4Cache")
+    code = _code(q.dtype, "q")
+    t, hq, d = q.shape
+    pages, _, hkv, page_size, d2 = cache.shape
+    if d2 != d or hq < 1 or hq % hkv:
+        raise ops.KernelError(f"fp4_paged_attention: q {tuple(q.shape)} vs cache {tuple(cache.shape)}")
+    table, token_seq, cu, lens = meta.block_table, meta.token_seq, meta.cu_q_lens, meta.seq_lens
+    _require(table, "block_table", torch.int32, 2)
+    b = table.shape[0]
+    _require_entries(token_seq, "token_seq", t)
+    _require_entries(cu, "cu_q_lens", b + 1)
+    _require_entries(lens, "seq_lens", b)
+    win = int(window) if window else 0
+    if win < 0:
+        raise ops.KernelError(f"fp4_paged_attention: a window of {win} keys")
+    device = cache.device
+    if q.device != device or table.device != device or token_seq.device != device or cu.device != device or lens.device != device:
+        _same_device("fp4_paged_attention", cache.data, q, table, token_seq, cu, lens)
+    out = torch.empty_like(q)
+    if t == 0:
+        return out
+    stream = _stream("fp4_paged_attention", device)
+    if _split_fits(d, page_size) and q.data_ptr() % 16 == 0 and cache.scales.data_ptr() % 8 == 0 and cache.exponents.data_ptr() % 4 == 0 \
+            and pages * 2 * hkv * page_size < 1 << 31:
+        for part in _parts(meta, hq // hkv, hkv, d, page_size, code == 0, bool(portions), device):
+            run = _prompt if isinstance(part, _PromptPart) else _split
+            run(q, out, cache, meta, part, float(scale), win, stream)
+        return out
+    st = _fn("dib_fp4_attention_any")(
+        q.data_ptr(), out.data_ptr(), *cache._pointers(), table.data_ptr(), table.shape[1], token_seq.data_ptr(), cu.data_ptr(),
+        lens.data_ptr(), t, hq, hkv, d, page_size, pages, float(scale), win, code, stream)
+    _done(st, "fp4_paged_attention", lambda: f"head_dim {d}, heads {hq}/{hkv}")
+    return out

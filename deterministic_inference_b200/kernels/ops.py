@@ -2092,8 +2092,9 @@ def masked_attention(q: torch.Tensor, kv_cache: torch.Tensor, meta, scale: float
     return out
 
 
-# ---------------------------------------------------------------- 8-bit integers
+# ---------------------------------------------------------------- 8-bit integers, 4-bit floating point
 
+from .fp4 import (Fp4Cache, Fp4Rows, Fp4Weight, fp4_cache_read, fp4_cache_write, fp4_linear,  # noqa: E402,F401
+                  fp4_paged_attention, fp4_qk_norm_rope_cache, fp4_quantize_rows)
 from .int8 import (Int8Cache, Int8Rows, Int8Weight, int8_cache_read, int8_cache_write, int8_linear,  # noqa: E402,F401
                    int8_paged_attention, int8_qk_norm_rope_cache, quantize_rows)
-from .fp4 import Fp4Rows, Fp4Weight, fp4_linear, fp4_quantize_rows  # noqa: E402,F401
