@@ -8,17 +8,9 @@
 // Forms: split (one new token, a few drafted ones, every float32 portion: the cache is streamed once) and one for every shape.
 // bfloat16 portions of prompts read the keys and values as bfloat16 pages (cache_fp4.cu) in the prompt attention of the
 // unquantised cache.
-#include "fp4.cuh"
+#include "attention_fp4.cuh"
 
 namespace {
-
-constexpr float LOG2E = 1.4426950408889634f;
-__device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // ---------------------------------------------------------------- split form
 // A sequence's rows (new token, query head of the kv group), ROWS = 8 NT at a time, against a run of its keys, by a CTA of four
@@ -45,107 +37,6 @@ constexpr int SP_WARPS = 4, SP_THREADS = 32 * SP_WARPS, SP_STEP = 32, SP_STAGES 
 constexpr int SP_K = 0, SP_V = SP_STEP * 64, SP_KS = 2 * SP_V, SP_VS = SP_KS + SP_STEP * 8, SP_KE = SP_VS + SP_STEP * 8,
               SP_VE = SP_KE + SP_STEP, SP_STAGE = SP_VE + SP_STEP;      // bytes of a step: codes, block scales, exponents
 constexpr int SP_ROW = 132;                                             // floats of a row's sums in shared memory: no two share banks
-constexpr float UNSET = -1e30f, RAISE = 5.f, LIFT = 10.f;
-
-// Keys of a run.
-__host__ __device__ __forceinline__ int split_keys(int kv_len, int rows) {
-  const int base = kv_len <= 4096 ? 256 : 512;
-  const int tiles = (rows + 15) / 16;
-  return tiles <= 2 ? base : base * ((tiles + 1) / 2);
-}
-
-struct SplitArgs {
-  const unsigned char* data;
-  const unsigned char* scales;
-  const unsigned char* exponents;
-  const int* block_table;       // [B, max_blocks]
-  const int* cu_q_lens;
-  const int* seq_lens;
-  const int* seq_list;          // the sequences of this launch, or null: seq_first ..
-  int seq_first, seq_count, max_blocks;
-  int Hq, Hkv, D, page_shift, window, num_pages;
-  float scale;
-  float* part_o;                // [seq_count, max_items, ROWS, 128]: sums, in the order of the registers
-  float2* part_ml;              // [seq_count, max_items, ROWS]: reference (log 2), sum
-  int max_items;
-};
-// A sequence of the launch and how it is cut.
-struct SplitSeq {
-  int seq, q_begin, n, kv_len, tiles, split, splits;
-  __device__ __forceinline__ long long items(int Hkv) const { return (long long)tiles * splits * Hkv; }
-  // what an item takes, in steps of a CTA, one for its beginning and end among them
-  __device__ __forceinline__ int item_work() const { return (min(split, kv_len) + SP_STEP * SP_WARPS - 1) / (SP_STEP * SP_WARPS) + 1; }
-};
-template <int ROWS> __device__ __forceinline__ SplitSeq split_seq(const SplitArgs& a, int i) {
-  SplitSeq s;
-  s.seq = a.seq_list != nullptr ? a.seq_list[i] : a.seq_first + i;
-  s.q_begin = a.cu_q_lens[s.seq];
-  s.n = a.cu_q_lens[s.seq + 1] - s.q_begin;
-  s.kv_len = max((int)min((long long)a.seq_lens[s.seq], min((long long)a.max_blocks << a.page_shift, 0x7fffff00ll)), 0);
-  const int rows = s.n * (a.Hq / a.Hkv);
-  s.tiles = (rows + ROWS - 1) / ROWS;
-  s.split = split_keys(s.kv_len, rows);
-  s.splits = s.n > 0 ? max(1, (s.kv_len + s.split - 1) / s.split) : 0;
-  return s;
-}
-
-__device__ __forceinline__ void cp_async16(unsigned to, const void* from, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async8(unsigned to, const void* from, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async4(unsigned to, const void* from, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// the four bytes of a word, two codes each, as pairs of float16
-__device__ __forceinline__ void codes_to_half(unsigned w, unsigned (&h)[4]) {
-  asm("{\n\t"
-      ".reg .b8 b0, b1, b2, b3;\n\t"
-      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t"
-      "}" : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
-}
-__device__ __forceinline__ unsigned scales_to_half(unsigned two) {
-  unsigned r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)two));
-  return r;
-}
-__device__ __forceinline__ unsigned mul_half(unsigned a, unsigned b) {
-  unsigned r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ unsigned pack_half(float lo, float hi) {
-  unsigned r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float2 unpack_half(unsigned two) {
-  float2 r;
-  asm("{ .reg .b16 l, h; mov.b32 {l, h}, %2; cvt.f32.f16 %0, l; cvt.f32.f16 %1, h; }" : "=f"(r.x), "=f"(r.y) : "r"(two));
-  return r;
-}
-__device__ __forceinline__ unsigned transposed(unsigned m) {
-  unsigned r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(m));
-  return r;
-}
-__device__ __forceinline__ void mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// the dimension that place p of a row's sums in the order of the registers stands for
-__device__ __forceinline__ int dim_of(int p) { return ((p & 15) >> 1) * 16 + (p >> 4) * 2 + (p & 1); }
-
 template <typename T> __device__ __forceinline__ float4 load_four(const T* p);
 template <> __device__ __forceinline__ float4 load_four<float>(const float* p) { return *reinterpret_cast<const float4*>(p); }
 template <> __device__ __forceinline__ float4 load_four<__nv_bfloat16>(const __nv_bfloat16* p) {
@@ -153,12 +44,6 @@ template <> __device__ __forceinline__ float4 load_four<__nv_bfloat16>(const __n
   return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
                      __uint_as_float(v.y & 0xffff0000u));
 }
-template <typename T> __device__ __forceinline__ void store_two(T* p, float x, float y);
-template <> __device__ __forceinline__ void store_two<float>(float* p, float x, float y) { *reinterpret_cast<float2*>(p) = make_float2(x, y); }
-template <> __device__ __forceinline__ void store_two<__nv_bfloat16>(__nv_bfloat16* p, float x, float y) {
-  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(x, y);
-}
-
 template <typename T, int NT> struct SplitShape {
   static constexpr int ROWS = 8 * NT, Q_PARTS = sizeof(T) == 4 ? 3 : 1, P_PARTS = sizeof(T) == 4 ? 2 : 1;
   static constexpr int CTAS = sizeof(T) == 4 ? 2 : NT == 1 ? 4 : 3;
@@ -554,90 +439,6 @@ attention_split_kernel(const T* __restrict__ q, T* __restrict__ out, const __gri
   }
 }
 
-// The runs' results of a row: out = sum_r 2^(M_r - top) O_r / sum_r 2^(M_r - top) l_r.  A block a row: warp w takes the
-// runs w, w + 4, ... in their order, a lane 4 places of the sums; the four warps' sums are added in the order of the warps.
-constexpr int SM_WARPS = 4;
-template <typename T, int ROWS>
-__global__ void __launch_bounds__(SM_WARPS * 32)
-attention_split_merge_kernel(T* __restrict__ out, const __grid_constant__ SplitArgs a) {
-  const float* part_o = a.part_o;
-  const float2* part_ml = a.part_ml;
-  __shared__ float4 s_o[SM_WARPS][32];
-  __shared__ float s_top[SM_WARPS], s_sum[SM_WARPS];
-  pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int i = blockIdx.y, G = a.Hq / a.Hkv;
-  const SplitSeq s = split_seq<ROWS>(a, i);
-  const int n_rows = s.n * G, id = blockIdx.x;     // rows of a kv head
-  // (every block waits, the one without work too: a grid none of whose blocks has waited ends ahead of the attention, and the
-  // kernel that follows takes this one's end for the attention's)
-  if (s.splits <= 1 || id >= n_rows * a.Hkv || s.items(a.Hkv) > a.max_items) {
-    pdl_wait();
-    return;
-  }
-  const int kvh = id / n_rows, row = id - kvh * n_rows, tile = row / ROWS, r = row % ROWS;
-  const int p0 = s.kv_len - s.n;
-  const int tok0 = tile * ROWS / G, tok1 = min((tile + 1) * ROWS - 1, n_rows - 1) / G;
-  // the runs that hold keys which some row of the tile sees
-  const int k_lo = first_visible_key(p0 + tok0, a.window), k_hi = p0 + tok1;
-  const int s0 = k_lo / s.split, s1 = k_hi < k_lo ? s0 - 1 : min(k_hi / s.split, s.splits - 1);
-  const long long base = ((long long)i * a.max_items + (long long)(kvh * s.tiles + tile) * s.splits) * ROWS + r;
-  pdl_wait(part_o, part_ml);
-  float top = UNSET;
-  for (int run = s0 + (int)threadIdx.x; run <= s1; run += SM_WARPS * 32) top = fmaxf(top, part_ml[base + (long long)run * ROWS].x);
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
-  constexpr int AHEAD = 8;
-  // the first results are on their way while the references are compared
-  float4 v[AHEAD];
-  float2 ml[AHEAD];
-  auto load = [&](int from) {
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      const int run = from + u * SM_WARPS;
-      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      ml[u] = make_float2(-INFINITY, 0.f);
-      if (run <= s1) {
-        const long long at = base + (long long)run * ROWS;
-        ml[u] = part_ml[at];
-        v[u] = *reinterpret_cast<const float4*>(part_o + at * 128 + lane * 4);
-      }
-    }
-  };
-  load(s0 + warp);
-  top = warp_max(top);
-  if (lane == 0) s_top[warp] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-  for (int from = s0 + warp; from <= s1; from += AHEAD * SM_WARPS) {
-    if (from != s0 + warp) load(from);
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      const float w = fast_exp2(ml[u].x - top);
-      sum = fmaf(w, ml[u].y, sum);
-      o.x = fmaf(w, v[u].x, o.x); o.y = fmaf(w, v[u].y, o.y);
-      o.z = fmaf(w, v[u].z, o.z); o.w = fmaf(w, v[u].w, o.w);
-    }
-  }
-  s_o[warp][lane] = o;
-  if (lane == 0) s_sum[warp] = sum;
-  __syncthreads();
-  if (warp != 0) return;
-  float4 y = s_o[0][lane];
-  sum = s_sum[0];
-#pragma unroll
-  for (int k = 1; k < SM_WARPS; ++k) {
-    const float4 z = s_o[k][lane];
-    y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
-    sum += s_sum[k];
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int tok = row / G, d0 = dim_of(lane * 4), d1 = dim_of(lane * 4 + 2);
-  T* dst = out + ((long long)(s.q_begin + tok) * a.Hq + kvh * G + row - tok * G) * a.D;
-  if (d0 < a.D) store_two<T>(dst + d0, y.x * inv, y.y * inv);
-  if (d1 < a.D) store_two<T>(dst + d1, y.z * inv, y.w * inv);
-}
-
 // ---------------------------------------------------------------- the form for every shape
 // Head sizes up to 256, any page size and group ratio: a warp takes a (token, head), a lane a key of 32 at a time for
 // the scores, then a lane D / 32 dimensions for the values.  Bound by a warp's chain over the keys.
@@ -744,22 +545,6 @@ int launch_split(const void* q, void* out, const SplitArgs& a, int max_rows, int
     DIB_CHECK_LAUNCH();
   }
   return DIB_OK;
-}
-
-SplitArgs cache_args(const void* data, const void* scales, const void* exponents, long long num_pages, const void* block_table,
-                     int max_blocks, const void* cu_q_lens, const void* seq_lens, int Hq, int Hkv, int D, float scale, int window) {
-  SplitArgs a = {};
-  a.data = reinterpret_cast<const unsigned char*>(data);
-  a.scales = reinterpret_cast<const unsigned char*>(scales);
-  a.exponents = reinterpret_cast<const unsigned char*>(exponents);
-  a.block_table = reinterpret_cast<const int*>(block_table);
-  a.cu_q_lens = reinterpret_cast<const int*>(cu_q_lens);
-  a.seq_lens = reinterpret_cast<const int*>(seq_lens);
-  a.max_blocks = max_blocks;
-  a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.window = window;
-  a.num_pages = (int)num_pages;
-  a.scale = scale;
-  return a;
 }
 
 }  // namespace

@@ -183,13 +183,18 @@ __device__ __forceinline__ void tc_ld32(unsigned taddr, unsigned (&r)[32]) {
         "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
+// Waits for tc_ld8 and tc_ld32, whose registers are handed on here: arithmetic on them must not be moved ahead of the wait.
+template <int N> __device__ __forceinline__ void tc_wait_ld(unsigned (&v)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(v[i]));
+}
 // 8 consecutive columns of this thread's lane; valid after tc_wait_ld()
 __device__ __forceinline__ void tc_ld8(unsigned taddr, unsigned (&r)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(taddr));
 }
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // K-major rows of 128 bytes, 128-byte swizzle: 8-row groups 1,024 bytes apart
 __device__ __forceinline__ unsigned long long operand_desc(unsigned addr) {
   return (unsigned long long)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((unsigned long long)(1024u >> 4) << 32) | (1ull << 46) |
@@ -485,7 +490,7 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         for (int h = 0; h < COLS; h += 32) {
           unsigned v[32];
           tc_ld32(src + buf * BN + h, v);
-          tc_wait_ld();
+          tc_wait_ld(v);
 #pragma unroll
           for (int j = 0; j < 32; ++j) acc[h + j] += __uint_as_float(v[j]);
         }
@@ -644,7 +649,7 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       for (int col = 0; col < a.cols; col += 8) {
         unsigned v[8];
         tc_ld8(tmem + ((unsigned)(quarter * 32) << 16) + col, v);
-        tc_wait_ld();
+        tc_wait_ld(v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) to[(col + j) * (SUM_ROW / 4)] = __uint_as_float(v[j]);
       }

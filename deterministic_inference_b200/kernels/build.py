@@ -57,6 +57,7 @@ SOURCES = {
     "gemm_fp4": "gemm_fp4.cu",
     "cache_fp4": "cache_fp4.cu",
     "attention_fp4": "attention_fp4.cu",
+    "attention_fp4_stream": "attention_fp4_stream.cu",
 }
 HEADERS = ("common.cuh", "attention_merge.cuh")
 # further headers a library includes
@@ -77,7 +78,8 @@ EXTRA_HEADERS = {
     "gemm_fp4": ("fp4.cuh",),
     "cache_int8": ("cache_rows.cuh",),
     "cache_fp4": ("cache_rows.cuh", "fp4.cuh"),
-    "attention_fp4": ("fp4.cuh",),
+    "attention_fp4": ("fp4.cuh", "attention_fp4.cuh"),
+    "attention_fp4_stream": ("fp4.cuh", "attention_fp4.cuh"),
 }
 
 NVCC_FLAGS = [

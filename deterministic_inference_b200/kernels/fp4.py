@@ -50,6 +50,8 @@ _SIGNATURES = {
     "dib_fp4_unpack_pages": ("cache_fp4", (_P, _P, _P, _L, _P, _I, _P, _P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _P)),
     "dib_fp4_attention_split": ("attention_fp4", (_P, _P, _P, _P, _P, _L, _P, _I, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _I, _I,
                                                   _I, _I, _F, _I, _I, _I, _P)),
+    "dib_fp4_attention_stream": ("attention_fp4_stream", (_P, _P, _P, _P, _P, _L, _P, _I, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _I,
+                                                          _I, _I, _I, _F, _I, _I, _I, _P)),
     "dib_fp4_attention_any": ("attention_fp4", (_P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _L, _F, _I, _I, _P)),
 }
 _functions: dict = {}
@@ -448,13 +450,14 @@ def _most_runs(kv_len: int) -> int:
 class _SplitPart:
     """The sequences of one launch: their number, the most rows of one, rows a tile, the most work items of one."""
 
-    def __init__(self, seqs: list, q_lens: list, kv_lens: list, group: int, hkv: int, device):
+    def __init__(self, seqs: list, q_lens: list, kv_lens: list, group: int, hkv: int, stream: bool, device):
+        self.form = "dib_fp4_attention_stream" if stream else "dib_fp4_attention_split"
         self.first, self.count, self.list = seqs[0], len(seqs), None
         if seqs != list(range(seqs[0], seqs[0] + len(seqs))):
             self.list = torch.tensor(seqs, dtype=torch.int32).to(device, non_blocking=True)
         self.list_pointer = _pointer(self.list)
         self.max_rows = max(q_lens[s] for s in seqs) * group
-        self.tile_rows = 8 if self.max_rows <= 8 else 16
+        self.tile_rows = 4 if stream and self.max_rows <= 4 else 8 if self.max_rows <= 8 else 16
         runs, tiles = _most_runs(max(kv_lens[s] for s in seqs)), -(-self.max_rows // self.tile_rows)
         # (runs get longer with the rows: tiles times runs is at most the tiles' number and twice that of the shortest runs)
         self.items = hkv * min(tiles * runs, tiles + 2 * runs)
@@ -488,10 +491,10 @@ class _PromptPart:
                                     kv_lens=[n if s in chosen else 0 for s, n in enumerate(kv_lens)], num_decode=0, scratch={})
 
 
-def _parts(meta, group: int, hkv: int, d: int, page_size: int, wide: bool, portions: bool, device) -> list:
+def _parts(meta, group: int, hkv: int, d: int, page_size: int, wide: bool, stream: bool, portions: bool, device) -> list:
     """The step's launches: the sequences with one new token, those with a few, those of the prompt form (bfloat16: all others
     that are portions of prompts, or those with many drafted tokens)."""
-    key = ("fp4", group, hkv, d, page_size, wide, portions)
+    key = ("fp4", group, hkv, d, page_size, wide, stream, portions)
     parts = meta.scratch.get(key)
     if parts is None:
         from . import attention_bf16
@@ -514,7 +517,7 @@ def _parts(meta, group: int, hkv: int, d: int, page_size: int, wide: bool, porti
             used += n
         if some:
             parts.append(_PromptPart(some, q_lens, kv_lens, meta, device))
-        parts += [_SplitPart(x, q_lens, kv_lens, group, hkv, device) for x in (one, few) if x]
+        parts += [_SplitPart(x, q_lens, kv_lens, group, hkv, stream, device) for x in (one, few) if x]
         meta.scratch[key] = parts
     return parts
 
@@ -540,7 +543,7 @@ def _split(q, out, cache: Fp4Cache, meta, part: _SplitPart, scale: float, window
     hq, rows = q.shape[1], part.rows
     held = torch.empty(rows * 130, dtype=torch.float32, device=q.device) if rows else None      # sums, (reference, sum)
     partial = _pointer(held)
-    st = _fn("dib_fp4_attention_split")(
+    st = _fn(part.form)(
         q.data_ptr(), out.data_ptr(), *cache._pointers(), pages, meta.block_table.data_ptr(), meta.block_table.shape[1],
         meta.cu_q_lens.data_ptr(), meta.seq_lens.data_ptr(), part.list_pointer, part.first, part.count, part.max_rows, part.tile_rows,
         partial, partial + rows * 512, part.items, 1 if rows else 0, hq, hkv, d, page_size, scale, window, _ops()._DT[q.dtype],
@@ -593,7 +596,9 @@ def fp4_paged_attention(q: torch.Tensor, cache: Fp4Cache, meta, scale: float, wi
     stream = _stream("fp4_paged_attention", device)
     if _split_fits(d, page_size) and q.data_ptr() % 16 == 0 and cache.scales.data_ptr() % 8 == 0 and cache.exponents.data_ptr() % 4 == 0 \
             and pages * 2 * hkv * page_size < 1 << 31:
-        for part in _parts(meta, hq // hkv, hkv, d, page_size, code == 0, bool(portions), device):
+        # (scores on the cache's codes as they are: bfloat16 queries, heads that are whole steps of 64 values)
+        stream_form = code == 1 and d % 64 == 0 and cache.scales.data_ptr() % 16 == 0
+        for part in _parts(meta, hq // hkv, hkv, d, page_size, code == 0, stream_form, bool(portions), device):
             run = _prompt if isinstance(part, _PromptPart) else _split
             run(q, out, cache, meta, part, float(scale), win, stream)
         return out

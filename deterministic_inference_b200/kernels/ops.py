@@ -113,6 +113,7 @@ _STATUS_FUNCTIONS = {
     "attention_int8_prompt": ("dib_attention_int8_prompt_status", "dib_attention_int8_prompt_status_clear"),
     "gemm_int8": ("dib_gemm_int8_status", "dib_gemm_int8_status_clear"),
     "gemm_fp4": ("dib_gemm_fp4_status", "dib_gemm_fp4_status_clear"),
+    "attention_fp4_stream": ("dib_attention_fp4_status", "dib_attention_fp4_status_clear"),
 }
 _extra_status: dict = {}
 
