@@ -83,8 +83,9 @@ attention_split_kernel(const T* __restrict__ q, T* __restrict__ out, const __gri
   }
   __syncthreads();
   const long long total = first[a.seq_count];
-  const long long from_work = total / gridDim.x * blockIdx.x + total % gridDim.x * blockIdx.x / gridDim.x;
-  const long long to_work = total / gridDim.x * (blockIdx.x + 1) + total % gridDim.x * (blockIdx.x + 1) / gridDim.x;
+  const int place = block_place(a);
+  const long long from_work = total / gridDim.x * place + total % gridDim.x * place / gridDim.x;
+  const long long to_work = total / gridDim.x * (place + 1) + total % gridDim.x * (place + 1) / gridDim.x;
   int i = 0;
   for (int hi = a.seq_count - 1; i < hi;) {      // the sequence in which the range begins
     const int mid = (i + hi + 1) >> 1;
@@ -518,7 +519,7 @@ attention_any_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_
 
 // ---------------------------------------------------------------- host side
 template <typename T, int NT>
-int launch_split(const void* q, void* out, const SplitArgs& a, int max_rows, int merge, int sm_count, cudaStream_t st) {
+int launch_split(const void* q, void* out, SplitArgs a, int max_rows, int merge, int sm_count, cudaStream_t st) {
   using SH = SplitShape<T, NT>;
   auto kern = attention_split_kernel<T, NT>;
   const size_t smem = SH::FIRST + ((size_t)a.seq_count + 1) * 8;
@@ -534,6 +535,7 @@ int launch_split(const void* q, void* out, const SplitArgs& a, int max_rows, int
   }
   const int by_smem = (int)(228 * 1024 / (smem + 1024)), per_sm = by_smem < SH::CTAS ? by_smem : SH::CTAS;
   const long long most = (long long)a.max_items * a.seq_count, grid = (long long)sm_count * (per_sm < 1 ? 1 : per_sm);
+  a.sms = most >= grid ? sm_count : 0;
   dib_launch(kern, dim3((unsigned)(grid < most ? grid : most)), dim3(SP_THREADS), smem, st, reinterpret_cast<const T*>(q),
              reinterpret_cast<T*>(out), a);
   DIB_CHECK_LAUNCH();

@@ -20,7 +20,7 @@ constexpr int SP_TILE = 128;      // keys that a CTA works on at a time
 
 // Keys of a run.
 __host__ __device__ __forceinline__ int split_keys(int kv_len, int rows) {
-  const int base = kv_len <= 4096 ? 256 : 512;
+  const int base = kv_len <= 2048 ? 256 : 512;
   const int tiles = (rows + 15) / 16;
   return tiles <= 2 ? base : base * ((tiles + 1) / 2);
 }
@@ -39,7 +39,13 @@ struct SplitArgs {
   float* part_o;                // [seq_count, max_items, ROWS, 128]: sums, in the order of the registers
   float2* part_ml;              // [seq_count, max_items, ROWS]: reference (log 2), sum
   int max_items;
+  int sms;                      // blocks b, b + sms, ... of the grid lie on one SM as a rule; 0: fewer blocks than would fill the GPU
 };
+// The place of a block among the grid's, by which it takes its share of the work: those that share an SM follow one another, so
+// that their shares, each rounded to whole items, add up to about the same on every SM.
+__device__ __forceinline__ int block_place(const SplitArgs& a) {
+  return a.sms == 0 ? (int)blockIdx.x : (int)blockIdx.x % a.sms * ((int)gridDim.x / a.sms) + (int)blockIdx.x / a.sms;
+}
 // A sequence of the launch and how it is cut.
 struct SplitSeq {
   int seq, q_begin, n, kv_len, tiles, split, splits;

@@ -37,7 +37,7 @@ constexpr int ST_COPY_WARP = 4, ST_SCORE_WARP = 5, ST_WALK_WARP = 6;      // and
 // a stage: codes of keys and values (rows of 64 bytes, swizzled), block scales of keys (two tiles of 128 rows x 64 values, as the products
 // take them) and values (a row a key), exponents
 constexpr int ST_V = SP_TILE * 64, ST_KS = 2 * ST_V, ST_VS = ST_KS + 1024, ST_KE = ST_VS + SP_TILE * 8, ST_VE = ST_KE + SP_TILE,
-              ST_STAGE = (ST_VE + SP_TILE + 1023) / 1024 * 1024;
+              ST_STAGE = (ST_VE + SP_TILE + 511) / 512 * 512;
 
 __device__ __forceinline__ void mbar_init(unsigned long long* bar, int count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
@@ -144,33 +144,35 @@ struct __align__(16) StreamItem {
 };
 
 template <int ROWS> struct StreamShape {
-  static constexpr int STAGES = ROWS <= 4 ? 3 : 2;
+  static constexpr int STAGES = 2;
   static constexpr int NT = (ROWS + 7) / 8, N = ROWS * ST_PARTS;      // tiles of 8 rows, columns of the scores
   static constexpr int SFK = 2 * N, SFQ = SFK + 8, TMEM = SFQ + 8 <= 64 ? 64 : SFQ + 8 <= 128 ? 128 : 256;
-  static constexpr int QUERIES = STAGES * ST_STAGE;                // [2][N][64], swizzled
+  static constexpr int QUERIES = (STAGES * ST_STAGE + 1023) / 1024 * 1024;              // [2][N][64], swizzled
   static constexpr int QSCALES = QUERIES + 2 * N * 64;                // [2] two tiles of 512 bytes
   static constexpr int WEIGHTS = QSCALES + 2 * 1024;                  // [4 warps][NT][32 keys][8 rows] float16
   static constexpr int SUMS = WEIGHTS + 4 * NT * 512;                 // [4 warps][ROWS][132]
   static constexpr int TOPS = SUMS + 4 * ROWS * 132 * 4;              // [4 warps][ROWS] references
-  static constexpr int PARTS = TOPS + 4 * ROWS * 4;                   // [4 warps][ROWS][32 lanes] parts of the sums of weights
-  static constexpr int UNITS = PARTS + 4 * ROWS * 128;                // [2][ROWS] of the scores
+  static constexpr int PARTS = TOPS + 4 * ROWS * 4;                   // [4 warps][ROWS][16 lanes] parts of the sums of weights
+  static constexpr int UNITS = PARTS + 4 * ROWS * 64;                // [2][ROWS] of the scores
   static constexpr int SEEN = UNITS + 2 * ROWS * 4;                   // [2][2][ROWS] first and last key
   static constexpr int ITEMS = SEEN + 2 * 2 * ROWS * 4;
   static constexpr int BARS = ITEMS + ST_ITEMS * 64;
   static constexpr int SEQS = BARS + 32 * 8;                          // [sequences] int4, then the work before each
   static constexpr size_t fixed = SEQS + 16 + 1024;
-  // CTAs an SM; they are launched with 80 (128) registers a thread, and the groups' shares add up to twice that
-  static constexpr int CTAS = ROWS <= 8 ? 3 : 2, REGS_MANY = ROWS <= 8 ? 104 : 200, REGS_FEW = 56;
+  // CTAs an SM; they are launched with 64, 80 or 128 registers a thread, and the groups' shares add up to twice that
+  static constexpr int CTAS = ROWS <= 4 ? 4 : ROWS <= 8 ? 3 : 2;
+  static constexpr int REGS_MANY = ROWS <= 4 ? 88 : ROWS <= 8 ? 104 : 200, REGS_FEW = ROWS <= 4 ? 40 : 56;
 };
 
-template <int ROWS>
+template <int ROWS, int D>
 __global__ void __launch_bounds__(ST_THREADS, StreamShape<ROWS>::CTAS)
 attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out,
                         const __grid_constant__ SplitArgs a, const int box_rows, const int late) {
   using SH = StreamShape<ROWS>;
   constexpr int NT = SH::NT, N = SH::N;
   extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  // (an offset, not a rounded address: what is known to be shared memory is read and written with 32-bit addresses)
+  unsigned char* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
   StreamItem* items = reinterpret_cast<StreamItem*>(smem + SH::ITEMS);
   unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + SH::BARS);
   unsigned long long* full = bars;             // [3] a tile's keys, values, scales and exponents have arrived
@@ -247,7 +249,8 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
   regs_give<SH::REGS_FEW>();
   if (warp == ST_COPY_WARP) {
     // ---- copies: lane l has the keys 4l .. 4l + 3 of a tile; the first lane of each page sends for its rows
-    const int page_mask = (1 << a.page_shift) - 1, half = a.Hkv << a.page_shift, row_scales = a.D >> 4;      // half: rows of a page's keys
+    const int page_mask = (1 << a.page_shift) - 1, half = a.Hkv << a.page_shift;
+    constexpr int row_scales = D >> 4;      // half: rows of a page's keys
     int n = 0, stage = 0;
     unsigned phase = 1;      // (the ring's first round finds it empty)
     for (int k = 0; ok; ++k) {
@@ -304,7 +307,7 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
     // ---- scores: a tile ahead of the weights
     const unsigned elected = elect_one(), base = smem_u32(smem);
     constexpr unsigned idesc = make_idesc(128, N);
-    const int k_steps = a.D >> 6;
+    constexpr int k_steps = D >> 6;
     int n = 0, q_used = -1, stage = 0;
     unsigned phase = 0;
     for (int k = 0; ok; ++k) {
@@ -346,8 +349,9 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
   } else if (warp == ST_WALK_WARP) {
     // ---- the walk over this CTA's items, a contiguous range of equal work
     const long long total = first[a.seq_count];
-    const long long from_work = total / gridDim.x * blockIdx.x + total % gridDim.x * blockIdx.x / gridDim.x;
-    const long long to_work = total / gridDim.x * (blockIdx.x + 1) + total % gridDim.x * (blockIdx.x + 1) / gridDim.x;
+    const int place = block_place(a);
+    const long long from_work = total / gridDim.x * place + total % gridDim.x * place / gridDim.x;
+    const long long to_work = total / gridDim.x * (place + 1) + total % gridDim.x * (place + 1) / gridDim.x;
     int i = 0, old_i = -1, old_kvh = -1, old_tile = -1, item = 0;
     SplitSeq s = {};
     if (total > 0) {
@@ -389,9 +393,9 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         if (it.end <= it.seen) {
           if (s.splits == 1) {             // a sequence of one run: rows that see no key are zeros, from here
             const int rows = min(ROWS, s.n * G - it.tile * ROWS);
-            for (int e = lane; e < rows * a.D; e += 32) {
-              const int row = it.tile * ROWS + e / a.D, tok = row / G;
-              Elem<__nv_bfloat16>::store(out + ((long long)(s.q_begin + tok) * a.Hq + it.kvh * G + row - tok * G) * a.D + e % a.D, 0.f);
+            for (int e = lane; e < rows * D; e += 32) {
+              const int row = it.tile * ROWS + e / D, tok = row / G;
+              Elem<__nv_bfloat16>::store(out + ((long long)(s.q_begin + tok) * a.Hq + it.kvh * G + row - tok * G) * D + e % D, 0.f);
             }
           }
           continue;
@@ -444,7 +448,7 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         for (int x = 0; x < 4; ++x) {
           f[x] = fast_exp2(f[x] - top);
           const float4 v = *reinterpret_cast<const float4*>(sums + (x * ROWS + r) * 132 + lane * 4);
-          sum = fmaf(f[x], parts[(x * ROWS + r) * 32 + lane], sum);
+          if (lane < 16) sum = fmaf(f[x], parts[(x * ROWS + r) * 16 + lane], sum);
           y.x = fmaf(f[x], v.x, y.x); y.y = fmaf(f[x], v.y, y.y);
           y.z = fmaf(f[x], v.z, y.z); y.w = fmaf(f[x], v.w, y.w);
         }
@@ -452,9 +456,9 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         if (it.splits == 1) {
           const int tok = (row0 + r) / G;
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          __nv_bfloat16* dst = out + ((long long)(it.q_begin + tok) * a.Hq + it.kvh * G + row0 + r - tok * G) * a.D;
-          if (d0 < a.D) store_two<__nv_bfloat16>(dst + d0, y.x * inv, y.y * inv);
-          if (d1 < a.D) store_two<__nv_bfloat16>(dst + d1, y.z * inv, y.w * inv);
+          __nv_bfloat16* dst = out + ((long long)(it.q_begin + tok) * a.Hq + it.kvh * G + row0 + r - tok * G) * D;
+          if (d0 < D) store_two<__nv_bfloat16>(dst + d0, y.x * inv, y.y * inv);
+          if (d1 < D) store_two<__nv_bfloat16>(dst + d1, y.z * inv, y.w * inv);
         } else if (it.local < a.max_items) {
           const long long to = ((long long)it.i * a.max_items + it.local) * ROWS + r;
           *reinterpret_cast<float4*>(a.part_o + to * 128 + lane * 4) = y;
@@ -468,12 +472,13 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
   } else {
     regs_take<SH::REGS_MANY>();
     // ---- weights and outputs: thread = key of the warp's 32, then a block of dimensions and pairs of rows
-    const int g = lane >> 2, t = lane & 3, row_scales = a.D >> 4;
+    constexpr int row_scales = D >> 4;
+    const int g = lane >> 2, t = lane & 3;
     const unsigned tm = tmem + ((unsigned)(warp * 32) << 16);
     unsigned char* weights = smem + SH::WEIGHTS + warp * NT * 512;
     float* sums = reinterpret_cast<float*>(smem + SH::SUMS) + warp * ROWS * 132;
     float* tops = reinterpret_cast<float*>(smem + SH::TOPS) + warp * ROWS;
-    float* parts = reinterpret_cast<float*>(smem + SH::PARTS) + warp * ROWS * 32;
+    float* parts = reinterpret_cast<float*>(smem + SH::PARTS) + warp * ROWS * 16;
     int n = 0, q_used = -1, done = 0, stage = 0;
     unsigned phase = 0;
     for (int k = 0; ok; ++k) {
@@ -496,8 +501,8 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         for (int x = 0; x < (ROWS + 7) / 8; ++x) {
           const int r = x * 8 + warp * 2 + (lane >> 4), tok = (row0 + r) / G;
           raw[x] = make_uint4(0, 0, 0, 0);
-          if (r < rows && hl * 8 < a.D)
-            raw[x] = *reinterpret_cast<const uint4*>(q + ((long long)(it.q_begin + tok) * a.Hq + it.kvh * G + row0 + r - tok * G) * a.D + hl * 8);
+          if (r < rows && hl * 8 < D)
+            raw[x] = *reinterpret_cast<const uint4*>(q + ((long long)(it.q_begin + tok) * a.Hq + it.kvh * G + row0 + r - tok * G) * D + hl * 8);
         }
         if (q_used >= 2) ok = mbar_wait_brief(&q_empty[qbuf], ((q_used >> 1) - 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
@@ -716,7 +721,8 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
       if (!ok) break;
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
-        parts[r * 32 + lane] = l[r];
+        const float v = l[r] + __shfl_xor_sync(0xffffffffu, l[r], 16);
+        if (lane < 16) parts[r * 16 + lane] = v;
         if (lane == r) tops[r] = M[r];
       }
 #pragma unroll
@@ -771,11 +777,11 @@ bool make_cache_map(CUtensorMap* map, const void* data, long long rows, int D, i
              CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int ROWS>
-int launch_stream(const CUtensorMap& map, const void* q, void* out, const SplitArgs& a, int box_rows, int max_rows, int merge, int sm_count,
+template <int ROWS, int D>
+int launch_stream(const CUtensorMap& map, const void* q, void* out, SplitArgs a, int box_rows, int max_rows, int merge, int sm_count,
                   cudaStream_t st) {
   using SH = StreamShape<ROWS>;
-  auto kern = attention_stream_kernel<ROWS>;
+  auto kern = attention_stream_kernel<ROWS, D>;
   const size_t smem = SH::fixed + (size_t)a.seq_count * 24 + 8;
   constexpr int MOST = 200 * 1024;
   if (smem > MOST) return DIB_BAD_SIZE;
@@ -794,6 +800,7 @@ int launch_stream(const CUtensorMap& map, const void* q, void* out, const SplitA
   int per_sm = by_smem < SH::CTAS ? by_smem : SH::CTAS;
   per_sm = per_sm < 512 / SH::TMEM ? per_sm : 512 / SH::TMEM;
   const long long most = (long long)a.max_items * a.seq_count, grid = (long long)sm_count * (per_sm < 1 ? 1 : per_sm);
+  a.sms = most >= grid ? sm_count : 0;
   dib_launch(kern, dim3((unsigned)(grid < most ? grid : most)), dim3(ST_THREADS), smem, st, map, reinterpret_cast<const __nv_bfloat16*>(q),
              reinterpret_cast<__nv_bfloat16*>(out), a, box_rows, most >= grid ? 1 : 0);
   DIB_CHECK_LAUNCH();
@@ -847,9 +854,9 @@ int dib_fp4_attention_stream(const void* q, void* out, const void* data, const v
   const int box_rows = page_size < SP_TILE ? page_size : SP_TILE;
   CUtensorMap map;
   if (!make_cache_map(&map, data, num_pages * 2 * Hkv * page_size, D, box_rows)) return DIB_LAUNCH_FAILED;
-  if (tile_rows == 4) return launch_stream<4>(map, q, out, a, box_rows, max_rows, merge, sm_count, st);
-  if (tile_rows == 8) return launch_stream<8>(map, q, out, a, box_rows, max_rows, merge, sm_count, st);
-  return launch_stream<16>(map, q, out, a, box_rows, max_rows, merge, sm_count, st);
+  auto launch = D == 128 ? (tile_rows == 4 ? launch_stream<4, 128> : tile_rows == 8 ? launch_stream<8, 128> : launch_stream<16, 128>)
+                         : (tile_rows == 4 ? launch_stream<4, 64> : tile_rows == 8 ? launch_stream<8, 64> : launch_stream<16, 64>);
+  return launch(map, q, out, a, box_rows, max_rows, merge, sm_count, st);
 }
 
 }  // extern "C"

@@ -322,7 +322,8 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   __shared__ unsigned long long full[STAGES], empty[STAGES];
   __shared__ unsigned long long acc_full[2], acc_empty[2];      // a part's accumulator is complete; the epilogue has read it
   __shared__ unsigned tmem_slot;
-  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  // (an offset, not a rounded address: what is known to be shared memory is read and written with 32-bit addresses)
+  unsigned char* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
   unsigned char* epi_stage = smem + STAGES * STAGE;
   if (!PAIR) pdl_trigger();
   if (threadIdx.x == 0) {
@@ -550,7 +551,8 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   extern __shared__ unsigned char smem_raw[];
   __shared__ unsigned long long full[MAX_STAGES], empty[MAX_STAGES], acc_full;
   __shared__ unsigned tmem_slot;
-  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  // (an offset, not a rounded address: what is known to be shared memory is read and written with 32-bit addresses)
+  unsigned char* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
   // a stage: channels, scales of channels, of tokens, tokens
   constexpr int WS_AT = 128 * ROW_BYTES, XS_AT = WS_AT + SCALES, X_AT = XS_AT + SCALES;
   pdl_trigger();

@@ -444,7 +444,7 @@ def _most_runs(kv_len: int) -> int:
     """The most runs of a sequence of at most ``kv_len`` keys, whatever its rows (the lengths on the device may be less than the
     host's)."""
     keys = _ops()._lib("attention_fp4").dib_fp4_attention_split_keys
-    return max(1, max(-(-n // keys(n, 1)) for n in (min(kv_len, 4096), kv_len)))
+    return max(1, max(-(-n // keys(n, 1)) for n in (min(kv_len, 2048), kv_len)))
 
 
 class _SplitPart:
