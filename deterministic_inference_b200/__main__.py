@@ -109,8 +109,8 @@ def main(argv=None) -> int:
     g.add_argument("--preset", help="a named shape with random weights instead of a folder")
     g.add_argument("--random-seed", type=int, default=0)
     g.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
-    g.add_argument("--weight-dtype", choices=["int8"], help="the layers' matrices in 8 bits")
-    g.add_argument("--cache-dtype", choices=["int8"], help="keys and values in 8 bits")
+    g.add_argument("--weight-dtype", choices=["int8", "fp4"], help="the layers' matrices in 8 or 4 bits")
+    g.add_argument("--cache-dtype", choices=["int8", "fp4"], help="keys and values in 8 or 4 bits")
     g.add_argument("--prompt-ids", action="append", help='"1,2,3"; may be repeated')
     g.add_argument("--prompt-lens", help='"5,17,33": random prompts of these lengths')
     g.add_argument("--prompt-seed", type=int, default=1)

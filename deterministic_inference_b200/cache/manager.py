@@ -51,7 +51,7 @@ class CacheView:
     kv: Optional[torch.Tensor] = None            # [pages, 2, Hkv, page_size, D] of this cache; with
                                                  # values of another size than keys [pages, Hkv *
                                                  # page_size * (D + Dv)]: a page's keys, then its values;
-                                                 # in 8 bits an ``ops.Int8Cache``
+                                                 # in 8 or 4 bits an ``ops.Int8Cache`` or ``ops.Fp4Cache``
     page_size: int = 0
     slot_mapping: Optional[torch.Tensor] = None  # int32 [T]: page * page_size + offset
     attention_meta: object = None                # the group's AttentionMeta of this step
@@ -79,7 +79,7 @@ class PageGroup:
         # per slot: the pages before this index (the kept first ones aside) have been given back, so the
         # next look starts there instead of walking the released run again every step
         self.first_live: list[int] = [0] * max_reqs
-        self.pool = None               # a tensor of all the group's caches; in 8 bits a list, one ``ops.Int8Cache`` each
+        self.pool = None               # a tensor of all the group's caches; in 8 or 4 bits a list, one ``ops.Int8Cache`` or ``ops.Fp4Cache`` each
 
     @property
     def num_free(self) -> int:
@@ -146,7 +146,10 @@ def _element_size(dtype: torch.dtype) -> int:
 
 
 def _row_bytes(spec: PagedKVSpec, dtype: torch.dtype) -> int:
-    """Bytes of a token's key and value of one head (int8: with their float32 scales)."""
+    """Bytes of a token's key and value of one head (int8: with their float32 scales; in 4 bits: with the block scales and
+    exponents)."""
+    if dtype == torch.float4_e2m1fn_x2:
+        return sum(d // 2 + d // 16 + 1 for d in (spec.head_dim, spec.value_dim))
     return (spec.head_dim + spec.value_dim) * _element_size(dtype) + (8 if dtype == torch.int8 else 0)
 
 
@@ -204,7 +207,7 @@ class CacheManager:
                  allocate_device: bool = True):
         """``num_pages``: pages of every group's pool (page 0 included), or a dict from
         group key to the pages of that group (``pages_for_budget``).  ``dtype``: the pages' type;
-        torch.int8: pools of ``ops.Int8Cache``."""
+        torch.int8: pools of ``ops.Int8Cache``; torch.float4_e2m1fn_x2: of ``ops.Fp4Cache``."""
         self.page_size, self.max_reqs = int(page_size), int(max_reqs)
         self.max_seq_len = int(max_seq_len)
         self.max_blocks = -(-self.max_seq_len // self.page_size)
@@ -251,11 +254,12 @@ class CacheManager:
 
     def allocate_device_memory(self) -> None:
         for g in self.page_groups.values():
-            if self.dtype == torch.int8:
+            if self.dtype in (torch.int8, torch.float4_e2m1fn_x2):
                 if g.spec.value_dim != g.spec.head_dim:
-                    raise CacheError(f"group {g.key}: values of another size than keys have no pages in 8 bits")
+                    raise CacheError(f"group {g.key}: values of another size than keys have no pages in 8 or 4 bits")
                 from ..kernels import ops
-                g.pool = [ops.Int8Cache.zeros(g.num_pages, g.spec.num_kv_heads, g.page_size, g.spec.head_dim, self.device)
+                made = ops.Int8Cache if self.dtype == torch.int8 else ops.Fp4Cache
+                g.pool = [made.zeros(g.num_pages, g.spec.num_kv_heads, g.page_size, g.spec.head_dim, self.device)
                           for _ in g.cache_ids]
             elif g.spec.value_dim == g.spec.head_dim:
                 g.pool = torch.zeros(len(g.cache_ids), g.num_pages, 2, g.spec.num_kv_heads, g.page_size,

@@ -29,6 +29,9 @@ class EngineConfig:
     # half the memory, and half of the cached bytes that a decode step reads.  None: ``dtype``.  (A
     # decode step of qwen3_8b, 8 / 64 requests of 2,100 tokens: 3.92 / 7.73 ms in bfloat16, with 8-bit
     # weights 3.34 / 6.74, cache 3.99 / 6.92, both 2.97 / 5.26.)
+    # "fp4": the same in 4-bit floating point, with a scale for each 16 values and a power of two per output
+    # channel, token and head: products on the block-scaled tensor cores with sums in float32, 0.57 bytes a
+    # cached value.
     weight_dtype: Optional[str] = None
     cache_dtype: Optional[str] = None
 
@@ -76,8 +79,8 @@ class EngineConfig:
             raise ValueError(f"dtype must be one of {sorted(set(_DTYPES))}, got {self.dtype!r}")
         self.dtype = _DTYPES[self.dtype]
         for name in ("weight_dtype", "cache_dtype"):
-            if getattr(self, name) not in (None, "int8"):
-                raise ValueError(f"{name} must be None or 'int8', got {getattr(self, name)!r}")
+            if getattr(self, name) not in (None, "int8", "fp4"):
+                raise ValueError(f"{name} must be None, 'int8' or 'fp4', got {getattr(self, name)!r}")
         if self.model_path is None and self.model_config is None:
             raise ValueError("EngineConfig needs model_path (a folder) or model_config")
         if self.model_path is None and self.random_seed is None:

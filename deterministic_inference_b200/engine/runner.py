@@ -49,13 +49,13 @@ class ModelRunner:
             else:
                 tensors = random_tensors_on_device(specs, cfg.random_seed, self.dtype, self.device)
             self.model.load(tensors)
-            if cfg.weight_dtype == "int8":
+            if cfg.weight_dtype is not None:
                 del tensors
-                self.model.quantize_weights()
+                self.model.quantize_weights(cfg.weight_dtype)
         cache_dtype = self.dtype
-        if cfg.cache_dtype == "int8":
-            self.model.check_int8_cache()
-            cache_dtype = torch.int8
+        if cfg.cache_dtype is not None:
+            self.model.check_int8_cache(cfg.cache_dtype)
+            cache_dtype = torch.int8 if cfg.cache_dtype == "int8" else torch.float4_e2m1fn_x2
         self.max_positions = self.model.plan.max_positions
         if self.dtype == torch.bfloat16 and self.device.type == "cuda":
             from ..kernels import gemm_bf16

@@ -491,10 +491,10 @@ class _PromptPart:
                                     kv_lens=[n if s in chosen else 0 for s, n in enumerate(kv_lens)], num_decode=0, scratch={})
 
 
-def _parts(meta, group: int, hkv: int, d: int, page_size: int, wide: bool, stream: bool, portions: bool, device) -> list:
+def _parts(meta, group: int, hkv: int, d: int, page_size: int, prompts: bool, stream: bool, portions: bool, device) -> list:
     """The step's launches: the sequences with one new token, those with a few, those of the prompt form (bfloat16: all others
     that are portions of prompts, or those with many drafted tokens)."""
-    key = ("fp4", group, hkv, d, page_size, wide, stream, portions)
+    key = ("fp4", group, hkv, d, page_size, prompts, stream, portions)
     parts = meta.scratch.get(key)
     if parts is None:
         from . import attention_bf16
@@ -502,7 +502,7 @@ def _parts(meta, group: int, hkv: int, d: int, page_size: int, wide: bool, strea
         if not len(q_lens) == len(meta.kv_lens) <= meta.block_table.shape[0]:
             raise _ops().KernelError(f"fp4_paged_attention: {len(q_lens)} q_lens and {len(meta.kv_lens)} kv_lens for a block table "
                                      f"of {meta.block_table.shape[0]} sequences")
-        prompts = not wide and attention_bf16.supports(group * hkv, hkv, d, PAGE)
+        prompts = prompts and attention_bf16.supports(group * hkv, hkv, d, PAGE)
         one = [s for s, n in enumerate(q_lens) if n == 1]
         many = [s for s, n in enumerate(q_lens) if n > 1 and prompts and (portions or n * group > PROMPT_ROWS)]
         few = sorted({s for s, n in enumerate(q_lens) if n > 1} - set(many))
@@ -598,7 +598,8 @@ def fp4_paged_attention(q: torch.Tensor, cache: Fp4Cache, meta, scale: float, wi
             and pages * 2 * hkv * page_size < 1 << 31:
         # (scores on the cache's codes as they are: bfloat16 queries, heads that are whole steps of 64 values)
         stream_form = code == 1 and d % 64 == 0 and cache.scales.data_ptr() % 16 == 0
-        for part in _parts(meta, hq // hkv, hkv, d, page_size, code == 0, stream_form, bool(portions), device):
+        # (the prompt attention masks scores before it scales them)
+        for part in _parts(meta, hq // hkv, hkv, d, page_size, code == 1 and scale > 0, stream_form, bool(portions), device):
             run = _prompt if isinstance(part, _PromptPart) else _split
             run(q, out, cache, meta, part, float(scale), win, stream)
         return out

@@ -572,10 +572,11 @@ def qk_norm_rope_cache(qkv: torch.Tensor, num_heads: int, num_kv_heads: int, hea
     the paged cache [pages, 2, Hkv, page_size, D] (when a cache is given;
     slot = page * page_size + offset, negative = skip).  ``cos_sin``, ``positions`` and ``slot_mapping`` are the
     step's constants: no kernel of this package that is still running when this one is launched may write them.
-    ``kv_cache`` may be an ``Int8Cache``: ``int8_qk_norm_rope_cache``."""
-    if isinstance(kv_cache, Int8Cache):
-        return int8_qk_norm_rope_cache(qkv, num_heads, num_kv_heads, head_dim, q_norm_weight, k_norm_weight, eps, cos_sin,
-                                       positions, kv_cache, slot_mapping)
+    ``kv_cache`` may be an ``Int8Cache`` (``int8_qk_norm_rope_cache``) or an ``Fp4Cache`` (``fp4_qk_norm_rope_cache``)."""
+    if isinstance(kv_cache, (Int8Cache, Fp4Cache)):
+        write = int8_qk_norm_rope_cache if isinstance(kv_cache, Int8Cache) else fp4_qk_norm_rope_cache
+        return write(qkv, num_heads, num_kv_heads, head_dim, q_norm_weight, k_norm_weight, eps, cos_sin, positions, kv_cache,
+                     slot_mapping)
     parts = None
     if isinstance(qkv, SplitSum):
         if head_dim in (64, 128, 256) and (cos_sin is None or cos_sin.shape[1] == head_dim):
@@ -636,7 +637,8 @@ def qkv_project(x: torch.Tensor, w_qkv: torch.Tensor, num_heads: int, num_kv_hea
     the two kernels."""
     x = as_tensor(x)
     if x.dtype == torch.bfloat16 and x.is_cuda and head_dim == 128 and kv_cache is not None \
-            and not isinstance(kv_cache, Int8Cache) and not isinstance(w_qkv, Int8Weight) and (cos_sin is None or cos_sin.shape[1] == head_dim):
+            and not isinstance(kv_cache, (Int8Cache, Fp4Cache)) and not isinstance(w_qkv, (Int8Weight, Fp4Weight)) \
+            and (cos_sin is None or cos_sin.shape[1] == head_dim):
         from . import gemm_bf16
         q = gemm_bf16.qkv_large(x, w_qkv, num_heads, num_kv_heads, q_norm_weight, k_norm_weight, eps,
                                 cos_sin, positions, kv_cache, slot_mapping, page_size)
@@ -651,6 +653,8 @@ def reshape_and_cache(k: torch.Tensor, v: torch.Tensor, kv_cache: torch.Tensor,
     """k, v [T, Hkv, D] into their slots of the paged cache (negative slot: skip)."""
     if isinstance(kv_cache, Int8Cache):
         return int8_cache_write(k, v, kv_cache, slot_mapping)
+    if isinstance(kv_cache, Fp4Cache):
+        return fp4_cache_write(k, v, kv_cache, slot_mapping)
     _need(k, "k", None, 3)
     _need(v, "v", k.dtype, 3)
     _need(kv_cache, "kv_cache", k.dtype, 5)
@@ -677,9 +681,11 @@ def paged_attention(q: torch.Tensor, kv_cache: torch.Tensor, meta, scale: float,
     sequences).  A query at position p sees keys max(0, p-window+1) .. p.
     ``defer``: a step of one-token sequences only may come back as a ``SplitAttention``
     (its splits not yet merged) for the matrix product that follows to merge.  ``kv_cache`` may be an
-    ``Int8Cache``: ``int8_paged_attention`` of portions of prompts."""
+    ``Int8Cache`` or an ``Fp4Cache``: ``int8_paged_attention`` or ``fp4_paged_attention`` of portions of prompts."""
     if isinstance(kv_cache, Int8Cache):
         return int8_paged_attention(q, kv_cache, meta, scale, window, portions=True)
+    if isinstance(kv_cache, Fp4Cache):
+        return fp4_paged_attention(q, kv_cache, meta, scale, window, portions=True)
     _need(q, "q", None, 3)
     _need(kv_cache, "kv_cache", q.dtype, 5)
     t, hq, d = q.shape
@@ -758,9 +764,12 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out_dtype=None) -> torch.Tenso
     accumulation on the tensor cores, and ``weight`` is a constant: a kernel of this package that is still running
     when the product is launched must not write it; ``out_dtype=torch.float32`` returns the
     accumulator unrounded (used for the logits).  With few rows and a split of k the
-    bfloat16 product comes back as a ``SplitSum`` (see there).  ``weight`` may be an ``Int8Weight``: ``int8_linear``."""
+    bfloat16 product comes back as a ``SplitSum`` (see there).  ``weight`` may be an ``Int8Weight``
+    or an ``Fp4Weight``: ``int8_linear``, ``fp4_linear``."""
     if isinstance(weight, Int8Weight):
         return int8_linear(x, weight, out_dtype)
+    if isinstance(weight, Fp4Weight):
+        return fp4_linear(x, weight, out_dtype)
     if isinstance(x, (GatedSplit, SplitAttention)) and weight.dtype == torch.bfloat16 \
             and tuple(x.shape)[1] == weight.shape[1]:
         from . import gemm_bf16
@@ -794,6 +803,8 @@ def gated_linear(x: torch.Tensor, w_gate_up: torch.Tensor):
     x = as_tensor(x)
     if isinstance(w_gate_up, Int8Weight):
         return silu_mul(int8_linear(x, w_gate_up))
+    if isinstance(w_gate_up, Fp4Weight):
+        return silu_mul(fp4_linear(x, w_gate_up))
     if x.dtype == torch.bfloat16 and x.is_cuda:
         _need(x, "x", None, 2)
         _need(w_gate_up, "w_gate_up", x.dtype, 2)

@@ -81,20 +81,20 @@ class DecoderModel:
             else:
                 part.load(tensors)
 
-    def quantize_weights(self) -> None:
-        """After ``load``: the layers' matrices in 8 bits (the embedding, the head and the norms stay as they are)."""
+    def quantize_weights(self, weight_dtype: str = "int8") -> None:
+        """After ``load``: the layers' matrices in 8 or 4 bits (the embedding, the head and the norms stay as they are)."""
         for b in self.blocks:
             for part in (b.mixer, b.feed_forward):
                 if not part.int8_weights and any(s.role == "matrix" for s in part.tensor_specs()):
-                    raise ValueError(f"weight_dtype 'int8': {type(part).__name__} has no products in 8 bits")
-                part.quantize_weights()
+                    raise ValueError(f"weight_dtype {weight_dtype!r}: {type(part).__name__} has no products in few bits")
+                part.quantize_weights(weight_dtype)
 
     # ---- caches ---------------------------------------------------------------
 
-    def check_int8_cache(self) -> None:
+    def check_int8_cache(self, cache_dtype: str = "int8") -> None:
         for m in self.mixers:
             if m.cache_spec() is not None and not m.int8_cache:
-                raise ValueError(f"cache_dtype 'int8': {type(m).__name__} does not read a cache in 8 bits")
+                raise ValueError(f"cache_dtype {cache_dtype!r}: {type(m).__name__} does not read a cache in few bits")
 
 
     def cache_specs(self) -> dict[int, object]:

@@ -36,7 +36,7 @@ from .spec import TensorSpec
 
 class Part:
     kind = "?"
-    # attributes that hold a weight [out, in] whose products may run in 8-bit integers
+    # attributes that hold a weight [out, in] whose products may run in 8-bit integers or 4-bit floating point
     int8_weights: tuple = ()
 
     def tensor_specs(self) -> list[TensorSpec]:
@@ -45,11 +45,12 @@ class Part:
     def load(self, tensors: dict[str, torch.Tensor]) -> None:
         pass
 
-    def quantize_weights(self) -> None:
-        """After ``load``: the weights named in ``int8_weights`` in 8 bits."""
+    def quantize_weights(self, weight_dtype: str = "int8") -> None:
+        """After ``load``: the weights named in ``int8_weights`` in 8 bits, or ("fp4") in 4."""
         from ..kernels import ops
+        made = ops.Fp4Weight if weight_dtype == "fp4" else ops.Int8Weight
         for name in self.int8_weights:
-            setattr(self, name, ops.Int8Weight.of(getattr(self, name)))
+            setattr(self, name, made.of(getattr(self, name)))
 
 
 class TokenEmbedding(Part):
@@ -88,7 +89,7 @@ class PositionEncoding(Part):
 
 
 class Mixer(Part):
-    int8_cache = False       # whether it takes its pages as an ``ops.Int8Cache``
+    int8_cache = False       # whether it takes its pages as an ``ops.Int8Cache`` or ``ops.Fp4Cache``
 
     def cache_spec(self):
         return None
