@@ -801,6 +801,9 @@ template <typename OutT, int BN, bool PAIR> int launch_form(const Operands& o, c
   return DIB_OK;
 }
 
+// CTAs that share an SM, by shared memory
+int few_per_sm(int cols) { return cols <= 32 ? 3 : 2; }
+
 template <typename OutT> int launch_few(const Operands& o, cudaStream_t st) {
   const int row_bytes = (o.K + 31) / 32 * 16, k_tiles = fp4_k_tiles(o.K);
   const Parts k(k_tiles / 4);
@@ -814,8 +817,8 @@ template <typename OutT> int launch_few(const Operands& o, cudaStream_t st) {
   a.tmem = a.cols + 32 <= 64 ? 64 : a.cols + 32 <= 128 ? 128 : 256;
   a.by_values = o.N % 4 != 0 || reinterpret_cast<uintptr_t>(o.out) % (4 * sizeof(OutT)) != 0;
   const int stage = few_stage(a.cols), parts = k.parts, longest = k.each + (k.longer > 0);
-  // three CTAs an SM, or two (228 KB, 1 KB of each block's own and 1 KB for its barriers)
-  const int per_sm = a.cols <= 32 ? 3 : 2;
+  // (228 KB an SM, 1 KB of each block's own and 1 KB for its barriers)
+  const int per_sm = few_per_sm(a.cols);
   a.stages = (228 * 1024 / per_sm - 3 * 1024) / stage;
   if (a.stages > longest) a.stages = longest;
   if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
@@ -844,30 +847,47 @@ int& forced_form() {
   static int v = -1;
   return v;
 }
-// Few rows, or the form in which the busiest SM fetches the fewest bytes: rounds of tiles times the bytes of a stage.  (The form
-// never changes a bit of the result.)
-int form(int M, int N, int sm_count) {
+// Of the forms the one whose time, in us, is estimated lowest, from lines through measured times (148 SMs, stages of 256 values):
+//   tiles      each round of tiles takes its stages; 4,096 x 4,096, 256 rows: 128 x 64 9.1, 128 x 128 9.8, 128 x 192 12.0, pair 13.8;
+//              2,048 rows: 34.4, 25.6, 24.9, 26.1; 24,576 x 4,096: 182, 120, 107, 101; 128 rows of it, bound by the weight: 18.2,
+//              18.2, 17.3
+//   clusters   8, 32, 64, 128 rows of 4,096 x 4,096 5.4, 6.4, 7.6, 10.3; of 4,096 x 12,288 8.2, 8.7, 10.4, 13.0; of 24,576 x 4,096
+//              11.6, 13.2, 20.6, 25.8; of 1,024 x 1,024 3.8, 5.1, 6.9, 10.5 (128 x 64: 4.4, 4.5, 4.6, 4.8)
+// (The form never changes a bit of the result.)
+int form(int M, int N, int K, int sm_count) {
   if (forced_form() >= 0 && (forced_form() < 4 || M <= FEW_TOKENS)) return forced_form();
-  if (M <= FEW_TOKENS) return 4;
-  long long best = 1ll << 62;
+  const int num_kb = fp4_k_tiles(K) / 4;
+  const float weight = 0.5625f * (float)N * (float)K;      // bytes
+  float best = 1e30f;
   int choice = 0;
-  auto consider = [&](int form, int bm, int bn, int ctas, int bytes) {
-    const long long tiles = (long long)((M + bm - 1) / bm) * ((N + bn - 1) / bn), at_once = sm_count / ctas;
-    const long long cost = (tiles + at_once - 1) / at_once * bytes;
-    if (cost <= best) {
-      best = cost;
+  auto consider = [&](int form, float us) {
+    if (us < best) {
+      best = us;
       choice = form;
     }
   };
-  consider(0, BM, 64, 1, Shape<64, false>::STAGE);
-  consider(1, BM, 128, 1, Shape<128, false>::STAGE);
-  consider(2, BM, 192, 1, Shape<192, false>::STAGE);
-  if (sm_count >= 2) consider(3, 2 * BM, 192, 2, Shape<192, true>::STAGE);
+  auto tiles = [&](int form, int bm, int bn, int ctas, float base, float stage) {
+    const long long n = (long long)((M + bm - 1) / bm) * ((N + bn - 1) / bn), at_once = sm_count / ctas;
+    const float run = stage * (float)((n + at_once - 1) / at_once) * (float)num_kb, read = weight / 4.6e6f;
+    const float busy = (float)(n < at_once ? n : at_once) / (float)at_once;
+    consider(form, base + 1.2f * busy + (run > read ? run : read));
+  };
+  tiles(0, BM, 64, 1, 2.8f, 0.28f);
+  tiles(1, BM, 128, 1, 3.4f, 0.325f);
+  tiles(2, BM, 192, 1, 4.f, 0.445f);
+  if (M > BM && sm_count >= 2) tiles(3, 2 * BM, 192, 2, 7.f, 0.4f);
+  if (M <= FEW_TOKENS) {
+    const Parts k(num_kb);
+    const int cols = (M + 7) / 8 * 8;
+    const float at_once = (float)(sm_count * few_per_sm(cols)), n = (float)((N + 127) / 128) * (float)k.parts;
+    consider(4, (2.9f + 0.2f * (float)(k.each + (k.longer > 0)) + weight / 7.9e6f) * (n > at_once ? n / at_once : 1.f) +
+                    (float)(cols - 8) * (0.02f + 0.036f / (float)k.parts));
+  }
   return choice;
 }
 
 template <typename OutT> int launch(const Operands& o, cudaStream_t st) {
-  switch (form(o.M, o.N, o.sm_count)) {
+  switch (form(o.M, o.N, o.K, o.sm_count)) {
     case 0: return launch_form<OutT, 64, false>(o, st);
     case 1: return launch_form<OutT, 128, false>(o, st);
     case 2: return launch_form<OutT, 192, false>(o, st);
