@@ -5,7 +5,10 @@
 // Cache: data [pages, 2, Hkv, page_size, D / 2] (two codes a byte, the first in the low half), scales e4m3
 // [pages, 2, Hkv, page_size, D / 16], exponents [pages, 2, Hkv, page_size] (E + 127).  128 values take 73 bytes.
 //
-// A lane has a block of 16 values: 32 (64) bytes of the unquantised row, 8 bytes of codes, a scale.  Bound by memory.
+// A lane has a block of 16 values: 32 (64) bytes of the unquantised row, 8 bytes of codes, a scale; of bfloat16 rows two such.  float32
+// rows are bound by memory (8,000 tokens of 8 heads of 128 written in 14.7 us, 5.1 TB/s; read in 13.2, 5.7 TB/s; a floor of
+// 11.4 at 6.55 TB/s), bfloat16 ones by what a row takes beside its values, its place, largest value and three outputs (10.1 us,
+// 4.2 TB/s; read in 8.7; a floor of 6.4).
 #include "cache_rows.cuh"
 #include "fp4.cuh"
 
@@ -18,32 +21,91 @@ struct Cache4 {
   unsigned char* exponents;
 };
 
-// LANES: 8 for rows up to 128, 16 up to 256
-template <typename T, bool WIDE, int LANES>
+// A block of threads has one head's keys or values of PER consecutive tokens, so that what a page holds of them side by side is
+// written and read side by side.
+struct Place {
+  long long at;      // row of the cache, or -1
+  int token;
+};
+struct BlockOf {
+  int kv, h, token0;
+};
+__device__ __forceinline__ BlockOf block_of(int per, const CacheShape& s) {
+  BlockOf b;
+  const unsigned t = quotient(blockIdx.x, s.per_token), rest = blockIdx.x - t * s.per_token.d;
+  b.kv = rest >= (unsigned)s.Hkv;
+  b.h = (int)rest - b.kv * s.Hkv;
+  b.token0 = (int)t * per;
+  return b;
+}
+__device__ __forceinline__ Place place(const BlockOf& b, int token, int tokens, const CacheShape& s, const int* slots) {
+  Place c;
+  c.at = -1;
+  c.token = token;
+  if (token >= tokens) return c;
+  const int slot = slots[token];
+  if (slot < 0) return c;
+  const unsigned page = quotient((unsigned)slot, s.page);
+  if (page < s.num_pages)
+    c.at = ((long long)page * s.per_token.d + b.kv * s.Hkv + b.h) * s.page.d + (slot - (int)(page * s.page.d));
+  return c;
+}
+
+// A lane has BLOCKS blocks of 16 side by side; ROWS rows a group, all asked for before the first is used.
+template <typename T, bool WIDE, int LANES, int BLOCKS, int ROWS>
 __global__ void __launch_bounds__(CACHE_THREADS)
 cache_write_kernel(const T* __restrict__ k, const T* __restrict__ v, long long k_stride, long long v_stride,
-                   const __grid_constant__ Cache4 cache, const int* __restrict__ slots, const __grid_constant__ CacheShape s) {
+                   const __grid_constant__ Cache4 cache, const int* __restrict__ slots, int tokens, const __grid_constant__ CacheShape s) {
+  constexpr int GROUPS = CACHE_THREADS / LANES;
   pdl_prologue(k, v, slots);
-  const int l = threadIdx.x & (LANES - 1);
-  const CacheRow c = cache_row(blockIdx.x * (CACHE_THREADS / LANES) + threadIdx.x / LANES, s, slots);
-  const T* src = (c.kv ? v + c.token * v_stride : k + c.token * k_stride) + c.h * s.D;
-  Block16<T> x;
-  x.template load<WIDE>(src, c.at >= 0 ? l * 16 : s.D, s.D);
-  const unsigned own = x.top();
-  unsigned top = own;
+  const int d = (threadIdx.x & (LANES - 1)) * BLOCKS * 16;
+  const BlockOf b = block_of(GROUPS * ROWS, s);
+  const T* from = (b.kv ? v : k) + b.h * s.D;
+  const long long stride = b.kv ? v_stride : k_stride;
+  Place c[ROWS];
+  Block16<T> x[ROWS][BLOCKS];
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (c.at < 0 || l * 16 >= s.D) return;
-  const unsigned exponent = fp4_row_exponent(top);
-  const float down = fp4_down(exponent);
-  const unsigned scale = fp4_block_scale(own, down);
-  const Fp4Scaler q = fp4_scaler(scale, down);
-  float y[16];
+  for (int g = 0; g < ROWS; ++g) c[g] = place(b, b.token0 + g * GROUPS + threadIdx.x / LANES, tokens, s, slots);
 #pragma unroll
-  for (int e = 0; e < 16; ++e) y[e] = x.get(e);
-  *reinterpret_cast<uint2*>(cache.data + c.at * (s.D / 2) + l * 8) = make_uint2(fp4_codes8(y, q), fp4_codes8(y + 8, q));
-  cache.scales[c.at * (s.D / 16) + l] = (unsigned char)scale;
-  if (l == 0) cache.exponents[c.at] = (unsigned char)exponent;
+  for (int g = 0; g < ROWS; ++g)
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i) x[g][i].template load<WIDE>(from + c[g].token * stride, c[g].at >= 0 ? d + i * 16 : s.D, s.D);
+#pragma unroll
+  for (int g = 0; g < ROWS; ++g) {
+    unsigned own[BLOCKS], top = 0;
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i) {
+      own[i] = x[g][i].top();
+      top = max(top, own[i]);
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (c[g].at < 0 || d >= s.D) continue;
+    const unsigned exponent = fp4_row_exponent(top);
+    const float down = fp4_down(exponent);
+    unsigned w[2 * BLOCKS], scales = 0;
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i) {
+      const unsigned scale = fp4_block_scale(own[i], down);
+      const Fp4Scaler q = fp4_scaler(scale, down);
+      float y[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) y[e] = x[g][i].get(e);
+      w[2 * i] = fp4_codes8(y, q);
+      w[2 * i + 1] = fp4_codes8(y + 8, q);
+      scales |= scale << (8 * i);
+    }
+    unsigned char* codes = cache.data + c[g].at * (s.D / 2) + d / 2;
+    unsigned char* tile = cache.scales + c[g].at * (s.D / 16) + d / 16;
+    if (BLOCKS == 2) {
+      *reinterpret_cast<uint4*>(codes) = make_uint4(w[0], w[1], w[2 * BLOCKS - 2], w[2 * BLOCKS - 1]);
+      *reinterpret_cast<unsigned short*>(tile) = (unsigned short)scales;
+    } else {
+      *reinterpret_cast<uint2*>(codes) = make_uint2(w[0], w[1]);
+      *tile = (unsigned char)scales;
+    }
+    if (d == 0) cache.exponents[c[g].at] = (unsigned char)exponent;
+  }
 }
 
 // a block of 16 of the row at `at` as numbers; zeros for a row that is not there
@@ -68,28 +130,46 @@ struct Held16 {
   }
 };
 
-// ROWS rows a group, all asked for before the first is used
-template <typename T, int LANES, int ROWS>
+// As above.
+template <typename T, int LANES, int BLOCKS, int ROWS>
 __global__ void __launch_bounds__(CACHE_THREADS)
 cache_read_kernel(const __grid_constant__ Cache4 cache, const int* __restrict__ slots, T* __restrict__ k, T* __restrict__ v,
-                  const __grid_constant__ CacheShape s) {
+                  int tokens, const __grid_constant__ CacheShape s) {
   constexpr int GROUPS = CACHE_THREADS / LANES;
   Cache4 held = cache;
   pdl_prologue(held.data, held.scales, held.exponents, slots);
-  const int l = threadIdx.x & (LANES - 1);
-  const unsigned r0 = blockIdx.x * (GROUPS * ROWS) + threadIdx.x / LANES;
-  CacheRow c[ROWS];
-  Held16 x[ROWS];
+  const int d = (threadIdx.x & (LANES - 1)) * BLOCKS * 16;
+  const BlockOf b = block_of(GROUPS * ROWS, s);
+  T* to = (b.kv ? v : k) + b.h * s.D + d;
+  Place c[ROWS];
+  Held16 x[ROWS][BLOCKS];
 #pragma unroll
-  for (int g = 0; g < ROWS; ++g) c[g] = cache_row(r0 + g * GROUPS, s, slots);
-#pragma unroll
-  for (int g = 0; g < ROWS; ++g) x[g].load(held, c[g].at, l, s.D);
+  for (int g = 0; g < ROWS; ++g) c[g] = place(b, b.token0 + g * GROUPS + threadIdx.x / LANES, tokens, s, slots);
 #pragma unroll
   for (int g = 0; g < ROWS; ++g) {
-    if (r0 + g * GROUPS >= s.rows || l * 16 >= s.D) return;
-    float y[16];
-    x[g].values(y);
-    store16((c[g].kv ? v : k) + ((long long)c[g].token * s.Hkv + c[g].h) * s.D + l * 16, y);
+    if (BLOCKS == 2) {
+      uint4 w = make_uint4(0, 0, 0, 0);
+      unsigned scales = 0, exponent = 0;
+      if (c[g].at >= 0 && d < s.D) {
+        w = *reinterpret_cast<const uint4*>(held.data + c[g].at * (s.D / 2) + d / 2);
+        scales = *reinterpret_cast<const unsigned short*>(held.scales + c[g].at * (s.D / 16) + d / 16);
+        exponent = held.exponents[c[g].at];
+      }
+      x[g][0] = {make_uint2(w.x, w.y), scales & 255, exponent};
+      x[g][BLOCKS - 1] = {make_uint2(w.z, w.w), scales >> 8, exponent};
+    } else {
+      x[g][0].load(held, c[g].at, d / 16, s.D);
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < ROWS; ++g) {
+    if (c[g].token >= tokens || d >= s.D) return;
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i) {
+      float y[16];
+      x[g][i].values(y);
+      store16(to + (long long)c[g].token * s.Hkv * s.D + i * 16, y);
+    }
   }
 }
 
@@ -208,26 +288,41 @@ unpack_pages_kernel(const __grid_constant__ UnpackArgs a) {
   }
 }
 
+// Two blocks of 16 a lane: bfloat16, rows and scales that allow it.  (8,000 tokens of 8 heads of 128 written, read: 10.1, 8.7 us, with one
+// 11.3, 9.2; float32 15.8, 17.4 with two and 14.7, 13.2 with one, then two rows a lane for reading.)
+template <typename T> bool two_blocks(const Cache4& cache, int D) {
+  return sizeof(T) == 2 && (D & 31) == 0 && (reinterpret_cast<uintptr_t>(cache.scales) & 1) == 0;
+}
+
 template <typename T>
 int launch_write(const void* k, const void* v, long long k_stride, long long v_stride, const Cache4& cache, const int* slots,
-                 const CacheShape& s, cudaStream_t st) {
+                 int tokens, const CacheShape& s, cudaStream_t st) {
   const bool wide = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 31) == 0 &&
                     (k_stride * sizeof(T)) % 32 == 0 && (v_stride * sizeof(T)) % 32 == 0;
-  const int groups = CACHE_THREADS / (s.D > 128 ? 16 : 8);
-  auto kern = s.D > 128 ? (wide ? cache_write_kernel<T, true, 16> : cache_write_kernel<T, false, 16>)
-                        : (wide ? cache_write_kernel<T, true, 8> : cache_write_kernel<T, false, 8>);
-  dib_launch(kern, dim3((s.rows + groups - 1) / groups), dim3(CACHE_THREADS), 0, st, reinterpret_cast<const T*>(k),
-             reinterpret_cast<const T*>(v), k_stride, v_stride, cache, slots, s);
+  const bool two = two_blocks<T>(cache, s.D);
+  const int per = CACHE_THREADS / ((s.D > 128 ? 16 : 8) >> two);
+  constexpr int TWO = sizeof(T) == 2 ? 2 : 1, NARROW = 8 / TWO, BROAD = 16 / TWO;
+  auto kern = two          ? s.D > 128 ? wide ? cache_write_kernel<T, true, BROAD, TWO, 1> : cache_write_kernel<T, false, BROAD, TWO, 1>
+                             : wide    ? cache_write_kernel<T, true, NARROW, TWO, 1>
+                                       : cache_write_kernel<T, false, NARROW, TWO, 1>
+              : s.D > 128  ? wide ? cache_write_kernel<T, true, 16, 1, 1> : cache_write_kernel<T, false, 16, 1, 1>
+              : wide       ? cache_write_kernel<T, true, 8, 1, 1>
+                           : cache_write_kernel<T, false, 8, 1, 1>;
+  dib_launch(kern, dim3((unsigned)((tokens + per - 1) / per) * 2u * s.Hkv), dim3(CACHE_THREADS), 0, st, reinterpret_cast<const T*>(k),
+             reinterpret_cast<const T*>(v), k_stride, v_stride, cache, slots, tokens, s);
   DIB_CHECK_LAUNCH();
   return DIB_OK;
 }
 template <typename T>
-int launch_read(const Cache4& cache, const int* slots, void* k, void* v, const CacheShape& s, cudaStream_t st) {
+int launch_read(const Cache4& cache, const int* slots, void* k, void* v, int tokens, const CacheShape& s, cudaStream_t st) {
   if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 31) != 0) return DIB_BAD_ALIGN;
-  constexpr int ROWS = 2;
-  const int per = CACHE_THREADS / (s.D > 128 ? 16 : 8) * ROWS;
-  dib_launch(s.D > 128 ? cache_read_kernel<T, 16, ROWS> : cache_read_kernel<T, 8, ROWS>, dim3((s.rows + per - 1) / per),
-             dim3(CACHE_THREADS), 0, st, cache, slots, reinterpret_cast<T*>(k), reinterpret_cast<T*>(v), s);
+  const bool two = two_blocks<T>(cache, s.D);
+  constexpr int TWO = sizeof(T) == 2 ? 2 : 1, ROWS = sizeof(T) == 2 ? 1 : 2;
+  const int per = CACHE_THREADS / ((s.D > 128 ? 16 : 8) >> two) * ROWS;
+  auto kern = two ? s.D > 128 ? cache_read_kernel<T, 16 / TWO, TWO, ROWS> : cache_read_kernel<T, 8 / TWO, TWO, ROWS>
+                  : s.D > 128 ? cache_read_kernel<T, 16, 1, ROWS> : cache_read_kernel<T, 8, 1, ROWS>;
+  dib_launch(kern, dim3((unsigned)((tokens + per - 1) / per) * 2u * s.Hkv), dim3(CACHE_THREADS), 0, st, cache, slots,
+             reinterpret_cast<T*>(k), reinterpret_cast<T*>(v), tokens, s);
   DIB_CHECK_LAUNCH();
   return DIB_OK;
 }
@@ -258,8 +353,8 @@ int dib_fp4_cache_write(const void* k, const void* v, long long k_stride, long l
   const CacheShape shape = make_shape((long long)T * 2 * Hkv, Hkv, D, page_size, num_pages);
   const Cache4 cache = make_cache(data, scales, exponents);
   const int* sl = reinterpret_cast<const int*>(slots);
-  if (dtype == 1) return launch_write<__nv_bfloat16>(k, v, k_stride, v_stride, cache, sl, shape, st);
-  return launch_write<float>(k, v, k_stride, v_stride, cache, sl, shape, st);
+  if (dtype == 1) return launch_write<__nv_bfloat16>(k, v, k_stride, v_stride, cache, sl, T, shape, st);
+  return launch_write<float>(k, v, k_stride, v_stride, cache, sl, T, shape, st);
 }
 
 // qkv [T, (Hq + 2 Hkv) D] -> q_out [T, Hq, D] and the cache; q_norm_w, k_norm_w float32 [D] or null; cos_sin float32
@@ -303,8 +398,8 @@ int dib_fp4_cache_read(const void* data, const void* scales, const void* exponen
   const CacheShape shape = make_shape((long long)T * 2 * Hkv, Hkv, D, page_size, num_pages);
   const Cache4 cache = make_cache(data, scales, exponents);
   const int* sl = reinterpret_cast<const int*>(slots);
-  if (dtype == 1) return launch_read<__nv_bfloat16>(cache, sl, k, v, shape, st);
-  return launch_read<float>(cache, sl, k, v, shape, st);
+  if (dtype == 1) return launch_read<__nv_bfloat16>(cache, sl, k, v, T, shape, st);
+  return launch_read<float>(cache, sl, k, v, T, shape, st);
 }
 
 int dib_fp4_unpack_page() { return UNPACK_PAGE; }

@@ -46,10 +46,15 @@ __device__ __forceinline__ float fp4_scale_value(unsigned code) {
   asm("{ .reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.f32.f16 %0, lo; }" : "=f"(y) : "r"(two));
   return y;
 }
+// x / d for a constant d, correctly rounded where x is not within 2^-24 of the smallest normal numbers
+__device__ __forceinline__ float fp4_divide(float x, float d, float inv) {
+  const float q = x * inv;
+  return fmaf(fmaf(-q, d, x), inv, q);
+}
 // The scale's code of a block whose largest |x| is `top` (finite, or down is 0).
 __device__ __forceinline__ unsigned fp4_block_scale(unsigned top, float down) {
   if (down == 0.f) return 0;
-  return fp4_scale_code(__fdiv_rn(__uint_as_float(top) * down, 6.f));
+  return fp4_scale_code(fp4_divide(__uint_as_float(top) * down, 6.f, 1.f / 6.f));
 }
 // Eight values' codes, the first in the lowest four bits.
 __device__ __forceinline__ unsigned fp4_pack8(const float* y) {
@@ -69,29 +74,36 @@ __device__ __forceinline__ unsigned fp4_pack4(const float* y) {
   const float x[8] = {y[0], y[1], y[2], y[3], 0.f, 0.f, 0.f, 0.f};
   return fp4_pack8(x) & 0xffffu;
 }
-// What the values of a block are multiplied with: 2^-E, and the block scale with its reciprocal (0 and 0: all codes are 0).
+// What the values of a block are divided by, 2^E b (2^-120 .. 448 * 2^117), and its reciprocal (0: all codes are 0).  Both are
+// exact multiples, by a power of two, of b and of b's rounded reciprocal: the division rounds as that of x 2^-E by b does.
 struct Fp4Scaler {
-  float down, b, inv;
+  float b, inv;
 };
 __device__ __forceinline__ Fp4Scaler fp4_scaler(unsigned scale_code, float down) {
   Fp4Scaler s;
-  s.b = fp4_scale_value(scale_code);
-  s.down = scale_code == 0 ? 0.f : down;
-  s.inv = scale_code == 0 ? 0.f : __frcp_rn(s.b);
+  const float b = fp4_scale_value(scale_code);
+  s.b = b * __uint_as_float(0x7f000000u - __float_as_uint(down));
+  s.inv = scale_code == 0 ? 0.f : __frcp_rn(b) * down;
   return s;
 }
-__device__ __forceinline__ float fp4_quotient(float x, const Fp4Scaler& s) {
-  const float u = x * s.down;                        // exact, or far below the smallest code
-  const float q = u * s.inv;
-  return fmaf(fmaf(-q, s.b, u), s.inv, q);
-}
-// Eight codes of values of one block.  (A block of zeros, and one of a row without finite numbers: codes of zero, whatever
-// 0 times an infinity makes.)
+__device__ __forceinline__ float fp4_quotient(float x, const Fp4Scaler& s) { return fp4_divide(x, s.b, s.inv); }
+// Eight codes of values of one block, two values a product.  (A block of zeros, and one of a row without finite numbers: codes of
+// zero, whatever 0 times an infinity makes.)
 __device__ __forceinline__ unsigned fp4_codes8(const float* x, const Fp4Scaler& s) {
   if (s.inv == 0.f) return 0;
   float y[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = fp4_quotient(x[i], s);
+  for (int i = 0; i < 8; i += 2)
+    asm("{\n\t"
+        ".reg .b64 x, b, v, q, r;\n\t"
+        "mov.b64 x, {%2, %3};\n\t"
+        "mov.b64 b, {%4, %4};\n\t"
+        "mov.b64 v, {%5, %5};\n\t"
+        "mul.rn.f32x2 q, x, v;\n\t"
+        "fma.rn.f32x2 r, q, b, x;\n\t"
+        "fma.rn.f32x2 q, r, v, q;\n\t"
+        "mov.b64 {%0, %1}, q;\n\t"
+        "}" : "=f"(y[i]), "=f"(y[i + 1]) : "f"(x[i]), "f"(x[i + 1]), "f"(-s.b), "f"(s.inv));
   return fp4_pack8(y);
 }
 // Eight codes as numbers, times `scale`.
@@ -144,6 +156,11 @@ template <typename T> struct Block16 {
   }
   __device__ __forceinline__ unsigned top() const {
     unsigned t = 0;
+    if (sizeof(T) == 2) {      // two at a time: as 16-bit integers magnitudes order like the numbers
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) asm("max.u16x2 %0, %0, %1;" : "+r"(t) : "r"(w[i] & 0x7fff7fffu));
+      return max(t << 16, t & 0xffff0000u);
+    }
 #pragma unroll
     for (int e = 0; e < 16; ++e) t = max(t, fp4_magnitude(get(e)));
     return t;

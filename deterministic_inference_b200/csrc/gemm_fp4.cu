@@ -930,13 +930,13 @@ int dib_gemm_fp4(const void* x, const void* xs, const void* ux, const void* w, c
 
 // The same with x [M, K] of values (x_dtype 0 float32, 1 bfloat16; rows `stride` values apart), which `quantize`
 // (dib_fp4_quantize_rows of the rows' library) first turns into tiles of scales, codes and units in `work`, one behind the other.
-int dib_fp4_linear(int (*quantize)(const void*, long long, void*, void*, void*, long long, int, int, cudaStream_t), const void* x,
-                   long long stride, int x_dtype, int K, void* work, const void* w, const void* ws, const void* uw, void* out, int M,
-                   int N, int out_dtype, int sm_count, cudaStream_t st) {
+int dib_fp4_linear(int (*quantize)(const void*, long long, void*, void*, void*, long long, int, int, int, cudaStream_t),
+                   const void* x, long long stride, int x_dtype, int K, void* work, const void* w, const void* ws, const void* uw,
+                   void* out, int M, int N, int out_dtype, int sm_count, cudaStream_t st) {
   if (M < 0 || K < 1) return DIB_BAD_SIZE;
   char* codes = reinterpret_cast<char*>(work) + (long long)(M + 127) / 128 * fp4_k_tiles(K) * 512;
   char* units = codes + (long long)M * ((K + 31) / 32 * 16);
-  const int rc = quantize(x, stride, codes, work, units, M, K, x_dtype, st);
+  const int rc = quantize(x, stride, codes, work, units, M, K, x_dtype, sm_count, st);
   if (rc != DIB_OK) return rc;
   return dib_gemm_fp4(codes, work, units, w, ws, uw, out, M, N, K, out_dtype, sm_count, st);
 }

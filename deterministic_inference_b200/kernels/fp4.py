@@ -39,7 +39,7 @@ BLOCK = 16
 # argument types; an argument is looked at in one expression, and the check that words the error runs only where that fails.
 _P, _I, _L, _F = c_void_p, c_int, c_longlong, c_float
 _SIGNATURES = {
-    "dib_fp4_quantize_rows": ("rows_fp4", (_P, _L, _P, _P, _P, _L, _I, _I, _P)),
+    "dib_fp4_quantize_rows": ("rows_fp4", (_P, _L, _P, _P, _P, _L, _I, _I, _I, _P)),
     "dib_fp4_read_rows": ("rows_fp4", (_P, _P, _P, _P, _L, _I, _I, _P)),
     "dib_fp4_layout_rows": ("rows_fp4", (_P, _P, _P, _P, _P, _P, _L, _I, _P)),
     "dib_gemm_fp4": ("gemm_fp4", (_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P)),
@@ -164,7 +164,7 @@ class _Rows:
         m, k = x.shape
         self._allocate(m, k, x.device)
         st = _fn("dib_fp4_quantize_rows")(x.data_ptr(), x.stride(0), self.codes.data_ptr(), self.tiles.data_ptr(),
-                                          self.units.data_ptr(), m, k, code, _stream("fp4_quantize_rows", x.device))
+                                          self.units.data_ptr(), m, k, code, _sms(x.device), _stream("fp4_quantize_rows", x.device))
         _done(st, "fp4_quantize_rows", lambda: f"rows {m} x {k}")
 
     @property

@@ -47,6 +47,13 @@ def test_rows_that_lie_apart(extra, at, dtype):
     _same_rows(ops.fp4_quantize_rows(wide[::2, at:at + 96]), wide[::2, at:at + 96])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m,k", [(10000, 48), (2500, 1000), (700, 4096), (300, 20000), (300, 33000)])
+def test_more_rows_than_are_worked_on_at_once(m, k, dtype):
+    x = _rand(m, k, seed=k, dtype=dtype) * (1 + torch.arange(m, device="cuda")[:, None] % 7).to(dtype)
+    _same_rows(ops.fp4_quantize_rows(x), x)
+
+
 def test_rows_next_to_borders():
     """Values on a border between two codes, and a float32 step to either side; blocks whose scale is rounded up and down, and
     blocks too small beside the row's largest for a scale of their own."""
@@ -59,6 +66,19 @@ def test_rows_next_to_borders():
     x = torch.stack(rows).cuda()
     _same_rows(ops.fp4_quantize_rows(x), x)
     _same_rows(ops.fp4_quantize_rows(x.to(BF16)), x.to(BF16))
+
+
+def test_every_code_of_every_block_scale():
+    """All finite block scales against multiples of a 64th of their units: what a code is rounded to, ties among them, does not
+    depend on whether its quotient is one of 8 or of 24 digits."""
+    scales = torch.arange(1, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).float()
+    at = torch.arange(-390, 391).float() / 64
+    blocks = (scales[:, None, None] * torch.cat([at, torch.full((15 * 53 - at.numel(),), 0.125)]).reshape(1, 53, 15))
+    blocks = torch.cat([(scales * 6.0)[:, None, None].expand(-1, 53, 1), blocks.clamp(-6 * scales[:, None, None], 6 * scales[:, None, None])], 2)
+    x = torch.cat([torch.full((126, 16), 2688.0), blocks.reshape(126, 53 * 16)], 1).cuda()
+    for unit in (2.0 ** -90, 1.0, 2.0 ** 100):
+        _same_rows(ops.fp4_quantize_rows(x * unit), x * unit)
+        _same_rows(ops.fp4_quantize_rows((x * unit).to(BF16)), (x * unit).to(BF16))
 
 
 def test_rows_of_no_numbers_zeros_and_extremes():
