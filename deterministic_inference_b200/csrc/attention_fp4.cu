@@ -519,7 +519,7 @@ attention_any_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_
 
 // ---------------------------------------------------------------- host side
 template <typename T, int NT>
-int launch_split(const void* q, void* out, SplitArgs a, int max_rows, int merge, int sm_count, cudaStream_t st) {
+int launch_split(const void* q, void* out, SplitArgs a, int max_rows, int runs, int sm_count, cudaStream_t st) {
   using SH = SplitShape<T, NT>;
   auto kern = attention_split_kernel<T, NT>;
   const size_t smem = SH::FIRST + ((size_t)a.seq_count + 1) * 8;
@@ -539,8 +539,8 @@ int launch_split(const void* q, void* out, SplitArgs a, int max_rows, int merge,
   dib_launch(kern, dim3((unsigned)(grid < most ? grid : most)), dim3(SP_THREADS), smem, st, reinterpret_cast<const T*>(q),
              reinterpret_cast<T*>(out), a);
   DIB_CHECK_LAUNCH();
-  if (merge) {
-    const long long blocks = (long long)max_rows * a.Hkv;
+  if (runs) {
+    const long long blocks = merge_blocks((long long)max_rows * a.Hkv, runs);
     if (blocks > 0x7fffffffll) return DIB_BAD_SIZE;
     dib_launch(attention_split_merge_kernel<T, SH::ROWS>, dim3((unsigned)blocks, a.seq_count), dim3(SM_WARPS * 32), 0, st,
                reinterpret_cast<T*>(out), a);
@@ -559,11 +559,11 @@ int dib_fp4_attention_split_keys(int kv_len, int rows) { return split_keys(kv_le
 // The split form, for the sequences seq_list[0 .. seq_count) or (null) seq_first ...: heads of 32, 64, 96 or 128, pages of a
 // power of two of rows, 4 at least.  max_rows: the most rows (new tokens x query heads of a kv head) of one of them; tile_rows: 8 or
 // 16 rows a tile; max_items: the most (tiles x runs x kv heads) of one; part_o float32 [seq_count, max_items, tile_rows, 128] and
-// part_ml [.., 2] take partial results where merge is not 0 (some sequence may have two runs).
+// part_ml [.., 2] take partial results where `runs`, the most runs of one of them, is not 0 (1 is given as 0).
 int dib_fp4_attention_split(const void* q, void* out, const void* data, const void* scales, const void* exponents, long long num_pages,
                             const void* block_table, int max_blocks, const void* cu_q_lens, const void* seq_lens,
                             const void* seq_list, int seq_first, int seq_count, int max_rows, int tile_rows, void* part_o,
-                            void* part_ml, int max_items, int merge, int Hq, int Hkv, int D, int page_size, float scale,
+                            void* part_ml, int max_items, int runs, int Hq, int Hkv, int D, int page_size, float scale,
                             int window, int dtype, int sm_count, cudaStream_t st) {
   if (dtype != 0 && dtype != 1) return DIB_BAD_DTYPE;
   if (seq_count < 0 || seq_count > 4096 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || D < 32 || D > 128 || D % 32 != 0 || page_size < 4 ||
@@ -584,9 +584,9 @@ int dib_fp4_attention_split(const void* q, void* out, const void* data, const vo
   a.max_items = max_items;
   using B = __nv_bfloat16;
   if (dtype == 1)
-    return tile_rows == 8 ? launch_split<B, 1>(q, out, a, max_rows, merge, sm_count, st) : launch_split<B, 2>(q, out, a, max_rows, merge, sm_count, st);
-  return tile_rows == 8 ? launch_split<float, 1>(q, out, a, max_rows, merge, sm_count, st)
-                        : launch_split<float, 2>(q, out, a, max_rows, merge, sm_count, st);
+    return tile_rows == 8 ? launch_split<B, 1>(q, out, a, max_rows, runs, sm_count, st) : launch_split<B, 2>(q, out, a, max_rows, runs, sm_count, st);
+  return tile_rows == 8 ? launch_split<float, 1>(q, out, a, max_rows, runs, sm_count, st)
+                        : launch_split<float, 2>(q, out, a, max_rows, runs, sm_count, st);
 }
 
 int dib_fp4_attention_any(const void* q, void* out, const void* data, const void* scales, const void* exponents, const void* block_table,

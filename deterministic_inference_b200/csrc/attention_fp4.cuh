@@ -136,9 +136,11 @@ template <> __device__ __forceinline__ void store_two<__nv_bfloat16>(__nv_bfloat
   *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(x, y);
 }
 
-// The runs' results of a row: out = sum_r 2^(M_r - top) O_r / sum_r 2^(M_r - top) l_r.  A block a row: warp w takes the
-// runs w, w + 4, ... in their order, a lane 4 places of the sums; the four warps' sums are added in the order of the warps.
-constexpr int SM_WARPS = 4;
+// The runs' results of a row: out = sum_r 2^(M_r - top) O_r / sum_r 2^(M_r - top) l_r, a lane 4 places of the sums.  Up to SM_RUNS runs
+// are a warp's, all asked for at once; more are those of a block: warp w takes the runs w, w + 4, ... in their order, the four warps'
+// sums are added in the order of the warps.  (16 sequences' 10 rows a head of some 8 runs: the attention and its merge 24.5 us with a warp a
+// row, 26.2 with a block.)
+constexpr int SM_WARPS = 4, SM_RUNS = 8;
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(SM_WARPS * 32)
 attention_split_merge_kernel(T* __restrict__ out, const __grid_constant__ SplitArgs a) {
@@ -146,18 +148,20 @@ attention_split_merge_kernel(T* __restrict__ out, const __grid_constant__ SplitA
   const float2* part_ml = a.part_ml;
   __shared__ float4 s_o[SM_WARPS][32];
   __shared__ float s_top[SM_WARPS], s_sum[SM_WARPS];
-  pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int i = blockIdx.y, G = a.Hq / a.Hkv;
   const SplitSeq s = split_seq<ROWS>(a, i);
-  const int n_rows = s.n * G, id = blockIdx.x;     // rows of a kv head
-  // (every block waits, the one without work too: a grid none of whose blocks has waited ends ahead of the attention, and the
+  const bool alone = s.splits <= SM_RUNS;      // a warp a row
+  const int n_rows = s.n * G;                  // of a kv head
+  const long long id = alone ? (long long)blockIdx.x * SM_WARPS + warp : blockIdx.x;
+  // (every warp waits, the one without work too: a grid none of whose blocks has waited ends ahead of the attention, and the
   // kernel that follows takes this one's end for the attention's)
-  if (s.splits <= 1 || id >= n_rows * a.Hkv || s.items(a.Hkv) > a.max_items) {
+  if (s.splits <= 1 || id >= (long long)n_rows * a.Hkv || s.items(a.Hkv) > a.max_items) {
     pdl_wait();
+    pdl_trigger();
     return;
   }
-  const int kvh = id / n_rows, row = id - kvh * n_rows, tile = row / ROWS, r = row % ROWS;
+  const int kvh = (int)(id / n_rows), row = (int)(id - (long long)kvh * n_rows), tile = row / ROWS, r = row % ROWS;
   const int p0 = s.kv_len - s.n;
   const int tok0 = tile * ROWS / G, tok1 = min((tile + 1) * ROWS - 1, n_rows - 1) / G;
   // the runs that hold keys which some row of the tile sees
@@ -165,18 +169,15 @@ attention_split_merge_kernel(T* __restrict__ out, const __grid_constant__ SplitA
   const int s0 = k_lo / s.split, s1 = k_hi < k_lo ? s0 - 1 : min(k_hi / s.split, s.splits - 1);
   const long long base = ((long long)i * a.max_items + (long long)(kvh * s.tiles + tile) * s.splits) * ROWS + r;
   pdl_wait(part_o, part_ml);
-  float top = UNSET;
-  for (int run = s0 + (int)threadIdx.x; run <= s1; run += SM_WARPS * 32) top = fmaxf(top, part_ml[base + (long long)run * ROWS].x);
+  pdl_trigger();      // (not before the attention is over: the blocks of the kernel that follows would take places among its own)
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
-  constexpr int AHEAD = 8;
-  // the first results are on their way while the references are compared
-  float4 v[AHEAD];
-  float2 ml[AHEAD];
-  auto load = [&](int from) {
+  float4 v[SM_RUNS];
+  float2 ml[SM_RUNS];
+  auto load = [&](int from, int step) {
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      const int run = from + u * SM_WARPS;
+    for (int u = 0; u < SM_RUNS; ++u) {
+      const int run = from + u * step;
       v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
       ml[u] = make_float2(-INFINITY, 0.f);
       if (run <= s1) {
@@ -186,39 +187,54 @@ attention_split_merge_kernel(T* __restrict__ out, const __grid_constant__ SplitA
       }
     }
   };
-  load(s0 + warp);
-  top = warp_max(top);
-  if (lane == 0) s_top[warp] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-  for (int from = s0 + warp; from <= s1; from += AHEAD * SM_WARPS) {
-    if (from != s0 + warp) load(from);
+  auto add = [&](float top) {
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
+    for (int u = 0; u < SM_RUNS; ++u) {
       const float w = fast_exp2(ml[u].x - top);
       sum = fmaf(w, ml[u].y, sum);
       o.x = fmaf(w, v[u].x, o.x); o.y = fmaf(w, v[u].y, o.y);
       o.z = fmaf(w, v[u].z, o.z); o.w = fmaf(w, v[u].w, o.w);
     }
-  }
-  s_o[warp][lane] = o;
-  if (lane == 0) s_sum[warp] = sum;
-  __syncthreads();
-  if (warp != 0) return;
-  float4 y = s_o[0][lane];
-  sum = s_sum[0];
+  };
+  if (alone) {
+    load(s0, 1);
+    float top = UNSET;
 #pragma unroll
-  for (int k = 1; k < SM_WARPS; ++k) {
-    const float4 z = s_o[k][lane];
-    y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
-    sum += s_sum[k];
+    for (int u = 0; u < SM_RUNS; ++u) top = fmaxf(top, ml[u].x);
+    add(top);
+  } else {
+    load(s0 + warp, SM_WARPS);      // on their way while the references are compared
+    float top = UNSET;
+    for (int run = s0 + (int)threadIdx.x; run <= s1; run += SM_WARPS * 32) top = fmaxf(top, part_ml[base + (long long)run * ROWS].x);
+    top = warp_max(top);
+    if (lane == 0) s_top[warp] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+    for (int from = s0 + warp; from <= s1; from += SM_RUNS * SM_WARPS) {
+      if (from != s0 + warp) load(from, SM_WARPS);
+      add(top);
+    }
+    s_o[warp][lane] = o;
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    if (warp != 0) return;
+    o = s_o[0][lane];
+    sum = s_sum[0];
+#pragma unroll
+    for (int k = 1; k < SM_WARPS; ++k) {
+      const float4 z = s_o[k][lane];
+      o.x += z.x; o.y += z.y; o.z += z.z; o.w += z.w;
+      sum += s_sum[k];
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int tok = row / G, d0 = dim_of(lane * 4), d1 = dim_of(lane * 4 + 2);
   T* dst = out + ((long long)(s.q_begin + tok) * a.Hq + kvh * G + row - tok * G) * a.D;
-  if (d0 < a.D) store_two<T>(dst + d0, y.x * inv, y.y * inv);
-  if (d1 < a.D) store_two<T>(dst + d1, y.z * inv, y.w * inv);
+  if (d0 < a.D) store_two<T>(dst + d0, o.x * inv, o.y * inv);
+  if (d1 < a.D) store_two<T>(dst + d1, o.z * inv, o.w * inv);
 }
+// blocks of the merge for a sequence of `rows` rows and at most `runs` runs
+inline long long merge_blocks(long long rows, int runs) { return runs <= SM_RUNS ? (rows + SM_WARPS - 1) / SM_WARPS : rows; }
 
 SplitArgs cache_args(const void* data, const void* scales, const void* exponents, long long num_pages, const void* block_table,
                      int max_blocks, const void* cu_q_lens, const void* seq_lens, int Hq, int Hkv, int D, float scale, int window) {

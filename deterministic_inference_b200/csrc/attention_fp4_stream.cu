@@ -778,7 +778,7 @@ bool make_cache_map(CUtensorMap* map, const void* data, long long rows, int D, i
 }
 
 template <int ROWS, int D>
-int launch_stream(const CUtensorMap& map, const void* q, void* out, SplitArgs a, int box_rows, int max_rows, int merge, int sm_count,
+int launch_stream(const CUtensorMap& map, const void* q, void* out, SplitArgs a, int box_rows, int max_rows, int runs, int sm_count,
                   cudaStream_t st) {
   using SH = StreamShape<ROWS>;
   auto kern = attention_stream_kernel<ROWS, D>;
@@ -804,8 +804,8 @@ int launch_stream(const CUtensorMap& map, const void* q, void* out, SplitArgs a,
   dib_launch(kern, dim3((unsigned)(grid < most ? grid : most)), dim3(ST_THREADS), smem, st, map, reinterpret_cast<const __nv_bfloat16*>(q),
              reinterpret_cast<__nv_bfloat16*>(out), a, box_rows, most >= grid ? 1 : 0);
   DIB_CHECK_LAUNCH();
-  if (merge) {
-    const long long blocks = (long long)max_rows * a.Hkv;
+  if (runs) {
+    const long long blocks = merge_blocks((long long)max_rows * a.Hkv, runs);
     if (blocks > 0x7fffffffll) return DIB_BAD_SIZE;
     dib_launch(attention_split_merge_kernel<__nv_bfloat16, ROWS>, dim3((unsigned)blocks, a.seq_count), dim3(SM_WARPS * 32), 0, st,
                reinterpret_cast<__nv_bfloat16*>(out), a);
@@ -832,7 +832,7 @@ int dib_attention_fp4_status_clear() {
 int dib_fp4_attention_stream(const void* q, void* out, const void* data, const void* scales, const void* exponents, long long num_pages,
                              const void* block_table, int max_blocks, const void* cu_q_lens, const void* seq_lens,
                              const void* seq_list, int seq_first, int seq_count, int max_rows, int tile_rows, void* part_o,
-                             void* part_ml, int max_items, int merge, int Hq, int Hkv, int D, int page_size, float scale,
+                             void* part_ml, int max_items, int runs, int Hq, int Hkv, int D, int page_size, float scale,
                              int window, int dtype, int sm_count, cudaStream_t st) {
   if (dtype != 1) return DIB_BAD_DTYPE;
   if (seq_count < 0 || seq_count > 4096 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || (D != 64 && D != 128) || page_size < 4 ||
@@ -856,7 +856,7 @@ int dib_fp4_attention_stream(const void* q, void* out, const void* data, const v
   if (!make_cache_map(&map, data, num_pages * 2 * Hkv * page_size, D, box_rows)) return DIB_LAUNCH_FAILED;
   auto launch = D == 128 ? (tile_rows == 4 ? launch_stream<4, 128> : tile_rows == 8 ? launch_stream<8, 128> : launch_stream<16, 128>)
                          : (tile_rows == 4 ? launch_stream<4, 64> : tile_rows == 8 ? launch_stream<8, 64> : launch_stream<16, 64>);
-  return launch(map, q, out, a, box_rows, max_rows, merge, sm_count, st);
+  return launch(map, q, out, a, box_rows, max_rows, runs, sm_count, st);
 }
 
 }  // extern "C"

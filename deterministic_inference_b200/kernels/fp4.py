@@ -461,6 +461,7 @@ class _SplitPart:
         runs, tiles = _most_runs(max(kv_lens[s] for s in seqs)), -(-self.max_rows // self.tile_rows)
         # (runs get longer with the rows: tiles times runs is at most the tiles' number and twice that of the shortest runs)
         self.items = hkv * min(tiles * runs, tiles + 2 * runs)
+        self.runs = runs if runs > 1 else 0      # 0: nothing to add up
         self.rows = self.count * self.items * self.tile_rows if runs > 1 else 0
 
 
@@ -546,7 +547,7 @@ def _split(q, out, cache: Fp4Cache, meta, part: _SplitPart, scale: float, window
     st = _fn(part.form)(
         q.data_ptr(), out.data_ptr(), *cache._pointers(), pages, meta.block_table.data_ptr(), meta.block_table.shape[1],
         meta.cu_q_lens.data_ptr(), meta.seq_lens.data_ptr(), part.list_pointer, part.first, part.count, part.max_rows, part.tile_rows,
-        partial, partial + rows * 512, part.items, 1 if rows else 0, hq, hkv, d, page_size, scale, window, _ops()._DT[q.dtype],
+        partial, partial + rows * 512, part.items, part.runs, hq, hkv, d, page_size, scale, window, _ops()._DT[q.dtype],
         _sms(q.device), stream)
     _done(st, "fp4_paged_attention", lambda: f"head_dim {d}, heads {hq}/{hkv}, {part.count} sequences", 2 if rows else 1)
 

@@ -446,6 +446,27 @@ def test_pages_that_are_none_of_the_pools(hkv, d, page, q_len, dtype):
         assert torch.equal(ops.fp4_paged_attention(q, case.cache(), meta, 0.003), want)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("q_len", [1, 4])
+@pytest.mark.parametrize("lens", [[2048, 100, 256, 257], [2049, 2048, 4096], [4096, 4097, 2048, 500], [4600, 4, 4608, 4609]])
+def test_attention_of_few_and_many_runs(lens, q_len, dtype):
+    """Sequences to either side of the lengths at which a run gets longer, and of those whose runs are added up in another way;
+    in steps of any of them alone, too, the same bits."""
+    case = Fp4Case(lens, 2, 128, 16, seed=len(lens))
+    out, _ = _check_attention(case, [q_len] * len(lens), 6, dtype, window=None)
+    _check_attention(case, [q_len] * len(lens), 6, dtype, window=1500)
+    q = _rand(q_len * len(lens), 6, 128, seed=100, dtype=dtype)
+    for s in range(len(lens)):
+        rows = slice(s * q_len, (s + 1) * q_len)
+        assert torch.equal(_attend(case.alone(s), q[rows], [q_len], 128 ** -0.5 / 32), out[rows])
+    # lengths of the device below the host's, as of a graph that is played again later
+    meta = case.meta([q_len] * len(lens))
+    short = [max(q_len, n - 1900) for n in lens]
+    meta.seq_lens.copy_(torch.tensor(short, dtype=torch.int32))
+    less = ops.fp4_paged_attention(q, case.cache(), meta, 128 ** -0.5 / 32)
+    assert torch.equal(less, _attend(case, q, [q_len] * len(lens), 128 ** -0.5 / 32, kv_lens=short))
+
+
 def test_attention_of_long_contexts():
     case = Fp4Case([20000, 9001, 17011], 2, 128, 16, seed=1)
     _check_attention(case, [1, 1, 5], 16, BF16)
