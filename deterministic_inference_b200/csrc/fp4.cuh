@@ -159,10 +159,11 @@ template <typename T> struct Block16 {
     if (sizeof(T) == 2) {      // two at a time: as 16-bit integers magnitudes order like the numbers
 #pragma unroll
       for (int i = 0; i < WORDS; ++i) asm("max.u16x2 %0, %0, %1;" : "+r"(t) : "r"(w[i] & 0x7fff7fffu));
-      return max(t << 16, t & 0xffff0000u);
-    }
+      t = max(t << 16, t & 0xffff0000u);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) t = max(t, fp4_magnitude(get(e)));
+      for (int e = 0; e < 16; ++e) t = max(t, fp4_magnitude(get(e)));
+    }
     return t;
   }
 };

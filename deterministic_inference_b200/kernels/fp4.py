@@ -151,36 +151,54 @@ def _tile_bytes(rows: int, k: int) -> int:
 
 class _Rows:
     """Rows [R, K] in the tensor cores' layout: ``codes`` uint8 [R, K rounded up to 32, / 2] (zeros behind K), ``tiles``
-    uint8, the block scales in tiles of 128 rows x 64 values, ``units`` float32 [R], 2^E (NaN: no numbers)."""
+    uint8, the block scales in tiles of 128 rows x 64 values, ``units`` float32 [R], 2^E (NaN: no numbers).  They lie in one
+    tensor, ``held``: the block scales, the codes, the units."""
 
     def _allocate(self, rows: int, k: int, device) -> None:
-        self.codes = torch.empty(rows, _code_bytes(k), dtype=torch.uint8, device=device)
-        self.tiles = torch.empty(_tile_bytes(rows, k), dtype=torch.uint8, device=device)
-        self.units = torch.empty(rows, dtype=torch.float32, device=device)
-        self.k = k
+        self.rows, self.k = rows, k
+        self.held = torch.empty(_tile_bytes(rows, k) + rows * (_code_bytes(k) + 4), dtype=torch.uint8, device=device)
+
+    def _pointers(self) -> tuple:
+        """Addresses of the codes, the block scales and the units."""
+        tiles, bytes_ = self.held.data_ptr(), _code_bytes(self.k)
+        codes = tiles + _tile_bytes(self.rows, self.k)
+        return codes, tiles, codes + self.rows * bytes_
 
     def _quantize(self, x: torch.Tensor, name: str) -> None:
         code = _check_rows(x, name)
         m, k = x.shape
-        self._allocate(m, k, x.device)
-        st = _fn("dib_fp4_quantize_rows")(x.data_ptr(), x.stride(0), self.codes.data_ptr(), self.tiles.data_ptr(),
-                                          self.units.data_ptr(), m, k, code, _sms(x.device), _stream("fp4_quantize_rows", x.device))
+        device = x.device
+        self._allocate(m, k, device)
+        st = _fn("dib_fp4_quantize_rows")(x.data_ptr(), x.stride(0), *self._pointers(), m, k, code, _sms(device),
+                                          _stream("fp4_quantize_rows", device))
         _done(st, "fp4_quantize_rows", lambda: f"rows {m} x {k}")
 
     @property
+    def tiles(self) -> torch.Tensor:
+        return self.held[:_tile_bytes(self.rows, self.k)]
+
+    @property
+    def codes(self) -> torch.Tensor:
+        at, n = _tile_bytes(self.rows, self.k), _code_bytes(self.k)
+        return self.held[at:at + self.rows * n].view(self.rows, n)
+
+    @property
+    def units(self) -> torch.Tensor:
+        return self.held[self.held.numel() - 4 * self.rows:].view(torch.float32)
+
+    @property
     def shape(self):
-        return torch.Size((self.codes.shape[0], self.k))
+        return torch.Size((self.rows, self.k))
 
     @property
     def device(self):
-        return self.codes.device
+        return self.held.device
 
     def tensor(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values the codes stand for [R, K]; exact in float32, rounded once in bfloat16."""
-        code, (m, k) = _code(dtype, "tensor"), self.shape
-        out = torch.empty(m, k, dtype=dtype, device=self.device)
-        st = _fn("dib_fp4_read_rows")(self.codes.data_ptr(), self.tiles.data_ptr(), self.units.data_ptr(), out.data_ptr(), m, k,
-                                      code, _stream("tensor", self.device))
+        code, m, k, device = _code(dtype, "tensor"), self.rows, self.k, self.held.device
+        out = torch.empty(m, k, dtype=dtype, device=device)
+        st = _fn("dib_fp4_read_rows")(*self._pointers(), out.data_ptr(), m, k, code, _stream("tensor", device))
         _done(st, "Fp4 rows as a tensor", lambda: f"rows {m} x {k}")
         return out
 
@@ -222,8 +240,8 @@ class Fp4Weight(_Rows):
                                   f"for each {BLOCK})")
         _same_device("Fp4Weight", codes, block_scales, exponents)
         self._allocate(n, k, codes.device)
-        st = _fn("dib_fp4_layout_rows")(codes.data_ptr(), block_scales.data_ptr(), exponents.data_ptr(), self.codes.data_ptr(),
-                                        self.tiles.data_ptr(), self.units.data_ptr(), n, k, _stream("Fp4Weight", codes.device))
+        st = _fn("dib_fp4_layout_rows")(codes.data_ptr(), block_scales.data_ptr(), exponents.data_ptr(), *self._pointers(), n, k,
+                                        _stream("Fp4Weight", codes.device))
         _done(st, "Fp4Weight", lambda: f"rows {n} x {k}")
         self._settle()
 
@@ -238,7 +256,8 @@ class Fp4Weight(_Rows):
     def _settle(self) -> None:
         # A copy stands between the kernel of this package that made the codes, which lets the next one start beside it, and a
         # product, which reads its weight ahead of its wait for the kernel in front: a copy waits for all of it.
-        self.units = self.units.clone()
+        units = self.units
+        units.copy_(units.clone())
 
 
 def _check_rows(x, name: str) -> int:
@@ -272,24 +291,20 @@ def fp4_linear(x, weight: Fp4Weight, out_dtype=None) -> torch.Tensor:
     m, k = x.shape
     if k != weight.k:
         raise _ops().KernelError(f"fp4_linear: x {tuple(x.shape)} against weight {tuple(weight.shape)}")
-    codes = weight.codes
-    device = codes.device
+    n, device = weight.rows, weight.held.device
     if x.device != device:
         _same_device("fp4_linear", x, weight)
-    n = codes.shape[0]
     out_dtype = out_dtype or x.dtype
     out_code = _code(out_dtype, "out")
     out = torch.empty(m, n, dtype=out_dtype, device=device)
     if rows:
-        st = _fn("dib_gemm_fp4")(x.codes.data_ptr(), x.tiles.data_ptr(), x.units.data_ptr(), codes.data_ptr(),
-                                 weight.tiles.data_ptr(), weight.units.data_ptr(), out.data_ptr(), m, n, k, out_code, _sms(device),
+        st = _fn("dib_gemm_fp4")(*x._pointers(), *weight._pointers(), out.data_ptr(), m, n, k, out_code, _sms(device),
                                  _stream("fp4_linear", device))
     else:
         # block scales, codes, units
         work = torch.empty(_tile_bytes(m, k) + m * (_code_bytes(k) + 4), dtype=torch.uint8, device=device)
         st = _fn("dib_fp4_linear")(_address("dib_fp4_quantize_rows"), x.data_ptr(), x.stride(0), code, k, work.data_ptr(),
-                                   codes.data_ptr(), weight.tiles.data_ptr(), weight.units.data_ptr(), out.data_ptr(), m, n,
-                                   out_code, _sms(device), _stream("fp4_linear", device))
+                                   *weight._pointers(), out.data_ptr(), m, n, out_code, _sms(device), _stream("fp4_linear", device))
     _done(st, "fp4_linear", lambda: f"M={m} N={n} K={k}", 1 if rows else 2)
     return out
 
