@@ -33,6 +33,9 @@ namespace {
 //
 // Work items: (sequence, kv head, tile of rows, run of keys), a CTA takes a contiguous range of them.  The length of a run follows
 // from the sequence's own lengths, so a row's bits do not depend on the rest of the step.
+//
+// Bound by instructions, some 700 for 32 keys: 64 requests of 2,048 keys, 16 / 4 heads: heads of 96 in bfloat16 41 us, of 128 in float32
+// 50 (the stream form 29 for heads of 128 in bfloat16).
 constexpr int SP_WARPS = 4, SP_THREADS = 32 * SP_WARPS, SP_STEP = 32, SP_STAGES = 3;
 constexpr int SP_K = 0, SP_V = SP_STEP * 64, SP_KS = 2 * SP_V, SP_VS = SP_KS + SP_STEP * 8, SP_KE = SP_VS + SP_STEP * 8,
               SP_VE = SP_KE + SP_STEP, SP_STAGE = SP_VE + SP_STEP;      // bytes of a step: codes, block scales, exponents
@@ -442,7 +445,8 @@ attention_split_kernel(const T* __restrict__ q, T* __restrict__ out, const __gri
 
 // ---------------------------------------------------------------- the form for every shape
 // Head sizes up to 256, any page size and group ratio: a warp takes a (token, head), a lane a key of 32 at a time for
-// the scores, then a lane D / 32 dimensions for the values.  Bound by a warp's chain over the keys.
+// the scores, then a lane D / 32 dimensions for the values.  Bound by a warp's chain over the keys: 2,048 of them 1.4 ms with heads of
+// 128, 2.4 with 256, for one request as for sixteen.
 constexpr int ANY_WARPS = 4;
 
 template <typename T>

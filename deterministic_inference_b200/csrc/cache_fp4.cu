@@ -176,6 +176,7 @@ cache_read_kernel(const __grid_constant__ Cache4 cache, const int* __restrict__ 
 // The step's fused projection rows [q heads | k heads | v heads]: q and k normed and rotated, q to its output, k and v rounded to T,
 // quantised and written to the token's slot.  A warp a (token, head), a lane 4 consecutive elements of 128 at a time: a block
 // of 16 is four lanes.
+// (32 / 8 heads of 128: 8 tokens 3.0 us, 2,048 tokens 41, bound by instructions.)
 constexpr int QKV_WARPS = 4;
 template <typename T>
 __global__ void __launch_bounds__(QKV_WARPS * 32)

@@ -13,6 +13,10 @@
 //
 // Few rows: a cluster has a tile of 128 channels, each of its CTAs a part of k; the channels are the products' 128 lanes, the tokens
 // their columns.  Many rows: tiles of 128 tokens x BN channels, or 256 x 192 for a pair of CTAs.
+//
+// What bounds it: few rows, the weight's bytes (8 x 24,576 x 4,096 11.6 us, 4.9 TB/s; 8 x 4,096 x 12,288 8.0 us, 3.5 TB/s, the rest
+// the cluster's start and sums); many rows, the tiles' operands from L2 (2,048 x 24,576 x 4,096 97 us, 4.3 PFLOP/s: 1.06 GB at 10.9 TB/s; the
+// copies without products take as long, the products without copies 67 us).
 #include <cuda.h>
 
 #include "fp4.cuh"
