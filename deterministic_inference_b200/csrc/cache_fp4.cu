@@ -237,7 +237,8 @@ qk_norm_rope_cache_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, cons
 // cache: what 4 bits stand for has 6 digits, so that bfloat16 holds it exactly.  Sequence number i of the launch, seq_list[i],
 // has its pages from first_page[i] on, one for every PAGE keys up to the host's bound of its length.  Keys behind its real length,
 // and those that are on no page of the pool, are zeros up to the page's end; pages wholly behind the last key, or ahead of the
-// window of the first new token, are left as they are.  (The new block table follows from the bounds: the host makes it.)
+// window of the first new token, are left as they are.  (The new block table follows from the bounds: the host makes it.)  Bound by memory:
+// 32,000 tokens of 8 heads of 128 in 33 us, 5.1 TB/s; 4,096 in 6.8.
 constexpr int UNPACK_PAGE = 128;
 struct UnpackArgs {
   Cache4 cache;
@@ -287,6 +288,20 @@ unpack_pages_kernel(const __grid_constant__ UnpackArgs a) {
       store16(out + (long long)(r0 + g * GROUPS) * a.D, y);
     }
   }
+}
+
+// Zeros for the new tokens of some sequences that lie in front of the first key (a sequence with fewer keys than new tokens), of
+// which the attention over the pages made above says nothing.  A launch behind it, 1.1 us where there are none.
+constexpr int UNSEEN_BLOCKS = 8;      // a sequence
+__global__ void __launch_bounds__(CACHE_THREADS)
+zero_unseen_kernel(const int* __restrict__ cu_q_lens, const int* __restrict__ seq_lens, const int* __restrict__ seq_list,
+                   __nv_bfloat16* __restrict__ out, long long max_keys, int row) {
+  pdl_prologue(out);
+  const int seq = seq_list[blockIdx.y], q_begin = cu_q_lens[seq], n = cu_q_lens[seq + 1] - q_begin;
+  const long long keys = max(min((long long)seq_lens[seq], max_keys), 0ll);
+  const long long pieces = max((long long)n - keys, 0ll) * (row / 8);      // of 16 bytes
+  uint4* to = reinterpret_cast<uint4*>(out + (long long)q_begin * row);
+  for (long long i = blockIdx.x * CACHE_THREADS + threadIdx.x; i < pieces; i += UNSEEN_BLOCKS * CACHE_THREADS) to[i] = make_uint4(0, 0, 0, 0);
 }
 
 // Two blocks of 16 a lane: bfloat16, rows and scales that allow it.  (8,000 tokens of 8 heads of 128 written, read: 10.1, 8.7 us, with one
@@ -427,6 +442,20 @@ int dib_fp4_unpack_pages(const void* data, const void* scales, const void* expon
   a.num_pages = num_pages;
   dib_launch(D > 128 ? unpack_pages_kernel<16> : unpack_pages_kernel<8>, dim3((unsigned)max_pages, 2u * Hkv, (unsigned)count),
              dim3(CACHE_THREADS), 0, st, a);
+  DIB_CHECK_LAUNCH();
+  return DIB_OK;
+}
+
+// out [T, Hq, D] of the sequences seq_list [count]: zeros for the tokens that lie in front of the first key (see zero_unseen_kernel).
+int dib_fp4_zero_unseen(const void* cu_q_lens, const void* seq_lens, const void* seq_list, int count, void* out, int Hq, int D,
+                        int max_blocks, int page_size, cudaStream_t st) {
+  if (count < 0 || count > 65535 || Hq < 1 || D < 16 || D % 16 != 0 || max_blocks < 1 || page_size < 1 || (long long)Hq * D > 0x7fffffffll)
+    return DIB_BAD_SIZE;
+  if ((reinterpret_cast<uintptr_t>(out) & 15) != 0) return DIB_BAD_ALIGN;
+  if (count == 0) return DIB_OK;
+  dib_launch(zero_unseen_kernel, dim3(UNSEEN_BLOCKS, (unsigned)count), dim3(CACHE_THREADS), 0, st,
+             reinterpret_cast<const int*>(cu_q_lens), reinterpret_cast<const int*>(seq_lens), reinterpret_cast<const int*>(seq_list),
+             reinterpret_cast<__nv_bfloat16*>(out), (long long)max_blocks * page_size, Hq * D);
   DIB_CHECK_LAUNCH();
   return DIB_OK;
 }

@@ -358,6 +358,22 @@ def test_attention_rows_that_see_nothing(hq, hkv, d, page, dtype):
     assert not out[:2].any() and not out[5:7].any() and not out[7:12].any() and out[2].any() and out[12].any()
 
 
+@pytest.mark.parametrize("portions", [False, True])
+@pytest.mark.parametrize("window", [None, 100])
+@pytest.mark.parametrize("lens,q_lens", [([20], [50]), ([300, 0, 70], [40, 50, 71]), ([0, 1, 130], [300, 400, 600]),
+                                         ([4200, 5], [4500, 40])])
+def test_portions_in_front_of_the_first_key(lens, q_lens, window, portions):
+    """More new tokens than keys, in numbers for which keys and values become bfloat16 pages; what those lay in before is no
+    number."""
+    case = Fp4Case(lens, 2, 128, 16, seed=9)
+    torch.full((1 << 26,), float("nan"), dtype=BF16, device="cuda")
+    out, _ = _check_attention(case, q_lens, 8, BF16, window=window, portions=portions)
+    at = 0
+    for keys, n in zip(lens, q_lens):
+        assert not out[at:at + max(0, n - keys)].any() and (keys == 0 or out[at + n - 1].any())
+        at += n
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("q_len", [1, 3, 9, 40])
 def test_attention_of_uneven_value_exponents(q_len, dtype):
