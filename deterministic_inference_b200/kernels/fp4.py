@@ -446,7 +446,8 @@ def fp4_cache_read(cache: Fp4Cache, slots: torch.Tensor, dtype: torch.dtype = to
 # Rows (new tokens x query heads of a kv head) of a sequence of drafted tokens above which they take the prompt form (bfloat16).  By
 # the sequence's own rows, so that its bits do not depend on the step; a prompt's portions take it whatever their rows.
 PROMPT_ROWS = 32
-# Bytes of bfloat16 pages that a launch of the prompt form makes of its sequences' keys and values, one sequence at least.
+# Bytes of bfloat16 pages that a launch of the prompt form makes of its sequences' keys and values, one sequence at least (and all
+# with 4,096 new tokens or more).
 PAGES_BYTES = 1 << 30
 PAGE = 128
 
@@ -523,11 +524,15 @@ def _parts(meta, group: int, hkv: int, d: int, page_size: int, prompts: bool, st
         one = [s for s, n in enumerate(q_lens) if n == 1]
         many = [s for s, n in enumerate(q_lens) if n > 1 and prompts and (portions or n * group > PROMPT_ROWS)]
         few = sorted({s for s, n in enumerate(q_lens) if n > 1} - set(many))
+        # A launch's attention adds up chunks of keys of every token of the step, and takes those of the other launches, whose
+        # sequences have no key there, for tokens in front of the first key: fewer than a chunk's number of them lie in the first
+        # chunk and are left alone.  Sequences of more are all in the last launch, which no other one follows.
+        long = [s for s in many if q_lens[s] >= attention_bf16.CHUNK_TILES * PAGE]
         parts, some, used = [], [], 0
         room = max(1, PAGES_BYTES // (4 * hkv * PAGE * d))
-        for s in many:
+        for s in [s for s in many if s not in long] + long:
             n = -(-kv_lens[s] // PAGE)
-            if some and used + n > room:
+            if some and used + n > room and s not in long[1:]:
                 parts.append(_PromptPart(some, q_lens, kv_lens, meta, device))
                 some, used = [], 0
             some.append(s)

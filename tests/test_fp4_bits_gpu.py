@@ -62,6 +62,22 @@ def test_prompts_in_several_launches(window, monkeypatch):
         assert sum(isinstance(p, fp4._PromptPart) for p in parts) == (3 if pages < 120 else 2)
 
 
+@pytest.mark.parametrize("hq,hkv", [(4, 2), (16, 1)])
+@pytest.mark.parametrize("long", [4094, 4095, 4096, 4500])
+def test_a_long_portion_beside_others_in_several_launches(long, hq, hkv, monkeypatch):
+    """Portions of more tokens than a chunk of keys, in front of other launches of the step with many keys: a launch adds up chunks of
+    its own sequences' rows alone."""
+    case, q_lens = Fp4Case([long, 5000, 130, 4600], hkv, 128, 16, seed=2), [long, 60, 100, 4300 if long == 4500 else 40]
+    q = _rand(sum(q_lens), hq, 128, seed=1, dtype=BF16)
+    want = ops.paged_attention(q, case.cache(), case.meta(q_lens), 0.003, None)
+    assert want.isfinite().all()
+    monkeypatch.setattr(fp4, "PAGES_BYTES", 1)
+    meta = case.meta(q_lens)
+    assert torch.equal(ops.paged_attention(q, case.cache(), meta, 0.003, None), want)
+    assert sum(isinstance(p, fp4._PromptPart) for p in next(iter(meta.scratch.values()))) >= 3
+    ops.check_kernel_status()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("hq,hkv,d", [(16, 8, 128), (4, 2, 64), (6, 2, 96), (8, 1, 128)])
 @pytest.mark.parametrize("window", [None, 100])
