@@ -106,6 +106,14 @@ __device__ __forceinline__ unsigned fp4_codes8(const float* x, const Fp4Scaler& 
         "}" : "=f"(y[i]), "=f"(y[i + 1]) : "f"(x[i]), "f"(x[i + 1]), "f"(-s.b), "f"(s.inv));
   return fp4_pack8(y);
 }
+// A sum of products of two rows' codes and block scales (2^-20 .. 2^48, or 0) times the rows' units, the smaller one first: it
+// overflows where the result does, and what a small unit makes too small for all digits is 2^-40 of the products' magnitude.
+__device__ __forceinline__ float fp4_times_units(float sum, float ua, float ub) {
+  float less, more;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(less) : "f"(ua), "f"(ub));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(more) : "f"(ua), "f"(ub));
+  return sum * less * more;
+}
 // Eight codes as numbers, times `scale`.
 __device__ __forceinline__ void fp4_values8(unsigned w, float scale, float* x) {
   unsigned h[4];

@@ -266,8 +266,8 @@ __device__ __forceinline__ void store_rows(const float (&acc)[COLS], const CUten
         w = make_float4(left > 0 ? uw[4 * j] : 0.f, left > 1 ? uw[4 * j + 1] : 0.f, left > 2 ? uw[4 * j + 2] : 0.f,
                         left > 3 ? uw[4 * j + 3] : 0.f);
       }
-      const float y0 = acc[col + 4 * j] * ux * w.x, y1 = acc[col + 4 * j + 1] * ux * w.y;
-      const float y2 = acc[col + 4 * j + 2] * ux * w.z, y3 = acc[col + 4 * j + 3] * ux * w.w;
+      const float y0 = fp4_times_units(acc[col + 4 * j], ux, w.x), y1 = fp4_times_units(acc[col + 4 * j + 1], ux, w.y);
+      const float y2 = fp4_times_units(acc[col + 4 * j + 2], ux, w.z), y3 = fp4_times_units(acc[col + 4 * j + 3], ux, w.w);
       if (sizeof(OutT) == 2) {
         const __nv_bfloat162 lo = __floats2bfloat162_rn(y0, y1), hi = __floats2bfloat162_rn(y2, y3);
         y[(2 * j) % WORDS] = *reinterpret_cast<const unsigned*>(&lo);
@@ -688,7 +688,7 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     OutT* out = reinterpret_cast<OutT*>(a.out) + (long long)token * a.N + n;
     float y[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = j < left ? s4[j] * ux * a.uw[n + j] : 0.f;
+    for (int j = 0; j < 4; ++j) y[j] = j < left ? fp4_times_units(s4[j], ux, a.uw[n + j]) : 0.f;
     if (!a.by_values && left >= 4) {
       store4(out, y);
     } else {

@@ -171,6 +171,19 @@ def test_product_of_rows_that_are_no_numbers():
     assert torch.equal(y.isnan(), bad) and torch.equal(y[~bad], good[~bad])
 
 
+@pytest.mark.parametrize("m", [3, 200])
+@pytest.mark.parametrize("x_scale,w_scale", [(2.0 ** 110, 2.0 ** -105), (2.0 ** -95, 2.0 ** 115), (2.0 ** 60, 2.0 ** 40), (2.0 ** -60, 2.0 ** -50)])
+def test_product_of_large_and_small_rows(m, x_scale, w_scale):
+    """Rows and channels whose powers of two are far apart: no step on the way overflows or vanishes where the result does not."""
+    x, w = _rand(m, 300, seed=m) * x_scale, ops.Fp4Weight.of(_rand(130, 300, seed=5) * w_scale)
+    y = ops.fp4_linear(x, w)
+    a, b = values(*quantised(x), 300, torch.float64), w.tensor().double()
+    want, mass = a @ b.t(), a.abs() @ b.abs().t()
+    assert y.isfinite().all() and ((y.double() - want).abs() <= 30 * 2.0 ** -23 * mass).all()      # as in _check_product
+    swapped = ops.fp4_linear(ops.fp4_quantize_rows(w.tensor()), ops.Fp4Weight.of(x))
+    assert ((swapped.double() - want.t()).abs() <= 30 * 2.0 ** -23 * mass.t()).all()
+
+
 def test_product_with_no_rows():
     w = ops.Fp4Weight.of(_rand(32, 64))
     assert ops.fp4_linear(torch.empty(0, 64, device="cuda"), w).shape == (0, 32)
