@@ -236,9 +236,9 @@ qk_norm_rope_cache_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, cons
 // ---- the keys and values of some sequences as bfloat16 pages of their own, [pages, 2, Hkv, PAGE, D], for attention over an unquantised
 // cache: what 4 bits stand for has 6 digits, so that bfloat16 holds it exactly.  Sequence number i of the launch, seq_list[i],
 // has its pages from first_page[i] on, one for every PAGE keys up to the host's bound of its length.  Keys behind its real length,
-// and those that are on no page of the pool, are zeros up to the page's end; pages wholly behind the last key, or ahead of the
+// those that are on no page of the pool, and those of which the key or the value is no number, are zeros up to the page's end; pages wholly behind the last key, or ahead of the
 // window of the first new token, are left as they are.  (The new block table follows from the bounds: the host makes it.)  Bound by memory:
-// 32,000 tokens of 8 heads of 128 in 33 us, 5.1 TB/s; 4,096 in 6.8.
+// 32,000 tokens of 8 heads of 128 in 35 us, 4.8 TB/s; 4,096 in 8.1.
 constexpr int UNPACK_PAGE = 128;
 struct UnpackArgs {
   Cache4 cache;
@@ -280,6 +280,8 @@ unpack_pages_kernel(const __grid_constant__ UnpackArgs a) {
         if (p >= 0 && p < a.num_pages) at = ((long long)p * 2 * a.Hkv + rows) * a.page_size + (key - of * a.page_size);
       }
       x[g].load(held, at, l, a.D);
+      if (at >= 0 && max(x[g].exponent, (unsigned)held.exponents[at + (rows < a.Hkv ? a.Hkv : -a.Hkv) * a.page_size]) == FP4_NO_NUMBER)
+        x[g].load(held, -1, l, a.D);
     }
 #pragma unroll
     for (int g = 0; g < ROWS; ++g) {
@@ -290,18 +292,80 @@ unpack_pages_kernel(const __grid_constant__ UnpackArgs a) {
   }
 }
 
-// Zeros for the new tokens of some sequences that lie in front of the first key (a sequence with fewer keys than new tokens), of
-// which the attention over the pages made above says nothing.  A launch behind it, 1.1 us where there are none.
-constexpr int UNSEEN_BLOCKS = 8;      // a sequence
+// What the attention over the pages made above leaves open, a launch behind it (32,000 keys of 8 heads 1.7 us): the new tokens in front of the first key (a sequence
+// with fewer keys than new tokens) are zeros; those that see a key whose row, or whose value's, is no number are none either.  (As such
+// numbers in the pages they would reach rows that do not see them, by way of probabilities of zero.)  A block looks through the
+// exponents of FINISH_KEYS keys of a kv head.
+constexpr int FINISH_KEYS = 4096;
 __global__ void __launch_bounds__(CACHE_THREADS)
-zero_unseen_kernel(const int* __restrict__ cu_q_lens, const int* __restrict__ seq_lens, const int* __restrict__ seq_list,
-                   __nv_bfloat16* __restrict__ out, long long max_keys, int row) {
-  pdl_prologue(out);
-  const int seq = seq_list[blockIdx.y], q_begin = cu_q_lens[seq], n = cu_q_lens[seq + 1] - q_begin;
-  const long long keys = max(min((long long)seq_lens[seq], max_keys), 0ll);
-  const long long pieces = max((long long)n - keys, 0ll) * (row / 8);      // of 16 bytes
-  uint4* to = reinterpret_cast<uint4*>(out + (long long)q_begin * row);
-  for (long long i = blockIdx.x * CACHE_THREADS + threadIdx.x; i < pieces; i += UNSEEN_BLOCKS * CACHE_THREADS) to[i] = make_uint4(0, 0, 0, 0);
+finish_portions_kernel(const __grid_constant__ UnpackArgs a, int Hq) {
+  __shared__ unsigned bits[FINISH_KEYS / 32];
+  constexpr int EACH = FINISH_KEYS / (4 * CACHE_THREADS);
+  pdl_trigger();
+  // (the step's metadata, which no kernel of a step writes, ahead of the wait)
+  const int seq = a.seq_list[blockIdx.z], q_begin = a.cu_q_lens[seq], n = a.cu_q_lens[seq + 1] - q_begin, kvh = blockIdx.y;
+  const int kv_len = (int)max(min((long long)a.seq_lens[seq], (long long)a.max_blocks * a.page_size), 0ll);
+  const int p0 = kv_len - n, key0 = blockIdx.x * FINISH_KEYS, G = Hq / a.Hkv;
+  // four keys a thread, on one page
+  const int* table = a.block_table + (long long)seq * a.max_blocks;
+  long long at[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int key = key0 + (i * CACHE_THREADS + threadIdx.x) * 4, of = key / a.page_size;
+    const int page = key < kv_len ? table[of] : -1;
+    at[i] = page < 0 || page >= a.num_pages ? -1 : ((long long)page * 2 * a.Hkv + kvh) * a.page_size + (key - of * a.page_size);
+  }
+  const unsigned char* exponents = a.cache.exponents;
+  __nv_bfloat16* out = a.out;
+  pdl_wait(exponents, out);
+  if (blockIdx.x == 0 && kvh == 0) {
+    const long long pieces = (long long)max(-p0, 0) * Hq * (a.D / 8);      // of 16 bytes
+    uint4* to = reinterpret_cast<uint4*>(out + (long long)q_begin * Hq * a.D);
+    for (long long i = threadIdx.x; i < pieces; i += CACHE_THREADS) to[i] = make_uint4(0, 0, 0, 0);
+  }
+  const int first = first_visible_key(max(p0, 0), a.window);
+  if (key0 >= kv_len || key0 + FINISH_KEYS <= first) return;
+  if (threadIdx.x < FINISH_KEYS / 32) bits[threadIdx.x] = 0;
+  __syncthreads();
+  unsigned found[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    unsigned keys = 0, values = 0;
+    if (at[i] >= 0) {
+      keys = *reinterpret_cast<const unsigned*>(exponents + at[i]);
+      values = *reinterpret_cast<const unsigned*>(exponents + at[i] + (long long)a.Hkv * a.page_size);
+    }
+    const unsigned both = __vcmpeq4(keys, 0xffffffffu) | __vcmpeq4(values, 0xffffffffu);
+    const int left = kv_len - (key0 + (i * CACHE_THREADS + threadIdx.x) * 4);      // keys that there are
+    found[i] = (both & 1) | (both >> 7 & 2) | (both >> 14 & 4) | (both >> 21 & 8);
+    if (left < 4) found[i] &= left <= 0 ? 0 : (1u << left) - 1;
+  }
+  unsigned any = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) any |= found[i];
+  if (!__syncthreads_or(any)) return;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int k = (i * CACHE_THREADS + threadIdx.x) * 4;
+    if (found[i]) atomicOr(&bits[k >> 5], found[i] << (k & 31));
+  }
+  __syncthreads();
+  // a warp a token
+  const int lane = threadIdx.x & 31;
+  for (int i = threadIdx.x >> 5; i < n; i += CACHE_THREADS / 32) {
+    const int pos = p0 + i;
+    if (pos < key0) continue;
+    const int lo = max(first_visible_key(pos, a.window) - key0, 0), hi = pos - key0;      // of the block's keys
+    unsigned hit = 0;
+#pragma unroll
+    for (int w = lane; w < FINISH_KEYS / 32; w += 32) {
+      const int from = lo - w * 32, to = hi - w * 32;      // bits from .. to
+      if (from < 32 && to >= 0) hit |= bits[w] & (0xffffffffu << max(from, 0)) & (0xffffffffu >> max(31 - to, 0));
+    }
+    if (!__any_sync(0xffffffffu, hit != 0)) continue;
+    uint4* row = reinterpret_cast<uint4*>(out + ((long long)(q_begin + i) * Hq + kvh * G) * a.D);
+    for (int e = lane; e < G * a.D / 8; e += 32) row[e] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+  }
 }
 
 // Two blocks of 16 a lane: bfloat16, rows and scales that allow it.  (8,000 tokens of 8 heads of 128 written, read: 10.1, 8.7 us, with one
@@ -446,16 +510,28 @@ int dib_fp4_unpack_pages(const void* data, const void* scales, const void* expon
   return DIB_OK;
 }
 
-// out [T, Hq, D] of the sequences seq_list [count]: zeros for the tokens that lie in front of the first key (see zero_unseen_kernel).
-int dib_fp4_zero_unseen(const void* cu_q_lens, const void* seq_lens, const void* seq_list, int count, void* out, int Hq, int D,
-                        int max_blocks, int page_size, cudaStream_t st) {
-  if (count < 0 || count > 65535 || Hq < 1 || D < 16 || D % 16 != 0 || max_blocks < 1 || page_size < 1 || (long long)Hq * D > 0x7fffffffll)
+// out [T, Hq, D], behind the attention over the pages of dib_fp4_unpack_pages: see finish_portions_kernel.
+int dib_fp4_finish_portions(const void* exponents, long long num_pages, const void* block_table, int max_blocks, const void* cu_q_lens,
+                            const void* seq_lens, const void* seq_list, int count, int max_pages, void* out, int Hq, int Hkv, int D,
+                            int page_size, int window, cudaStream_t st) {
+  if (!shape_fits(0, Hkv, D, page_size, num_pages) || count < 0 || count > 65535 || max_pages < 1 || Hkv > 65535 || max_blocks < 1 ||
+      Hq < 1 || Hq % Hkv != 0 || page_size % 4 != 0)
     return DIB_BAD_SIZE;
-  if ((reinterpret_cast<uintptr_t>(out) & 15) != 0) return DIB_BAD_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(exponents) & 3) != 0 || (reinterpret_cast<uintptr_t>(out) & 15) != 0) return DIB_BAD_ALIGN;
   if (count == 0) return DIB_OK;
-  dib_launch(zero_unseen_kernel, dim3(UNSEEN_BLOCKS, (unsigned)count), dim3(CACHE_THREADS), 0, st,
-             reinterpret_cast<const int*>(cu_q_lens), reinterpret_cast<const int*>(seq_lens), reinterpret_cast<const int*>(seq_list),
-             reinterpret_cast<__nv_bfloat16*>(out), (long long)max_blocks * page_size, Hq * D);
+  UnpackArgs a = {};
+  a.cache = make_cache(nullptr, nullptr, exponents);
+  a.block_table = reinterpret_cast<const int*>(block_table);
+  a.cu_q_lens = reinterpret_cast<const int*>(cu_q_lens);
+  a.seq_lens = reinterpret_cast<const int*>(seq_lens);
+  a.seq_list = reinterpret_cast<const int*>(seq_list);
+  a.out = reinterpret_cast<__nv_bfloat16*>(out);
+  a.max_blocks = max_blocks;
+  a.Hkv = Hkv; a.D = D; a.page_size = page_size; a.window = window;
+  a.num_pages = num_pages;
+  const int per = FINISH_KEYS / UNPACK_PAGE;
+  dib_launch(finish_portions_kernel, dim3((unsigned)((max_pages + per - 1) / per), (unsigned)Hkv, (unsigned)count), dim3(CACHE_THREADS),
+             0, st, a, Hq);
   DIB_CHECK_LAUNCH();
   return DIB_OK;
 }

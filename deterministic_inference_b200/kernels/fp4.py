@@ -48,7 +48,7 @@ _SIGNATURES = {
     "dib_fp4_cache_read": ("cache_fp4", (_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _L, _I, _P)),
     "dib_fp4_qk_norm_rope_cache": ("cache_fp4", (_P, _P, _P, _P, _P, _P, _P, _F, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _L, _I, _P)),
     "dib_fp4_unpack_pages": ("cache_fp4", (_P, _P, _P, _L, _P, _I, _P, _P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _P)),
-    "dib_fp4_zero_unseen": ("cache_fp4", (_P, _P, _P, _I, _P, _I, _I, _I, _I, _P)),
+    "dib_fp4_finish_portions": ("cache_fp4", (_P, _L, _P, _I, _P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _I, _P)),
     "dib_fp4_attention_split": ("attention_fp4", (_P, _P, _P, _P, _P, _L, _P, _I, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _I, _I,
                                                   _I, _I, _F, _I, _I, _I, _P)),
     "dib_fp4_attention_stream": ("attention_fp4_stream", (_P, _P, _P, _P, _P, _L, _P, _I, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _I,
@@ -558,9 +558,10 @@ def _prompt(q, out, cache: Fp4Cache, meta, part: _PromptPart, scale: float, wind
                                      held.data_ptr(), hkv, d, page_size, window, stream)
     _done(st, "fp4_paged_attention", lambda: f"head_dim {d}, kv heads {hkv}, {part.pages} pages")
     attention_bf16.run(q, out, held, own, scale, window)
-    # (tokens in front of the first key: that attention says nothing of them)
-    st = _fn("dib_fp4_zero_unseen")(meta.cu_q_lens.data_ptr(), meta.seq_lens.data_ptr(), part.seqs, part.count, out.data_ptr(),
-                                    q.shape[1], d, meta.block_table.shape[1], page_size, stream)
+    # (tokens in front of the first key, and those that see a row that is no number)
+    st = _fn("dib_fp4_finish_portions")(cache.exponents.data_ptr(), pages, meta.block_table.data_ptr(), meta.block_table.shape[1],
+                                        meta.cu_q_lens.data_ptr(), meta.seq_lens.data_ptr(), part.seqs, part.count, part.most,
+                                        out.data_ptr(), q.shape[1], hkv, d, page_size, window, stream)
     _done(st, "fp4_paged_attention", lambda: f"head_dim {d}, heads {q.shape[1]}")
 
 

@@ -456,6 +456,30 @@ def test_attention_rows_of_the_cache_that_are_no_numbers(q_len, kv, d, dtype, pa
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kv", [0, 1])
+@pytest.mark.parametrize("window", [None, 50])
+@pytest.mark.parametrize("q_len", [2, 60, 250])
+@pytest.mark.parametrize("hkv,d,page", [(1, 128, 16), (2, 128, 8), (1, 144, 16)])
+def test_portions_beside_rows_of_the_cache_that_are_no_numbers(hkv, d, page, q_len, window, kv, dtype):
+    """As above for portions of prompts: in the first and the last head's row of a key that some of the tokens see, and of one that a
+    window has left."""
+    case = Fp4Case([300], hkv, d, page, seed=2)
+    q = _rand(q_len, 2 * hkv, d, seed=5, dtype=dtype)
+    good = _attend(case, q, [q_len], 0.003, window, portions=True)
+    for at, head in ((300 - q_len // 2 - 1, 0), (299, hkv - 1), (300 - q_len - 10, 0), (0, hkv - 1)):
+        place = (case.tables[0][at // page], kv, head, at % page)
+        held = case.exponents[place].clone()
+        case.exponents[place] = 255
+        out = _attend(case, q, [q_len], 0.003, window, portions=True)
+        case.exponents[place] = held
+        pos = torch.arange(300 - q_len, 300)
+        sees = torch.zeros(q_len, 2 * hkv, dtype=torch.bool)
+        sees[:, 2 * head:2 * head + 2] = ((pos >= at) & (pos < at + (window or 1000)))[:, None]
+        sees = sees.cuda()
+        assert out[sees].isnan().all() and torch.equal(out[~sees], good[~sees]), (at, head)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("q_len", [1, 5, 90])
 @pytest.mark.parametrize("hkv,d,page", [(2, 128, 16), (2, 64, 4), (2, 96, 16), (2, 144, 16), (2, 64, 24)])
 def test_pages_that_are_none_of_the_pools(hkv, d, page, q_len, dtype):
