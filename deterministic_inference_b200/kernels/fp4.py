@@ -526,13 +526,15 @@ def _parts(meta, group: int, hkv: int, d: int, page_size: int, prompts: bool, st
         few = sorted({s for s, n in enumerate(q_lens) if n > 1} - set(many))
         # A launch's attention adds up chunks of keys of every token of the step, and takes those of the other launches, whose
         # sequences have no key there, for tokens in front of the first key: fewer than a chunk's number of them lie in the first
-        # chunk and are left alone.  Sequences of more are all in the last launch, which no other one follows.
-        long = [s for s in many if q_lens[s] >= attention_bf16.CHUNK_TILES * PAGE]
+        # chunk and are left alone.  Sequences of more are all in the last launch that adds up chunks.  Those of more keys than it
+        # adds up take another kernel, which is by the launch's longest: they follow in launches of their own.
+        far = [s for s in many if kv_lens[s] > attention_bf16.MAX_CHUNKS * attention_bf16.CHUNK_TILES * PAGE]
+        long = [s for s in many if q_lens[s] >= attention_bf16.CHUNK_TILES * PAGE and s not in far]
         parts, some, used = [], [], 0
         room = max(1, PAGES_BYTES // (4 * hkv * PAGE * d))
-        for s in [s for s in many if s not in long] + long:
+        for s in [s for s in many if s not in long and s not in far] + long + far:
             n = -(-kv_lens[s] // PAGE)
-            if some and used + n > room and s not in long[1:]:
+            if some and (used + n > room and s not in long[1:] or s in far[:1]):
                 parts.append(_PromptPart(some, q_lens, kv_lens, meta, device))
                 some, used = [], 0
             some.append(s)

@@ -62,6 +62,20 @@ def test_prompts_in_several_launches(window, monkeypatch):
         assert sum(isinstance(p, fp4._PromptPart) for p in parts) == (3 if pages < 120 else 2)
 
 
+@pytest.mark.parametrize("lens,q_lens", [([66000, 5000, 300], [60, 70, 80]), ([5000, 66000, 4500], [40, 5, 4300])])
+def test_portions_beside_one_of_many_keys(lens, q_lens):
+    """More than 65,536 keys, which another kernel attends to: the step's other portions keep theirs."""
+    case = Fp4Case(lens, 1, 128, 16, seed=2)
+    q = _rand(sum(q_lens), 4, 128, seed=1, dtype=BF16)
+    got = ops.paged_attention(q, case.cache(), case.meta(q_lens), 0.003, None)
+    at = 0
+    for s, n in enumerate(q_lens):
+        alone = case.alone(s)
+        assert torch.equal(got[at:at + n], ops.paged_attention(q[at:at + n].contiguous(), alone.cache(), alone.meta([n]), 0.003, None)), s
+        at += n
+    ops.check_kernel_status()
+
+
 @pytest.mark.parametrize("hq,hkv", [(4, 2), (16, 1)])
 @pytest.mark.parametrize("long", [4094, 4095, 4096, 4500])
 def test_a_long_portion_beside_others_in_several_launches(long, hq, hkv, monkeypatch):
