@@ -450,6 +450,7 @@ PROMPT_ROWS = 32
 # with 4,096 new tokens or more).
 PAGES_BYTES = 1 << 30
 PAGE = 128
+SPLIT_SEQS = 4096      # sequences of a launch of the stream and split forms, whose CTAs keep their lengths in shared memory
 
 
 def _split_fits(d: int, page_size: int) -> bool:
@@ -541,7 +542,8 @@ def _parts(meta, group: int, hkv: int, d: int, page_size: int, prompts: bool, st
             used += n
         if some:
             parts.append(_PromptPart(some, q_lens, kv_lens, meta, device))
-        parts += [_SplitPart(x, q_lens, kv_lens, group, hkv, stream, device) for x in (one, few) if x]
+        parts += [_SplitPart(x[i:i + SPLIT_SEQS], q_lens, kv_lens, group, hkv, stream, device)
+                  for x in (one, few) for i in range(0, len(x), SPLIT_SEQS)]
         meta.scratch[key] = parts
     return parts
 

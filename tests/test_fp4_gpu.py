@@ -527,6 +527,18 @@ def test_attention_of_long_contexts():
     _check_attention(case, [1, 1, 2], 16, F32)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attention_of_more_sequences_than_a_launch_takes(dtype, monkeypatch):
+    monkeypatch.setattr(fp4, "SPLIT_SEQS", 40)
+    case = Fp4Case([1 + i % 7 * 50 for i in range(150)], 1, 64, 4, seed=1)
+    _check_attention(case, [2 if i % 3 == 0 else 1 for i in range(150)], 2, dtype)
+
+
+def test_attention_of_thousands_of_sequences():
+    n = fp4.SPLIT_SEQS + 5
+    _check_attention(Fp4Case([1 + i % 7 for i in range(n)], 1, 64, 4, seed=1), [1] * n, 2, BF16)
+
+
 def test_attention_beyond_32_bits():
     """A cache of more than 2^32 bytes, the sequences on its last pages."""
     first = 2 ** 32 // (2 * 8 * 64 * 64) + 100
