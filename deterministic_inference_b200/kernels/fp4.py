@@ -156,14 +156,15 @@ class _Rows:
     tensor, ``held``: the block scales, the codes, the units."""
 
     def _allocate(self, rows: int, k: int, device) -> None:
-        self.rows, self.k = rows, k
-        self.held = torch.empty(_tile_bytes(rows, k) + rows * (_code_bytes(k) + 4), dtype=torch.uint8, device=device)
+        codes_at = _tile_bytes(rows, k)
+        units_at = codes_at + rows * _code_bytes(k)
+        self.rows, self.k, self._at = rows, k, (codes_at, units_at)
+        self.held = torch.empty(units_at + 4 * rows, dtype=torch.uint8, device=device)
 
     def _pointers(self) -> tuple:
         """Addresses of the codes, the block scales and the units."""
-        tiles, bytes_ = self.held.data_ptr(), _code_bytes(self.k)
-        codes = tiles + _tile_bytes(self.rows, self.k)
-        return codes, tiles, codes + self.rows * bytes_
+        tiles, (codes_at, units_at) = self.held.data_ptr(), self._at
+        return tiles + codes_at, tiles, tiles + units_at
 
     def _quantize(self, x: torch.Tensor, name: str) -> None:
         code = _check_rows(x, name)
@@ -176,16 +177,15 @@ class _Rows:
 
     @property
     def tiles(self) -> torch.Tensor:
-        return self.held[:_tile_bytes(self.rows, self.k)]
+        return self.held[:self._at[0]]
 
     @property
     def codes(self) -> torch.Tensor:
-        at, n = _tile_bytes(self.rows, self.k), _code_bytes(self.k)
-        return self.held[at:at + self.rows * n].view(self.rows, n)
+        return self.held[self._at[0]:self._at[1]].view(self.rows, _code_bytes(self.k))
 
     @property
     def units(self) -> torch.Tensor:
-        return self.held[self.held.numel() - 4 * self.rows:].view(torch.float32)
+        return self.held[self._at[1]:].view(torch.float32)
 
     @property
     def shape(self):
@@ -264,6 +264,10 @@ class Fp4Weight(_Rows):
 def _check_rows(x, name: str) -> int:
     """The type's code of a matrix whose rows are consecutive values, at any distance from one another."""
     ops = _ops()
+    if isinstance(x, torch.Tensor) and x.is_cuda and x.dim() == 2 and x.stride(1) == 1 and 1 <= x.shape[1] <= MAX_K:
+        code = ops._DT.get(x.dtype)
+        if code is not None:
+            return code
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ops.KernelError(f"{name} must be a CUDA tensor: this package has no CPU path")
     if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
@@ -610,17 +614,21 @@ def fp4_paged_attention(q: torch.Tensor, cache: Fp4Cache, meta, scale: float, wi
     if d2 != d or hq < 1 or hq % hkv:
         raise ops.KernelError(f"fp4_paged_attention: q {tuple(q.shape)} vs cache {tuple(cache.shape)}")
     table, token_seq, cu, lens = meta.block_table, meta.token_seq, meta.cu_q_lens, meta.seq_lens
-    _require(table, "block_table", torch.int32, 2)
+    device, whole = cache.data.device, torch.int32
+    _require(table, "block_table", whole, 2)
     b = table.shape[0]
-    _require_entries(token_seq, "token_seq", t)
-    _require_entries(cu, "cu_q_lens", b + 1)
-    _require_entries(lens, "seq_lens", b)
+    if not (isinstance(token_seq, torch.Tensor) and token_seq.dtype is whole and token_seq.dim() == 1 and token_seq.shape[0] >= t
+            and isinstance(cu, torch.Tensor) and cu.dtype is whole and cu.dim() == 1 and cu.shape[0] > b
+            and isinstance(lens, torch.Tensor) and lens.dtype is whole and lens.dim() == 1 and lens.shape[0] >= b
+            and q.device == device and table.device == device and token_seq.device == device and cu.device == device
+            and lens.device == device and token_seq.is_contiguous() and cu.is_contiguous() and lens.is_contiguous()):
+        _require_entries(token_seq, "token_seq", t)
+        _require_entries(cu, "cu_q_lens", b + 1)
+        _require_entries(lens, "seq_lens", b)
+        _same_device("fp4_paged_attention", cache.data, q, table, token_seq, cu, lens)
     win = int(window) if window else 0
     if win < 0:
         raise ops.KernelError(f"fp4_paged_attention: a window of {win} keys")
-    device = cache.device
-    if q.device != device or table.device != device or token_seq.device != device or cu.device != device or lens.device != device:
-        _same_device("fp4_paged_attention", cache.data, q, table, token_seq, cu, lens)
     out = torch.empty_like(q)
     if t == 0:
         return out
