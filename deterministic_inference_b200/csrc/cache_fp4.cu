@@ -236,9 +236,9 @@ qk_norm_rope_cache_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, cons
 // ---- the keys and values of some sequences as bfloat16 pages of their own, [pages, 2, Hkv, PAGE, D], for attention over an unquantised
 // cache: what 4 bits stand for has 6 digits, so that bfloat16 holds it exactly.  Sequence number i of the launch, seq_list[i],
 // has its pages from first_page[i] on, one for every PAGE keys up to the host's bound of its length.  Keys behind its real length,
-// those that are on no page of the pool, and those of which the key or the value is no number, are zeros up to the page's end; pages wholly behind the last key, or ahead of the
-// window of the first new token, are left as they are.  (The new block table follows from the bounds: the host makes it.)  Bound by memory:
-// 32,000 tokens of 8 heads of 128 in 35 us, 4.8 TB/s; 4,096 in 8.1.
+// those that are on no page of the pool, and those of which the key or the value is no number, are zeros up to the page's end;
+// pages wholly behind the last key, or ahead of the window of the first new token, are left as they are.  (The new block table
+// follows from the bounds: the host makes it.)  Bound by memory: 32,000 tokens of 8 heads of 128 in 35 us, 4.8 TB/s; 4,096 in 8.1.
 constexpr int UNPACK_PAGE = 128;
 struct UnpackArgs {
   Cache4 cache;
