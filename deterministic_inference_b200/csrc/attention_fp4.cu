@@ -26,8 +26,8 @@ namespace {
 // key's codes for every other four keys: then neither reading keys (two a quarter warp) nor values (four keys a half warp)
 // meets a bank twice.
 //
-// The weights w = 2^(s + E_v - M + 10) are rounded to float16 (11 digits; two such parts of a float32 query's): M, a row's reference, is
-// raised when a weight would pass 2^15, so that what lies 2^-29 below the largest still has all digits, and sums are in
+// The outputs' weights 2^(a + E_v - D + LIFT) (the references of attention_fp4.cuh, a warp's own until the run's end) are rounded to float16 (11
+// digits; two such parts of a float32 query's): at most 2^15, so that what lies 2^-29 below the largest still has all digits.  Sums are in
 // float32.  Queries are scaled by a power of two to a largest element between 2^8 and 2^9, in which float16 holds bfloat16 values exactly
 // down to 2^-23 of it (three parts of a float32 query's).
 //
@@ -50,7 +50,7 @@ template <> __device__ __forceinline__ float4 load_four<__nv_bfloat16>(const __n
 template <typename T, int NT> struct SplitShape {
   static constexpr int ROWS = 8 * NT, Q_PARTS = sizeof(T) == 4 ? 3 : 1, P_PARTS = sizeof(T) == 4 ? 2 : 1;
   static constexpr int CTAS = sizeof(T) == 4 ? 2 : NT == 1 ? 4 : 3;
-  static constexpr int RING = SP_WARPS * SP_STAGES * SP_STAGE, ML = RING, FIRST = ML + SP_WARPS * ROWS * 8;
+  static constexpr int RING = SP_WARPS * SP_STAGES * SP_STAGE, ML = RING, FIRST = ML + SP_WARPS * ROWS * 16;
 };
 
 template <typename T, int NT>
@@ -59,7 +59,7 @@ attention_split_kernel(const T* __restrict__ q, T* __restrict__ out, const __gri
   using SH = SplitShape<T, NT>;
   constexpr int ROWS = SH::ROWS, QP = SH::Q_PARTS, PP = SH::P_PARTS;
   extern __shared__ __align__(128) unsigned char smem[];
-  float2* ml = reinterpret_cast<float2*>(smem + SH::ML);
+  float4* ml = reinterpret_cast<float4*>(smem + SH::ML);      // of a warp's rows: references (at, D), sum of weights
   long long* first = reinterpret_cast<long long*>(smem + SH::FIRST);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int G = a.Hq / a.Hkv;
@@ -223,10 +223,11 @@ attention_split_kernel(const T* __restrict__ q, T* __restrict__ out, const __gri
 #pragma unroll
       for (int c = 0; c < 2; ++c) pos[nt][c] = p0 + (row0 + nt * 8 + 2 * t + c) / G;
 
-    float M[NT][2], l[NT][2], o[8][NT][4];
+    float ref[NT][2], l[NT][2], o[8][NT][4];
+    bool odd = false;         // some row's D is not 0 (those are in `ml`)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      M[nt][0] = M[nt][1] = UNSET;
+      ref[nt][0] = ref[nt][1] = UNSET;
       l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
       for (int d = 0; d < 8; ++d) o[d][nt][0] = o[d][nt][1] = o[d][nt][2] = o[d][nt][3] = 0.f;
@@ -281,47 +282,122 @@ attention_split_kernel(const T* __restrict__ q, T* __restrict__ out, const __gri
             }
         }
       }
-      // scores plus the values' exponents: log 2 of the weights.  An exponent of no number, the key's or the value's, makes the
-      // scores of the rows that see it NaN.
-      float back[2][2];      // 2^-E_v
-      bool over = false;
+      // scores off their references.  An exponent of no number, the key's or the value's, makes those of the rows that see it NaN.
+      float lv[2][2], back[2][2];      // E_v, 2^-E_v
+      bool wild = false, over = odd;
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = m * 16 + h * 8 + (g ^ (g >> 1 & 1)), key = kb + r;
           const unsigned ke = st[SP_KE + r], ve = st[SP_VE + r];
-          const float ks = fp4_unit(ke), lv = ve == FP4_NO_NUMBER ? __uint_as_float(0x7fc00000u) : (float)(int)ve - 127.f;
-          back[m][h] = __uint_as_float(ve >= 254u ? 0x00400000u : (254u - ve) << 23);
+          const float ks = fp4_unit(ve == FP4_NO_NUMBER ? ve : ke);
+          lv[m][h] = (float)(int)ve - 127.f;
+          back[m][h] = off_value(ve);
+          wild |= !is_tame(ve) && (plain || (key >= seen && key < end));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              float z = fmaf(sc[m][nt][2 * h + c], ks * unit[nt][c], lv);
+              float z = __fmul_rn(sc[m][nt][2 * h + c], ks * unit[nt][c]);      // (rounded by itself: keys that are alike have one score)
               if (!plain && (key < run_at || key >= end || key > pos[nt][c] || key < first_visible_key(pos[nt][c], a.window))) z = -INFINITY;
               sc[m][nt][2 * h + c] = z;
-              over |= z > M[nt][c] + RAISE;
+              over |= z - ref[nt][c] + (lv[m][h] + LIFT) > LIFT + RAISE;
             }
         }
-      if (__any_sync(0xffffffffu, over)) {
+      bool apart = false;
+      if (__any_sync(0xffffffffu, over || wild)) {
+        // the largest of a column's scores, off `at`, each with `values` of its value's exponent (by all lanes)
+        auto column_top = [&](int nt, int c, float at, float values, float add) {
+          float top = -INFINITY;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[i >> 1][nt][2 * (i & 1) + c] - at + (values * lv[i >> 1][i & 1] + add));
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float top = fmaxf(fmaxf(sc[0][nt][c], sc[0][nt][2 + c]), fmaxf(sc[1][nt][c], sc[1][nt][2 + c]));
+          for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+          return top;
+        };
+        auto scale_outputs = [&](int nt, int c, float f) {
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-            if (top > M[nt][c] + RAISE) {
-              const float factor = fast_exp2(M[nt][c] - top);
-              M[nt][c] = top;
-              l[nt][c] *= factor;
-#pragma unroll
-              for (int d = 0; d < 8; ++d) {
-                o[d][nt][c] *= factor;
-                o[d][nt][2 + c] *= factor;
-              }
-            }
+          for (int d = 0; d < 8; ++d) {
+            o[d][nt][c] *= f;
+            o[d][nt][2 + c] *= f;
           }
+        };
+        apart = __any_sync(0xffffffffu, odd || wild);
+        if (!apart) {
+          float to[NT][2];
+          bool far = false;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const bool fresh = ref[nt][c] == UNSET;
+              const float base = fresh ? 0.f : ref[nt][c], top = column_top(nt, c, base, 1.f, LIFT);
+              to[nt][c] = top > (fresh ? -INFINITY : LIFT + RAISE) ? base + (top - LIFT) : ref[nt][c];
+              far |= to[nt][c] != UNSET && fabsf(to[nt][c]) >= FAR;
+            }
+          apart = __any_sync(0xffffffffu, far);
+          if (!apart) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const float f = fast_exp2(ref[nt][c] - to[nt][c]);
+                l[nt][c] *= f;
+                scale_outputs(nt, c, f);
+                ref[nt][c] = to[nt][c];
+              }
+          }
+        }
+        if (apart) {      // values or scores far from one another: the step's part of the sums of weights from here
+          bool any_d = false;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const bool fresh = ref[nt][c] == UNSET;
+              const int r = nt * 8 + 2 * t + c;
+              const float base = fresh ? 0.f : ref[nt][c], old = odd ? ml[warp * ROWS + r].y : 0.f;
+              const float top = column_top(nt, c, base, 1.f, LIFT - old);
+              float by = top > (fresh ? -INFINITY : LIFT + RAISE) ? top - LIFT : 0.f, d = old;
+              bool wide = false;      // a value that is not tame among the keys that the row sees
+#pragma unroll
+              for (int i = 0; i < 4; ++i) wide |= fabsf(lv[i >> 1][i & 1]) > TAME && sc[i >> 1][nt][2 * (i & 1) + c] > -INFINITY;
+              const unsigned wide_lanes = __ballot_sync(0xffffffffu, wide);
+              const float top_a = column_top(nt, c, base, 0.f, 0.f);
+              const float by_a = top_a > (fresh ? -INFINITY : HIGH) ? rintf(top_a) : 0.f;
+              const float top_v = column_top(nt, c, base + by_a, 1.f, 0.f);
+              if (old != 0.f || fabsf(base + by) >= FAR || (wide_lanes & 0x11111111u << t) != 0) {
+                by = by_a;
+                d -= by;
+                if (fresh || top_v - d > RAISE) d = top_v > -INFINITY ? rintf(top_v) : 0.f;
+              }
+              const float to = !fresh || top > -INFINITY ? base + by : UNSET;
+              l[nt][c] *= fresh ? 0.f : fast_exp2(base - to);
+              scale_outputs(nt, c, fresh ? 0.f : fast_exp2(base - to + old - d));
+              ref[nt][c] = to;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float value = lv[i >> 1][i & 1], off = sc[i >> 1][nt][2 * (i & 1) + c] - to, y = off + (value - d + LIFT);
+                sc[i >> 1][nt][2 * (i & 1) + c] = y;
+                l[nt][c] = d != 0.f || fabsf(value) > TAME ? l[nt][c] + fast_exp2(off + LIFT) : fmaf(fast_exp2(y), back[i >> 1][i & 1], l[nt][c]);
+              }
+              __syncwarp();
+              if (g == 0) ml[warp * ROWS + r].y = d;
+              any_d |= d != 0.f;
+            }
+          back[0][0] = back[0][1] = back[1][0] = back[1][1] = 0.f;
+          __syncwarp();
+          odd = __any_sync(0xffffffffu, any_d);
+        }
+      }
+      if (!apart) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[m][nt][i] = sc[m][nt][i] - ref[nt][i & 1] + (lv[m][i >> 1] + LIFT);
       }
       // ---- weights, as B operands
       unsigned pw[PP][2][NT][2];
@@ -334,7 +410,7 @@ attention_split_kernel(const T* __restrict__ q, T* __restrict__ out, const __gri
             float w[2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              w[c] = fast_exp2(sc[m][nt][2 * h + c] - (M[nt][c] - LIFT));
+              w[c] = fast_exp2(sc[m][nt][2 * h + c]);
               l[nt][c] = fmaf(w[c], back[m][h], l[nt][c]);
             }
             const unsigned two = pack_half(w[0], w[1]);
@@ -400,7 +476,7 @@ attention_split_kernel(const T* __restrict__ q, T* __restrict__ out, const __gri
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
         const int r = nt * 8 + 2 * t + c;
-        if (g == 0) ml[warp * ROWS + r] = make_float2(M[nt][c], v);
+        if (g == 0) ml[warp * ROWS + r] = make_float4(ref[nt][c], odd ? ml[warp * ROWS + r].y : 0.f, v, 0.f);
 #pragma unroll
         for (int d = 0; d < 8; ++d)
           *reinterpret_cast<float2*>(sums + r * SP_ROW + d * 16 + g * 2) = make_float2(o[d][nt][c], o[d][nt][2 + c]);
@@ -410,32 +486,45 @@ attention_split_kernel(const T* __restrict__ q, T* __restrict__ out, const __gri
       const int two = threadIdx.x & 63, dim = dim_of(2 * two);
 #pragma unroll 2
       for (int r = threadIdx.x >> 6; r < rows; r += 2) {
-        float2 w[SP_WARPS];
-        float top = UNSET;
+        float4 w[SP_WARPS];
+        float top = UNSET, top_d = 0.f;
+        bool any_d = false;      // some D is not 0
 #pragma unroll
         for (int x = 0; x < SP_WARPS; ++x) {
           w[x] = ml[x * ROWS + r];
           top = fmaxf(top, w[x].x);
+          any_d |= w[x].y != 0.f;
+        }
+        if (any_d) {
+          top_d = UNSET;
+#pragma unroll
+          for (int x = 0; x < SP_WARPS; ++x) top_d = fmaxf(top_d, rintf(w[x].x - top + w[x].y));
         }
         float sum = 0.f;
         float2 y = make_float2(0.f, 0.f);
 #pragma unroll
         for (int x = 0; x < SP_WARPS; ++x) {
-          const float f = fast_exp2(w[x].x - top);
+          float f = fast_exp2(w[x].x - top);
           const float2 v = *reinterpret_cast<const float2*>(smem + x * (SP_STAGES * SP_STAGE) + (r * SP_ROW + 2 * two) * 4);
-          sum = fmaf(f, w[x].y, sum);
+          sum = fmaf(f, w[x].z, sum);
+          if (any_d) f = fast_exp2(w[x].x - top + w[x].y - top_d);
           y.x = fmaf(f, v.x, y.x);
           y.y = fmaf(f, v.y, y.y);
         }
         if (s.splits == 1) {
           const int row = row0 + r, tok = row / G;
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          if (dim < a.D)
-            store_two<T>(out + ((long long)(s.q_begin + tok) * a.Hq + kvh * G + row - tok * G) * a.D + dim, y.x * inv, y.y * inv);
+          y.x *= inv;
+          y.y *= inv;
+          if (any_d) {
+            y.x = times_power(y.x, top_d);
+            y.y = times_power(y.y, top_d);
+          }
+          if (dim < a.D) store_two<T>(out + ((long long)(s.q_begin + tok) * a.Hq + kvh * G + row - tok * G) * a.D + dim, y.x, y.y);
         } else if (local < a.max_items) {
           const long long to = ((long long)i * a.max_items + local) * ROWS + r;
           *reinterpret_cast<float2*>(a.part_o + to * 128 + 2 * two) = y;
-          if (two == 0) a.part_ml[to] = make_float2(top, sum);
+          if (two == 0) a.part_ml[to] = make_float4(top, top_d, sum, 0.f);
         }
       }
     }
@@ -563,7 +652,7 @@ int dib_fp4_attention_split_keys(int kv_len, int rows) { return split_keys(kv_le
 // The split form, for the sequences seq_list[0 .. seq_count) or (null) seq_first ...: heads of 32, 64, 96 or 128, pages of a
 // power of two of rows, 4 at least.  max_rows: the most rows (new tokens x query heads of a kv head) of one of them; tile_rows: 8 or
 // 16 rows a tile; max_items: the most (tiles x runs x kv heads) of one; part_o float32 [seq_count, max_items, tile_rows, 128] and
-// part_ml [.., 2] take partial results where `runs`, the most runs of one of them, is not 0 (1 is given as 0).
+// part_ml [.., 4] take partial results where `runs`, the most runs of one of them, is not 0 (1 is given as 0).
 int dib_fp4_attention_split(const void* q, void* out, const void* data, const void* scales, const void* exponents, long long num_pages,
                             const void* block_table, int max_blocks, const void* cu_q_lens, const void* seq_lens,
                             const void* seq_list, int seq_first, int seq_count, int max_rows, int tile_rows, void* part_o,
@@ -584,7 +673,7 @@ int dib_fp4_attention_split(const void* q, void* out, const void* data, const vo
   a.seq_count = seq_count;
   while ((1 << a.page_shift) < page_size) ++a.page_shift;
   a.part_o = reinterpret_cast<float*>(part_o);
-  a.part_ml = reinterpret_cast<float2*>(part_ml);
+  a.part_ml = reinterpret_cast<float4*>(part_ml);
   a.max_items = max_items;
   using B = __nv_bfloat16;
   if (dtype == 1)

@@ -14,7 +14,22 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
-constexpr float UNSET = -1e30f, RAISE = 5.f, LIFT = 10.f;      // references of rows (see the kernels)
+// A row's references: `at` of its scores s (log 2) and D, a whole number, of its values.  With a = s - at a key adds 2^(a + LIFT) to the sum of
+// weights and 2^(a + E_v - D + LIFT) v to the outputs: the value's power of two has no part in the sum, and keys whose values are
+// zero, or next to it, may have all of the weight.
+// As a rule D is 0, `at` next to the largest s + E_v, raised when an output's weight would pass 2^(LIFT + RAISE), and a key's part of the sum
+// is that weight times 2^-E_v.  Rows that see values beyond 2^TAME either way, or scores next to which E_v is lost, have both references
+// found: `at` next to the largest score, raised when 2^a would pass 2^HIGH, D next to the largest a + E_v.  Which it is follows from
+// what the row has seen, so that its bits do.  A row that has seen no key has UNSET, 0.
+constexpr float RAISE = 5.f, LIFT = 10.f, HIGH = 60.f, FAR = 1048576.f, UNSET = -3.40282347e38f;
+constexpr int TAME = 40;
+__device__ __forceinline__ bool is_tame(unsigned byte) { return byte - (127u - TAME) <= 2u * TAME; }      // of a value's exponent
+__device__ __forceinline__ float off_value(unsigned byte) { return __uint_as_float((unsigned)max(254 - (int)byte, 0) << 23); }      // 2^-E_v
+// 2^d, which may be beyond a float32, times x
+__device__ __forceinline__ float times_power(float x, float d) {
+  const int e = (int)d, half = e >> 1;
+  return x * __uint_as_float((unsigned)(half + 127) << 23) * __uint_as_float((unsigned)(e - half + 127) << 23);
+}
 
 constexpr int SP_TILE = 128;      // keys that a CTA works on at a time
 
@@ -37,7 +52,7 @@ struct SplitArgs {
   int Hq, Hkv, D, page_shift, window, num_pages;
   float scale;
   float* part_o;                // [seq_count, max_items, ROWS, 128]: sums, in the order of the registers
-  float2* part_ml;              // [seq_count, max_items, ROWS]: reference (log 2), sum
+  float4* part_ml;              // [seq_count, max_items, ROWS]: references (at, D), sum of weights, nothing
   int max_items;
   int sms;                      // blocks b, b + sms, ... of the grid lie on one SM as a rule; 0: fewer blocks than would fill the GPU
 };
@@ -136,7 +151,7 @@ template <> __device__ __forceinline__ void store_two<__nv_bfloat16>(__nv_bfloat
   *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(x, y);
 }
 
-// The runs' results of a row: out = sum_r 2^(M_r - top) O_r / sum_r 2^(M_r - top) l_r, a lane 4 places of the sums.  Up to SM_RUNS runs
+// The runs' results of a row: out = sum_r 2^(at_r + D_r - top) O_r / sum_r 2^(at_r - top) l_r, a lane 4 places of the sums.  Up to SM_RUNS runs
 // are a warp's, all asked for at once; more are those of a block: warp w takes the runs w, w + 4, ... in their order, the four warps'
 // sums are added in the order of the warps.  (16 sequences' 10 rows a head of some 8 runs: the attention and its merge 24.5 us with a warp a
 // row, 26.2 with a block.)
@@ -145,9 +160,9 @@ template <typename T, int ROWS>
 __global__ void __launch_bounds__(SM_WARPS * 32)
 attention_split_merge_kernel(T* __restrict__ out, const __grid_constant__ SplitArgs a) {
   const float* part_o = a.part_o;
-  const float2* part_ml = a.part_ml;
+  const float4* part_ml = a.part_ml;
   __shared__ float4 s_o[SM_WARPS][32];
-  __shared__ float s_top[SM_WARPS], s_sum[SM_WARPS];
+  __shared__ float s_top[SM_WARPS], s_d[SM_WARPS], s_sum[SM_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int i = blockIdx.y, G = a.Hq / a.Hkv;
   const SplitSeq s = split_seq<ROWS>(a, i);
@@ -173,46 +188,70 @@ attention_split_merge_kernel(T* __restrict__ out, const __grid_constant__ SplitA
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
   float4 v[SM_RUNS];
-  float2 ml[SM_RUNS];
+  float3 ml[SM_RUNS];
   auto load = [&](int from, int step) {
 #pragma unroll
     for (int u = 0; u < SM_RUNS; ++u) {
       const int run = from + u * step;
       v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      ml[u] = make_float2(-INFINITY, 0.f);
+      ml[u] = make_float3(UNSET, 0.f, 0.f);
       if (run <= s1) {
         const long long at = base + (long long)run * ROWS;
-        ml[u] = part_ml[at];
+        const float4 m = part_ml[at];
+        ml[u] = make_float3(m.x, m.y, m.z);
         v[u] = *reinterpret_cast<const float4*>(part_o + at * 128 + lane * 4);
       }
     }
   };
-  auto add = [&](float top) {
+  // (top_d: the largest D, relative to the highest reference, to a whole number)
+  auto add = [&](float top, float top_d, bool odd) {
 #pragma unroll
     for (int u = 0; u < SM_RUNS; ++u) {
-      const float w = fast_exp2(ml[u].x - top);
-      sum = fmaf(w, ml[u].y, sum);
+      float w = fast_exp2(ml[u].x - top);
+      sum = fmaf(w, ml[u].z, sum);
+      if (odd) w = fast_exp2(ml[u].x - top + ml[u].y - top_d);
       o.x = fmaf(w, v[u].x, o.x); o.y = fmaf(w, v[u].y, o.y);
       o.z = fmaf(w, v[u].z, o.z); o.w = fmaf(w, v[u].w, o.w);
     }
   };
+  float top = UNSET, top_d = UNSET;
+  bool odd = false;      // some D is not 0
   if (alone) {
     load(s0, 1);
-    float top = UNSET;
 #pragma unroll
-    for (int u = 0; u < SM_RUNS; ++u) top = fmaxf(top, ml[u].x);
-    add(top);
+    for (int u = 0; u < SM_RUNS; ++u) {
+      top = fmaxf(top, ml[u].x);
+      odd |= ml[u].y != 0.f;
+    }
+    if (odd) {
+#pragma unroll
+      for (int u = 0; u < SM_RUNS; ++u) top_d = fmaxf(top_d, rintf(ml[u].x - top + ml[u].y));
+    }
+    add(top, top_d, odd);
   } else {
     load(s0 + warp, SM_WARPS);      // on their way while the references are compared
-    float top = UNSET;
-    for (int run = s0 + (int)threadIdx.x; run <= s1; run += SM_WARPS * 32) top = fmaxf(top, part_ml[base + (long long)run * ROWS].x);
+    for (int run = s0 + (int)threadIdx.x; run <= s1; run += SM_WARPS * 32) {
+      const float4 m = part_ml[base + (long long)run * ROWS];
+      top = fmaxf(top, m.x);
+      odd |= m.y != 0.f;
+    }
     top = warp_max(top);
     if (lane == 0) s_top[warp] = top;
-    __syncthreads();
+    odd = __syncthreads_or(odd);
     top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+    if (odd) {
+      for (int run = s0 + (int)threadIdx.x; run <= s1; run += SM_WARPS * 32) {
+        const float4 m = part_ml[base + (long long)run * ROWS];
+        top_d = fmaxf(top_d, rintf(m.x - top + m.y));
+      }
+      top_d = warp_max(top_d);
+      if (lane == 0) s_d[warp] = top_d;
+      __syncthreads();
+      top_d = fmaxf(fmaxf(s_d[0], s_d[1]), fmaxf(s_d[2], s_d[3]));
+    }
     for (int from = s0 + warp; from <= s1; from += SM_RUNS * SM_WARPS) {
       if (from != s0 + warp) load(from, SM_WARPS);
-      add(top);
+      add(top, top_d, odd);
     }
     s_o[warp][lane] = o;
     if (lane == 0) s_sum[warp] = sum;
@@ -230,8 +269,13 @@ attention_split_merge_kernel(T* __restrict__ out, const __grid_constant__ SplitA
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int tok = row / G, d0 = dim_of(lane * 4), d1 = dim_of(lane * 4 + 2);
   T* dst = out + ((long long)(s.q_begin + tok) * a.Hq + kvh * G + row - tok * G) * a.D;
-  if (d0 < a.D) store_two<T>(dst + d0, o.x * inv, o.y * inv);
-  if (d1 < a.D) store_two<T>(dst + d1, o.z * inv, o.w * inv);
+  o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
+  if (odd) {
+    o.x = times_power(o.x, top_d); o.y = times_power(o.y, top_d);
+    o.z = times_power(o.z, top_d); o.w = times_power(o.w, top_d);
+  }
+  if (d0 < a.D) store_two<T>(dst + d0, o.x, o.y);
+  if (d1 < a.D) store_two<T>(dst + d1, o.z, o.w);
 }
 // blocks of the merge for a sequence of `rows` rows and at most `runs` runs
 inline long long merge_blocks(long long rows, int runs) { return runs <= SM_RUNS ? (rows + SM_WARPS - 1) / SM_WARPS : rows; }

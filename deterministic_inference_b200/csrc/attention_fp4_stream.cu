@@ -12,9 +12,9 @@
 //     codes of two keys are interleaved (two instructions a word), so that a byte is a pair of keys, and become float16 (one
 //     instruction a pair), times the two block scales.  Keys 2 and 3, 6 and 7 of each eight change places, so that no two rows
 //     that are read at a time share banks.
-// The weights w = 2^(s + E_v - M + 10) are rounded to float16 (11 digits): M, a row's reference in a warp, is raised when a weight would
-// pass 2^15, so that what lies 2^-29 below the largest still has all digits.  Sums are in float32, the warps' own until the end of
-// the run, where they are added in the order of the warps.
+// The outputs' weights 2^(a + E_v - D + LIFT) (the references of attention_fp4.cuh, a warp's own) are rounded to float16 (11 digits): at
+// most 2^15, so that what lies 2^-29 below the largest still has all digits.  Sums are in float32, the warps' own until the end of the
+// run, where they are added in the order of the warps.
 //
 // What bounds it: instructions, some 300 for 32 keys of a warp (130 of them conversions and scales of values; with keys converted the
 // same way some 700), and the chain of a tile, some 3,000 cycles of which three or four CTAs an SM run side by side: an instruction issues
@@ -153,9 +153,10 @@ template <int ROWS> struct StreamShape {
   static constexpr int QSCALES = QUERIES + 2 * N * 64;                // [2] two tiles of 512 bytes
   static constexpr int WEIGHTS = QSCALES + 2 * 1024;                  // [4 warps][NT][32 keys][8 rows] float16
   static constexpr int SUMS = WEIGHTS + 4 * NT * 512;                 // [4 warps][ROWS][132]
-  static constexpr int TOPS = SUMS + 4 * ROWS * 132 * 4;              // [4 warps][ROWS] references
-  static constexpr int PARTS = TOPS + 4 * ROWS * 4;                   // [4 warps][ROWS][16 lanes] parts of the sums of weights
-  static constexpr int UNITS = PARTS + 4 * ROWS * 64;                // [2][ROWS] of the scores
+  static constexpr int TOPS = SUMS + 4 * ROWS * 132 * 4;              // [4 warps][ROWS] references (at, D)
+  static constexpr int PARTS = TOPS + 4 * ROWS * 8;                   // [4 warps][ROWS][16 lanes] parts of the sums of weights
+  static constexpr int FOUND = PARTS + 4 * ROWS * 64;                 // [4 warps][ROWS + 4] D of the rows, whether one is not 0
+  static constexpr int UNITS = FOUND + 4 * (ROWS + 4) * 4;            // [2][ROWS] of the scores
   static constexpr int SEEN = UNITS + 2 * ROWS * 4;                   // [2][2][ROWS] first and last key
   static constexpr int ITEMS = SEEN + 2 * 2 * ROWS * 4;
   static constexpr int BARS = ITEMS + ST_ITEMS * 64;
@@ -421,7 +422,7 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
   } else {
     // ---- an item's sums: a lane four places of a row; finished where the sequence has one run, else partial results for the merge
     const float* sums = reinterpret_cast<const float*>(smem + SH::SUMS);
-    const float* tops = reinterpret_cast<const float*>(smem + SH::TOPS);
+    const float2* tops = reinterpret_cast<const float2*>(smem + SH::TOPS);
     const float* parts = reinterpret_cast<const float*>(smem + SH::PARTS);
     const int d0 = dim_of(lane * 4), d1 = dim_of(lane * 4 + 2);
     for (int k = 0; ok; ++k) {
@@ -437,34 +438,57 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
       ok = mbar_wait_brief(sum_full, k & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
+      // a lane finds what the warps' sums of a row are taken times; it is handed to the others, a row after another
+      float2 refs[4];
+      float f[4], fo[4], top = UNSET, top_d = 0.f;
+      bool odd = false;      // some D is not 0
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        refs[x] = tops[x * ROWS + lane % ROWS];
+        top = fmaxf(top, refs[x].x);
+        odd |= refs[x].y != 0.f;
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) fo[x] = f[x] = fast_exp2(refs[x].x - top);
+      odd = __any_sync(0xffffffffu, odd);
+      if (odd) {
+        top_d = UNSET;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) top_d = fmaxf(top_d, rintf(refs[x].x - top + refs[x].y));
+#pragma unroll
+        for (int x = 0; x < 4; ++x) fo[x] = fast_exp2(refs[x].x - top + refs[x].y - top_d);
+      }
+      const long long to = ((long long)it.i * a.max_items + it.local) * ROWS;
+      const bool partial = it.splits > 1 && it.local < a.max_items;
+      if (partial && lane < rows) *reinterpret_cast<float2*>(a.part_ml + to + lane) = make_float2(top, top_d);
 #pragma unroll 1
       for (int r = 0; r < rows; ++r) {
-        float f[4], top = UNSET, sum = 0.f;
+        float sum = 0.f;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          f[x] = tops[x * ROWS + r];
-          top = fmaxf(top, f[x]);
-        }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          f[x] = fast_exp2(f[x] - top);
+          const float w = __shfl_sync(0xffffffffu, f[x], r), wo = __shfl_sync(0xffffffffu, fo[x], r);
           const float4 v = *reinterpret_cast<const float4*>(sums + (x * ROWS + r) * 132 + lane * 4);
-          if (lane < 16) sum = fmaf(f[x], parts[(x * ROWS + r) * 16 + lane], sum);
-          y.x = fmaf(f[x], v.x, y.x); y.y = fmaf(f[x], v.y, y.y);
-          y.z = fmaf(f[x], v.z, y.z); y.w = fmaf(f[x], v.w, y.w);
+          if (lane < 16) sum = fmaf(w, parts[(x * ROWS + r) * 16 + lane], sum);
+          y.x = fmaf(wo, v.x, y.x); y.y = fmaf(wo, v.y, y.y);
+          y.z = fmaf(wo, v.z, y.z); y.w = fmaf(wo, v.w, y.w);
         }
         sum = warp_sum(sum);
         if (it.splits == 1) {
           const int tok = (row0 + r) / G;
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
           __nv_bfloat16* dst = out + ((long long)(it.q_begin + tok) * a.Hq + it.kvh * G + row0 + r - tok * G) * D;
-          if (d0 < D) store_two<__nv_bfloat16>(dst + d0, y.x * inv, y.y * inv);
-          if (d1 < D) store_two<__nv_bfloat16>(dst + d1, y.z * inv, y.w * inv);
-        } else if (it.local < a.max_items) {
-          const long long to = ((long long)it.i * a.max_items + it.local) * ROWS + r;
-          *reinterpret_cast<float4*>(a.part_o + to * 128 + lane * 4) = y;
-          if (lane == 0) a.part_ml[to] = make_float2(top, sum);
+          y.x *= inv; y.y *= inv; y.z *= inv; y.w *= inv;
+          if (odd) {
+            const float d = __shfl_sync(0xffffffffu, top_d, r);
+            y.x = times_power(y.x, d); y.y = times_power(y.y, d);
+            y.z = times_power(y.z, d); y.w = times_power(y.w, d);
+          }
+          if (d0 < D) store_two<__nv_bfloat16>(dst + d0, y.x, y.y);
+          if (d1 < D) store_two<__nv_bfloat16>(dst + d1, y.z, y.w);
+        } else if (partial) {
+          *reinterpret_cast<float4*>(a.part_o + (to + r) * 128 + lane * 4) = y;
+          if (lane == 0) a.part_ml[to + r].z = sum;
         }
       }
       __syncwarp();
@@ -479,8 +503,9 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
     const unsigned tm = tmem + ((unsigned)(warp * 32) << 16);
     unsigned char* weights = smem + SH::WEIGHTS + warp * NT * 512;
     float* sums = reinterpret_cast<float*>(smem + SH::SUMS) + warp * ROWS * 132;
-    float* tops = reinterpret_cast<float*>(smem + SH::TOPS) + warp * ROWS;
+    float2* tops = reinterpret_cast<float2*>(smem + SH::TOPS) + warp * ROWS;
     float* parts = reinterpret_cast<float*>(smem + SH::PARTS) + warp * ROWS * 16;
+    float* found = reinterpret_cast<float*>(smem + SH::FOUND) + warp * (ROWS + 4);
     int n = 0, q_used = -1, done = 0, stage = 0;
     unsigned phase = 0;
     for (int k = 0; ok; ++k) {
@@ -573,10 +598,12 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
       }
       const float* units = reinterpret_cast<const float*>(smem + SH::UNITS) + (q_used & 1) * ROWS;
       const int* row_seen = reinterpret_cast<const int*>(smem + SH::SEEN) + (q_used & 1) * 2 * ROWS;
-      float M[ROWS], l[ROWS], o[8][NT][4];
+      float ref[ROWS], l[ROWS], o[8][NT][4];
+      if (lane <= ROWS) found[lane] = 0.f;
+      __syncwarp();
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
-        M[r] = UNSET;
+        ref[r] = UNSET;
         l[r] = 0.f;
       }
 #pragma unroll
@@ -593,8 +620,8 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         const unsigned char* st = smem + stage * ST_STAGE;
         const int in_tile = warp * 32 + lane, key = kb + in_tile;
         const bool plain = kb >= it.lo_all && kb + SP_TILE - 1 <= it.hi_all;        // every row sees every key
-        // ---- scores plus the value's exponent: log 2 of the weights.  An exponent of no number, the key's or the value's, makes
-        // the scores of the rows that see it NaN.
+        // ---- scores off their references.  An exponent of no number, the key's or the value's, makes those of the rows that see it
+        // NaN.
         float z[ROWS];
         {
           unsigned v[N];
@@ -610,36 +637,120 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_empty[buf]);
         const unsigned ke = st[ST_KE + in_tile], ve = st[ST_VE + in_tile];
-        const float ks = fp4_unit(ke), lv = ve == FP4_NO_NUMBER ? __uint_as_float(0x7fc00000u) : (float)(int)ve - 127.f;
-        const float back = __uint_as_float(ve >= 254u ? 0x00400000u : (254u - ve) << 23);      // 2^-E_v
-        bool over = false;
+        const float ks = fp4_unit(ve == FP4_NO_NUMBER ? ve : ke), lv = (float)(int)ve - 127.f;
+        float back = off_value(ve), y[ROWS];      // y: log 2 of the weights
+        const bool odd = found[ROWS] != 0.f;
+        bool over = odd || !is_tame(ve);
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-          z[r] = fmaf(z[r], ks * units[r], lv);
+          z[r] = __fmul_rn(z[r], ks * units[r]);      // (rounded by itself: keys that are alike have one score)
           if (!plain && (key < it.seen || key >= it.end || key < row_seen[r] || key > row_seen[ROWS + r])) z[r] = -INFINITY;
-          over |= z[r] > M[r] + RAISE;
+          y[r] = z[r] - ref[r] + (lv + LIFT);
+          over |= y[r] > LIFT + RAISE;
         }
         if (__any_sync(0xffffffffu, over)) {
+          const bool wild = !is_tame(ve) && (plain || (key >= it.seen && key < it.end)), first = kb == it.at;
+          bool apart = odd || __any_sync(0xffffffffu, wild);
           float f[NT * 8];
 #pragma unroll
           for (int r = 0; r < NT * 8; ++r) f[r] = 1.f;
+          if (!apart) {
+            float most = 0.f;
+            if (first) {      // (a row that sees none of the tile's keys while another does: below)
 #pragma unroll
-          for (int r = 0; r < ROWS; ++r) {
-            const float top = warp_top(z[r]);
-            if (top > M[r] + RAISE) {
-              f[r] = fast_exp2(M[r] - top);
-              M[r] = top;
-              l[r] *= f[r];
+              for (int r = 0; r < ROWS; ++r) {
+                ref[r] = warp_top(z[r] + (lv + LIFT)) - LIFT;
+                most = fmaxf(most, fabsf(ref[r]));
+                y[r] = z[r] - ref[r] + (lv + LIFT);
+              }
+            } else {
+#pragma unroll
+              for (int r = 0; r < ROWS; ++r) {
+                const bool fresh = ref[r] == UNSET;
+                const float top = warp_top(fresh ? z[r] + (lv + LIFT) : y[r]);
+                if (top > (fresh ? -INFINITY : LIFT + RAISE)) {
+                  const float to = (fresh ? 0.f : ref[r]) + (top - LIFT);
+                  most = fmaxf(most, fabsf(to));
+                  if (fabsf(to) < FAR) {
+                    f[r] = fast_exp2(ref[r] - to);
+                    l[r] *= f[r];
+                    ref[r] = to;
+                    y[r] = z[r] - to + (lv + LIFT);
+                  }
+                }
+              }
+            }
+            apart = most >= FAR;
+            if (apart && first) {
+#pragma unroll
+              for (int r = 0; r < ROWS; ++r) ref[r] = UNSET;
             }
           }
+          if (apart) {
+            // Values or scores far from one another: the tile's part of the sums of weights from here, a row at a time, by way of the
+            // sums' memory (unrolled, it costs those that never come here 6 of 78 us: 16 drafts on 4,096 keys, 32 heads).
+            if (done > 0) ok = mbar_wait_brief(sum_empty, (done - 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const float f0 = t < 2 ? (t == 0 ? f[nt * 8] : f[nt * 8 + 2]) : (t == 2 ? f[nt * 8 + 4] : f[nt * 8 + 6]);
-            const float f1 = t < 2 ? (t == 0 ? f[nt * 8 + 1] : f[nt * 8 + 3]) : (t == 2 ? f[nt * 8 + 5] : f[nt * 8 + 7]);
+            for (int r = 0; r < ROWS; ++r) {
+              sums[r * 132 + lane] = z[r];
+              sums[r * 132 + 32 + lane] = l[r];
+              if (lane == 0) *reinterpret_cast<float2*>(sums + r * 132 + 64) = make_float2(ref[r], f[r]);
+            }
+            __syncwarp();
+            bool any_d = false;
+#pragma unroll 1
+            for (int r = 0; r < ROWS; ++r) {
+              float* row = sums + r * 132;
+              const float2 was = *reinterpret_cast<const float2*>(row + 64);
+              const bool fresh = was.x == UNSET, wide = __any_sync(0xffffffffu, wild && row[lane] > -INFINITY);
+              const float base = fresh ? 0.f : was.x, old = odd ? found[r] : 0.f, score = row[lane];
+              float top = warp_top(score - base + (lv - old + LIFT)), d = old;
+              const bool seen = top > -INFINITY;
+              float by = top > (fresh ? -INFINITY : LIFT + RAISE) ? top - LIFT : 0.f;
+              if (old != 0.f || fabsf(base + by) >= FAR || wide) {
+                top = warp_top(score - base);
+                by = top > (fresh ? -INFINITY : HIGH) ? rintf(top) : 0.f;
+                d -= by;
+                top = warp_top(score - (base + by) + lv);
+                if (fresh || top - d > RAISE) d = top > -INFINITY ? rintf(top) : 0.f;
+              }
+              const float to = seen || !fresh ? base + by : UNSET, off = score - to, y = off + (lv - d + LIFT);
+              const float sum = row[32 + lane] * (fresh ? 0.f : fast_exp2(base - to));
+              row[lane] = y;
+              row[32 + lane] = d != 0.f || wild ? sum + fast_exp2(off + LIFT) : fmaf(fast_exp2(y), back, sum);
+              any_d |= d != 0.f;
+              __syncwarp();
+              if (lane == 0) {
+                *reinterpret_cast<float2*>(row + 64) = make_float2(to, was.y * (fresh ? 0.f : fast_exp2(base - to + old - d)));
+                found[r] = d;
+              }
+            }
+            __syncwarp();
 #pragma unroll
-            for (int d = 0; d < 8; ++d) {
-              o[d][nt][0] *= f0; o[d][nt][2] *= f0;
-              o[d][nt][1] *= f1; o[d][nt][3] *= f1;
+            for (int r = 0; r < ROWS; ++r) {
+              const float2 is = *reinterpret_cast<const float2*>(sums + r * 132 + 64);
+              y[r] = sums[r * 132 + lane];
+              l[r] = sums[r * 132 + 32 + lane];
+              ref[r] = is.x;
+              f[r] = is.y;
+            }
+            __syncwarp();
+            back = 0.f;
+            if (lane == 0) found[ROWS] = any_d ? 1.f : 0.f;
+            __syncwarp();
+          }
+          if (!first) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const float f0 = t < 2 ? (t == 0 ? f[nt * 8] : f[nt * 8 + 2]) : (t == 2 ? f[nt * 8 + 4] : f[nt * 8 + 6]);
+              const float f1 = t < 2 ? (t == 0 ? f[nt * 8 + 1] : f[nt * 8 + 3]) : (t == 2 ? f[nt * 8 + 5] : f[nt * 8 + 7]);
+#pragma unroll
+              for (int d = 0; d < 8; ++d) {
+                o[d][nt][0] *= f0; o[d][nt][2] *= f0;
+                o[d][nt][1] *= f1; o[d][nt][3] *= f1;
+              }
             }
           }
         }
@@ -651,7 +762,7 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
 #pragma unroll
           for (int c = 0; c < 2; ++c)
             if (r + c < ROWS) {
-              w[c] = fast_exp2(z[(r + c) % ROWS] - (M[(r + c) % ROWS] - LIFT));
+              w[c] = fast_exp2(y[(r + c) % ROWS]);
               l[(r + c) % ROWS] = fmaf(w[c], back, l[(r + c) % ROWS]);
             }
           two[r / 2] = pack_half(w[0], w[1]);
@@ -717,6 +828,7 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         }
       }
       if (!ok) break;
+      const float d_of_lane = found[lane % ROWS];
       // ---- this warp's sums of the run
       if (done > 0) ok = mbar_wait_brief(sum_empty, (done - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
@@ -725,7 +837,7 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
       for (int r = 0; r < ROWS; ++r) {
         const float v = l[r] + __shfl_xor_sync(0xffffffffu, l[r], 16);
         if (lane < 16) parts[r * 16 + lane] = v;
-        if (lane == r) tops[r] = M[r];
+        if (lane == r) tops[r] = make_float2(ref[r], d_of_lane);
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -851,7 +963,7 @@ int dib_fp4_attention_stream(const void* q, void* out, const void* data, const v
   a.seq_count = seq_count;
   while ((1 << a.page_shift) < page_size) ++a.page_shift;
   a.part_o = reinterpret_cast<float*>(part_o);
-  a.part_ml = reinterpret_cast<float2*>(part_ml);
+  a.part_ml = reinterpret_cast<float4*>(part_ml);
   a.max_items = max_items;
   const int box_rows = page_size < SP_TILE ? page_size : SP_TILE;
   CUtensorMap map;

@@ -576,7 +576,7 @@ def _prompt(q, out, cache: Fp4Cache, meta, part: _PromptPart, scale: float, wind
 def _split(q, out, cache: Fp4Cache, meta, part: _SplitPart, scale: float, window: int, stream: int) -> None:
     pages, _, hkv, page_size, d = cache.shape
     hq, rows = q.shape[1], part.rows
-    held = torch.empty(rows * 130, dtype=torch.float32, device=q.device) if rows else None      # sums, (reference, sum)
+    held = torch.empty(rows * 132, dtype=torch.float32, device=q.device) if rows else None      # sums, (references, sum of weights)
     partial = _pointer(held)
     st = _fn(part.form)(
         q.data_ptr(), out.data_ptr(), *cache._pointers(), pages, meta.block_table.data_ptr(), meta.block_table.shape[1],
