@@ -25,6 +25,7 @@ E + 127; 255: no numbers).
 from __future__ import annotations
 
 import ctypes
+import functools
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from types import SimpleNamespace
 
@@ -455,6 +456,10 @@ PROMPT_ROWS = 32
 PAGES_BYTES = 1 << 30
 PAGE = 128
 SPLIT_SEQS = 4096      # sequences of a launch of the stream and split forms, whose CTAs keep their lengths in shared memory
+# Bytes of partial results up to which a launch takes sequences of any sizes.  Every sequence of a launch has the room of the one with the most;
+# beyond this, sequences whose own room is less than half of that are launched by themselves.
+PARTIAL_BYTES = 1 << 28
+PARTIAL_ROW = 528      # bytes: 128 sums, two references, a sum of weights
 
 
 def _split_fits(d: int, page_size: int) -> bool:
@@ -462,6 +467,7 @@ def _split_fits(d: int, page_size: int) -> bool:
     return d <= 128 and d % 32 == 0 and page_size >= 4 and page_size & (page_size - 1) == 0
 
 
+@functools.lru_cache(maxsize=1 << 16)
 def _most_runs(kv_len: int) -> int:
     """The most runs of a sequence of at most ``kv_len`` keys, whatever its rows (the lengths on the device may be less than the
     host's)."""
@@ -472,19 +478,54 @@ def _most_runs(kv_len: int) -> int:
 class _SplitPart:
     """The sequences of one launch: their number, the most rows of one, rows a tile, the most work items of one."""
 
-    def __init__(self, seqs: list, q_lens: list, kv_lens: list, group: int, hkv: int, stream: bool, device):
+    def __init__(self, seqs: list, q_lens: list, kv_lens: list, group: int, hkv: int, stream: bool, device, sizes=None):
         self.form = "dib_fp4_attention_stream" if stream else "dib_fp4_attention_split"
         self.first, self.count, self.list = seqs[0], len(seqs), None
         if seqs != list(range(seqs[0], seqs[0] + len(seqs))):
             self.list = torch.tensor(seqs, dtype=torch.int32).to(device, non_blocking=True)
         self.list_pointer = _pointer(self.list)
-        self.max_rows = max(q_lens[s] for s in seqs) * group
-        self.tile_rows = 4 if stream and self.max_rows <= 4 else 8 if self.max_rows <= 8 else 16
-        runs, tiles = _most_runs(max(kv_lens[s] for s in seqs)), -(-self.max_rows // self.tile_rows)
+        self.max_rows, self.tile_rows, self.items, self.runs = sizes or _split_sizes(seqs, q_lens, kv_lens, group, hkv, stream)
+        self.rows = self.count * self.items * self.tile_rows if self.runs else 0
+
+
+def _split_sizes(seqs: list, q_lens: list, kv_lens: list, group: int, hkv: int, stream: bool) -> tuple:
+    """Of a launch: the most rows of a sequence, rows a tile, the most work items of a sequence, the most runs of one (0: all have
+    one, and there is nothing to add up)."""
+    longest: dict = {}      # keys, by new tokens: the bounds below grow with both
+    for s in seqs:
+        n, keys = q_lens[s], kv_lens[s]
+        if keys > longest.get(n, -1):
+            longest[n] = keys
+    max_rows = max(longest) * group
+    tile_rows = 4 if stream and max_rows <= 4 else 8 if max_rows <= 8 else 16
+    items = most = 1
+    for n, keys in longest.items():
+        tiles, runs = -(-n * group // tile_rows), _most_runs(keys)
         # (runs get longer with the rows: tiles times runs is at most the tiles' number and twice that of the shortest runs)
-        self.items = hkv * min(tiles * runs, tiles + 2 * runs)
-        self.runs = runs if runs > 1 else 0      # 0: nothing to add up
-        self.rows = self.count * self.items * self.tile_rows if runs > 1 else 0
+        items, most = max(items, hkv * min(tiles * runs, tiles + 2 * runs)), max(most, runs)
+    return max_rows, tile_rows, items, most if most > 1 else 0
+
+
+def _split_launches(seqs: list, q_lens: list, kv_lens: list, group: int, hkv: int, stream: bool) -> list:
+    """Every launch's sequences and sizes: one launch, but for sequences that would only widen the others' partial results."""
+    def measured(some: list) -> tuple:      # sizes, bytes of partial results
+        sizes = _split_sizes(some, q_lens, kv_lens, group, hkv, stream)
+        return sizes, len(some) * sizes[2] * sizes[1] * PARTIAL_ROW if sizes[3] else 0
+
+    launches = []
+    for i in range(0, len(seqs), SPLIT_SEQS):
+        some = seqs[i:i + SPLIT_SEQS]
+        sizes, room = measured(some)
+        while room > PARTIAL_BYTES:
+            own = {s: measured([s])[1] for s in some}
+            half = max(own.values()) // 2
+            large, rest = [s for s in some if own[s] > half], [s for s in some if own[s] <= half]
+            if not rest:
+                break
+            launches.append((large, measured(large)[0]))
+            some, (sizes, room) = rest, measured(rest)
+        launches.append((some, sizes))
+    return launches
 
 
 class _PromptPart:
@@ -546,8 +587,8 @@ def _parts(meta, group: int, hkv: int, d: int, page_size: int, prompts: bool, st
             used += n
         if some:
             parts.append(_PromptPart(some, q_lens, kv_lens, meta, device))
-        parts += [_SplitPart(x[i:i + SPLIT_SEQS], q_lens, kv_lens, group, hkv, stream, device)
-                  for x in (one, few) for i in range(0, len(x), SPLIT_SEQS)]
+        parts += [_SplitPart(x, q_lens, kv_lens, group, hkv, stream, device, sizes)
+                  for y in (one, few) for x, sizes in _split_launches(y, q_lens, kv_lens, group, hkv, stream)]
         meta.scratch[key] = parts
     return parts
 
@@ -576,7 +617,7 @@ def _prompt(q, out, cache: Fp4Cache, meta, part: _PromptPart, scale: float, wind
 def _split(q, out, cache: Fp4Cache, meta, part: _SplitPart, scale: float, window: int, stream: int) -> None:
     pages, _, hkv, page_size, d = cache.shape
     hq, rows = q.shape[1], part.rows
-    held = torch.empty(rows * 132, dtype=torch.float32, device=q.device) if rows else None      # sums, (references, sum of weights)
+    held = torch.empty(rows * PARTIAL_ROW, dtype=torch.uint8, device=q.device) if rows else None      # sums, (references, sum of weights)
     partial = _pointer(held)
     st = _fn(part.form)(
         q.data_ptr(), out.data_ptr(), *cache._pointers(), pages, meta.block_table.data_ptr(), meta.block_table.shape[1],
