@@ -141,20 +141,16 @@ def extend_tiles(q_lens: list, first_seq: int, tokens_per_tile: int):
     return seqs, starts
 
 
-def _pair_lists(meta, nd: int, tpt: int, window: int, hkv: int, max_chunks: int, t: int, hq: int,
-                d: int, device):
+def _pair_lists(meta, nd: int, tpt: int, window: int, hkv: int, max_chunks: int, device):
     """The CTA list of the two-tile prompt kernel for this step, on the device: (sequences,
-    first tokens of A, count, first tokens of B), the chunk of each entry (or None) and
-    the scratch for partial results (or Nones).  How tiles are paired depends on the step
+    first tokens of A, count, first tokens of B), and the chunk of each entry (or None).  How tiles are paired depends on the step
     (few tiles: each alone; more CTAs than SMs: neighbours; else from both ends); the
     arithmetic of a tile does not depend on its partner."""
     if max_chunks > 1:
         seqs, starts, starts_b, chunks = extend_chunk_units(meta.q_lens, meta.kv_lens, nd, tpt,
                                                             CHUNK_TILES)
         both = torch.tensor([seqs, starts, chunks, starts_b], dtype=torch.int32).to(device, non_blocking=True)
-        ws = (torch.empty(t, hq, max_chunks, d, dtype=torch.float32, device=device),
-              torch.empty(t, hq, max_chunks, 2, dtype=torch.float32, device=device))
-        return (both[0], both[1], len(seqs), both[3]), both[2], ws
+        return (both[0], both[1], len(seqs), both[3]), both[2]
     n_tiles = sum(-(-n // tpt) for n in meta.q_lens[nd:])
     ctas = (n_tiles + 1) // 2 * hkv
     how = SWITCHES["prefill_pair"]
@@ -162,7 +158,7 @@ def _pair_lists(meta, nd: int, tpt: int, window: int, hkv: int, max_chunks: int,
     neighbours = how == "2" or (how == "auto" and ctas > _sm_count(device))
     seqs, starts, starts_b = extend_tile_pairs(meta.q_lens, meta.kv_lens, nd, tpt, window, alone, neighbours)
     both = torch.tensor([seqs, starts, starts_b], dtype=torch.int32).to(device, non_blocking=True)
-    return (both[0], both[1], len(seqs), both[2]), None, (None, None)
+    return (both[0], both[1], len(seqs), both[2]), None
 
 
 def run(q, out, kv_cache, meta, scale: float, window: int, defer: bool = False, sink=None):
@@ -225,9 +221,14 @@ def run(q, out, kv_cache, meta, scale: float, window: int, defer: bool = False, 
         if max_chunks <= MAX_CHUNKS:
             got = meta.scratch.get(("extend_pairs", tpt, window))
             if got is None:
-                got = _pair_lists(meta, nd, tpt, window, hkv, max_chunks, t, hq, d, q.device)
+                got = _pair_lists(meta, nd, tpt, window, hkv, max_chunks, q.device)
                 meta.scratch[("extend_pairs", tpt, window)] = got
-            tiles, chunk_list, ws = got
+            tiles, chunk_list = got
+            # (partial results are the call's own, not the step's: calls on one step may run on two streams, or be replayed side
+            # by side)
+            ws = (None, None) if max_chunks == 1 else \
+                (torch.empty(t, hq, max_chunks, d, dtype=torch.float32, device=q.device),
+                 torch.empty(t, hq, max_chunks, 2, dtype=torch.float32, device=q.device))
             st = tc_lib.dib_extend_attention_tc_pair_sink(
                 _ptr(q), _ptr(out), _ptr(kv_cache), c_longlong(kv_cache.shape[0]), _ptr(bt),
                 c_int(bt.shape[1]), _ptr(meta.cu_q_lens), _ptr(meta.seq_lens), _ptr(tiles[0]),

@@ -555,6 +555,22 @@ class _PromptPart:
                                     kv_lens=[n if s in chosen else 0 for s, n in enumerate(kv_lens)], num_decode=0, scratch={})
 
 
+class _Parts(list):
+    """A step's launches.  Their lists, and those that the prompt attention keeps with them, are copied to the device by the first call
+    on the step, on its stream: calls on other streams wait for ``ready``."""
+    stream, ready = None, None
+
+    def wait(self, stream: int) -> None:
+        if self.stream != stream and self.ready is not None and not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream().wait_event(self.ready)      # (a capture begins when the device is idle)
+
+    def made(self, stream: int) -> None:
+        self.stream = stream
+        if any(isinstance(p, _PromptPart) or p.list is not None for p in self) and not torch.cuda.is_current_stream_capturing():
+            self.ready = torch.cuda.Event()
+            self.ready.record()
+
+
 def _parts(meta, group: int, hkv: int, d: int, page_size: int, prompts: bool, stream: bool, portions: bool, device) -> list:
     """The step's launches: the sequences with one new token, those with a few, those of the prompt form (bfloat16: all others
     that are portions of prompts, or those with many drafted tokens)."""
@@ -576,7 +592,7 @@ def _parts(meta, group: int, hkv: int, d: int, page_size: int, prompts: bool, st
         # adds up take another kernel, which is by the launch's longest: they follow in launches of their own.
         far = [s for s in many if kv_lens[s] > attention_bf16.MAX_CHUNKS * attention_bf16.CHUNK_TILES * PAGE]
         long = [s for s in many if q_lens[s] >= attention_bf16.CHUNK_TILES * PAGE and s not in far]
-        parts, some, used = [], [], 0
+        parts, some, used = _Parts(), [], 0
         room = max(1, PAGES_BYTES // (4 * hkv * PAGE * d))
         for s in [s for s in many if s not in long and s not in far] + long + far:
             n = -(-kv_lens[s] // PAGE)
@@ -597,9 +613,7 @@ def _prompt(q, out, cache: Fp4Cache, meta, part: _PromptPart, scale: float, wind
     from . import attention_bf16
     pages, _, hkv, page_size, d = cache.shape
     held = torch.empty(part.pages, 2, hkv, PAGE, d, dtype=torch.bfloat16, device=q.device)
-    own = part.meta
-    own.cu_q_lens, own.token_seq = meta.cu_q_lens, meta.token_seq
-    own.seq_lens = meta.seq_lens
+    own = SimpleNamespace(**vars(part.meta), cu_q_lens=meta.cu_q_lens, token_seq=meta.token_seq, seq_lens=meta.seq_lens)
     if part.mask is not None and max(own.kv_lens) > attention_bf16.CHUNK_TILES * PAGE:
         own.seq_lens = meta.seq_lens[:len(own.q_lens)] * part.mask
     st = _fn("dib_fp4_unpack_pages")(*cache._pointers(), pages, meta.block_table.data_ptr(), meta.block_table.shape[1],
@@ -636,10 +650,11 @@ def _require_entries(t, name: str, n: int) -> None:
 def fp4_paged_attention(q: torch.Tensor, cache: Fp4Cache, meta, scale: float, window=None,
                         portions: bool = False) -> torch.Tensor:
     """Causal attention of every token of the step over its sequence's keys in the cache, as ``ops.paged_attention``: q
-    [T, Hq, D] float32 or bfloat16, ``meta`` the step's ``AttentionMeta``.  A sequence's new tokens are its last ones
-    (``seq_lens`` counts them); each sees the keys up to its own position, the last ``window`` of them if given.  Keys and
-    values enter the products as what their codes and block scales stand for, exactly; the rows' powers of two join scores and
-    probabilities in float32.  A token that sees no key gives zeros.
+    [T, Hq, D] float32 or bfloat16, ``meta`` the step's ``AttentionMeta`` (lists that it keeps for later calls are the same for
+    all of them; calls on one step may run on several streams).  A sequence's new tokens are its last ones (``seq_lens`` counts
+    them); each sees the keys up to its own position, the last ``window`` of them if given.  Keys and values enter the products
+    as what their codes and block scales stand for, exactly; the rows' powers of two join scores and probabilities in float32.
+    A token that sees no key gives zeros.
 
     ``portions``: the sequences with more than one new token bring portions of prompts.  In bfloat16 they then all take one
     form, which makes bfloat16 pages of their keys and values and runs the prompt attention of the unquantised cache over
@@ -679,9 +694,14 @@ def fp4_paged_attention(q: torch.Tensor, cache: Fp4Cache, meta, scale: float, wi
         # (scores on the cache's codes as they are: bfloat16 queries, heads that are whole steps of 64 values)
         stream_form = code == 1 and d % 64 == 0 and cache.scales.data_ptr() % 16 == 0
         # (the prompt attention masks scores before it scales them)
-        for part in _parts(meta, hq // hkv, hkv, d, page_size, code == 1 and scale > 0, stream_form, bool(portions), device):
+        parts = _parts(meta, hq // hkv, hkv, d, page_size, code == 1 and scale > 0, stream_form, bool(portions), device)
+        if parts.stream != stream:
+            parts.wait(stream)
+        for part in parts:
             run = _prompt if isinstance(part, _PromptPart) else _split
             run(q, out, cache, meta, part, float(scale), win, stream)
+        if parts.stream is None:
+            parts.made(stream)
         return out
     st = _fn("dib_fp4_attention_any")(
         q.data_ptr(), out.data_ptr(), *cache._pointers(), table.data_ptr(), table.shape[1], token_seq.data_ptr(), cu.data_ptr(),

@@ -52,3 +52,38 @@ def test_ordinary_steps_are_one_launch_for_single_tokens_and_one_for_drafts():
         q_lens = sorted(rng.choice([1, 1, 1, 5]) for _ in range(64))
         parts = _parts(q_lens, [rng.randrange(5, 9000) for _ in range(64)], portions=False)
         assert len(parts) == len(set(q_lens))
+
+
+def test_a_step_keeps_no_partial_results_of_prompts(monkeypatch):
+    """Calls on one step, on two streams or in two captured graphs, must not write the same partial results: what the step keeps between
+    calls is lists of whole numbers."""
+    from deterministic_inference_b200.kernels import attention_bf16, ops
+
+    calls = []
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: calls.append((name, args)) or 0
+
+    made = []
+    empty = torch.empty
+    monkeypatch.setattr(ops, "_lib", lambda name: Library())
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: made.append(empty(*a, **k)) or made[-1])
+    q = torch.zeros(5000, 4, 128, dtype=torch.bfloat16)
+    cache = torch.zeros(1, 2, 2, 128, 128, dtype=torch.bfloat16)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32)
+    meta = SimpleNamespace(block_table=ints([[0]]), token_seq=ints([0]), cu_q_lens=ints([0, 5000]), seq_lens=ints([9000]), q_lens=[5000],
+                           kv_lens=[9000], num_decode=0, scratch={})
+    for _ in range(2):
+        attention_bf16.run(q, torch.zeros_like(q), cache, meta, 0.1, 0)
+
+    def tensors(x):
+        if isinstance(x, torch.Tensor):
+            yield x
+        elif isinstance(x, (list, tuple)):
+            for y in x:
+                yield from tensors(y)
+
+    assert meta.scratch and not [t for t in tensors(list(meta.scratch.values())) if t.is_floating_point()]
+    assert len(calls) == 2 and len(made) == 4 and len({t.data_ptr() for t in made}) == 4       # (held on to by `made`: each its own)

@@ -1,4 +1,4 @@
-"""What attention over the 4-bit cache allocates beside its output."""
+"""What attention over the 4-bit cache allocates beside its output, and calls that share what a step keeps."""
 
 from __future__ import annotations
 
@@ -41,3 +41,51 @@ def test_room_of_a_long_portion_beside_short_ones():
     assert torch.cuda.max_memory_allocated() - before < out.numel() * 4 + (1 << 28) + (1 << 20)
     want = ops.fp4_paged_attention(q[:2000].contiguous(), cache, case.alone(0).meta([2000]), 0.003)
     assert torch.equal(out[:2000], want)
+
+
+@pytest.mark.parametrize("q_lens,lens", [([300, 1, 90], [9000, 700, 5000]), ([4, 1, 2], [9000, 700, 300])])
+def test_two_streams_on_one_step(q_lens, lens):
+    """Calls on one step, on two streams at the same time: prompts of more keys than a chunk (partial results), and drafts."""
+    case = Fp4Case(lens, 2, 128, 16, seed=1)
+    cache, portions = case.cache(), q_lens[0] > 4
+    queries = [_rand(sum(q_lens), 8, 128, seed=s, dtype=BF16) for s in (3, 4)]
+    want = [ops.fp4_paged_attention(q, cache, case.meta(q_lens), 0.003, None, portions) for q in queries]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        meta, got = case.meta(q_lens), [[], []]
+        streams = [torch.cuda.Stream() for _ in (0, 1)]
+        torch.cuda.synchronize()
+        for _ in range(10):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[i].append(ops.fp4_paged_attention(queries[i], cache, meta, 0.003, None, portions))
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            assert all(torch.equal(y, want[i]) for y in got[i])
+    ops.check_kernel_status()
+
+
+def test_two_captured_graphs_of_one_step_side_by_side():
+    """Two graphs of the same step, with other queries, replayed on two streams at the same time."""
+    q_lens = [300, 1, 90]
+    case = Fp4Case([9000, 700, 5000], 2, 128, 16, seed=1)
+    cache, meta = case.cache(), case.meta(q_lens)
+    queries = [_rand(sum(q_lens), 8, 128, seed=s, dtype=BF16) for s in (3, 4)]
+    want = [ops.fp4_paged_attention(q, cache, meta, 0.003, None, True) for q in queries]
+    torch.cuda.synchronize()
+    graphs = []
+    for q in queries:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = ops.fp4_paged_attention(q, cache, meta, 0.003, None, True)
+        graphs.append((graph, y))
+    streams = [torch.cuda.Stream() for _ in (0, 1)]
+    for _ in range(10):
+        torch.cuda.synchronize()
+        for (graph, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            assert torch.equal(graphs[i][1], want[i])
+    ops.check_kernel_status()
