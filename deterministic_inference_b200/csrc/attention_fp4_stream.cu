@@ -194,7 +194,6 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int G = a.Hq / a.Hkv;
   if (threadIdx.x == 0) prefetch_tensormap(&map);
-  if (!late) pdl_trigger();
   // ---- the work before each sequence (metadata alone, which no kernel of a step writes)
   for (int i = threadIdx.x; i < a.seq_count; i += ST_THREADS) {
     const int4 m = load_seq(a, i);
@@ -228,6 +227,8 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
   __syncthreads();
+  // (with its tensor memory taken: the blocks of the kernel that follows wait for this grid, and must not hold what one of it waits for)
+  if (!late) pdl_trigger();
   if (warp == 0) {
     long long base = 0;
     for (int i0 = 0; i0 < a.seq_count; i0 += 32) {

@@ -329,7 +329,6 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   // (an offset, not a rounded address: what is known to be shared memory is read and written with 32-bit addresses)
   unsigned char* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
   unsigned char* epi_stage = smem + STAGES * STAGE;
-  if (!PAIR) pdl_trigger();
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_x);
     prefetch_tensormap(&map_w);
@@ -363,6 +362,8 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   }
   tc_fence_before();
   __syncthreads();
+  // (with its tensor memory taken: the blocks of the kernel that follows wait for this grid, and must not hold what one of it waits for)
+  if (!PAIR) pdl_trigger();
   if (PAIR) cluster_sync_all();       // both CTAs' barriers and tensor memory exist before either is used
   tc_fence_after();
   const unsigned tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
@@ -559,7 +560,6 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   unsigned char* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
   // a stage: channels, scales of channels, of tokens, tokens
   constexpr int WS_AT = 128 * ROW_BYTES, XS_AT = WS_AT + SCALES, X_AT = XS_AT + SCALES;
-  pdl_trigger();
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_x);
     prefetch_tensormap(&map_w);
@@ -584,6 +584,7 @@ gemm_fp4_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   }
   tc_fence_before();
   __syncthreads();
+  pdl_trigger();      // (as in the kernel above)
   tc_fence_after();
   const unsigned tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
   bool ok = true;
