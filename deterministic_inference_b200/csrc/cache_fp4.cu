@@ -239,7 +239,7 @@ qk_norm_rope_cache_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, cons
 // those that are on no page of the pool, and those of which the key or the value is no number, are zeros up to the page's end;
 // pages wholly behind the last key, or ahead of the window of the first new token, are left as they are.  (The new block table
 // follows from the bounds: the host makes it.)  Bound by memory: 32,000 tokens of 8 heads of 128 in 35 us, 4.8 TB/s; 4,096 in 8.1.
-constexpr int UNPACK_PAGE = 128;
+constexpr int UNPACK_PAGE = 128;      // (the host lists as many: kernels/fp4.py)
 struct UnpackArgs {
   Cache4 cache;
   const int* block_table;
@@ -481,8 +481,6 @@ int dib_fp4_cache_read(const void* data, const void* scales, const void* exponen
   if (dtype == 1) return launch_read<__nv_bfloat16>(cache, sl, k, v, T, shape, st);
   return launch_read<float>(cache, sl, k, v, T, shape, st);
 }
-
-int dib_fp4_unpack_page() { return UNPACK_PAGE; }
 
 // The keys and values of the sequences seq_list [count] as bfloat16 pages [first_page[count], 2, Hkv, 128, D] (see
 // unpack_pages_kernel); first_page int32 [count + 1], max_pages the most pages of one of them.

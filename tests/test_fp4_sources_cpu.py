@@ -33,3 +33,20 @@ def test_the_next_kernel_is_let_in_when_tensor_memory_is_taken(name):
         triggers = [m.start() for m in re.finditer(r"pdl_trigger\(|pdl_prologue\(", body)]
         assert triggers and min(triggers) > barrier, f"{name}: {kernel}"
     assert found == (2 if name == "gemm_fp4.cu" else 1)
+
+
+def test_every_exported_function_is_called():
+    """What a 4-bit library exports is called by the package (or by another of its libraries, by address)."""
+    package = "".join(p.read_text() for p in (CSRC.parent / "kernels").glob("*.py"))
+    for name in ("rows_fp4.cu", "cache_fp4.cu", "gemm_fp4.cu", "attention_fp4.cu", "attention_fp4_stream.cu"):
+        text = re.sub(r"//[^\n]*", "", (CSRC / name).read_text())
+        exported = re.findall(r"^(?:int|void) (dib_\w+)\(", text[text.index('extern "C"'):], re.M)
+        assert exported
+        for f in exported:
+            assert f in package, f"{name}: nobody calls {f}"
+
+
+def test_pages_made_for_prompts_are_those_the_host_lists():
+    from deterministic_inference_b200.kernels import fp4
+    text = (CSRC / "cache_fp4.cu").read_text()
+    assert int(re.search(r"UNPACK_PAGE = (\d+);", text).group(1)) == fp4.PAGE
