@@ -14,6 +14,26 @@
 
 namespace {
 
+struct CacheRow {
+  long long at;      // row of the cache, or -1
+  int token, kv, h;
+};
+// row r = (token, key or value, kv head)
+__device__ __forceinline__ CacheRow cache_row(unsigned r, const CacheShape& s, const int* slots) {
+  CacheRow c;
+  c.at = -1;
+  c.token = (int)quotient(r, s.per_token);
+  const int rest = (int)(r - (unsigned)c.token * s.per_token.d);
+  c.kv = rest >= s.Hkv;
+  c.h = rest - c.kv * s.Hkv;
+  if (r >= s.rows) return c;
+  const int slot = slots[c.token];
+  if (slot < 0) return c;
+  const unsigned page = quotient((unsigned)slot, s.page);
+  if (page < s.num_pages) c.at = ((long long)page * s.per_token.d + rest) * s.page.d + (slot - (int)(page * s.page.d));
+  return c;
+}
+
 constexpr float ROW_FLOOR = 7.888609052210118e-31f;      // 2^-100
 
 struct RowScale {

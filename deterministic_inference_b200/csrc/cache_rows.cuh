@@ -1,5 +1,5 @@
-// What the kernels share that write and read a paged cache of quantised rows, whatever the rows' format: where a token's row lies,
-// and the norm and rotation of the fused projection's rows in front of their quantising.
+// What the kernels share that write and read a paged cache of quantised rows, whatever the rows' format: a cache's shape with divisions
+// by products, and the norm and rotation of the fused projection's rows in front of their quantising.
 #pragma once
 
 #include "common.cuh"
@@ -32,25 +32,6 @@ struct CacheShape {
   int Hkv, D;
   unsigned num_pages;
 };
-struct CacheRow {
-  long long at;      // row of the cache, or -1
-  int token, kv, h;
-};
-// row r = (token, key or value, kv head)
-__device__ __forceinline__ CacheRow cache_row(unsigned r, const CacheShape& s, const int* slots) {
-  CacheRow c;
-  c.at = -1;
-  c.token = (int)quotient(r, s.per_token);
-  const int rest = (int)(r - (unsigned)c.token * s.per_token.d);
-  c.kv = rest >= s.Hkv;
-  c.h = rest - c.kv * s.Hkv;
-  if (r >= s.rows) return c;
-  const int slot = slots[c.token];
-  if (slot < 0) return c;
-  const unsigned page = quotient((unsigned)slot, s.page);
-  if (page < s.num_pages) c.at = ((long long)page * s.per_token.d + rest) * s.page.d + (slot - (int)(page * s.page.d));
-  return c;
-}
 static inline CacheShape make_shape(long long rows, int Hkv, int D, int page_size, long long num_pages) {
   CacheShape s;
   s.per_token = make_divisor(2u * Hkv);
