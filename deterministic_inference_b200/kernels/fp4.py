@@ -685,6 +685,8 @@ def fp4_paged_attention(q: torch.Tensor, cache: Fp4Cache, meta, scale: float, wi
     win = int(window) if window else 0
     if win < 0:
         raise ops.KernelError(f"fp4_paged_attention: a window of {win} keys")
+    if win >= table.shape[1] * page_size:      # every key that the table has room for (and what is beyond 32 bits is cut there)
+        win = 0
     out = torch.empty_like(q)
     if t == 0:
         return out

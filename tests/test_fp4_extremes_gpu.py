@@ -135,3 +135,16 @@ def test_absent_pages_hold_zeros(hq, hkv, d, dtype, page, q_len):
             (2 * (smax * 2.0 ** -18 + most * 2.0 ** -9.9) + 2.0 ** -8) * vmax + 2.0 ** -8 * want.abs()
         assert ((out.double() - want).abs() <= tol).all()
     ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("hq,hkv,d,page,dtype", FORMS)
+@pytest.mark.parametrize("q_lens", [[1, 1, 1], [4, 3, 2], [60, 40, 50]])
+def test_windows_of_any_size(hq, hkv, d, page, dtype, q_lens):
+    """Windows as long as the sequences and longer, beyond 32 bits too, are no windows; sequences with fewer keys than new tokens among
+    them."""
+    case = Fp4Case([700, 2, 30], hkv, d, page, seed=d)
+    q = _rand(sum(q_lens), hq, d, seed=2, dtype=dtype)
+    for portions in (False, True):
+        want = ops.fp4_paged_attention(q, case.cache(), case.meta(q_lens), 0.003, None, portions)
+        for window in (700, 5000, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, 2 ** 40):
+            assert torch.equal(ops.fp4_paged_attention(q, case.cache(), case.meta(q_lens), 0.003, window, portions), want), window
