@@ -26,7 +26,7 @@ namespace {
 // key's codes for every other four keys: then neither reading keys (two a quarter warp) nor values (four keys a half warp)
 // meets a bank twice.
 //
-// The outputs' weights 2^(a + E_v - D + LIFT) (the references of attention_fp4.cuh, a warp's own until the run's end) are rounded to float16 (11
+// The outputs' weights 2^(s - at + E_v - D) (the references of attention_fp4.cuh, a warp's own until the run's end) are rounded to float16 (11
 // digits; two such parts of a float32 query's): at most 2^15, so that what lies 2^-29 below the largest still has all digits.  Sums are in
 // float32.  Queries are scaled by a power of two to a largest element between 2^8 and 2^9, in which float16 holds bfloat16 values exactly
 // down to 2^-23 of it (three parts of a float32 query's).
@@ -282,7 +282,7 @@ attention_split_kernel(const T* __restrict__ q, T* __restrict__ out, const __gri
             }
         }
       }
-      // scores off their references.  An exponent of no number, the key's or the value's, makes those of the rows that see it NaN.
+      // scores and the value's power of two.  An exponent of no number, the key's or the value's, makes those of the rows that see it NaN.
       float lv[2][2], back[2][2];      // E_v, 2^-E_v
       bool wild = false, over = odd;
 #pragma unroll
@@ -299,22 +299,33 @@ attention_split_kernel(const T* __restrict__ q, T* __restrict__ out, const __gri
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              float z = __fmul_rn(sc[m][nt][2 * h + c], ks * unit[nt][c]);      // (rounded by itself: keys that are alike have one score)
+              float z = fmaf(sc[m][nt][2 * h + c], ks * unit[nt][c], lv[m][h]);
               if (!plain && (key < run_at || key >= end || key > pos[nt][c] || key < first_visible_key(pos[nt][c], a.window))) z = -INFINITY;
               sc[m][nt][2 * h + c] = z;
-              over |= z - ref[nt][c] + (lv[m][h] + LIFT) > LIFT + RAISE;
+              over |= z > ref[nt][c] + (LIFT + RAISE);
             }
         }
       bool apart = false;
       if (__any_sync(0xffffffffu, over || wild)) {
-        // the largest of a column's scores, off `at`, each with `values` of its value's exponent (by all lanes)
-        auto column_top = [&](int nt, int c, float at, float values, float add) {
-          float top = -INFINITY;
+        // a column's largest, by all lanes: with the values' powers of two as they are, and of the scores off `at` without them and with them
+        auto column_most = [&](float (&x)[4]) {
+          float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[i >> 1][nt][2 * (i & 1) + c] - at + (values * lv[i >> 1][i & 1] + add));
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+          for (int i = 4; i < 32; i <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
           return top;
+        };
+        auto column_top = [&](int nt, int c) {
+          float x[4] = {sc[0][nt][c], sc[0][nt][2 + c], sc[1][nt][c], sc[1][nt][2 + c]};
+          return column_most(x);
+        };
+        auto column_scores = [&](int nt, int c, float at, bool values) {
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float value = lv[i >> 1][i & 1];
+            x[i] = sc[i >> 1][nt][2 * (i & 1) + c] - value - at + (values ? value : 0.f);
+          }
+          return column_most(x);
         };
         auto scale_outputs = [&](int nt, int c, float f) {
 #pragma unroll
@@ -331,9 +342,8 @@ attention_split_kernel(const T* __restrict__ q, T* __restrict__ out, const __gri
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              const bool fresh = ref[nt][c] == UNSET;
-              const float base = fresh ? 0.f : ref[nt][c], top = column_top(nt, c, base, 1.f, LIFT);
-              to[nt][c] = top > (fresh ? -INFINITY : LIFT + RAISE) ? base + (top - LIFT) : ref[nt][c];
+              const float top = column_top(nt, c);
+              to[nt][c] = top > ref[nt][c] + (LIFT + RAISE) ? top - LIFT : ref[nt][c];
               far |= to[nt][c] != UNSET && fabsf(to[nt][c]) >= FAR;
             }
           apart = __any_sync(0xffffffffu, far);
@@ -357,30 +367,34 @@ attention_split_kernel(const T* __restrict__ q, T* __restrict__ out, const __gri
             for (int c = 0; c < 2; ++c) {
               const bool fresh = ref[nt][c] == UNSET;
               const int r = nt * 8 + 2 * t + c;
-              const float base = fresh ? 0.f : ref[nt][c], old = odd ? ml[warp * ROWS + r].y : 0.f;
-              const float top = column_top(nt, c, base, 1.f, LIFT - old);
-              float by = top > (fresh ? -INFINITY : LIFT + RAISE) ? top - LIFT : 0.f, d = old;
+              const float was = ref[nt][c], base = fresh ? 0.f : was, old = odd ? ml[warp * ROWS + r].y : 0.f;
+              const float top = column_top(nt, c);
+              float to = top > was + (LIFT + RAISE) ? top - LIFT : was, d = old;
               bool wide = false;      // a value that is not tame among the keys that the row sees
 #pragma unroll
               for (int i = 0; i < 4; ++i) wide |= fabsf(lv[i >> 1][i & 1]) > TAME && sc[i >> 1][nt][2 * (i & 1) + c] > -INFINITY;
               const unsigned wide_lanes = __ballot_sync(0xffffffffu, wide);
-              const float top_a = column_top(nt, c, base, 0.f, 0.f);
-              const float by_a = top_a > (fresh ? -INFINITY : HIGH) ? rintf(top_a) : 0.f;
-              const float top_v = column_top(nt, c, base + by_a, 1.f, 0.f);
-              if (old != 0.f || fabsf(base + by) >= FAR || (wide_lanes & 0x11111111u << t) != 0) {
-                by = by_a;
+              const float top_s = column_scores(nt, c, base, false);
+              const float by = top_s > (fresh ? -INFINITY : HIGH) ? rintf(top_s) - LIFT : 0.f;
+              const float top_v = column_scores(nt, c, base + by, true);
+              const bool both = old != 0.f || (fabsf(to) >= FAR && to != UNSET) || (wide_lanes & 0x11111111u << t) != 0;
+              float f_l = fast_exp2(was - to), f_o = f_l;
+              if (both) {
+                to = base + by;
                 d -= by;
-                if (fresh || top_v - d > RAISE) d = top_v > -INFINITY ? rintf(top_v) : 0.f;
+                if (fresh || top_v - d > LIFT + RAISE) d = top_v > -INFINITY ? rintf(top_v) - LIFT : 0.f;
+                f_l = fresh ? 0.f : fast_exp2(-by);
+                f_o = fresh ? 0.f : fast_exp2(old - by - d);
               }
-              const float to = !fresh || top > -INFINITY ? base + by : UNSET;
-              l[nt][c] *= fresh ? 0.f : fast_exp2(base - to);
-              scale_outputs(nt, c, fresh ? 0.f : fast_exp2(base - to + old - d));
+              l[nt][c] *= f_l;
+              scale_outputs(nt, c, f_o);
               ref[nt][c] = to;
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const float value = lv[i >> 1][i & 1], off = sc[i >> 1][nt][2 * (i & 1) + c] - to, y = off + (value - d + LIFT);
-                sc[i >> 1][nt][2 * (i & 1) + c] = y;
-                l[nt][c] = d != 0.f || fabsf(value) > TAME ? l[nt][c] + fast_exp2(off + LIFT) : fmaf(fast_exp2(y), back[i >> 1][i & 1], l[nt][c]);
+                float& z = sc[i >> 1][nt][2 * (i & 1) + c];
+                const float value = lv[i >> 1][i & 1], off = z - value - to;
+                z = both ? off + (value - d) : z - to;
+                l[nt][c] = d != 0.f || fabsf(value) > TAME ? l[nt][c] + fast_exp2(off) : fmaf(fast_exp2(z), back[i >> 1][i & 1], l[nt][c]);
               }
               __syncwarp();
               if (g == 0) ml[warp * ROWS + r].y = d;
@@ -397,7 +411,7 @@ attention_split_kernel(const T* __restrict__ q, T* __restrict__ out, const __gri
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sc[m][nt][i] = sc[m][nt][i] - ref[nt][i & 1] + (lv[m][i >> 1] + LIFT);
+            for (int i = 0; i < 4; ++i) sc[m][nt][i] -= ref[nt][i & 1];
       }
       // ---- weights, as B operands
       unsigned pw[PP][2][NT][2];

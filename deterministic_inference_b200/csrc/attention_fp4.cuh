@@ -14,13 +14,13 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
-// A row's references: `at` of its scores s (log 2) and D, a whole number, of its values.  With a = s - at a key adds 2^(a + LIFT) to the sum of
-// weights and 2^(a + E_v - D + LIFT) v to the outputs: the value's power of two has no part in the sum, and keys whose values are
-// zero, or next to it, may have all of the weight.
-// As a rule D is 0, `at` next to the largest s + E_v, raised when an output's weight would pass 2^(LIFT + RAISE), and a key's part of the sum
-// is that weight times 2^-E_v.  Rows that see values beyond 2^TAME either way, or scores next to which E_v is lost, have both references
-// found: `at` next to the largest score, raised when 2^a would pass 2^HIGH, D next to the largest a + E_v.  Which it is follows from
-// what the row has seen, so that its bits do.  A row that has seen no key has UNSET, 0.
+// A row's references: `at` of its scores s (log 2) and D, a whole number, of its values.  A key adds 2^(s - at) to the sum of weights and
+// 2^(s - at + E_v - D) v to the outputs: the value's power of two has no part in the sum, and keys whose values are zero, or next to
+// it, may have all of the weight.
+// As a rule D is 0, `at` LIFT below the largest s + E_v, raised when an output's weight would pass 2^(LIFT + RAISE), and a key's part of the
+// sum is that weight times 2^-E_v.  Rows that see values beyond 2^TAME either way, or scores next to which E_v is lost (FAR), have both
+// references found: `at` LIFT below the largest score, raised when 2^(s - at) would pass 2^HIGH, D by the largest s - at + E_v.
+// Which it is follows from what the row has seen, so that its bits do.  A row that has seen no key has UNSET, 0.
 constexpr float RAISE = 5.f, LIFT = 10.f, HIGH = 60.f, FAR = 1048576.f, UNSET = -3.40282347e38f;
 constexpr int TAME = 40;
 __device__ __forceinline__ bool is_tame(unsigned byte) { return byte - (127u - TAME) <= 2u * TAME; }      // of a value's exponent

@@ -145,6 +145,9 @@ struct __align__(16) StreamItem {
                                            // items; the keys that every row sees
 };
 
+template <bool V> struct Flag {
+  static constexpr bool value = V;
+};
 template <int ROWS> struct StreamShape {
   static constexpr int STAGES = 2;
   static constexpr int NT = (ROWS + 7) / 8, N = ROWS * ST_PARTS;      // tiles of 8 rows, columns of the scores
@@ -439,9 +442,44 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
       ok = mbar_wait_brief(sum_full, k & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      // a lane finds what the warps' sums of a row are taken times; it is handed to the others, a row after another
+      // A lane finds what the warps' sums of a row are taken times, f those of the weights, fo those of the outputs; it is handed to the
+      // others, a row after another.
+      const long long to = ((long long)it.i * a.max_items + it.local) * ROWS;
+      auto finish = [&](const float (&f)[4], const float (&fo)[4], const float top_d, auto odd) {
+#pragma unroll 1
+        for (int r = 0; r < rows; ++r) {
+          float sum = 0.f;
+          float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float w = __shfl_sync(0xffffffffu, f[x], r);
+            const float4 v = *reinterpret_cast<const float4*>(sums + (x * ROWS + r) * 132 + lane * 4);
+            if (lane < 16) sum = fmaf(w, parts[(x * ROWS + r) * 16 + lane], sum);
+            if (odd.value) w = __shfl_sync(0xffffffffu, fo[x], r);
+            y.x = fmaf(w, v.x, y.x); y.y = fmaf(w, v.y, y.y);
+            y.z = fmaf(w, v.z, y.z); y.w = fmaf(w, v.w, y.w);
+          }
+          sum = warp_sum(sum);
+          if (it.splits == 1) {
+            const int tok = (row0 + r) / G;
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            __nv_bfloat16* dst = out + ((long long)(it.q_begin + tok) * a.Hq + it.kvh * G + row0 + r - tok * G) * D;
+            y.x *= inv; y.y *= inv; y.z *= inv; y.w *= inv;
+            if (odd.value) {
+              const float d = __shfl_sync(0xffffffffu, top_d, r);
+              y.x = times_power(y.x, d); y.y = times_power(y.y, d);
+              y.z = times_power(y.z, d); y.w = times_power(y.w, d);
+            }
+            if (d0 < D) store_two<__nv_bfloat16>(dst + d0, y.x, y.y);
+            if (d1 < D) store_two<__nv_bfloat16>(dst + d1, y.z, y.w);
+          } else if (it.local < a.max_items) {
+            *reinterpret_cast<float4*>(a.part_o + (to + r) * 128 + lane * 4) = y;
+            if (lane == 0) a.part_ml[to + r].z = sum;
+          }
+        }
+      };
       float2 refs[4];
-      float f[4], fo[4], top = UNSET, top_d = 0.f;
+      float f[4], top = UNSET, top_d = 0.f;
       bool odd = false;      // some D is not 0
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
@@ -450,48 +488,19 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         odd |= refs[x].y != 0.f;
       }
 #pragma unroll
-      for (int x = 0; x < 4; ++x) fo[x] = f[x] = fast_exp2(refs[x].x - top);
-      odd = __any_sync(0xffffffffu, odd);
-      if (odd) {
+      for (int x = 0; x < 4; ++x) f[x] = fast_exp2(refs[x].x - top);
+      if (!__any_sync(0xffffffffu, odd)) {
+        finish(f, f, 0.f, Flag<false>());
+      } else {
+        float fo[4];
         top_d = UNSET;
 #pragma unroll
         for (int x = 0; x < 4; ++x) top_d = fmaxf(top_d, rintf(refs[x].x - top + refs[x].y));
 #pragma unroll
         for (int x = 0; x < 4; ++x) fo[x] = fast_exp2(refs[x].x - top + refs[x].y - top_d);
+        finish(f, fo, top_d, Flag<true>());
       }
-      const long long to = ((long long)it.i * a.max_items + it.local) * ROWS;
-      const bool partial = it.splits > 1 && it.local < a.max_items;
-      if (partial && lane < rows) *reinterpret_cast<float2*>(a.part_ml + to + lane) = make_float2(top, top_d);
-#pragma unroll 1
-      for (int r = 0; r < rows; ++r) {
-        float sum = 0.f;
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float w = __shfl_sync(0xffffffffu, f[x], r), wo = __shfl_sync(0xffffffffu, fo[x], r);
-          const float4 v = *reinterpret_cast<const float4*>(sums + (x * ROWS + r) * 132 + lane * 4);
-          if (lane < 16) sum = fmaf(w, parts[(x * ROWS + r) * 16 + lane], sum);
-          y.x = fmaf(wo, v.x, y.x); y.y = fmaf(wo, v.y, y.y);
-          y.z = fmaf(wo, v.z, y.z); y.w = fmaf(wo, v.w, y.w);
-        }
-        sum = warp_sum(sum);
-        if (it.splits == 1) {
-          const int tok = (row0 + r) / G;
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          __nv_bfloat16* dst = out + ((long long)(it.q_begin + tok) * a.Hq + it.kvh * G + row0 + r - tok * G) * D;
-          y.x *= inv; y.y *= inv; y.z *= inv; y.w *= inv;
-          if (odd) {
-            const float d = __shfl_sync(0xffffffffu, top_d, r);
-            y.x = times_power(y.x, d); y.y = times_power(y.y, d);
-            y.z = times_power(y.z, d); y.w = times_power(y.w, d);
-          }
-          if (d0 < D) store_two<__nv_bfloat16>(dst + d0, y.x, y.y);
-          if (d1 < D) store_two<__nv_bfloat16>(dst + d1, y.z, y.w);
-        } else if (partial) {
-          *reinterpret_cast<float4*>(a.part_o + (to + r) * 128 + lane * 4) = y;
-          if (lane == 0) a.part_ml[to + r].z = sum;
-        }
-      }
+      if (it.splits > 1 && it.local < a.max_items && lane < rows) *reinterpret_cast<float2*>(a.part_ml + to + lane) = make_float2(top, top_d);
       __syncwarp();
       if (lane == 0) mbar_arrive(sum_empty);
     }
@@ -621,8 +630,8 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         const unsigned char* st = smem + stage * ST_STAGE;
         const int in_tile = warp * 32 + lane, key = kb + in_tile;
         const bool plain = kb >= it.lo_all && kb + SP_TILE - 1 <= it.hi_all;        // every row sees every key
-        // ---- scores off their references.  An exponent of no number, the key's or the value's, makes those of the rows that see it
-        // NaN.
+        // ---- scores and the value's power of two.  An exponent of no number, the key's or the value's, makes those of the rows that see
+        // it NaN.
         float z[ROWS];
         {
           unsigned v[N];
@@ -639,15 +648,14 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
         if (lane == 0) mbar_arrive(&s_empty[buf]);
         const unsigned ke = st[ST_KE + in_tile], ve = st[ST_VE + in_tile];
         const float ks = fp4_unit(ve == FP4_NO_NUMBER ? ve : ke), lv = (float)(int)ve - 127.f;
-        float back = off_value(ve), y[ROWS];      // y: log 2 of the weights
+        float back = off_value(ve), less = -1.f;      // (0 where the references are off the scores already)
         const bool odd = found[ROWS] != 0.f;
         bool over = odd || !is_tame(ve);
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-          z[r] = __fmul_rn(z[r], ks * units[r]);      // (rounded by itself: keys that are alike have one score)
+          z[r] = fmaf(z[r], ks * units[r], lv);
           if (!plain && (key < it.seen || key >= it.end || key < row_seen[r] || key > row_seen[ROWS + r])) z[r] = -INFINITY;
-          y[r] = z[r] - ref[r] + (lv + LIFT);
-          over |= y[r] > LIFT + RAISE;
+          over |= z[r] > ref[r] + (LIFT + RAISE);
         }
         if (__any_sync(0xffffffffu, over)) {
           const bool wild = !is_tame(ve) && (plain || (key >= it.seen && key < it.end)), first = kb == it.at;
@@ -660,23 +668,20 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
             if (first) {      // (a row that sees none of the tile's keys while another does: below)
 #pragma unroll
               for (int r = 0; r < ROWS; ++r) {
-                ref[r] = warp_top(z[r] + (lv + LIFT)) - LIFT;
+                ref[r] = warp_top(z[r]) - LIFT;
                 most = fmaxf(most, fabsf(ref[r]));
-                y[r] = z[r] - ref[r] + (lv + LIFT);
               }
             } else {
 #pragma unroll
               for (int r = 0; r < ROWS; ++r) {
-                const bool fresh = ref[r] == UNSET;
-                const float top = warp_top(fresh ? z[r] + (lv + LIFT) : y[r]);
-                if (top > (fresh ? -INFINITY : LIFT + RAISE)) {
-                  const float to = (fresh ? 0.f : ref[r]) + (top - LIFT);
+                const float top = warp_top(z[r]);
+                if (top > ref[r] + (LIFT + RAISE)) {
+                  const float to = top - LIFT;
                   most = fmaxf(most, fabsf(to));
                   if (fabsf(to) < FAR) {
                     f[r] = fast_exp2(ref[r] - to);
                     l[r] *= f[r];
                     ref[r] = to;
-                    y[r] = z[r] - to + (lv + LIFT);
                   }
                 }
               }
@@ -689,7 +694,7 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
           }
           if (apart) {
             // Values or scores far from one another: the tile's part of the sums of weights from here, a row at a time, by way of the
-            // sums' memory (unrolled, it costs those that never come here 6 of 78 us: 16 drafts on 4,096 keys, 32 heads).
+            // sums' memory (unrolled, it costs those that never come here: 6 of 78 us for 16 drafts on 4,096 keys, 32 heads).
             if (done > 0) ok = mbar_wait_brief(sum_empty, (done - 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -705,26 +710,29 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
             for (int r = 0; r < ROWS; ++r) {
               float* row = sums + r * 132;
               const float2 was = *reinterpret_cast<const float2*>(row + 64);
-              const bool fresh = was.x == UNSET, wide = __any_sync(0xffffffffu, wild && row[lane] > -INFINITY);
-              const float base = fresh ? 0.f : was.x, old = odd ? found[r] : 0.f, score = row[lane];
-              float top = warp_top(score - base + (lv - old + LIFT)), d = old;
-              const bool seen = top > -INFINITY;
-              float by = top > (fresh ? -INFINITY : LIFT + RAISE) ? top - LIFT : 0.f;
-              if (old != 0.f || fabsf(base + by) >= FAR || wide) {
+              const float at = row[lane], score = at - lv, old = odd ? found[r] : 0.f;
+              const bool fresh = was.x == UNSET, wide = __any_sync(0xffffffffu, wild && at > -INFINITY);
+              float top = warp_top(at), to = top > was.x + (LIFT + RAISE) ? top - LIFT : was.x, d = old, y = at - to;
+              float f_l = fast_exp2(was.x - to), f_o = f_l;
+              if (old != 0.f || (fabsf(to) >= FAR && to != UNSET) || wide) {
+                const float base = fresh ? 0.f : was.x;
                 top = warp_top(score - base);
-                by = top > (fresh ? -INFINITY : HIGH) ? rintf(top) : 0.f;
+                const float by = top > (fresh ? -INFINITY : HIGH) ? rintf(top) - LIFT : 0.f;
+                to = base + by;
                 d -= by;
-                top = warp_top(score - (base + by) + lv);
-                if (fresh || top - d > RAISE) d = top > -INFINITY ? rintf(top) : 0.f;
+                top = warp_top(score - to + lv);
+                if (fresh || top - d > LIFT + RAISE) d = top > -INFINITY ? rintf(top) - LIFT : 0.f;
+                y = score - to + (lv - d);
+                f_l = fresh ? 0.f : fast_exp2(-by);
+                f_o = fresh ? 0.f : fast_exp2(old - by - d);
               }
-              const float to = seen || !fresh ? base + by : UNSET, off = score - to, y = off + (lv - d + LIFT);
-              const float sum = row[32 + lane] * (fresh ? 0.f : fast_exp2(base - to));
+              const float sum = row[32 + lane] * f_l;
               row[lane] = y;
-              row[32 + lane] = d != 0.f || wild ? sum + fast_exp2(off + LIFT) : fmaf(fast_exp2(y), back, sum);
+              row[32 + lane] = d != 0.f || wild ? sum + fast_exp2(score - to) : fmaf(fast_exp2(y), back, sum);
               any_d |= d != 0.f;
               __syncwarp();
               if (lane == 0) {
-                *reinterpret_cast<float2*>(row + 64) = make_float2(to, was.y * (fresh ? 0.f : fast_exp2(base - to + old - d)));
+                *reinterpret_cast<float2*>(row + 64) = make_float2(to, was.y * f_o);
                 found[r] = d;
               }
             }
@@ -732,13 +740,13 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
               const float2 is = *reinterpret_cast<const float2*>(sums + r * 132 + 64);
-              y[r] = sums[r * 132 + lane];
+              z[r] = sums[r * 132 + lane];
               l[r] = sums[r * 132 + 32 + lane];
               ref[r] = is.x;
               f[r] = is.y;
             }
             __syncwarp();
-            back = 0.f;
+            back = less = 0.f;
             if (lane == 0) found[ROWS] = any_d ? 1.f : 0.f;
             __syncwarp();
           }
@@ -763,7 +771,7 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
 #pragma unroll
           for (int c = 0; c < 2; ++c)
             if (r + c < ROWS) {
-              w[c] = fast_exp2(y[(r + c) % ROWS]);
+              w[c] = fast_exp2(fmaf(ref[(r + c) % ROWS], less, z[(r + c) % ROWS]));
               l[(r + c) % ROWS] = fmaf(w[c], back, l[(r + c) % ROWS]);
             }
           two[r / 2] = pack_half(w[0], w[1]);
