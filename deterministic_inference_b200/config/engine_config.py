@@ -27,11 +27,12 @@ class EngineConfig:
     # per token in front of every product, whose sums are exact integers (embedding and head stay in
     # ``dtype``).  "int8" for the cache: keys and values in 8 bits with a scale per token and head;
     # half the memory, and half of the cached bytes that a decode step reads.  None: ``dtype``.  (A
-    # decode step of qwen3_8b, 8 / 64 requests of 2,100 tokens: 3.92 / 7.73 ms in bfloat16, with 8-bit
-    # weights 3.34 / 6.74, cache 3.99 / 6.92, both 2.97 / 5.26.)
+    # decode step of qwen3_8b, 1 / 8 / 64 requests of 2,100 tokens: 3.27 / 3.91 / 7.58 ms in bfloat16, with 8-bit
+    # weights 2.66 / 3.37 / 6.78, cache 3.55 / 3.92 / 6.92, both 2.90 / 3.00 / 5.28.)
     # "fp4": the same in 4-bit floating point, with a scale for each 16 values and a power of two per output
     # channel, token and head: products on the block-scaled tensor cores with sums in float32, 0.57 bytes a
-    # cached value.  (The same steps: 4-bit weights 2.57 / 6.19 ms, cache 3.91 / 6.30, both 2.51 / 4.23.)
+    # cached value.  (The same steps: 4-bit weights 2.03 / 2.59 / 6.22 ms, cache 3.68 / 3.94 / 6.34, both
+    # 2.46 / 2.61 / 4.33: for few requests a quantised cache saves memory alone.)
     weight_dtype: Optional[str] = None
     cache_dtype: Optional[str] = None
 

@@ -7,7 +7,7 @@
 //
 // Forms: split (one new token, a few drafted ones, every float32 portion: the cache is streamed once) and one for every shape.
 // bfloat16 portions of prompts read the keys and values as bfloat16 pages (cache_fp4.cu) in the prompt attention of the
-// unquantised cache.
+// unquantised cache, whose probabilities are bfloat16 numbers (outputs off by 0.0023 of the norm instead of 0.0017).
 #include "attention_fp4.cuh"
 
 namespace {
@@ -34,8 +34,8 @@ namespace {
 // Work items: (sequence, kv head, tile of rows, run of keys), a CTA takes a contiguous range of them.  The length of a run follows
 // from the sequence's own lengths, so a row's bits do not depend on the rest of the step.
 //
-// Bound by instructions, some 700 for 32 keys: 64 requests of 2,048 keys, 16 / 4 heads: heads of 96 in bfloat16 41 us, of 128 in float32
-// 50 (the stream form 29 for heads of 128 in bfloat16).
+// Bound by instructions, some 700 for 32 keys: 64 requests of 2,048 keys, 16 / 4 heads: heads of 96 in bfloat16 45 us, of 128 in float32
+// 54 (the stream form 31 for heads of 128 in bfloat16).
 constexpr int SP_WARPS = 4, SP_THREADS = 32 * SP_WARPS, SP_STEP = 32, SP_STAGES = 3;
 constexpr int SP_K = 0, SP_V = SP_STEP * 64, SP_KS = 2 * SP_V, SP_VS = SP_KS + SP_STEP * 8, SP_KE = SP_VS + SP_STEP * 8,
               SP_VE = SP_KE + SP_STEP, SP_STAGE = SP_VE + SP_STEP;      // bytes of a step: codes, block scales, exponents

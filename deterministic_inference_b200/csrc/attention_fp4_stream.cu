@@ -3,8 +3,9 @@
 // run of its keys, by one CTA, in tiles of 128 keys.
 //   S^T = K Q^T on the tensor cores' block-scaled 4-bit products (tcgen05.mma kind::mxf4nvf4): the keys' codes and block scales
 //     enter as they lie in the cache, nothing of them is converted.  A query row is the sum of four rows in 4 bits, each the quantised rest
-//     of those before it, in a unit of a quarter (a column of the product each): an element is off by some 2^-14 of its block's
-//     largest.
+//     of those before it, in a unit of a quarter (a column of the product each): an element is off by 2^-14.8 of its block's largest
+//     in the root mean square and by 2^-10 at most (each row leaves 0.1771 of it, a sixth and e4m3's rounding of the scale), by 2^-24
+//     of the row's largest where the block is so far below that its scales vanish.
 //     Lane k of the accumulator holds key k's products with all of them; a thread, who has a key, adds the four up, joins the
 //     key's and the value's powers of two and makes the weights of its key.
 //   O^T = V^T P^T on mma.sync (m16n8k16, A = 16 dimensions x 16 keys): a warp has the 32 keys whose weights its threads made, so that
@@ -18,8 +19,8 @@
 //
 // What bounds it: instructions, some 300 for 32 keys of a warp (130 of them conversions and scales of values; with keys converted the
 // same way some 700), and the chain of a tile, some 3,000 cycles of which three or four CTAs an SM run side by side: an instruction issues
-// in 54 % of the cycles.  With the merge, 32 / 8 heads of 128: 64 requests of up to 4,096 keys 51 us, 3.4 TB/s; 64 / 8 heads, four of 32,000
-// keys 55 us, 2.7 TB/s; 16 / 8 heads, 16 drafts of 5 tokens on up to 1,500 keys 24 us; one of 2,048 keys 8.7 us.
+// in 54 % of the cycles.  With the merge, 32 / 8 heads of 128: 64 requests of up to 4,096 keys 53 us, 3.3 TB/s; 64 / 8 heads, four of 32,000
+// keys 56 us, 2.7 TB/s; 16 / 8 heads, 16 drafts of 5 tokens on up to 1,500 keys 26 us; one of 2,048 keys 8.9 us.
 //
 // Roles in a CTA: warps 0-3 as above, warp 4 copies (TMA, a box a page; scales by cp.async), warp 5 issues the scores' products, warp
 // 6 finds the next work items, warp 7 adds the four warps' sums of an item up under the next one.  The first group of warps gets a
@@ -530,7 +531,7 @@ attention_stream_kernel(const __grid_constant__ CUtensorMap map, const __nv_bflo
       const int row0 = it.tile * ROWS, rows = min(ROWS, it.n * G - row0);
       if (it.fresh) {
         // ---- the query rows: half a warp has a row, a lane 8 of its dimensions.  (How a rest is rounded is of no account: the next
-        // part has what is left.  The last is off by some 2^-14 of its block's largest.)
+        // part has what is left.)
         ++q_used;
         const int hl = lane & 15, qbuf = q_used & 1;
         uint4 raw[(ROWS + 7) / 8];

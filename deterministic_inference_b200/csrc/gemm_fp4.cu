@@ -15,8 +15,8 @@
 // their columns.  Many rows: tiles of 128 tokens x BN channels, or 256 x 192 for a pair of CTAs.
 //
 // What bounds it: few rows, the weight's bytes (8 x 24,576 x 4,096 11.6 us, 4.9 TB/s; 8 x 4,096 x 12,288 8.0 us, 3.5 TB/s, the rest
-// the cluster's start and sums); many rows, the tiles' operands from L2 (2,048 x 24,576 x 4,096 97 us, 4.3 PFLOP/s: 1.06 GB at 10.9 TB/s; the
-// copies without products take as long, the products without copies 67 us).
+// the cluster's start and sums); many rows, the tiles' operands from L2 (2,048 x 24,576 x 4,096 101 us among others, 97 by itself,
+// 4.3 PFLOP/s: 1.06 GB at 10.9 TB/s; the copies without products take as long, the products without copies 67 us).
 #include <cuda.h>
 
 #include "fp4.cuh"
@@ -31,9 +31,9 @@ constexpr int SMEM_MOST = 232448 - 1024;                // (1 KB left to static 
 __device__ int dib_gemm_fp4_error_word = 0;
 
 // How k, num_kb stages, is cut into parts: eight stages each at least, eight parts at most, the first ones a stage longer than the
-// others where that does not go even.  (Parts of four: 8 x 4,096 x 4,096 5.0 us instead of 6.0, but 8 x 24,576 x 4,096 15.6 instead
-// of 11.6, and 2,048 x 24,576 x 4,096 126 instead of 105: with many rows each part is read from tensor memory.  One part: 8 x 4,096
-// x 12,288 20.5 us instead of 8.0.)
+// others where that does not go even.  (Parts of four: 8 x 4,096 x 4,096 5.4 us instead of 6.3, but 8 x 24,576 x 4,096 22.9 instead
+// of 11.7, and 2,048 x 24,576 x 4,096 127 instead of 101: with many rows each part is read from tensor memory.  One part: 8 x 4,096
+// x 12,288 20.4 us instead of 8.3.)
 struct Parts {
   int parts, each, longer;      // stages of a part, number of parts that have one more
   explicit Parts(int num_kb) {
@@ -239,7 +239,7 @@ struct Args {
 
 // A warp's 32 token rows from row0 on and COLS columns from n0 on, 32 columns at a time: a lane turns its row's sums into the
 // output's type, stages them (swizzled) and the copy engine writes whole rows, clipped at M and N.  (Written straight from the
-// registers, a row's 32 bytes at a time: 2,048 x 24,576 x 4,096 117 us instead of 104.)
+// registers, a row's 32 bytes at a time, 2,048 x 24,576 x 4,096 took 13 us more.)
 template <typename OutT, int COLS>
 __device__ __forceinline__ void store_rows(const float (&acc)[COLS], const CUtensorMap* map_out, unsigned char* staging, int& turn_buffer,
                                            int lane, int row0, int n0, const Args& a) {
